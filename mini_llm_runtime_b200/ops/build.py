@@ -63,6 +63,7 @@ LIBRARIES: dict[str, tuple[str, ...]] = {
     "delta_chunks": (),
     "attention_shaped_mma": (),
     "matrix_memory": (),
+    "logit_rules": (),
 }
 
 _loaded: dict[str, ctypes.CDLL] = {}

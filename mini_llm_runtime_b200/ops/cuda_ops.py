@@ -68,6 +68,14 @@ def _need(tensor: torch.Tensor, name: str, dtype: torch.dtype | None = None, dim
         raise KernelError(f"{name} must have {dims} dimensions, got shape {tuple(tensor.shape)}")
 
 
+def _need_here(**tensors: torch.Tensor | None) -> None:
+    """A launch goes to the current device's stream: tensors of another device are refused."""
+    current = torch.cuda.current_device()
+    for name, tensor in tensors.items():
+        if tensor is not None and tensor.device.index != current:
+            raise KernelError(f"{name} is on {tensor.device}, the current device is cuda:{current}")
+
+
 def _ptr(tensor: torch.Tensor | None) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if tensor is None else tensor.data_ptr())
 
@@ -88,6 +96,7 @@ _PROTOTYPES = {
     "attention_tcgen05": {"mlr_attention_prefill_tcgen05": "ppppppppppp" "iiiiiiiii" "fi" "ppp" "l" "pip"},
     "attention_sigmoid_tcgen05": {"mlr_attention_sigmoid_tcgen05": "ppppp" "ppppppp" "iiiiiiii" "f" "pppp" "iii" "pp",
                                   "mlr_attention_sigmoid_tcgen05_scratch": "iiiii"},
+    "logit_rules": {"mlr_logit_rules": "pppiii" "pppppip" "p", "mlr_count_tokens": "ppippiiip"},
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 _declared: dict[str, ctypes.CDLL] = {}
@@ -136,6 +145,28 @@ class AttentionBatch:
     @property
     def num_decode(self) -> int:
         return self.counts.get("decode", 0)
+
+
+@dataclass
+class LogitTables:
+    """What the requests of the slots do to their logits, resident on the device and read by slot.
+
+    ``penalties`` float32 [slots, 3]: repetition, presence, frequency (1, 0, 0 change nothing); with it ``counts`` int32
+    [slots, vocab], the history (``IN_PROMPT`` for a token of the prompt plus how often the token was generated), and ``seen``
+    int32 [slots, ceil(vocab / 32)], bit t % 32 of word t // 32 set where the history is not zero (``count_tokens`` keeps the
+    two).  ``bias_tokens`` int32 and ``bias_values`` float32 [slots, n]: tokens in ascending order, unused entries at the end
+    hold ``NO_TOKEN``; a token listed twice gets both.  ``allowed`` int32 [slots, ceil(vocab / 32)]: the tokens a grammar
+    allows, as bits.  Each of the three may be None."""
+
+    penalties: torch.Tensor | None = None
+    counts: torch.Tensor | None = None
+    seen: torch.Tensor | None = None
+    bias_tokens: torch.Tensor | None = None
+    bias_values: torch.Tensor | None = None
+    allowed: torch.Tensor | None = None
+
+    IN_PROMPT = 1 << 30
+    NO_TOKEN = (1 << 31) - 1
 
 
 # Rows of one work item of the three prompt-attention kernels.
@@ -2216,3 +2247,79 @@ class CudaOps:
         _check(lib.mlr_sample(_ptr(logits), _ptr(temperatures), _ptr(seeds), _ptr(counters), _ptr(tokens),
                               rows, logits.shape[1], _stream()), "sample")
         return tokens
+
+    # ------------------------------------------------------------------ rules on logits
+    @staticmethod
+    def _logit_tables(tables: LogitTables, vocab: int) -> int:
+        """Check the tables against one another and the vocabulary; returns the number of slots."""
+        words = -(-vocab // 32)
+        slots = None
+        for name, dtype, width in (("penalties", torch.float32, 3), ("counts", torch.int32, vocab), ("seen", torch.int32, words),
+                                   ("bias_tokens", torch.int32, None), ("bias_values", torch.float32, None),
+                                   ("allowed", torch.int32, words)):
+            tensor = getattr(tables, name)
+            if tensor is None:
+                continue
+            _need(tensor, name, dtype, 2)
+            if width is not None and tensor.shape[1] != width:
+                raise KernelError(f"{name} must have {width} columns for {vocab} tokens, got {tensor.shape[1]}")
+            if slots is not None and tensor.shape[0] != slots:
+                raise KernelError(f"{name} has {tensor.shape[0]} slots, the tables before it {slots}")
+            slots = tensor.shape[0]
+        history = (tables.penalties is None, tables.counts is None, tables.seen is None)
+        if any(history) and not all(history):
+            raise KernelError("penalties, counts and seen come together")
+        if (tables.bias_tokens is None) != (tables.bias_values is None) or (
+                tables.bias_tokens is not None and tables.bias_tokens.shape != tables.bias_values.shape):
+            raise KernelError("bias_tokens and bias_values come together, in one shape")
+        if not slots:
+            raise KernelError("the tables hold no rule, or no slot")
+        return slots
+
+    def _shape_logits(self, logits, row_slot, tables, out):
+        _need(logits, "logits", torch.float32, 2)
+        _need(row_slot, "row_slot", torch.int32, 1)
+        if row_slot.shape[0] != logits.shape[0]:
+            raise KernelError("row_slot needs one entry per logits row")
+        slots = self._logit_tables(tables, logits.shape[1])
+        _need_here(logits=logits, row_slot=row_slot, penalties=tables.penalties, counts=tables.counts, seen=tables.seen,
+                   bias_tokens=tables.bias_tokens, bias_values=tables.bias_values, allowed=tables.allowed)
+        if out is None:
+            out = torch.empty_like(logits)
+        if logits.shape[0] == 0:
+            return out
+        _check(_declared_library("logit_rules").mlr_logit_rules(
+            logits.data_ptr(), out.data_ptr(), row_slot.data_ptr(), logits.shape[0], logits.shape[1], slots,
+            _address(tables.penalties), _address(tables.counts), _address(tables.seen), _address(tables.bias_tokens),
+            _address(tables.bias_values), 0 if tables.bias_tokens is None else tables.bias_tokens.shape[1],
+            _address(tables.allowed), _raw_stream()), "shape_logits")
+        return out
+
+    def shape_logits(self, logits: torch.Tensor, row_slot: torch.Tensor, tables: LogitTables) -> torch.Tensor:
+        """The rules of each row's request on its logits, float32 [rows, vocab]; ``row_slot`` int32 [rows] names the slot whose
+        row of the tables holds (a row of no slot passes unchanged).  A token of the history: x / repetition where x > 0, else
+        x * repetition; then less frequency times how often it was generated, less presence if it was; then its bias; tokens
+        that are not allowed get -inf.  A row that allows nothing is -inf throughout (greedy sampling then takes token 0)."""
+        return self._shape_logits(logits, row_slot, tables, None)
+
+    def shape_logits_(self, logits: torch.Tensor, row_slot: torch.Tensor, tables: LogitTables) -> torch.Tensor:
+        """The same in place: logits that no rule touches are neither read nor written."""
+        return self._shape_logits(logits, row_slot, tables, logits)
+
+    def count_tokens(self, tokens: torch.Tensor, slots: torch.Tensor, tables: LogitTables, prompt: bool = False) -> None:
+        """Add ``tokens`` int32 [n] to the histories of ``slots`` int32 [n]: as generated tokens, or as tokens of the prompt.
+        A slot may come several times; a token or slot outside the tables is passed over."""
+        _need(tokens, "tokens", torch.int32, 1)
+        _need(slots, "slots", torch.int32, 1)
+        if tokens.shape != slots.shape:
+            raise KernelError("tokens and slots need equal lengths")
+        if tables.counts is None:
+            raise KernelError("the tables hold no history")
+        _need(tables.counts, "counts", torch.int32, 2)
+        count = self._logit_tables(tables, tables.counts.shape[1])
+        _need_here(tokens=tokens, slots=slots, counts=tables.counts, seen=tables.seen)
+        if tokens.shape[0] == 0:
+            return
+        _check(_declared_library("logit_rules").mlr_count_tokens(
+            tokens.data_ptr(), slots.data_ptr(), tokens.shape[0], tables.counts.data_ptr(), tables.seen.data_ptr(), count,
+            tables.counts.shape[1], int(bool(prompt)), _raw_stream()), "count_tokens")

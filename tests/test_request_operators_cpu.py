@@ -1,0 +1,91 @@
+"""What the operators of requests refuse, before anything reaches a kernel: argument checks run here without a GPU, with the
+question whether a tensor lies on the device left out and a library that must not be reached."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from mini_llm_runtime_b200.ops import CudaOps, KernelError, LogitTables, cuda_ops
+
+
+@pytest.fixture
+def kernels(monkeypatch):
+    def need(tensor, name, dtype=None, dims=None):
+        if not isinstance(tensor, torch.Tensor):
+            raise KernelError(f"{name} must be a tensor")
+        if not tensor.is_contiguous():
+            raise KernelError(f"{name} must be contiguous")
+        if dtype is not None and tensor.dtype != dtype:
+            raise KernelError(f"{name} must be {dtype}")
+        if dims is not None and tensor.dim() != dims:
+            raise KernelError(f"{name} must have {dims} dimensions")
+
+    def library(name):
+        raise AssertionError("a refused call reached the library")
+
+    monkeypatch.setattr(cuda_ops, "_need", need)
+    monkeypatch.setattr(cuda_ops, "_need_here", lambda **tensors: None)
+    monkeypatch.setattr(cuda_ops, "_declared_library", library)
+    monkeypatch.setattr(cuda_ops.build, "load_library", library)
+    return CudaOps()
+
+
+def history(slots=2, vocab=40):
+    return dict(penalties=torch.ones((slots, 3)), counts=torch.zeros((slots, vocab), dtype=torch.int32),
+                seen=torch.zeros((slots, -(-vocab // 32)), dtype=torch.int32))
+
+
+@pytest.mark.parametrize("change", [
+    {"counts": None}, {"penalties": None}, {"seen": None},
+    {"counts": torch.zeros((2, 41), dtype=torch.int32)}, {"seen": torch.zeros((2, 1), dtype=torch.int32)},
+    {"penalties": torch.ones((2, 2))}, {"penalties": torch.ones((3, 3))}, {"counts": torch.zeros((2, 40))},
+    {"bias_tokens": torch.zeros((2, 4), dtype=torch.int32)}, {"bias_values": torch.zeros((2, 4))},
+    {"bias_tokens": torch.zeros((2, 4), dtype=torch.int32), "bias_values": torch.zeros((2, 5))},
+    {"bias_tokens": torch.zeros((2, 4), dtype=torch.int64), "bias_values": torch.zeros((2, 4))},
+    {"allowed": torch.zeros((2, 3), dtype=torch.int32)}, {"allowed": torch.zeros((1, 2), dtype=torch.int32)},
+    {"seen": torch.zeros((2, 4), dtype=torch.int32)[:, ::2]},
+])
+def test_tables_that_do_not_fit(kernels, change):
+    tables = LogitTables(**{**history(), **change})
+    with pytest.raises(KernelError):
+        kernels.shape_logits(torch.zeros((1, 40)), torch.zeros(1, dtype=torch.int32), tables)
+
+
+@pytest.mark.parametrize("logits,row_slot", [
+    (torch.zeros((1, 40), dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32)),
+    (torch.zeros((2, 40)), torch.zeros(1, dtype=torch.int32)),
+    (torch.zeros((1, 40)), torch.zeros(1, dtype=torch.int64)),
+    (torch.zeros((1, 80))[:, ::2], torch.zeros(1, dtype=torch.int32)),
+    (torch.zeros(40), torch.zeros(1, dtype=torch.int32)),
+])
+def test_logits_that_do_not_fit(kernels, logits, row_slot):
+    for call in (kernels.shape_logits, kernels.shape_logits_):
+        with pytest.raises(KernelError):
+            call(logits, row_slot, LogitTables(**history()))
+
+
+def test_tables_without_a_rule(kernels):
+    with pytest.raises(KernelError):
+        kernels.shape_logits(torch.zeros((1, 40)), torch.zeros(1, dtype=torch.int32), LogitTables())
+
+
+@pytest.mark.parametrize("tokens,slots,tables", [
+    (torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), LogitTables(**history())),
+    (torch.zeros(3, dtype=torch.int64), torch.zeros(3, dtype=torch.int32), LogitTables(**history())),
+    (torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), LogitTables(allowed=torch.zeros((2, 2), dtype=torch.int32))),
+    (torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), LogitTables(**{**history(), "seen": None})),
+])
+def test_histories_that_do_not_fit(kernels, tokens, slots, tables):
+    with pytest.raises(KernelError):
+        kernels.count_tokens(tokens, slots, tables)
+
+
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+
+    class Elsewhere:
+        device = torch.device("cuda", 1)
+
+    with pytest.raises(KernelError, match="current device"):
+        cuda_ops._need_here(x=None, weight=Elsewhere())
