@@ -31,105 +31,151 @@ struct RuleTables {
   int biases, slots;
 };
 
-// Four bits of a plane from token t0 >= 0 on (bits past the last word are zero).
+// Four bits of a plane from token t0 on: t0 a multiple of four, or any with WHOLE false (bits past the last word are zero).
+template <bool WHOLE>
 __device__ __forceinline__ unsigned four_bits(const unsigned* plane, int t0, int words) {
+  if (WHOLE) return (unsigned)__ldcg(reinterpret_cast<const unsigned char*>(plane) + (t0 >> 3)) >> (t0 & 4) & 15u;
   const int at = t0 >> 5, shift = t0 & 31;
   unsigned bits = __ldcg(plane + at) >> shift;
   if (shift > 28 && at + 1 < words) bits |= __ldcg(plane + at + 1) << (32 - shift);
   return bits & 15u;
 }
 
-__device__ __forceinline__ float penalised(float x, int word, float repetition, float presence, float frequency) {
-  x = x > 0.f ? x / repetition : x * repetition;
+// Without branches: every second warp has a known token among its 128.  x / repetition is x times the reciprocal, which is rounded
+// once per row: up to a second half step of float32 (2^-24), and the division took a third of the kernel's instructions.
+__device__ __forceinline__ float penalised(float x, int word, float repetition, float reciprocal, float presence, float frequency) {
   const int made = word & (IN_PROMPT - 1);
-  if (made > 0) x = __fsub_rn(__fsub_rn(x, __fmul_rn(frequency, (float)made)), presence);
-  return x;
+  x *= x > 0.f ? reciprocal : repetition;
+  x = fmaf(-frequency, (float)made, x);
+  return made > 0 ? x - presence : x;
 }
 
-// A CTA takes PIECES * 256 pieces of four logits of one row.  Pieces lie on 16-byte boundaries (the vocabulary need not be
-// a multiple of four: a row then starts inside a piece, and its first and last piece go entry by entry).
+// A CTA takes a stretch of one row, 256 pieces of four logits (a portion) at a time.  What a token may need hangs together (slot,
+// then bits, then the words of known tokens), so three portions are under way: the bits of the one after next, the logits and
+// words of the next, the arithmetic of the present one.  (A CTA per portion lives through that chain, 4 us, for 16 KB: 64 x
+// 152,064 logits took 38 us, 256 x 151,936 124 us; with the words fetched where they are used 31 and 80; now 29 and 76, where a
+// copy of the same logits takes 18.5 and 55.)
+// Pieces lie on 16-byte boundaries.  WHOLE: the vocabulary is a multiple of four and every piece is one row's; else a row
+// starts inside a piece, and its first and last piece go entry by entry.
 // IN_PLACE: logits that no rule touches are neither read nor written.
-template <int PIECES, bool IN_PLACE>
+template <bool IN_PLACE, bool WHOLE>
 __global__ void __launch_bounds__(RULE_THREADS)
-logit_rules_kernel(const float* logits, float* out, const int* row_slot, int vocab, const RuleTables tables) {
+logit_rules_kernel(const float* logits, float* out, const int* row_slot, int vocab, int stretch, const RuleTables tables) {
+  constexpr int PORTION = RULE_THREADS * 4;
   pdl_trigger();
   pdl_wait();
   const int row = blockIdx.y;
   const size_t base = (size_t)row * vocab;
-  const int lead = (int)(base & 3);                  // entries of the row's first piece that belong to the row before
+  const int lead = WHOLE ? 0 : (int)(base & 3);      // entries of the row's first piece that belong to the row before
   const int words = (vocab + 31) >> 5;
-  const int slot = __ldcg(row_slot + row);
-  const bool ruled = slot >= 0 && slot < tables.slots;
   const float* in = logits + base;
   float* to = out + base;
+  const int first = blockIdx.x * stretch - lead;     // first token of this CTA's pieces; may be negative in the first CTA
+  const int end = min(vocab, first + stretch);
+  int t0 = first + (int)threadIdx.x * 4;             // first token of this thread's present piece
+
+  auto mine = [&](int t) { return (WHOLE || t > -4) && t < end; };
+  auto inside = [&](int t) { return WHOLE || (t >= 0 && t + 4 <= vocab); };
+  float value[4], ahead[4];
+  auto load_values = [&](int t, float* v) {
+    if (!mine(t)) return;
+    if (inside(t)) {
+      const float4 four = *reinterpret_cast<const float4*>(in + t);
+      v[0] = four.x; v[1] = four.y; v[2] = four.z; v[3] = four.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = t + e >= 0 && t + e < vocab ? in[t + e] : 0.f;
+    }
+  };
+  if (!IN_PLACE) load_values(t0, value);             // needs no slot
+
+  const int slot = __ldcg(row_slot + row);
+  const bool ruled = slot >= 0 && slot < tables.slots;
   const unsigned* seen = ruled && tables.penalties != nullptr ? tables.seen + (size_t)slot * words : nullptr;
   const unsigned* allowed = ruled && tables.allowed != nullptr ? tables.allowed + (size_t)slot * words : nullptr;
   const int* counts = seen != nullptr ? tables.counts + (size_t)slot * vocab : nullptr;
-  const int first = blockIdx.x * (PIECES * RULE_THREADS * 4) - lead;      // first token of this CTA's pieces
+  const int biases = ruled && tables.bias_tokens != nullptr ? tables.biases : 0;
+  const int* bias_tokens = tables.bias_tokens + (size_t)(biases > 0 ? slot : 0) * tables.biases;
 
-  float4 value[PIECES];
-  unsigned known[PIECES], open[PIECES];
+  // bits 0..3: known and allowed; bits 4..7: not allowed
+  auto load_bits = [&](int t) {
+    if (!mine(t)) return 0u;
+    const int shift = !WHOLE && t < 0 ? -t : 0;
+    unsigned known = 0u, open = 15u;
+    if (seen != nullptr) known = four_bits<WHOLE>(seen, t + shift, words) << shift & 15u;
+    if (allowed != nullptr) open = (four_bits<WHOLE>(allowed, t + shift, words) << shift & 15u) | ((1u << shift) - 1u);
+    return (known & open) | (open ^ 15u) << 4;
+  };
+  const bool aligned = WHOLE || ((size_t)(ruled ? slot : 0) * vocab + first & 3) == 0;
+  int word[4], word_ahead[4];
+  auto load_words = [&](int t, unsigned bits, int* w, float* v) {
+    if ((bits & 15u) == 0u) return;
+    if (WHOLE || (aligned && inside(t))) {
+      const int4 four = __ldcg(reinterpret_cast<const int4*>(counts + t));
+      w[0] = four.x; w[1] = four.y; w[2] = four.z; w[3] = four.w;
+    } else {
 #pragma unroll
-  for (int p = 0; p < PIECES; ++p) {
-    const int t0 = first + (p * RULE_THREADS + (int)threadIdx.x) * 4;
-    known[p] = 0u;
-    open[p] = 15u;
-    if (t0 <= -4 || t0 >= vocab) continue;
-    const bool whole = t0 >= 0 && t0 + 4 <= vocab;
-    const int shift = t0 < 0 ? -t0 : 0;
-    if (seen != nullptr) known[p] = four_bits(seen, t0 + shift, words) << shift & 15u;
-    if (allowed != nullptr) open[p] = (four_bits(allowed, t0 + shift, words) << shift & 15u) | ((1u << shift) - 1u);
-    if (!IN_PLACE) {
-      if (whole) {
-        value[p] = __ldcs(reinterpret_cast<const float4*>(in + t0));
-      } else {
-        float* v = reinterpret_cast<float*>(&value[p]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = t0 + e >= 0 && t0 + e < vocab ? in[t0 + e] : 0.f;
-      }
+      for (int e = 0; e < 4; ++e)
+        if (bits >> e & 1u) w[e] = __ldcg(counts + t + e);
     }
-  }
+    if (IN_PLACE) load_values(t, v);
+  };
+  unsigned bits = load_bits(t0), bits_ahead = load_bits(t0 + PORTION);
+  const int bias_token = (int)threadIdx.x < biases ? __ldcg(bias_tokens + threadIdx.x) : -1;
   float repetition = 1.f, presence = 0.f, frequency = 0.f;
   if (seen != nullptr) {
     repetition = __ldcg(tables.penalties + 3 * (size_t)slot);
     presence = __ldcg(tables.penalties + 3 * (size_t)slot + 1);
     frequency = __ldcg(tables.penalties + 3 * (size_t)slot + 2);
   }
+  load_words(t0, bits, word, value);
+  const float reciprocal = 1.f / repetition;
+
+  for (int from = first; from < end; from += PORTION, t0 += PORTION) {
+    if (!IN_PLACE) load_values(t0 + PORTION, ahead);
+    load_words(t0 + PORTION, bits_ahead, word_ahead, ahead);
+    const unsigned bits_after = load_bits(t0 + 2 * PORTION);
+    if (mine(t0)) {
+      if ((bits & 15u) != 0u) {
 #pragma unroll
-  for (int p = 0; p < PIECES; ++p) {
-    const int t0 = first + (p * RULE_THREADS + (int)threadIdx.x) * 4;
-    if (t0 <= -4 || t0 >= vocab) continue;
-    const bool whole = t0 >= 0 && t0 + 4 <= vocab;
-    float* v = reinterpret_cast<float*>(&value[p]);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int t = t0 + e;
-      if (t < 0 || t >= vocab) continue;
-      const bool touched = (known[p] >> e & 1u) != 0u || (open[p] >> e & 1u) == 0u;
-      if (IN_PLACE && !touched) continue;
-      if ((open[p] >> e & 1u) == 0u) {
-        v[e] = -INFINITY;
-      } else {
-        if (IN_PLACE) v[e] = in[t];
-        if (known[p] >> e & 1u) v[e] = penalised(v[e], __ldcg(counts + t), repetition, presence, frequency);
+        for (int e = 0; e < 4; ++e) {
+          const float y = penalised(value[e], word[e], repetition, reciprocal, presence, frequency);
+          value[e] = bits >> e & 1u ? y : value[e];
+        }
       }
-      if (IN_PLACE || !whole) to[t] = v[e];
+      if (bits >> 4 != 0u) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) value[e] = bits >> (4 + e) & 1u ? -INFINITY : value[e];
+      }
+      if (!IN_PLACE && inside(t0)) {
+        *reinterpret_cast<float4*>(to + t0) = make_float4(value[0], value[1], value[2], value[3]);
+      } else {
+        const unsigned write = IN_PLACE ? (bits | bits >> 4) & 15u : 15u;
+        if (IN_PLACE && write == 15u && inside(t0)) {
+          *reinterpret_cast<float4*>(to + t0) = make_float4(value[0], value[1], value[2], value[3]);
+        } else if (write != 0u) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if ((write >> e & 1u) != 0u && (WHOLE || (t0 + e >= 0 && t0 + e < vocab))) to[t0 + e] = value[e];
+        }
+      }
     }
-    if (!IN_PLACE && whole) *reinterpret_cast<float4*>(to + t0) = value[p];
+    bits = bits_ahead;
+    bits_ahead = bits_after;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { value[e] = ahead[e]; word[e] = word_ahead[e]; }
   }
 
   // Biases of this CTA's tokens, by the thread that holds the first entry of a token: after the stores above.
-  if (!ruled || tables.bias_tokens == nullptr) return;
+  if (biases == 0) return;
   __syncthreads();
-  const int low = max(0, first), high = min(vocab, first + PIECES * RULE_THREADS * 4);
-  const int* tokens = tables.bias_tokens + (size_t)slot * tables.biases;
-  const float* values = tables.bias_values + (size_t)slot * tables.biases;
-  for (int i = threadIdx.x; i < tables.biases; i += RULE_THREADS) {
-    const int t = __ldcg(tokens + i);
-    if (t < low || t >= high || (i > 0 && __ldcg(tokens + i - 1) == t)) continue;
+  const float* values = tables.bias_values + (size_t)slot * biases;
+  for (int i = threadIdx.x; i < biases; i += RULE_THREADS) {
+    const int t = i < RULE_THREADS ? bias_token : __ldcg(bias_tokens + i);
+    if (t < max(0, first) || t >= end || (i > 0 && __ldcg(bias_tokens + i - 1) == t)) continue;
     if (allowed != nullptr && (__ldcg(allowed + (t >> 5)) >> (t & 31) & 1u) == 0u) continue;
     float sum = __ldcg(values + i);
-    for (int j = i + 1; j < tables.biases && __ldcg(tokens + j) == t; ++j) sum += __ldcg(values + j);
+    for (int j = i + 1; j < biases && __ldcg(bias_tokens + j) == t; ++j) sum += __ldcg(values + j);
     to[t] += sum;
   }
 }
@@ -149,14 +195,18 @@ __global__ void count_tokens_kernel(const int* tokens, const int* slots, int pai
   atomicOr(seen + (size_t)slot * ((vocab + 31) >> 5) + (token >> 5), 1u << (token & 31));
 }
 
-template <int PIECES>
 static void launch_rules(const float* logits, float* out, const int* row_slot, int rows, int vocab, const RuleTables& tables,
                          cudaStream_t stream) {
-  const dim3 grid((vocab + 3 + PIECES * RULE_THREADS * 4 - 1) / (PIECES * RULE_THREADS * 4), rows);
-  if (logits == out)
-    launch_kernel(logit_rules_kernel<PIECES, true>, grid, dim3(RULE_THREADS), 0, stream, logits, out, row_slot, vocab, tables);
-  else
-    launch_kernel(logit_rules_kernel<PIECES, false>, grid, dim3(RULE_THREADS), 0, stream, logits, out, row_slot, vocab, tables);
+  // Up to four portions per CTA, as far as every SM still has eight CTAs (64 x 152,064 and 256 x 151,936 logits with one portion
+  // each 43 and 100 us, with four 29 and 76, with sixteen 37 and 78; a single row with one 8.2, with sixteen 18.5).
+  constexpr int PORTION = RULE_THREADS * 4;
+  const int portions = (vocab + 3 + PORTION - 1) / PORTION;
+  const int each = (int)min(4ll, 1 + (long long)rows * portions / (8 * sm_count()));
+  const dim3 grid((portions + each - 1) / each, rows);
+  const bool whole = (vocab & 3) == 0;
+  auto kernel = logits == out ? (whole ? logit_rules_kernel<true, true> : logit_rules_kernel<true, false>)
+                              : (whole ? logit_rules_kernel<false, true> : logit_rules_kernel<false, false>);
+  launch_kernel(kernel, grid, dim3(RULE_THREADS), 0, stream, logits, out, row_slot, vocab, each * PORTION, tables);
 }
 
 }  // namespace mlr
@@ -176,7 +226,7 @@ MLR_EXPORT int mlr_logit_rules(const float* logits, float* out, const int* row_s
   if ((penalties != nullptr) != (counts != nullptr) || (penalties != nullptr) != (seen != nullptr)) return MLR_BAD_SIZE;
   RuleTables tables{penalties, counts, (const unsigned*)seen, biases > 0 ? bias_tokens : nullptr, bias_values,
                     (const unsigned*)allowed, biases, slots};
-  launch_rules<4>(logits, out, row_slot, rows, vocab, tables, stream);
+  launch_rules(logits, out, row_slot, rows, vocab, tables, stream);
   return launch_status();
 }
 

@@ -76,6 +76,11 @@ def _need_here(**tensors: torch.Tensor | None) -> None:
             raise KernelError(f"{name} is on {tensor.device}, the current device is cuda:{current}")
 
 
+def _need_together(*tensors: torch.Tensor | None) -> None:
+    if len({tensor.device for tensor in tensors if tensor is not None}) > 1:
+        raise KernelError("the tensors lie on different devices")
+
+
 def _ptr(tensor: torch.Tensor | None) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if tensor is None else tensor.data_ptr())
 
@@ -147,7 +152,7 @@ class AttentionBatch:
         return self.counts.get("decode", 0)
 
 
-@dataclass
+@dataclass(frozen=True)
 class LogitTables:
     """What the requests of the slots do to their logits, resident on the device and read by slot.
 
@@ -156,7 +161,8 @@ class LogitTables:
     int32 [slots, ceil(vocab / 32)], bit t % 32 of word t // 32 set where the history is not zero (``count_tokens`` keeps the
     two).  ``bias_tokens`` int32 and ``bias_values`` float32 [slots, n]: tokens in ascending order, unused entries at the end
     hold ``NO_TOKEN``; a token listed twice gets both.  ``allowed`` int32 [slots, ceil(vocab / 32)]: the tokens a grammar
-    allows, as bits.  Each of the three may be None."""
+    allows, as bits.  Each of the three may be None.  The tables are checked against one another here, once, and against the
+    logits at each call."""
 
     penalties: torch.Tensor | None = None
     counts: torch.Tensor | None = None
@@ -167,6 +173,42 @@ class LogitTables:
 
     IN_PROMPT = 1 << 30
     NO_TOKEN = (1 << 31) - 1
+
+    def __post_init__(self) -> None:
+        slots = vocab = words = None
+        for name, dtype in (("penalties", torch.float32), ("counts", torch.int32), ("seen", torch.int32), ("bias_tokens", torch.int32),
+                            ("bias_values", torch.float32), ("allowed", torch.int32)):
+            tensor = getattr(self, name)
+            if tensor is None:
+                continue
+            _need(tensor, name, dtype, 2)
+            if slots is not None and tensor.shape[0] != slots:
+                raise KernelError(f"{name} has {tensor.shape[0]} slots, the tables before it {slots}")
+            slots = tensor.shape[0]
+            if name == "counts":
+                vocab, words = tensor.shape[1], -(-tensor.shape[1] // 32)
+            elif name in ("seen", "allowed") and words is not None and tensor.shape[1] != words:
+                raise KernelError(f"{name} must have {words} columns, got {tensor.shape[1]}")
+            elif name in ("seen", "allowed"):
+                words = tensor.shape[1]
+        history = (self.penalties is None, self.counts is None, self.seen is None)
+        if any(history) and not all(history):
+            raise KernelError("penalties, counts and seen come together")
+        if self.penalties is not None and self.penalties.shape[1] != 3:
+            raise KernelError("penalties must have three columns: repetition, presence, frequency")
+        if (self.bias_tokens is None) != (self.bias_values is None) or (
+                self.bias_tokens is not None and self.bias_tokens.shape != self.bias_values.shape):
+            raise KernelError("bias_tokens and bias_values come together, in one shape")
+        if not slots:
+            raise KernelError("the tables hold no rule, or no slot")
+        _need_together(self.penalties, self.counts, self.seen, self.bias_tokens, self.bias_values, self.allowed)
+        object.__setattr__(self, "slots", slots)
+        object.__setattr__(self, "vocab", vocab)       # None where only biases or bits say something
+        object.__setattr__(self, "words", words)
+
+    @property
+    def device(self) -> torch.device:
+        return next(t for t in (self.penalties, self.bias_tokens, self.allowed) if t is not None).device
 
 
 # Rows of one work item of the three prompt-attention kernels.
@@ -2249,47 +2291,21 @@ class CudaOps:
         return tokens
 
     # ------------------------------------------------------------------ rules on logits
-    @staticmethod
-    def _logit_tables(tables: LogitTables, vocab: int) -> int:
-        """Check the tables against one another and the vocabulary; returns the number of slots."""
-        words = -(-vocab // 32)
-        slots = None
-        for name, dtype, width in (("penalties", torch.float32, 3), ("counts", torch.int32, vocab), ("seen", torch.int32, words),
-                                   ("bias_tokens", torch.int32, None), ("bias_values", torch.float32, None),
-                                   ("allowed", torch.int32, words)):
-            tensor = getattr(tables, name)
-            if tensor is None:
-                continue
-            _need(tensor, name, dtype, 2)
-            if width is not None and tensor.shape[1] != width:
-                raise KernelError(f"{name} must have {width} columns for {vocab} tokens, got {tensor.shape[1]}")
-            if slots is not None and tensor.shape[0] != slots:
-                raise KernelError(f"{name} has {tensor.shape[0]} slots, the tables before it {slots}")
-            slots = tensor.shape[0]
-        history = (tables.penalties is None, tables.counts is None, tables.seen is None)
-        if any(history) and not all(history):
-            raise KernelError("penalties, counts and seen come together")
-        if (tables.bias_tokens is None) != (tables.bias_values is None) or (
-                tables.bias_tokens is not None and tables.bias_tokens.shape != tables.bias_values.shape):
-            raise KernelError("bias_tokens and bias_values come together, in one shape")
-        if not slots:
-            raise KernelError("the tables hold no rule, or no slot")
-        return slots
-
     def _shape_logits(self, logits, row_slot, tables, out):
         _need(logits, "logits", torch.float32, 2)
         _need(row_slot, "row_slot", torch.int32, 1)
-        if row_slot.shape[0] != logits.shape[0]:
+        rows, vocab = logits.shape
+        if row_slot.shape[0] != rows:
             raise KernelError("row_slot needs one entry per logits row")
-        slots = self._logit_tables(tables, logits.shape[1])
-        _need_here(logits=logits, row_slot=row_slot, penalties=tables.penalties, counts=tables.counts, seen=tables.seen,
-                   bias_tokens=tables.bias_tokens, bias_values=tables.bias_values, allowed=tables.allowed)
+        if (tables.vocab is not None and tables.vocab != vocab) or (tables.words is not None and tables.words != -(-vocab // 32)):
+            raise KernelError(f"the tables are not those of {vocab} tokens")
+        _need_here(logits=logits, row_slot=row_slot, tables=tables)
         if out is None:
             out = torch.empty_like(logits)
-        if logits.shape[0] == 0:
+        if rows == 0:
             return out
         _check(_declared_library("logit_rules").mlr_logit_rules(
-            logits.data_ptr(), out.data_ptr(), row_slot.data_ptr(), logits.shape[0], logits.shape[1], slots,
+            logits.data_ptr(), out.data_ptr(), row_slot.data_ptr(), rows, vocab, tables.slots,
             _address(tables.penalties), _address(tables.counts), _address(tables.seen), _address(tables.bias_tokens),
             _address(tables.bias_values), 0 if tables.bias_tokens is None else tables.bias_tokens.shape[1],
             _address(tables.allowed), _raw_stream()), "shape_logits")
@@ -2315,11 +2331,9 @@ class CudaOps:
             raise KernelError("tokens and slots need equal lengths")
         if tables.counts is None:
             raise KernelError("the tables hold no history")
-        _need(tables.counts, "counts", torch.int32, 2)
-        count = self._logit_tables(tables, tables.counts.shape[1])
-        _need_here(tokens=tokens, slots=slots, counts=tables.counts, seen=tables.seen)
+        _need_here(tokens=tokens, slots=slots, tables=tables)
         if tokens.shape[0] == 0:
             return
         _check(_declared_library("logit_rules").mlr_count_tokens(
-            tokens.data_ptr(), slots.data_ptr(), tokens.shape[0], tables.counts.data_ptr(), tables.seen.data_ptr(), count,
-            tables.counts.shape[1], int(bool(prompt)), _raw_stream()), "count_tokens")
+            tokens.data_ptr(), slots.data_ptr(), tokens.shape[0], tables.counts.data_ptr(), tables.seen.data_ptr(), tables.slots,
+            tables.vocab, int(bool(prompt)), _raw_stream()), "count_tokens")

@@ -38,7 +38,7 @@ def history(slots=2, vocab=40):
 
 @pytest.mark.parametrize("change", [
     {"counts": None}, {"penalties": None}, {"seen": None},
-    {"counts": torch.zeros((2, 41), dtype=torch.int32)}, {"seen": torch.zeros((2, 1), dtype=torch.int32)},
+    {"counts": torch.zeros((2, 65), dtype=torch.int32)}, {"seen": torch.zeros((2, 1), dtype=torch.int32)},
     {"penalties": torch.ones((2, 2))}, {"penalties": torch.ones((3, 3))}, {"counts": torch.zeros((2, 40))},
     {"bias_tokens": torch.zeros((2, 4), dtype=torch.int32)}, {"bias_values": torch.zeros((2, 4))},
     {"bias_tokens": torch.zeros((2, 4), dtype=torch.int32), "bias_values": torch.zeros((2, 5))},
@@ -47,9 +47,8 @@ def history(slots=2, vocab=40):
     {"seen": torch.zeros((2, 4), dtype=torch.int32)[:, ::2]},
 ])
 def test_tables_that_do_not_fit(kernels, change):
-    tables = LogitTables(**{**history(), **change})
     with pytest.raises(KernelError):
-        kernels.shape_logits(torch.zeros((1, 40)), torch.zeros(1, dtype=torch.int32), tables)
+        LogitTables(**{**history(), **change})
 
 
 @pytest.mark.parametrize("logits,row_slot", [
@@ -65,20 +64,26 @@ def test_logits_that_do_not_fit(kernels, logits, row_slot):
             call(logits, row_slot, LogitTables(**history()))
 
 
-def test_tables_without_a_rule(kernels):
+def test_tables_without_a_rule_or_slot(kernels):
+    for tables in ({}, {"allowed": torch.zeros((0, 2), dtype=torch.int32)}):
+        with pytest.raises(KernelError):
+            LogitTables(**tables)
+
+
+@pytest.mark.parametrize("tables", [history(vocab=41), {"allowed": torch.zeros((2, 3), dtype=torch.int32)}])
+def test_tables_of_another_vocabulary(kernels, tables):
     with pytest.raises(KernelError):
-        kernels.shape_logits(torch.zeros((1, 40)), torch.zeros(1, dtype=torch.int32), LogitTables())
+        kernels.shape_logits(torch.zeros((1, 40)), torch.zeros(1, dtype=torch.int32), LogitTables(**tables))
 
 
 @pytest.mark.parametrize("tokens,slots,tables", [
-    (torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), LogitTables(**history())),
-    (torch.zeros(3, dtype=torch.int64), torch.zeros(3, dtype=torch.int32), LogitTables(**history())),
-    (torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), LogitTables(allowed=torch.zeros((2, 2), dtype=torch.int32))),
-    (torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), LogitTables(**{**history(), "seen": None})),
+    (torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), history()),
+    (torch.zeros(3, dtype=torch.int64), torch.zeros(3, dtype=torch.int32), history()),
+    (torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), {"allowed": torch.zeros((2, 2), dtype=torch.int32)}),
 ])
 def test_histories_that_do_not_fit(kernels, tokens, slots, tables):
     with pytest.raises(KernelError):
-        kernels.count_tokens(tokens, slots, tables)
+        kernels.count_tokens(tokens, slots, LogitTables(**tables))
 
 
 def test_tensors_of_another_device_are_refused(monkeypatch):
