@@ -1,0 +1,242 @@
+// Low-rank adapters of many requests beside a shared projection: row m of y = x W^T + b gains
+//
+//   scale[a] * (x[m] A[a]^T) B[a]^T        a = row_adapter[m], nothing where a is no adapter
+//
+// with A [adapters, rank, K] and B [adapters, N, rank].  Two kernels around the shared product:
+//
+//   down   u[m][r] = scale[a] * sum_k x[m][k] A[a][r][k], float32 [rows, rank].
+//   up     y[m][n] = base[m][n] + sum_r u[m][r] B[a][n][r], base being x W^T + b in float32, rounded once.
+//
+// Which adapter a row has is device memory: a captured step finds the adapters of whatever requests its rows belong to.
+// The shared product dominates; an adapter costs rank (K + N) elements, read once per step where its rows lie together.
+#include "mma_attention.cuh"
+
+namespace mlr {
+
+constexpr int DOWN_RANKS = 16;       // rank rows per CTA of the few-rows kernel
+constexpr int DOWN_WARPS = 4;
+constexpr int TILE_DOWN = 32;        // rows per CTA of the many-rows kernel
+constexpr int TILE_RANKS = 64;       // rank rows it takes at a time
+
+__device__ __forceinline__ uint32_t rank_in_cluster() {
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  return rank;
+}
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float read_from_cta(const float* mine, uint32_t rank) {
+  uint32_t remote;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(shared_address(mine)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return v;
+}
+
+// 16 bytes of bfloat16 or float32 as floats.
+template <typename T> struct Pack { static constexpr int N = 16 / sizeof(T); };
+__device__ __forceinline__ void unpack(const uint4& raw, float* v, bf16) {
+  const __nv_bfloat162* pair = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(pair[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void unpack(const uint4& raw, float* v, float) {
+  v[0] = __uint_as_float(raw.x); v[1] = __uint_as_float(raw.y); v[2] = __uint_as_float(raw.z); v[3] = __uint_as_float(raw.w);
+}
+
+// Few rows, each with an adapter of its own as a rule: CTA = (row, 16 rank rows, part of K), bound by reading A.  A warp walks
+// its stretch of K 32 pieces of 16 bytes at a time and holds 16 sums; the parts of K meet through the cluster's shared memory,
+// in order.  WIDE: rows are whole 16-byte pieces.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(DOWN_WARPS * 32)
+adapter_down_rows_kernel(const T* x, const T* __restrict__ down, const float* __restrict__ scales, const int* row_adapter, float* u,
+                         int adapters, int rank, int K, int parts) {
+  constexpr int PIECE = WIDE ? Pack<T>::N : 1;
+  __shared__ float sums[DOWN_WARPS][DOWN_RANKS];
+  __shared__ float total[DOWN_RANKS];
+  const int part = blockIdx.x % parts, row = blockIdx.x / parts;
+  const int r0 = blockIdx.y * DOWN_RANKS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
+  pdl_wait();
+  const int adapter = __ldcg(row_adapter + row);
+  const bool live = adapter >= 0 && adapter < adapters;      // the same in all CTAs of a cluster
+  if (live) {
+    float acc[DOWN_RANKS];
+#pragma unroll
+    for (int r = 0; r < DOWN_RANKS; ++r) acc[r] = 0.f;
+    const int pieces = K / PIECE;
+    const int stretch = (pieces + parts * DOWN_WARPS - 1) / (parts * DOWN_WARPS);
+    const int begin = (part * DOWN_WARPS + warp) * stretch, end = min(pieces, begin + stretch);
+    const T* xr = x + (size_t)row * K;
+    const T* ar = down + ((size_t)adapter * rank + r0) * K;
+    const int ranks = min(DOWN_RANKS, rank - r0);
+    for (int p = begin + lane; p < end; p += 32) {
+      if (WIDE) {
+        float xv[PIECE];
+        unpack(__ldcg(reinterpret_cast<const uint4*>(xr) + p), xv, T());
+        uint4 raw[DOWN_RANKS];
+#pragma unroll
+        for (int r = 0; r < DOWN_RANKS; ++r)
+          raw[r] = r < ranks ? __ldg(reinterpret_cast<const uint4*>(ar + (size_t)r * K) + p) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int r = 0; r < DOWN_RANKS; ++r) {
+          float av[PIECE];
+          unpack(raw[r], av, T());
+#pragma unroll
+          for (int e = 0; e < PIECE; ++e) acc[r] = fmaf(xv[e], av[e], acc[r]);
+        }
+      } else {
+        const float xv = to_float(xr[p]);
+#pragma unroll
+        for (int r = 0; r < DOWN_RANKS; ++r)
+          if (r < ranks) acc[r] = fmaf(xv, to_float(ar[(size_t)r * K + p]), acc[r]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < DOWN_RANKS; ++r) {
+      const float sum = warp_sum(acc[r]);
+      if (lane == 0) sums[warp][r] = sum;
+    }
+  }
+  __syncthreads();
+  if (live && threadIdx.x < DOWN_RANKS) {
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < DOWN_WARPS; ++w) sum += sums[w][threadIdx.x];
+    total[threadIdx.x] = sum;
+  }
+  cluster_meet();
+  if (live && part == 0 && threadIdx.x < DOWN_RANKS && r0 + (int)threadIdx.x < rank) {
+    float sum = 0.f;
+    for (int other = 0; other < parts; ++other) sum += read_from_cta(&total[threadIdx.x], other);
+    u[(size_t)row * rank + r0 + threadIdx.x] = scales[adapter] * sum;
+  }
+  cluster_meet();      // no CTA leaves while another reads its sums
+}
+
+// Up: a thread owns one output column and eight rows; B's row of the column is read once per run of rows with one adapter.
+template <typename T, typename Out, bool WIDE>
+__global__ void __launch_bounds__(128)
+adapter_up_kernel(const float* u, const T* __restrict__ up, const int* row_adapter, const float* base, Out* out, int rows, int adapters,
+                  int rank, int N) {
+  constexpr int ROWS = 8, CHUNK = 16;
+  __shared__ float low[ROWS][128];
+  __shared__ int ids[ROWS];
+  pdl_trigger();
+  pdl_wait();
+  const int row0 = blockIdx.y * ROWS;
+  const int n = blockIdx.x * 128 + threadIdx.x;
+  if (threadIdx.x < ROWS) {
+    const int m = row0 + threadIdx.x;
+    const int id = m < rows ? __ldcg(row_adapter + m) : -1;
+    ids[threadIdx.x] = id >= 0 && id < adapters ? id : -1;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < ROWS * rank; i += 128) {
+    const int r = i / rank;
+    low[r][i - r * rank] = ids[r] >= 0 ? __ldcg(u + (size_t)(row0 + r) * rank + (i - r * rank)) : 0.f;
+  }
+  __syncthreads();
+  if (n >= N) return;
+  float acc[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) acc[r] = row0 + r < rows ? __ldcg(base + (size_t)(row0 + r) * N + n) : 0.f;
+  for (int k0 = 0; k0 < rank; k0 += CHUNK) {
+    float b[CHUNK];
+    int held = -1;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const int id = ids[r];
+      if (id < 0) continue;
+      if (id != held) {
+        held = id;
+        const T* from = up + ((size_t)id * N + n) * rank + k0;
+        if (WIDE) {
+#pragma unroll
+          for (int i = 0; i < CHUNK; i += Pack<T>::N) {
+            if (k0 + i < rank) unpack(__ldg(reinterpret_cast<const uint4*>(from + i)), b + i, T());
+            else
+#pragma unroll
+              for (int e = 0; e < Pack<T>::N; ++e) b[i + e] = 0.f;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < CHUNK; ++i) b[i] = k0 + i < rank ? to_float(from[i]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < CHUNK; ++i) acc[r] = fmaf(k0 + i < rank ? low[r][k0 + i] : 0.f, b[i], acc[r]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+    if (row0 + r < rows) out[(size_t)(row0 + r) * N + n] = from_float<Out>(acc[r]);
+}
+
+template <typename T>
+static int launch_down(const void* x, const void* down, const float* scales, const int* row_adapter, float* u, int rows, int adapters,
+                       int rank, int K, cudaStream_t stream) {
+  // parts of K: as many CTAs as fill the device twice, at most eight (a cluster), none below 32 pieces per warp
+  const bool wide = K % Pack<T>::N == 0;
+  const int pieces = wide ? K / Pack<T>::N : K;
+  const int groups = (rank + DOWN_RANKS - 1) / DOWN_RANKS;
+  int parts = 1;
+  while (parts < 8 && (long long)rows * groups * parts < 4ll * sm_count() && pieces >= 2 * parts * DOWN_WARPS * 32) parts *= 2;
+  if ((long long)rows * parts > 0x7fffffff || groups > 65535) return MLR_TOO_LARGE;
+  const dim3 grid(rows * parts, groups);
+  auto kernel = wide ? adapter_down_rows_kernel<T, true> : adapter_down_rows_kernel<T, false>;
+  launch_kernel_clustered(kernel, grid, dim3(DOWN_WARPS * 32), 0, stream, parts, (const T*)x, (const T*)down, scales, row_adapter, u,
+                          adapters, rank, K, parts);
+  return launch_status();
+}
+
+template <typename T, typename Out>
+static int launch_up(const float* u, const void* up, const int* row_adapter, const float* base, void* out, int rows, int adapters, int rank,
+                     int N, cudaStream_t stream) {
+  const bool wide = rank % Pack<T>::N == 0;
+  if ((rows + 7) / 8 > 65535) return MLR_TOO_LARGE;
+  const dim3 grid((N + 127) / 128, (rows + 7) / 8);
+  auto kernel = wide ? adapter_up_kernel<T, Out, true> : adapter_up_kernel<T, Out, false>;
+  launch_kernel(kernel, grid, dim3(128), 0, stream, u, (const T*)up, row_adapter, base, (Out*)out, rows, adapters, rank, N);
+  return launch_status();
+}
+
+}  // namespace mlr
+
+using namespace mlr;
+
+MLR_DEFINE_PDL_SWITCH
+
+// x [rows, K], down [adapters, rank, K] of one dtype on 16-byte boundaries; u float32 [rows, rank].  Rows without an adapter are
+// not written.
+MLR_EXPORT int mlr_adapter_down(const void* x, const void* down, const float* scales, const int* row_adapter, float* u, int rows,
+                                int adapters, int rank, int K, int dtype, cudaStream_t stream) {
+  if (rows < 0 || adapters <= 0 || rank <= 0 || rank > 128 || K <= 0) return MLR_BAD_SIZE;
+  if (rows == 0) return MLR_OK;
+  if (((uintptr_t)x & 15) != 0 || ((uintptr_t)down & 15) != 0) return MLR_BAD_ALIGNMENT;
+  if (dtype == MLR_BF16) return launch_down<bf16>(x, down, scales, row_adapter, u, rows, adapters, rank, K, stream);
+  if (dtype == MLR_F32) return launch_down<float>(x, down, scales, row_adapter, u, rows, adapters, rank, K, stream);
+  return MLR_BAD_DTYPE;
+}
+
+// up [adapters, N, rank], base float32 [rows, N], out [rows, N] in out_dtype (float32: may be base itself).
+MLR_EXPORT int mlr_adapter_up(const float* u, const void* up, const int* row_adapter, const float* base, void* out, int rows, int adapters,
+                              int rank, int N, int dtype, int out_dtype, cudaStream_t stream) {
+  if (rows < 0 || adapters <= 0 || rank <= 0 || rank > 128 || N <= 0) return MLR_BAD_SIZE;
+  if (rows == 0) return MLR_OK;
+  if (((uintptr_t)up & 15) != 0) return MLR_BAD_ALIGNMENT;
+  if (dtype == MLR_BF16 && out_dtype == MLR_BF16)
+    return launch_up<bf16, bf16>(u, up, row_adapter, base, out, rows, adapters, rank, N, stream);
+  if (dtype == MLR_BF16 && out_dtype == MLR_F32)
+    return launch_up<bf16, float>(u, up, row_adapter, base, out, rows, adapters, rank, N, stream);
+  if (dtype == MLR_F32 && out_dtype == MLR_F32)
+    return launch_up<float, float>(u, up, row_adapter, base, out, rows, adapters, rank, N, stream);
+  return MLR_BAD_DTYPE;
+}

@@ -64,6 +64,7 @@ LIBRARIES: dict[str, tuple[str, ...]] = {
     "attention_shaped_mma": (),
     "matrix_memory": (),
     "logit_rules": (),
+    "adapters": (),
 }
 
 _loaded: dict[str, ctypes.CDLL] = {}

@@ -69,8 +69,8 @@ def _need(tensor: torch.Tensor, name: str, dtype: torch.dtype | None = None, dim
 
 
 def _need_here(**tensors: torch.Tensor | None) -> None:
-    """A launch goes to the current device's stream: tensors of another device are refused."""
-    current = torch.cuda.current_device()
+    """A launch goes to the current device's stream: tensors (and tables of tensors) of another device are refused."""
+    current = torch._C._cuda_getDevice()
     for name, tensor in tensors.items():
         if tensor is not None and tensor.device.index != current:
             raise KernelError(f"{name} is on {tensor.device}, the current device is cuda:{current}")
@@ -101,6 +101,7 @@ _PROTOTYPES = {
     "attention_tcgen05": {"mlr_attention_prefill_tcgen05": "ppppppppppp" "iiiiiiiii" "fi" "ppp" "l" "pip"},
     "attention_sigmoid_tcgen05": {"mlr_attention_sigmoid_tcgen05": "ppppp" "ppppppp" "iiiiiiii" "f" "pppp" "iii" "pp",
                                   "mlr_attention_sigmoid_tcgen05_scratch": "iiiii"},
+    "adapters": {"mlr_adapter_down": "pppppiiiiip", "mlr_adapter_up": "pppppiiiiiip"},
     "logit_rules": {"mlr_logit_rules": "pppiii" "pppppip" "p", "mlr_count_tokens": "ppippiiip"},
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
@@ -209,6 +210,38 @@ class LogitTables:
     @property
     def device(self) -> torch.device:
         return next(t for t in (self.penalties, self.bias_tokens, self.allowed) if t is not None).device
+
+
+@dataclass(frozen=True)
+class AdapterStack:
+    """The low-rank adapters of one projection [N, K], one behind the other: ``down`` [adapters, rank, K], ``up`` [adapters, N, rank]
+    in the projection's dtype, ``scales`` float32 [adapters].  An adapter of a smaller rank has zeros in its last rows of ``down``
+    (or columns of ``up``).  Checked here, once, and against the projection at each call."""
+
+    down: torch.Tensor
+    up: torch.Tensor
+    scales: torch.Tensor
+
+    MAX_RANK = 128
+
+    def __post_init__(self) -> None:
+        _code(self.down.dtype)
+        _need(self.down, "down", dims=3)
+        _need(self.up, "up", self.down.dtype, 3)
+        _need(self.scales, "scales", torch.float32, 1)
+        adapters, rank, _ = self.down.shape
+        if not 1 <= rank <= self.MAX_RANK or adapters < 1:
+            raise KernelError(f"an adapter stack needs at least one adapter of rank 1 to {self.MAX_RANK}, got {adapters} of rank {rank}")
+        if self.up.shape[0] != adapters or self.up.shape[2] != rank or self.scales.shape[0] != adapters:
+            raise KernelError(f"down {tuple(self.down.shape)}, up {tuple(self.up.shape)} and scales {tuple(self.scales.shape)} "
+                              "do not describe the same adapters")
+        if min(self.down.shape[2], self.up.shape[1]) < 1 or self.down.data_ptr() % 16 or self.up.data_ptr() % 16:
+            raise KernelError("adapters need at least one column and 16-byte boundaries")
+        _need_together(self.down, self.up, self.scales)
+
+    @property
+    def device(self) -> torch.device:
+        return self.down.device
 
 
 # Rows of one work item of the three prompt-attention kernels.
@@ -756,6 +789,41 @@ class CudaOps:
         _check(lib.mlr_linear_simt(_ptr(x), _ptr(weight), _ptr(bias), _ptr(out), x.shape[0],
                                    weight.shape[0], x.shape[1], _ptr(partial), _code(x.dtype), _code(out_dtype),
                                    _stream()), "linear")
+        return out
+
+    def linear_adapters(self, x: torch.Tensor, weight: torch.Tensor, adapters: AdapterStack, row_adapter: torch.Tensor,
+                        bias: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+        """``linear`` beside which row m passes through adapter ``row_adapter[m]`` (int32 [M]; no adapter where it is negative or
+        not in the stack): x W^T + bias + scale (x A^T) B^T, rounded once to ``out_dtype`` (default: that of x)."""
+        _need(x, "x", dims=2)
+        _need(row_adapter, "row_adapter", torch.int32, 1)
+        _need(weight, "weight", x.dtype, 2)
+        out_dtype = out_dtype or x.dtype
+        (rows, K), N, (count, rank, _) = x.shape, weight.shape[0], adapters.down.shape
+        if adapters.down.dtype != x.dtype or out_dtype not in (x.dtype, torch.float32):
+            raise KernelError(f"x in {x.dtype} needs adapters of that dtype and a result in it or float32")
+        if adapters.down.shape[2] != K or adapters.up.shape[1] != N or weight.shape[1] != K:
+            raise KernelError(f"the adapters are those of a projection {(adapters.up.shape[1], adapters.down.shape[2])}, x has {K} "
+                              f"columns and the weight is {tuple(weight.shape)}")
+        if row_adapter.shape[0] != rows:
+            raise KernelError("row_adapter needs one entry per row of x")
+        if x.data_ptr() % 16:
+            raise KernelError("x must start on a 16-byte boundary")
+        if bias is not None:
+            _need(bias, "bias", x.dtype, 1)
+            if bias.shape[0] != N:
+                raise KernelError("bias length differs from the weight's output rows")
+        _need_here(x=x, weight=weight, adapters=adapters, row_adapter=row_adapter, bias=bias)
+        if rows == 0:
+            return torch.empty((0, N), dtype=out_dtype, device=x.device)
+        low = torch.empty((rows, rank), dtype=torch.float32, device=x.device)
+        library = _declared_library("adapters")
+        _check(library.mlr_adapter_down(x.data_ptr(), adapters.down.data_ptr(), adapters.scales.data_ptr(), row_adapter.data_ptr(),
+                                        low.data_ptr(), rows, count, rank, K, _code(x.dtype), _raw_stream()), "linear_adapters (down)")
+        base = self.linear(x, weight, bias, out_dtype=torch.float32)
+        out = base if out_dtype == torch.float32 else torch.empty((rows, N), dtype=out_dtype, device=x.device)
+        _check(library.mlr_adapter_up(low.data_ptr(), adapters.up.data_ptr(), row_adapter.data_ptr(), base.data_ptr(), out.data_ptr(),
+                                      rows, count, rank, N, _code(x.dtype), _code(out_dtype), _raw_stream()), "linear_adapters (up)")
         return out
 
     # ------------------------------------------------------------------ attention

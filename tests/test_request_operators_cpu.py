@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from mini_llm_runtime_b200.ops import CudaOps, KernelError, LogitTables, cuda_ops
+from mini_llm_runtime_b200.ops import AdapterStack, CudaOps, KernelError, LogitTables, cuda_ops
 
 
 @pytest.fixture
@@ -86,8 +86,37 @@ def test_histories_that_do_not_fit(kernels, tokens, slots, tables):
         kernels.count_tokens(tokens, slots, LogitTables(**tables))
 
 
+def stack(**change):
+    return AdapterStack(**{**dict(down=torch.zeros((3, 4, 16)), up=torch.zeros((3, 24, 4)), scales=torch.ones(3)), **change})
+
+
+@pytest.mark.parametrize("change", [
+    {"down": torch.zeros((3, 4, 16), dtype=torch.float16)}, {"down": torch.zeros((3, 4, 16), dtype=torch.bfloat16)},
+    {"down": torch.zeros((2, 4, 16))}, {"down": torch.zeros((3, 5, 16))}, {"down": torch.zeros((4, 16))},
+    {"down": torch.zeros((3, 0, 16)), "up": torch.zeros((3, 24, 0))}, {"scales": torch.ones(2)},
+    {"scales": torch.ones(3, dtype=torch.float64)}, {"down": torch.zeros((3, 129, 16)), "up": torch.zeros((3, 24, 129))},
+    {"down": torch.zeros((0, 4, 16)), "up": torch.zeros((0, 24, 4)), "scales": torch.ones(0)},
+    {"down": torch.zeros((3, 4, 32))[:, :, ::2]}, {"down": torch.zeros(3 * 4 * 16 + 1)[1:].view(3, 4, 16)},
+])
+def test_stacks_that_do_not_fit(kernels, change):
+    with pytest.raises(KernelError):
+        stack(**change)
+
+
+@pytest.mark.parametrize("change", [
+    {"x": torch.zeros((5, 17))}, {"x": torch.zeros((5, 16), dtype=torch.bfloat16)}, {"x": torch.zeros((5, 32))[:, ::2]},
+    {"weight": torch.zeros((25, 16))}, {"weight": torch.zeros((24, 17))}, {"row_adapter": torch.zeros(4, dtype=torch.int32)},
+    {"row_adapter": torch.zeros(5, dtype=torch.int64)}, {"out_dtype": torch.bfloat16}, {"bias": torch.zeros(23)},
+    {"x": torch.zeros(5 * 16 + 1)[1:].view(5, 16)},
+])
+def test_projections_that_do_not_fit(kernels, change):
+    call = dict(x=torch.zeros((5, 16)), weight=torch.zeros((24, 16)), adapters=stack(), row_adapter=torch.zeros(5, dtype=torch.int32))
+    with pytest.raises(KernelError):
+        kernels.linear_adapters(**{**call, **change})
+
+
 def test_tensors_of_another_device_are_refused(monkeypatch):
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
 
     class Elsewhere:
         device = torch.device("cuda", 1)
