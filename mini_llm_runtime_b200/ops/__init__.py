@@ -11,7 +11,7 @@ from __future__ import annotations
 
 from contextlib import contextmanager
 
-from .cuda_ops import AdapterStack, AttentionBatch, CudaOps, KernelError, LogitTables
+from .cuda_ops import AdapterStack, AttentionBatch, CudaOps, KernelError, LogitTables, SharedPrefix
 
 _default = CudaOps()
 _active = _default
@@ -33,4 +33,4 @@ def use(backend):
         _active = previous
 
 
-__all__ = ["AdapterStack", "AttentionBatch", "CudaOps", "KernelError", "LogitTables", "current", "use"]
+__all__ = ["AdapterStack", "AttentionBatch", "CudaOps", "KernelError", "LogitTables", "SharedPrefix", "current", "use"]

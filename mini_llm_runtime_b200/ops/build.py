@@ -65,6 +65,7 @@ LIBRARIES: dict[str, tuple[str, ...]] = {
     "matrix_memory": (),
     "logit_rules": (),
     "adapters": (),
+    "attention_prefix": (),
 }
 
 _loaded: dict[str, ctypes.CDLL] = {}

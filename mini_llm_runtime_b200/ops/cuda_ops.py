@@ -101,6 +101,7 @@ _PROTOTYPES = {
     "attention_tcgen05": {"mlr_attention_prefill_tcgen05": "ppppppppppp" "iiiiiiiii" "fi" "ppp" "l" "pip"},
     "attention_sigmoid_tcgen05": {"mlr_attention_sigmoid_tcgen05": "ppppp" "ppppppp" "iiiiiiii" "f" "pppp" "iii" "pp",
                                   "mlr_attention_sigmoid_tcgen05_scratch": "iiiii"},
+    "attention_prefix": {"mlr_attention_prefix": "pppppppp" "ppppp" "pp" "iiiiiiiiiii" "fip"},
     "adapters": {"mlr_adapter_down": "pppppiiiiip", "mlr_adapter_up": "pppppiiiiiip"},
     "logit_rules": {"mlr_logit_rules": "pppiii" "pppppip" "p", "mlr_count_tokens": "ppippiiip"},
 }
@@ -305,6 +306,53 @@ def plan_attention(lengths: np.ndarray, position_start: np.ndarray) -> tuple[dic
               "wide": int(wide_seg.shape[0]), "big": int(big_seg.shape[0]),
               "prompt_keys": int((position_start + lengths)[longer].max()) if longer.shape[0] else 0}
     return arrays, counts
+
+
+@dataclass(frozen=True)
+class SharedPrefix:
+    """Which segments of a step share leading keys: ``plan`` holds the arrays of ``plan_shared_prefix`` on the device, ``counts``
+    what the host knows of them."""
+
+    plan: dict
+    counts: dict
+
+
+PREFIX_TILE_ROWS = 128    # attention_prefix.cu: query rows of one work item of a prefix
+
+
+def plan_shared_prefix(groups, num_segments: int, heads_per_kv: int) -> tuple[dict, dict]:
+    """Work lists of ``shared_prefix_attention`` for a step of ``num_segments`` decoded tokens: ``groups`` lists (segments, keys)
+    pairs, the requests of ``segments`` having their first ``keys`` keys on the same pages.  A segment belongs to one group at
+    most, and ``keys`` reaches no further than the shortest context of the group.  int32 arrays by name, and counts by name, as from
+    ``plan_attention``.
+
+    ``seg_keys``: shared keys before each segment's own.  ``members``: the segments of the groups, one behind the other.
+    ``tile_*``: work items of up to 128 query rows of one kv head: first member, members, keys."""
+    if not 1 <= heads_per_kv <= PREFIX_TILE_ROWS:
+        raise KernelError(f"a kv head serves 1 to {PREFIX_TILE_ROWS} query heads, not {heads_per_kv}")
+    seg_keys = np.zeros(num_segments, dtype=np.int32)
+    grouped = np.zeros(num_segments, dtype=bool)
+    members, first, count, keys_of = [], [], [], []
+    each = PREFIX_TILE_ROWS // heads_per_kv
+    for segments, keys in groups:
+        segments = [int(segment) for segment in segments]
+        if keys < 0 or any(not 0 <= segment < num_segments for segment in segments):
+            raise KernelError(f"a group of segments {segments} with {keys} keys does not fit a step of {num_segments} segments")
+        if len(set(segments)) != len(segments) or grouped[segments].any():
+            raise KernelError("a segment belongs to one group of a shared prefix, once")
+        grouped[segments] = True
+        if keys == 0 or not segments:
+            continue
+        seg_keys[segments] = keys
+        for at in range(0, len(segments), each):
+            first.append(len(members) + at)
+            count.append(min(each, len(segments) - at))
+            keys_of.append(int(keys))
+        members += segments
+    arrays = {"seg_keys": seg_keys, **{name: np.asarray(values, dtype=np.int32) for name, values in (
+        ("members", members), ("tile_first", first), ("tile_count", count), ("tile_keys", keys_of))}}
+    return arrays, {"segments": int(num_segments), "heads_per_kv": int(heads_per_kv), "tiles": len(first), "tile_keys": tuple(keys_of),
+                    "least_shared": int(seg_keys.min()) if num_segments else 0}
 
 
 def prompt_keys(batch: AttentionBatch, window: int, keep_first: int = 0) -> int:
@@ -933,6 +981,73 @@ class CudaOps:
                 *common, generic_tiles, num_heads, num_kv_heads, head_dim, value_dim,
                 page_size, int(window or 0), ctypes.c_float(scale), _code(q.dtype), _stream()),
                 "paged_attention")
+        return out
+
+    def plan_shared_prefix(self, groups, num_segments, heads_per_kv):
+        return plan_shared_prefix(groups, num_segments, heads_per_kv)
+
+    PREFIX_SCRATCH_BYTES = 256 << 20      # states of the parts of one call, at most
+    PREFIX_LEAST_CHUNK = 256              # keys of a part, at least
+
+    def _prefix_parts(self, batch, prefix, heads, kv_heads, dim, sms) -> tuple[int, int, int]:
+        """(keys of a prefix part, their number, parts of the own keys)."""
+        most = max(2, self.PREFIX_SCRATCH_BYTES // max(1, batch.num_segments * heads * (dim + 2) * 4))
+        keys = prefix.counts["tile_keys"]
+        chunk = prefix_parts = 0
+        if keys:
+            # work items of about equal length, two for every SM
+            chunk = max(self.PREFIX_LEAST_CHUNK, -(-(-(-sum(keys) * kv_heads // (2 * sms))) // 64) * 64)
+            while -(-max(keys) // chunk) > min(64, most - 1):
+                chunk *= 2
+            prefix_parts = -(-max(keys) // chunk)
+        own = max(1, batch.max_kv_len - prefix.counts["least_shared"])
+        own_parts = min(64, most - prefix_parts, -(-own // self.PREFIX_LEAST_CHUNK), 4 * sms // max(1, batch.num_segments * kv_heads))
+        return chunk, prefix_parts, max(1, own_parts)
+
+    def shared_prefix_attention(self, q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, batch: AttentionBatch,
+                                prefix: SharedPrefix, num_heads: int, num_kv_heads: int, head_dim: int, scale: float) -> torch.Tensor:
+        """``paged_attention`` of a step of decoded tokens whose requests share leading pages: the keys and values of a prefix are
+        read once for all its requests instead of once for each.  ``batch`` is the step as ``paged_attention`` takes it (a request's
+        row of the block table names the shared pages as its first); ``prefix`` says which segments share how many keys.
+        Segments of no group attend by themselves."""
+        _need(q, "q", dims=2)
+        _need(k_pool, "k_pool", q.dtype, 4)
+        _need(v_pool, "v_pool", q.dtype, 4)
+        if num_kv_heads < 1 or num_heads < 1 or num_heads % num_kv_heads or not 1 <= head_dim <= 256:
+            raise KernelError(f"{num_heads} heads over {num_kv_heads} kv heads of {head_dim} are not supported")
+        if q.shape[1] != num_heads * head_dim:
+            raise KernelError(f"q rows have {q.shape[1]} entries, expected {num_heads * head_dim}")
+        if k_pool.shape != v_pool.shape or k_pool.shape[1] != num_kv_heads or k_pool.shape[3] != head_dim:
+            raise KernelError(f"page pools have shapes {tuple(k_pool.shape)} and {tuple(v_pool.shape)}, expected "
+                              f"[pages, {num_kv_heads}, page_size, {head_dim}]")
+        segments, counts, plan = batch.num_segments, prefix.counts, prefix.plan
+        if batch.num_decode != segments or q.shape[0] != segments:
+            raise KernelError("shared_prefix_attention takes steps of one decoded token per request")
+        if counts["segments"] != segments or counts["heads_per_kv"] != num_heads // num_kv_heads:
+            raise KernelError(f"the prefix was planned for {counts['segments']} segments and {counts['heads_per_kv']} heads per kv head")
+        if counts["tile_keys"] and max(counts["tile_keys"]) > batch.max_kv_len:
+            raise KernelError(f"a prefix of {max(counts['tile_keys'])} keys in contexts of at most {batch.max_kv_len}")
+        for name, length in (("seg_keys", segments), ("tile_first", counts["tiles"]), ("tile_count", counts["tiles"]),
+                             ("tile_keys", counts["tiles"])):
+            _need(plan[name], name, torch.int32, 1)
+            if plan[name].shape[0] != length:
+                raise KernelError(f"{name} must have {length} entries, got {plan[name].shape[0]}")
+        _need(plan["members"], "members", torch.int32, 1)
+        _need(batch.block_table, "block_table", torch.int32, 2)
+        _need_here(q=q, k_pool=k_pool, v_pool=v_pool, seg_keys=plan["seg_keys"], members=plan["members"], block_table=batch.block_table)
+        out = torch.empty_like(q)
+        if segments == 0:
+            return out
+        chunk, prefix_parts, own_parts = self._prefix_parts(batch, prefix, num_heads, num_kv_heads, head_dim, self.sm_count(q.device))
+        states = (prefix_parts + own_parts) * segments * num_heads
+        scratch = torch.empty(states * (head_dim + 2), dtype=torch.float32, device=q.device)
+        _check(_declared_library("attention_prefix").mlr_attention_prefix(
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), batch.seg_q_start.data_ptr(), batch.seg_pos0.data_ptr(),
+            batch.seg_slot.data_ptr(), batch.block_table.data_ptr(), plan["seg_keys"].data_ptr(), plan["members"].data_ptr(),
+            plan["tile_first"].data_ptr(), plan["tile_count"].data_ptr(), plan["tile_keys"].data_ptr(), scratch.data_ptr(),
+            scratch.data_ptr() + states * head_dim * 4, segments, counts["tiles"], num_heads, num_kv_heads, head_dim, k_pool.shape[2],
+            k_pool.shape[0], batch.block_table.shape[1], chunk, prefix_parts, own_parts, scale, _code(q.dtype), _raw_stream()),
+            "shared_prefix_attention")
         return out
 
     def plan_decode(self, num_decode: int, num_kv_heads: int, longest: int, sms: int) -> tuple[int, int]:

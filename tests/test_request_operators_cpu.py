@@ -123,3 +123,62 @@ def test_tensors_of_another_device_are_refused(monkeypatch):
 
     with pytest.raises(KernelError, match="current device"):
         cuda_ops._need_here(x=None, weight=Elsewhere())
+
+
+# ------------------------------------------------------------------ shared prefixes
+def test_plan_of_shared_prefixes():
+    arrays, counts = cuda_ops.plan_shared_prefix([((4, 0, 2), 100), ((), 50), ((1,), 0), ((3,), 7)], 6, 50)
+    assert arrays["seg_keys"].tolist() == [100, 0, 100, 7, 100, 0]
+    assert arrays["members"].tolist() == [4, 0, 2, 3]
+    assert arrays["tile_first"].tolist() == [0, 2, 3] and arrays["tile_count"].tolist() == [2, 1, 1]
+    assert arrays["tile_keys"].tolist() == [100, 100, 7] and counts["tile_keys"] == (100, 100, 7)
+    assert counts["tiles"] == 3 and counts["least_shared"] == 0 and counts["segments"] == 6
+    assert all(array.dtype.name == "int32" for array in arrays.values())
+    empty, counts = cuda_ops.plan_shared_prefix([], 0, 7)
+    assert counts["tiles"] == 0 and empty["seg_keys"].shape == (0,)
+
+
+@pytest.mark.parametrize("groups,segments,per", [
+    ([((0, 6), 5)], 6, 1), ([((-1,), 5)], 6, 1), ([((1, 1), 5)], 6, 1), ([((0, 1), 5), ((1, 2), 5)], 6, 1), ([((0,), -1)], 6, 1),
+    ([((0, 1), 0), ((1,), 5)], 6, 1), ([], 6, 0), ([], 6, 129),
+])
+def test_groups_that_do_not_fit(groups, segments, per):
+    with pytest.raises(KernelError):
+        cuda_ops.plan_shared_prefix(groups, segments, per)
+
+
+def decoded(count, longest=50, pages=8):
+    arrays, counts = cuda_ops.plan_attention([1] * count, [longest - 1] * count)
+    index = torch.arange(count, dtype=torch.int32)
+    return cuda_ops.AttentionBatch(index, torch.ones_like(index), torch.full((count,), longest - 1, dtype=torch.int32), index,
+                                   torch.zeros((count, pages), dtype=torch.int32), count, 1, longest,
+                                   {name: torch.from_numpy(a) for name, a in arrays.items()}, counts)
+
+
+def shared(groups, count, per):
+    arrays, counts = cuda_ops.plan_shared_prefix(groups, count, per)
+    return cuda_ops.SharedPrefix({name: torch.from_numpy(a) for name, a in arrays.items()}, counts)
+
+
+@pytest.mark.parametrize("change", [
+    {"q": torch.zeros((3, 31))}, {"q": torch.zeros((2, 32))}, {"q": torch.zeros((3, 64))[:, ::2]}, {"k_pool": torch.zeros((9, 3, 16, 8))},
+    {"v_pool": torch.zeros((9, 2, 16, 16))}, {"v_pool": torch.zeros((8, 2, 16, 8))}, {"k_pool": torch.zeros((9, 2, 16, 8), dtype=torch.bfloat16)},
+    {"batch": decoded(4)}, {"prefix": shared([((0, 1), 16)], 4, 2)}, {"prefix": shared([((0, 1), 16)], 3, 4)},
+    {"prefix": shared([((0, 1), 51)], 3, 2)}, {"num_heads": 5}, {"num_kv_heads": 0}, {"head_dim": 0},
+    {"prefix": cuda_ops.SharedPrefix({**shared([((0, 1), 16)], 3, 2).plan, "tile_keys": torch.zeros(2, dtype=torch.int32)},
+                                     shared([((0, 1), 16)], 3, 2).counts)},
+])
+def test_attention_that_does_not_fit(kernels, change):
+    call = dict(q=torch.zeros((3, 32)), k_pool=torch.zeros((9, 2, 16, 8)), v_pool=torch.zeros((9, 2, 16, 8)), batch=decoded(3),
+                prefix=shared([((0, 1), 16)], 3, 2), num_heads=4, num_kv_heads=2, head_dim=8, scale=0.3)
+    with pytest.raises(KernelError):
+        kernels.shared_prefix_attention(**{**call, **change})
+
+
+def test_a_prompt_portion_is_refused(kernels):
+    arrays, counts = cuda_ops.plan_attention([1, 2, 1], [5, 5, 5])
+    batch = decoded(3)
+    batch.counts = counts
+    with pytest.raises(KernelError, match="decoded token"):
+        kernels.shared_prefix_attention(torch.zeros((3, 32)), torch.zeros((9, 2, 16, 8)), torch.zeros((9, 2, 16, 8)), batch,
+                                        shared([], 3, 2), 4, 2, 8, 0.3)
