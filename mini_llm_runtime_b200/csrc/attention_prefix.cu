@@ -12,6 +12,7 @@
 // Rows of a work item: of a prefix, the query heads of one kv head of up to 128 / heads_per_kv requests; of own keys, those of
 // one request.
 #include "mma_attention.cuh"
+#include "tcgen05.cuh"
 
 namespace mlr {
 
@@ -152,6 +153,417 @@ prefix_parts_plain_kernel(const PrefixCall c) {
   }
 }
 
+// ------------------------------------------------------------------ prefixes on tcgen05 (bfloat16, heads of 64 and 128)
+// One work item is 128 query rows of one kv head (the query heads of up to 128 / heads_per_kv requests) over one part of the
+// prefix: bound by the products once a few dozen requests share it, by its keys' bytes below.  Six warps: four of softmax, one
+// thread per query row (tensor-memory lane); one that issues S = Q K^T two key tiles ahead and O += P V; one that loads, K and V
+// page by page through bulk tensor copies into a ring.  The output stays in tensor memory relative to a base exponent that
+// follows the running max in steps of 2^8.  The query rows lie in the q of as many requests: the softmax threads gather them.
+constexpr int PT_ROWS = 128, PT_KEYS = 64, PT_THREADS = 192;
+constexpr uint32_t PT_TMEM_COLS = 256, PT_TMEM_O = 2 * PT_KEYS;      // S0 | S1 | O
+constexpr int PT_P_BYTES = PT_ROWS * PT_KEYS * 2;
+constexpr float PT_LAZY = 8.f;
+
+template <int D>
+struct PrefixShape {
+  static constexpr int HALVES = D / 64;
+  static constexpr int STAGES = D == 64 ? 4 : 2;
+  static constexpr int Q_BYTES = PT_ROWS * D * 2, Q_HALF = PT_ROWS * 128;
+  static constexpr int TILE_BYTES = PT_KEYS * D * 2, HALF = PT_KEYS * 128, STAGE_BYTES = 2 * TILE_BYTES;
+  static constexpr int DATA_BYTES = Q_BYTES + PT_P_BYTES + STAGES * STAGE_BYTES;
+};
+
+struct PrefixControl {
+  uint64_t q_full, k_full[4], v_full[4], qk_done[4], pv_done[4], p_ready;
+  uint32_t tmem_holder;
+};
+
+template <int D>
+__global__ void __launch_bounds__(PT_THREADS, 2)
+prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const PrefixCall c,
+                            int page_shift, int* error_word) {
+  using Shape = PrefixShape<D>;
+  constexpr int STAGES = Shape::STAGES;
+  extern __shared__ uint8_t prefix_raw[];
+  uint8_t* q_tile = (uint8_t*)(((uintptr_t)prefix_raw + 1023) & ~(uintptr_t)1023);      // [halves][128][64]
+  uint8_t* p_tile = q_tile + Shape::Q_BYTES;                                             // [128][64]
+  uint8_t* ring = p_tile + PT_P_BYTES;                                                   // stages of (K, V), each [halves][64][64]
+  __shared__ PrefixControl ctl;
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int tile = blockIdx.y, kv_head = blockIdx.z, part = blockIdx.x;
+  if (threadIdx.x == 0) {
+    mbar_init(&ctl.q_full, 4);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&ctl.k_full[s], 1); mbar_init(&ctl.qk_done[s], 1);
+      mbar_init(&ctl.v_full[s], 1); mbar_init(&ctl.pv_done[s], 1);
+    }
+    mbar_init(&ctl.p_ready, 4);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
+  }
+  if (warp == 4) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_holder)), "r"(PT_TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fa_fence_before();
+  __syncthreads();
+  fa_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl.tmem_holder, 0);
+  pdl_wait();                       // before the first read of q, tables and cache
+  pdl_trigger();                    // after it: see prefix_own_mma_kernel
+
+  const int begin = part * c.chunk, end = min(c.tile_keys[tile], begin + c.chunk);
+  if (begin >= end) {               // a shorter prefix has fewer parts
+    if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(PT_TMEM_COLS) : "memory");
+    return;
+  }
+  const int per = c.heads / c.kv_heads;
+  const int first_member = c.tile_first[tile], rows = c.tile_count[tile] * per;
+  const int tiles = (end - begin + PT_KEYS - 1) / PT_KEYS;
+  bool gave_up = false;
+
+  if (warp == 5) {
+    // ------------------------------------------------------------ loads
+    const int boxes = c.page_size >= PT_KEYS ? 1 : PT_KEYS >> page_shift;
+    const int box_rows = c.page_size >= PT_KEYS ? PT_KEYS : c.page_size;
+    const int* table = c.block_table + (size_t)__ldcg(c.seg_slot + c.members[first_member]) * c.table_width;
+    auto lookup = [&](int j) -> int {                     // the page of this lane's box, a tile before its copies
+      if (j >= tiles || lane >= boxes * Shape::HALVES) return 0;
+      const int logical = (begin + j * PT_KEYS + (lane % boxes) * box_rows) >> page_shift;
+      return logical < c.table_width ? max(0, __ldcg(table + logical)) : 0;
+    };
+    auto load = [&](int j, int page, bool values) {
+      const int stage = j % STAGES;
+      if (j >= STAGES) fa_wait(values ? &ctl.pv_done[stage] : &ctl.qk_done[stage], (unsigned)(j / STAGES - 1) & 1u, error_word, 0x71, gave_up);
+      gave_up = __any_sync(0xffffffffu, gave_up);
+      if (gave_up) return;
+      uint64_t* full = values ? &ctl.v_full[stage] : &ctl.k_full[stage];
+      if (lane == 0) mbar_expect_tx(full, Shape::TILE_BYTES);
+      __syncwarp();
+      if (lane < boxes * Shape::HALVES) {
+        const int box = lane % boxes, half = lane / boxes;
+        const int offset = (begin + j * PT_KEYS + box * box_rows) & (c.page_size - 1);
+        uint8_t* dst = ring + (size_t)stage * Shape::STAGE_BYTES + (values ? Shape::TILE_BYTES : 0) + half * Shape::HALF + box * box_rows * 128;
+        tma_load_2d(values ? &v_map : &k_map, full, dst, half * 64, (page * c.kv_heads + kv_head) * c.page_size + offset);
+      }
+    };
+    // K of tile j + 1 goes out before V of tile j: the scores come first.  pages: of tiles j, j + 1 and j + 2
+    int page = lookup(0), next = lookup(1);
+    load(0, page, false);
+    for (int j = 0; j < tiles; ++j) {
+      const int after = lookup(j + 2);
+      if (j + 1 < tiles) load(j + 1, next, false);
+      load(j, page, true);
+      page = next;
+      next = after;
+    }
+  } else if (warp == 4) {
+    // ------------------------------------------------------------ MMAs
+    constexpr uint32_t idesc_qk = fa_idesc(PT_ROWS, PT_KEYS, false);
+    constexpr uint32_t idesc_pv = fa_idesc(PT_ROWS, D, true);
+    const uint64_t q_desc = fa_desc_k_major(smem_u32(q_tile)), k_desc0 = fa_desc_k_major(smem_u32(ring));
+    const uint64_t v_desc0 = fa_desc_mn_major(smem_u32(ring) + Shape::TILE_BYTES, Shape::HALF), p_desc = fa_desc_k_major(smem_u32(p_tile));
+    auto issue_qk = [&](int j) {      // the score buffer j & 1 is free: tile j - 2's scores were read before its probabilities arrived
+      const int stage = j % STAGES;
+      fa_wait(&ctl.k_full[stage], (unsigned)(j / STAGES) & 1u, error_word, 0x72, gave_up);
+      gave_up = __any_sync(0xffffffffu, gave_up);
+      fa_fence_after();
+      if (!gave_up && elect_one()) {
+        const uint64_t k_desc = k_desc0 + (uint64_t)((stage * Shape::STAGE_BYTES) >> 4);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          fa_mma(tmem_base + (j & 1) * PT_KEYS, q_desc + (uint64_t)(((k >> 2) * Shape::Q_HALF + (k & 3) * 32) >> 4),
+                 k_desc + (uint64_t)(((k >> 2) * Shape::HALF + (k & 3) * 32) >> 4), idesc_qk, k > 0 ? 1u : 0u);
+        fa_commit(&ctl.qk_done[stage]);
+      }
+      __syncwarp();
+    };
+    fa_wait(&ctl.q_full, 0u, error_word, 0x73, gave_up);
+    issue_qk(0);
+    if (tiles > 1) issue_qk(1);
+    for (int j = 0; j < tiles; ++j) {
+      const int stage = j % STAGES;
+      fa_wait(&ctl.p_ready, (unsigned)j & 1u, error_word, 0x74, gave_up);
+      fa_wait(&ctl.v_full[stage], (unsigned)(j / STAGES) & 1u, error_word, 0x75, gave_up);
+      gave_up = __any_sync(0xffffffffu, gave_up);
+      fa_fence_after();
+      if (!gave_up && elect_one()) {
+        const uint64_t v_desc = v_desc0 + (uint64_t)((stage * Shape::STAGE_BYTES) >> 4);
+#pragma unroll
+        for (int k = 0; k < PT_KEYS / 16; ++k)
+          fa_mma(tmem_base + PT_TMEM_O, p_desc + (uint64_t)((k * 32) >> 4), v_desc + (uint64_t)((k * 2048) >> 4), idesc_pv,
+                 (j > 0 || k > 0) ? 1u : 0u);
+        fa_commit(&ctl.pv_done[stage]);
+      }
+      __syncwarp();
+      if (j + 2 < tiles) issue_qk(j + 2);
+    }
+  } else {
+    // ------------------------------------------------------------ softmax, one thread per query row
+    const int r = threadIdx.x;
+    const bool live = r < rows;
+    const int segment = live ? c.members[first_member + r / per] : 0, head = kv_head * per + r % per;
+    {
+      const uint4* from = reinterpret_cast<const uint4*>((const bf16*)c.q + ((size_t)(live ? c.q_row[segment] : 0) * c.heads + head) * D);
+      uint4 piece[D / 8];
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) piece[i] = live ? __ldcg(from + i) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+        *reinterpret_cast<uint4*>(q_tile + (i >> 3) * Shape::Q_HALF + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = piece[i];
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.q_full);
+    }
+    const uint32_t lane_base = tmem_base + ((uint32_t)(warp * 32) << 16);
+    const bool warp_live = warp * 32 < rows;      // a warp of no rows only keeps the barriers going
+    float m_run = -INFINITY, m_base = -INFINITY, l = 0.f;
+    const float2 scale2 = make_float2(c.scale_log2, c.scale_log2);
+    for (int j = 0; j < tiles; ++j) {
+      const int stage = j % STAGES, key0 = begin + j * PT_KEYS;
+      const bool ragged = key0 + PT_KEYS > end;
+      fa_wait(&ctl.qk_done[stage], (unsigned)(j / STAGES) & 1u, error_word, 0x76, gave_up);
+      fa_fence_after();
+      float s[PT_KEYS];
+      bool step = false;
+      float alpha = 1.f;
+      if (warp_live) {
+#pragma unroll
+        for (int i = 0; i < PT_KEYS; i += 16) fa_tmem_load16(lane_base + (j & 1) * PT_KEYS + i, reinterpret_cast<uint32_t*>(s) + i);
+        fa_tmem_wait_ld();
+        fa_fence_before();
+        if (ragged) {
+#pragma unroll
+          for (int i = 0; i < PT_KEYS; ++i)
+            if (key0 + i >= end) s[i] = -INFINITY;
+        }
+        float part_max[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int i = 4; i < PT_KEYS - 4; i += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) part_max[e] = fa_max3(part_max[e], s[i + 2 * e], s[i + 2 * e + 1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part_max[e] = fmaxf(part_max[e], s[PT_KEYS - 4 + e]);
+        const float tile_max = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
+        m_run = fmaxf(m_run, tile_max * c.scale_log2);
+        step = m_run - m_base > PT_LAZY;          // nothing seen yet: NaN, no step
+        alpha = step ? fa_exp2(m_base - m_run) : 1.f;
+        if (step) m_base = m_run;
+        const float base = m_base == -INFINITY ? 0.f : m_base;
+        const float2 minus_base = make_float2(-base, -base);
+        float2 part_sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int i = 0; i < PT_KEYS; i += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 x = __ffma2_rn(make_float2(s[i + 2 * e], s[i + 2 * e + 1]), scale2, minus_base);
+            s[i + 2 * e] = fa_exp2(x.x);
+            s[i + 2 * e + 1] = fa_exp2(x.y);
+            part_sum[e] = __fadd2_rn(part_sum[e], make_float2(s[i + 2 * e], s[i + 2 * e + 1]));
+          }
+        const float2 sum2 = __fadd2_rn(__fadd2_rn(part_sum[0], part_sum[1]), __fadd2_rn(part_sum[2], part_sum[3]));
+        l = fmaf(l, alpha, sum2.x + sum2.y);
+      }
+      const bool rescale = j > 0 && __any_sync(0xffffffffu, step);
+      if (j > 0) {      // the previous tile's P V: it has read the probabilities, and the output may be touched
+        fa_wait(&ctl.pv_done[(j - 1) % STAGES], (unsigned)((j - 1) / STAGES) & 1u, error_word, 0x77, gave_up);
+        fa_fence_after();
+      }
+      if (rescale) {
+        const float2 alpha2 = make_float2(alpha, alpha);
+#pragma unroll
+        for (int d0 = 0; d0 < D; d0 += 32) {
+          float o[32];
+          fa_tmem_load16(lane_base + PT_TMEM_O + d0, reinterpret_cast<uint32_t*>(o));
+          fa_tmem_load16(lane_base + PT_TMEM_O + d0 + 16, reinterpret_cast<uint32_t*>(o) + 16);
+          fa_tmem_wait_ld();
+#pragma unroll
+          for (int d = 0; d < 32; d += 2) {
+            const float2 scaled = __fmul2_rn(make_float2(o[d], o[d + 1]), alpha2);
+            o[d] = scaled.x;
+            o[d + 1] = scaled.y;
+          }
+          fa_tmem_store16(lane_base + PT_TMEM_O + d0, reinterpret_cast<const uint32_t*>(o));
+          fa_tmem_store16(lane_base + PT_TMEM_O + d0 + 16, reinterpret_cast<const uint32_t*>(o) + 16);
+        }
+        fa_tmem_wait_st();
+      }
+      if (ragged) {      // what stands behind the last key becomes zero: a weight of zero times NaN is NaN
+        fa_wait(&ctl.v_full[stage], (unsigned)(j / STAGES) & 1u, error_word, 0x78, gave_up);
+        uint8_t* v_tile = ring + (size_t)stage * Shape::STAGE_BYTES + Shape::TILE_BYTES;
+        for (int i = threadIdx.x; i < PT_KEYS * 8 * Shape::HALVES; i += 128) {
+          const int half = i / (PT_KEYS * 8), within = i - half * (PT_KEYS * 8);
+          if (key0 + (within >> 3) >= end)
+            *reinterpret_cast<uint4*>(v_tile + half * Shape::HALF + (within >> 3) * 128 + (within & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+      if (warp_live || j == 0) {      // rows past the last are zeros, written once
+        uint8_t* p_row = p_tile + r * 128;
+#pragma unroll
+        for (int chunk = 0; chunk < 8; ++chunk) {
+          uint32_t packed[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) packed[e] = warp_live ? pack_bf16(s[chunk * 8 + 2 * e], s[chunk * 8 + 2 * e + 1]) : 0u;
+          *reinterpret_cast<uint4*>(p_row + ((chunk ^ (r & 7)) << 4)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      fa_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.p_ready);
+    }
+    fa_wait(&ctl.pv_done[(tiles - 1) % STAGES], (unsigned)((tiles - 1) / STAGES) & 1u, error_word, 0x79, gave_up);
+    fa_fence_after();
+    const size_t at = ((size_t)part * c.segments + segment) * c.heads + head;
+#pragma unroll
+    for (int d0 = 0; d0 < D; d0 += 32) {
+      float o[32];
+      fa_tmem_load16(lane_base + PT_TMEM_O + d0, reinterpret_cast<uint32_t*>(o));
+      fa_tmem_load16(lane_base + PT_TMEM_O + d0 + 16, reinterpret_cast<uint32_t*>(o) + 16);
+      fa_tmem_wait_ld();
+      if (live) {
+        float4* to = reinterpret_cast<float4*>(c.acc + at * D + d0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+      }
+    }
+    if (live) {
+      c.state[2 * at] = m_base;
+      c.state[2 * at + 1] = l;
+    }
+    fa_fence_before();
+  }
+  __syncthreads();
+  if (warp == 4) {
+    fa_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(PT_TMEM_COLS) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------ own keys on mma.sync (bfloat16, heads of 64 and 128)
+// CTA = (request, part of its own keys, kv head): bound by reading them, each once.  The rows of the MMA are the query heads
+// of the kv head (up to 16); the four warps take 16 keys each of a 64-key tile, three or four tiles in flight.  The warps'
+// states meet in shared memory.
+// AFTER_PREFIX: launched behind the prefix kernel, which lets the next kernel in after its own wait: everything before both is
+// done then, and what this kernel reads is written by neither; it starts beside the prefix kernel and waits for it at its end.
+template <int D>
+struct OwnShape {
+  static constexpr int STAGES = D == 64 ? 4 : 3;
+  static constexpr int STAGE_BYTES = 2 * 64 * D * 2;
+  static constexpr int SHARED = STAGES * STAGE_BYTES;
+  static constexpr int PITCH = D + 4;
+  static_assert(4 * 16 * (PITCH + 2) * 4 <= SHARED, "the warps' states fit where the tiles were");
+};
+
+template <int D, bool AFTER_PREFIX>
+__global__ void __launch_bounds__(128)
+prefix_own_mma_kernel(const PrefixCall c, int page_shift) {
+  using Shape = OwnShape<D>;
+  constexpr int STAGES = Shape::STAGES, CHUNKS = D / 8;
+  extern __shared__ __align__(128) uint8_t own_shared[];
+  if (!AFTER_PREFIX) pdl_wait();
+  pdl_trigger();
+  const int segment = blockIdx.y, kv_head = blockIdx.z, part = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int begin, end;
+  own_range(c, segment, part, &begin, &end);
+  if (begin < end) {
+    const int per = c.heads / c.kv_heads;
+    const int* table = c.block_table + (size_t)__ldcg(c.seg_slot + segment) * c.table_width;
+    const int tiles = (end - begin + 63) / 64;
+    auto load = [&](int j) {
+      if (j < tiles) {
+        bf16* k_tile = reinterpret_cast<bf16*>(own_shared + (j % STAGES) * Shape::STAGE_BYTES);
+        bf16* v_tile = k_tile + 64 * D;
+        for (int i = threadIdx.x; i < 64 * CHUNKS; i += 128) {
+          const int row = i / CHUNKS, chunk = i - row * CHUNKS, key = begin + j * 64 + row;
+          size_t at = 0;
+          bool held = key < end;
+          if (held) {
+            const int logical = page_shift >= 0 ? key >> page_shift : key / c.page_size;
+            const int page = logical < c.table_width ? __ldcg(table + logical) : -1;
+            held = page >= 0 && page < c.pages;
+            if (held) at = (((size_t)page * c.kv_heads + kv_head) * c.page_size + (key - logical * c.page_size)) * D + chunk * 8;
+          }
+          cp_async_16(tile_at<D>(k_tile, row, chunk), (const bf16*)c.k_pool + at, held);
+          cp_async_16(tile_at<D>(v_tile, row, chunk), (const bf16*)c.v_pool + at, held);
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int j = 0; j < STAGES - 1; ++j) load(j);
+    // fragments of q: rows lane / 4 and lane / 4 + 8, columns 2 * (lane & 3) and 8 further
+    uint32_t q_frag[D / 16][4];
+    const bf16* q = (const bf16*)c.q + ((size_t)c.q_row[segment] * c.heads + kv_head * per) * D;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = (lane >> 2) + (e & 1) * 8, column = ks * 16 + (lane & 3) * 2 + (e >> 1) * 8;
+        q_frag[ks][e] = row < per ? __ldcg(reinterpret_cast<const unsigned*>(q + (size_t)row * D + column)) : 0u;
+      }
+    float o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const int low[2] = {0, 0}, high[2] = {end - 1, end - 1};
+    for (int j = 0; j < tiles; ++j) {
+      load(j + STAGES - 1);
+      cp_async_wait<STAGES - 1>();
+      __syncthreads();
+      bf16* k_tile = reinterpret_cast<bf16*>(own_shared + (j % STAGES) * Shape::STAGE_BYTES);
+      const int key0 = begin + j * 64 + warp * 16;
+      float s[2][4];
+      warp_qk<D, 2>(s, q_frag, k_tile, warp * 16, lane);
+      if (key0 + 15 < end) softmax_step<2, D / 8, false>(s, o, m, l, key0, low, high, c.scale_log2, lane);
+      else softmax_step<2, D / 8>(s, o, m, l, key0, low, high, c.scale_log2, lane);
+      warp_pv<D, 2>(o, s, k_tile + 64 * D, warp * 16, lane);
+      __syncthreads();
+    }
+    // the four warps' states, then their sum
+    float* states = reinterpret_cast<float*>(own_shared);          // [4][16][PITCH], then [4][16][2]
+    float* sums = states + 4 * 16 * Shape::PITCH;
+    cp_async_wait<0>();
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        states[(warp * 16 + (lane >> 2) + (e >> 1) * 8) * Shape::PITCH + i * 8 + (lane & 3) * 2 + (e & 1)] = o[i][e];
+    if ((lane & 3) == 0)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        sums[2 * (warp * 16 + (lane >> 2) + i * 8)] = m[i];
+        sums[2 * (warp * 16 + (lane >> 2) + i * 8) + 1] = l[i];
+      }
+    __syncthreads();
+    const size_t at0 = ((size_t)(c.prefix_parts + part) * c.segments + segment) * c.heads + kv_head * per;
+    for (int i = threadIdx.x; i < per * D; i += 128) {
+      const int row = i / D, d = i - row * D;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, sums[2 * (w * 16 + row)]);
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, value = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float factor = exp2f(sums[2 * (w * 16 + row)] - base);
+        sum = fmaf(sums[2 * (w * 16 + row) + 1], factor, sum);
+        value = fmaf(states[(w * 16 + row) * Shape::PITCH + d], factor, value);
+      }
+      c.acc[(at0 + row) * D + d] = value;
+      if (d == 0) {
+        c.state[2 * (at0 + row)] = top;
+        c.state[2 * (at0 + row) + 1] = sum;
+      }
+    }
+  }
+  if (AFTER_PREFIX) pdl_wait();
+}
+
 // ------------------------------------------------------------------ the parts put together
 // One warp per (segment, head); a row that sees no key is zero.
 template <typename T>
@@ -214,6 +626,32 @@ static int run_plain(const PrefixCall& c, cudaStream_t stream) {
   return launch_status();
 }
 
+template <int D>
+static int run_fast(const PrefixCall& c, int* error_word, cudaStream_t stream) {
+  using Shape = PrefixShape<D>;
+  static OncePerDevice once[3];
+  const size_t prefix_shared = Shape::DATA_BYTES + 1024, own_shared = OwnShape<D>::SHARED;
+  auto allow = [](auto kernel, size_t bytes) { return [=] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes); }; };
+  if (cudaError_t err = once[0](allow(prefix_parts_tcgen05_kernel<D>, prefix_shared))) return (int)err;
+  if (cudaError_t err = once[1](allow(prefix_own_mma_kernel<D, true>, own_shared))) return (int)err;
+  if (cudaError_t err = once[2](allow(prefix_own_mma_kernel<D, false>, own_shared))) return (int)err;
+  int page_shift = -1;
+  for (int shift = 0; shift < 31; ++shift)
+    if (c.page_size == 1 << shift) page_shift = shift;
+  if (c.tiles > 0) {
+    CUtensorMap k_map, v_map;
+    const long long rows = (long long)c.pages * c.kv_heads * c.page_size;
+    const int box = c.page_size < PT_KEYS ? c.page_size : PT_KEYS;
+    if (!cached_tile_map(&k_map, c.k_pool, rows, D, box) || !cached_tile_map(&v_map, c.v_pool, rows, D, box)) return MLR_BAD_ALIGNMENT;
+    launch_kernel(prefix_parts_tcgen05_kernel<D>, dim3(c.prefix_parts, c.tiles, c.kv_heads), dim3(PT_THREADS), prefix_shared, stream, k_map, v_map,
+                  c, page_shift, error_word);
+  }
+  auto own = c.tiles > 0 ? prefix_own_mma_kernel<D, true> : prefix_own_mma_kernel<D, false>;
+  launch_kernel(own, dim3(c.own_parts, c.segments, c.kv_heads), dim3(128), own_shared, stream, c, page_shift);
+  launch_kernel(prefix_merge_kernel<bf16>, dim3((c.segments * c.heads + 3) / 4), dim3(128), 0, stream, c);
+  return launch_status();
+}
+
 }  // namespace mlr
 
 using namespace mlr;
@@ -221,12 +659,13 @@ using namespace mlr;
 MLR_DEFINE_PDL_SWITCH
 
 // q, out [rows, heads * dim], pools [pages, kv_heads, page_size, dim] of one dtype.  acc, state: float32, (prefix_parts + own_parts) *
-// segments * heads * dim and * 2 of them.  chunk: keys of a prefix part (prefix_parts of them reach the longest prefix).
+// segments * heads * dim and * 2 of them.  fast: the tensor cores (bfloat16, dim 64 or 128, at most 16 heads per kv head, pages of a
+// power of two from 8 on); else any type and size.  chunk: keys of a prefix part (prefix_parts of them reach the longest prefix).
 MLR_EXPORT int mlr_attention_prefix(const void* q, const void* k_pool, const void* v_pool, void* out, const int* q_row, const int* pos0,
                                     const int* seg_slot, const int* block_table, const int* seg_keys, const int* members,
                                     const int* tile_first, const int* tile_count, const int* tile_keys, float* acc, float* state,
                                     int segments, int tiles, int heads, int kv_heads, int dim, int page_size, int pages, int table_width,
-                                    int chunk, int prefix_parts, int own_parts, float scale, int dtype, cudaStream_t stream) {
+                                    int chunk, int prefix_parts, int own_parts, float scale, int dtype, int fast, int* error_word, cudaStream_t stream) {
   if (segments < 0 || tiles < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || dim <= 0 || page_size <= 0 || pages <= 0 ||
       table_width <= 0 || own_parts <= 0 || prefix_parts < 0 || (tiles > 0 && (chunk <= 0 || prefix_parts <= 0)))
     return MLR_BAD_SIZE;
@@ -235,6 +674,15 @@ MLR_EXPORT int mlr_attention_prefix(const void* q, const void* k_pool, const voi
   const PrefixCall c{q, k_pool, v_pool, q_row, pos0, seg_slot, block_table, seg_keys, members, tile_first, tile_count, tile_keys, acc, state, out,
                      segments, tiles, heads, kv_heads, dim, page_size, pages, table_width, chunk, prefix_parts, own_parts,
                      scale * 1.4426950408889634f};
+  if (fast) {
+    const bool boxes = page_size >= 8 && (page_size & (page_size - 1)) == 0;      // a box of a tile is eight rows at least
+    const bool rows_fit = (long long)pages * kv_heads * page_size <= 0x7fffffff && chunk % PT_KEYS == 0;
+    if (dtype != MLR_BF16 || heads / kv_heads > 16 || !boxes || !rows_fit) return MLR_BAD_SIZE;
+    if ((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)acc) & 15) != 0) return MLR_BAD_ALIGNMENT;
+    if (dim == 64) return run_fast<64>(c, error_word, stream);
+    if (dim == 128) return run_fast<128>(c, error_word, stream);
+    return MLR_BAD_SIZE;
+  }
   if (dtype == MLR_BF16) return run_plain<bf16>(c, stream);
   if (dtype == MLR_F32) return run_plain<float>(c, stream);
   return MLR_BAD_DTYPE;

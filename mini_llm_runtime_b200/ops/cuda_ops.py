@@ -101,7 +101,7 @@ _PROTOTYPES = {
     "attention_tcgen05": {"mlr_attention_prefill_tcgen05": "ppppppppppp" "iiiiiiiii" "fi" "ppp" "l" "pip"},
     "attention_sigmoid_tcgen05": {"mlr_attention_sigmoid_tcgen05": "ppppp" "ppppppp" "iiiiiiii" "f" "pppp" "iii" "pp",
                                   "mlr_attention_sigmoid_tcgen05_scratch": "iiiii"},
-    "attention_prefix": {"mlr_attention_prefix": "pppppppp" "ppppp" "pp" "iiiiiiiiiii" "fip"},
+    "attention_prefix": {"mlr_attention_prefix": "pppppppp" "ppppp" "pp" "iiiiiiiiiii" "fiipp"},
     "adapters": {"mlr_adapter_down": "pppppiiiiip", "mlr_adapter_up": "pppppiiiiiip"},
     "logit_rules": {"mlr_logit_rules": "pppiii" "pppppip" "p", "mlr_count_tokens": "ppippiiip"},
 }
@@ -1039,15 +1039,19 @@ class CudaOps:
         if segments == 0:
             return out
         chunk, prefix_parts, own_parts = self._prefix_parts(batch, prefix, num_heads, num_kv_heads, head_dim, self.sm_count(q.device))
+        page_size = k_pool.shape[2]
+        fast = (self.use_mma_attention and q.dtype == torch.bfloat16 and head_dim in (64, 128) and num_heads // num_kv_heads <= 16
+                and page_size >= 8 and page_size & (page_size - 1) == 0 and k_pool.shape[0] * num_kv_heads * page_size < 1 << 31
+                and not (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr()) % 16)
         states = (prefix_parts + own_parts) * segments * num_heads
         scratch = torch.empty(states * (head_dim + 2), dtype=torch.float32, device=q.device)
         _check(_declared_library("attention_prefix").mlr_attention_prefix(
             q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), batch.seg_q_start.data_ptr(), batch.seg_pos0.data_ptr(),
             batch.seg_slot.data_ptr(), batch.block_table.data_ptr(), plan["seg_keys"].data_ptr(), plan["members"].data_ptr(),
             plan["tile_first"].data_ptr(), plan["tile_count"].data_ptr(), plan["tile_keys"].data_ptr(), scratch.data_ptr(),
-            scratch.data_ptr() + states * head_dim * 4, segments, counts["tiles"], num_heads, num_kv_heads, head_dim, k_pool.shape[2],
-            k_pool.shape[0], batch.block_table.shape[1], chunk, prefix_parts, own_parts, scale, _code(q.dtype), _raw_stream()),
-            "shared_prefix_attention")
+            scratch.data_ptr() + states * head_dim * 4, segments, counts["tiles"], num_heads, num_kv_heads, head_dim, page_size,
+            k_pool.shape[0], batch.block_table.shape[1], chunk, prefix_parts, own_parts, scale, _code(q.dtype),
+            int(fast), self._error_word(q.device).data_ptr(), _raw_stream()), "shared_prefix_attention")
         return out
 
     def plan_decode(self, num_decode: int, num_kv_heads: int, longest: int, sms: int) -> tuple[int, int]:
