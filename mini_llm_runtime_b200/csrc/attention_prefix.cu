@@ -32,13 +32,14 @@ struct PrefixCall {
   float scale_log2;
 };
 
-// A segment's own keys [begin, end) of part `part`; empty if there are fewer parts.  Multiples of 64 keys from the first own key on.
-__device__ __forceinline__ void own_range(const PrefixCall& c, int segment, int part, int* begin, int* end) {
-  const int first = c.seg_keys[segment], last = __ldcg(c.pos0 + segment) + 1;
+// A segment's own keys [begin, end) of part `part`, and how many parts have any.
+__device__ __forceinline__ int own_range(const PrefixCall& c, int segment, int part, int* begin, int* end) {
+  const int first = c.seg_keys[segment], last = c.pos0[segment] + 1;
   const int own = max(0, last - first);
   const int each = max(OWN_LEAST, ((own + c.own_parts - 1) / c.own_parts + 63) & ~63);
   *begin = min(last, first + part * each);
   *end = min(last, *begin + each);
+  return (own + each - 1) / each;
 }
 
 // A cached row's place: null where the request holds no such page.
@@ -178,6 +179,14 @@ struct PrefixControl {
   uint32_t tmem_holder;
 };
 
+constexpr int PT_CONTROL_BYTES = 256;
+static_assert(sizeof(PrefixControl) <= PT_CONTROL_BYTES, "control block");
+// Two CTAs share the 228 KB of an SM, of which each costs 1 KB by itself: 768 bytes are left for the alignment of the tiles (the
+// buffer starts on a 1,024-byte boundary where a kernel has no other shared memory).  With 1,024 there was one CTA per SM:
+// 2.5 us instead of 1.3 for two key tiles.
+template <int D> constexpr int PT_SHARED = PrefixShape<D>::DATA_BYTES + PT_CONTROL_BYTES + 512;
+static_assert(2 * (PT_SHARED<128> + 1024) <= 228 * 1024, "two CTAs per SM");
+
 template <int D>
 __global__ void __launch_bounds__(PT_THREADS, 2)
 prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const PrefixCall c,
@@ -186,12 +195,40 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
   constexpr int STAGES = Shape::STAGES;
   extern __shared__ uint8_t prefix_raw[];
   uint8_t* q_tile = (uint8_t*)(((uintptr_t)prefix_raw + 1023) & ~(uintptr_t)1023);      // [halves][128][64]
+  if (q_tile + Shape::DATA_BYTES + PT_CONTROL_BYTES > prefix_raw + PT_SHARED<D>) {      // no room for the alignment
+    if (threadIdx.x == 0) atomicCAS(error_word, 0, 0x70);
+    return;
+  }
   uint8_t* p_tile = q_tile + Shape::Q_BYTES;                                             // [128][64]
   uint8_t* ring = p_tile + PT_P_BYTES;                                                   // stages of (K, V), each [halves][64][64]
-  __shared__ PrefixControl ctl;
+  PrefixControl& ctl = *reinterpret_cast<PrefixControl*>(ring + STAGES * Shape::STAGE_BYTES);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int tile = blockIdx.y, kv_head = blockIdx.z, part = blockIdx.x;
+  // Which item and part this CTA is: the parts of all items in a row.  Like the segments' slots and the block table these are
+  // the step's metadata, complete before any kernel of the step lets the next one in.
+  const int kv_head = blockIdx.y;
+  int tile = 0, part = blockIdx.x, keys = 0;
+  for (int t0 = 0; t0 < c.tiles; t0 += 32) {
+    const int mine = t0 + lane < c.tiles ? c.tile_keys[t0 + lane] : 0;
+    const int parts = (mine + c.chunk - 1) / c.chunk;
+    int upto = parts;      // parts of the items up to and with this lane's
+#pragma unroll
+    for (int step = 1; step < 32; step <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, upto, step);
+      if (lane >= step) upto += other;
+    }
+    const unsigned found = __ballot_sync(0xffffffffu, part < upto);
+    if (found != 0u) {
+      const int at = __ffs(found) - 1;
+      tile = t0 + at;
+      part -= __shfl_sync(0xffffffffu, upto - parts, at);
+      keys = __shfl_sync(0xffffffffu, mine, at);
+      break;
+    }
+    part -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  const int begin = part * c.chunk, end = min(keys, begin + c.chunk);
+  const int first_member = c.tile_first[tile];
   if (threadIdx.x == 0) {
     mbar_init(&ctl.q_full, 4);
     for (int s = 0; s < STAGES; ++s) {
@@ -203,6 +240,20 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
     asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
   }
+  const int boxes = c.page_size >= PT_KEYS ? 1 : PT_KEYS >> page_shift;
+  const int box_rows = c.page_size >= PT_KEYS ? PT_KEYS : c.page_size;
+  const int tiles = (end - begin + PT_KEYS - 1) / PT_KEYS;
+  const int* table = c.block_table + (size_t)c.seg_slot[c.members[first_member]] * c.table_width;
+  auto lookup = [&](int j) -> int {                     // the page of this lane's box of key tile j
+    if (j >= tiles || lane >= boxes * Shape::HALVES) return 0;
+    const int logical = (begin + j * PT_KEYS + (lane % boxes) * box_rows) >> page_shift;
+    return logical < c.table_width ? max(0, table[logical]) : 0;
+  };
+  int first_pages[STAGES + 2];
+  if (warp == 5) {
+#pragma unroll
+    for (int j = 0; j < STAGES + 2; ++j) first_pages[j] = lookup(j);
+  }
   if (warp == 4) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_holder)), "r"(PT_TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -211,29 +262,15 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
   __syncthreads();
   fa_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl.tmem_holder, 0);
-  pdl_wait();                       // before the first read of q, tables and cache
+  pdl_wait();                       // before the first read of q and cache
   pdl_trigger();                    // after it: see prefix_own_mma_kernel
 
-  const int begin = part * c.chunk, end = min(c.tile_keys[tile], begin + c.chunk);
-  if (begin >= end) {               // a shorter prefix has fewer parts
-    if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(PT_TMEM_COLS) : "memory");
-    return;
-  }
   const int per = c.heads / c.kv_heads;
-  const int first_member = c.tile_first[tile], rows = c.tile_count[tile] * per;
-  const int tiles = (end - begin + PT_KEYS - 1) / PT_KEYS;
+  const int rows = c.tile_count[tile] * per;
   bool gave_up = false;
 
   if (warp == 5) {
     // ------------------------------------------------------------ loads
-    const int boxes = c.page_size >= PT_KEYS ? 1 : PT_KEYS >> page_shift;
-    const int box_rows = c.page_size >= PT_KEYS ? PT_KEYS : c.page_size;
-    const int* table = c.block_table + (size_t)__ldcg(c.seg_slot + c.members[first_member]) * c.table_width;
-    auto lookup = [&](int j) -> int {                     // the page of this lane's box, a tile before its copies
-      if (j >= tiles || lane >= boxes * Shape::HALVES) return 0;
-      const int logical = (begin + j * PT_KEYS + (lane % boxes) * box_rows) >> page_shift;
-      return logical < c.table_width ? max(0, __ldcg(table + logical)) : 0;
-    };
     auto load = [&](int j, int page, bool values) {
       const int stage = j % STAGES;
       if (j >= STAGES) fa_wait(values ? &ctl.pv_done[stage] : &ctl.qk_done[stage], (unsigned)(j / STAGES - 1) & 1u, error_word, 0x71, gave_up);
@@ -249,15 +286,20 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
         tma_load_2d(values ? &v_map : &k_map, full, dst, half * 64, (page * c.kv_heads + kv_head) * c.page_size + offset);
       }
     };
-    // K of tile j + 1 goes out before V of tile j: the scores come first.  pages: of tiles j, j + 1 and j + 2
-    int page = lookup(0), next = lookup(1);
-    load(0, page, false);
+    // In the order in which the MMA warp frees the stages: a K stage once the scores that read it exist, and they run two tiles
+    // ahead of the softmax; a V stage once its product is done.  pages: of tiles j + STAGES - 1, + 1 and + 2
+    int pages[3] = {first_pages[STAGES - 1], first_pages[STAGES], first_pages[STAGES + 1]};
+#pragma unroll
+    for (int j = 0; j < STAGES; ++j)
+      if (j < tiles) { load(j, first_pages[j], false); load(j, first_pages[j], true); }
+    if (STAGES < tiles) load(STAGES, pages[1], false);
     for (int j = 0; j < tiles; ++j) {
-      const int after = lookup(j + 2);
-      if (j + 1 < tiles) load(j + 1, next, false);
-      load(j, page, true);
-      page = next;
-      next = after;
+      const int after = lookup(j + STAGES + 2);
+      if (j >= 1 && j + STAGES - 1 < tiles) load(j + STAGES - 1, pages[0], true);
+      if (j + STAGES + 1 < tiles) load(j + STAGES + 1, pages[2], false);
+      pages[0] = pages[1];
+      pages[1] = pages[2];
+      pages[2] = after;
     }
   } else if (warp == 4) {
     // ------------------------------------------------------------ MMAs
@@ -443,116 +485,218 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
 }
 
 // ------------------------------------------------------------------ own keys on mma.sync (bfloat16, heads of 64 and 128)
-// CTA = (request, part of its own keys, kv head): bound by reading them, each once.  The rows of the MMA are the query heads
-// of the kv head (up to 16); the four warps take 16 keys each of a 64-key tile, three or four tiles in flight.  The warps'
-// states meet in shared memory.
+// CTA = (request, part of its own keys, kv head): bound by reading them, each once.  Keys are the MMA's rows and the query heads
+// its eight columns (S^T = K Q^T, O^T = V^T P^T), so that the usual five to eight heads of a kv head fill them: half the
+// products and registers of heads as rows, and three CTAs per SM.  Four warps take 16 keys each of a 64-key tile; a fifth loads,
+// page by page through bulk tensor copies, as far ahead as the ring is deep (by asynchronous copies of the four warps each table
+// read stood in front of its copies: 68 MB of own keys took 72 us from cold caches).  The warps' states meet in shared memory.
 // AFTER_PREFIX: launched behind the prefix kernel, which lets the next kernel in after its own wait: everything before both is
 // done then, and what this kernel reads is written by neither; it starts beside the prefix kernel and waits for it at its end.
+constexpr int OWN_THREADS = 160;
+
 template <int D>
 struct OwnShape {
-  static constexpr int STAGES = D == 64 ? 4 : 3;
-  static constexpr int STAGE_BYTES = 2 * 64 * D * 2;
-  static constexpr int SHARED = STAGES * STAGE_BYTES;
+  static constexpr int HALVES = D / 64;
+  static constexpr int STAGES = D == 64 ? 4 : 2;
+  static constexpr int TILE_BYTES = 64 * D * 2, HALF = 64 * 128, STAGE_BYTES = 2 * TILE_BYTES;
+  static constexpr int DATA_BYTES = STAGES * STAGE_BYTES;
   static constexpr int PITCH = D + 4;
-  static_assert(4 * 16 * (PITCH + 2) * 4 <= SHARED, "the warps' states fit where the tiles were");
+  static_assert(4 * 16 * (PITCH + 2) * 4 <= DATA_BYTES, "the warps' states fit where the tiles were");
 };
 
-template <int D, bool AFTER_PREFIX>
-__global__ void __launch_bounds__(128)
-prefix_own_mma_kernel(const PrefixCall c, int page_shift) {
+// An 8 x 8 matrix of 16-bit elements turned over: row g, columns 2t and 2t + 1 of lane 4g + t.
+__device__ __forceinline__ uint32_t turned(uint32_t v) {
+  uint32_t w;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(w) : "r"(v));
+  return w;
+}
+
+template <int D, int NT, bool AFTER_PREFIX>
+__global__ void __launch_bounds__(OWN_THREADS)
+prefix_own_mma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const PrefixCall c,
+                      int page_shift, int* error_word) {
   using Shape = OwnShape<D>;
-  constexpr int STAGES = Shape::STAGES, CHUNKS = D / 8;
-  extern __shared__ __align__(128) uint8_t own_shared[];
-  if (!AFTER_PREFIX) pdl_wait();
-  pdl_trigger();
+  constexpr int STAGES = Shape::STAGES, HEADS = NT * 8;
+  extern __shared__ uint8_t own_raw[];
+  uint8_t* ring = (uint8_t*)(((uintptr_t)own_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t full[4], empty[4];
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 4); }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   const int segment = blockIdx.y, kv_head = blockIdx.z, part = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int begin, end;
   own_range(c, segment, part, &begin, &end);
-  if (begin < end) {
+  const int first = begin & ~63;      // tiles start where pages and copies do; keys before `begin` are masked
+  const int tiles = begin < end ? (end - first + 63) / 64 : 0;
+  const int boxes = c.page_size >= 64 ? 1 : 64 >> page_shift, box_rows = c.page_size >= 64 ? 64 : c.page_size;
+  const int* table = c.block_table + (size_t)c.seg_slot[segment] * c.table_width;
+  auto lookup = [&](int j) -> int {
+    if (j >= tiles || lane >= boxes * Shape::HALVES) return 0;
+    const int logical = (first + j * 64 + (lane % boxes) * box_rows) >> page_shift;
+    return logical < c.table_width ? max(0, table[logical]) : 0;
+  };
+  int pages[STAGES];
+  if (warp == 4) {
+#pragma unroll
+    for (int j = 0; j < STAGES; ++j) pages[j] = lookup(j);
+  }
+  __syncthreads();
+  if (!AFTER_PREFIX) pdl_wait();
+  pdl_trigger();
+  if (tiles > 0) {
     const int per = c.heads / c.kv_heads;
-    const int* table = c.block_table + (size_t)__ldcg(c.seg_slot + segment) * c.table_width;
-    const int tiles = (end - begin + 63) / 64;
-    auto load = [&](int j) {
-      if (j < tiles) {
-        bf16* k_tile = reinterpret_cast<bf16*>(own_shared + (j % STAGES) * Shape::STAGE_BYTES);
-        bf16* v_tile = k_tile + 64 * D;
-        for (int i = threadIdx.x; i < 64 * CHUNKS; i += 128) {
-          const int row = i / CHUNKS, chunk = i - row * CHUNKS, key = begin + j * 64 + row;
-          size_t at = 0;
-          bool held = key < end;
-          if (held) {
-            const int logical = page_shift >= 0 ? key >> page_shift : key / c.page_size;
-            const int page = logical < c.table_width ? __ldcg(table + logical) : -1;
-            held = page >= 0 && page < c.pages;
-            if (held) at = (((size_t)page * c.kv_heads + kv_head) * c.page_size + (key - logical * c.page_size)) * D + chunk * 8;
+    bool gave_up = false;
+    if (warp == 4) {
+      for (int j0 = 0; j0 < tiles; j0 += STAGES) {
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) {
+          const int j = j0 + i;
+          if (j < tiles) {
+            const int page = pages[i];
+            pages[i] = lookup(j + STAGES);
+            if (j0 > 0) fa_wait(&empty[i], (unsigned)(j0 / STAGES - 1) & 1u, error_word, 0x7a, gave_up);
+            gave_up = __any_sync(0xffffffffu, gave_up);
+            if (!gave_up) {
+              if (lane == 0) mbar_expect_tx(&full[i], Shape::STAGE_BYTES);
+              __syncwarp();
+              if (lane < boxes * Shape::HALVES) {
+                const int box = lane % boxes, half = lane / boxes;
+                const int y = (page * c.kv_heads + kv_head) * c.page_size + ((first + j * 64 + box * box_rows) & (c.page_size - 1));
+                uint8_t* dst = ring + i * Shape::STAGE_BYTES + half * Shape::HALF + box * box_rows * 128;
+                tma_load_2d(&k_map, &full[i], dst, half * 64, y);
+                tma_load_2d(&v_map, &full[i], dst + Shape::TILE_BYTES, half * 64, y);
+              }
+            }
           }
-          cp_async_16(tile_at<D>(k_tile, row, chunk), (const bf16*)c.k_pool + at, held);
-          cp_async_16(tile_at<D>(v_tile, row, chunk), (const bf16*)c.v_pool + at, held);
         }
       }
-      cp_async_commit();
-    };
+    }
+    // of heads 2t and 2t + 1 (t = lane & 3) of each eight: output rows d = 16 i + g and 8 further (g = lane / 4)
+    float o[D / 16][NT][4];
+    float m[NT][2], l[NT][2];
+    if (warp < 4) {
+      uint32_t q_frag[D / 16][NT][2];
+      const bf16* q = (const bf16*)c.q + ((size_t)c.q_row[segment] * c.heads + kv_head * per) * D;
 #pragma unroll
-    for (int j = 0; j < STAGES - 1; ++j) load(j);
-    // fragments of q: rows lane / 4 and lane / 4 + 8, columns 2 * (lane & 3) and 8 further
-    uint32_t q_frag[D / 16][4];
-    const bf16* q = (const bf16*)c.q + ((size_t)c.q_row[segment] * c.heads + kv_head * per) * D;
+      for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = (lane >> 2) + (e & 1) * 8, column = ks * 16 + (lane & 3) * 2 + (e >> 1) * 8;
-        q_frag[ks][e] = row < per ? __ldcg(reinterpret_cast<const unsigned*>(q + (size_t)row * D + column)) : 0u;
+          for (int e = 0; e < 2; ++e) {
+            const int head = n * 8 + (lane >> 2), column = ks * 16 + (lane & 3) * 2 + e * 8;
+            q_frag[ks][n][e] = head < per ? __ldcg(reinterpret_cast<const unsigned*>(q + (size_t)head * D + column)) : 0u;
+          }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
       }
-    float o[D / 8][4];
+      for (int j = 0; j < tiles; ++j) {
+        const int stage = j % STAGES;
+        fa_wait(&full[stage], (unsigned)(j / STAGES) & 1u, error_word, 0x7b, gave_up);
+        bf16* k_tile = reinterpret_cast<bf16*>(ring + stage * Shape::STAGE_BYTES);
+        bf16* v_tile = k_tile + 64 * D;
+        const int key0 = first + j * 64 + warp * 16;
+        const bool ragged = key0 < begin || key0 + 15 >= end;
+        if (key0 < end && key0 + 15 >= begin) {
+          if (ragged) {      // what stands in front of and behind the keys becomes zero: a weight of zero times NaN is NaN
+            for (int i = lane; i < 16 * D / 8; i += 32) {
+              const int row = i / (D / 8), chunk = i - row * (D / 8);
+              if (key0 + row < begin || key0 + row >= end)
+                *reinterpret_cast<uint4*>(tile_at<D, true>(v_tile, warp * 16 + row, chunk)) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            __syncwarp();
+          }
+          float s[NT][4];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    const int low[2] = {0, 0}, high[2] = {end - 1, end - 1};
-    for (int j = 0; j < tiles; ++j) {
-      load(j + STAGES - 1);
-      cp_async_wait<STAGES - 1>();
-      __syncthreads();
-      bf16* k_tile = reinterpret_cast<bf16*>(own_shared + (j % STAGES) * Shape::STAGE_BYTES);
-      const int key0 = begin + j * 64 + warp * 16;
-      float s[2][4];
-      warp_qk<D, 2>(s, q_frag, k_tile, warp * 16, lane);
-      if (key0 + 15 < end) softmax_step<2, D / 8, false>(s, o, m, l, key0, low, high, c.scale_log2, lane);
-      else softmax_step<2, D / 8>(s, o, m, l, key0, low, high, c.scale_log2, lane);
-      warp_pv<D, 2>(o, s, k_tile + 64 * D, warp * 16, lane);
-      __syncthreads();
+          for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            uint32_t a[4];
+            ldmatrix_x4(a, tile_at<D, true>(k_tile, warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, ks * 2 + (lane >> 4)));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_bf16(s[n], a, q_frag[ks][n][0], q_frag[ks][n][1]);
+          }
+          uint32_t p[NT][2];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const int low = key0 + (lane >> 2), high = low + 8;
+            const bool see_low = !ragged || (low >= begin && low < end), see_high = !ragged || (high >= begin && high < end);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              s[n][e] = see_low ? s[n][e] * c.scale_log2 : -INFINITY;
+              s[n][e + 2] = see_high ? s[n][e + 2] * c.scale_log2 : -INFINITY;
+              float top = fmaxf(s[n][e], s[n][e + 2]);
+#pragma unroll
+              for (int step = 4; step < 32; step <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+              const float now = fmaxf(m[n][e], top), base = now == -INFINITY ? 0.f : now;
+              const float alpha = exp2f(m[n][e] - base);
+              m[n][e] = now;
+              s[n][e] = exp2f(s[n][e] - base);
+              s[n][e + 2] = exp2f(s[n][e + 2] - base);
+              l[n][e] = fmaf(l[n][e], alpha, s[n][e] + s[n][e + 2]);      // of this lane's keys; the lanes' sums meet at the end
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) { o[i][n][e] *= alpha; o[i][n][e + 2] *= alpha; }
+            }
+            p[n][0] = turned(pack_bf16(s[n][0], s[n][1]));
+            p[n][1] = turned(pack_bf16(s[n][2], s[n][3]));
+          }
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t a[4];
+            ldmatrix_x4_trans(a, tile_at<D, true>(v_tile, warp * 16 + (lane & 7) + (lane >> 4) * 8, i * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_bf16(o[i][n], a, p[n][0], p[n][1]);
+          }
+          // the zeros before the tensor copy that reuses the stage
+          if (ragged) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stage]);
+      }
     }
     // the four warps' states, then their sum
-    float* states = reinterpret_cast<float*>(own_shared);          // [4][16][PITCH], then [4][16][2]
-    float* sums = states + 4 * 16 * Shape::PITCH;
-    cp_async_wait<0>();
+    float* states = reinterpret_cast<float*>(ring);                // [4][HEADS][PITCH], then [4][HEADS][2]
+    float* sums = states + 4 * HEADS * Shape::PITCH;
     __syncthreads();
+    if (warp < 4) {
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        states[(warp * 16 + (lane >> 2) + (e >> 1) * 8) * Shape::PITCH + i * 8 + (lane & 3) * 2 + (e & 1)] = o[i][e];
-    if ((lane & 3) == 0)
+        for (int e = 0; e < 2; ++e) {
+          const int head = n * 8 + (lane & 3) * 2 + e;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        sums[2 * (warp * 16 + (lane >> 2) + i * 8)] = m[i];
-        sums[2 * (warp * 16 + (lane >> 2) + i * 8) + 1] = l[i];
-      }
+          for (int i = 0; i < D / 16; ++i) {
+            states[(warp * HEADS + head) * Shape::PITCH + i * 16 + (lane >> 2)] = o[i][n][e];
+            states[(warp * HEADS + head) * Shape::PITCH + i * 16 + (lane >> 2) + 8] = o[i][n][e + 2];
+          }
+          float sum = l[n][e];
+#pragma unroll
+          for (int step = 4; step < 32; step <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, step);
+          if (lane < 4) {
+            sums[2 * (warp * HEADS + head)] = m[n][e];
+            sums[2 * (warp * HEADS + head) + 1] = sum;
+          }
+        }
+    }
     __syncthreads();
     const size_t at0 = ((size_t)(c.prefix_parts + part) * c.segments + segment) * c.heads + kv_head * per;
-    for (int i = threadIdx.x; i < per * D; i += 128) {
+    for (int i = threadIdx.x; i < per * D; i += OWN_THREADS) {
       const int row = i / D, d = i - row * D;
       float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) top = fmaxf(top, sums[2 * (w * 16 + row)]);
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, sums[2 * (w * HEADS + row)]);
       const float base = top == -INFINITY ? 0.f : top;
       float sum = 0.f, value = 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const float factor = exp2f(sums[2 * (w * 16 + row)] - base);
-        sum = fmaf(sums[2 * (w * 16 + row) + 1], factor, sum);
-        value = fmaf(states[(w * 16 + row) * Shape::PITCH + d], factor, value);
+        const float factor = exp2f(sums[2 * (w * HEADS + row)] - base);
+        sum = fmaf(sums[2 * (w * HEADS + row) + 1], factor, sum);
+        value = fmaf(states[(w * HEADS + row) * Shape::PITCH + d], factor, value);
       }
       c.acc[(at0 + row) * D + d] = value;
       if (d == 0) {
@@ -565,46 +709,82 @@ prefix_own_mma_kernel(const PrefixCall c, int page_shift) {
 }
 
 // ------------------------------------------------------------------ the parts put together
-// One warp per (segment, head); a row that sees no key is zero.
-template <typename T>
+// One warp per (segment, head); a row that sees no key is zero.  W floats per lane and load (4 where rows are whole 16-byte
+// pieces); the states of up to 32 parts come with one load, the outputs of eight parts are in flight together.
+template <typename T, int W>
 __global__ void __launch_bounds__(128)
 prefix_merge_kernel(const PrefixCall c) {
+  constexpr int PIECES = 8 / W, AHEAD = W == 4 ? 8 : 4;
   pdl_trigger();
-  pdl_wait();
   const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= c.segments * c.heads) return;
+  if (row >= c.segments * c.heads) { pdl_wait(); return; }
   const int segment = row / c.heads;
-  const int shared = c.seg_keys[segment];
-  const int prefix = c.chunk > 0 ? (shared + c.chunk - 1) / c.chunk : 0;
-  int own = 0;
-  for (int part = 0; part < c.own_parts; ++part) {
-    int begin, end;
-    own_range(c, segment, part, &begin, &end);
-    own += begin < end;
-  }
-  const int parts = prefix + own;
+  int begin, end;
+  const int own = own_range(c, segment, 0, &begin, &end);
+  const int prefix = c.chunk > 0 ? (c.seg_keys[segment] + c.chunk - 1) / c.chunk : 0;
+  const int parts = prefix + own, q_row = c.q_row[segment];
   const size_t pitch = (size_t)c.segments * c.heads;
   auto place = [&](int part) { return (size_t)(part < prefix ? part : c.prefix_parts + part - prefix) * pitch + row; };
-  float top = -INFINITY;
-  for (int part = lane; part < parts; part += 32) top = fmaxf(top, __ldcg(c.state + 2 * place(part)));
-  top = warp_max(top);
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int part = 0; part < parts; ++part) {
-    const size_t at = place(part);
-    const float factor = exp2f(__ldcg(c.state + 2 * at) - base);
-    sum = fmaf(__ldcg(c.state + 2 * at + 1), factor, sum);
+  pdl_wait();
+  float top = -INFINITY, sum = 0.f;
+  float o[PIECES][W];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < c.dim) o[i] = fmaf(__ldcg(c.acc + at * c.dim + lane + 32 * i), factor, o[i]);
+  for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+    for (int e = 0; e < W; ++e) o[i][e] = 0.f;
+  for (int part0 = 0; part0 < parts; part0 += 32) {
+    float2 state = make_float2(-INFINITY, 0.f);
+    if (part0 + lane < parts) state = __ldcg(reinterpret_cast<const float2*>(c.state) + place(part0 + lane));
+    const float now = fmaxf(top, warp_max(state.x)), base = now == -INFINITY ? 0.f : now;
+    const float before = exp2f(top - base), mine = exp2f(state.x - base);
+    top = now;
+    sum = sum * before + warp_sum(mine * state.y);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+      for (int e = 0; e < W; ++e) o[i][e] *= before;
+    const int count = min(32, parts - part0);
+    for (int k0 = 0; k0 < count; k0 += AHEAD) {
+      float v[AHEAD][PIECES][W];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          const int d = (i * 32 + lane) * W;
+          const bool there = k0 + k < count && d < c.dim;
+          const float* from = c.acc + place(part0 + k0 + k) * c.dim + d;
+          if (W == 4) {
+            const float4 four = there ? __ldcg(reinterpret_cast<const float4*>(from)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[k][i][0] = four.x; v[k][i][W > 1 ? 1 : 0] = four.y; v[k][i][W > 2 ? 2 : 0] = four.z; v[k][i][W > 3 ? 3 : 0] = four.w;
+          } else {
+            v[k][i][0] = there ? __ldcg(from) : 0.f;
+          }
+        }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const float factor = __shfl_sync(0xffffffffu, mine, min(31, k0 + k));
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+          for (int e = 0; e < W; ++e)
+            if (k0 + k < count) o[i][e] = fmaf(v[k][i][e], factor, o[i][e]);
+      }
+    }
   }
   const float inverse = sum == 0.f ? 0.f : 1.f / sum;      // NaN stays
-  T* to = (T*)c.out + ((size_t)c.q_row[segment] * c.heads + (row - segment * c.heads)) * c.dim;
+  T* to = (T*)c.out + ((size_t)q_row * c.heads + (row - segment * c.heads)) * c.dim;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (lane + 32 * i < c.dim) to[lane + 32 * i] = from_float<T>(o[i] * inverse);
+  for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      const int d = (i * 32 + lane) * W + e;
+      if (d < c.dim) to[d] = from_float<T>(o[i][e] * inverse);
+    }
+}
+
+template <typename T>
+static void launch_merge(const PrefixCall& c, cudaStream_t stream) {
+  launch_kernel(c.dim % 4 == 0 ? prefix_merge_kernel<T, 4> : prefix_merge_kernel<T, 1>, dim3((c.segments * c.heads + 3) / 4), dim3(128), 0, stream, c);
 }
 
 template <typename T>
@@ -622,33 +802,30 @@ static int run_plain(const PrefixCall& c, cudaStream_t stream) {
                   stream, c);
   launch_kernel(prefix_parts_plain_kernel<T, false>, dim3(c.own_parts * ((per + PLAIN_ROWS - 1) / PLAIN_ROWS), c.segments, c.kv_heads),
                 dim3(PLAIN_THREADS), shared, stream, c);
-  launch_kernel(prefix_merge_kernel<T>, dim3((c.segments * c.heads + 3) / 4), dim3(128), 0, stream, c);
+  launch_merge<T>(c, stream);
   return launch_status();
 }
 
-template <int D>
-static int run_fast(const PrefixCall& c, int* error_word, cudaStream_t stream) {
-  using Shape = PrefixShape<D>;
+template <int D, int NT>
+static int run_fast(const PrefixCall& c, int units, int* error_word, cudaStream_t stream) {
   static OncePerDevice once[3];
-  const size_t prefix_shared = Shape::DATA_BYTES + 1024, own_shared = OwnShape<D>::SHARED;
+  const size_t prefix_shared = PT_SHARED<D>, own_shared = OwnShape<D>::DATA_BYTES + 1024;
   auto allow = [](auto kernel, size_t bytes) { return [=] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes); }; };
   if (cudaError_t err = once[0](allow(prefix_parts_tcgen05_kernel<D>, prefix_shared))) return (int)err;
-  if (cudaError_t err = once[1](allow(prefix_own_mma_kernel<D, true>, own_shared))) return (int)err;
-  if (cudaError_t err = once[2](allow(prefix_own_mma_kernel<D, false>, own_shared))) return (int)err;
-  int page_shift = -1;
-  for (int shift = 0; shift < 31; ++shift)
-    if (c.page_size == 1 << shift) page_shift = shift;
-  if (c.tiles > 0) {
-    CUtensorMap k_map, v_map;
-    const long long rows = (long long)c.pages * c.kv_heads * c.page_size;
-    const int box = c.page_size < PT_KEYS ? c.page_size : PT_KEYS;
-    if (!cached_tile_map(&k_map, c.k_pool, rows, D, box) || !cached_tile_map(&v_map, c.v_pool, rows, D, box)) return MLR_BAD_ALIGNMENT;
-    launch_kernel(prefix_parts_tcgen05_kernel<D>, dim3(c.prefix_parts, c.tiles, c.kv_heads), dim3(PT_THREADS), prefix_shared, stream, k_map, v_map,
-                  c, page_shift, error_word);
-  }
-  auto own = c.tiles > 0 ? prefix_own_mma_kernel<D, true> : prefix_own_mma_kernel<D, false>;
-  launch_kernel(own, dim3(c.own_parts, c.segments, c.kv_heads), dim3(128), own_shared, stream, c, page_shift);
-  launch_kernel(prefix_merge_kernel<bf16>, dim3((c.segments * c.heads + 3) / 4), dim3(128), 0, stream, c);
+  if (cudaError_t err = once[1](allow(prefix_own_mma_kernel<D, NT, true>, own_shared))) return (int)err;
+  if (cudaError_t err = once[2](allow(prefix_own_mma_kernel<D, NT, false>, own_shared))) return (int)err;
+  int page_shift = 0;
+  while (1 << page_shift < c.page_size) ++page_shift;
+  CUtensorMap k_map, v_map;
+  const long long rows = (long long)c.pages * c.kv_heads * c.page_size;
+  const int box = c.page_size < PT_KEYS ? c.page_size : PT_KEYS;
+  if (!cached_tile_map(&k_map, c.k_pool, rows, D, box) || !cached_tile_map(&v_map, c.v_pool, rows, D, box)) return MLR_BAD_ALIGNMENT;
+  if (units > 0)
+    launch_kernel(prefix_parts_tcgen05_kernel<D>, dim3(units, c.kv_heads), dim3(PT_THREADS), prefix_shared, stream, k_map, v_map, c, page_shift,
+                  error_word);
+  auto own = units > 0 ? prefix_own_mma_kernel<D, NT, true> : prefix_own_mma_kernel<D, NT, false>;
+  launch_kernel(own, dim3(c.own_parts, c.segments, c.kv_heads), dim3(OWN_THREADS), own_shared, stream, k_map, v_map, c, page_shift, error_word);
+  launch_merge<bf16>(c, stream);
   return launch_status();
 }
 
@@ -660,14 +837,15 @@ MLR_DEFINE_PDL_SWITCH
 
 // q, out [rows, heads * dim], pools [pages, kv_heads, page_size, dim] of one dtype.  acc, state: float32, (prefix_parts + own_parts) *
 // segments * heads * dim and * 2 of them.  fast: the tensor cores (bfloat16, dim 64 or 128, at most 16 heads per kv head, pages of a
-// power of two from 8 on); else any type and size.  chunk: keys of a prefix part (prefix_parts of them reach the longest prefix).
+// power of two from 8 on); else any type and size.  chunk: keys of a prefix part; prefix_parts of them
+// reach the longest prefix, and all items have `units` parts together.
 MLR_EXPORT int mlr_attention_prefix(const void* q, const void* k_pool, const void* v_pool, void* out, const int* q_row, const int* pos0,
                                     const int* seg_slot, const int* block_table, const int* seg_keys, const int* members,
                                     const int* tile_first, const int* tile_count, const int* tile_keys, float* acc, float* state,
                                     int segments, int tiles, int heads, int kv_heads, int dim, int page_size, int pages, int table_width,
-                                    int chunk, int prefix_parts, int own_parts, float scale, int dtype, int fast, int* error_word, cudaStream_t stream) {
+                                    int chunk, int prefix_parts, int own_parts, int units, float scale, int dtype, int fast, int* error_word, cudaStream_t stream) {
   if (segments < 0 || tiles < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || dim <= 0 || page_size <= 0 || pages <= 0 ||
-      table_width <= 0 || own_parts <= 0 || prefix_parts < 0 || (tiles > 0 && (chunk <= 0 || prefix_parts <= 0)))
+      table_width <= 0 || own_parts <= 0 || prefix_parts < 0 || (tiles > 0 && (chunk <= 0 || prefix_parts <= 0 || units < tiles)))
     return MLR_BAD_SIZE;
   if (segments == 0) return MLR_OK;
   if (dim > 256 || heads / kv_heads > 128 || segments > 65535 || tiles > 65535 || kv_heads > 65535) return MLR_TOO_LARGE;
@@ -679,8 +857,8 @@ MLR_EXPORT int mlr_attention_prefix(const void* q, const void* k_pool, const voi
     const bool rows_fit = (long long)pages * kv_heads * page_size <= 0x7fffffff && chunk % PT_KEYS == 0;
     if (dtype != MLR_BF16 || heads / kv_heads > 16 || !boxes || !rows_fit) return MLR_BAD_SIZE;
     if ((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)acc) & 15) != 0) return MLR_BAD_ALIGNMENT;
-    if (dim == 64) return run_fast<64>(c, error_word, stream);
-    if (dim == 128) return run_fast<128>(c, error_word, stream);
+    if (dim == 64) return heads / kv_heads <= 8 ? run_fast<64, 1>(c, units, error_word, stream) : run_fast<64, 2>(c, units, error_word, stream);
+    if (dim == 128) return heads / kv_heads <= 8 ? run_fast<128, 1>(c, units, error_word, stream) : run_fast<128, 2>(c, units, error_word, stream);
     return MLR_BAD_SIZE;
   }
   if (dtype == MLR_BF16) return run_plain<bf16>(c, stream);

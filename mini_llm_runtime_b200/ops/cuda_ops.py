@@ -101,7 +101,7 @@ _PROTOTYPES = {
     "attention_tcgen05": {"mlr_attention_prefill_tcgen05": "ppppppppppp" "iiiiiiiii" "fi" "ppp" "l" "pip"},
     "attention_sigmoid_tcgen05": {"mlr_attention_sigmoid_tcgen05": "ppppp" "ppppppp" "iiiiiiii" "f" "pppp" "iii" "pp",
                                   "mlr_attention_sigmoid_tcgen05_scratch": "iiiii"},
-    "attention_prefix": {"mlr_attention_prefix": "pppppppp" "ppppp" "pp" "iiiiiiiiiii" "fiipp"},
+    "attention_prefix": {"mlr_attention_prefix": "pppppppp" "ppppp" "pp" "iiiiiiiiiiii" "fiipp"},
     "adapters": {"mlr_adapter_down": "pppppiiiiip", "mlr_adapter_up": "pppppiiiiiip"},
     "logit_rules": {"mlr_logit_rules": "pppiii" "pppppip" "p", "mlr_count_tokens": "ppippiiip"},
 }
@@ -995,11 +995,13 @@ class CudaOps:
         keys = prefix.counts["tile_keys"]
         chunk = prefix_parts = 0
         if keys:
-            # work items of about equal length, two for every SM
-            chunk = max(self.PREFIX_LEAST_CHUNK, -(-(-(-sum(keys) * kv_heads // (2 * sms))) // 64) * 64)
-            while -(-max(keys) // chunk) > min(64, most - 1):
-                chunk *= 2
-            prefix_parts = -(-max(keys) // chunk)
+            # the shortest parts whose work items are all resident at once, two on an SM (a few short of that many: one item in a
+            # second round would take as long as the first)
+            chunk, longest, resident = self.PREFIX_LEAST_CHUNK, max(keys), 2 * sms - sms // 16
+            while chunk < longest and (-(-longest // chunk) > min(64, most - 1)
+                                       or sum(-(-n // chunk) for n in keys) * kv_heads > resident):
+                chunk += 64
+            prefix_parts = -(-longest // chunk)
         own = max(1, batch.max_kv_len - prefix.counts["least_shared"])
         own_parts = min(64, most - prefix_parts, -(-own // self.PREFIX_LEAST_CHUNK), 4 * sms // max(1, batch.num_segments * kv_heads))
         return chunk, prefix_parts, max(1, own_parts)
@@ -1050,8 +1052,8 @@ class CudaOps:
             batch.seg_slot.data_ptr(), batch.block_table.data_ptr(), plan["seg_keys"].data_ptr(), plan["members"].data_ptr(),
             plan["tile_first"].data_ptr(), plan["tile_count"].data_ptr(), plan["tile_keys"].data_ptr(), scratch.data_ptr(),
             scratch.data_ptr() + states * head_dim * 4, segments, counts["tiles"], num_heads, num_kv_heads, head_dim, page_size,
-            k_pool.shape[0], batch.block_table.shape[1], chunk, prefix_parts, own_parts, scale, _code(q.dtype),
-            int(fast), self._error_word(q.device).data_ptr(), _raw_stream()), "shared_prefix_attention")
+            k_pool.shape[0], batch.block_table.shape[1], chunk, prefix_parts, own_parts,
+            sum(-(-keys // chunk) for keys in counts["tile_keys"]), scale, _code(q.dtype), int(fast), self._error_word(q.device).data_ptr(), _raw_stream()), "shared_prefix_attention")
         return out
 
     def plan_decode(self, num_decode: int, num_kv_heads: int, longest: int, sms: int) -> tuple[int, int]:
