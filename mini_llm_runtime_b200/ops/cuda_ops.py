@@ -12,6 +12,7 @@ The reference reaches its one kernel through a similar checked wrapper
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from dataclasses import dataclass
 
@@ -311,10 +312,24 @@ def plan_attention(lengths: np.ndarray, position_start: np.ndarray) -> tuple[dic
 @dataclass(frozen=True)
 class SharedPrefix:
     """Which segments of a step share leading keys: ``plan`` holds the arrays of ``plan_shared_prefix`` on the device, ``counts``
-    what the host knows of them."""
+    what the host knows of them.  Checked against one another here, once, and against the step at each call."""
 
     plan: dict
     counts: dict
+
+    def __post_init__(self) -> None:
+        for name, length in (("seg_keys", self.counts["segments"]), ("members", self.counts["members"]), ("tile_first", self.counts["tiles"]),
+                             ("tile_count", self.counts["tiles"]), ("tile_keys", self.counts["tiles"])):
+            _need(self.plan[name], name, torch.int32, 1)
+            if self.plan[name].shape[0] != length:
+                raise KernelError(f"{name} must have {length} entries, got {self.plan[name].shape[0]}")
+        if len(self.counts["tile_keys"]) != self.counts["tiles"]:
+            raise KernelError("the plan's counts do not belong together")
+        _need_together(*self.plan.values())
+
+    @property
+    def device(self) -> torch.device:
+        return self.plan["seg_keys"].device
 
 
 PREFIX_TILE_ROWS = 128    # attention_prefix.cu: query rows of one work item of a prefix
@@ -351,8 +366,30 @@ def plan_shared_prefix(groups, num_segments: int, heads_per_kv: int) -> tuple[di
         members += segments
     arrays = {"seg_keys": seg_keys, **{name: np.asarray(values, dtype=np.int32) for name, values in (
         ("members", members), ("tile_first", first), ("tile_count", count), ("tile_keys", keys_of))}}
-    return arrays, {"segments": int(num_segments), "heads_per_kv": int(heads_per_kv), "tiles": len(first), "tile_keys": tuple(keys_of),
-                    "least_shared": int(seg_keys.min()) if num_segments else 0}
+    return arrays, {"segments": int(num_segments), "heads_per_kv": int(heads_per_kv), "members": len(members),
+                    "tiles": len(first), "tile_keys": tuple(keys_of), "least_shared": int(seg_keys.min()) if num_segments else 0}
+
+
+PREFIX_SCRATCH_BYTES = 256 << 20      # states of the parts of one call, at most
+PREFIX_LEAST_CHUNK = 256              # keys of a part, at least
+
+
+@functools.lru_cache(maxsize=256)
+def prefix_parts(tile_keys: tuple, least_shared: int, segments: int, longest: int, heads: int, kv_heads: int, dim: int,
+                 sms: int) -> tuple[int, int, int, int]:
+    """(keys of a prefix part, parts of the longest prefix, parts of all work items, parts of a segment's own keys), for contexts of
+    up to ``longest`` keys."""
+    most = max(2, PREFIX_SCRATCH_BYTES // max(1, segments * heads * (dim + 2) * 4))
+    chunk = parts = units = 0
+    if tile_keys:
+        # the shortest parts whose work items are all resident at once, two on an SM (a few short of that many: one item in a
+        # second round would take as long as the first)
+        chunk, far, resident = PREFIX_LEAST_CHUNK, max(tile_keys), 2 * sms - sms // 16
+        while chunk < far and (-(-far // chunk) > min(64, most - 1) or sum(-(-keys // chunk) for keys in tile_keys) * kv_heads > resident):
+            chunk += 64
+        parts, units = -(-far // chunk), sum(-(-keys // chunk) for keys in tile_keys)
+    own = max(1, longest - least_shared)
+    return chunk, parts, units, max(1, min(64, most - parts, -(-own // PREFIX_LEAST_CHUNK), 4 * sms // max(1, segments * kv_heads)))
 
 
 def prompt_keys(batch: AttentionBatch, window: int, keep_first: int = 0) -> int:
@@ -986,26 +1023,6 @@ class CudaOps:
     def plan_shared_prefix(self, groups, num_segments, heads_per_kv):
         return plan_shared_prefix(groups, num_segments, heads_per_kv)
 
-    PREFIX_SCRATCH_BYTES = 256 << 20      # states of the parts of one call, at most
-    PREFIX_LEAST_CHUNK = 256              # keys of a part, at least
-
-    def _prefix_parts(self, batch, prefix, heads, kv_heads, dim, sms) -> tuple[int, int, int]:
-        """(keys of a prefix part, their number, parts of the own keys)."""
-        most = max(2, self.PREFIX_SCRATCH_BYTES // max(1, batch.num_segments * heads * (dim + 2) * 4))
-        keys = prefix.counts["tile_keys"]
-        chunk = prefix_parts = 0
-        if keys:
-            # the shortest parts whose work items are all resident at once, two on an SM (a few short of that many: one item in a
-            # second round would take as long as the first)
-            chunk, longest, resident = self.PREFIX_LEAST_CHUNK, max(keys), 2 * sms - sms // 16
-            while chunk < longest and (-(-longest // chunk) > min(64, most - 1)
-                                       or sum(-(-n // chunk) for n in keys) * kv_heads > resident):
-                chunk += 64
-            prefix_parts = -(-longest // chunk)
-        own = max(1, batch.max_kv_len - prefix.counts["least_shared"])
-        own_parts = min(64, most - prefix_parts, -(-own // self.PREFIX_LEAST_CHUNK), 4 * sms // max(1, batch.num_segments * kv_heads))
-        return chunk, prefix_parts, max(1, own_parts)
-
     def shared_prefix_attention(self, q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, batch: AttentionBatch,
                                 prefix: SharedPrefix, num_heads: int, num_kv_heads: int, head_dim: int, scale: float) -> torch.Tensor:
         """``paged_attention`` of a step of decoded tokens whose requests share leading pages: the keys and values of a prefix are
@@ -1029,31 +1046,25 @@ class CudaOps:
             raise KernelError(f"the prefix was planned for {counts['segments']} segments and {counts['heads_per_kv']} heads per kv head")
         if counts["tile_keys"] and max(counts["tile_keys"]) > batch.max_kv_len:
             raise KernelError(f"a prefix of {max(counts['tile_keys'])} keys in contexts of at most {batch.max_kv_len}")
-        for name, length in (("seg_keys", segments), ("tile_first", counts["tiles"]), ("tile_count", counts["tiles"]),
-                             ("tile_keys", counts["tiles"])):
-            _need(plan[name], name, torch.int32, 1)
-            if plan[name].shape[0] != length:
-                raise KernelError(f"{name} must have {length} entries, got {plan[name].shape[0]}")
-        _need(plan["members"], "members", torch.int32, 1)
         _need(batch.block_table, "block_table", torch.int32, 2)
-        _need_here(q=q, k_pool=k_pool, v_pool=v_pool, seg_keys=plan["seg_keys"], members=plan["members"], block_table=batch.block_table)
+        _need_here(q=q, k_pool=k_pool, v_pool=v_pool, prefix=prefix, block_table=batch.block_table)
         out = torch.empty_like(q)
         if segments == 0:
             return out
-        chunk, prefix_parts, own_parts = self._prefix_parts(batch, prefix, num_heads, num_kv_heads, head_dim, self.sm_count(q.device))
+        chunk, parts, units, own_parts = prefix_parts(counts["tile_keys"], counts["least_shared"], segments, batch.max_kv_len, num_heads,
+                                                      num_kv_heads, head_dim, self.sm_count(q.device))
         page_size = k_pool.shape[2]
         fast = (self.use_mma_attention and q.dtype == torch.bfloat16 and head_dim in (64, 128) and num_heads // num_kv_heads <= 16
                 and page_size >= 8 and page_size & (page_size - 1) == 0 and k_pool.shape[0] * num_kv_heads * page_size < 1 << 31
                 and not (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr()) % 16)
-        states = (prefix_parts + own_parts) * segments * num_heads
+        states = (parts + own_parts) * segments * num_heads
         scratch = torch.empty(states * (head_dim + 2), dtype=torch.float32, device=q.device)
         _check(_declared_library("attention_prefix").mlr_attention_prefix(
             q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), batch.seg_q_start.data_ptr(), batch.seg_pos0.data_ptr(),
             batch.seg_slot.data_ptr(), batch.block_table.data_ptr(), plan["seg_keys"].data_ptr(), plan["members"].data_ptr(),
             plan["tile_first"].data_ptr(), plan["tile_count"].data_ptr(), plan["tile_keys"].data_ptr(), scratch.data_ptr(),
             scratch.data_ptr() + states * head_dim * 4, segments, counts["tiles"], num_heads, num_kv_heads, head_dim, page_size,
-            k_pool.shape[0], batch.block_table.shape[1], chunk, prefix_parts, own_parts,
-            sum(-(-keys // chunk) for keys in counts["tile_keys"]), scale, _code(q.dtype), int(fast), self._error_word(q.device).data_ptr(), _raw_stream()), "shared_prefix_attention")
+            k_pool.shape[0], batch.block_table.shape[1], chunk, parts, own_parts, units, scale, _code(q.dtype), int(fast), self._error_word(q.device).data_ptr(), _raw_stream()), "shared_prefix_attention")
         return out
 
     def plan_decode(self, num_decode: int, num_kv_heads: int, longest: int, sms: int) -> tuple[int, int]:

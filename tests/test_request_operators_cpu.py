@@ -163,16 +163,39 @@ def shared(groups, count, per):
 @pytest.mark.parametrize("change", [
     {"q": torch.zeros((3, 31))}, {"q": torch.zeros((2, 32))}, {"q": torch.zeros((3, 64))[:, ::2]}, {"k_pool": torch.zeros((9, 3, 16, 8))},
     {"v_pool": torch.zeros((9, 2, 16, 16))}, {"v_pool": torch.zeros((8, 2, 16, 8))}, {"k_pool": torch.zeros((9, 2, 16, 8), dtype=torch.bfloat16)},
-    {"batch": decoded(4)}, {"prefix": shared([((0, 1), 16)], 4, 2)}, {"prefix": shared([((0, 1), 16)], 3, 4)},
-    {"prefix": shared([((0, 1), 51)], 3, 2)}, {"num_heads": 5}, {"num_kv_heads": 0}, {"head_dim": 0},
-    {"prefix": cuda_ops.SharedPrefix({**shared([((0, 1), 16)], 3, 2).plan, "tile_keys": torch.zeros(2, dtype=torch.int32)},
-                                     shared([((0, 1), 16)], 3, 2).counts)},
+    {"batch": decoded(4)}, {"prefix": ([((0, 1), 16)], 4, 2)}, {"prefix": ([((0, 1), 16)], 3, 4)},
+    {"prefix": ([((0, 1), 51)], 3, 2)}, {"num_heads": 5}, {"num_kv_heads": 0}, {"head_dim": 0},
 ])
 def test_attention_that_does_not_fit(kernels, change):
     call = dict(q=torch.zeros((3, 32)), k_pool=torch.zeros((9, 2, 16, 8)), v_pool=torch.zeros((9, 2, 16, 8)), batch=decoded(3),
-                prefix=shared([((0, 1), 16)], 3, 2), num_heads=4, num_kv_heads=2, head_dim=8, scale=0.3)
+                prefix=([((0, 1), 16)], 3, 2), num_heads=4, num_kv_heads=2, head_dim=8, scale=0.3)
+    call.update(change)
+    call["prefix"] = shared(*call["prefix"])
     with pytest.raises(KernelError):
-        kernels.shared_prefix_attention(**{**call, **change})
+        kernels.shared_prefix_attention(**call)
+
+
+@pytest.mark.parametrize("name,value", [
+    ("tile_keys", torch.zeros(2, dtype=torch.int32)), ("seg_keys", torch.zeros(2, dtype=torch.int32)), ("members", torch.zeros(3, dtype=torch.int32)),
+    ("tile_first", torch.zeros(1, dtype=torch.int64)), ("tile_count", torch.zeros((1, 1), dtype=torch.int32)),
+])
+def test_a_prefix_whose_arrays_do_not_belong_together(kernels, name, value):
+    whole = shared([((0, 1), 16)], 3, 2)
+    with pytest.raises(KernelError):
+        cuda_ops.SharedPrefix({**whole.plan, name: value}, whole.counts)
+
+
+def test_parts_of_prefixes():
+    """Every key has its part, whatever the sizes; the parts fit their bounds."""
+    for keys in ((), (1,), (300,), (16384,) * 3 + (9001,) * 2 + (4100,), (131072,), tuple(range(1, 40))):
+        for segments, heads, kv_heads, dim, longest in ((2, 14, 2, 64, 400), (64, 28, 4, 128, 9000), (256, 64, 8, 128, 131072), (1, 1, 1, 16, 1)):
+            chunk, parts, units, own = cuda_ops.prefix_parts(keys, 0, segments, max((longest,) + keys), heads, kv_heads, dim, 148)
+            assert 1 <= own <= 64 and parts <= 64
+            if keys:
+                assert chunk % 64 == 0 and chunk * parts >= max(keys) > chunk * (parts - 1)
+                assert units == sum(-(-n // chunk) for n in keys) >= len(keys)
+            else:
+                assert chunk == parts == units == 0
 
 
 def test_a_prompt_portion_is_refused(kernels):
