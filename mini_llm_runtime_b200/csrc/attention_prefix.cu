@@ -249,6 +249,13 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
     const int logical = (begin + j * PT_KEYS + (lane % boxes) * box_rows) >> page_shift;
     return logical < c.table_width ? max(0, table[logical]) : 0;
   };
+  const int per = c.heads / c.kv_heads;
+  const int rows = c.tile_count[tile] * per;
+  // softmax threads: the row's segment and head, and where its q stands
+  const int r = threadIdx.x;
+  const bool live = r < rows;
+  const int segment = live ? c.members[first_member + r / per] : 0, head = kv_head * per + r % per;
+  const int q_at = live ? c.q_row[segment] * c.heads + head : -1;      // in units of a head
   int first_pages[STAGES + 2];
   if (warp == 5) {
 #pragma unroll
@@ -265,8 +272,6 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
   pdl_wait();                       // before the first read of q and cache
   pdl_trigger();                    // after it: see prefix_own_mma_kernel
 
-  const int per = c.heads / c.kv_heads;
-  const int rows = c.tile_count[tile] * per;
   bool gave_up = false;
 
   if (warp == 5) {
@@ -344,17 +349,20 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
     }
   } else {
     // ------------------------------------------------------------ softmax, one thread per query row
-    const int r = threadIdx.x;
-    const bool live = r < rows;
-    const int segment = live ? c.members[first_member + r / per] : 0, head = kv_head * per + r % per;
     {
-      const uint4* from = reinterpret_cast<const uint4*>((const bf16*)c.q + ((size_t)(live ? c.q_row[segment] : 0) * c.heads + head) * D);
-      uint4 piece[D / 8];
+      // a warp's 32 rows, whole rows at a time (a row per lane would touch 32 lines with every load: 4.4 us instead of 1.5)
+      constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;      // lanes per row, rows per load
+      uint4 piece[LANES];
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) piece[i] = live ? __ldcg(from + i) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < LANES; ++i) {
+        const int at = __shfl_sync(0xffffffffu, q_at, i * AT_ONCE + lane / LANES);
+        piece[i] = at >= 0 ? __ldcg(reinterpret_cast<const uint4*>((const bf16*)c.q + (size_t)at * D) + lane % LANES) : make_uint4(0u, 0u, 0u, 0u);
+      }
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i)
-        *reinterpret_cast<uint4*>(q_tile + (i >> 3) * Shape::Q_HALF + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = piece[i];
+      for (int i = 0; i < LANES; ++i) {
+        const int row = warp * 32 + i * AT_ONCE + lane / LANES, chunk = lane % LANES;
+        *reinterpret_cast<uint4*>(q_tile + (chunk >> 3) * Shape::Q_HALF + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = piece[i];
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.q_full);
@@ -458,23 +466,33 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
     }
     fa_wait(&ctl.pv_done[(tiles - 1) % STAGES], (unsigned)((tiles - 1) / STAGES) & 1u, error_word, 0x79, gave_up);
     fa_fence_after();
-    const size_t at = ((size_t)part * c.segments + segment) * c.heads + head;
+    // The output rows through shared memory, so that a warp writes whole rows (a row per lane: 3.7 us, now 2).  All products
+    // of this CTA are done: the warp takes its share of the probabilities' and the ring's space.
+    const int at = live ? segment * c.heads + head : -1;
+    constexpr int PITCH = D + 4;
+    static_assert(4 * 32 * PITCH * 4 <= PT_P_BYTES + STAGES * Shape::STAGE_BYTES, "the rows fit behind the queries");
+    float* mine = reinterpret_cast<float*>(p_tile) + warp * 32 * PITCH;
+    asm volatile("bar.sync 1, 128;" ::: "memory");      // every warp's last wait is behind it
 #pragma unroll
     for (int d0 = 0; d0 < D; d0 += 32) {
       float o[32];
       fa_tmem_load16(lane_base + PT_TMEM_O + d0, reinterpret_cast<uint32_t*>(o));
       fa_tmem_load16(lane_base + PT_TMEM_O + d0 + 16, reinterpret_cast<uint32_t*>(o) + 16);
       fa_tmem_wait_ld();
-      if (live) {
-        float4* to = reinterpret_cast<float4*>(c.acc + at * D + d0);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-      }
+      for (int e = 0; e < 32; e += 4)
+        *reinterpret_cast<float4*>(mine + lane * PITCH + d0 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
     }
-    if (live) {
-      c.state[2 * at] = m_base;
-      c.state[2 * at + 1] = l;
+    __syncwarp();
+    float* acc = c.acc + (size_t)part * c.segments * c.heads * D;
+    constexpr int LANES = D / 4, AT_ONCE = 32 / LANES;
+#pragma unroll 8
+    for (int i = 0; i < 32 / AT_ONCE; ++i) {
+      const int row = i * AT_ONCE + lane / LANES, to = __shfl_sync(0xffffffffu, at, row);
+      if (to >= 0) *reinterpret_cast<float4*>(acc + (size_t)to * D + lane % LANES * 4) = *reinterpret_cast<const float4*>(mine + row * PITCH + lane % LANES * 4);
     }
+    if (live)
+      *reinterpret_cast<float2*>(c.state + 2 * ((size_t)part * c.segments * c.heads + at)) = make_float2(m_base, l);
     fa_fence_before();
   }
   __syncthreads();
@@ -542,6 +560,7 @@ prefix_own_mma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
 #pragma unroll
     for (int j = 0; j < STAGES; ++j) pages[j] = lookup(j);
   }
+  const int q_row = c.q_row[segment];
   __syncthreads();
   if (!AFTER_PREFIX) pdl_wait();
   pdl_trigger();
@@ -578,7 +597,7 @@ prefix_own_mma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     float m[NT][2], l[NT][2];
     if (warp < 4) {
       uint32_t q_frag[D / 16][NT][2];
-      const bf16* q = (const bf16*)c.q + ((size_t)c.q_row[segment] * c.heads + kv_head * per) * D;
+      const bf16* q = (const bf16*)c.q + ((size_t)q_row * c.heads + kv_head * per) * D;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
