@@ -347,7 +347,7 @@ def plan_shared_prefix(groups, num_segments: int, heads_per_kv: int) -> tuple[di
         raise KernelError(f"a kv head serves 1 to {PREFIX_TILE_ROWS} query heads, not {heads_per_kv}")
     seg_keys = np.zeros(num_segments, dtype=np.int32)
     grouped = np.zeros(num_segments, dtype=bool)
-    members, first, count, keys_of = [], [], [], []
+    members, first, count, keys_of, saved = [], [], [], [], 0
     each = PREFIX_TILE_ROWS // heads_per_kv
     for segments, keys in groups:
         segments = [int(segment) for segment in segments]
@@ -359,6 +359,7 @@ def plan_shared_prefix(groups, num_segments: int, heads_per_kv: int) -> tuple[di
         if keys == 0 or not segments:
             continue
         seg_keys[segments] = keys
+        saved += (len(segments) - 1) * int(keys)
         for at in range(0, len(segments), each):
             first.append(len(members) + at)
             count.append(min(each, len(segments) - at))
@@ -367,7 +368,7 @@ def plan_shared_prefix(groups, num_segments: int, heads_per_kv: int) -> tuple[di
     arrays = {"seg_keys": seg_keys, **{name: np.asarray(values, dtype=np.int32) for name, values in (
         ("members", members), ("tile_first", first), ("tile_count", count), ("tile_keys", keys_of))}}
     return arrays, {"segments": int(num_segments), "heads_per_kv": int(heads_per_kv), "members": len(members),
-                    "tiles": len(first), "tile_keys": tuple(keys_of), "least_shared": int(seg_keys.min()) if num_segments else 0}
+                    "tiles": len(first), "tile_keys": tuple(keys_of), "saved_keys": saved, "least_shared": int(seg_keys.min()) if num_segments else 0}
 
 
 PREFIX_SCRATCH_BYTES = 256 << 20      # states of the parts of one call, at most
@@ -450,6 +451,8 @@ class CudaOps:
         self.use_fused_rope = True
         self.use_grouped_experts = True     # routed experts of many rows: sorted pairs through the grouped tcgen05 product
         self.use_cluster_merge = True       # chunks of a decode row merge through a cluster's shared memory
+        # bytes of keys and values that a shared prefix must save to be walked by itself (see shared_prefix_attention)
+        self.shared_prefix_least = self.SHARED_PREFIX_LEAST
         self.split_prefill_items = True     # the tcgen05 prompt attention may cut long items into parts
         # MLR_TCGEN05_ATTENTION=0 in the environment keeps prompt attention on the mma.sync kernels
         self.use_tcgen05_attention = os.environ.get("MLR_TCGEN05_ATTENTION", "1") != "0"
@@ -1023,12 +1026,20 @@ class CudaOps:
     def plan_shared_prefix(self, groups, num_segments, heads_per_kv):
         return plan_shared_prefix(groups, num_segments, heads_per_kv)
 
+    # Prefixes that save less go through paged_attention, which reads them once per request, most of it from L2, in one launch instead of
+    # three.  Captured steps, us, shared / paged, by bytes saved: 14 heads of 64, 8 x 2,048 keys (7 MB) 10.4 / 7.2, 32 x 2,048 (32 MB) 11.1 /
+    # 9.6, 16 x 8,192 (63 MB) 14.4 / 14.5, 64 x 2,048 (66 MB) 11.4 / 13.2, 64 x 8,192 (264 MB) 21.4 / 28.1; 28 heads of 128, 2 x 8,192
+    # (17 MB) 16.0 / 15.2, 32 x 512 (32 MB) 11.9 / 12.3, 4 x 8,192 (50 MB) 17.1 / 16.1, 64 x 512 (66 MB) 13.5 / 16.7, 64 x 8,192 (1 GB) 29 / 127;
+    # 40 heads of 128, 2 x 8,192 (33 MB) 17.1 / 15.7, 8 x 2,048 (59 MB) 12.4 / 13.2, 64 x 8,192 (2 GB) 37 / 181.
+    SHARED_PREFIX_LEAST = 48 << 20
+
     def shared_prefix_attention(self, q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, batch: AttentionBatch,
                                 prefix: SharedPrefix, num_heads: int, num_kv_heads: int, head_dim: int, scale: float) -> torch.Tensor:
         """``paged_attention`` of a step of decoded tokens whose requests share leading pages: the keys and values of a prefix are
         read once for all its requests instead of once for each.  ``batch`` is the step as ``paged_attention`` takes it (a request's
         row of the block table names the shared pages as its first); ``prefix`` says which segments share how many keys.
-        Segments of no group attend by themselves."""
+        Segments of no group attend by themselves.  Where sharing saves too little for it (``SHARED_PREFIX_LEAST``) the step goes
+        through ``paged_attention``."""
         _need(q, "q", dims=2)
         _need(k_pool, "k_pool", q.dtype, 4)
         _need(v_pool, "v_pool", q.dtype, 4)
@@ -1048,15 +1059,17 @@ class CudaOps:
             raise KernelError(f"a prefix of {max(counts['tile_keys'])} keys in contexts of at most {batch.max_kv_len}")
         _need(batch.block_table, "block_table", torch.int32, 2)
         _need_here(q=q, k_pool=k_pool, v_pool=v_pool, prefix=prefix, block_table=batch.block_table)
-        out = torch.empty_like(q)
-        if segments == 0:
-            return out
-        chunk, parts, units, own_parts = prefix_parts(counts["tile_keys"], counts["least_shared"], segments, batch.max_kv_len, num_heads,
-                                                      num_kv_heads, head_dim, self.sm_count(q.device))
         page_size = k_pool.shape[2]
         fast = (self.use_mma_attention and q.dtype == torch.bfloat16 and head_dim in (64, 128) and num_heads // num_kv_heads <= 16
                 and page_size >= 8 and page_size & (page_size - 1) == 0 and k_pool.shape[0] * num_kv_heads * page_size < 1 << 31
                 and not (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr()) % 16)
+        if segments == 0:
+            return torch.empty_like(q)
+        if fast and 4 * counts["saved_keys"] * num_kv_heads * head_dim < self.shared_prefix_least:
+            return self.paged_attention(q, k_pool, v_pool, batch, num_heads, num_kv_heads, head_dim, scale, None)
+        out = torch.empty_like(q)
+        chunk, parts, units, own_parts = prefix_parts(counts["tile_keys"], counts["least_shared"], segments, batch.max_kv_len, num_heads,
+                                                      num_kv_heads, head_dim, self.sm_count(q.device))
         states = (parts + own_parts) * segments * num_heads
         scratch = torch.empty(states * (head_dim + 2), dtype=torch.float32, device=q.device)
         _check(_declared_library("attention_prefix").mlr_attention_prefix(

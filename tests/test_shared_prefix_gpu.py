@@ -15,6 +15,12 @@ pytestmark = pytest.mark.gpu
 DEVICE = "cuda:0"
 
 
+@pytest.fixture(autouse=True)
+def every_prefix_by_itself(monkeypatch):
+    """Small steps too; the rule that sends them through ``paged_attention`` has a test of its own."""
+    monkeypatch.setattr(ops.current(), "shared_prefix_least", 0)
+
+
 class Step:
     """A step of decoded tokens: groups of (number of requests, shared keys), requests alone, own keys of each in turn."""
 
@@ -207,3 +213,18 @@ def test_pages_beyond_32_bit_offsets():
         setattr(step, name, pool)
     step.table[step.table >= 0] += shift
     step.check(step.run())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_the_rule_of_small_savings(monkeypatch, dim):
+    """On both sides of the bytes from which a prefix is walked by itself: the same numbers, and ``paged_attention`` just below."""
+    kernels = ops.current()
+    saved = 4 * 3 * 512 * 2 * dim              # three of four requests spared 512 keys of two kv heads
+    calls = []
+    paged = kernels.paged_attention
+    monkeypatch.setattr(kernels, "paged_attention", lambda *args: calls.append(1) or paged(*args))
+    for least, expected in ((saved, 0), (saved + 1, 1)):
+        monkeypatch.setattr(kernels, "shared_prefix_least", least)
+        step = Step([(4, 512)], 1, (9, 200, 1), 8, 2, dim, 16, torch.bfloat16, seed=dim)
+        step.check(step.run())
+        assert len(calls) == expected
