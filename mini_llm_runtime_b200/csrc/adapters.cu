@@ -121,6 +121,102 @@ adapter_down_rows_kernel(const T* x, const T* __restrict__ down, const float* __
   cluster_meet();      // no CTA leaves while another reads its sums
 }
 
+// Many rows, prompts as a rule: a CTA takes 32 rows, a part of K and up to 64 rank rows of one adapter after another (those that
+// its rows have), on mma.sync.  Both operands are read straight from global memory, 16 bytes of a row per lane: the four
+// lanes that share a row hold 32 columns, and since both operands are dealt out alike, which of them an MMA calls column 0
+// does not matter.  The warps' and the parts' sums meet in shared memory, in order.
+constexpr int TILE_WARPS = 8;
+
+__global__ void __launch_bounds__(TILE_WARPS * 32)
+adapter_down_tile_kernel(const bf16* x, const bf16* __restrict__ down, const float* __restrict__ scales, const int* row_adapter, float* u,
+                         int rows, int adapters, int rank, int K, int parts) {
+  constexpr int PITCH = TILE_RANKS + 4;
+  __shared__ float sums[2][TILE_DOWN][PITCH];          // of a pair of warps at a time
+  __shared__ float total[TILE_DOWN][PITCH];
+  __shared__ int ids[TILE_DOWN];
+  pdl_trigger();
+  pdl_wait();
+  const int part = blockIdx.x % parts, row0 = blockIdx.x / parts * TILE_DOWN, r0 = blockIdx.y * TILE_RANKS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (threadIdx.x < TILE_DOWN) {
+    const int m = row0 + threadIdx.x;
+    const int id = m < rows ? __ldcg(row_adapter + m) : -1;
+    ids[threadIdx.x] = id >= 0 && id < adapters ? id : -1;
+  }
+  __syncthreads();
+  // the tile's adapters: bit of every row that is its adapter's first
+  const int my_id = ids[lane];
+  bool leads = my_id >= 0;
+  for (int j = 0; j < lane; ++j) leads = leads && ids[j] != my_id;
+  unsigned leaders = __ballot_sync(0xffffffffu, leads);      // the same in every warp and every CTA of the cluster
+  const int pieces = K / 8;                                  // of 16 bytes
+  const int groups = (pieces + 3) / 4;                       // of 32 columns
+  const int stretch = (groups + parts * TILE_WARPS - 1) / (parts * TILE_WARPS);
+  const int begin = (part * TILE_WARPS + warp) * stretch, end = min(groups, begin + stretch);
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  while (leaders != 0u) {
+    const int adapter = ids[__ffs(leaders) - 1];
+    leaders &= leaders - 1u;
+    const int ranks = min(TILE_RANKS, rank - r0);
+    float acc[2][8][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int n = 0; n < 8; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
+    const uint4* ar = reinterpret_cast<const uint4*>(down + ((size_t)adapter * rank + r0) * K);
+    const uint4* xr = reinterpret_cast<const uint4*>(x + (size_t)row0 * K);
+    for (int k = begin; k < end; ++k) {
+      const int piece = k * 4 + t;
+      const bool there = piece < pieces;
+      uint4 a[4], b[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // rows of another adapter count as zeros (whatever they hold stays out of the sums that are kept anyway)
+        const int row = g + i * 8;
+        a[i] = there && ids[row] == adapter ? __ldcg(xr + (size_t)row * pieces + piece) : zero;
+      }
+#pragma unroll
+      for (int n = 0; n < 8; ++n) b[n] = there && n * 8 + g < ranks ? __ldg(ar + (size_t)(n * 8 + g) * pieces + piece) : zero;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const uint32_t low[4] = {a[2 * i].x, a[2 * i + 1].x, a[2 * i].y, a[2 * i + 1].y};
+          mma_bf16(acc[i][n], low, b[n].x, b[n].y);
+          const uint32_t high[4] = {a[2 * i].z, a[2 * i + 1].z, a[2 * i].w, a[2 * i + 1].w};
+          mma_bf16(acc[i][n], high, b[n].z, b[n].w);
+        }
+    }
+    // sum over the warps, two at a time, in order
+    for (int w = 0; w < TILE_WARPS; w += 2) {
+      __syncthreads();
+      if (warp == w || warp == w + 1)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sums[warp - w][i * 16 + g + (e >> 1) * 8][n * 8 + t * 2 + (e & 1)] = acc[i][n][e];
+      __syncthreads();
+      for (int i = threadIdx.x; i < TILE_DOWN * TILE_RANKS; i += TILE_WARPS * 32) {
+        const int row = i / TILE_RANKS, r = i - row * TILE_RANKS;
+        const float both = sums[0][row][r] + sums[1][row][r];
+        total[row][r] = w == 0 ? both : total[row][r] + both;
+      }
+    }
+    if (parts > 1) cluster_meet(); else __syncthreads();
+    // each CTA of the cluster finishes its share of the rows
+    for (int i = threadIdx.x; i < TILE_DOWN * TILE_RANKS; i += TILE_WARPS * 32) {
+      const int row = i / TILE_RANKS, r = i - row * TILE_RANKS;
+      if (row % parts != part || r >= ranks || ids[row] != adapter) continue;
+      float sum = 0.f;
+      for (int other = 0; other < parts; ++other) sum += parts > 1 ? read_from_cta(&total[row][r], other) : total[row][r];
+      u[(size_t)(row0 + row) * rank + r0 + r] = scales[adapter] * sum;
+    }
+    if (parts > 1) cluster_meet(); else __syncthreads();
+  }
+}
+
 // Up: a thread owns one output column and eight rows; B's row of the column is read once per run of rows with one adapter.
 template <typename T, typename Out, bool WIDE>
 __global__ void __launch_bounds__(128)
@@ -180,6 +276,16 @@ adapter_up_kernel(const float* u, const T* __restrict__ up, const int* row_adapt
     if (row0 + r < rows) out[(size_t)(row0 + r) * N + n] = from_float<Out>(acc[r]);
 }
 
+static int launch_down_tile(const void* x, const void* down, const float* scales, const int* row_adapter, float* u, int rows, int adapters,
+                            int rank, int K, cudaStream_t stream) {
+  const int tiles = (rows + TILE_DOWN - 1) / TILE_DOWN, groups = (rank + TILE_RANKS - 1) / TILE_RANKS;
+  int parts = 1;
+  while (parts < 8 && tiles * groups * parts < 2 * sm_count() && K >= 2 * parts * TILE_WARPS * 32) parts *= 2;
+  launch_kernel_clustered(adapter_down_tile_kernel, dim3(tiles * parts, groups), dim3(TILE_WARPS * 32), 0, stream, parts, (const bf16*)x,
+                          (const bf16*)down, scales, row_adapter, u, rows, adapters, rank, K, parts);
+  return launch_status();
+}
+
 template <typename T>
 static int launch_down(const void* x, const void* down, const float* scales, const int* row_adapter, float* u, int rows, int adapters,
                        int rank, int K, cudaStream_t stream) {
@@ -221,6 +327,7 @@ MLR_EXPORT int mlr_adapter_down(const void* x, const void* down, const float* sc
   if (rows < 0 || adapters <= 0 || rank <= 0 || rank > 128 || K <= 0) return MLR_BAD_SIZE;
   if (rows == 0) return MLR_OK;
   if (((uintptr_t)x & 15) != 0 || ((uintptr_t)down & 15) != 0) return MLR_BAD_ALIGNMENT;
+  if (dtype == MLR_BF16 && rows > 64 && K % 8 == 0) return launch_down_tile(x, down, scales, row_adapter, u, rows, adapters, rank, K, stream);
   if (dtype == MLR_BF16) return launch_down<bf16>(x, down, scales, row_adapter, u, rows, adapters, rank, K, stream);
   if (dtype == MLR_F32) return launch_down<float>(x, down, scales, row_adapter, u, rows, adapters, rank, K, stream);
   return MLR_BAD_DTYPE;

@@ -104,6 +104,7 @@ _PROTOTYPES = {
                                   "mlr_attention_sigmoid_tcgen05_scratch": "iiiii"},
     "attention_prefix": {"mlr_attention_prefix": "pppppppp" "ppppp" "pp" "iiiiiiiiiiii" "fiipp"},
     "adapters": {"mlr_adapter_down": "pppppiiiiip", "mlr_adapter_up": "pppppiiiiiip"},
+    "adapters_tcgen05": {"mlr_adapter_gemm": "ppppppp" "iiiiii" "pp"},
     "logit_rules": {"mlr_logit_rules": "pppiii" "pppppip" "p", "mlr_count_tokens": "ppippiiip"},
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
@@ -879,6 +880,8 @@ class CudaOps:
                                    _stream()), "linear")
         return out
 
+    ADAPTER_ROWS = 128      # rows from which the adapters extend the shared product's sum over K
+
     def linear_adapters(self, x: torch.Tensor, weight: torch.Tensor, adapters: AdapterStack, row_adapter: torch.Tensor,
                         bias: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
         """``linear`` beside which row m passes through adapter ``row_adapter[m]`` (int32 [M]; no adapter where it is negative or
@@ -908,6 +911,14 @@ class CudaOps:
         library = _declared_library("adapters")
         _check(library.mlr_adapter_down(x.data_ptr(), adapters.down.data_ptr(), adapters.scales.data_ptr(), row_adapter.data_ptr(),
                                         low.data_ptr(), rows, count, rank, K, _code(x.dtype), _raw_stream()), "linear_adapters (down)")
+        if (self.use_tensor_cores and x.dtype == torch.bfloat16 and rows > self.ADAPTER_ROWS and K % 8 == 0 and rank % 8 == 0
+                and not weight.data_ptr() % 16 and count * N < 1 << 31):
+            out = torch.empty((rows, N), dtype=out_dtype, device=x.device)
+            _check(_declared_library("adapters_tcgen05").mlr_adapter_gemm(
+                x.data_ptr(), weight.data_ptr(), adapters.up.data_ptr(), low.data_ptr(), row_adapter.data_ptr(), _address(bias), out.data_ptr(),
+                rows, N, K, count, rank, int(out_dtype == torch.float32), self._error_word(x.device).data_ptr(), _raw_stream()),
+                "linear_adapters (tcgen05)")
+            return out
         base = self.linear(x, weight, bias, out_dtype=torch.float32)
         out = base if out_dtype == torch.float32 else torch.empty((rows, N), dtype=out_dtype, device=x.device)
         _check(library.mlr_adapter_up(low.data_ptr(), adapters.up.data_ptr(), row_adapter.data_ptr(), base.data_ptr(), out.data_ptr(),

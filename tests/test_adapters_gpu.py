@@ -129,6 +129,18 @@ def test_a_row_not_finite_stays_alone(rows):
     assert not bool(torch.isfinite(got[rows // 2]).all())
 
 
+@pytest.mark.parametrize("rows,rank", [(6, 16), (60, 8), (300, 16), (300, 128), (300, 12)])
+def test_an_adapter_not_finite_stays_with_its_rows(rows, rank):
+    case = made(rows, 128, 264, rank, 4, torch.bfloat16, 8)
+    ids = some_ids(rows, 4, "mixed", 1)
+    want = run(case, ids)
+    case["down"][1], case["up"][2] = float("inf"), float("nan")
+    got = run(case, ids)
+    others = (ids != 1) & (ids != 2)
+    assert torch.equal(got[others], want[others])
+    assert not bool(torch.isfinite(got[~others]).any())
+
+
 @pytest.mark.parametrize("rows", [5, 280])
 def test_a_captured_projection_follows_its_adapters(rows):
     case = made(rows, 256, 512, 16, 6, torch.bfloat16, 9)
