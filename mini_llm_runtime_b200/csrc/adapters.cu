@@ -15,6 +15,10 @@ namespace mlr {
 
 constexpr int DOWN_RANKS = 16;       // rank rows per CTA of the few-rows kernel
 constexpr int DOWN_WARPS = 4;
+constexpr int MOST_PARTS = 8;        // of K: CTAs of a cluster
+// Rows up to which every row reads its adapter by itself.  (16 ranks of 3,584 columns, each row an adapter of its own: 64 rows 8 us, 128 rows
+// as tiles 49; one adapter for 2,048 rows of 64 ranks as tiles 23.)
+constexpr int DOWN_ROWS = 128;
 constexpr int TILE_DOWN = 32;        // rows per CTA of the many-rows kernel
 constexpr int TILE_RANKS = 64;       // rank rows it takes at a time
 
@@ -50,21 +54,24 @@ __device__ __forceinline__ void unpack(const uint4& raw, float* v, float) {
   v[0] = __uint_as_float(raw.x); v[1] = __uint_as_float(raw.y); v[2] = __uint_as_float(raw.z); v[3] = __uint_as_float(raw.w);
 }
 
+// Both down kernels: `early` says that the kernel in front is the shared product of the same x, which lets the next kernel in
+// after its own wait: what is read here was complete then, and the sums are taken beside it; this kernel waits for it at its end.
+//
 // Few rows, each with an adapter of its own as a rule: CTA = (row, 16 rank rows, part of K), bound by reading A.  A warp walks
 // its stretch of K 32 pieces of 16 bytes at a time and holds 16 sums; the parts of K meet through the cluster's shared memory,
 // in order.  WIDE: rows are whole 16-byte pieces.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(DOWN_WARPS * 32)
 adapter_down_rows_kernel(const T* x, const T* __restrict__ down, const float* __restrict__ scales, const int* row_adapter, float* u,
-                         int adapters, int rank, int K, int parts) {
+                         int adapters, int rank, int K, int parts, int early) {
   constexpr int PIECE = WIDE ? Pack<T>::N : 1;
   __shared__ float sums[DOWN_WARPS][DOWN_RANKS];
   __shared__ float total[DOWN_RANKS];
   const int part = blockIdx.x % parts, row = blockIdx.x / parts;
   const int r0 = blockIdx.y * DOWN_RANKS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_trigger();
-  pdl_wait();
+  if (!early) pdl_wait();
+  pdl_trigger();      // after the wait: adapter_up_kernel relies on it
   const int adapter = __ldcg(row_adapter + row);
   const bool live = adapter >= 0 && adapter < adapters;      // the same in all CTAs of a cluster
   if (live) {
@@ -115,27 +122,30 @@ adapter_down_rows_kernel(const T* x, const T* __restrict__ down, const float* __
   cluster_meet();
   if (live && part == 0 && threadIdx.x < DOWN_RANKS && r0 + (int)threadIdx.x < rank) {
     float sum = 0.f;
-    for (int other = 0; other < parts; ++other) sum += read_from_cta(&total[threadIdx.x], other);
+#pragma unroll
+    for (int other = 0; other < MOST_PARTS; ++other) sum += other < parts ? read_from_cta(&total[threadIdx.x], other) : 0.f;
     u[(size_t)row * rank + r0 + threadIdx.x] = scales[adapter] * sum;
   }
   cluster_meet();      // no CTA leaves while another reads its sums
+  if (early) pdl_wait();
 }
 
 // Many rows, prompts as a rule: a CTA takes 32 rows, a part of K and up to 64 rank rows of one adapter after another (those that
-// its rows have), on mma.sync.  Both operands are read straight from global memory, 16 bytes of a row per lane: the four
-// lanes that share a row hold 32 columns, and since both operands are dealt out alike, which of them an MMA calls column 0
-// does not matter.  The warps' and the parts' sums meet in shared memory, in order.
-constexpr int TILE_WARPS = 8;
+// its rows have; TILE_SPLIT CTAs take turns at them), on mma.sync.  Both operands are read straight from global memory, 16
+// bytes of a row per lane: the four lanes that share a row hold 32 columns, and since both operands are dealt out alike, which
+// of them an MMA calls column 0 does not matter.  The warps' and the parts' sums meet in shared memory, in order.
+constexpr int TILE_WARPS = 8, TILE_SPLIT = 4, TILE_PITCH = TILE_RANKS + 4;
+constexpr int TILE_SHARED = (TILE_WARPS + 1) * TILE_DOWN * TILE_PITCH * 4;
 
 __global__ void __launch_bounds__(TILE_WARPS * 32)
 adapter_down_tile_kernel(const bf16* x, const bf16* __restrict__ down, const float* __restrict__ scales, const int* row_adapter, float* u,
-                         int rows, int adapters, int rank, int K, int parts) {
-  constexpr int PITCH = TILE_RANKS + 4;
-  __shared__ float sums[2][TILE_DOWN][PITCH];          // of a pair of warps at a time
-  __shared__ float total[TILE_DOWN][PITCH];
+                         int rows, int adapters, int rank, int K, int parts, int early) {
+  extern __shared__ float tile_shared[];
+  float* sums = tile_shared;                                               // [warps][32][pitch]
+  float* total = tile_shared + TILE_WARPS * TILE_DOWN * TILE_PITCH;        // [32][pitch]
   __shared__ int ids[TILE_DOWN];
+  if (!early) pdl_wait();
   pdl_trigger();
-  pdl_wait();
   const int part = blockIdx.x % parts, row0 = blockIdx.x / parts * TILE_DOWN, r0 = blockIdx.y * TILE_RANKS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (threadIdx.x < TILE_DOWN) {
@@ -154,17 +164,18 @@ adapter_down_tile_kernel(const bf16* x, const bf16* __restrict__ down, const flo
   const int stretch = (groups + parts * TILE_WARPS - 1) / (parts * TILE_WARPS);
   const int begin = (part * TILE_WARPS + warp) * stretch, end = min(groups, begin + stretch);
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  while (leaders != 0u) {
+  const int ranks = min(TILE_RANKS, rank - r0);
+  const uint4* xr = reinterpret_cast<const uint4*>(x + (size_t)row0 * K);
+  for (int turn = 0; leaders != 0u; ++turn) {
     const int adapter = ids[__ffs(leaders) - 1];
     leaders &= leaders - 1u;
-    const int ranks = min(TILE_RANKS, rank - r0);
+    if (turn % TILE_SPLIT != (int)blockIdx.z) continue;
     float acc[2][8][4];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int n = 0; n < 8; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
     const uint4* ar = reinterpret_cast<const uint4*>(down + ((size_t)adapter * rank + r0) * K);
-    const uint4* xr = reinterpret_cast<const uint4*>(x + (size_t)row0 * K);
     for (int k = begin; k < end; ++k) {
       const int piece = k * 4 + t;
       const bool there = piece < pieces;
@@ -187,85 +198,100 @@ adapter_down_tile_kernel(const bf16* x, const bf16* __restrict__ down, const flo
           mma_bf16(acc[i][n], high, b[n].z, b[n].w);
         }
     }
-    // sum over the warps, two at a time, in order
-    for (int w = 0; w < TILE_WARPS; w += 2) {
-      __syncthreads();
-      if (warp == w || warp == w + 1)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int n = 0; n < 8; ++n)
+      for (int n = 0; n < 8; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sums[warp - w][i * 16 + g + (e >> 1) * 8][n * 8 + t * 2 + (e & 1)] = acc[i][n][e];
-      __syncthreads();
-      for (int i = threadIdx.x; i < TILE_DOWN * TILE_RANKS; i += TILE_WARPS * 32) {
-        const int row = i / TILE_RANKS, r = i - row * TILE_RANKS;
-        const float both = sums[0][row][r] + sums[1][row][r];
-        total[row][r] = w == 0 ? both : total[row][r] + both;
-      }
+        for (int e = 0; e < 4; e += 2)
+          *reinterpret_cast<float2*>(sums + (warp * TILE_DOWN + i * 16 + g + e * 4) * TILE_PITCH + n * 8 + t * 2) =
+              make_float2(acc[i][n][e], acc[i][n][e + 1]);
+    __syncthreads();
+    for (int i = threadIdx.x; i < TILE_DOWN * TILE_RANKS; i += TILE_WARPS * 32) {
+      const int at = i / TILE_RANKS * TILE_PITCH + i % TILE_RANKS;
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < TILE_WARPS; ++w) sum += sums[w * TILE_DOWN * TILE_PITCH + at];
+      total[at] = sum;
     }
     if (parts > 1) cluster_meet(); else __syncthreads();
     // each CTA of the cluster finishes its share of the rows
     for (int i = threadIdx.x; i < TILE_DOWN * TILE_RANKS; i += TILE_WARPS * 32) {
       const int row = i / TILE_RANKS, r = i - row * TILE_RANKS;
       if (row % parts != part || r >= ranks || ids[row] != adapter) continue;
+      const float* at = total + row * TILE_PITCH + r;
       float sum = 0.f;
-      for (int other = 0; other < parts; ++other) sum += parts > 1 ? read_from_cta(&total[row][r], other) : total[row][r];
+      if (parts == 1) sum = *at;
+      else
+#pragma unroll
+        for (int other = 0; other < MOST_PARTS; ++other) sum += other < parts ? read_from_cta(at, other) : 0.f;
       u[(size_t)(row0 + row) * rank + r0 + r] = scales[adapter] * sum;
     }
     if (parts > 1) cluster_meet(); else __syncthreads();
   }
+  if (early) pdl_wait();
 }
 
-// Up: a thread owns one output column and eight rows; B's row of the column is read once per run of rows with one adapter.
-template <typename T, typename Out, bool WIDE>
+// Up: a thread owns one output column and ROWS rows; B's row of the column is read once per run of rows with one adapter.  The
+// first CHUNK columns of it are asked for before the wait: which adapter a row has was complete before the down kernel, in
+// front of this one on the stream, let the kernels behind it in.
+template <typename T, typename Out, int ROWS, bool WIDE>
 __global__ void __launch_bounds__(128)
 adapter_up_kernel(const float* u, const T* __restrict__ up, const int* row_adapter, const float* base, Out* out, int rows, int adapters,
                   int rank, int N) {
-  constexpr int ROWS = 8, CHUNK = 16;
+  constexpr int CHUNK = 16;
   __shared__ float low[ROWS][128];
-  __shared__ int ids[ROWS];
-  pdl_trigger();
-  pdl_wait();
   const int row0 = blockIdx.y * ROWS;
   const int n = blockIdx.x * 128 + threadIdx.x;
-  if (threadIdx.x < ROWS) {
-    const int m = row0 + threadIdx.x;
-    const int id = m < rows ? __ldcg(row_adapter + m) : -1;
-    ids[threadIdx.x] = id >= 0 && id < adapters ? id : -1;
+  int ids[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int id = row0 + r < rows ? __ldcg(row_adapter + row0 + r) : -1;
+    ids[r] = id >= 0 && id < adapters ? id : -1;
   }
-  __syncthreads();
+  auto load = [&](int id, int k0, float* b) {
+    const T* from = up + ((size_t)id * N + n) * rank + k0;
+    if (WIDE) {
+#pragma unroll
+      for (int i = 0; i < CHUNK; i += Pack<T>::N) {
+        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+        if (n < N && k0 + i < rank) raw = __ldg(reinterpret_cast<const uint4*>(from + i));
+        unpack(raw, b + i, T());
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < CHUNK; ++i) b[i] = n < N && k0 + i < rank ? to_float(from[i]) : 0.f;
+    }
+  };
+  float first[ROWS > 2 ? 1 : ROWS][CHUNK];      // of every row where they are few
+  if (ROWS <= 2)
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (ids[r] >= 0) load(ids[r], 0, first[r]);
+  pdl_wait();
+  pdl_trigger();
   for (int i = threadIdx.x; i < ROWS * rank; i += 128) {
-    const int r = i / rank;
-    low[r][i - r * rank] = ids[r] >= 0 ? __ldcg(u + (size_t)(row0 + r) * rank + (i - r * rank)) : 0.f;
+    const int r = i / rank, m = row0 + r;
+    const int id = m < rows ? __ldcg(row_adapter + m) : -1;
+    low[r][i - r * rank] = id >= 0 && id < adapters ? __ldcg(u + (size_t)m * rank + (i - r * rank)) : 0.f;
   }
-  __syncthreads();
-  if (n >= N) return;
   float acc[ROWS];
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) acc[r] = row0 + r < rows ? __ldcg(base + (size_t)(row0 + r) * N + n) : 0.f;
+  for (int r = 0; r < ROWS; ++r) acc[r] = n < N && row0 + r < rows ? __ldcg(base + (size_t)(row0 + r) * N + n) : 0.f;
+  __syncthreads();
+  if (n >= N) return;
   for (int k0 = 0; k0 < rank; k0 += CHUNK) {
     float b[CHUNK];
     int held = -1;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      const int id = ids[r];
-      if (id < 0) continue;
-      if (id != held) {
-        held = id;
-        const T* from = up + ((size_t)id * N + n) * rank + k0;
-        if (WIDE) {
+      if (ids[r] < 0) continue;
+      if (ROWS <= 2 && k0 == 0) {
 #pragma unroll
-          for (int i = 0; i < CHUNK; i += Pack<T>::N) {
-            if (k0 + i < rank) unpack(__ldg(reinterpret_cast<const uint4*>(from + i)), b + i, T());
-            else
-#pragma unroll
-              for (int e = 0; e < Pack<T>::N; ++e) b[i + e] = 0.f;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < CHUNK; ++i) b[i] = k0 + i < rank ? to_float(from[i]) : 0.f;
-        }
+        for (int i = 0; i < CHUNK; ++i) b[i] = first[r][i];
+      } else if (ids[r] != held) {
+        load(ids[r], k0, b);
+        held = ids[r];
       }
 #pragma unroll
       for (int i = 0; i < CHUNK; ++i) acc[r] = fmaf(k0 + i < rank ? low[r][k0 + i] : 0.f, b[i], acc[r]);
@@ -277,41 +303,51 @@ adapter_up_kernel(const float* u, const T* __restrict__ up, const int* row_adapt
 }
 
 static int launch_down_tile(const void* x, const void* down, const float* scales, const int* row_adapter, float* u, int rows, int adapters,
-                            int rank, int K, cudaStream_t stream) {
+                            int rank, int K, int early, cudaStream_t stream) {
   const int tiles = (rows + TILE_DOWN - 1) / TILE_DOWN, groups = (rank + TILE_RANKS - 1) / TILE_RANKS;
-  int parts = 1;
-  while (parts < 8 && tiles * groups * parts < 2 * sm_count() && K >= 2 * parts * TILE_WARPS * 32) parts *= 2;
-  launch_kernel_clustered(adapter_down_tile_kernel, dim3(tiles * parts, groups), dim3(TILE_WARPS * 32), 0, stream, parts, (const bf16*)x,
-                          (const bf16*)down, scales, row_adapter, u, rows, adapters, rank, K, parts);
+  int parts = 1;      // of K: one CTA per SM
+  while (parts < MOST_PARTS && 2 * tiles * groups * parts <= sm_count() && K >= 4 * parts * TILE_WARPS * 32) parts *= 2;
+  static OncePerDevice once;
+  if (cudaError_t err = once([] { return cudaFuncSetAttribute(adapter_down_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_SHARED); }))
+    return (int)err;
+  launch_kernel_clustered(adapter_down_tile_kernel, dim3(tiles * parts, groups, TILE_SPLIT), dim3(TILE_WARPS * 32), TILE_SHARED, stream, parts,
+                          (const bf16*)x, (const bf16*)down, scales, row_adapter, u, rows, adapters, rank, K, parts, early);
   return launch_status();
 }
 
 template <typename T>
 static int launch_down(const void* x, const void* down, const float* scales, const int* row_adapter, float* u, int rows, int adapters,
-                       int rank, int K, cudaStream_t stream) {
-  // parts of K: as many CTAs as fill the device twice, at most eight (a cluster), none below 32 pieces per warp
+                       int rank, int K, int early, cudaStream_t stream) {
+  // parts of K: as many CTAs as fill the device four times, at most eight (a cluster), none below 32 pieces per warp
   const bool wide = K % Pack<T>::N == 0;
   const int pieces = wide ? K / Pack<T>::N : K;
   const int groups = (rank + DOWN_RANKS - 1) / DOWN_RANKS;
   int parts = 1;
-  while (parts < 8 && (long long)rows * groups * parts < 4ll * sm_count() && pieces >= 2 * parts * DOWN_WARPS * 32) parts *= 2;
+  while (parts < MOST_PARTS && (long long)rows * groups * parts < 4ll * sm_count() && pieces >= 2 * parts * DOWN_WARPS * 32) parts *= 2;
   if ((long long)rows * parts > 0x7fffffff || groups > 65535) return MLR_TOO_LARGE;
   const dim3 grid(rows * parts, groups);
   auto kernel = wide ? adapter_down_rows_kernel<T, true> : adapter_down_rows_kernel<T, false>;
   launch_kernel_clustered(kernel, grid, dim3(DOWN_WARPS * 32), 0, stream, parts, (const T*)x, (const T*)down, scales, row_adapter, u,
-                          adapters, rank, K, parts);
+                          adapters, rank, K, parts, early);
+  return launch_status();
+}
+
+template <typename T, typename Out, int ROWS>
+static int launch_up_rows(const float* u, const void* up, const int* row_adapter, const float* base, void* out, int rows, int adapters, int rank,
+                          int N, cudaStream_t stream) {
+  const bool wide = rank % Pack<T>::N == 0;
+  if ((rows + ROWS - 1) / ROWS > 65535) return MLR_TOO_LARGE;
+  const dim3 grid((N + 127) / 128, (rows + ROWS - 1) / ROWS);
+  auto kernel = wide ? adapter_up_kernel<T, Out, ROWS, true> : adapter_up_kernel<T, Out, ROWS, false>;
+  launch_kernel(kernel, grid, dim3(128), 0, stream, u, (const T*)up, row_adapter, base, (Out*)out, rows, adapters, rank, N);
   return launch_status();
 }
 
 template <typename T, typename Out>
 static int launch_up(const float* u, const void* up, const int* row_adapter, const float* base, void* out, int rows, int adapters, int rank,
                      int N, cudaStream_t stream) {
-  const bool wide = rank % Pack<T>::N == 0;
-  if ((rows + 7) / 8 > 65535) return MLR_TOO_LARGE;
-  const dim3 grid((N + 127) / 128, (rows + 7) / 8);
-  auto kernel = wide ? adapter_up_kernel<T, Out, true> : adapter_up_kernel<T, Out, false>;
-  launch_kernel(kernel, grid, dim3(128), 0, stream, u, (const T*)up, row_adapter, base, (Out*)out, rows, adapters, rank, N);
-  return launch_status();
+  return rows <= 256 ? launch_up_rows<T, Out, 2>(u, up, row_adapter, base, out, rows, adapters, rank, N, stream)
+                     : launch_up_rows<T, Out, 8>(u, up, row_adapter, base, out, rows, adapters, rank, N, stream);
 }
 
 }  // namespace mlr
@@ -321,15 +357,15 @@ using namespace mlr;
 MLR_DEFINE_PDL_SWITCH
 
 // x [rows, K], down [adapters, rank, K] of one dtype on 16-byte boundaries; u float32 [rows, rank].  Rows without an adapter are
-// not written.
+// not written.  early: the kernel in front on the stream is the product of the same x, and lets the next one in after its own wait.
 MLR_EXPORT int mlr_adapter_down(const void* x, const void* down, const float* scales, const int* row_adapter, float* u, int rows,
-                                int adapters, int rank, int K, int dtype, cudaStream_t stream) {
+                                int adapters, int rank, int K, int dtype, int early, cudaStream_t stream) {
   if (rows < 0 || adapters <= 0 || rank <= 0 || rank > 128 || K <= 0) return MLR_BAD_SIZE;
   if (rows == 0) return MLR_OK;
   if (((uintptr_t)x & 15) != 0 || ((uintptr_t)down & 15) != 0) return MLR_BAD_ALIGNMENT;
-  if (dtype == MLR_BF16 && rows > 64 && K % 8 == 0) return launch_down_tile(x, down, scales, row_adapter, u, rows, adapters, rank, K, stream);
-  if (dtype == MLR_BF16) return launch_down<bf16>(x, down, scales, row_adapter, u, rows, adapters, rank, K, stream);
-  if (dtype == MLR_F32) return launch_down<float>(x, down, scales, row_adapter, u, rows, adapters, rank, K, stream);
+  if (dtype == MLR_BF16 && rows > DOWN_ROWS && K % 8 == 0) return launch_down_tile(x, down, scales, row_adapter, u, rows, adapters, rank, K, early, stream);
+  if (dtype == MLR_BF16) return launch_down<bf16>(x, down, scales, row_adapter, u, rows, adapters, rank, K, early, stream);
+  if (dtype == MLR_F32) return launch_down<float>(x, down, scales, row_adapter, u, rows, adapters, rank, K, early, stream);
   return MLR_BAD_DTYPE;
 }
 

@@ -92,12 +92,12 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
       };
       auto load_w = [&](int s, int k) { tma_load_2d(&w_map, &full[s], tiles + (size_t)s * STAGE_BYTES + A_BYTES, k, n0); };
       const int ahead = min(stages, base_blocks);
-      for (int i = 0; i < ahead; ++i) {      // the weights do not depend on the kernel before
+      // The kernel before, which makes u, let this one in after its own wait: x was complete then.  The warps that read u wait.
+      for (int i = 0; i < ahead; ++i) {
         mbar_expect_tx(&full[i], STAGE_BYTES);
+        load_x(i, i * 64);
         load_w(i, i * 64);
       }
-      pdl_wait();
-      for (int i = 0; i < ahead; ++i) load_x(i, i * 64);
       for (int i = ahead; i < base_blocks; ++i) {
         const int s = i % stages;
         at_wait(&empty[s], (unsigned)(i / stages - 1) & 1u, p.error_word, 0x91, gave_up);
@@ -336,6 +336,7 @@ using namespace mlr;
 
 MLR_DEFINE_PDL_SWITCH
 
+// To be launched right behind mlr_adapter_down, which lets the next kernel in only after its own wait.
 // x [M, K], w [N, K], up [adapters, N, rank], bias [N] or null in bfloat16 on 16-byte boundaries, K % 8 == 0 and rank % 8 == 0;
 // u float32 [M, rank] (rows without an adapter are not read); out [M, N] bfloat16 or float32.
 MLR_EXPORT int mlr_adapter_gemm(const void* x, const void* w, const void* up, const float* u, const int* row_adapter, const void* bias,

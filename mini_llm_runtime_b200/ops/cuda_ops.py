@@ -98,12 +98,13 @@ def _stream() -> ctypes.c_void_p:
 # for twice, one step of 64 rows 3,120 -> 2,840 us, of 1,000 rows 3,380 -> 3,020.
 _PROTOTYPES = {
     "gemm_tcgen05": {"mlr_gemm_tcgen05": "ppppiiiiiffplpipp"},
+    "gemm_skinny": {"mlr_gemm_skinny": "pppppiiiiifp"},
     "elementwise": {"mlr_rms_norm": "ppppiifiip", "mlr_rope_kv_write": "pppppppiiiiiiip"},
     "attention_tcgen05": {"mlr_attention_prefill_tcgen05": "ppppppppppp" "iiiiiiiii" "fi" "ppp" "l" "pip"},
     "attention_sigmoid_tcgen05": {"mlr_attention_sigmoid_tcgen05": "ppppp" "ppppppp" "iiiiiiii" "f" "pppp" "iii" "pp",
                                   "mlr_attention_sigmoid_tcgen05_scratch": "iiiii"},
     "attention_prefix": {"mlr_attention_prefix": "pppppppp" "ppppp" "pp" "iiiiiiiiiiii" "fiipp"},
-    "adapters": {"mlr_adapter_down": "pppppiiiiip", "mlr_adapter_up": "pppppiiiiiip"},
+    "adapters": {"mlr_adapter_down": "pppppiiiiiip", "mlr_adapter_up": "pppppiiiiiip"},
     "adapters_tcgen05": {"mlr_adapter_gemm": "ppppppp" "iiiiii" "pp"},
     "logit_rules": {"mlr_logit_rules": "pppiii" "pppppip" "p", "mlr_count_tokens": "ppippiiip"},
 }
@@ -820,11 +821,9 @@ class CudaOps:
             out = residual      # the kernel adds the product into it
         else:
             out = torch.empty((M, N // 2 if swiglu else N), dtype=out_dtype, device=x.device)
-        lib = build.load_library("gemm_skinny")
-        _check(lib.mlr_gemm_skinny(_ptr(x), _ptr(weight), _ptr(bias), _ptr(out), _ptr(residual), M, N, K,
-                                   int(out_dtype == torch.float32), int(swiglu),
-                                   ctypes.c_float(-1.0 if rms_eps is None else rms_eps), _stream()),
-               "linear (few rows)")
+        _check(_declared_library("gemm_skinny").mlr_gemm_skinny(
+            x.data_ptr(), weight.data_ptr(), _address(bias), out.data_ptr(), _address(residual), M, N, K, int(out_dtype == torch.float32),
+            int(swiglu), -1.0 if rms_eps is None else rms_eps, _raw_stream()), "linear (few rows)")
         return out
 
     def _linear_tcgen05(self, x, weight, bias, out_dtype, swiglu=False, gate=(0.0, 0.0)):
@@ -909,17 +908,29 @@ class CudaOps:
             return torch.empty((0, N), dtype=out_dtype, device=x.device)
         low = torch.empty((rows, rank), dtype=torch.float32, device=x.device)
         library = _declared_library("adapters")
-        _check(library.mlr_adapter_down(x.data_ptr(), adapters.down.data_ptr(), adapters.scales.data_ptr(), row_adapter.data_ptr(),
-                                        low.data_ptr(), rows, count, rank, K, _code(x.dtype), _raw_stream()), "linear_adapters (down)")
+
+        def down(early: bool) -> None:
+            _check(library.mlr_adapter_down(x.data_ptr(), adapters.down.data_ptr(), adapters.scales.data_ptr(), row_adapter.data_ptr(),
+                                            low.data_ptr(), rows, count, rank, K, _code(x.dtype), int(early), _raw_stream()),
+                   "linear_adapters (down)")
+
         if (self.use_tensor_cores and x.dtype == torch.bfloat16 and rows > self.ADAPTER_ROWS and K % 8 == 0 and rank % 8 == 0
                 and not weight.data_ptr() % 16 and count * N < 1 << 31):
+            down(False)
             out = torch.empty((rows, N), dtype=out_dtype, device=x.device)
             _check(_declared_library("adapters_tcgen05").mlr_adapter_gemm(
                 x.data_ptr(), weight.data_ptr(), adapters.up.data_ptr(), low.data_ptr(), row_adapter.data_ptr(), _address(bias), out.data_ptr(),
                 rows, N, K, count, rank, int(out_dtype == torch.float32), self._error_word(x.device).data_ptr(), _raw_stream()),
                 "linear_adapters (tcgen05)")
             return out
+        # bfloat16 products that let the next kernel in after their own wait have the small sums taken beside them
+        beside = (self.use_tensor_cores and x.dtype == torch.bfloat16 and K % 8 == 0 and not weight.data_ptr() % 16
+                  and (rows <= 8 or not self._skinny_fits(x, weight)))
+        if not beside:
+            down(False)
         base = self.linear(x, weight, bias, out_dtype=torch.float32)
+        if beside:
+            down(True)
         out = base if out_dtype == torch.float32 else torch.empty((rows, N), dtype=out_dtype, device=x.device)
         _check(library.mlr_adapter_up(low.data_ptr(), adapters.up.data_ptr(), row_adapter.data_ptr(), base.data_ptr(), out.data_ptr(),
                                       rows, count, rank, N, _code(x.dtype), _code(out_dtype), _raw_stream()), "linear_adapters (up)")
