@@ -34,6 +34,13 @@ def _int_list(raw: str) -> tuple[int, ...]:
     return values
 
 
+def _bias_list(raw: str) -> dict[int, float]:
+    try:
+        return {int(token): float(value) for token, value in (part.split(":") for part in raw.split(",") if part.strip())}
+    except ValueError as error:
+        raise argparse.ArgumentTypeError("expected comma-separated token:bias pairs") from error
+
+
 def build_parser() -> argparse.ArgumentParser:
     parser = argparse.ArgumentParser(prog="mini_llm_runtime_b200", description=__doc__,
                                      formatter_class=argparse.RawDescriptionHelpFormatter)
@@ -52,6 +59,10 @@ def build_parser() -> argparse.ArgumentParser:
         sub.add_argument("--max-model-len", type=int, default=None)
         sub.add_argument("--temperature", type=float, default=0.0, help="0 selects greedy")
         sub.add_argument("--seed", type=int, default=0)
+        sub.add_argument("--repetition-penalty", type=float, default=1.0, help="for tokens of the prompt and the output; 1 changes nothing")
+        sub.add_argument("--presence-penalty", type=float, default=0.0, help="off the logit of every generated token")
+        sub.add_argument("--frequency-penalty", type=float, default=0.0, help="the same for each time it was generated")
+        sub.add_argument("--logit-bias", type=_bias_list, default=None, help="comma-separated token:bias pairs (-inf bans a token)")
         sub.add_argument("--eos-id", type=_int_list, default=None, help="comma-separated EOS token ids")
         sub.add_argument("--output-dir", type=Path, default=None, help="optional folder for result.json")
         sub.add_argument("--device", default="cuda:0")
@@ -79,6 +90,15 @@ def build_parser() -> argparse.ArgumentParser:
     return parser
 
 
+def _rules(args) -> dict:
+    """The request's rules on its logits, empty where all have their defaults."""
+    from .sampling import SamplingParams
+
+    rules = {"repetition_penalty": args.repetition_penalty, "presence_penalty": args.presence_penalty,
+             "frequency_penalty": args.frequency_penalty, "logit_bias": args.logit_bias or {}}
+    return rules if SamplingParams(**rules).has_rules else {}
+
+
 def _engine(args):
     import torch
 
@@ -90,7 +110,7 @@ def _engine(args):
         args.model, dtype=args.dtype, device=args.device, block_size=args.block_size,
         total_blocks=args.total_blocks, max_running_requests=args.max_running_requests,
         max_batch_tokens=args.max_batch_tokens, max_mixed_prefill_tokens=args.max_mixed_prefill_tokens,
-        max_model_len=args.max_model_len, step_ahead=args.step_ahead)
+        max_model_len=args.max_model_len, step_ahead=args.step_ahead, logit_rules=bool(_rules(args)))
 
 
 def _write(args, record: dict) -> None:
@@ -104,7 +124,7 @@ def command_generate(args) -> int:
     engine = _engine(args)
     started = time.perf_counter()
     engine.submit("cli", list(args.prompt_ids), max_new_tokens=args.max_new_tokens,
-                  eos_token_ids=args.eos_id, temperature=args.temperature, seed=args.seed)
+                  eos_token_ids=args.eos_id, temperature=args.temperature, seed=args.seed, **_rules(args))
     engine.run()
     request = engine.scheduler.get_request("cli")
     _write(args, {"prompt_ids": list(args.prompt_ids), "generated_ids": list(request.generated_token_ids),
@@ -128,7 +148,7 @@ def command_serve_batch(args) -> int:
                 torch.randint(0, vocab, (args.prompt_length,), generator=generator).tolist()
             rid = f"run{run}-req{index}"
             engine.submit(rid, prompt, max_new_tokens=args.generation_lengths[index % len(args.generation_lengths)],
-                          eos_token_ids=args.eos_id, temperature=args.temperature, seed=args.seed + index)
+                          eos_token_ids=args.eos_id, temperature=args.temperature, seed=args.seed + index, **_rules(args))
             ids.append(rid)
         steps = engine.run()
         seconds = time.perf_counter() - started

@@ -22,14 +22,15 @@ import time
 from collections.abc import Callable, Collection, Sequence
 from dataclasses import dataclass
 
+import numpy as np
 import torch
 
 from .. import ops
 from ..cache.manager import CacheManager
 from ..models.decoder import DecoderModel
-from ..sampling import SamplingParams
+from ..sampling import LogitRules, SamplingParams
 from .metrics import RequestMetricsCollector
-from .scheduler import BatchingPolicy, CacheGate, Request, RequestScheduler, StepOutcome, StepPlan, WorkKind
+from .scheduler import BatchingPolicy, CacheGate, Request, RequestScheduler, RequestStatus, StepOutcome, StepPlan, WorkKind
 from .step import ModelRunner, StepEntry
 
 
@@ -88,6 +89,7 @@ class ContinuousBatchEngine:
         self._ahead: _TokensInFlight | None = None
         self._token_buffers: list[torch.Tensor] = []
         self._next_buffer = 0
+        self._allowed: dict[str, np.ndarray] = {}      # grammars of requests that wait, until they own a slot
 
     # ------------------------------------------------------------------ assembly
     DEFAULT_MODEL_LEN = 32768
@@ -98,7 +100,8 @@ class ContinuousBatchEngine:
                    max_mixed_prefill_tokens: int | None = None, max_model_len: int | None = None,
                    batching_policy: BatchingPolicy = BatchingPolicy.CONTINUOUS,
                    chunked_prefill: bool = True, enable_nvtx: bool = False,
-                   step_ahead: bool = False) -> "ContinuousBatchEngine":
+                   step_ahead: bool = False, logit_rules: bool = False) -> "ContinuousBatchEngine":
+        """``logit_rules``: requests may bring penalties, biases and grammars (``submit``, ``allow_tokens``); every step then applies them."""
         # a model without a position limit of its own gets this engine's default
         max_model_len = min(max_model_len or min(model.spec.max_positions, cls.DEFAULT_MODEL_LEN),
                             model.spec.max_positions)
@@ -110,8 +113,10 @@ class ContinuousBatchEngine:
         scheduler = RequestScheduler(max_running_requests=max_running_requests, max_batch_tokens=max_batch_tokens,
                                      max_mixed_prefill_tokens=max_mixed_prefill_tokens, gate=CacheGate(cache),
                                      batching_policy=batching_policy, chunked_prefill=chunked_prefill)
-        return cls(scheduler=scheduler, runner=ModelRunner(model, cache), enable_nvtx=enable_nvtx,
-                   step_ahead=step_ahead)
+        runner = ModelRunner(model, cache)
+        if logit_rules:
+            runner.rules = LogitRules(max_running_requests, runner.vocab_size, model.device)
+        return cls(scheduler=scheduler, runner=runner, enable_nvtx=enable_nvtx, step_ahead=step_ahead)
 
     @classmethod
     def from_model_dir(cls, model_dir, *, dtype="bfloat16", device="cuda:0", **options) -> "ContinuousBatchEngine":
@@ -131,7 +136,9 @@ class ContinuousBatchEngine:
     # ------------------------------------------------------------------ requests
     def submit(self, request_id: str, prompt_token_ids: Sequence[int], *, max_new_tokens: int,
                eos_token_ids: int | Collection[int] | None = None, temperature: float = 0.0,
-               seed: int = 0) -> Request:
+               seed: int = 0, **rules) -> Request:
+        """``rules``: ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty``, ``logit_bias`` of ``SamplingParams`` (an engine
+        made with ``logit_rules=True``)."""
         arrival_ns = self._clock_ns()
         vocab = self.runner.vocab_size
         outside = [t for t in prompt_token_ids if not isinstance(t, int) or isinstance(t, bool) or not 0 <= t < vocab]
@@ -141,11 +148,41 @@ class ContinuousBatchEngine:
         if longest > self.manager.max_tokens_per_request:
             raise ValueError(f"prompt + max_new_tokens - 1 = {longest} exceeds the engine's limit of "
                              f"{self.manager.max_tokens_per_request} tokens per request")
+        sampling = SamplingParams(temperature, seed, **rules)
+        if self.runner.rules is not None:
+            self.runner.rules.check(sampling)
+        elif sampling.has_rules:
+            raise ValueError("rules on logits need an engine made with logit_rules=True")
         request = self.scheduler.submit(request_id, prompt_token_ids, max_new_tokens=max_new_tokens,
-                                        eos_token_ids=eos_token_ids,
-                                        sampling=SamplingParams(temperature, seed))
+                                        eos_token_ids=eos_token_ids, sampling=sampling)
         self.metrics.register_request(request_id, arrival_ns)
         return request
+
+    def allow_tokens(self, request_id: str, tokens: "Collection[int] | None") -> None:
+        """The tokens that the request may choose from its next step on (None: all), as a grammar finds them after each token.  A
+        request that allows nothing chooses token 0 if greedy."""
+        if self.runner.rules is None:
+            raise ValueError("allowed tokens need an engine made with logit_rules=True")
+        if self.step_ahead:
+            raise ValueError("an engine that steps ahead chooses a request's next token before its grammar can follow the last one")
+        request = self.scheduler.get_request(request_id)
+        if request.status is RequestStatus.FINISHED:
+            raise ValueError(f"request {request_id!r} has finished")
+        words = self.runner.rules.words_of(tokens)
+        held = self.manager.requests.get(request_id)
+        if held is None:
+            self._allowed[request_id] = words
+        else:
+            self._allowed.pop(request_id, None)
+            self.runner.rules.allow(held.slot, words)
+
+    def _admit_rules(self, request_id: str) -> None:
+        """The request owns a slot now: its rules go there.  (A step that fails gives the slot back, and its request is admitted
+        once more: a grammar named while it waited is kept until the request has a token.)"""
+        request, slot = self.scheduler.get_request(request_id), self.manager.get(request_id).slot
+        self.runner.rules.admit(slot, request.sampling, request.prompt)
+        if request_id in self._allowed:
+            self.runner.rules.allow(slot, self._allowed[request_id])
 
     # ------------------------------------------------------------------ one step
     @torch.inference_mode()
@@ -175,6 +212,8 @@ class ContinuousBatchEngine:
                     request = self.scheduler.get_request(item.request_id)     # a prompt portion: starts at the cursor
                     tokens = request.prompt_span(request.cursor, len(tokens))
                 entries.append(StepEntry(item.request_id, tokens, [len(tokens) - 1] if item.emits else []))
+                if item.admitted and self.runner.rules is not None:
+                    self._admit_rules(item.request_id)
                 if item.admitted:
                     self.metrics.record_prefill_started(item.request_id, self._clock_ns())
                 if item.emits:
@@ -210,6 +249,8 @@ class ContinuousBatchEngine:
         tokens_ready_ns = self._clock_ns()
         with self._range("scheduler.apply_and_release"):
             outcome = self.scheduler.apply_step_results(generated)
+        for request_id in generated if self._allowed else ():
+            self._allowed.pop(request_id, None)
         completed_ns = self._clock_ns()
         self.metrics.record_tokens(outcome.emitted_tokens, tokens_ready_ns)
         self.metrics.record_completed(outcome.finished_request_ids, completed_ns)
@@ -279,15 +320,15 @@ class ContinuousBatchEngine:
 
     def generate(self, prompts: Sequence[Sequence[int]], *, max_new_tokens: int,
                  eos_token_ids: int | Collection[int] | None = None, temperature: float = 0.0,
-                 seed: int = 0) -> list[list[int]]:
-        """Token ids in, generated token ids out, for a list of prompts (host lists both ways)."""
+                 seed: int = 0, **rules) -> list[list[int]]:
+        """Token ids in, generated token ids out, for a list of prompts (host lists both ways); ``rules`` as for ``submit``."""
         scheduler = self.scheduler
         first = (len(scheduler.finished_request_ids) + len(scheduler.running_request_ids)
                  + len(scheduler.waiting_request_ids))
         ids = [f"generate-{first + i}" for i in range(len(prompts))]
         for i, (request_id, prompt) in enumerate(zip(ids, prompts)):
             self.submit(request_id, list(prompt), max_new_tokens=max_new_tokens,
-                        eos_token_ids=eos_token_ids, temperature=temperature, seed=seed + i)
+                        eos_token_ids=eos_token_ids, temperature=temperature, seed=seed + i, **rules)
         self.run()
         return [list(scheduler.get_request(request_id).generated_token_ids) for request_id in ids]
 

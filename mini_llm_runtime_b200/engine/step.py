@@ -214,6 +214,9 @@ class ModelRunner:
         self._graphs: dict[tuple[int, bool, bool, int], _CapturedStep] = {}       # (batch, sample, feed, context limit)
         self._graph_seen: dict[tuple[int, bool, bool, int], int] = {}
         self.graph_replays = 0
+        # Rules of the requests on their logits (sampling/rules.py), or None.  To be set before the first step: a captured step
+        # holds the launches of its time.
+        self.rules = None
 
     # ------------------------------------------------------------------ metadata
     def _upload(self, packer: _Packer, device_buffer: torch.Tensor | None = None) -> dict[str, torch.Tensor]:
@@ -418,7 +421,11 @@ class ModelRunner:
         logits = self.model.forward(ctx)
         tokens = None
         if sample:
+            if self.rules is not None:
+                kernels.shape_logits_(logits, ctx.wanted_slot, self.rules.tables)
             tokens = kernels.sample_slots(logits, ctx.wanted_slot, state, advance=lengths_by_device)
+            if self.rules is not None:
+                kernels.count_tokens(tokens, ctx.wanted_slot, self.rules.tables)
         if lengths_by_device:
             if not sample:
                 kernels.advance_slots(ctx.seg_slot, state)
@@ -551,7 +558,8 @@ class ModelRunner:
         device, in the order of the entries and of each entry's ``want``.  With ``sample`` it
         returns ``(logits, tokens)``: one int32 token per wanted place (at most one per request),
         chosen on the device with the temperature, seed and counter of the request's slot record,
-        which also receives the token.  ``borrow=True`` may return buffers that the next step
+        which also receives the token; with ``rules`` set, the logits that come back have the requests' rules applied.
+        ``borrow=True`` may return buffers that the next step
         overwrites (no copy is made).  ``feed=True``: every entry holds one placeholder token and the
         real input is the token the request sampled last, taken from its slot record on the device
         without the host having seen it."""

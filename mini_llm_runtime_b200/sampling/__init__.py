@@ -1,3 +1,4 @@
 from .params import GREEDY, SamplingParams
+from .rules import LogitRules
 
-__all__ = ["GREEDY", "SamplingParams"]
+__all__ = ["GREEDY", "LogitRules", "SamplingParams"]

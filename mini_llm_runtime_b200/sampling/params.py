@@ -7,10 +7,16 @@ device when it is admitted (cache/slots.py); the sampling kernel (csrc/sampling.
 slot, draws from softmax(logits / temperature) with a counter-based generator keyed by the seed
 and the index of the token being produced, and keeps that index in the record.  A request's tokens
 therefore depend neither on what else is in its batch nor on how its prompt was cut.
+
+Beside that a request may carry rules on its logits (sampling/rules.py): penalties for the tokens of its prompt and its output,
+and biases.  A repetition penalty r divides the logit of every known token by r where it is positive and multiplies it by r
+where it is not; frequency and presence penalties are taken off a generated token's logit, once per occurrence and once.
 """
 
 from __future__ import annotations
 
+import math
+from collections.abc import Mapping
 from dataclasses import dataclass
 
 
@@ -18,6 +24,10 @@ from dataclasses import dataclass
 class SamplingParams:
     temperature: float = 0.0
     seed: int = 0
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: tuple[tuple[int, float], ...] = ()      # (token, what is added), ascending; a mapping is taken too
 
     def __post_init__(self) -> None:
         if isinstance(self.temperature, bool) or not isinstance(self.temperature, (int, float)) \
@@ -26,10 +36,30 @@ class SamplingParams:
         if isinstance(self.seed, bool) or not isinstance(self.seed, int) or not 0 <= self.seed < (1 << 63):
             raise ValueError("seed must be an integer in [0, 2^63)")
         object.__setattr__(self, "temperature", float(self.temperature))
+        for name in ("repetition_penalty", "presence_penalty", "frequency_penalty"):
+            value = getattr(self, name)
+            if isinstance(value, bool) or not isinstance(value, (int, float)) or not math.isfinite(value):
+                raise ValueError(f"{name} must be a finite number")
+            object.__setattr__(self, name, float(value))
+        if self.repetition_penalty <= 0:
+            raise ValueError("repetition_penalty must be > 0 (1 changes nothing)")
+        pairs = self.logit_bias.items() if isinstance(self.logit_bias, Mapping) else self.logit_bias
+        biases = tuple(sorted((token, float(value)) for token, value in pairs))
+        if any(isinstance(token, bool) or not isinstance(token, int) or token < 0 for token, _ in biases):
+            raise ValueError("logit_bias names tokens by integers >= 0")
+        if any(math.isnan(value) or value == math.inf for _, value in biases):
+            raise ValueError("a bias must be a number; -inf bans its token")
+        if len({token for token, _ in biases}) != len(biases):
+            raise ValueError("logit_bias names a token twice")
+        object.__setattr__(self, "logit_bias", biases)
 
     @property
     def greedy(self) -> bool:
         return self.temperature == 0.0
+
+    @property
+    def has_rules(self) -> bool:
+        return bool(self.logit_bias) or (self.repetition_penalty, self.presence_penalty, self.frequency_penalty) != (1.0, 0.0, 0.0)
 
 
 GREEDY = SamplingParams()
