@@ -65,6 +65,7 @@ LIBRARIES: dict[str, tuple[str, ...]] = {
     "matrix_memory": (),
     "logit_rules": (),
     "adapters": (),
+    "adapters_small": (),
     "adapters_tcgen05": (),
     "attention_prefix": (),
 }

@@ -105,6 +105,7 @@ _PROTOTYPES = {
                                   "mlr_attention_sigmoid_tcgen05_scratch": "iiiii"},
     "attention_prefix": {"mlr_attention_prefix": "pppppppp" "ppppp" "pp" "iiiiiiiiiiii" "fiipp"},
     "adapters": {"mlr_adapter_down": "pppppiiiiiip", "mlr_adapter_up": "pppppiiiiiip"},
+    "adapters_small": {"mlr_adapter_small": "pppppppp" "iiiiiii" "p"},
     "adapters_tcgen05": {"mlr_adapter_gemm": "ppppppp" "iiiiii" "pp"},
     "logit_rules": {"mlr_logit_rules": "pppiii" "pppppip" "p", "mlr_count_tokens": "ppippiiip"},
 }
@@ -242,10 +243,10 @@ class AdapterStack:
         if min(self.down.shape[2], self.up.shape[1]) < 1 or self.down.data_ptr() % 16 or self.up.data_ptr() % 16:
             raise KernelError("adapters need at least one column and 16-byte boundaries")
         _need_together(self.down, self.up, self.scales)
-
-    @property
-    def device(self) -> torch.device:
-        return self.down.device
+        # what a call asks for, once
+        for name, value in (("count", adapters), ("rank", rank), ("inner", self.down.shape[2]), ("outer", self.up.shape[1]),
+                            ("dtype", self.down.dtype), ("device", self.down.device)):
+            object.__setattr__(self, name, value)
 
 
 # Rows of one work item of the three prompt-attention kernels.
@@ -879,6 +880,19 @@ class CudaOps:
                                    _stream()), "linear")
         return out
 
+    # What a single launch must stay below: the bytes of the adapters that every CTA reads by itself, times the rows, and the elements of
+    # the weight.  Captured, us, one launch / three: bfloat16, one row, 256 x 256, rank 8 (4 KB) 2.9 / 6.4, rank 64 (32 KB) 8.0 / 8.7; 1,152 x
+    # 896, rank 8 (14 KB) 5.2 / 6.3, rank 16 (28 KB) 7.0 / 7.2, rank 64 17.6 / 8.8; 2,048 x 2,048, rank 8 7.2 / 6.2; 9,728 x 896, rank 8 21 / 8;
+    # two rows, 256 x 256, rank 16 (16 KB) 5.6 / 7.5; 1,152 x 896, rank 8 (28 KB) 9.5 / 6.5; four rows, 256 x 256, rank 8 6.5 / 6.5; float32, one
+    # row, 1,152 x 896, rank 8 (28 KB) 4.8 / 11.3.  From the host, where launches count, 11 / 30.
+    SMALL_ADAPTER_BYTES, SMALL_ADAPTER_WEIGHT = 28 << 10, 5 << 18
+
+    def _adapters_small(self, rows: int, outer: int, inner: int, rank: int, dtype: torch.dtype) -> bool:
+        """Whether a projection with adapters goes through one launch."""
+        row = inner * (2 if dtype == torch.bfloat16 else 4)
+        return (rows <= 4 and row % 16 == 0 and rows * rows * rank * row <= self.SMALL_ADAPTER_BYTES
+                and outer * inner <= self.SMALL_ADAPTER_WEIGHT)
+
     ADAPTER_ROWS = 128      # rows from which the adapters extend the shared product's sum over K
 
     def linear_adapters(self, x: torch.Tensor, weight: torch.Tensor, adapters: AdapterStack, row_adapter: torch.Tensor,
@@ -889,12 +903,13 @@ class CudaOps:
         _need(row_adapter, "row_adapter", torch.int32, 1)
         _need(weight, "weight", x.dtype, 2)
         out_dtype = out_dtype or x.dtype
-        (rows, K), N, (count, rank, _) = x.shape, weight.shape[0], adapters.down.shape
-        if adapters.down.dtype != x.dtype or out_dtype not in (x.dtype, torch.float32):
+        rows, K = x.shape
+        N, count, rank = adapters.outer, adapters.count, adapters.rank
+        if adapters.dtype != x.dtype or out_dtype not in (x.dtype, torch.float32):
             raise KernelError(f"x in {x.dtype} needs adapters of that dtype and a result in it or float32")
-        if adapters.down.shape[2] != K or adapters.up.shape[1] != N or weight.shape[1] != K:
-            raise KernelError(f"the adapters are those of a projection {(adapters.up.shape[1], adapters.down.shape[2])}, x has {K} "
-                              f"columns and the weight is {tuple(weight.shape)}")
+        if adapters.inner != K or weight.shape != (N, K):
+            raise KernelError(f"the adapters are those of a projection {(N, adapters.inner)}, x has {K} columns and the weight is "
+                              f"{tuple(weight.shape)}")
         if row_adapter.shape[0] != rows:
             raise KernelError("row_adapter needs one entry per row of x")
         if x.data_ptr() % 16:
@@ -905,8 +920,15 @@ class CudaOps:
                 raise KernelError("bias length differs from the weight's output rows")
         _need_here(x=x, weight=weight, adapters=adapters, row_adapter=row_adapter, bias=bias)
         if rows == 0:
-            return torch.empty((0, N), dtype=out_dtype, device=x.device)
-        low = torch.empty((rows, rank), dtype=torch.float32, device=x.device)
+            return x.new_empty((0, N), dtype=out_dtype)
+        if self._adapters_small(rows, N, K, rank, x.dtype) and not weight.data_ptr() % 16:
+            out = x.new_empty((rows, N), dtype=out_dtype)
+            _check(_declared_library("adapters_small").mlr_adapter_small(
+                x.data_ptr(), weight.data_ptr(), _address(bias), adapters.down.data_ptr(), adapters.up.data_ptr(), adapters.scales.data_ptr(),
+                row_adapter.data_ptr(), out.data_ptr(), rows, N, K, count, rank, _code(x.dtype), _code(out_dtype), _raw_stream()),
+                "linear_adapters (small)")
+            return out
+        low = x.new_empty((rows, rank), dtype=torch.float32)
         library = _declared_library("adapters")
 
         def down(early: bool) -> None:
@@ -917,7 +939,7 @@ class CudaOps:
         if (self.use_tensor_cores and x.dtype == torch.bfloat16 and rows > self.ADAPTER_ROWS and K % 8 == 0 and rank % 8 == 0
                 and not weight.data_ptr() % 16 and count * N < 1 << 31):
             down(False)
-            out = torch.empty((rows, N), dtype=out_dtype, device=x.device)
+            out = x.new_empty((rows, N), dtype=out_dtype)
             _check(_declared_library("adapters_tcgen05").mlr_adapter_gemm(
                 x.data_ptr(), weight.data_ptr(), adapters.up.data_ptr(), low.data_ptr(), row_adapter.data_ptr(), _address(bias), out.data_ptr(),
                 rows, N, K, count, rank, int(out_dtype == torch.float32), self._error_word(x.device).data_ptr(), _raw_stream()),
@@ -931,7 +953,7 @@ class CudaOps:
         base = self.linear(x, weight, bias, out_dtype=torch.float32)
         if beside:
             down(True)
-        out = base if out_dtype == torch.float32 else torch.empty((rows, N), dtype=out_dtype, device=x.device)
+        out = base if out_dtype == torch.float32 else x.new_empty((rows, N), dtype=out_dtype)
         _check(library.mlr_adapter_up(low.data_ptr(), adapters.up.data_ptr(), row_adapter.data_ptr(), base.data_ptr(), out.data_ptr(),
                                       rows, count, rank, N, _code(x.dtype), _code(out_dtype), _raw_stream()), "linear_adapters (up)")
         return out

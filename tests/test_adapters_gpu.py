@@ -71,7 +71,7 @@ def some_ids(rows, count, pattern, seed):
 @pytest.mark.parametrize("pattern", ["one", "none", "runs", "mixed"])
 @pytest.mark.parametrize("rows,K,N,rank,count", [
     (1, 8, 8, 1, 1), (1, 896, 1152, 8, 4), (3, 100, 37, 5, 3), (7, 256, 136, 16, 4), (16, 520, 264, 24, 9), (33, 1000, 200, 64, 3),
-    (64, 896, 520, 12, 40), (130, 640, 392, 32, 6), (257, 384, 1000, 128, 7), (300, 72, 264, 40, 5),
+    (1, 16, 5, 128, 2), (2, 128, 72, 16, 4), (3, 64, 41, 7, 5), (4, 40, 100, 33, 6), (2, 896, 1152, 8, 3), (64, 896, 520, 12, 40), (130, 640, 392, 32, 6), (257, 384, 1000, 128, 7), (300, 72, 264, 40, 5),
 ])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_adapters_against_their_formula(dtype, rows, K, N, rank, count, pattern):
