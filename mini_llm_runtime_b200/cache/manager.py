@@ -26,6 +26,11 @@ rows changed (a page taken, a page given back, a request admitted or released).
 along with its own metadata; a step that changes no row sends none.  Kernels reach a request's
 row through its slot.
 
+Shared pages.  A request may start with the leading whole pages of another one that holds the same tokens (``create_request(...,
+prefix=(request, tokens))``): its block table names them, its own pages follow, and the tokens on them count as committed.  The
+request they belong to cannot be released before those that share its pages.  (Whole pages of groups that keep every key; a
+window gives pages back and a fixed-size state has none.)
+
 Two admission modes.  With a *promise* (``create_request(..., lifetime_tokens=n)``) the pages of
 the request's whole life are counted against the pool at creation, as the reference reserves them
 (src/mini_llm_runtime/block_admission.py:35-67), so the pool cannot run dry mid-request; pages are
@@ -91,9 +96,16 @@ class RequestCache:
     first_live: list[int] = field(default_factory=list)       # per group: lowest logical page held
     promised: list[int] = field(default_factory=list)         # per group pages promised (0: none)
     step_new_pages: list[list[int]] = field(default_factory=list)
+    shared_pages: int = 0             # leading pages, of every group, that belong to ``prefix_of``
+    prefix_of: str | None = None
+    sharers: int = 0                  # requests that start with pages of this one
+
+    def own(self, group: int) -> list[int]:
+        """The pages the request itself holds."""
+        return [p for p in self.pages[group][self.shared_pages:] if p >= 0]
 
     def held(self, group: int) -> int:
-        return sum(1 for p in self.pages[group] if p >= 0)
+        return len(self.own(group))
 
 
 @dataclass(frozen=True)
@@ -220,12 +232,15 @@ class CacheManager:
 
     # ------------------------------------------------------------------ requests
     def create_request(self, request_id: str, *, lifetime_tokens: int | None = None,
-                       temperature: float = 0.0, seed: int = 0) -> RequestCache | None:
+                       temperature: float = 0.0, seed: int = 0,
+                       prefix: tuple[str, int] | None = None) -> RequestCache | None:
         """Register a request and give it a slot.  With ``lifetime_tokens`` its pages are promised
         now; returns None (nothing changed) if the promise cannot be kept or no slot is free.
-        ``temperature`` and ``seed`` go into the slot's record for the sampling kernel."""
+        ``temperature`` and ``seed`` go into the slot's record for the sampling kernel.  ``prefix``: the request
+        starts with that many tokens of another one, on its pages."""
         if request_id in self.requests:
             raise ValueError(f"request {request_id!r} already has a cache")
+        source, shared = self._shared_pages(request_id, lifetime_tokens, prefix)
         if self.slots.free_count == 0:
             if lifetime_tokens is None:
                 raise OutOfPages(f"no free request slot (max_requests={self.max_requests})")
@@ -240,7 +255,7 @@ class CacheManager:
                                  f"{lifetime_tokens} tokens; the pools hold "
                                  f"{tuple(g.num_pages for g in self.groups)} pages and requests "
                                  f"are limited to {self.max_tokens_per_request} tokens")
-            wanted = self.lifetime_pages(lifetime_tokens)
+            wanted = tuple(count - shared for count in self.lifetime_pages(lifetime_tokens))
             done = []
             for group, count in zip(self.groups, wanted):
                 if not group.allocator.promise(count):
@@ -255,12 +270,39 @@ class CacheManager:
                                first_live=[0] * len(self.groups),
                                promised=promised,
                                step_new_pages=[[] for _ in self.groups])
+        if source is not None:
+            source.sharers += 1
+            request.shared_pages, request.prefix_of, request.committed = shared, source.request_id, shared * self.page_size
+            for group in self.groups:
+                request.pages[group.index] = source.pages[group.index][:shared]
+                group.table[slot, :shared] = request.pages[group.index]
+                group.dirty.add(slot)
         self.requests[request_id] = request
         for tensor in self._state_tensors():
             tensor[slot].zero_()
-        self.slot_mirror[slot] = slot_record(temperature=temperature, seed=seed)
+        self.slot_mirror[slot] = slot_record(length=request.committed, temperature=temperature, seed=seed)
         self._new_records.add(slot)
         return request
+
+    @property
+    def can_share_pages(self) -> bool:
+        """Whether requests may start with one another's pages: every group keeps all keys, and there is no fixed-size state."""
+        return bool(self.groups) and all(group.need.span is None for group in self.groups) and not any(
+            isinstance(need, StateNeed) for parts in self.entry_needs for need in parts)
+
+    def _shared_pages(self, request_id: str, lifetime_tokens: int | None, prefix) -> tuple["RequestCache | None", int]:
+        """The request whose pages are to be shared and how many of them, checked."""
+        if prefix is None:
+            return None, 0
+        source, tokens = self.get(prefix[0]), int(prefix[1])
+        if not self.can_share_pages:
+            raise ValueError("pages are shared by models whose layers keep every key, without windows or states")
+        if tokens <= 0 or tokens % self.page_size or tokens > source.committed:
+            raise ValueError(f"request {request_id!r} cannot share {tokens} tokens of {source.request_id!r}: whole pages of "
+                             f"{self.page_size} of its {source.committed} tokens")
+        if tokens >= (lifetime_tokens if lifetime_tokens is not None else self.max_tokens_per_request):
+            raise ValueError(f"request {request_id!r} would have no token of its own behind {tokens} shared ones")
+        return source, tokens // self.page_size
 
     def _state_tensors(self):
         for by_name in self.states.values():
@@ -277,9 +319,11 @@ class CacheManager:
         request = self.get(request_id)
         if self._step is not None and any(r is request for r, _ in self._step):
             raise RuntimeError(f"request {request_id!r} is part of the step in flight")
+        if request.sharers:
+            raise RuntimeError(f"request {request_id!r} has pages that {request.sharers} other requests start with")
         freed: dict[int, list[int]] = {}
         for group in self.groups:
-            ids = [p for p in request.pages[group.index] if p >= 0]
+            ids = request.own(group.index)
             group.allocator.free(ids, promised=bool(request.promised[group.index]))
             group.allocator.unpromise(request.promised[group.index])
             group.table[request.slot, :] = -1
@@ -287,6 +331,8 @@ class CacheManager:
             freed[group.index] = ids
         self.slots.free([request.slot])
         del self.requests[request_id]
+        if request.prefix_of is not None:
+            self.requests[request.prefix_of].sharers -= 1
         return freed
 
     # ------------------------------------------------------------------ the step transaction
@@ -474,14 +520,21 @@ class CacheManager:
         )
 
     def check_consistency(self) -> None:
-        """Every held page belongs to exactly one request; tables mirror the lists (tests)."""
+        """Every held page belongs to exactly one request, shared pages are those of the request they are shared with; tables mirror
+        the lists (tests)."""
+        for request in self.requests.values():
+            sharers = sum(other.prefix_of == request.request_id for other in self.requests.values())
+            if sharers != request.sharers:
+                raise AssertionError(f"{request.request_id!r} counts {request.sharers} sharers, {sharers} share its pages")
+            if request.prefix_of is not None:
+                source = self.requests[request.prefix_of]
+                if any(request.pages[g.index][:request.shared_pages] != source.pages[g.index][:request.shared_pages] for g in self.groups):
+                    raise AssertionError(f"{request.request_id!r} does not start with the pages of {source.request_id!r}")
         for group in self.groups:
             owners: dict[int, str] = {}
             for request in self.requests.values():
                 pages = request.pages[group.index]
-                for logical, page_id in enumerate(pages):
-                    if page_id < 0:
-                        continue
+                for page_id in request.own(group.index):
                     if page_id in owners:
                         raise AssertionError(f"page {page_id} of group {group.index} is held by "
                                              f"{owners[page_id]!r} and {request.request_id!r}")

@@ -26,6 +26,7 @@ import numpy as np
 import torch
 
 from .. import ops
+from ..cache.allocator import OutOfPages
 from ..cache.manager import CacheManager
 from ..models.decoder import DecoderModel
 from ..sampling import LogitRules, SamplingParams
@@ -89,6 +90,7 @@ class ContinuousBatchEngine:
         self._ahead: _TokensInFlight | None = None
         self._token_buffers: list[torch.Tensor] = []
         self._next_buffer = 0
+        self._prefixes: dict[str, tuple[int, ...]] = {}      # tokens of the prefixes that requests may share, by name
         self._allowed: dict[str, np.ndarray] = {}      # grammars of requests that wait, until they own a slot
 
     # ------------------------------------------------------------------ assembly
@@ -100,22 +102,25 @@ class ContinuousBatchEngine:
                    max_mixed_prefill_tokens: int | None = None, max_model_len: int | None = None,
                    batching_policy: BatchingPolicy = BatchingPolicy.CONTINUOUS,
                    chunked_prefill: bool = True, enable_nvtx: bool = False,
-                   step_ahead: bool = False, logit_rules: bool = False) -> "ContinuousBatchEngine":
-        """``logit_rules``: requests may bring penalties, biases and grammars (``submit``, ``allow_tokens``); every step then applies them."""
+                   step_ahead: bool = False, logit_rules: bool = False, max_prefixes: int = 0) -> "ContinuousBatchEngine":
+        """``logit_rules``: requests may bring penalties, biases and grammars (``submit``, ``allow_tokens``); every step then applies them.
+        ``max_prefixes``: how many prefixes the cache may hold for requests to share (``add_prefix``)."""
         # a model without a position limit of its own gets this engine's default
         max_model_len = min(max_model_len or min(model.spec.max_positions, cls.DEFAULT_MODEL_LEN),
                             model.spec.max_positions)
+        if max_prefixes < 0:
+            raise ValueError("max_prefixes must be >= 0")
         if total_blocks is None:
-            total_blocks = max_running_requests * -(-max_model_len // block_size)
+            total_blocks = (max_running_requests + max_prefixes) * -(-max_model_len // block_size)
         cache = CacheManager(model.cache_needs(), page_size=block_size, num_pages=total_blocks,
-                             max_requests=max_running_requests, max_tokens_per_request=max_model_len,
+                             max_requests=max_running_requests + max_prefixes, max_tokens_per_request=max_model_len,
                              dtype=model.compute_dtype, device=model.device, max_step_tokens=max_batch_tokens)
         scheduler = RequestScheduler(max_running_requests=max_running_requests, max_batch_tokens=max_batch_tokens,
                                      max_mixed_prefill_tokens=max_mixed_prefill_tokens, gate=CacheGate(cache),
                                      batching_policy=batching_policy, chunked_prefill=chunked_prefill)
         runner = ModelRunner(model, cache)
         if logit_rules:
-            runner.rules = LogitRules(max_running_requests, runner.vocab_size, model.device)
+            runner.rules = LogitRules(cache.max_requests, runner.vocab_size, model.device)
         return cls(scheduler=scheduler, runner=runner, enable_nvtx=enable_nvtx, step_ahead=step_ahead)
 
     @classmethod
@@ -136,8 +141,8 @@ class ContinuousBatchEngine:
     # ------------------------------------------------------------------ requests
     def submit(self, request_id: str, prompt_token_ids: Sequence[int], *, max_new_tokens: int,
                eos_token_ids: int | Collection[int] | None = None, temperature: float = 0.0,
-               seed: int = 0, **rules) -> Request:
-        """``rules``: ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty``, ``logit_bias`` of ``SamplingParams`` (an engine
+               seed: int = 0, prefix: str | None = None, **rules) -> Request:
+        """``prefix``: a prefix of ``add_prefix`` that the prompt starts with; its whole pages are shared, not computed again.  ``rules``: ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty``, ``logit_bias`` of ``SamplingParams`` (an engine
         made with ``logit_rules=True``)."""
         arrival_ns = self._clock_ns()
         vocab = self.runner.vocab_size
@@ -153,10 +158,70 @@ class ContinuousBatchEngine:
             self.runner.rules.check(sampling)
         elif sampling.has_rules:
             raise ValueError("rules on logits need an engine made with logit_rules=True")
+        holder, shared = self._shared_by(prefix, prompt_token_ids)
         request = self.scheduler.submit(request_id, prompt_token_ids, max_new_tokens=max_new_tokens,
-                                        eos_token_ids=eos_token_ids, sampling=sampling)
+                                        eos_token_ids=eos_token_ids, sampling=sampling, prefix=holder, shared=shared)
         self.metrics.register_request(request_id, arrival_ns)
         return request
+
+    # ------------------------------------------------------------------ shared prefixes
+    @staticmethod
+    def _holder(name: str) -> str:
+        return f"prefix {name}"
+
+    @torch.inference_mode()
+    def add_prefix(self, name: str, token_ids: Sequence[int]) -> int:
+        """Compute a prefix that requests may start with (a system prompt, a document) and keep its pages until ``drop_prefix``; to be
+        called between steps.  Returns how many of its tokens are shared: those on whole pages."""
+        tokens = tuple(int(t) for t in token_ids)
+        page = self.manager.page_size
+        if not self.manager.can_share_pages:
+            raise ValueError("pages are shared by models whose layers keep every key, without windows or states")
+        if name in self._prefixes:
+            raise ValueError(f"prefix {name!r} exists already")
+        if len(tokens) < page:
+            raise ValueError(f"a prefix of {len(tokens)} tokens fills no page of {page}")
+        if any(not 0 <= t < self.runner.vocab_size for t in tokens):
+            raise ValueError(f"prefix token ids must lie in [0, {self.runner.vocab_size})")
+        shared = len(tokens) // page * page
+        holder = self._holder(name)
+        if self.manager.slots.free_count <= self.scheduler.max_running_requests - len(self.scheduler.running_request_ids):
+            raise ValueError(f"the engine was made for {self.manager.max_requests - self.scheduler.max_running_requests} prefixes")
+        if self.manager.create_request(holder, lifetime_tokens=shared) is None:
+            raise OutOfPages(f"no room for the {shared // page} pages of prefix {name!r}")
+        try:
+            portion = self.scheduler.max_batch_tokens
+            for start in range(0, shared, portion):
+                self.runner.step([StepEntry(holder, tokens[start:min(shared, start + portion)])])
+        except BaseException:
+            self.manager.release(holder)
+            raise
+        self._prefixes[name] = tokens
+        return shared
+
+    def drop_prefix(self, name: str) -> None:
+        """Give a prefix's pages back; every request that shares them must have ended."""
+        if name not in self._prefixes:
+            raise KeyError(f"no prefix {name!r}")
+        holder = self._holder(name)
+        users = [rid for rid in (*self.scheduler.waiting_request_ids, *self.scheduler.running_request_ids)
+                 if self.scheduler.get_request(rid).prefix == holder]
+        if users:
+            raise RuntimeError(f"prefix {name!r} is shared by requests {users[:5]}")
+        self.manager.release(holder)
+        del self._prefixes[name]
+
+    def _shared_by(self, name: str | None, prompt: Sequence[int]) -> tuple[str | None, int]:
+        """The cached request that holds the prefix and the tokens the prompt shares with it: whole pages, and fewer than the prompt's."""
+        if name is None:
+            return None, 0
+        if name not in self._prefixes:
+            raise ValueError(f"no prefix {name!r}; known: {sorted(self._prefixes)}")
+        tokens, page = self._prefixes[name], self.manager.page_size
+        if tuple(prompt[:len(tokens)]) != tokens[:len(prompt)]:
+            raise ValueError(f"the prompt does not start with the tokens of prefix {name!r}")
+        shared = min(len(tokens), len(prompt) - 1) // page * page
+        return (self._holder(name), shared) if shared else (None, 0)
 
     def allow_tokens(self, request_id: str, tokens: "Collection[int] | None") -> None:
         """The tokens that the request may choose from its next step on (None: all), as a grammar finds them after each token.  A

@@ -89,6 +89,8 @@ class Request:
     output: list[int] = field(default_factory=list, repr=False)
     finish_reason: FinishReason | None = None
     slot: int | None = None
+    prefix: str | None = None                   # the cached request whose pages hold the prompt's first ``shared`` tokens
+    shared: int = 0
     _prompt_array: "np.ndarray | None" = field(default=None, repr=False, compare=False)
 
     @property
@@ -201,7 +203,8 @@ class CacheGate:
 
     def admit(self, request: Request) -> int | None:
         held = self.cache.create_request(request.request_id, lifetime_tokens=request.lifetime_tokens,
-                                         temperature=request.sampling.temperature, seed=request.sampling.seed)
+                                         temperature=request.sampling.temperature, seed=request.sampling.seed,
+                                         prefix=None if request.prefix is None else (request.prefix, request.shared))
         return None if held is None else held.slot
 
     def release(self, request_id: str):
@@ -285,8 +288,10 @@ class RequestScheduler:
     # ------------------------------------------------------------------ arrival
     def submit(self, request_id: str, prompt_token_ids: Sequence[int], *, max_new_tokens: int,
                eos_token_ids: int | Collection[int] | None = None, temperature: float = 0.0,
-               seed: int = 0, sampling: SamplingParams | None = None) -> Request:
-        """Queue a request; allowed at any time, also while a plan is outstanding."""
+               seed: int = 0, sampling: SamplingParams | None = None, prefix: str | None = None,
+               shared: int = 0) -> Request:
+        """Queue a request; allowed at any time, also while a plan is outstanding.  ``prefix``, ``shared``: the prompt's first tokens
+        are on the pages of that cached request; only those behind them run through the model."""
         if not request_id:
             raise ValueError("request_id must not be empty")
         if request_id in self._by_id:
@@ -294,8 +299,10 @@ class RequestScheduler:
         prompt = tuple(_token(t, "prompt_token_ids") for t in prompt_token_ids)
         if not prompt:
             raise ValueError("prompt_token_ids must not be empty")
-        if not self.chunked_prefill and len(prompt) > self.max_batch_tokens:
-            raise ValueError(f"prompt length={len(prompt)} exceeds max_batch_tokens={self.max_batch_tokens} "
+        if (prefix is None) != (shared == 0) or not 0 <= shared < len(prompt):
+            raise ValueError("a shared prefix is shorter than the prompt and names the request it belongs to")
+        if not self.chunked_prefill and len(prompt) - shared > self.max_batch_tokens:
+            raise ValueError(f"prompt length={len(prompt) - shared} exceeds max_batch_tokens={self.max_batch_tokens} "
                              "and chunked prefill is off")
         if isinstance(max_new_tokens, bool) or not isinstance(max_new_tokens, int) or max_new_tokens <= 0:
             raise ValueError("max_new_tokens must be a positive integer")
@@ -306,7 +313,8 @@ class RequestScheduler:
                              for t in ((eos_token_ids,) if isinstance(eos_token_ids, int) else eos_token_ids))
         if sampling is None:
             sampling = SamplingParams(temperature, seed) if (temperature or seed) else GREEDY
-        request = Request(request_id, prompt, max_new_tokens, stop, sampling, order=self._arrivals)
+        request = Request(request_id, prompt, max_new_tokens, stop, sampling, order=self._arrivals, cursor=shared, prefix=prefix,
+                          shared=shared)
         self._arrivals += 1
         self._by_id[request_id] = request
         self._queue.append(request)
@@ -344,7 +352,7 @@ class RequestScheduler:
         while may_admit and self._queue and len(self._live) < self.max_running_requests:   # 3. admission
             request = self._queue[0]
             room = budget.room_for_prompt()
-            if room <= 0 or (not self.chunked_prefill and len(request.prompt) > room):
+            if room <= 0 or (not self.chunked_prefill and len(request.prompt) - request.shared > room):
                 break
             if self.gate is not None:
                 slot = self.gate.admit(request)
@@ -421,7 +429,7 @@ class RequestScheduler:
             raise RuntimeError("no plan to abort")
         returned = [self._by_id[rid] for rid in plan.admitted_request_ids]
         for request in returned:
-            if request.cursor or request.output:
+            if request.cursor != request.shared or request.output:
                 raise RuntimeError(f"request {request.request_id!r} already has results; its step cannot be aborted")
         for request in reversed(returned):
             del self._live[request.request_id]

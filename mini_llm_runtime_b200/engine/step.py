@@ -63,6 +63,8 @@ class HostBatch:
     row_start: np.ndarray        # int32: its first row in the packed batch
     position_start: np.ndarray   # int32: position of its first row
     num_rows: int
+    # of a step of decoded tokens: (segments, keys) of requests whose first keys are on the same pages
+    shared: tuple = ()
 
     @property
     def num_segments(self) -> int:
@@ -179,6 +181,8 @@ class _CapturedStep:
     slots_now: tuple[int, ...] = ()        # the slots the device copy currently holds
     stagings: list = field(default_factory=list)     # pinned [2 * batch] int32 buffers with their events
     cursor: int = 0
+    shared_now: tuple = ()                 # groups of shared prefixes whose work lists the device copy currently holds
+    plans: dict = field(default_factory=dict)
 
 
 _TORCH_OF = {np.dtype(np.int32): torch.int32, np.dtype(np.int64): torch.int64,
@@ -211,8 +215,8 @@ class ModelRunner:
         # milliseconds, which a size that passes by once (requests finishing one after another)
         # never earns back.
         self.graph_capture_after = 3
-        self._graphs: dict[tuple[int, bool, bool, int], _CapturedStep] = {}       # (batch, sample, feed, context limit)
-        self._graph_seen: dict[tuple[int, bool, bool, int], int] = {}
+        self._graphs: dict[tuple, _CapturedStep] = {}       # by _graph_key: (batch, sample, feed, context limit, groups of shared prefixes ..)
+        self._graph_seen: dict[tuple, int] = {}
         self.graph_replays = 0
         # Rules of the requests on their logits (sampling/rules.py), or None.  To be set before the first step: a captured step
         # holds the launches of its time.
@@ -279,7 +283,23 @@ class ModelRunner:
         row_start = np.zeros(len(entries), dtype=np.int32)
         np.cumsum(lengths[:-1], out=row_start[1:])
         position_start = np.array([r.pending[0] for r in requests], dtype=np.int32)
-        return HostBatch(lengths, row_start, position_start, int(lengths.sum()))
+        shared = self._shared_groups(requests) if (lengths == 1).all() else ()
+        return HostBatch(lengths, row_start, position_start, int(lengths.sum()), shared)
+
+    def _shared_groups(self, requests: list[RequestCache]) -> tuple:
+        """(segments, keys) of the requests that start with the same pages, two of them at least; longest prefixes first."""
+        groups: dict[tuple, list[int]] = {}
+        for index, request in enumerate(requests):
+            if request.prefix_of is not None:
+                groups.setdefault((request.prefix_of, request.shared_pages), []).append(index)
+        found = [(tuple(segments), pages * self.cache.page_size) for (_, pages), segments in groups.items() if len(segments) > 1]
+        return tuple(sorted(found, key=lambda group: (-group[1], -len(group[0]), group[0])))
+
+    def _graph_key(self, requests: list[RequestCache], sample: bool, feed: bool) -> tuple:
+        """What a captured decode step depends on: its size, what it does, the context limit it plans for, and the sizes of its
+        groups of shared prefixes (which requests they are is refreshed like the slots)."""
+        shapes = tuple((len(segments), keys) for segments, keys in self._shared_groups(requests))
+        return (len(requests), sample, feed, self._context_limit(requests), *shapes)
 
     def _step_plans(self, host: HostBatch) -> dict:
         """Work lists from the mixers, one per plan key (mixers with equal keys share one)."""
@@ -454,7 +474,7 @@ class ModelRunner:
                 and isinstance(ops.current(), ops.CudaOps)
                 and all(len(e.tokens) == 1 and len(e.want) == 1 for e in entries)):
             return False
-        key = (len(entries), sample, feed, self._context_limit(requests))
+        key = self._graph_key(requests, sample, feed)
         if key in self._graphs:
             return True
         seen = self._graph_seen.get(key, 0) + 1
@@ -484,7 +504,7 @@ class ModelRunner:
         size runs eagerly on the graph's fixed buffers and is then captured; later steps refresh at
         most the slots and the host's tokens, send changed table rows, and replay."""
         count = len(entries)
-        key = (count, sample, feed, self._context_limit(requests))
+        key = self._graph_key(requests, sample, feed)
         captured = self._graphs.get(key)
         slots = tuple(r.slot for r in requests)
         if captured is not None and captured.graph is not None:
@@ -509,6 +529,14 @@ class ModelRunner:
                     staging[1] = event = torch.cuda.Event()
                 event.record()
                 captured.slots_now = slots
+            shared = self._shared_groups(requests)
+            if shared != captured.shared_now:      # the same sizes, other requests
+                for name, (arrays, _) in self._step_plans(self._host_batch(entries, requests)).items():
+                    for array_name, array in arrays.items():
+                        if array_name.startswith("shared."):
+                            captured.plans[name][0][array_name].copy_(torch.from_numpy(array))
+                            self.bytes_sent += array.nbytes
+                captured.shared_now = shared
             captured.graph.replay()
             self.graph_replays += 1
             return captured.logits, captured.tokens
@@ -523,6 +551,7 @@ class ModelRunner:
                                   device_buffer=captured.metadata, kv_limit=key[3])
         self._graphs[key] = captured
         captured.slots_now = slots
+        captured.shared_now, captured.plans = packed[1].shared, ctx.plans
         self._prepare_decode(ctx, feed)
         logits, tokens = self._forward(ctx, sample, lengths_by_device=True)     # this step's real result
         torch.cuda.synchronize(self.device)
@@ -539,7 +568,7 @@ class ModelRunner:
 
     def launches_per_replay(self, batch: int, sampling: bool, feed: bool | None = None) -> int:
         """Kernels one replay of the captured step of this batch size launches (0 if not captured)."""
-        for (count, sample, fed, _), captured in self._graphs.items():
+        for (count, sample, fed, *_), captured in self._graphs.items():
             if count == batch and sample == sampling and (feed is None or fed == feed) and captured.graph is not None:
                 return captured.launches
         return 0

@@ -1077,6 +1077,11 @@ class CudaOps:
     # 40 heads of 128, 2 x 8,192 (33 MB) 17.1 / 15.7, 8 x 2,048 (59 MB) 12.4 / 13.2, 64 x 8,192 (2 GB) 37 / 181.
     SHARED_PREFIX_LEAST = 48 << 20
 
+    def shares_prefix(self, dtype: torch.dtype, counts: dict, num_kv_heads: int, head_dim: int) -> bool:
+        """Whether the prefixes of ``plan_shared_prefix`` are worth their own walk on the tensor cores."""
+        return (self.use_mma_attention and dtype == torch.bfloat16 and head_dim in (64, 128) and counts["heads_per_kv"] <= 16
+                and 4 * counts["saved_keys"] * num_kv_heads * head_dim >= self.shared_prefix_least)
+
     def shared_prefix_attention(self, q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, batch: AttentionBatch,
                                 prefix: SharedPrefix, num_heads: int, num_kv_heads: int, head_dim: int, scale: float) -> torch.Tensor:
         """``paged_attention`` of a step of decoded tokens whose requests share leading pages: the keys and values of a prefix are
@@ -1109,7 +1114,7 @@ class CudaOps:
                 and not (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr()) % 16)
         if segments == 0:
             return torch.empty_like(q)
-        if fast and 4 * counts["saved_keys"] * num_kv_heads * head_dim < self.shared_prefix_least:
+        if fast and not self.shares_prefix(q.dtype, counts, num_kv_heads, head_dim):
             return self.paged_attention(q, k_pool, v_pool, batch, num_heads, num_kv_heads, head_dim, scale, None)
         out = torch.empty_like(q)
         chunk, parts, units, own_parts = prefix_parts(counts["tile_keys"], counts["least_shared"], segments, batch.max_kv_len, num_heads,

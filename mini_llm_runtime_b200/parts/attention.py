@@ -14,7 +14,7 @@ import torch
 
 from .. import ops
 from ..config.spec import PartSpec
-from ..ops import AttentionBatch
+from ..ops import AttentionBatch, SharedPrefix
 from .base import KVCacheNeed, Mixer, TensorSpec, build_part, register_part
 
 
@@ -108,6 +108,29 @@ class GQAAttention(PagedAttention):
         self.w_qkv = folded.to(self.compute_dtype).contiguous()
         self.input_norm_eps = float(eps)
 
+    def step_plan(self, host):
+        """The attention kernels' work lists and, where requests of the step share enough leading pages, those of their prefixes."""
+        arrays, counts = super().step_plan(host)
+        shared = getattr(host, "shared", ())
+        if shared and self.window is None:
+            k = ops.current()
+            lists, numbers = k.plan_shared_prefix(shared, host.num_segments, self.num_heads // self.num_kv_heads)
+            if k.shares_prefix(self.compute_dtype, numbers, self.num_kv_heads, self.head_dim):
+                arrays = {**arrays, **{"shared." + name: array for name, array in lists.items()}}
+                counts = {**counts, "shared": numbers}
+        return arrays, counts
+
+    def _shared_prefix(self, batch, view):
+        """The step's shared prefixes if its work lists hold them for this layer's heads, else None."""
+        numbers = batch.counts.get("shared")
+        if numbers is None or self.window is not None or numbers["heads_per_kv"] != self.num_heads // self.num_kv_heads:
+            return None
+        if "shared_prefix" not in view.shared:
+            head = "shared."
+            view.shared["shared_prefix"] = SharedPrefix(
+                {name[len(head):]: array for name, array in batch.plan.items() if name.startswith(head)}, numbers)
+        return view.shared["shared_prefix"]
+
     def forward(self, x, ctx, view, writes_cache, raw_input=False, residual=None):
         """``raw_input``: x is the un-normalised stream and the q/k/v product applies the row scale
         of the folded norm.  ``residual``: the output product adds into it in place."""
@@ -115,7 +138,16 @@ class GQAAttention(PagedAttention):
         qkv = k.linear(x, self.w_qkv, self.b_qkv, rms_eps=self.input_norm_eps if raw_input else None)
         batch = self._batch(ctx, view)
         frequencies = self._no_rotation if self.position is None else self.position.rotary_frequencies()
-        if frequencies is not None:
+        prefix = self._shared_prefix(batch, view)
+        if prefix is not None:
+            if frequencies is not None:
+                q = k.rope_kv_write(qkv, ctx.positions, frequencies, view.slots, view.k_pool, view.v_pool, self.num_heads,
+                                    self.num_kv_heads, self.head_dim, writes_cache)
+            else:
+                q = self.position.rotate_and_store(qkv, ctx, view, self.num_heads, self.num_kv_heads, self.head_dim, writes_cache)
+            mixed = k.shared_prefix_attention(q, view.k_pool, view.v_pool, batch, prefix, self.num_heads, self.num_kv_heads,
+                                              self.head_dim, self.scale)
+        elif frequencies is not None:
             # a plain rotary encoding (or none): rotation, cache write and attention may share kernels
             mixed = k.rope_paged_attention(qkv, ctx.positions, frequencies, view.slots, view.k_pool, view.v_pool,
                                            batch, self.num_heads, self.num_kv_heads, self.head_dim, self.scale,
