@@ -511,6 +511,7 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
 // AFTER_PREFIX: launched behind the prefix kernel, which lets the next kernel in after its own wait: everything before both is
 // done then, and what this kernel reads is written by neither; it starts beside the prefix kernel and waits for it at its end.
 constexpr int OWN_THREADS = 160;
+constexpr int FINISH_PARTS = 64;      // parts of a prefix, at most
 
 template <int D>
 struct OwnShape {
@@ -529,7 +530,9 @@ __device__ __forceinline__ uint32_t turned(uint32_t v) {
   return w;
 }
 
-template <int D, int NT, bool AFTER_PREFIX>
+// FINISH: one own part per request; the CTA then holds everything but the prefix's parts, and puts them together itself (a
+// kernel behind that reads all parts again costs its launch and wait, 5 to 10 us).
+template <int D, int NT, bool AFTER_PREFIX, bool FINISH>
 __global__ void __launch_bounds__(OWN_THREADS)
 prefix_own_mma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const PrefixCall c,
                       int page_shift, int* error_word) {
@@ -703,28 +706,87 @@ prefix_own_mma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
         }
     }
     __syncthreads();
-    const size_t at0 = ((size_t)(c.prefix_parts + part) * c.segments + segment) * c.heads + kv_head * per;
-    for (int i = threadIdx.x; i < per * D; i += OWN_THREADS) {
-      const int row = i / D, d = i - row * D;
-      float top = -INFINITY;
+    if (!FINISH) {
+      const size_t at0 = ((size_t)(c.prefix_parts + part) * c.segments + segment) * c.heads + kv_head * per;
+      for (int i = threadIdx.x; i < per * D; i += OWN_THREADS) {
+        const int row = i / D, d = i - row * D;
+        float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) top = fmaxf(top, sums[2 * (w * HEADS + row)]);
-      const float base = top == -INFINITY ? 0.f : top;
-      float sum = 0.f, value = 0.f;
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, sums[2 * (w * HEADS + row)]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, value = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float factor = exp2f(sums[2 * (w * HEADS + row)] - base);
-        sum = fmaf(sums[2 * (w * HEADS + row) + 1], factor, sum);
-        value = fmaf(states[(w * HEADS + row) * Shape::PITCH + d], factor, value);
-      }
-      c.acc[(at0 + row) * D + d] = value;
-      if (d == 0) {
-        c.state[2 * (at0 + row)] = top;
-        c.state[2 * (at0 + row) + 1] = sum;
+        for (int w = 0; w < 4; ++w) {
+          const float factor = exp2f(sums[2 * (w * HEADS + row)] - base);
+          sum = fmaf(sums[2 * (w * HEADS + row) + 1], factor, sum);
+          value = fmaf(states[(w * HEADS + row) * Shape::PITCH + d], factor, value);
+        }
+        c.acc[(at0 + row) * D + d] = value;
+        if (d == 0) {
+          c.state[2 * (at0 + row)] = top;
+          c.state[2 * (at0 + row) + 1] = sum;
+        }
       }
     }
   }
   if (AFTER_PREFIX) pdl_wait();
+  if (FINISH) {
+    // parts of a row: the prefix's, then the four warps' states; their factors first, then the sums of whole rows
+    constexpr int LANES = D / 4, ROWS_AT_ONCE = 32 / LANES;
+    __shared__ float factors[HEADS][FINISH_PARTS + 4], inverses[HEADS];
+    const int per = c.heads / c.kv_heads;
+    const int parts = c.chunk > 0 ? (c.seg_keys[segment] + c.chunk - 1) / c.chunk : 0;
+    const float* states = reinterpret_cast<const float*>(ring);
+    const float* sums = states + 4 * HEADS * Shape::PITCH;
+    const size_t row0 = (size_t)segment * c.heads + kv_head * per, pitch = (size_t)c.segments * c.heads;
+    for (int row = warp; row < per; row += OWN_THREADS / 32) {
+      float2 state[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const int at = lane + 32 * i;
+        state[i] = make_float2(-INFINITY, 0.f);
+        if (at < parts) state[i] = __ldcg(reinterpret_cast<const float2*>(c.state) + at * pitch + row0 + row);
+        else if (at < parts + 4 && tiles > 0) state[i] = *reinterpret_cast<const float2*>(sums + 2 * ((at - parts) * HEADS + row));
+      }
+      const float top = warp_max(fmaxf(state[0].x, fmaxf(state[1].x, state[2].x))), base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const int at = lane + 32 * i;
+        const float factor = exp2f(state[i].x - base);
+        sum = fmaf(state[i].y, factor, sum);
+        if (at < parts + 4) factors[row][at] = factor;
+      }
+      sum = warp_sum(sum);
+      if (lane == 0) inverses[row] = sum == 0.f ? 0.f : 1.f / sum;      // NaN stays
+    }
+    __syncthreads();
+    for (int r0 = warp * ROWS_AT_ONCE; r0 < per; r0 += OWN_THREADS / 32 * ROWS_AT_ONCE) {
+      const int row = r0 + lane / LANES, d = lane % LANES * 4;
+      if (row >= per) continue;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      auto add = [&](const float4& v, float factor) {
+        o.x = fmaf(v.x, factor, o.x); o.y = fmaf(v.y, factor, o.y); o.z = fmaf(v.z, factor, o.z); o.w = fmaf(v.w, factor, o.w);
+      };
+      const float* from = c.acc + (row0 + row) * D + d;
+      for (int k0 = 0; k0 < parts; k0 += 8) {
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          v[k] = k0 + k < parts ? __ldcg(reinterpret_cast<const float4*>(from + (size_t)(k0 + k) * pitch * D)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k0 + k < parts) add(v[k], factors[row][k0 + k]);
+      }
+      if (tiles > 0)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          add(*reinterpret_cast<const float4*>(states + (w * HEADS + row) * Shape::PITCH + d), factors[row][parts + w]);
+      const float inverse = inverses[row];
+      *reinterpret_cast<uint2*>((bf16*)c.out + ((size_t)q_row * c.heads + kv_head * per + row) * D + d) =
+          make_uint2(pack_bf16(o.x * inverse, o.y * inverse), pack_bf16(o.z * inverse, o.w * inverse));
+    }
+  }
 }
 
 // ------------------------------------------------------------------ the parts put together
@@ -827,12 +889,14 @@ static int run_plain(const PrefixCall& c, cudaStream_t stream) {
 
 template <int D, int NT>
 static int run_fast(const PrefixCall& c, int units, int* error_word, cudaStream_t stream) {
-  static OncePerDevice once[3];
+  static OncePerDevice once[5];
   const size_t prefix_shared = PT_SHARED<D>, own_shared = OwnShape<D>::DATA_BYTES + 1024;
   auto allow = [](auto kernel, size_t bytes) { return [=] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes); }; };
   if (cudaError_t err = once[0](allow(prefix_parts_tcgen05_kernel<D>, prefix_shared))) return (int)err;
-  if (cudaError_t err = once[1](allow(prefix_own_mma_kernel<D, NT, true>, own_shared))) return (int)err;
-  if (cudaError_t err = once[2](allow(prefix_own_mma_kernel<D, NT, false>, own_shared))) return (int)err;
+  if (cudaError_t err = once[1](allow(prefix_own_mma_kernel<D, NT, true, true>, own_shared))) return (int)err;
+  if (cudaError_t err = once[2](allow(prefix_own_mma_kernel<D, NT, true, false>, own_shared))) return (int)err;
+  if (cudaError_t err = once[3](allow(prefix_own_mma_kernel<D, NT, false, true>, own_shared))) return (int)err;
+  if (cudaError_t err = once[4](allow(prefix_own_mma_kernel<D, NT, false, false>, own_shared))) return (int)err;
   int page_shift = 0;
   while (1 << page_shift < c.page_size) ++page_shift;
   CUtensorMap k_map, v_map;
@@ -842,9 +906,11 @@ static int run_fast(const PrefixCall& c, int units, int* error_word, cudaStream_
   if (units > 0)
     launch_kernel(prefix_parts_tcgen05_kernel<D>, dim3(units, c.kv_heads), dim3(PT_THREADS), prefix_shared, stream, k_map, v_map, c, page_shift,
                   error_word);
-  auto own = units > 0 ? prefix_own_mma_kernel<D, NT, true> : prefix_own_mma_kernel<D, NT, false>;
+  const bool finish = c.own_parts == 1 && c.prefix_parts <= FINISH_PARTS;
+  auto own = units > 0 ? (finish ? prefix_own_mma_kernel<D, NT, true, true> : prefix_own_mma_kernel<D, NT, true, false>)
+                       : (finish ? prefix_own_mma_kernel<D, NT, false, true> : prefix_own_mma_kernel<D, NT, false, false>);
   launch_kernel(own, dim3(c.own_parts, c.segments, c.kv_heads), dim3(OWN_THREADS), own_shared, stream, k_map, v_map, c, page_shift, error_word);
-  launch_merge<bf16>(c, stream);
+  if (!finish) launch_merge<bf16>(c, stream);
   return launch_status();
 }
 
