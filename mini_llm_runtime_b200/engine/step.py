@@ -217,6 +217,8 @@ class ModelRunner:
         self.graph_capture_after = 3
         self._graphs: dict[tuple, _CapturedStep] = {}       # by _graph_key: (batch, sample, feed, context limit, groups of shared prefixes ..)
         self._graph_seen: dict[tuple, int] = {}
+        # Groups of shared prefixes come in many sizes: of the captured steps that hold any, the ones used last are kept.
+        self.graph_max_shared = 32
         self.graph_replays = 0
         # Rules of the requests on their logits (sampling/rules.py), or None.  To be set before the first step: a captured step
         # holds the launches of its time.
@@ -508,6 +510,7 @@ class ModelRunner:
         captured = self._graphs.get(key)
         slots = tuple(r.slot for r in requests)
         if captured is not None and captured.graph is not None:
+            self._graphs[key] = self._graphs.pop(key)      # in the order of their use
             self._send_resident_updates()
             refresh_slots = slots != captured.slots_now
             if refresh_slots or not feed:
@@ -541,6 +544,11 @@ class ModelRunner:
             self.graph_replays += 1
             return captured.logits, captured.tokens
 
+        shaped = [other for other in self._graphs if len(other) > 4]
+        if len(key) > 4 and len(shaped) >= self.graph_max_shared:
+            torch.cuda.synchronize(self.device)            # its last replay has ended
+            del self._graphs[shaped[0]]
+            self._graph_seen.pop(shaped[0], None)
         # first time at this size: give the graph its own buffer for the step's layout, run the
         # step eagerly on it, then capture
         packed = self._pack(entries, requests, want_slots=sample, fixed=True)

@@ -945,14 +945,19 @@ class CudaOps:
                 rows, N, K, count, rank, int(out_dtype == torch.float32), self._error_word(x.device).data_ptr(), _raw_stream()),
                 "linear_adapters (tcgen05)")
             return out
-        # bfloat16 products that let the next kernel in after their own wait have the small sums taken beside them
-        beside = (self.use_tensor_cores and x.dtype == torch.bfloat16 and K % 8 == 0 and not weight.data_ptr() % 16
-                  and (rows <= 8 or not self._skinny_fits(x, weight)))
-        if not beside:
-            down(False)
-        base = self.linear(x, weight, bias, out_dtype=torch.float32)
-        if beside:
+        # The two bfloat16 products that let the next kernel in after their own wait have the small sums taken beside them.
+        base = None
+        if self.use_tensor_cores and x.dtype == torch.bfloat16 and K % 8 == 0 and not weight.data_ptr() % 16:
+            few = self._skinny_fits(x, weight)
+            if few and rows <= 8:
+                base = self._linear_skinny(x, weight, bias, torch.float32, swiglu=False)
+            elif not few:
+                base = self._linear_tcgen05(x, weight, bias, torch.float32)
+        if base is not None:
             down(True)
+        else:
+            down(False)
+            base = self.linear(x, weight, bias, out_dtype=torch.float32)
         out = base if out_dtype == torch.float32 else x.new_empty((rows, N), dtype=out_dtype)
         _check(library.mlr_adapter_up(low.data_ptr(), adapters.up.data_ptr(), row_adapter.data_ptr(), base.data_ptr(), out.data_ptr(),
                                       rows, count, rank, N, _code(x.dtype), _code(out_dtype), _raw_stream()), "linear_adapters (up)")
@@ -2574,7 +2579,7 @@ class CudaOps:
         return out
 
     def shape_logits(self, logits: torch.Tensor, row_slot: torch.Tensor, tables: LogitTables) -> torch.Tensor:
-        """The rules of each row's request on its logits, float32 [rows, vocab]; ``row_slot`` int32 [rows] names the slot whose
+        """The rules of each row's request on its logits, float32 [rows, vocab] on a 16-byte boundary; ``row_slot`` int32 [rows] names the slot whose
         row of the tables holds (a row of no slot passes unchanged).  A token of the history: x / repetition where x > 0, else
         x * repetition; then less frequency times how often it was generated, less presence if it was; then its bias; tokens
         that are not allowed get -inf.  A row that allows nothing is -inf throughout (greedy sampling then takes token 0)."""

@@ -190,3 +190,30 @@ def test_a_stack_of_more_than_32_bit_offsets():
     got = run(case, ids)
     small = {**case, "down": down[count - 1:], "up": case["up"][count - 1:], "scales": case["scales"][count - 1:]}
     check(got, small, torch.tensor([0, -1], device=DEVICE), torch.bfloat16)
+
+
+@pytest.mark.parametrize("rows", [1, 20, 200])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_weight_on_no_16_byte_boundary(dtype, rows):
+    case = made(rows, 256, 264, 16, 4, dtype, 13)
+    buffer = torch.empty(264 * 256 + 1, dtype=dtype, device=DEVICE)
+    buffer[1:] = case["weight"].flatten()
+    case["weight"] = buffer[1:].view(264, 256)
+    ids = some_ids(rows, 4, "mixed", 2)
+    check(run(case, ids), case, ids, dtype)
+
+
+def test_x_on_no_16_byte_boundary_is_refused():
+    case = made(3, 64, 40, 8, 2, torch.bfloat16, 14)
+    case["x"] = torch.zeros(3 * 64 + 1, dtype=torch.bfloat16, device=DEVICE)[1:].view(3, 64)
+    with pytest.raises(ops.KernelError, match="boundary"):
+        run(case, some_ids(3, 2, "one", 1))
+
+
+def test_without_the_tensor_cores(monkeypatch):
+    """The switch that keeps products on the CUDA cores."""
+    monkeypatch.setattr(ops.current(), "use_tensor_cores", False)
+    for rows in (5, 40, 200):
+        case = made(rows, 256, 264, 16, 4, torch.bfloat16, 15)
+        ids = some_ids(rows, 4, "mixed", 2)
+        check(run(case, ids), case, ids, torch.bfloat16)

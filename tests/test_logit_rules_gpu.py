@@ -254,3 +254,10 @@ def test_history_words_beyond_32_bit_offsets():
     want[0, vocab - 1] = 0.5 - 0.5 - 0.5
     assert torch.equal(got.cpu(), want)
     assert int(device.counts.sum()) == 2
+
+
+def test_logits_on_no_16_byte_boundary_are_refused():
+    tables = on_device(made(31, 2, 3))
+    logits = torch.zeros((2, 31), device=DEVICE)[1:]
+    with pytest.raises(ops.KernelError, match="aligned"):
+        ops.current().shape_logits(logits, torch.zeros(1, dtype=torch.int32, device=DEVICE), tables)

@@ -63,6 +63,30 @@ def test_decode_steps_behind_shared_prefixes(name, graphs, shared_calls):
     cache.check_consistency()
 
 
+def test_captured_steps_of_many_group_sizes_are_bounded(shared_calls):
+    config, page = CONFIGS["E"]
+    tiny = TinyEngine(config, page, torch.bfloat16, "cuda:0", num_pages=80, max_requests=9)
+    tiny.runner.graph_max_shared = 2
+    cache, runner = tiny.cache, tiny.runner
+    prefix = random_prompt(config.vocab_size, 2 * page, 1)
+    cache.create_request("p")
+    runner.step([StepEntry("p", prefix)])
+    texts = {f"r{i}": prefix + [i + 1] for i in range(6)}
+    for name, text in texts.items():
+        cache.create_request(name, prefix=("p", 2 * page))
+        runner.step([StepEntry(name, text[2 * page:])])
+    for turn, count in enumerate((2, 3, 4, 2, 5, 2, 3, 6, 2)):
+        for _ in range(2):
+            batch = list(texts)[:count]
+            for name in batch:
+                texts[name].append(7 * turn + 1)
+            logits = runner.step([StepEntry(name, texts[name][-1:], [0]) for name in batch])
+            for row, name in enumerate(batch):
+                assert_close(logits[row][None], tiny.plain_logits(texts[name])[-1][None], torch.bfloat16, f"{turn} {name}")
+        assert sum(len(key) > 4 for key in runner._graphs) <= 2
+    assert runner.graph_replays > 0
+
+
 def engine_of(tiny, page, **options):
     engine = ContinuousBatchEngine.from_model(tiny.model, block_size=page, max_running_requests=4, max_batch_tokens=64, max_model_len=384, **options)
     engine.runner.graph_capture_after = 1
