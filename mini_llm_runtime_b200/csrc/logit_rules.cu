@@ -215,18 +215,18 @@ using namespace mlr;
 
 MLR_DEFINE_PDL_SWITCH
 
-// logits, out: float32 [rows, vocab] on 16-byte boundaries, the same memory or apart.  row_slot: int32 [rows].
-MLR_EXPORT int mlr_logit_rules(const float* logits, float* out, const int* row_slot, int rows, int vocab, int slots,
-                               const float* penalties, const int* counts, const void* seen, const int* bias_tokens,
-                               const float* bias_values, int biases, const void* allowed, cudaStream_t stream) {
-  if (rows < 0 || vocab <= 0 || vocab > (1 << 30) || slots <= 0 || biases < 0) return MLR_BAD_SIZE;
+// logits, out: float32 [rows, vocab] on 16-byte boundaries, the same memory or apart.  row_slot: int32 [rows].  `tables` is read on
+// the host.
+MLR_EXPORT int mlr_logit_rules(const float* logits, float* out, const int* row_slot, int rows, int vocab, const RuleTables* tables,
+                               cudaStream_t stream) {
+  if (tables == nullptr || rows < 0 || vocab <= 0 || vocab > (1 << 30) || tables->slots <= 0 || tables->biases < 0) return MLR_BAD_SIZE;
   if (rows == 0) return MLR_OK;
   if (rows > 65535) return MLR_TOO_LARGE;
   if (((uintptr_t)logits & 15) != 0 || ((uintptr_t)out & 15) != 0) return MLR_BAD_ALIGNMENT;
-  if ((penalties != nullptr) != (counts != nullptr) || (penalties != nullptr) != (seen != nullptr)) return MLR_BAD_SIZE;
-  RuleTables tables{penalties, counts, (const unsigned*)seen, biases > 0 ? bias_tokens : nullptr, bias_values,
-                    (const unsigned*)allowed, biases, slots};
-  launch_rules(logits, out, row_slot, rows, vocab, tables, stream);
+  RuleTables t = *tables;
+  if ((t.penalties != nullptr) != (t.counts != nullptr) || (t.penalties != nullptr) != (t.seen != nullptr)) return MLR_BAD_SIZE;
+  if (t.biases == 0) t.bias_tokens = nullptr;
+  launch_rules(logits, out, row_slot, rows, vocab, t, stream);
   return launch_status();
 }
 

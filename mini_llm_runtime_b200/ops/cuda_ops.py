@@ -98,6 +98,8 @@ def _stream() -> ctypes.c_void_p:
 # for twice, one step of 64 rows 3,120 -> 2,840 us, of 1,000 rows 3,380 -> 3,020.
 _PROTOTYPES = {
     "gemm_tcgen05": {"mlr_gemm_tcgen05": "ppppiiiiiffplpipp"},
+    "attention_mma": {"mlr_attention_decode_tma": "ppppppppp" "iiiiiiii" "f" "iiii" "pppppp" "iip"},
+    "linear_split": {"mlr_linear_split": "ppppiiiippp", "mlr_linear_split_rows": "ii"},
     "gemm_skinny": {"mlr_gemm_skinny": "pppppiiiiifp"},
     "elementwise": {"mlr_rms_norm": "ppppiifiip", "mlr_rope_kv_write": "pppppppiiiiiiip"},
     "attention_tcgen05": {"mlr_attention_prefill_tcgen05": "ppppppppppp" "iiiiiiiii" "fi" "ppp" "l" "pip"},
@@ -107,7 +109,7 @@ _PROTOTYPES = {
     "adapters": {"mlr_adapter_down": "pppppiiiiiip", "mlr_adapter_up": "pppppiiiiiip"},
     "adapters_small": {"mlr_adapter_small": "pppppppp" "iiiiiii" "p"},
     "adapters_tcgen05": {"mlr_adapter_gemm": "ppppppp" "iiiiii" "pp"},
-    "logit_rules": {"mlr_logit_rules": "pppiii" "pppppip" "p", "mlr_count_tokens": "ppippiiip"},
+    "logit_rules": {"mlr_logit_rules": "pppiipp", "mlr_count_tokens": "ppippiiip"},
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 _declared: dict[str, ctypes.CDLL] = {}
@@ -156,6 +158,13 @@ class AttentionBatch:
     @property
     def num_decode(self) -> int:
         return self.counts.get("decode", 0)
+
+
+class _RuleTables(ctypes.Structure):
+    """``struct RuleTables`` of csrc/logit_rules.cu."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in ("penalties", "counts", "seen", "bias_tokens", "bias_values", "allowed")] + [
+        ("biases", ctypes.c_int), ("slots", ctypes.c_int)]
 
 
 @dataclass(frozen=True)
@@ -208,13 +217,14 @@ class LogitTables:
         if not slots:
             raise KernelError("the tables hold no rule, or no slot")
         _need_together(self.penalties, self.counts, self.seen, self.bias_tokens, self.bias_values, self.allowed)
-        object.__setattr__(self, "slots", slots)
-        object.__setattr__(self, "vocab", vocab)       # None where only biases or bits say something
-        object.__setattr__(self, "words", words)
-
-    @property
-    def device(self) -> torch.device:
-        return next(t for t in (self.penalties, self.bias_tokens, self.allowed) if t is not None).device
+        first = next(t for t in (self.penalties, self.bias_tokens, self.allowed) if t is not None)
+        # vocab, words: None where only biases or bits say something.  rules: what the kernel takes, addresses of tensors held here
+        for name, value in (("slots", slots), ("vocab", vocab), ("words", words), ("device", first.device),
+                            ("rules", _RuleTables(_address(self.penalties), _address(self.counts), _address(self.seen),
+                                                  _address(self.bias_tokens), _address(self.bias_values), _address(self.allowed),
+                                                  0 if self.bias_tokens is None else self.bias_tokens.shape[1], slots))):
+            object.__setattr__(self, name, value)
+        object.__setattr__(self, "rules_at", ctypes.addressof(self.rules))
 
 
 @dataclass(frozen=True)
@@ -371,7 +381,8 @@ def plan_shared_prefix(groups, num_segments: int, heads_per_kv: int) -> tuple[di
     arrays = {"seg_keys": seg_keys, **{name: np.asarray(values, dtype=np.int32) for name, values in (
         ("members", members), ("tile_first", first), ("tile_count", count), ("tile_keys", keys_of))}}
     return arrays, {"segments": int(num_segments), "heads_per_kv": int(heads_per_kv), "members": len(members),
-                    "tiles": len(first), "tile_keys": tuple(keys_of), "saved_keys": saved, "least_shared": int(seg_keys.min()) if num_segments else 0}
+                    "tiles": len(first), "tile_keys": tuple(keys_of), "saved_keys": saved, "longest": max(keys_of, default=0),
+                    "least_shared": int(seg_keys.min()) if num_segments else 0}
 
 
 PREFIX_SCRATCH_BYTES = 256 << 20      # states of the parts of one call, at most
@@ -858,12 +869,12 @@ class CudaOps:
     def _linear_split(self, x, weight, bias, gated=False):
         M, K = x.shape
         N = weight.shape[0]
-        lib = build.load_library("linear_split")
-        out = torch.empty((M, N // 2 if gated else N), dtype=torch.float32, device=x.device)
+        lib = _declared_library("linear_split")
+        out = x.new_empty((M, N // 2 if gated else N))
         rows = lib.mlr_linear_split_rows(M, K)
         parts = torch.empty((3, rows, -(-K // 8) * 8), dtype=torch.bfloat16, device=x.device) if rows else None
-        _check(lib.mlr_linear_split(_ptr(x), _ptr(weight), _ptr(bias), _ptr(out), M, N, K, int(gated), _ptr(parts),
-                                    _ptr(self._error_word(x.device)), _stream()), "linear (32-bit operands in parts)")
+        _check(lib.mlr_linear_split(x.data_ptr(), weight.data_ptr(), _address(bias), out.data_ptr(), M, N, K, int(gated), _address(parts),
+                                    self._error_word(x.device).data_ptr(), _raw_stream()), "linear (32-bit operands in parts)")
         return out
 
     def _linear_simt(self, x, weight, bias, out_dtype):
@@ -1094,33 +1105,34 @@ class CudaOps:
         row of the block table names the shared pages as its first); ``prefix`` says which segments share how many keys.
         Segments of no group attend by themselves.  Where sharing saves too little for it (``SHARED_PREFIX_LEAST``) the step goes
         through ``paged_attention``."""
-        _need(q, "q", dims=2)
-        _need(k_pool, "k_pool", q.dtype, 4)
-        _need(v_pool, "v_pool", q.dtype, 4)
+        segments, counts, plan = batch.num_segments, prefix.counts, prefix.plan
         if num_kv_heads < 1 or num_heads < 1 or num_heads % num_kv_heads or not 1 <= head_dim <= 256:
             raise KernelError(f"{num_heads} heads over {num_kv_heads} kv heads of {head_dim} are not supported")
+        if counts["segments"] != segments or counts["heads_per_kv"] != num_heads // num_kv_heads:
+            raise KernelError(f"the prefix was planned for {counts['segments']} segments and {counts['heads_per_kv']} heads per kv head")
+        if counts["longest"] > batch.max_kv_len:
+            raise KernelError(f"a prefix of {counts['longest']} keys in contexts of at most {batch.max_kv_len}")
+        _need(q, "q", dims=2)
+        if batch.num_decode != segments or q.shape[0] != segments:
+            raise KernelError("shared_prefix_attention takes steps of one decoded token per request")
+        _need(batch.block_table, "block_table", torch.int32, 2)
+        _need_here(q=q, k_pool=k_pool, v_pool=v_pool, prefix=prefix, block_table=batch.block_table)
+        page_size = k_pool.shape[2] if k_pool.dim() == 4 else 0
+        fast = (self.use_mma_attention and q.dtype == torch.bfloat16 and head_dim in (64, 128) and num_heads // num_kv_heads <= 16
+                and page_size >= 8 and page_size & (page_size - 1) == 0)
+        if fast and segments > 0 and not self.shares_prefix(q.dtype, counts, num_kv_heads, head_dim):
+            return self.paged_attention(q, k_pool, v_pool, batch, num_heads, num_kv_heads, head_dim, scale, None)
+        _need(k_pool, "k_pool", q.dtype, 4)
+        _need(v_pool, "v_pool", q.dtype, 4)
         if q.shape[1] != num_heads * head_dim:
             raise KernelError(f"q rows have {q.shape[1]} entries, expected {num_heads * head_dim}")
         if k_pool.shape != v_pool.shape or k_pool.shape[1] != num_kv_heads or k_pool.shape[3] != head_dim:
             raise KernelError(f"page pools have shapes {tuple(k_pool.shape)} and {tuple(v_pool.shape)}, expected "
                               f"[pages, {num_kv_heads}, page_size, {head_dim}]")
-        segments, counts, plan = batch.num_segments, prefix.counts, prefix.plan
-        if batch.num_decode != segments or q.shape[0] != segments:
-            raise KernelError("shared_prefix_attention takes steps of one decoded token per request")
-        if counts["segments"] != segments or counts["heads_per_kv"] != num_heads // num_kv_heads:
-            raise KernelError(f"the prefix was planned for {counts['segments']} segments and {counts['heads_per_kv']} heads per kv head")
-        if counts["tile_keys"] and max(counts["tile_keys"]) > batch.max_kv_len:
-            raise KernelError(f"a prefix of {max(counts['tile_keys'])} keys in contexts of at most {batch.max_kv_len}")
-        _need(batch.block_table, "block_table", torch.int32, 2)
-        _need_here(q=q, k_pool=k_pool, v_pool=v_pool, prefix=prefix, block_table=batch.block_table)
-        page_size = k_pool.shape[2]
-        fast = (self.use_mma_attention and q.dtype == torch.bfloat16 and head_dim in (64, 128) and num_heads // num_kv_heads <= 16
-                and page_size >= 8 and page_size & (page_size - 1) == 0 and k_pool.shape[0] * num_kv_heads * page_size < 1 << 31
-                and not (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr()) % 16)
         if segments == 0:
             return torch.empty_like(q)
-        if fast and not self.shares_prefix(q.dtype, counts, num_kv_heads, head_dim):
-            return self.paged_attention(q, k_pool, v_pool, batch, num_heads, num_kv_heads, head_dim, scale, None)
+        fast = (fast and k_pool.shape[0] * num_kv_heads * page_size < 1 << 31
+                and not (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr()) % 16)
         out = torch.empty_like(q)
         chunk, parts, units, own_parts = prefix_parts(counts["tile_keys"], counts["least_shared"], segments, batch.max_kv_len, num_heads,
                                                       num_kv_heads, head_dim, self.sm_count(q.device))
@@ -1196,19 +1208,19 @@ class CudaOps:
         decode_seg = batch.plan["decode_seg"]
         if tma:
             # pages arrive by the tensor memory accelerator, one bulk copy per page and kv head
-            entry = build.load_library("attention_mma").mlr_attention_decode_tma
+            entry = _declared_library("attention_mma").mlr_attention_decode_tma
 
             # every segment one decoded row: segment and row are the index itself, the kernel skips the list
             listed = None if batch.num_decode == batch.num_segments else decode_seg
 
             def launch(clustered: bool) -> int:
                 return entry(
-                    _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(out), _ptr(listed), _ptr(batch.seg_q_start),
-                    _ptr(batch.seg_pos0), _ptr(batch.block_table), _ptr(batch.seg_slot), batch.block_table.shape[1],
+                    _address(q), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), _address(listed), batch.seg_q_start.data_ptr(),
+                    batch.seg_pos0.data_ptr(), batch.block_table.data_ptr(), batch.seg_slot.data_ptr(), batch.block_table.shape[1],
                     batch.num_decode, num_heads, num_kv_heads, head_dim, page_size, k_pool.shape[0], int(window or 0),
-                    ctypes.c_float(scale), chunk, int(even_split), splits, stages,
-                    _ptr(space["attention_scratch"]), _ptr(space["attention_counters"]), _ptr(space["error_word"]),
-                    _ptr(qkv), _ptr(inv_freq), _ptr(slots), int(bool(write_kv)), int(clustered), _stream())
+                    scale, chunk, int(even_split), splits, stages,
+                    space["attention_scratch"].data_ptr(), space["attention_counters"].data_ptr(), space["error_word"].data_ptr(),
+                    _address(qkv), _address(inv_freq), _address(slots), int(bool(write_kv)), int(clustered), _raw_stream())
 
             clustered = cluster == splits and cluster >= 2
             # head_dim 64: a warp that walks more than two 64-key tiles does better with 32-key tiles
@@ -2572,10 +2584,7 @@ class CudaOps:
         if rows == 0:
             return out
         _check(_declared_library("logit_rules").mlr_logit_rules(
-            logits.data_ptr(), out.data_ptr(), row_slot.data_ptr(), rows, vocab, tables.slots,
-            _address(tables.penalties), _address(tables.counts), _address(tables.seen), _address(tables.bias_tokens),
-            _address(tables.bias_values), 0 if tables.bias_tokens is None else tables.bias_tokens.shape[1],
-            _address(tables.allowed), _raw_stream()), "shape_logits")
+            logits.data_ptr(), out.data_ptr(), row_slot.data_ptr(), rows, vocab, tables.rules_at, _raw_stream()), "shape_logits")
         return out
 
     def shape_logits(self, logits: torch.Tensor, row_slot: torch.Tensor, tables: LogitTables) -> torch.Tensor:
