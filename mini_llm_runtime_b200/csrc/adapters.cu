@@ -356,6 +356,12 @@ using namespace mlr;
 
 MLR_DEFINE_PDL_SWITCH
 
+// The entry points of the shared product, of the libraries they live in.
+typedef int (*SkinnyProduct)(const void*, const void*, const void*, void*, const void*, int, int, int, int, int, float, cudaStream_t);
+typedef int (*TensorProduct)(const void*, const void*, const void*, void*, int, int, int, int, int, float, float, void*, long long, int*, int, int*,
+                             cudaStream_t);
+typedef int (*SplitProduct)(const float*, const float*, const float*, float*, int, int, int, int, void*, int*, cudaStream_t);
+
 // x [rows, K], down [adapters, rank, K] of one dtype on 16-byte boundaries; u float32 [rows, rank].  Rows without an adapter are
 // not written.  early: the kernel in front on the stream is the product of the same x, and lets the next one in after its own wait.
 MLR_EXPORT int mlr_adapter_down(const void* x, const void* down, const float* scales, const int* row_adapter, float* u, int rows,
@@ -382,4 +388,29 @@ MLR_EXPORT int mlr_adapter_up(const float* u, const void* up, const int* row_ada
   if (dtype == MLR_F32 && out_dtype == MLR_F32)
     return launch_up<float, float>(u, up, row_adapter, base, out, rows, adapters, rank, N, stream);
   return MLR_BAD_DTYPE;
+}
+
+// The three in one call from the host, whose own steps per launch cost more than few rows' products: small sums, shared product into
+// `base` (float32 [rows, N]), adapters' share into `out`.  route: 1 mlr_gemm_skinny, 2 mlr_gemm_tcgen05 (with its scratch and
+// counters), 3 mlr_linear_split (with its scratch); `product` is that entry point.  The products that let the next kernel in
+// after their own wait (2, and 1 of up to eight rows) come first, with the sums beside them.  A status other than MLR_OK of the
+// product is handed on: nothing but it and the sums was launched then.
+MLR_EXPORT int mlr_linear_adapters(const void* x, const void* weight, const void* bias, const void* down, const void* up, const float* scales,
+                                   const int* row_adapter, float* low, float* base, void* out, int rows, int N, int K, int adapters, int rank,
+                                   int dtype, int out_dtype, int route, void* product, void* scratch, long long scratch_bytes, int* counters,
+                                   int counters_len, int* error_word, cudaStream_t stream) {
+  if (product == nullptr || route < 1 || route > 3) return MLR_BAD_SIZE;
+  const bool early = route == 2 || (route == 1 && rows <= 8);
+  int status = MLR_OK;
+  if (!early) status = mlr_adapter_down(x, down, scales, row_adapter, low, rows, adapters, rank, K, dtype, 0, stream);
+  if (status != MLR_OK) return status;
+  if (route == 1) status = ((SkinnyProduct)product)(x, weight, bias, base, nullptr, rows, N, K, 1, 0, -1.f, stream);
+  else if (route == 2)
+    status = ((TensorProduct)product)(x, weight, bias, base, rows, N, K, 1, 0, 0.f, 0.f, scratch, scratch_bytes, counters, counters_len, error_word, stream);
+  else
+    status = ((SplitProduct)product)((const float*)x, (const float*)weight, (const float*)bias, base, rows, N, K, 0, scratch, error_word, stream);
+  if (status != MLR_OK) return status;
+  if (early) status = mlr_adapter_down(x, down, scales, row_adapter, low, rows, adapters, rank, K, dtype, 1, stream);
+  if (status != MLR_OK) return status;
+  return mlr_adapter_up(low, up, row_adapter, base, out, rows, adapters, rank, N, dtype, out_dtype, stream);
 }

@@ -106,7 +106,8 @@ _PROTOTYPES = {
     "attention_sigmoid_tcgen05": {"mlr_attention_sigmoid_tcgen05": "ppppp" "ppppppp" "iiiiiiii" "f" "pppp" "iii" "pp",
                                   "mlr_attention_sigmoid_tcgen05_scratch": "iiiii"},
     "attention_prefix": {"mlr_attention_prefix": "pppppppp" "ppppp" "pp" "iiiiiiiiiiii" "fiipp"},
-    "adapters": {"mlr_adapter_down": "pppppiiiiiip", "mlr_adapter_up": "pppppiiiiiip"},
+    "adapters": {"mlr_adapter_down": "pppppiiiiiip", "mlr_adapter_up": "pppppiiiiiip",
+                 "mlr_linear_adapters": "pppppppppp" "iiiiiiii" "pp" "l" "pip" "p"},
     "adapters_small": {"mlr_adapter_small": "pppppppp" "iiiiiii" "p"},
     "adapters_tcgen05": {"mlr_adapter_gemm": "ppppppp" "iiiiii" "pp"},
     "logit_rules": {"mlr_logit_rules": "pppiipp", "mlr_count_tokens": "ppippiiip"},
@@ -123,6 +124,17 @@ def _declared_library(name: str) -> ctypes.CDLL:
             getattr(library, symbol).argtypes = [_CTYPES[code] for code in codes]
         _declared[name] = library
     return library
+
+
+_entries: dict[str, int] = {}
+
+
+def _entry(library: str, symbol: str) -> int:
+    """The address of an entry point, for one that calls it."""
+    at = _entries.get(symbol)
+    if at is None:
+        at = _entries[symbol] = ctypes.cast(getattr(_declared_library(library), symbol), ctypes.c_void_p).value
+    return at
 
 
 def _address(tensor: torch.Tensor | None) -> int | None:
@@ -939,38 +951,55 @@ class CudaOps:
                 row_adapter.data_ptr(), out.data_ptr(), rows, N, K, count, rank, _code(x.dtype), _code(out_dtype), _raw_stream()),
                 "linear_adapters (small)")
             return out
-        low = x.new_empty((rows, rank), dtype=torch.float32)
+        aligned = not weight.data_ptr() % 16
         library = _declared_library("adapters")
-
-        def down(early: bool) -> None:
-            _check(library.mlr_adapter_down(x.data_ptr(), adapters.down.data_ptr(), adapters.scales.data_ptr(), row_adapter.data_ptr(),
-                                            low.data_ptr(), rows, count, rank, K, _code(x.dtype), int(early), _raw_stream()),
-                   "linear_adapters (down)")
-
         if (self.use_tensor_cores and x.dtype == torch.bfloat16 and rows > self.ADAPTER_ROWS and K % 8 == 0 and rank % 8 == 0
-                and not weight.data_ptr() % 16 and count * N < 1 << 31):
-            down(False)
+                and aligned and count * N < 1 << 31):
+            low = x.new_empty((rows, rank), dtype=torch.float32)
             out = x.new_empty((rows, N), dtype=out_dtype)
+            _check(library.mlr_adapter_down(x.data_ptr(), adapters.down.data_ptr(), adapters.scales.data_ptr(), row_adapter.data_ptr(),
+                                            low.data_ptr(), rows, count, rank, K, _code(x.dtype), 0, _raw_stream()), "linear_adapters (down)")
             _check(_declared_library("adapters_tcgen05").mlr_adapter_gemm(
                 x.data_ptr(), weight.data_ptr(), adapters.up.data_ptr(), low.data_ptr(), row_adapter.data_ptr(), _address(bias), out.data_ptr(),
                 rows, N, K, count, rank, int(out_dtype == torch.float32), self._error_word(x.device).data_ptr(), _raw_stream()),
                 "linear_adapters (tcgen05)")
             return out
-        # The two bfloat16 products that let the next kernel in after their own wait have the small sums taken beside them.
-        base = None
-        if self.use_tensor_cores and x.dtype == torch.bfloat16 and K % 8 == 0 and not weight.data_ptr() % 16:
-            few = self._skinny_fits(x, weight)
-            if few and rows <= 8:
-                base = self._linear_skinny(x, weight, bias, torch.float32, swiglu=False)
-            elif not few:
-                base = self._linear_tcgen05(x, weight, bias, torch.float32)
-        if base is not None:
-            down(True)
+        # The shared product's sums in 32 bits behind the small sums, in one piece of memory (the result itself where it is in 32 bits).
+        head = -(-rows * rank // 4) * 4
+        if out_dtype == torch.float32:
+            low, out = x.new_empty(head, dtype=torch.float32), x.new_empty((rows, N), dtype=torch.float32)
+            low_at, base_at = low.data_ptr(), out.data_ptr()
         else:
-            down(False)
-            base = self.linear(x, weight, bias, out_dtype=torch.float32)
-        out = base if out_dtype == torch.float32 else x.new_empty((rows, N), dtype=out_dtype)
-        _check(library.mlr_adapter_up(low.data_ptr(), adapters.up.data_ptr(), row_adapter.data_ptr(), base.data_ptr(), out.data_ptr(),
+            low, out = x.new_empty(head + rows * N, dtype=torch.float32), x.new_empty((rows, N), dtype=out_dtype)
+            low_at = low.data_ptr()
+            base_at = low_at + 4 * head
+        route, product, space, scratch, counters = 0, None, self._workspace(x.device), None, None
+        scratch_bytes = counters_len = 0
+        if self.use_tensor_cores and aligned:
+            if x.dtype == torch.bfloat16 and K % 8 == 0:
+                if self._skinny_fits(x, weight):
+                    route, product = 1, _entry("gemm_skinny", "mlr_gemm_skinny")
+                else:
+                    route, product, scratch, counters = 2, _entry("gemm_tcgen05", "mlr_gemm_tcgen05"), space["gemm_scratch"], space["gemm_counters"]
+                    scratch_bytes, counters_len = scratch.numel(), counters.numel()
+            elif x.dtype == torch.float32 and self._split_fits(x, weight):
+                route, product = 3, _entry("linear_split", "mlr_linear_split")
+                parts = _declared_library("linear_split").mlr_linear_split_rows(rows, K)
+                scratch = torch.empty((3, parts, -(-K // 8) * 8), dtype=torch.bfloat16, device=x.device) if parts else None
+        if route:
+            status = library.mlr_linear_adapters(
+                x.data_ptr(), weight.data_ptr(), _address(bias), adapters.down.data_ptr(), adapters.up.data_ptr(), adapters.scales.data_ptr(),
+                row_adapter.data_ptr(), low_at, base_at, out.data_ptr(), rows, N, K, count, rank, _code(x.dtype), _code(out_dtype), route,
+                product, _address(scratch), scratch_bytes, _address(counters), counters_len, space["error_word"].data_ptr(), _raw_stream())
+            if status != _NO_ROOM:      # the product's partial tiles do not fit its scratch memory: by the general way
+                global launches
+                _check(status, "linear_adapters")
+                launches += 2
+                return out
+        _check(library.mlr_adapter_down(x.data_ptr(), adapters.down.data_ptr(), adapters.scales.data_ptr(), row_adapter.data_ptr(), low_at,
+                                        rows, count, rank, K, _code(x.dtype), 0, _raw_stream()), "linear_adapters (down)")
+        base = self.linear(x, weight, bias, out_dtype=torch.float32)
+        _check(library.mlr_adapter_up(low_at, adapters.up.data_ptr(), row_adapter.data_ptr(), base.data_ptr(), out.data_ptr(),
                                       rows, count, rank, N, _code(x.dtype), _code(out_dtype), _raw_stream()), "linear_adapters (up)")
         return out
 
