@@ -20,7 +20,6 @@ constexpr int MOST_PARTS = 8;        // of K: CTAs of a cluster
 // as tiles 49; one adapter for 2,048 rows of 64 ranks as tiles 23.)
 constexpr int DOWN_ROWS = 128;
 constexpr int TILE_DOWN = 32;        // rows per CTA of the many-rows kernel
-constexpr int TILE_RANKS = 64;       // rank rows it takes at a time
 
 __device__ __forceinline__ uint32_t rank_in_cluster() {
   uint32_t rank;
@@ -130,16 +129,18 @@ adapter_down_rows_kernel(const T* x, const T* __restrict__ down, const float* __
   if (early) pdl_wait();
 }
 
-// Many rows, prompts as a rule: a CTA takes 32 rows, a part of K and up to 64 rank rows of one adapter after another (those that
+// Many rows, prompts as a rule: a CTA takes 32 rows, a part of K and up to 8 NT rank rows of one adapter after another (those that
 // its rows have; TILE_SPLIT CTAs take turns at them), on mma.sync.  Both operands are read straight from global memory, 16
 // bytes of a row per lane: the four lanes that share a row hold 32 columns, and since both operands are dealt out alike, which
 // of them an MMA calls column 0 does not matter.  The warps' and the parts' sums meet in shared memory, in order.
-constexpr int TILE_WARPS = 8, TILE_SPLIT = 4, TILE_PITCH = TILE_RANKS + 4;
-constexpr int TILE_SHARED = (TILE_WARPS + 1) * TILE_DOWN * TILE_PITCH * 4;
+constexpr int TILE_WARPS = 8, TILE_SPLIT = 8;
+template <int NT> constexpr int TILE_SHARED = (TILE_WARPS + 1) * TILE_DOWN * (8 * NT + 4) * 4;
 
+template <int NT>
 __global__ void __launch_bounds__(TILE_WARPS * 32)
 adapter_down_tile_kernel(const bf16* x, const bf16* __restrict__ down, const float* __restrict__ scales, const int* row_adapter, float* u,
                          int rows, int adapters, int rank, int K, int parts, int early) {
+  constexpr int TILE_RANKS = 8 * NT, TILE_PITCH = TILE_RANKS + 4;
   extern __shared__ float tile_shared[];
   float* sums = tile_shared;                                               // [warps][32][pitch]
   float* total = tile_shared + TILE_WARPS * TILE_DOWN * TILE_PITCH;        // [32][pitch]
@@ -170,16 +171,16 @@ adapter_down_tile_kernel(const bf16* x, const bf16* __restrict__ down, const flo
     const int adapter = ids[__ffs(leaders) - 1];
     leaders &= leaders - 1u;
     if (turn % TILE_SPLIT != (int)blockIdx.z) continue;
-    float acc[2][8][4];
+    float acc[2][NT][4];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int n = 0; n < 8; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
+      for (int n = 0; n < NT; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
     const uint4* ar = reinterpret_cast<const uint4*>(down + ((size_t)adapter * rank + r0) * K);
     for (int k = begin; k < end; ++k) {
       const int piece = k * 4 + t;
       const bool there = piece < pieces;
-      uint4 a[4], b[8];
+      uint4 a[4], b[NT];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         // rows of another adapter count as zeros (whatever they hold stays out of the sums that are kept anyway)
@@ -187,11 +188,11 @@ adapter_down_tile_kernel(const bf16* x, const bf16* __restrict__ down, const flo
         a[i] = there && ids[row] == adapter ? __ldcg(xr + (size_t)row * pieces + piece) : zero;
       }
 #pragma unroll
-      for (int n = 0; n < 8; ++n) b[n] = there && n * 8 + g < ranks ? __ldg(ar + (size_t)(n * 8 + g) * pieces + piece) : zero;
+      for (int n = 0; n < NT; ++n) b[n] = there && n * 8 + g < ranks ? __ldg(ar + (size_t)(n * 8 + g) * pieces + piece) : zero;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
+        for (int n = 0; n < NT; ++n) {
           const uint32_t low[4] = {a[2 * i].x, a[2 * i + 1].x, a[2 * i].y, a[2 * i + 1].y};
           mma_bf16(acc[i][n], low, b[n].x, b[n].y);
           const uint32_t high[4] = {a[2 * i].z, a[2 * i + 1].z, a[2 * i].w, a[2 * i + 1].w};
@@ -201,7 +202,7 @@ adapter_down_tile_kernel(const bf16* x, const bf16* __restrict__ down, const flo
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int n = 0; n < 8; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; e += 2)
           *reinterpret_cast<float2*>(sums + (warp * TILE_DOWN + i * 16 + g + e * 4) * TILE_PITCH + n * 8 + t * 2) =
@@ -302,16 +303,17 @@ adapter_up_kernel(const float* u, const T* __restrict__ up, const int* row_adapt
     if (row0 + r < rows) out[(size_t)(row0 + r) * N + n] = from_float<Out>(acc[r]);
 }
 
+template <int NT>
 static int launch_down_tile(const void* x, const void* down, const float* scales, const int* row_adapter, float* u, int rows, int adapters,
                             int rank, int K, int early, cudaStream_t stream) {
-  const int tiles = (rows + TILE_DOWN - 1) / TILE_DOWN, groups = (rank + TILE_RANKS - 1) / TILE_RANKS;
+  const int tiles = (rows + TILE_DOWN - 1) / TILE_DOWN, groups = (rank + 8 * NT - 1) / (8 * NT);
   int parts = 1;      // of K: one CTA per SM
   while (parts < MOST_PARTS && 2 * tiles * groups * parts <= sm_count() && K >= 4 * parts * TILE_WARPS * 32) parts *= 2;
   static OncePerDevice once;
-  if (cudaError_t err = once([] { return cudaFuncSetAttribute(adapter_down_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_SHARED); }))
+  if (cudaError_t err = once([] { return cudaFuncSetAttribute(adapter_down_tile_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_SHARED<NT>); }))
     return (int)err;
-  launch_kernel_clustered(adapter_down_tile_kernel, dim3(tiles * parts, groups, TILE_SPLIT), dim3(TILE_WARPS * 32), TILE_SHARED, stream, parts,
-                          (const bf16*)x, (const bf16*)down, scales, row_adapter, u, rows, adapters, rank, K, parts, early);
+  launch_kernel_clustered(adapter_down_tile_kernel<NT>, dim3(tiles * parts, groups, TILE_SPLIT), dim3(TILE_WARPS * 32), TILE_SHARED<NT>, stream,
+                          parts, (const bf16*)x, (const bf16*)down, scales, row_adapter, u, rows, adapters, rank, K, parts, early);
   return launch_status();
 }
 
@@ -369,7 +371,11 @@ MLR_EXPORT int mlr_adapter_down(const void* x, const void* down, const float* sc
   if (rows < 0 || adapters <= 0 || rank <= 0 || rank > 128 || K <= 0) return MLR_BAD_SIZE;
   if (rows == 0) return MLR_OK;
   if (((uintptr_t)x & 15) != 0 || ((uintptr_t)down & 15) != 0) return MLR_BAD_ALIGNMENT;
-  if (dtype == MLR_BF16 && rows > DOWN_ROWS && K % 8 == 0) return launch_down_tile(x, down, scales, row_adapter, u, rows, adapters, rank, K, early, stream);
+  if (dtype == MLR_BF16 && rows > DOWN_ROWS && K % 8 == 0) {
+    if (rank <= 16) return launch_down_tile<2>(x, down, scales, row_adapter, u, rows, adapters, rank, K, early, stream);
+    if (rank <= 32) return launch_down_tile<4>(x, down, scales, row_adapter, u, rows, adapters, rank, K, early, stream);
+    return launch_down_tile<8>(x, down, scales, row_adapter, u, rows, adapters, rank, K, early, stream);
+  }
   if (dtype == MLR_BF16) return launch_down<bf16>(x, down, scales, row_adapter, u, rows, adapters, rank, K, early, stream);
   if (dtype == MLR_F32) return launch_down<float>(x, down, scales, row_adapter, u, rows, adapters, rank, K, early, stream);
   return MLR_BAD_DTYPE;

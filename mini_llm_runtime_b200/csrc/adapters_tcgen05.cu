@@ -3,15 +3,18 @@
 //   y = [x | u_a ..] [W | B_a ..]^T + b        u[m] = scale (x[m] A[a]^T), computed before (adapters.cu)
 //
 // The adapters extend the sum over K: behind the k blocks of x and W come, for every adapter a that a row of this tile has,
-// blocks of rank columns whose left operand is u and whose right operand is B[a], accumulated in the rows of a alone (the lanes
-// of the other rows are switched off, so that an adapter that is not finite stays with its own rows).  They accumulate where the shared product does, in float32 in tensor memory, so the result is rounded once and an adapter
-// costs its products and the reading of B, no pass over y.  (A kernel that adds the adapters to a shared product in float32
-// reads and writes 0.5 GB more at 2,048 x 37,888: 1,135 us against 500.)  u comes in two bfloat16 parts, u = high + low
-// to 2^-17, as two blocks with the same right operand.
+// blocks of rank columns.  Their left operand is u, every row with the sums of its own adapter, the same for all adapters; their
+// right operand is B[a]; and they accumulate in the rows of a alone: the lanes of the other rows are switched off, so nothing
+// needs zeros, and an adapter that is not finite stays with its own rows.  All of it accumulates where the shared product
+// does, in float32 in tensor memory, so the result is rounded once and an adapter costs its products and the reading of
+// B, no pass over y.  (A kernel that adds the adapters to a shared product in float32 reads and writes 0.5 GB more at
+// 2,048 x 37,888: 1,135 us against 520.)  u comes in two bfloat16 parts, u = high + low to 2^-17, two left operands for
+// one right one.
 //
 // One CTA computes 128 or 256 rows (one or two accumulators) x BN columns.  Warp 0 loads (bulk tensor copies into a ring of
-// 128-byte-swizzled tiles), warp 1 issues the products, warps 2 to 5 list the tile's adapters, build the left operands of
-// the extension in the ring's stages while the shared product runs, and write the result.
+// 128-byte-swizzled tiles), warp 1 issues the products, warps 2 to 5 list the tile's adapters while the shared product runs,
+// lay out u where the first two stages held x, and write the result.  (Left operands of each adapter by itself, with zeros in
+// the other rows, built anew for each: 160 rows of 40 adapters, 896 x 1,152, 105 us.)
 // Every wait is bounded; one that runs out stores a code into the error word, and the CTA frees its tensor memory and ends.
 #include "tcgen05.cuh"
 
@@ -51,19 +54,21 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
   constexpr uint32_t TMEM_COLS = BN * HALVES;
   extern __shared__ uint8_t at_raw[];
   uint8_t* tiles = (uint8_t*)(((uintptr_t)at_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t full[AT_MAX_STAGES], empty[AT_MAX_STAGES], built[AT_MAX_STAGES], listed, near, done;
+  __shared__ uint64_t full[AT_MAX_STAGES], empty[AT_MAX_STAGES], listed, base_done, u_ready, u_free, done;
   __shared__ uint32_t tmem_holder;
-  __shared__ uint4 rows_off[AT_MAX_STAGES][HALVES];
-  __shared__ int ids[BM], list[BM], list_count, failed;
+  __shared__ uint4 rows_off[BM][HALVES];      // of a listed adapter: the rows that are not its own
+  __shared__ int ids[BM], list[BM], place[BM], list_count, failed;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int stages = p.stages;
   const int row0 = blockIdx.x * BM, n0 = blockIdx.y * BN;
   const int base_blocks = (p.K + 63) / 64, chunks = (p.rank + 63) / 64;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); mbar_init(&built[s], 4); }
+    for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     mbar_init(&listed, 1);
-    mbar_init(&near, 1);
+    mbar_init(&base_done, 1);
+    mbar_init(&u_ready, 4);
+    mbar_init(&u_free, 1);
     mbar_init(&done, 1);
     list_count = 0;
     failed = 0;
@@ -107,13 +112,13 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
         load_w(s, i * 64);
       }
       at_wait(&listed, 0u, p.error_word, 0x92, gave_up);
-      const int blocks = gave_up ? 0 : list_count * chunks * 2;
+      const int blocks = gave_up ? 0 : list_count * chunks;
       for (int e = 0; e < blocks; ++e) {
         const int i = base_blocks + e, s = i % stages;
         if (i >= stages) at_wait(&empty[s], (unsigned)(i / stages - 1) & 1u, p.error_word, 0x93, gave_up);
         if (gave_up) break;
         mbar_expect_tx(&full[s], B_BYTES);
-        const int chunk = (e >> 1) % chunks, adapter = list[(e >> 1) / chunks];
+        const int chunk = e / list_count, adapter = list[e - chunk * list_count];
         tma_load_2d(&up_map, &full[s], tiles + (size_t)s * STAGE_BYTES + A_BYTES, chunk * 64, adapter * p.N + n0);
       }
     }
@@ -121,38 +126,54 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
     // ------------------------------------------------------------ products
     constexpr uint32_t idesc = fa_idesc(128, BN, false);
     const uint64_t a_desc0 = fa_desc_k_major(smem_u32(tiles)), b_desc0 = fa_desc_k_major(smem_u32(tiles) + A_BYTES);
-    auto issue = [&](int i, int steps, bool some_rows) {
+    for (int i = 0; i < base_blocks && !gave_up; ++i) {
       const int s = i % stages;
+      at_wait(&full[s], (unsigned)(i / stages) & 1u, p.error_word, 0x94, gave_up);
+      gave_up = __any_sync(0xffffffffu, gave_up);
+      if (gave_up) break;
       fa_fence_after();
       if (elect_one()) {
         const uint64_t a = a_desc0 + (uint64_t)((s * STAGE_BYTES) >> 4), b = b_desc0 + (uint64_t)((s * STAGE_BYTES) >> 4);
-        for (int k = 0; k < steps; ++k)
 #pragma unroll
-          for (int half = 0; half < HALVES; ++half) {
-            const uint64_t a_half = a + (uint64_t)((half * HALF_BYTES + k * 32) >> 4), b_k = b + (uint64_t)((k * 32) >> 4);
-            if (some_rows) at_mma_rows(tmem_base + half * BN, a_half, b_k, idesc, rows_off[s][half]);
-            else fa_mma(tmem_base + half * BN, a_half, b_k, idesc, (i > 0 || k > 0) ? 1u : 0u);
-          }
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int half = 0; half < HALVES; ++half)
+            fa_mma(tmem_base + half * BN, a + (uint64_t)((half * HALF_BYTES + k * 32) >> 4), b + (uint64_t)((k * 32) >> 4), idesc,
+                   (i > 0 || k > 0) ? 1u : 0u);
         fa_commit(&empty[s]);
       }
       __syncwarp();
-    };
-    for (int i = 0; i < base_blocks && !gave_up; ++i) {
-      at_wait(&full[i % stages], (unsigned)(i / stages) & 1u, p.error_word, 0x94, gave_up);
-      gave_up = __any_sync(0xffffffffu, gave_up);
-      if (!gave_up) issue(i, 4, false);
-      if (i == base_blocks - stages - 1 && elect_one()) fa_commit(&near);
-      __syncwarp();
     }
+    if (elect_one()) fa_commit(&base_done);
+    __syncwarp();
     at_wait(&listed, 0u, p.error_word, 0x95, gave_up);
     gave_up = __any_sync(0xffffffffu, gave_up);
-    const int blocks = gave_up ? 0 : list_count * chunks * 2;
-    for (int e = 0; e < blocks && !gave_up; ++e) {
-      const int i = base_blocks + e, s = i % stages;
-      at_wait(&full[s], (unsigned)(i / stages) & 1u, p.error_word, 0x96, gave_up);
-      at_wait(&built[s], (unsigned)(e / stages) & 1u, p.error_word, 0x97, gave_up);
-      gave_up = __any_sync(0xffffffffu, gave_up);
-      if (!gave_up) issue(i, min(4, (p.rank - (e >> 1) % chunks * 64 + 15) / 16), true);
+    const int count = list_count;
+    for (int chunk = 0; chunk < chunks && count > 0 && !gave_up; ++chunk) {
+      at_wait(&u_ready, (unsigned)chunk & 1u, p.error_word, 0x97, gave_up);
+      const int steps = min(4, (p.rank - chunk * 64 + 15) / 16);
+      for (int l = 0; l < count; ++l) {
+        const int i = base_blocks + chunk * count + l, s = i % stages;
+        at_wait(&full[s], (unsigned)(i / stages) & 1u, p.error_word, 0x96, gave_up);
+        gave_up = __any_sync(0xffffffffu, gave_up);
+        if (gave_up) break;
+        fa_fence_after();
+        if (elect_one()) {
+          const uint64_t b = b_desc0 + (uint64_t)((s * STAGE_BYTES) >> 4);
+          for (int half = 0; half < HALVES; ++half) {
+            const uint4 off = rows_off[l][half];
+            if ((off.x & off.y & off.z & off.w) == 0xffffffffu) continue;      // none of its rows are in this half
+            for (int part = 0; part < 2; ++part)
+              for (int k = 0; k < steps; ++k)
+                at_mma_rows(tmem_base + half * BN, a_desc0 + (uint64_t)((part * STAGE_BYTES + half * HALF_BYTES + k * 32) >> 4),
+                            b + (uint64_t)((k * 32) >> 4), idesc, off);
+          }
+          fa_commit(&empty[s]);
+        }
+        __syncwarp();
+      }
+      if (elect_one()) fa_commit(&u_free);
+      __syncwarp();
     }
     if (elect_one()) fa_commit(&done);
     __syncwarp();
@@ -169,66 +190,75 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
       ids[half * 128 + t] = id >= 0 && id < p.adapters ? id : -1;
     }
     asm volatile("bar.sync 1, 128;" ::: "memory");
+    int leader[HALVES];      // the first row with this row's adapter
 #pragma unroll
     for (int half = 0; half < HALVES; ++half) {
       const int at = half * 128 + t, id = ids[at];
-      bool leads = id >= 0 && (at == 0 || ids[at - 1] != id);
-      for (int j = 0; j < at && leads; ++j) leads = ids[j] != id;
+      int j = 0;
+      if (id >= 0)
+        while (ids[j] != id) ++j;
+      leader[half] = id >= 0 ? j : -1;
       // this warp's leaders behind those of the warps (and halves) before it
+      const bool leads = id >= 0 && j == at;
       const unsigned mine = __ballot_sync(0xffffffffu, leads);
       for (int turn = 0; turn < 4; ++turn) {
         if (turn == quarter) {
-          if (leads) list[list_count + __popc(mine & ((1u << lane) - 1u))] = id;
+          const int to = list_count + __popc(mine & ((1u << lane) - 1u));
+          if (leads) {
+            list[to] = id;
+            place[at] = to;
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) rows_off[to][h] = make_uint4(0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu);
+          }
           __syncwarp();
           if (lane == 0) list_count += __popc(mine);
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");
       }
     }
+#pragma unroll
+    for (int half = 0; half < HALVES; ++half)
+      if (leader[half] >= 0) atomicAnd(reinterpret_cast<unsigned*>(&rows_off[place[leader[half]]][half]) + quarter, ~(1u << lane));
+    asm volatile("bar.sync 1, 128;" ::: "memory");
     if (t == 0) mbar_arrive(&listed);
-    const int blocks = list_count * chunks * 2;
-    // A barrier's parity tells two neighbouring rounds apart, no more: these warps look at a stage's barrier only once each
-    // stage is in its last round of the shared product.
-    if (blocks > 0 && base_blocks > stages) at_wait(&near, 0u, p.error_word, 0x9a, gave_up);
-    for (int e = 0; e < blocks; ++e) {
-      const int i = base_blocks + e, s = i % stages, chunk = (e >> 1) % chunks, adapter = list[(e >> 1) / chunks];
-      // the sums are asked for before the stage is free
+    const int count = list_count;
+    for (int chunk = 0; chunk < chunks && count > 0; ++chunk) {
+      // the sums are asked for before their place is free
       float v[HALVES][64];
 #pragma unroll
       for (int half = 0; half < HALVES; ++half) {
-        const bool own = ids[half * 128 + t] == adapter;
         const float* from = p.u + (size_t)(row0 + half * 128 + t) * p.rank + chunk * 64;
 #pragma unroll
         for (int c = 0; c < 64; c += 4) {
-          const float4 four = own && chunk * 64 + c < p.rank ? __ldcg(reinterpret_cast<const float4*>(from + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 four = leader[half] >= 0 && chunk * 64 + c < p.rank ? __ldcg(reinterpret_cast<const float4*>(from + c))
+                                                                          : make_float4(0.f, 0.f, 0.f, 0.f);
           v[half][c] = four.x; v[half][c + 1] = four.y; v[half][c + 2] = four.z; v[half][c + 3] = four.w;
         }
       }
-      if (i >= stages) at_wait(&empty[s], (unsigned)(i / stages - 1) & 1u, p.error_word, 0x98, gave_up);
+      if (chunk == 0) at_wait(&base_done, 0u, p.error_word, 0x9a, gave_up);
+      else at_wait(&u_free, (unsigned)(chunk - 1) & 1u, p.error_word, 0x98, gave_up);
 #pragma unroll
       for (int half = 0; half < HALVES; ++half) {
-        const unsigned off = __ballot_sync(0xffffffffu, ids[half * 128 + t] != adapter);
-        if (lane == 0) reinterpret_cast<unsigned*>(&rows_off[s][half])[quarter] = off;
-        uint8_t* row = tiles + (size_t)s * STAGE_BYTES + half * HALF_BYTES + t * 128;
+        uint8_t* row = tiles + half * HALF_BYTES + t * 128;      // high parts; the low ones a stage on
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          uint32_t packed[4];
+          uint32_t high[4], low[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            float a = v[half][c * 8 + 2 * q], b = v[half][c * 8 + 2 * q + 1];
-            if (e & 1) {
-              a -= __bfloat162float(__float2bfloat16_rn(a));
-              b -= __bfloat162float(__float2bfloat16_rn(b));
-            }
-            __nv_bfloat162 pair = __floats2bfloat162_rn(a, b);
-            packed[q] = *reinterpret_cast<uint32_t*>(&pair);
+            const float x0 = v[half][c * 8 + 2 * q], x1 = v[half][c * 8 + 2 * q + 1];
+            const __nv_bfloat162 pair = __floats2bfloat162_rn(x0, x1);
+            const __nv_bfloat162 rest = __floats2bfloat162_rn(x0 - __bfloat162float(pair.x), x1 - __bfloat162float(pair.y));
+            high[q] = *reinterpret_cast<const uint32_t*>(&pair);
+            low[q] = *reinterpret_cast<const uint32_t*>(&rest);
           }
-          *reinterpret_cast<uint4*>(row + ((c ^ (t & 7)) << 4)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+          const int at = (c ^ (t & 7)) << 4;
+          *reinterpret_cast<uint4*>(row + at) = make_uint4(high[0], high[1], high[2], high[3]);
+          *reinterpret_cast<uint4*>(row + STAGE_BYTES + at) = make_uint4(low[0], low[1], low[2], low[3]);
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&built[s]);
+      if (lane == 0) mbar_arrive(&u_ready);
     }
     at_wait(&done, 0u, p.error_word, 0x99, gave_up);
     if (gave_up) atomicOr(&failed, 1);
@@ -294,8 +324,8 @@ static int launch(const void* x, const void* w, const void* up, AdapterGemm p, i
   constexpr size_t STAGE = HALVES * 128 * 128 + BN * 128;
   p.stages = stages;
   static OncePerDevice once;
-  if (cudaError_t err = once([=] {
-        return cudaFuncSetAttribute(adapter_gemm_kernel<BN, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(stages * STAGE + 1024));
+  if (cudaError_t err = once([] {
+        return cudaFuncSetAttribute(adapter_gemm_kernel<BN, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, 193 * 1024);
       }))
     return (int)err;
   CUtensorMap x_map, w_map, up_map;
@@ -308,24 +338,27 @@ static int launch(const void* x, const void* w, const void* up, AdapterGemm p, i
   return launch_status();
 }
 
-// Which tile: 128 x 128 (three stages), 128 x 256 (two stages; two CTAs per SM either way) or 256 x 256 (three stages, one CTA).  A
-// k block costs the largest of its MMAs (0.14 us per 128 x 128), its copies' latency spread over the ring and the SM's share of
-// operand bandwidth, a CTA 1.5 us and its epilogue, and a launch so many rounds of CTAs.
-static int plan(int M, int N, int K, int sms) {
+// Which tile and ring: 128 x 128, 128 x 256 or 256 x 256, with rings that leave an SM to two CTAs (three and two stages) where there are
+// more CTAs than SMs, else as deep as 192 KB (six, four, three).  A k block costs the largest of its MMAs (0.14 us per 128 x
+// 128), its copies' latency spread over the ring and the SM's share of operand bandwidth, a CTA 1.5 us and its epilogue, and
+// a launch so many rounds of CTAs.
+struct AdapterPlan { int shape, stages; };
+static AdapterPlan plan(int M, int N, int K, int sms) {
   const double kb = (K + 63) / 64;
-  int best = 0;
+  AdapterPlan best{0, 3};
   double least = 1e30;
   for (int shape = 0; shape < 3; ++shape) {
-    const int bn = shape == 0 ? 128 : 256, halves = shape == 2 ? 2 : 1, stages = shape == 1 ? 2 : 3, per_sm = shape == 2 ? 1 : 2;
+    const int bn = shape == 0 ? 128 : 256, halves = shape == 2 ? 2 : 1;
     const long long ctas = (long long)((M + 128 * halves - 1) / (128 * halves)) * ((N + bn - 1) / bn);
+    const bool alone = ctas <= sms || shape == 2;
+    const int stages = shape == 2 ? 3 : alone ? (shape == 0 ? 6 : 4) : (shape == 0 ? 3 : 2), per_sm = alone ? 1 : 2;
     const long long rounds = (ctas + (long long)per_sm * sms - 1) / ((long long)per_sm * sms);
-    const int sharing = ctas <= sms ? 1 : per_sm;
     const double stage_kb = 16.0 * halves + bn / 8.0;
-    double each = 0.14 * (bn / 128) * halves * sharing;
+    double each = 0.14 * (bn / 128) * halves * per_sm;
     if ((0.5 + 0.03 * stage_kb) / stages > each) each = (0.5 + 0.03 * stage_kb) / stages;
-    if (sharing * stage_kb / 112.0 > each) each = sharing * stage_kb / 112.0;
+    if (per_sm * stage_kb / 112.0 > each) each = per_sm * stage_kb / 112.0;
     const double cost = rounds * (1.5 + kb * each + 1.5 * (bn / 128) * halves + (per_sm == 1 && rounds > 1 ? 4.0 : 0.0));
-    if (cost < least) { least = cost; best = shape; }
+    if (cost < least) { least = cost; best = {shape, stages}; }
   }
   return best;
 }
@@ -346,8 +379,8 @@ MLR_EXPORT int mlr_adapter_gemm(const void* x, const void* w, const void* up, co
   if (K % 8 != 0 || rank % 8 != 0 || (((uintptr_t)x | (uintptr_t)w | (uintptr_t)up | (uintptr_t)u | (uintptr_t)out) & 15) != 0) return MLR_BAD_ALIGNMENT;
   if ((long long)adapters * N > 0x7fffffffll) return MLR_TOO_LARGE;
   AdapterGemm p{M, N, K, adapters, rank, 0, (const bf16*)bias, u, row_adapter, out, out_f32, error_word};
-  const int shape = plan(M, N, K, sm_count());
-  if (shape == 2) return launch<256, 2>(x, w, up, p, 3, stream);
-  if (shape == 1) return launch<256, 1>(x, w, up, p, 2, stream);
-  return launch<128, 1>(x, w, up, p, 3, stream);
+  const AdapterPlan chosen = plan(M, N, K, sm_count());
+  if (chosen.shape == 2) return launch<256, 2>(x, w, up, p, chosen.stages, stream);
+  if (chosen.shape == 1) return launch<256, 1>(x, w, up, p, chosen.stages, stream);
+  return launch<128, 1>(x, w, up, p, chosen.stages, stream);
 }
