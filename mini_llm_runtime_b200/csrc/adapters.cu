@@ -38,6 +38,10 @@ __device__ __forceinline__ float read_from_cta(const float* mine, uint32_t rank)
   return v;
 }
 
+template <bool FIRST, typename A, typename B> struct Choice { typedef A type; };
+template <typename A, typename B> struct Choice<false, A, B> { typedef B type; };
+template <int N> struct Count { static constexpr int value = N; };
+
 // 16 bytes of bfloat16 or float32 as floats.
 template <typename T> struct Pack { static constexpr int N = 16 / sizeof(T); };
 __device__ __forceinline__ void unpack(const uint4& raw, float* v, bf16) {
@@ -56,74 +60,113 @@ __device__ __forceinline__ void unpack(const uint4& raw, float* v, float) {
 // Both down kernels: `early` says that the kernel in front is the shared product of the same x, which lets the next kernel in
 // after its own wait: what is read here was complete then, and the sums are taken beside it; this kernel waits for it at its end.
 //
-// Few rows, each with an adapter of its own as a rule: CTA = (row, 16 rank rows, part of K), bound by reading A.  A warp walks
-// its stretch of K 32 pieces of 16 bytes at a time and holds 16 sums; the parts of K meet through the cluster's shared memory,
-// in order.  WIDE: rows are whole 16-byte pieces.
-template <typename T, bool WIDE>
+// Few rows, each with an adapter of its own as a rule, and 32-bit rows: CTA = (ROWS neighbouring rows, 16 rank rows, part of K), bound
+// by reading A.  A warp walks its stretch of K 32 pieces of 16 bytes at a time and holds 16 sums of every row; rows of one
+// adapter (a prompt's) share what is read of it, others take turns.  The parts of K meet through the cluster's shared memory, in
+// order.  WIDE: rows are whole 16-byte pieces.
+template <typename T, int ROWS, bool WIDE>
 __global__ void __launch_bounds__(DOWN_WARPS * 32)
 adapter_down_rows_kernel(const T* x, const T* __restrict__ down, const float* __restrict__ scales, const int* row_adapter, float* u,
-                         int adapters, int rank, int K, int parts, int early) {
+                         int rows, int adapters, int rank, int K, int parts, int early) {
   constexpr int PIECE = WIDE ? Pack<T>::N : 1;
-  __shared__ float sums[DOWN_WARPS][DOWN_RANKS];
-  __shared__ float total[DOWN_RANKS];
-  const int part = blockIdx.x % parts, row = blockIdx.x / parts;
+  __shared__ float sums[DOWN_WARPS][ROWS][DOWN_RANKS];
+  __shared__ float total[ROWS][DOWN_RANKS];
+  const int part = blockIdx.x % parts, row0 = blockIdx.x / parts * ROWS;
   const int r0 = blockIdx.y * DOWN_RANKS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (!early) pdl_wait();
   pdl_trigger();      // after the wait: adapter_up_kernel relies on it
-  const int adapter = __ldcg(row_adapter + row);
-  const bool live = adapter >= 0 && adapter < adapters;      // the same in all CTAs of a cluster
-  if (live) {
-    float acc[DOWN_RANKS];
+  int ids[ROWS];
+  bool together = true;
 #pragma unroll
-    for (int r = 0; r < DOWN_RANKS; ++r) acc[r] = 0.f;
-    const int pieces = K / PIECE;
-    const int stretch = (pieces + parts * DOWN_WARPS - 1) / (parts * DOWN_WARPS);
-    const int begin = (part * DOWN_WARPS + warp) * stretch, end = min(pieces, begin + stretch);
-    const T* xr = x + (size_t)row * K;
+  for (int m = 0; m < ROWS; ++m) {
+    const int id = row0 + m < rows ? __ldcg(row_adapter + row0 + m) : -1;
+    ids[m] = id >= 0 && id < adapters ? id : -1;      // the same in all CTAs of a cluster
+    together = together && ids[m] == ids[0];
+  }
+  const int pieces = K / PIECE;
+  const int stretch = (pieces + parts * DOWN_WARPS - 1) / (parts * DOWN_WARPS);
+  const int begin = (part * DOWN_WARPS + warp) * stretch, end = min(pieces, begin + stretch);
+  const int ranks = min(DOWN_RANKS, rank - r0);
+  // the sums of rows m0 .. m0 + COUNT - 1 with one adapter
+  auto take = [&](auto count, int m0, int adapter) {
+    constexpr int COUNT = decltype(count)::value;
+    float acc[COUNT][DOWN_RANKS];
+#pragma unroll
+    for (int m = 0; m < COUNT; ++m)
+#pragma unroll
+      for (int r = 0; r < DOWN_RANKS; ++r) acc[m][r] = 0.f;
+    const T* xr = x + (size_t)(row0 + m0) * K;
     const T* ar = down + ((size_t)adapter * rank + r0) * K;
-    const int ranks = min(DOWN_RANKS, rank - r0);
     for (int p = begin + lane; p < end; p += 32) {
       if (WIDE) {
-        float xv[PIECE];
-        unpack(__ldcg(reinterpret_cast<const uint4*>(xr) + p), xv, T());
-        uint4 raw[DOWN_RANKS];
+        float xv[COUNT][PIECE];
 #pragma unroll
-        for (int r = 0; r < DOWN_RANKS; ++r)
-          raw[r] = r < ranks ? __ldg(reinterpret_cast<const uint4*>(ar + (size_t)r * K) + p) : make_uint4(0u, 0u, 0u, 0u);
+        for (int m = 0; m < COUNT; ++m) unpack(__ldcg(reinterpret_cast<const uint4*>(xr + (size_t)m * K) + p), xv[m], T());
+        constexpr int BATCH = 8;
 #pragma unroll
-        for (int r = 0; r < DOWN_RANKS; ++r) {
-          float av[PIECE];
-          unpack(raw[r], av, T());
+        for (int rb = 0; rb < DOWN_RANKS; rb += BATCH) {
+          uint4 raw[BATCH];
 #pragma unroll
-          for (int e = 0; e < PIECE; ++e) acc[r] = fmaf(xv[e], av[e], acc[r]);
+          for (int r = 0; r < BATCH; ++r)
+            raw[r] = __ldg(reinterpret_cast<const uint4*>(ar + (size_t)min(rb + r, ranks - 1) * K) + p);      // past the last: unused sums
+#pragma unroll
+          for (int r = 0; r < BATCH; ++r) {
+            float av[PIECE];
+            unpack(raw[r], av, T());
+#pragma unroll
+            for (int m = 0; m < COUNT; ++m)
+#pragma unroll
+              for (int e = 0; e < PIECE; ++e) acc[m][rb + r] = fmaf(xv[m][e], av[e], acc[m][rb + r]);
+          }
         }
       } else {
-        const float xv = to_float(xr[p]);
 #pragma unroll
-        for (int r = 0; r < DOWN_RANKS; ++r)
-          if (r < ranks) acc[r] = fmaf(xv, to_float(ar[(size_t)r * K + p]), acc[r]);
+        for (int m = 0; m < COUNT; ++m) {
+          const float xv = to_float(xr[(size_t)m * K + p]);
+#pragma unroll
+          for (int r = 0; r < DOWN_RANKS; ++r)
+            if (r < ranks) acc[m][r] = fmaf(xv, to_float(ar[(size_t)r * K + p]), acc[m][r]);
+        }
       }
     }
 #pragma unroll
-    for (int r = 0; r < DOWN_RANKS; ++r) {
-      const float sum = warp_sum(acc[r]);
-      if (lane == 0) sums[warp][r] = sum;
+    for (int m = 0; m < COUNT; ++m)
+#pragma unroll
+      for (int r = 0; r < DOWN_RANKS; ++r) {
+        const float sum = warp_sum(acc[m][r]);
+        if (lane == 0) sums[warp][m0 + m][r] = sum;
+      }
+  };
+  if (ROWS > 1 && together) {
+    if (ids[0] >= 0) take(Count<ROWS>(), 0, ids[0]);
+  } else {
+    for (int m = 0; m < ROWS; ++m) {
+      int id = ids[0];
+#pragma unroll
+      for (int q = 1; q < ROWS; ++q)
+        if (q == m) id = ids[q];
+      if (id >= 0) take(Count<1>(), m, id);
     }
   }
   __syncthreads();
-  if (live && threadIdx.x < DOWN_RANKS) {
+  for (int i = threadIdx.x; i < ROWS * DOWN_RANKS; i += DOWN_WARPS * 32) {
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < DOWN_WARPS; ++w) sum += sums[w][threadIdx.x];
-    total[threadIdx.x] = sum;
+    for (int w = 0; w < DOWN_WARPS; ++w) sum += sums[w][i / DOWN_RANKS][i % DOWN_RANKS];
+    total[i / DOWN_RANKS][i % DOWN_RANKS] = sum;      // of rows without an adapter: never looked at
   }
   cluster_meet();
-  if (live && part == 0 && threadIdx.x < DOWN_RANKS && r0 + (int)threadIdx.x < rank) {
-    float sum = 0.f;
+  if (part == 0) {
+    for (int i = threadIdx.x; i < ROWS * DOWN_RANKS; i += DOWN_WARPS * 32) {
+      const int m = i / DOWN_RANKS, r = i % DOWN_RANKS;
+      const int id = row0 + m < rows ? __ldcg(row_adapter + row0 + m) : -1;
+      if (id < 0 || id >= adapters || r0 + r >= rank) continue;
+      float sum = 0.f;
 #pragma unroll
-    for (int other = 0; other < MOST_PARTS; ++other) sum += other < parts ? read_from_cta(&total[threadIdx.x], other) : 0.f;
-    u[(size_t)row * rank + r0 + threadIdx.x] = scales[adapter] * sum;
+      for (int other = 0; other < MOST_PARTS; ++other) sum += other < parts ? read_from_cta(&total[m][r], other) : 0.f;
+      u[(size_t)(row0 + m) * rank + r0 + r] = scales[id] * sum;
+    }
   }
   cluster_meet();      // no CTA leaves while another reads its sums
   if (early) pdl_wait();
@@ -233,42 +276,47 @@ adapter_down_tile_kernel(const bf16* x, const bf16* __restrict__ down, const flo
   if (early) pdl_wait();
 }
 
-// Up: a thread owns one output column and ROWS rows; B's row of the column is read once per run of rows with one adapter.  The
-// first CHUNK columns of it are asked for before the wait: which adapter a row has was complete before the down kernel, in
-// front of this one on the stream, let the kernels behind it in.
+// Up: a thread owns one output column and ROWS rows; B's row of the column is read once per run of rows with one adapter, 16
+// ranks at a time, the next ones under way.  The first are asked for before the wait: which adapter a row has was complete
+// before the down kernel, in front of this one on the stream, let the kernels behind it in.
 template <typename T, typename Out, int ROWS, bool WIDE>
 __global__ void __launch_bounds__(128)
 adapter_up_kernel(const float* u, const T* __restrict__ up, const int* row_adapter, const float* base, Out* out, int rows, int adapters,
                   int rank, int N) {
-  constexpr int CHUNK = 16;
+  constexpr int CHUNK = 16, PIECES = WIDE ? CHUNK / Pack<T>::N : CHUNK;
+  typedef typename Choice<WIDE, uint4, T>::type Raw;
   __shared__ float low[ROWS][128];
   const int row0 = blockIdx.y * ROWS;
   const int n = blockIdx.x * 128 + threadIdx.x;
   int ids[ROWS];
+  bool same = true;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     const int id = row0 + r < rows ? __ldcg(row_adapter + row0 + r) : -1;
     ids[r] = id >= 0 && id < adapters ? id : -1;
+    same = same && (ids[r] == ids[0] || row0 + r >= rows);
   }
-  auto load = [&](int id, int k0, float* b) {
-    const T* from = up + ((size_t)id * N + n) * rank + k0;
-    if (WIDE) {
+  // (no test per piece, so that the loads go out together: past the last rank or column others are read and not used)
+  auto load = [&](int id, int k0, Raw* raw) {
+    if (id < 0 || k0 >= rank) return;
+    const T* from = up + ((size_t)id * N + min(n, N - 1)) * rank;
+    constexpr int W = CHUNK / PIECES;
 #pragma unroll
-      for (int i = 0; i < CHUNK; i += Pack<T>::N) {
-        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        if (n < N && k0 + i < rank) raw = __ldg(reinterpret_cast<const uint4*>(from + i));
-        unpack(raw, b + i, T());
-      }
-    } else {
+    for (int i = 0; i < PIECES; ++i) raw[i] = *reinterpret_cast<const Raw*>(from + min(k0 + i * W, rank - W));
+  };
+  auto values = [&](const Raw* raw, float* b) {
 #pragma unroll
-      for (int i = 0; i < CHUNK; ++i) b[i] = n < N && k0 + i < rank ? to_float(from[i]) : 0.f;
+    for (int i = 0; i < PIECES; ++i) {
+      if constexpr (WIDE) unpack(raw[i], b + i * (CHUNK / PIECES), T());
+      else b[i] = to_float(raw[i]);
     }
   };
-  float first[ROWS > 2 ? 1 : ROWS][CHUNK];      // of every row where they are few
-  if (ROWS <= 2)
+  // of a thread's rows if they are few; of a run of many, what its first row needs
+  constexpr int HELD = ROWS <= 2 ? ROWS : 1;
+  Raw next[HELD][PIECES];
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-      if (ids[r] >= 0) load(ids[r], 0, first[r]);
+  for (int r = 0; r < HELD; ++r)
+    if (r == 0 || ids[r] != ids[0]) load(ids[r], 0, next[r]);
   pdl_wait();
   pdl_trigger();
   for (int i = threadIdx.x; i < ROWS * rank; i += 128) {
@@ -282,20 +330,42 @@ adapter_up_kernel(const float* u, const T* __restrict__ up, const int* row_adapt
   __syncthreads();
   if (n >= N) return;
   for (int k0 = 0; k0 < rank; k0 += CHUNK) {
-    float b[CHUNK];
-    int held = -1;
+    float b[HELD][CHUNK];
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      if (ids[r] < 0) continue;
-      if (ROWS <= 2 && k0 == 0) {
+    for (int r = 0; r < HELD; ++r) {
+      if (r > 0 && ids[r] == ids[0]) continue;      // the first row's values
+      values(next[r], b[r]);
+      load(ids[r], k0 + CHUNK, next[r]);
+    }
+    auto add = [&](int r, const float* w) {
 #pragma unroll
-        for (int i = 0; i < CHUNK; ++i) b[i] = first[r][i];
-      } else if (ids[r] != held) {
-        load(ids[r], k0, b);
-        held = ids[r];
+      for (int i = 0; i < CHUNK; ++i)
+        if (k0 + i < rank) acc[r] = fmaf(low[r][k0 + i], w[i], acc[r]);
+    };
+    if (ROWS <= 2) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        if (ids[r] < 0) continue;
+        if (r > 0 && ids[r] == ids[0]) add(r, b[0]);
+        else add(r, b[r < HELD ? r : 0]);
       }
+    } else if (same) {
+      if (ids[0] >= 0)
 #pragma unroll
-      for (int i = 0; i < CHUNK; ++i) acc[r] = fmaf(k0 + i < rank ? low[r][k0 + i] : 0.f, b[i], acc[r]);
+        for (int r = 0; r < ROWS; ++r) add(r, b[0]);
+    } else {
+      int held = ids[0];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        if (ids[r] < 0) continue;
+        if (ids[r] != held) {
+          held = ids[r];
+          Raw raw[PIECES];
+          load(held, k0, raw);
+          values(raw, b[0]);
+        }
+        add(r, b[0]);
+      }
     }
   }
 #pragma unroll
@@ -317,21 +387,28 @@ static int launch_down_tile(const void* x, const void* down, const float* scales
   return launch_status();
 }
 
-template <typename T>
-static int launch_down(const void* x, const void* down, const float* scales, const int* row_adapter, float* u, int rows, int adapters,
-                       int rank, int K, int early, cudaStream_t stream) {
+template <typename T, int ROWS>
+static int launch_down_rows(const void* x, const void* down, const float* scales, const int* row_adapter, float* u, int rows, int adapters,
+                            int rank, int K, int early, cudaStream_t stream) {
   // parts of K: as many CTAs as fill the device four times, at most eight (a cluster), none below 32 pieces per warp
   const bool wide = K % Pack<T>::N == 0;
   const int pieces = wide ? K / Pack<T>::N : K;
-  const int groups = (rank + DOWN_RANKS - 1) / DOWN_RANKS;
+  const int groups = (rank + DOWN_RANKS - 1) / DOWN_RANKS, blocks = (rows + ROWS - 1) / ROWS;
   int parts = 1;
-  while (parts < MOST_PARTS && (long long)rows * groups * parts < 4ll * sm_count() && pieces >= 2 * parts * DOWN_WARPS * 32) parts *= 2;
-  if ((long long)rows * parts > 0x7fffffff || groups > 65535) return MLR_TOO_LARGE;
-  const dim3 grid(rows * parts, groups);
-  auto kernel = wide ? adapter_down_rows_kernel<T, true> : adapter_down_rows_kernel<T, false>;
+  while (parts < MOST_PARTS && (long long)blocks * groups * parts < 4ll * sm_count() && pieces >= 2 * parts * DOWN_WARPS * 32) parts *= 2;
+  if ((long long)blocks * parts > 0x7fffffff || groups > 65535) return MLR_TOO_LARGE;
+  const dim3 grid(blocks * parts, groups);
+  auto kernel = wide ? adapter_down_rows_kernel<T, ROWS, true> : adapter_down_rows_kernel<T, ROWS, false>;
   launch_kernel_clustered(kernel, grid, dim3(DOWN_WARPS * 32), 0, stream, parts, (const T*)x, (const T*)down, scales, row_adapter, u,
-                          adapters, rank, K, parts, early);
+                          rows, adapters, rank, K, parts, early);
   return launch_status();
+}
+
+template <typename T>
+static int launch_down(const void* x, const void* down, const float* scales, const int* row_adapter, float* u, int rows, int adapters,
+                       int rank, int K, int early, cudaStream_t stream) {
+  return rows <= DOWN_ROWS ? launch_down_rows<T, 1>(x, down, scales, row_adapter, u, rows, adapters, rank, K, early, stream)
+                           : launch_down_rows<T, 4>(x, down, scales, row_adapter, u, rows, adapters, rank, K, early, stream);
 }
 
 template <typename T, typename Out, int ROWS>
