@@ -916,15 +916,20 @@ class CudaOps:
         return (rows <= 4 and row % 16 == 0 and rows * rows * rank * row <= self.SMALL_ADAPTER_BYTES
                 and outer * inner <= self.SMALL_ADAPTER_WEIGHT)
 
-    # Rows from which the adapters extend the shared product's sum over K, unless few tiles of 128 x 128 walk a long K (that product has no
-    # split): K up to so many times the tiles.  Captured, us, extended / three kernels, rank 16, one adapter per portion (40 adapters among
-    # the rows): 200 rows 9,728 x 896 14 / 37 (42 / 45), 4,608 x 3,584 23 / 32 (47 / 49), 896 x 4,864 29 / 22 (55 / 38), 3,584 x 18,944 91 / 66
+    # The adapters extend the shared product's sum over K from so many rows, or above 16 rows from so many products rows x N x rank of the
+    # second pass, which reads B once per row (64 MB in 25 us), unless few tiles of 128 x 128 walk a long K (that product has no split): K up to so many
+    # times the tiles.  Captured, us, extended / three kernels, rank 16, one adapter per portion (40 adapters among the rows):
+    # 200 rows 9,728 x 896 14 / 37 (42 / 45), 4,608 x 3,584 23 / 32 (47 / 49), 896 x 4,864 29 / 22 (55 / 38), 3,584 x 18,944 91 / 66
     # (144 / 121), 1,152 x 896 11 / 14 (41 / 22); 1,000 rows 34 / 102 (92 / 119), 32 / 64 (108 / 119), 34 / 34 (90 / 85), 125 / 156 (291 / 312),
-    # 12 / 20 (42 / 34); 100 rows 11 / 20 (28 / 21), 22 / 22 (36 / 22), 28 / 17 (42 / 18).
-    ADAPTER_ROWS, ADAPTER_K_PER_TILE = 128, 160
+    # 12 / 20 (42 / 34); 100 rows 11 / 20 (28 / 21), 22 / 22 (36 / 22), 28 / 17 (42 / 18).  Up to 128 rows of four adapters (of 40):
+    # 9,728 x 896 128 rows rank 128 22 / 109 (67 / 113), rank 64 16 / 61 (39 / 62), 64 rows 17 / 61 (60 / 63) and 13 / 33 (36 / 33), 33 rows
+    # 15 / 36 (50 / 38) and 11 / 22 (29 / 22); 4,608 x 3,584 128 rows 38 / 77 (84 / 86) and 32 / 50 (52 / 53), 64 rows 32 / 48 (76 / 56) and
+    # 26 / 31 (46 / 32); 1,152 x 896 128 rows 22 / 35 (63 / 34).
+    ADAPTER_ROWS, ADAPTER_PRODUCTS, ADAPTER_K_PER_TILE = 128, 32 << 20, 160
 
-    def _adapters_extend(self, rows: int, outer: int, inner: int) -> bool:
-        return rows > self.ADAPTER_ROWS and inner <= self.ADAPTER_K_PER_TILE * -(-rows // 128) * -(-outer // 128)
+    def _adapters_extend(self, rows: int, outer: int, inner: int, rank: int) -> bool:
+        return ((rows > self.ADAPTER_ROWS or rows > 16 and rows * outer * rank >= self.ADAPTER_PRODUCTS)
+                and inner <= self.ADAPTER_K_PER_TILE * -(-rows // 128) * -(-outer // 128))
 
     def linear_adapters(self, x: torch.Tensor, weight: torch.Tensor, adapters: AdapterStack, row_adapter: torch.Tensor,
                         bias: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -961,7 +966,7 @@ class CudaOps:
             return out
         aligned = not weight.data_ptr() % 16
         library = _declared_library("adapters")
-        if (self.use_tensor_cores and x.dtype == torch.bfloat16 and self._adapters_extend(rows, N, K) and K % 8 == 0 and rank % 8 == 0
+        if (self.use_tensor_cores and x.dtype == torch.bfloat16 and self._adapters_extend(rows, N, K, rank) and K % 8 == 0 and rank % 8 == 0
                 and aligned and count * N < 1 << 31):
             low = x.new_empty((rows, rank), dtype=torch.float32)
             out = x.new_empty((rows, N), dtype=out_dtype)

@@ -85,6 +85,7 @@ def test_adapters_against_their_formula(dtype, rows, K, N, rank, count, pattern)
 @pytest.mark.parametrize("rows,K,N,rank,count,pattern", [
     (600, 896, 2048, 16, 5, "runs"), (1025, 512, 1160, 64, 3, "mixed"), (513, 2048, 4608, 48, 20, "runs"),
     (2048, 1024, 3584, 8, 2, "runs"), (700, 640, 776, 128, 600, "mixed"),
+    (17, 640, 15880, 128, 3, "runs"), (40, 896, 9728, 128, 50, "mixed"), (128, 200, 4608, 64, 2, "one"),
 ])
 def test_prompt_steps(rows, K, N, rank, count, pattern):
     case = made(rows, K, N, rank, count, torch.bfloat16, rows, bias=rows % 2 == 1)
