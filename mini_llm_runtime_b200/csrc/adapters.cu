@@ -103,7 +103,7 @@ adapter_down_rows_kernel(const T* x, const T* __restrict__ down, const float* __
         float xv[COUNT][PIECE];
 #pragma unroll
         for (int m = 0; m < COUNT; ++m) unpack(__ldcg(reinterpret_cast<const uint4*>(xr + (size_t)m * K) + p), xv[m], T());
-        constexpr int BATCH = 8;
+        constexpr int BATCH = ROWS == 1 ? DOWN_RANKS : 8;
 #pragma unroll
         for (int rb = 0; rb < DOWN_RANKS; rb += BATCH) {
           uint4 raw[BATCH];
