@@ -20,6 +20,9 @@ from collections.abc import Mapping
 from dataclasses import dataclass
 
 
+_LEAST_FLOAT32, _MOST_FLOAT32 = 2.0 ** -126, (2.0 - 2.0 ** -23) * 2.0 ** 127
+
+
 @dataclass(frozen=True)
 class SamplingParams:
     temperature: float = 0.0
@@ -43,12 +46,18 @@ class SamplingParams:
             object.__setattr__(self, name, float(value))
         if self.repetition_penalty <= 0:
             raise ValueError("repetition_penalty must be > 0 (1 changes nothing)")
+        # The device holds them in 32 bits, where less would be 0 (and a logit divided by it infinite) and more infinite.
+        if not _LEAST_FLOAT32 <= self.repetition_penalty <= _MOST_FLOAT32 or max(abs(self.presence_penalty),
+                                                                                abs(self.frequency_penalty)) > _MOST_FLOAT32:
+            raise ValueError("penalties must fit 32 bits")
         pairs = self.logit_bias.items() if isinstance(self.logit_bias, Mapping) else self.logit_bias
         biases = tuple(sorted((token, float(value)) for token, value in pairs))
         if any(isinstance(token, bool) or not isinstance(token, int) or token < 0 for token, _ in biases):
             raise ValueError("logit_bias names tokens by integers >= 0")
         if any(math.isnan(value) or value == math.inf for _, value in biases):
             raise ValueError("a bias must be a number; -inf bans its token")
+        if any(math.isfinite(value) and abs(value) > _MOST_FLOAT32 for _, value in biases):
+            raise ValueError("biases must fit 32 bits")
         if len({token for token, _ in biases}) != len(biases):
             raise ValueError("logit_bias names a token twice")
         object.__setattr__(self, "logit_bias", biases)

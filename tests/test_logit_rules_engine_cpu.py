@@ -148,6 +148,7 @@ def test_grammars_and_stepping_ahead_exclude_each_other(tiny):
     dict(frequency_penalty="1"), dict(presence_penalty=True), dict(logit_bias={-1: 1.0}), dict(logit_bias={1.5: 1.0}),
     dict(logit_bias={1: math.nan}), dict(logit_bias={1: math.inf}), dict(logit_bias=((1, 1.0), (1, 2.0))), dict(logit_bias={256: 1.0}),
     dict(logit_bias={t: 1.0 for t in range(301)}), dict(no_such_rule=1),
+    dict(repetition_penalty=1e-39), dict(repetition_penalty=1e39), dict(presence_penalty=-1e39), dict(logit_bias={1: 1e39}),      # not in 32 bits
 ])
 def test_rules_that_are_refused(tiny, bad):
     config, _ = TINY["A"]
