@@ -142,7 +142,8 @@ class ContinuousBatchEngine:
     def submit(self, request_id: str, prompt_token_ids: Sequence[int], *, max_new_tokens: int,
                eos_token_ids: int | Collection[int] | None = None, temperature: float = 0.0,
                seed: int = 0, prefix: str | None = None, **rules) -> Request:
-        """``prefix``: a prefix of ``add_prefix`` that the prompt starts with; its whole pages are shared, not computed again.  ``rules``: ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty``, ``logit_bias`` of ``SamplingParams`` (an engine
+        """``prefix``: a prefix of ``add_prefix`` that the prompt starts with; its whole pages are shared, not computed again.
+        ``rules``: ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty``, ``logit_bias`` of ``SamplingParams`` (an engine
         made with ``logit_rules=True``)."""
         arrival_ns = self._clock_ns()
         vocab = self.runner.vocab_size
@@ -158,6 +159,8 @@ class ContinuousBatchEngine:
             self.runner.rules.check(sampling)
         elif sampling.has_rules:
             raise ValueError("rules on logits need an engine made with logit_rules=True")
+        if any(request_id == self._holder(name) for name in self._prefixes):
+            raise ValueError(f"{request_id!r} is the name under which the cache holds a prefix")
         holder, shared = self._shared_by(prefix, prompt_token_ids)
         request = self.scheduler.submit(request_id, prompt_token_ids, max_new_tokens=max_new_tokens,
                                         eos_token_ids=eos_token_ids, sampling=sampling, prefix=holder, shared=shared)
@@ -179,6 +182,8 @@ class ContinuousBatchEngine:
             raise ValueError("pages are shared by models whose layers keep every key, without windows or states")
         if name in self._prefixes:
             raise ValueError(f"prefix {name!r} exists already")
+        if self._holder(name) in (*self.scheduler.waiting_request_ids, *self.scheduler.running_request_ids):
+            raise ValueError(f"a request is called {self._holder(name)!r}, as the cache would call prefix {name!r}")
         if len(tokens) < page:
             raise ValueError(f"a prefix of {len(tokens)} tokens fills no page of {page}")
         if any(not 0 <= t < self.runner.vocab_size for t in tokens):

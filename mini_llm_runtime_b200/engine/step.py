@@ -219,6 +219,7 @@ class ModelRunner:
         self._graph_seen: dict[tuple, int] = {}
         # Groups of shared prefixes come in many sizes: of the captured steps that hold any, the ones used last are kept.
         self.graph_max_shared = 32
+        self._shared_shapes: dict[tuple, bool] = {}      # by (requests, sizes of their groups): whether the step's work lists hold them
         self.graph_replays = 0
         # Rules of the requests on their logits (sampling/rules.py), or None.  To be set before the first step: a captured step
         # holds the launches of its time.
@@ -300,8 +301,24 @@ class ModelRunner:
     def _graph_key(self, requests: list[RequestCache], sample: bool, feed: bool) -> tuple:
         """What a captured decode step depends on: its size, what it does, the context limit it plans for, and the sizes of its
         groups of shared prefixes (which requests they are is refreshed like the slots)."""
-        shapes = tuple((len(segments), keys) for segments, keys in self._shared_groups(requests))
+        shared = self._shared_groups(requests)
+        shapes = tuple((len(segments), keys) for segments, keys in shared)
+        if shapes and not self._has_shared_plans(len(requests), shapes, shared):
+            shapes = ()
         return (len(requests), sample, feed, self._context_limit(requests), *shapes)
+
+    def _has_shared_plans(self, count: int, shapes: tuple, shared: tuple) -> bool:
+        """Whether a decode step of ``count`` requests with groups of these sizes has work lists for their prefixes (groups too small
+        to be worth it have none, and need no captured step of their own)."""
+        known = self._shared_shapes.get((count, shapes))
+        if known is None:
+            if len(self._shared_shapes) >= 4096:
+                self._shared_shapes.clear()
+            ones = np.ones(count, dtype=np.int32)
+            host = HostBatch(ones, np.arange(count, dtype=np.int32), np.full(count, shapes[0][1], dtype=np.int32), count, shared)
+            known = any(name.startswith("shared.") for arrays, _ in self._step_plans(host).values() for name in arrays)
+            self._shared_shapes[count, shapes] = known
+        return known
 
     def _step_plans(self, host: HostBatch) -> dict:
         """Work lists from the mixers, one per plan key (mixers with equal keys share one)."""
@@ -532,7 +549,7 @@ class ModelRunner:
                     staging[1] = event = torch.cuda.Event()
                 event.record()
                 captured.slots_now = slots
-            shared = self._shared_groups(requests)
+            shared = self._shared_groups(requests) if len(key) > 4 else captured.shared_now
             if shared != captured.shared_now:      # the same sizes, other requests
                 for name, (arrays, _) in self._step_plans(self._host_batch(entries, requests)).items():
                     for array_name, array in arrays.items():

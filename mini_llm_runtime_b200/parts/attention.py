@@ -125,6 +125,9 @@ class GQAAttention(PagedAttention):
         numbers = batch.counts.get("shared")
         if numbers is None or self.window is not None or numbers["heads_per_kv"] != self.num_heads // self.num_kv_heads:
             return None
+        page_size = view.k_pool.shape[2]
+        if page_size < 8 or page_size & (page_size - 1):      # pages that the walk on the tensor cores does not take
+            return None
         if "shared_prefix" not in view.shared:
             head = "shared."
             view.shared["shared_prefix"] = SharedPrefix(

@@ -287,6 +287,50 @@ def test_prefixes_that_are_refused(tiny, kernels):
         none.add_prefix("p", tokens)
 
 
+def test_requests_and_prefixes_do_not_share_names(tiny, kernels):
+    engine = engine_of(tiny)
+    tokens = random_prompt(tiny.config.vocab_size, 40, 1)
+    engine.submit("prefix p", tokens, max_new_tokens=2)
+    with pytest.raises(ValueError, match="is called"):
+        engine.add_prefix("p", tokens)
+    engine.run()
+    engine.add_prefix("p", tokens)
+    engine.add_prefix("q", tokens)
+    with pytest.raises(ValueError, match="holds a prefix"):
+        engine.submit("prefix q", tokens, max_new_tokens=2)
+    engine.submit("b", tokens, max_new_tokens=2, prefix="p")
+    engine.run()
+    assert list(engine.scheduler.get_request("b").generated_token_ids) == plain_tokens(tiny, tokens, 2)
+
+
+def test_groups_too_small_for_lists_need_no_step_of_their_own(tiny, kernels, monkeypatch):
+    cache, runner = tiny.cache, tiny.runner
+    page = TINY["A"][1]
+    cache.create_request("p")
+    runner.step([StepEntry("p", random_prompt(tiny.config.vocab_size, 2 * page, 1))])
+    requests = [cache.create_request(name, prefix=("p", 2 * page)) for name in "abc"]
+    cache.begin_step([(request.request_id, 1) for request in requests])
+    assert runner._graph_key(requests, True, False)[4:] == ((3, 2 * page),)
+    monkeypatch.setattr(kernels, "shares_prefix", lambda dtype, counts, kv_heads, dim: counts["members"] > 2)
+    assert runner._graph_key(requests[:2], True, False)[4:] == ()
+    assert runner._graph_key(requests, True, False)[4:] == ((3, 2 * page),)
+    cache.abort_step()
+
+
+def test_pages_of_odd_sizes_take_no_shared_attention(kernels):
+    odd = TinyEngine(TINY["A"][0], 12, torch.float32, "cpu")
+    cache, runner = odd.cache, odd.runner
+    prefix = random_prompt(odd.config.vocab_size, 24, 1)
+    cache.create_request("p")
+    runner.step([StepEntry("p", prefix)])
+    for name in "ab":
+        cache.create_request(name, prefix=("p", 24))
+    got = runner.step([StepEntry(name, [token], [0]) for name, token in (("a", 3), ("b", 4))])
+    assert not kernels.shared_calls
+    for row, token in enumerate((3, 4)):
+        assert torch.allclose(got[row], odd.plain_logits(prefix + [token])[-1], atol=1e-4)
+
+
 def test_a_model_with_windows_has_no_prefixes(kernels):
     windowed = TinyEngine(*TINY["C"], torch.float32, "cpu")
     engine = engine_of(windowed, "C")
