@@ -476,6 +476,7 @@ class CudaOps:
         self.use_tma_attention = True
         self.use_fused_rope = True
         self.use_grouped_experts = True     # routed experts of many rows: sorted pairs through the grouped tcgen05 product
+        self._even_splits: dict[tuple, tuple[int, int]] = {}      # by the sizes of a decode step: see _even_split
         self.use_cluster_merge = True       # chunks of a decode row merge through a cluster's shared memory
         # bytes of keys and values that a shared prefix must save to be walked by itself (see shared_prefix_attention)
         self.shared_prefix_least = self.SHARED_PREFIX_LEAST
@@ -1145,8 +1146,8 @@ class CudaOps:
         """``paged_attention`` of a step of decoded tokens whose requests share leading pages: the keys and values of a prefix are
         read once for all its requests instead of once for each.  ``batch`` is the step as ``paged_attention`` takes it (a request's
         row of the block table names the shared pages as its first); ``prefix`` says which segments share how many keys.
-        Segments of no group attend by themselves.  Where sharing saves too little for it (``SHARED_PREFIX_LEAST``) the step goes
-        through ``paged_attention``."""
+        Segments of no group attend by themselves.  Where sharing saves too little for it (``SHARED_PREFIX_LEAST``) the step
+        takes the kernel of ``paged_attention``."""
         segments, counts, plan = batch.num_segments, prefix.counts, prefix.plan
         if num_kv_heads < 1 or num_heads < 1 or num_heads % num_kv_heads or not 1 <= head_dim <= 256:
             raise KernelError(f"{num_heads} heads over {num_kv_heads} kv heads of {head_dim} are not supported")
@@ -1162,8 +1163,6 @@ class CudaOps:
         page_size = k_pool.shape[2] if k_pool.dim() == 4 else 0
         fast = (self.use_mma_attention and q.dtype == torch.bfloat16 and head_dim in (64, 128) and num_heads // num_kv_heads <= 16
                 and page_size >= 8 and page_size & (page_size - 1) == 0)
-        if fast and segments > 0 and not self.shares_prefix(q.dtype, counts, num_kv_heads, head_dim):
-            return self.paged_attention(q, k_pool, v_pool, batch, num_heads, num_kv_heads, head_dim, scale, None)
         _need(k_pool, "k_pool", q.dtype, 4)
         _need(v_pool, "v_pool", q.dtype, 4)
         if q.shape[1] != num_heads * head_dim:
@@ -1171,11 +1170,16 @@ class CudaOps:
         if k_pool.shape != v_pool.shape or k_pool.shape[1] != num_kv_heads or k_pool.shape[3] != head_dim:
             raise KernelError(f"page pools have shapes {tuple(k_pool.shape)} and {tuple(v_pool.shape)}, expected "
                               f"[pages, {num_kv_heads}, page_size, {head_dim}]")
+        out = torch.empty_like(q)
         if segments == 0:
-            return torch.empty_like(q)
+            return out
+        if (fast and segments * num_kv_heads <= self.ATTENTION_COUNTERS and "decode_seg" in batch.plan
+                and not self.shares_prefix(q.dtype, counts, num_kv_heads, head_dim)):
+            # what paged_attention runs for such a step
+            self._decode_attention(q, k_pool, v_pool, out, batch, num_heads, num_kv_heads, head_dim, scale, None, mma=True)
+            return out
         fast = (fast and k_pool.shape[0] * num_kv_heads * page_size < 1 << 31
                 and not (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr()) % 16)
-        out = torch.empty_like(q)
         chunk, parts, units, own_parts = prefix_parts(counts["tile_keys"], counts["least_shared"], segments, batch.max_kv_len, num_heads,
                                                       num_kv_heads, head_dim, self.sm_count(q.device))
         states = (parts + own_parts) * segments * num_heads
@@ -1197,6 +1201,26 @@ class CudaOps:
             chunk *= 2
         return chunk, max(1, -(-longest // chunk))
 
+    def _even_split(self, pairs: int, longest: int, most_splits: int, sms: int, use_cluster_merge: bool) -> tuple[int, int]:
+        """(splits, chunks that merge through a cluster or 0) of a decode step with even chunks, for ``pairs`` of a request and a kv head."""
+        resident = self.TMA_CTAS_PER_SM * sms
+        pairs = max(1, pairs)
+        cluster = 0
+        # More (request, kv head) pairs than resident CTAs: whole contexts per CTA would leave a
+        # second, nearly empty wave; four chunks each even it out (14B sizes, 64 requests:
+        # 320 -> 305 us per layer; below that number of pairs, cutting further only costs).
+        wanted = resident // pairs if pairs <= resident else 4
+        splits = max(1, min(64, most_splits, wanted, -(-longest // self.TMA_MIN_CHUNK)))
+        # Up to 16 chunks can merge through their thread-block cluster's shared memory, which
+        # saves several microseconds of global round trips; worth fewer chunks of up to 768 keys.
+        for size in self.CLUSTER_SIZES:
+            if (use_cluster_merge and size <= splits and pairs <= self.clusters_together(size)
+                    and (size == splits or longest <= size * self.CLUSTER_MAX_CHUNK)):
+                cluster = size
+                if longest <= size * self.CLUSTER_CHUNK:
+                    break
+        return (cluster or splits), cluster
+
     def _decode_attention(self, q, k_pool, v_pool, out, batch, num_heads, num_kv_heads, head_dim, scale, window,
                           mma=False, rope=None):
         page_size = k_pool.shape[2]
@@ -1214,23 +1238,13 @@ class CudaOps:
         if even_split:
             # the kernel divides each request's context over `splits` chunks of at least `chunk` keys
             chunk = self.TMA_MIN_CHUNK
-            pairs = max(1, batch.num_decode * num_kv_heads)
-            resident = self.TMA_CTAS_PER_SM * sms
-            # More (request, kv head) pairs than resident CTAs: whole contexts per CTA would leave a
-            # second, nearly empty wave; four chunks each even it out (14B sizes, 64 requests:
-            # 320 -> 305 us per layer; below that number of pairs, cutting further only costs).
-            wanted = resident // pairs if pairs <= resident else 4
-            splits = max(1, min(64, most_splits, wanted, -(-batch.max_kv_len // chunk)))
-            # Up to 16 chunks can merge through their thread-block cluster's shared memory, which
-            # saves several microseconds of global round trips; worth fewer chunks of up to 768 keys.
-            for size in self.CLUSTER_SIZES:
-                if (self.use_cluster_merge and size <= splits and pairs <= self.clusters_together(size)
-                        and (size == splits or batch.max_kv_len <= size * self.CLUSTER_MAX_CHUNK)):
-                    cluster = size
-                    if batch.max_kv_len <= size * self.CLUSTER_CHUNK:
-                        break
-            if cluster:
-                splits = cluster
+            sizes = (batch.num_decode * num_kv_heads, batch.max_kv_len, most_splits, sms, self.use_cluster_merge)
+            planned = self._even_splits.get(sizes)
+            if planned is None:
+                if len(self._even_splits) >= 1 << 14:
+                    self._even_splits.clear()
+                planned = self._even_splits[sizes] = self._even_split(*sizes)
+            splits, cluster = planned
         else:
             chunk, splits = self.plan_decode(batch.num_decode, num_kv_heads, batch.max_kv_len, sms)
             if self.decode_chunk is not None:

@@ -221,8 +221,8 @@ def test_the_rule_of_small_savings(monkeypatch, dim):
     kernels = ops.current()
     saved = 4 * 3 * 512 * 2 * dim              # three of four requests spared 512 keys of two kv heads
     calls = []
-    paged = kernels.paged_attention
-    monkeypatch.setattr(kernels, "paged_attention", lambda *args: calls.append(1) or paged(*args))
+    decode = kernels._decode_attention
+    monkeypatch.setattr(kernels, "_decode_attention", lambda *args, **named: calls.append(1) or decode(*args, **named))
     for least, expected in ((saved, 0), (saved + 1, 1)):
         monkeypatch.setattr(kernels, "shared_prefix_least", least)
         step = Step([(4, 512)], 1, (9, 200, 1), 8, 2, dim, 16, torch.bfloat16, seed=dim)
