@@ -104,6 +104,22 @@ def test_no_rows():
     assert run(case, torch.empty(0, dtype=torch.int32, device=DEVICE)).shape == (0, 32)
 
 
+@pytest.mark.parametrize("rows", [2, 20, 300])
+def test_an_infinite_sum_stays_infinite(rows):
+    """x A^T infinite and B positive: infinity, not the NaN of an infinity taken from itself; the other rows are what they were."""
+    case = made(rows, 128, 1152, 16, 2, torch.bfloat16, 8)
+    ids = some_ids(rows, 2, "one", 1)
+    want = run(case, ids)
+    case["x"][1, 0] = float("inf")
+    case["weight"][:, 0], case["down"][:, :, 0], case["up"][:], case["scales"][:] = 0.5, 0.25, 0.125, 1.0
+    got = run(case, ids)
+    assert (got[1] == float("inf")).all()
+    case["x"][1, 0] = 0.0
+    again = run(case, ids)
+    others = torch.arange(rows, device=DEVICE) != 1
+    assert torch.equal(got[others], again[others]) and torch.isfinite(want).all()
+
+
 def test_what_other_adapters_hold_does_not_matter():
     """Infinities and NaN in adapters that no row of the batch uses, and in the rows of x that use none."""
     case = made(20, 128, 264, 16, 4, torch.bfloat16, 6)
