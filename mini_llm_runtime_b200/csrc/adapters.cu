@@ -16,8 +16,8 @@ namespace mlr {
 constexpr int DOWN_RANKS = 16;       // rank rows per CTA of the few-rows kernel
 constexpr int DOWN_WARPS = 4;
 constexpr int MOST_PARTS = 8;        // of K: CTAs of a cluster
-// Rows up to which every row reads its adapter by itself.  (16 ranks of 3,584 columns, each row an adapter of its own: 64 rows 8 us, 128 rows
-// as tiles 49; one adapter for 2,048 rows of 64 ranks as tiles 23.)
+// Rows up to which every row reads its adapter by itself.  (bfloat16, rows of many adapters, captured, us: 16 ranks of 896 columns 64 rows
+// 3.4, of 18,944 11.2 (25 MB, 2.2 TB/s); 128 rows as tiles 49; prompts as tiles: one adapter of 64 ranks for 2,048 rows of 3,584 columns 20.)
 constexpr int DOWN_ROWS = 128;
 constexpr int TILE_DOWN = 32;        // rows per CTA of the many-rows kernel
 
@@ -60,10 +60,10 @@ __device__ __forceinline__ void unpack(const uint4& raw, float* v, float) {
 // Both down kernels: `early` says that the kernel in front is the shared product of the same x, which lets the next kernel in
 // after its own wait: what is read here was complete then, and the sums are taken beside it; this kernel waits for it at its end.
 //
-// Few rows, each with an adapter of its own as a rule, and 32-bit rows: CTA = (ROWS neighbouring rows, 16 rank rows, part of K), bound
-// by reading A.  A warp walks its stretch of K 32 pieces of 16 bytes at a time and holds 16 sums of every row; rows of one
-// adapter (a prompt's) share what is read of it, others take turns.  The parts of K meet through the cluster's shared memory, in
-// order.  WIDE: rows are whole 16-byte pieces.
+// Few rows, each with an adapter of its own as a rule, and 32-bit rows: CTA = (ROWS neighbouring rows, 16 rank rows, part of K), bound by
+// reading A.  A warp walks its stretch of K 32 pieces of 16 bytes at a time and holds 16 sums of every row; rows of one adapter (a
+// prompt's) share what is read of it, others take turns (float32, 800 rows of 4,864 columns, rank 128: 54 us, each row by itself 157).
+// The parts of K meet through the cluster's shared memory, in order.  WIDE: rows are whole 16-byte pieces.
 template <typename T, int ROWS, bool WIDE>
 __global__ void __launch_bounds__(DOWN_WARPS * 32)
 adapter_down_rows_kernel(const T* x, const T* __restrict__ down, const float* __restrict__ scales, const int* row_adapter, float* u,
@@ -276,9 +276,10 @@ adapter_down_tile_kernel(const bf16* x, const bf16* __restrict__ down, const flo
   if (early) pdl_wait();
 }
 
-// Up: a thread owns one output column and ROWS rows; B's row of the column is read once per run of rows with one adapter, 16
-// ranks at a time, the next ones under way.  The first are asked for before the wait: which adapter a row has was complete
-// before the down kernel, in front of this one on the stream, let the kernels behind it in.
+// Up: a thread owns one output column and ROWS rows; B's row of the column is read once per run of rows with one adapter, 16 ranks at a
+// time, the next ones under way (64 rows of as many adapters, rank 16, N = 3,584: 4 us; rank 64, N = 9,728: 26 us, 80 MB).  The first are
+// asked for before the wait: which adapter a row has was complete before the down kernel, in front of this one on the stream, let the
+// kernels behind it in.
 template <typename T, typename Out, int ROWS, bool WIDE>
 __global__ void __launch_bounds__(128)
 adapter_up_kernel(const float* u, const T* __restrict__ up, const int* row_adapter, const float* base, Out* out, int rows, int adapters,

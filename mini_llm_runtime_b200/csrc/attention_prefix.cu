@@ -54,7 +54,9 @@ __device__ __forceinline__ const T* cached_row(const PrefixCall& c, const void* 
 // ------------------------------------------------------------------ any type, any head size up to 256
 constexpr int PLAIN_ROWS = 8, PLAIN_KEYS = 32, PLAIN_THREADS = 128;
 
-// CTA = (eight rows of an item, one part of its keys).  PREFIX: y is a tile of the prefixes, else a segment.
+// CTA = (eight rows of an item, one part of its keys).  PREFIX: y is a tile of the prefixes, else a segment.  Bound by the shared-memory reads of
+// its multiply-adds (a 32-bit word for each): float32, 8 requests with 14 heads of 64 over 2, 2,048 shared and 500 own keys 166 us, 32 with 28
+// heads of 128 over 4, 4,096 shared keys 530 us; each request by itself (the generic kernel of every other step) 1,032 and 7,906 us.
 template <typename T, bool PREFIX>
 __global__ void __launch_bounds__(PLAIN_THREADS)
 prefix_parts_plain_kernel(const PrefixCall c) {
@@ -155,11 +157,12 @@ prefix_parts_plain_kernel(const PrefixCall c) {
 }
 
 // ------------------------------------------------------------------ prefixes on tcgen05 (bfloat16, heads of 64 and 128)
-// One work item is 128 query rows of one kv head (the query heads of up to 128 / heads_per_kv requests) over one part of the
-// prefix: bound by the products once a few dozen requests share it, by its keys' bytes below.  Six warps: four of softmax, one
-// thread per query row (tensor-memory lane); one that issues S = Q K^T two key tiles ahead and O += P V; one that loads, K and V
-// page by page through bulk tensor copies into a ring.  The output stays in tensor memory relative to a base exponent that
-// follows the running max in steps of 2^8.  The query rows lie in the q of as many requests: the softmax threads gather them.
+// One work item is 128 query rows of one kv head (the query heads of up to 128 / heads_per_kv requests) over one part of the prefix: bound
+// by the softmax beside the products once a few dozen requests share it (70, 33 and 25 requests behind 16,384, 9,001 and 4,100 keys, 40
+// heads over 8: 58 us, tensor pipe 31 %, 0.67 us per 128 x 64 scores and SM), by its keys' bytes below.  Six warps: four of softmax, one
+// thread per query row (tensor-memory lane); one that issues S = Q K^T two key tiles ahead and O += P V; one that loads, K and V page by
+// page through bulk tensor copies into a ring.  The output stays in tensor memory relative to a base exponent that follows the running max
+// in steps of 2^8. The query rows lie in the q of as many requests: the softmax threads gather them.
 constexpr int PT_ROWS = 128, PT_KEYS = 64, PT_THREADS = 192;
 constexpr uint32_t PT_TMEM_COLS = 256, PT_TMEM_O = 2 * PT_KEYS;      // S0 | S1 | O
 constexpr int PT_P_BYTES = PT_ROWS * PT_KEYS * 2;
@@ -503,13 +506,13 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
 }
 
 // ------------------------------------------------------------------ own keys on mma.sync (bfloat16, heads of 64 and 128)
-// CTA = (request, part of its own keys, kv head): bound by reading them, each once.  Keys are the MMA's rows and the query heads
-// its eight columns (S^T = K Q^T, O^T = V^T P^T), so that the usual five to eight heads of a kv head fill them: half the
-// products and registers of heads as rows, and three CTAs per SM.  Four warps take 16 keys each of a 64-key tile; a fifth loads,
-// page by page through bulk tensor copies, as far ahead as the ring is deep (by asynchronous copies of the four warps each table
-// read stood in front of its copies: 68 MB of own keys took 72 us from cold caches).  The warps' states meet in shared memory.
-// AFTER_PREFIX: launched behind the prefix kernel, which lets the next kernel in after its own wait: everything before both is
-// done then, and what this kernel reads is written by neither; it starts beside the prefix kernel and waits for it at its end.
+// CTA = (request, part of its own keys, kv head): bound by reading them, each once (231 MB in 51 us, 4.5 TB/s).  Keys are the MMA's rows
+// and the query heads its eight columns (S^T = K Q^T, O^T = V^T P^T), so that the usual five to eight heads of a kv head fill them: half
+// the products and registers of heads as rows, and three CTAs per SM.  Four warps take 16 keys each of a 64-key tile; a fifth loads, page
+// by page through bulk tensor copies, as far ahead as the ring is deep (by asynchronous copies of the four warps each table read stood in
+// front of its copies: 68 MB of own keys took 72 us from cold caches).  The warps' states meet in shared memory.
+// AFTER_PREFIX: launched behind the prefix kernel, which lets the next kernel in after its own wait: everything before both is done then,
+// and what this kernel reads is written by neither; it starts beside the prefix kernel and waits for it at its end.
 constexpr int OWN_THREADS = 160;
 constexpr int FINISH_PARTS = 64;      // parts of a prefix, at most
 
@@ -790,8 +793,9 @@ prefix_own_mma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
 }
 
 // ------------------------------------------------------------------ the parts put together
-// One warp per (segment, head); a row that sees no key is zero.  W floats per lane and load (4 where rows are whole 16-byte
-// pieces); the states of up to 32 parts come with one load, the outputs of eight parts are in flight together.
+// One warp per (segment, head); a row that sees no key is zero.  Bound by the latency of its reads (64 requests, 28 heads of 128, up to 18
+// parts: 11 us from cold caches).  W floats per lane and load (4 where rows are whole 16-byte pieces); the states of up to 32 parts come
+// with one load, the outputs of eight parts are in flight together.
 template <typename T, int W>
 __global__ void __launch_bounds__(128)
 prefix_merge_kernel(const PrefixCall c) {

@@ -50,13 +50,13 @@ __device__ __forceinline__ float penalised(float x, int word, float repetition, 
   return made > 0 ? x - presence : x;
 }
 
-// A CTA takes a stretch of one row, 256 pieces of four logits (a portion) at a time.  What a token may need hangs together (slot,
-// then bits, then the words of known tokens), so three portions are under way: the bits of the one after next, the logits and
-// words of the next, the arithmetic of the present one.  (A CTA per portion lives through that chain, 4 us, for 16 KB: 64 x
-// 152,064 logits took 38 us, 256 x 151,936 124 us; with the words fetched where they are used 31 and 80; now 29 and 76, where a
-// copy of the same logits takes 18.5 and 55.)
-// Pieces lie on 16-byte boundaries.  WHOLE: the vocabulary is a multiple of four and every piece is one row's; else a row
-// starts inside a piece, and its first and last piece go entry by entry.
+// A CTA takes a stretch of one row, 256 pieces of four logits (a portion) at a time.  What a token may need hangs together (slot, then
+// bits, then the words of known tokens), so three portions are under way: the bits of the one after next, the logits and words of the
+// next, the arithmetic of the present one.  (A CTA per portion lives through that chain, 4 us, for 16 KB: 64 x 152,064 logits 36 us, 256 x
+// 151,936 94 us; as it stands 23 and 68, 4.75 TB/s, where a copy of the same logits takes 18.5 and 55 and the bytes alone 12.6 and 50. Few
+// rows are latency: a row of 151,936 4.1 us in a captured step, 8 from the host.)
+// Pieces lie on 16-byte boundaries.  WHOLE: the vocabulary is a multiple of four and every piece is one row's; else a row starts inside a
+// piece, and its first and last piece go entry by entry.
 // IN_PLACE: logits that no rule touches are neither read nor written.
 template <bool IN_PLACE, bool WHOLE>
 __global__ void __launch_bounds__(RULE_THREADS)
@@ -180,7 +180,8 @@ logit_rules_kernel(const float* logits, float* out, const int* row_slot, int voc
   }
 }
 
-// One thread per (slot, token) pair.  Sums of whole numbers: the order of the atomics changes nothing.
+// One thread per (slot, token) pair; sums of whole numbers: the order of the atomics changes nothing.  Bound by its launch: 64 pairs 0.9 us, 4,000
+// 1.2, calls one behind the other.
 __global__ void count_tokens_kernel(const int* tokens, const int* slots, int pairs, int* counts, unsigned* seen, int num_slots,
                                     int vocab, int prompt) {
   pdl_trigger();
@@ -198,7 +199,7 @@ __global__ void count_tokens_kernel(const int* tokens, const int* slots, int pai
 static void launch_rules(const float* logits, float* out, const int* row_slot, int rows, int vocab, const RuleTables& tables,
                          cudaStream_t stream) {
   // Up to four portions per CTA, as far as every SM still has eight CTAs (64 x 152,064 and 256 x 151,936 logits with one portion
-  // each 43 and 100 us, with four 29 and 76, with sixteen 37 and 78; a single row with one 8.2, with sixteen 18.5).
+  // each 36 and 94 us, with two 25 and 71, with four 23 and 68, with eight 25 and 70, with sixteen 24 and 72).
   constexpr int PORTION = RULE_THREADS * 4;
   const int portions = (vocab + 3 + PORTION - 1) / PORTION;
   const int each = (int)min(4ll, 1 + (long long)rows * portions / (8 * sm_count()));
