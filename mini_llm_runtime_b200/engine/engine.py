@@ -198,6 +198,13 @@ class ContinuousBatchEngine:
             portion = self.scheduler.max_batch_tokens
             for start in range(0, shared, portion):
                 self.runner.step([StepEntry(holder, tokens[start:min(shared, start + portion)])])
+            if self.manager.slot_state.is_cuda:
+                torch.cuda.synchronize(self.manager.slot_state.device)
+            try:
+                self.runner.check_device()
+            except ops.KernelError:
+                self._give_up_after_device_error(())
+                raise
         except BaseException:
             self.manager.release(holder)
             raise
@@ -313,7 +320,7 @@ class ContinuousBatchEngine:
             try:
                 self.runner.check_device()
             except ops.KernelError:
-                self._give_up_after_device_error(plan)
+                self._give_up_after_device_error([item.request_id for item in plan.items])
                 raise
             generated = {rid: generated[rid] for rid in plan.emitting_request_ids}   # drops rows of ended requests
         tokens_ready_ns = self._clock_ns()
@@ -326,13 +333,13 @@ class ContinuousBatchEngine:
         self.metrics.record_completed(outcome.finished_request_ids, completed_ns)
         return EngineStepResult(plan, outcome, started_ns, tokens_ready_ns, completed_ns)
 
-    def _give_up_after_device_error(self, plan: StepPlan) -> None:
+    def _give_up_after_device_error(self, request_ids: Sequence[str]) -> None:
         """A kernel reported that a bounded wait ran out: nothing computed since the last check can
         be trusted, and the cache already holds those steps' keys and values.  The requests of the
         step (and of the step launched ahead of it) end with ``FinishReason.ERROR`` and give their
         pages back; waiting requests and the engine itself stay usable."""
         with self._range("engine.rollback"):
-            touched = [item.request_id for item in plan.items]
+            touched = list(request_ids)
             if self._ahead is not None:
                 touched += [rid for rid in self._ahead.request_ids if rid not in touched]
                 self._ahead.wait()

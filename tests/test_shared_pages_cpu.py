@@ -264,6 +264,24 @@ def test_a_prefix_that_fails_gives_its_pages_back(tiny, kernels, monkeypatch):
     assert engine.manager.stats().live_requests == 0 and engine.manager.stats().free_pages == engine.manager.stats().total_pages
 
 
+def test_a_device_error_while_a_prefix_is_computed(tiny, kernels):
+    """Found at the end of ``add_prefix``, not by the requests that would start with it."""
+    engine = engine_of(tiny)
+    tokens = random_prompt(tiny.config.vocab_size, 40, 1)
+    engine.submit("a", tokens[:9], max_new_tokens=3)
+    engine.step()
+    kernels.error_code = 3
+    with pytest.raises(KernelError, match="bounded wait"):
+        engine.add_prefix("p", tokens)
+    assert list(engine.manager.requests) == ["a"]
+    engine.run()
+    assert list(engine.scheduler.get_request("a").generated_token_ids) == plain_tokens(tiny, tokens[:9], 3)
+    engine.add_prefix("p", tokens)
+    engine.submit("b", tokens, max_new_tokens=3, prefix="p")
+    engine.run()
+    assert list(engine.scheduler.get_request("b").generated_token_ids) == plain_tokens(tiny, tokens, 3)
+
+
 def test_prefixes_that_are_refused(tiny, kernels):
     engine = engine_of(tiny, max_prefixes=1)
     vocab = tiny.config.vocab_size

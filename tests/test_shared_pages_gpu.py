@@ -124,6 +124,28 @@ def test_the_engine_with_prefixes(name, dtype, step_ahead, shared_calls):
         assert [(o[0], len(o)) for o in outputs[0]] == [(o[0], len(o)) for o in outputs[1]]
 
 
+@pytest.mark.parametrize("step_ahead", [False, True])
+def test_a_prefix_that_comes_while_others_run(step_ahead, shared_calls):
+    config, page = CONFIGS["E"]
+    tiny = TinyEngine(config, page, torch.float32, "cuda:0")
+    prefix = random_prompt(config.vocab_size, 3 * page, 1)
+    others = [random_prompt(config.vocab_size, n, n) for n in (5, 20)]
+    outputs = []
+    for shared in (True, False):
+        engine = engine_of(tiny, page, step_ahead=step_ahead, max_prefixes=1)
+        for i, other in enumerate(others):
+            engine.submit(f"o{i}", other, max_new_tokens=20)
+        for _ in range(6):
+            engine.step()
+        if shared:
+            engine.add_prefix("late", prefix)
+        for i in range(2):
+            engine.submit(f"s{i}", prefix + [i + 1], max_new_tokens=9, prefix="late" if shared else None)
+        engine.run()
+        outputs.append([list(engine.scheduler.get_request(name).generated_token_ids) for name in ("o0", "o1", "s0", "s1")])
+    assert outputs[0] == outputs[1]
+
+
 def test_below_the_rule_decode_steps_stay_as_they_were(monkeypatch):
     """Prefixes that save little: the fused decode attention, on shared pages."""
     config, page = CONFIGS["E"]
