@@ -163,9 +163,9 @@ prefix_parts_plain_kernel(const PrefixCall c) {
 // thread per query row (tensor-memory lane); one that issues S = Q K^T two key tiles ahead and O += P V; one that loads, K and V page by
 // page through bulk tensor copies into a ring.  The output stays in tensor memory relative to a base exponent that follows the running max
 // in steps of 2^8. The query rows lie in the q of as many requests: the softmax threads gather them.
-constexpr int PT_ROWS = 128, PT_KEYS = 64, PT_THREADS = 192;
-constexpr uint32_t PT_TMEM_COLS = 256, PT_TMEM_O = 2 * PT_KEYS;      // S0 | S1 | O
-constexpr int PT_P_BYTES = PT_ROWS * PT_KEYS * 2;
+constexpr int PT_ROWS = 128, PT_KEYS = 64, PT_SOFTMAX = 256, PT_THREADS = PT_SOFTMAX + 64;
+constexpr int PT_MMA_WARP = PT_SOFTMAX / 32, PT_LOAD_WARP = PT_MMA_WARP + 1, PT_HALF = PT_KEYS / 2;
+constexpr uint32_t PT_TMEM_COLS = 256, PT_TMEM_O = 2 * PT_KEYS;      // S0 | S1, which their probabilities replace | O
 constexpr float PT_LAZY = 8.f;
 
 template <int D>
@@ -174,20 +174,18 @@ struct PrefixShape {
   static constexpr int STAGES = D == 64 ? 4 : 2;
   static constexpr int Q_BYTES = PT_ROWS * D * 2, Q_HALF = PT_ROWS * 128;
   static constexpr int TILE_BYTES = PT_KEYS * D * 2, HALF = PT_KEYS * 128, STAGE_BYTES = 2 * TILE_BYTES;
-  static constexpr int DATA_BYTES = Q_BYTES + PT_P_BYTES + STAGES * STAGE_BYTES;
+  static constexpr int DATA_BYTES = Q_BYTES + STAGES * STAGE_BYTES;
 };
 
 struct PrefixControl {
   uint64_t q_full, k_full[4], v_full[4], qk_done[4], pv_done[4], p_ready;
   uint32_t tmem_holder;
+  float half_max[2][2][PT_ROWS];      // of tiles in turn: the largest score of either half of a row's keys
 };
 
-constexpr int PT_CONTROL_BYTES = 256;
+constexpr int PT_CONTROL_BYTES = 2304;
 static_assert(sizeof(PrefixControl) <= PT_CONTROL_BYTES, "control block");
-// Two CTAs share the 228 KB of an SM, of which each costs 1 KB by itself: 768 bytes are left for the alignment of the tiles (the
-// buffer starts on a 1,024-byte boundary where a kernel has no other shared memory).  With 1,024 there was one CTA per SM:
-// 2.5 us instead of 1.3 for two key tiles.
-template <int D> constexpr int PT_SHARED = PrefixShape<D>::DATA_BYTES + PT_CONTROL_BYTES + 512;
+template <int D> constexpr int PT_SHARED = PrefixShape<D>::DATA_BYTES + PT_CONTROL_BYTES + 1024;
 static_assert(2 * (PT_SHARED<128> + 1024) <= 228 * 1024, "two CTAs per SM");
 
 template <int D>
@@ -202,8 +200,7 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
     if (threadIdx.x == 0) atomicCAS(error_word, 0, 0x70);
     return;
   }
-  uint8_t* p_tile = q_tile + Shape::Q_BYTES;                                             // [128][64]
-  uint8_t* ring = p_tile + PT_P_BYTES;                                                   // stages of (K, V), each [halves][64][64]
+  uint8_t* ring = q_tile + Shape::Q_BYTES;                                               // stages of (K, V), each [halves][64][64]
   PrefixControl& ctl = *reinterpret_cast<PrefixControl*>(ring + STAGES * Shape::STAGE_BYTES);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -233,12 +230,12 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
   const int begin = part * c.chunk, end = min(keys, begin + c.chunk);
   const int first_member = c.tile_first[tile];
   if (threadIdx.x == 0) {
-    mbar_init(&ctl.q_full, 4);
+    mbar_init(&ctl.q_full, PT_SOFTMAX / 32);
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&ctl.k_full[s], 1); mbar_init(&ctl.qk_done[s], 1);
       mbar_init(&ctl.v_full[s], 1); mbar_init(&ctl.pv_done[s], 1);
     }
-    mbar_init(&ctl.p_ready, 4);
+    mbar_init(&ctl.p_ready, PT_SOFTMAX / 32);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
@@ -254,17 +251,17 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
   };
   const int per = c.heads / c.kv_heads;
   const int rows = c.tile_count[tile] * per;
-  // softmax threads: the row's segment and head, and where its q stands
-  const int r = threadIdx.x;
+  // softmax threads: the row's segment and head, and where its q stands; warps w and w + 4 share the rows
+  const int r = threadIdx.x & (PT_ROWS - 1);
   const bool live = r < rows;
   const int segment = live ? c.members[first_member + r / per] : 0, head = kv_head * per + r % per;
   const int q_at = live ? c.q_row[segment] * c.heads + head : -1;      // in units of a head
   int first_pages[STAGES + 2];
-  if (warp == 5) {
+  if (warp == PT_LOAD_WARP) {
 #pragma unroll
     for (int j = 0; j < STAGES + 2; ++j) first_pages[j] = lookup(j);
   }
-  if (warp == 4) {
+  if (warp == PT_MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_holder)), "r"(PT_TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -277,7 +274,7 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
 
   bool gave_up = false;
 
-  if (warp == 5) {
+  if (warp == PT_LOAD_WARP) {
     // ------------------------------------------------------------ loads
     auto load = [&](int j, int page, bool values) {
       const int stage = j % STAGES;
@@ -309,13 +306,13 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
       pages[1] = pages[2];
       pages[2] = after;
     }
-  } else if (warp == 4) {
+  } else if (warp == PT_MMA_WARP) {
     // ------------------------------------------------------------ MMAs
     constexpr uint32_t idesc_qk = fa_idesc(PT_ROWS, PT_KEYS, false);
     constexpr uint32_t idesc_pv = fa_idesc(PT_ROWS, D, true);
     const uint64_t q_desc = fa_desc_k_major(smem_u32(q_tile)), k_desc0 = fa_desc_k_major(smem_u32(ring));
-    const uint64_t v_desc0 = fa_desc_mn_major(smem_u32(ring) + Shape::TILE_BYTES, Shape::HALF), p_desc = fa_desc_k_major(smem_u32(p_tile));
-    auto issue_qk = [&](int j) {      // the score buffer j & 1 is free: tile j - 2's scores were read before its probabilities arrived
+    const uint64_t v_desc0 = fa_desc_mn_major(smem_u32(ring) + Shape::TILE_BYTES, Shape::HALF);
+    auto issue_qk = [&](int j) {      // the columns j & 1 are free: the product with tile j - 2's probabilities is in front of this one
       const int stage = j % STAGES;
       fa_wait(&ctl.k_full[stage], (unsigned)(j / STAGES) & 1u, error_word, 0x72, gave_up);
       gave_up = __any_sync(0xffffffffu, gave_up);
@@ -343,35 +340,36 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
         const uint64_t v_desc = v_desc0 + (uint64_t)((stage * Shape::STAGE_BYTES) >> 4);
 #pragma unroll
         for (int k = 0; k < PT_KEYS / 16; ++k)
-          fa_mma(tmem_base + PT_TMEM_O, p_desc + (uint64_t)((k * 32) >> 4), v_desc + (uint64_t)((k * 2048) >> 4), idesc_pv,
-                 (j > 0 || k > 0) ? 1u : 0u);
+          fa_mma_tmem(tmem_base + PT_TMEM_O, tmem_base + (j & 1) * PT_KEYS + k * 8, v_desc + (uint64_t)((k * 2048) >> 4), idesc_pv,
+                      (j > 0 || k > 0) ? 1u : 0u);
         fa_commit(&ctl.pv_done[stage]);
       }
       __syncwarp();
       if (j + 2 < tiles) issue_qk(j + 2);
     }
   } else {
-    // ------------------------------------------------------------ softmax, one thread per query row
+    // ------------------------------------------------------------ softmax, two threads per query row: 32 keys of a tile each
+    const int quarter = warp & 3, side = warp >> 2;
     {
-      // a warp's 32 rows, whole rows at a time (a row per lane would touch 32 lines with every load: 4.4 us instead of 1.5)
-      constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;      // lanes per row, rows per load
-      uint4 piece[LANES];
+      // a warp's 16 of 32 rows, whole rows at a time (a row per lane would touch 32 lines with every load: 4.4 us instead of 1.5)
+      constexpr int LANES = D / 8, AT_ONCE = 32 / LANES, LOADS = LANES / 2;      // lanes per row, rows per load
+      uint4 piece[LOADS];
 #pragma unroll
-      for (int i = 0; i < LANES; ++i) {
-        const int at = __shfl_sync(0xffffffffu, q_at, i * AT_ONCE + lane / LANES);
+      for (int i = 0; i < LOADS; ++i) {
+        const int at = __shfl_sync(0xffffffffu, q_at, side * 16 + i * AT_ONCE + lane / LANES);
         piece[i] = at >= 0 ? __ldcg(reinterpret_cast<const uint4*>((const bf16*)c.q + (size_t)at * D) + lane % LANES) : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
-      for (int i = 0; i < LANES; ++i) {
-        const int row = warp * 32 + i * AT_ONCE + lane / LANES, chunk = lane % LANES;
+      for (int i = 0; i < LOADS; ++i) {
+        const int row = quarter * 32 + side * 16 + i * AT_ONCE + lane / LANES, chunk = lane % LANES;
         *reinterpret_cast<uint4*>(q_tile + (chunk >> 3) * Shape::Q_HALF + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = piece[i];
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.q_full);
     }
-    const uint32_t lane_base = tmem_base + ((uint32_t)(warp * 32) << 16);
-    const bool warp_live = warp * 32 < rows;      // a warp of no rows only keeps the barriers going
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const bool warp_live = quarter * 32 < rows;      // a warp of no rows only keeps the barriers going
     float m_run = -INFINITY, m_base = -INFINITY, l = 0.f;
     const float2 scale2 = make_float2(c.scale_log2, c.scale_log2);
     for (int j = 0; j < tiles; ++j) {
@@ -379,27 +377,35 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
       const bool ragged = key0 + PT_KEYS > end;
       fa_wait(&ctl.qk_done[stage], (unsigned)(j / STAGES) & 1u, error_word, 0x76, gave_up);
       fa_fence_after();
-      float s[PT_KEYS];
+      const uint32_t scores = lane_base + (j & 1) * PT_KEYS;
+      float s[PT_HALF];
       bool step = false;
       float alpha = 1.f;
       if (warp_live) {
+        const int mine = key0 + side * PT_HALF;      // this thread's first key
 #pragma unroll
-        for (int i = 0; i < PT_KEYS; i += 16) fa_tmem_load16(lane_base + (j & 1) * PT_KEYS + i, reinterpret_cast<uint32_t*>(s) + i);
+        for (int i = 0; i < PT_HALF; i += 16)
+          fa_tmem_load16(scores + side * PT_HALF + i, reinterpret_cast<uint32_t*>(s) + i);
         fa_tmem_wait_ld();
         fa_fence_before();
         if (ragged) {
 #pragma unroll
-          for (int i = 0; i < PT_KEYS; ++i)
-            if (key0 + i >= end) s[i] = -INFINITY;
+          for (int i = 0; i < PT_HALF; ++i)
+            if (mine + i >= end) s[i] = -INFINITY;
         }
         float part_max[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int i = 4; i < PT_KEYS - 4; i += 8)
+        for (int i = 4; i < PT_HALF - 4; i += 8)
 #pragma unroll
           for (int e = 0; e < 4; ++e) part_max[e] = fa_max3(part_max[e], s[i + 2 * e], s[i + 2 * e + 1]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) part_max[e] = fmaxf(part_max[e], s[PT_KEYS - 4 + e]);
-        const float tile_max = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
+        for (int e = 0; e < 4; ++e) part_max[e] = fmaxf(part_max[e], s[PT_HALF - 4 + e]);
+        float tile_max = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
+        // the row's, with the other half's (two places in turn: the tile after next comes behind the next one's barrier)
+        ctl.half_max[j & 1][side][r] = tile_max;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+        fa_fence_after();
+        tile_max = fmaxf(tile_max, ctl.half_max[j & 1][side ^ 1][r]);
         m_run = fmaxf(m_run, tile_max * c.scale_log2);
         step = m_run - m_base > PT_LAZY;          // nothing seen yet: NaN, no step
         alpha = step ? fa_exp2(m_base - m_run) : 1.f;
@@ -408,7 +414,7 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
         const float2 minus_base = make_float2(-base, -base);
         float2 part_sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int i = 0; i < PT_KEYS; i += 8)
+        for (int i = 0; i < PT_HALF; i += 8)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float2 x = __ffma2_rn(make_float2(s[i + 2 * e], s[i + 2 * e + 1]), scale2, minus_base);
@@ -417,7 +423,7 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
             part_sum[e] = __fadd2_rn(part_sum[e], make_float2(s[i + 2 * e], s[i + 2 * e + 1]));
           }
         const float2 sum2 = __fadd2_rn(__fadd2_rn(part_sum[0], part_sum[1]), __fadd2_rn(part_sum[2], part_sum[3]));
-        l = fmaf(l, alpha, sum2.x + sum2.y);
+        l = fmaf(l, alpha, sum2.x + sum2.y);      // of this thread's keys
       }
       const bool rescale = j > 0 && __any_sync(0xffffffffu, step);
       if (j > 0) {      // the previous tile's P V: it has read the probabilities, and the output may be touched
@@ -427,7 +433,7 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
       if (rescale) {
         const float2 alpha2 = make_float2(alpha, alpha);
 #pragma unroll
-        for (int d0 = 0; d0 < D; d0 += 32) {
+        for (int d0 = side * (D / 2); d0 < (side + 1) * (D / 2); d0 += 32) {
           float o[32];
           fa_tmem_load16(lane_base + PT_TMEM_O + d0, reinterpret_cast<uint32_t*>(o));
           fa_tmem_load16(lane_base + PT_TMEM_O + d0 + 16, reinterpret_cast<uint32_t*>(o) + 16);
@@ -446,60 +452,58 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
       if (ragged) {      // what stands behind the last key becomes zero: a weight of zero times NaN is NaN
         fa_wait(&ctl.v_full[stage], (unsigned)(j / STAGES) & 1u, error_word, 0x78, gave_up);
         uint8_t* v_tile = ring + (size_t)stage * Shape::STAGE_BYTES + Shape::TILE_BYTES;
-        for (int i = threadIdx.x; i < PT_KEYS * 8 * Shape::HALVES; i += 128) {
+        for (int i = threadIdx.x; i < PT_KEYS * 8 * Shape::HALVES; i += PT_SOFTMAX) {
           const int half = i / (PT_KEYS * 8), within = i - half * (PT_KEYS * 8);
           if (key0 + (within >> 3) >= end)
             *reinterpret_cast<uint4*>(v_tile + half * Shape::HALF + (within >> 3) * 128 + (within & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
         }
       }
-      if (warp_live || j == 0) {      // rows past the last are zeros, written once
-        uint8_t* p_row = p_tile + r * 128;
+      if (warp_live) {      // where the row's scores were, which both its threads have read; other rows' outputs are not written
+        uint32_t packed[PT_HALF / 2];
 #pragma unroll
-        for (int chunk = 0; chunk < 8; ++chunk) {
-          uint32_t packed[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) packed[e] = warp_live ? pack_bf16(s[chunk * 8 + 2 * e], s[chunk * 8 + 2 * e + 1]) : 0u;
-          *reinterpret_cast<uint4*>(p_row + ((chunk ^ (r & 7)) << 4)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-        }
+        for (int e = 0; e < PT_HALF / 2; ++e) packed[e] = pack_bf16(s[2 * e], s[2 * e + 1]);
+        fa_tmem_store16(scores + side * (PT_HALF / 2), packed);
+        fa_tmem_wait_st();
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (ragged) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the zeros, for the product
       fa_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.p_ready);
     }
     fa_wait(&ctl.pv_done[(tiles - 1) % STAGES], (unsigned)((tiles - 1) / STAGES) & 1u, error_word, 0x79, gave_up);
     fa_fence_after();
-    // The output rows through shared memory, so that a warp writes whole rows (a row per lane: 3.7 us, now 2).  All products
-    // of this CTA are done: the warp takes its share of the probabilities' and the ring's space.
+    // The output rows through shared memory, so that a warp writes 128 bytes of a row together (a row per lane: 3.7 us, so 2).  All
+    // products of this CTA are done: the warp takes its share of the ring's space.
     const int at = live ? segment * c.heads + head : -1;
-    constexpr int PITCH = D + 4;
-    static_assert(4 * 32 * PITCH * 4 <= PT_P_BYTES + STAGES * Shape::STAGE_BYTES, "the rows fit behind the queries");
-    float* mine = reinterpret_cast<float*>(p_tile) + warp * 32 * PITCH;
-    asm volatile("bar.sync 1, 128;" ::: "memory");      // every warp's last wait is behind it
+    constexpr int PITCH = 32 + 4;
+    static_assert(PT_SOFTMAX * PITCH * 4 <= Shape::DATA_BYTES, "the rows fit");
+    float* mine = reinterpret_cast<float*>(ring) + warp * 32 * PITCH;
+    if (side == 1) ctl.half_max[tiles & 1][1][r] = l;   // the row's sum: that of both halves
+    asm volatile("bar.sync 5, 256;" ::: "memory");      // every warp's last wait is behind it
 #pragma unroll
-    for (int d0 = 0; d0 < D; d0 += 32) {
+    for (int d0 = side * (D / 2); d0 < (side + 1) * (D / 2); d0 += 32) {
       float o[32];
       fa_tmem_load16(lane_base + PT_TMEM_O + d0, reinterpret_cast<uint32_t*>(o));
       fa_tmem_load16(lane_base + PT_TMEM_O + d0 + 16, reinterpret_cast<uint32_t*>(o) + 16);
       fa_tmem_wait_ld();
 #pragma unroll
       for (int e = 0; e < 32; e += 4)
-        *reinterpret_cast<float4*>(mine + lane * PITCH + d0 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        *reinterpret_cast<float4*>(mine + lane * PITCH + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+      __syncwarp();
+      float* acc = c.acc + (size_t)part * c.segments * c.heads * D + d0 + lane % 8 * 4;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = i * 4 + lane / 8, to = __shfl_sync(0xffffffffu, at, row);
+        if (to >= 0) *reinterpret_cast<float4*>(acc + (size_t)to * D) = *reinterpret_cast<const float4*>(mine + row * PITCH + lane % 8 * 4);
+      }
+      __syncwarp();
     }
-    __syncwarp();
-    float* acc = c.acc + (size_t)part * c.segments * c.heads * D;
-    constexpr int LANES = D / 4, AT_ONCE = 32 / LANES;
-#pragma unroll 8
-    for (int i = 0; i < 32 / AT_ONCE; ++i) {
-      const int row = i * AT_ONCE + lane / LANES, to = __shfl_sync(0xffffffffu, at, row);
-      if (to >= 0) *reinterpret_cast<float4*>(acc + (size_t)to * D + lane % LANES * 4) = *reinterpret_cast<const float4*>(mine + row * PITCH + lane % LANES * 4);
-    }
-    if (live)
-      *reinterpret_cast<float2*>(c.state + 2 * ((size_t)part * c.segments * c.heads + at)) = make_float2(m_base, l);
+    if (live && side == 0)
+      *reinterpret_cast<float2*>(c.state + 2 * ((size_t)part * c.segments * c.heads + at)) = make_float2(m_base, l + ctl.half_max[tiles & 1][1][r]);
     fa_fence_before();
   }
   __syncthreads();
-  if (warp == 4) {
+  if (warp == PT_MMA_WARP) {
     fa_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(PT_TMEM_COLS) : "memory");
   }
