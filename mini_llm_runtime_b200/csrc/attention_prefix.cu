@@ -163,8 +163,8 @@ prefix_parts_plain_kernel(const PrefixCall c) {
 // thread per query row (tensor-memory lane); one that issues S = Q K^T two key tiles ahead and O += P V; one that loads, K and V page by
 // page through bulk tensor copies into a ring.  The output stays in tensor memory relative to a base exponent that follows the running max
 // in steps of 2^8. The query rows lie in the q of as many requests: the softmax threads gather them.
-constexpr int PT_ROWS = 128, PT_KEYS = 64, PT_SOFTMAX = 256, PT_THREADS = PT_SOFTMAX + 64;
-constexpr int PT_MMA_WARP = PT_SOFTMAX / 32, PT_LOAD_WARP = PT_MMA_WARP + 1, PT_HALF = PT_KEYS / 2;
+constexpr int PT_ROWS = 128, PT_KEYS = 64, PT_SOFTMAX = 256, PT_THREADS = PT_SOFTMAX + 96;
+constexpr int PT_MMA_WARP = PT_SOFTMAX / 32, PT_LOAD_WARP = PT_MMA_WARP + 1 /* keys; values one on */, PT_HALF = PT_KEYS / 2;
 constexpr uint32_t PT_TMEM_COLS = 256, PT_TMEM_O = 2 * PT_KEYS;      // S0 | S1, which their probabilities replace | O
 constexpr float PT_LAZY = 8.f;
 
@@ -257,7 +257,7 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
   const int segment = live ? c.members[first_member + r / per] : 0, head = kv_head * per + r % per;
   const int q_at = live ? c.q_row[segment] * c.heads + head : -1;      // in units of a head
   int first_pages[STAGES + 2];
-  if (warp == PT_LOAD_WARP) {
+  if (warp >= PT_LOAD_WARP) {
 #pragma unroll
     for (int j = 0; j < STAGES + 2; ++j) first_pages[j] = lookup(j);
   }
@@ -274,10 +274,12 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
 
   bool gave_up = false;
 
-  if (warp == PT_LOAD_WARP) {
-    // ------------------------------------------------------------ loads
-    auto load = [&](int j, int page, bool values) {
+  if (warp >= PT_LOAD_WARP) {
+    // ------------------------------------------------------------ loads: keys by one warp, values by another
+    const bool values = warp > PT_LOAD_WARP;
+    auto load = [&](int j, int page) {
       const int stage = j % STAGES;
+      // a stage of keys is free once the scores that read it exist, one of values once its product is done
       if (j >= STAGES) fa_wait(values ? &ctl.pv_done[stage] : &ctl.qk_done[stage], (unsigned)(j / STAGES - 1) & 1u, error_word, 0x71, gave_up);
       gave_up = __any_sync(0xffffffffu, gave_up);
       if (gave_up) return;
@@ -291,20 +293,15 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
         tma_load_2d(values ? &v_map : &k_map, full, dst, half * 64, (page * c.kv_heads + kv_head) * c.page_size + offset);
       }
     };
-    // In the order in which the MMA warp frees the stages: a K stage once the scores that read it exist, and they run two tiles
-    // ahead of the softmax; a V stage once its product is done.  pages: of tiles j + STAGES - 1, + 1 and + 2
-    int pages[3] = {first_pages[STAGES - 1], first_pages[STAGES], first_pages[STAGES + 1]};
 #pragma unroll
     for (int j = 0; j < STAGES; ++j)
-      if (j < tiles) { load(j, first_pages[j], false); load(j, first_pages[j], true); }
-    if (STAGES < tiles) load(STAGES, pages[1], false);
-    for (int j = 0; j < tiles; ++j) {
-      const int after = lookup(j + STAGES + 2);
-      if (j >= 1 && j + STAGES - 1 < tiles) load(j + STAGES - 1, pages[0], true);
-      if (j + STAGES + 1 < tiles) load(j + STAGES + 1, pages[2], false);
+      if (j < tiles) load(j, first_pages[j]);
+    int pages[2] = {first_pages[STAGES], first_pages[STAGES + 1]};      // of tiles j and j + 1
+    for (int j = STAGES; j < tiles; ++j) {
+      const int after = lookup(j + 2);
+      load(j, pages[0]);
       pages[0] = pages[1];
-      pages[1] = pages[2];
-      pages[2] = after;
+      pages[1] = after;
     }
   } else if (warp == PT_MMA_WARP) {
     // ------------------------------------------------------------ MMAs
