@@ -157,12 +157,15 @@ prefix_parts_plain_kernel(const PrefixCall c) {
 }
 
 // ------------------------------------------------------------------ prefixes on tcgen05 (bfloat16, heads of 64 and 128)
-// One work item is 128 query rows of one kv head (the query heads of up to 128 / heads_per_kv requests) over one part of the prefix: bound
-// by the softmax beside the products once a few dozen requests share it (70, 33 and 25 requests behind 16,384, 9,001 and 4,100 keys, 40
-// heads over 8: 58 us, tensor pipe 31 %, 0.67 us per 128 x 64 scores and SM), by its keys' bytes below.  Six warps: four of softmax, one
-// thread per query row (tensor-memory lane); one that issues S = Q K^T two key tiles ahead and O += P V; one that loads, K and V page by
-// page through bulk tensor copies into a ring.  The output stays in tensor memory relative to a base exponent that follows the running max
-// in steps of 2^8. The query rows lie in the q of as many requests: the softmax threads gather them.
+// One work item is 128 query rows of one kv head (the query heads of up to 128 / heads_per_kv requests) over one part of the prefix.
+// Bound by its softmax once a few dozen requests share the prefix, by the keys' bytes below: 70, 33 and 25 requests behind 16,384, 9,001 and
+// 4,100 keys, 40 heads of 128 over 8, 54 us; a CTA's tile of 64 keys takes 1,450 cycles, 690 of them exponentials (two CTAs on an SM), its
+// products 700.  Eleven warps: eight of softmax, two threads per query row (tensor-memory lane), 32 keys of a tile each, which lend each
+// other their largest score; one that issues S = Q K^T two key tiles ahead and O += P V, P in tensor memory where S was; one that loads K and
+// one that loads V, page by page through bulk tensor copies into a ring (one warp for both, sixteen copies per tile with pages of 16 keys, was
+// the limit before: 58 us).  The output stays in tensor memory relative to a base exponent that follows the running max in steps of 2^8.
+// The query rows lie in the q of as many requests: the softmax threads gather them.  (One thread per row with P in shared memory: 2,020
+// cycles per tile.  Q in tensor memory too leaves room for one tile's scores: 2,180, softmax and products in turn.)
 constexpr int PT_ROWS = 128, PT_KEYS = 64, PT_SOFTMAX = 256, PT_THREADS = PT_SOFTMAX + 96;
 constexpr int PT_MMA_WARP = PT_SOFTMAX / 32, PT_LOAD_WARP = PT_MMA_WARP + 1 /* keys; values one on */, PT_HALF = PT_KEYS / 2;
 constexpr uint32_t PT_TMEM_COLS = 256, PT_TMEM_O = 2 * PT_KEYS;      // S0 | S1, which their probabilities replace | O
