@@ -231,6 +231,7 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
     part -= __shfl_sync(0xffffffffu, upto, 31);
   }
   const int begin = part * c.chunk, end = min(keys, begin + c.chunk);
+  if (begin >= end) { pdl_wait(); return; }      // no such part: lists that do not belong to the launch
   const int first_member = c.tile_first[tile];
   if (threadIdx.x == 0) {
     mbar_init(&ctl.q_full, PT_SOFTMAX / 32);

@@ -1129,11 +1129,12 @@ class CudaOps:
     def plan_shared_prefix(self, groups, num_segments, heads_per_kv):
         return plan_shared_prefix(groups, num_segments, heads_per_kv)
 
-    # Prefixes that save less go through paged_attention, which reads them once per request, most of it from L2, in one launch instead of
-    # three.  Captured steps, us, shared / paged, by bytes saved: 14 heads of 64, 8 x 2,048 keys (7 MB) 10.4 / 7.2, 32 x 2,048 (32 MB) 11.1 /
-    # 9.6, 16 x 8,192 (63 MB) 14.4 / 14.5, 64 x 2,048 (66 MB) 11.4 / 13.2, 64 x 8,192 (264 MB) 21.4 / 28.1; 28 heads of 128, 2 x 8,192
-    # (17 MB) 16.0 / 15.2, 32 x 512 (32 MB) 11.9 / 12.3, 4 x 8,192 (50 MB) 17.1 / 16.1, 64 x 512 (66 MB) 13.5 / 16.7, 64 x 8,192 (1 GB) 29 / 127;
-    # 40 heads of 128, 2 x 8,192 (33 MB) 17.1 / 15.7, 8 x 2,048 (59 MB) 12.4 / 13.2, 64 x 8,192 (2 GB) 37 / 181.
+    # Prefixes that save less go through paged_attention's kernel, which reads them once per request, most of it from L2, in one launch
+    # instead of two or three (and which a layer's rotation can share, another launch).  Captured steps, us, shared / paged, by bytes saved: 14 heads
+    # of 64 over 2, 8 x 2,048 keys (7 MB) 9.7 / 7.3, 32 x 2,048 (32 MB) 10.2 / 9.3, 16 x 8,192 (63 MB) 13.0 / 14.6, 64 x 2,048 (66 MB) 10.3 / 13.2,
+    # 64 x 8,192 (264 MB) 19 / 28; 28 heads of 128 over 4, 2 x 8,192 (17 MB) 15.6 / 14.9, 8 x 2,048 (29 MB) 11.3 / 12.1, 32 x 512 (32 MB) 11.1 /
+    # 12.3, 4 x 8,192 (50 MB) 14.2 / 15.7, 64 x 512 (66 MB) 13.5 / 16.7, 64 x 8,192 (1 GB) 25 / 126; 40 heads of 128 over 8, 2 x 8,192 (33 MB) 13.0 /
+    # 15.6, 8 x 2,048 (59 MB) 9.8 / 13.2, 64 x 8,192 (2 GB) 33 / 181.  From the host 21 / 17 where neither's kernels take longer.
     SHARED_PREFIX_LEAST = 48 << 20
 
     def shares_prefix(self, dtype: torch.dtype, counts: dict, num_kv_heads: int, head_dim: int) -> bool:
