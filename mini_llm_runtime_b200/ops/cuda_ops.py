@@ -978,33 +978,32 @@ class CudaOps:
                 rows, N, K, count, rank, int(out_dtype == torch.float32), self._error_word(x.device).data_ptr(), _raw_stream()),
                 "linear_adapters (tcgen05)")
             return out
-        # The shared product's sums in 32 bits behind the small sums, in one piece of memory (the result itself where it is in 32 bits).
-        head = -(-rows * rank // 4) * 4
-        if out_dtype == torch.float32:
-            low, out = x.new_empty(head, dtype=torch.float32), x.new_empty((rows, N), dtype=torch.float32)
-            low_at, base_at = low.data_ptr(), out.data_ptr()
-        else:
-            low, out = x.new_empty(head + rows * N, dtype=torch.float32), x.new_empty((rows, N), dtype=out_dtype)
-            low_at = low.data_ptr()
-            base_at = low_at + 4 * head
-        route, product, space, scratch, counters = 0, None, self._workspace(x.device), None, None
-        scratch_bytes = counters_len = 0
+        route, product, space, scratch_at, counters = 0, None, self._workspace(x.device), None, None
+        scratch_bytes = counters_len = behind = 0
         if self.use_tensor_cores and aligned:
             if x.dtype == torch.bfloat16 and K % 8 == 0:
                 if self._skinny_fits(x, weight):
                     route, product = 1, _entry("gemm_skinny", "mlr_gemm_skinny")
                 else:
                     route, product, scratch, counters = 2, _entry("gemm_tcgen05", "mlr_gemm_tcgen05"), space["gemm_scratch"], space["gemm_counters"]
-                    scratch_bytes, counters_len = scratch.numel(), counters.numel()
+                    scratch_at, scratch_bytes, counters_len = scratch.data_ptr(), scratch.numel(), counters.numel()
             elif x.dtype == torch.float32 and self._split_fits(x, weight):
                 route, product = 3, _entry("linear_split", "mlr_linear_split")
-                parts = _declared_library("linear_split").mlr_linear_split_rows(rows, K)
-                scratch = torch.empty((3, parts, -(-K // 8) * 8), dtype=torch.bfloat16, device=x.device) if parts else None
+                behind = 3 * _declared_library("linear_split").mlr_linear_split_rows(rows, K) * (-(-K // 8) * 4)      # x in three bfloat16 parts
+        # Behind the small sums, in one piece of memory: the shared product's sums in 32 bits (the result itself where it is in 32 bits), or
+        # what that product needs.
+        head = -(-rows * rank // 32) * 32
+        out = x.new_empty((rows, N), dtype=out_dtype)
+        low = x.new_empty(head + (behind if out_dtype == torch.float32 else rows * N), dtype=torch.float32)
+        low_at = low.data_ptr()
+        base_at = out.data_ptr() if out_dtype == torch.float32 else low_at + 4 * head
+        if behind:
+            scratch_at = low_at + 4 * head
         if route:
             status = library.mlr_linear_adapters(
                 x.data_ptr(), weight.data_ptr(), _address(bias), adapters.down.data_ptr(), adapters.up.data_ptr(), adapters.scales.data_ptr(),
                 row_adapter.data_ptr(), low_at, base_at, out.data_ptr(), rows, N, K, count, rank, _code(x.dtype), _code(out_dtype), route,
-                product, _address(scratch), scratch_bytes, _address(counters), counters_len, space["error_word"].data_ptr(), _raw_stream())
+                product, scratch_at, scratch_bytes, _address(counters), counters_len, space["error_word"].data_ptr(), _raw_stream())
             if status != _NO_ROOM:      # the product's partial tiles do not fit its scratch memory: by the general way
                 global launches
                 _check(status, "linear_adapters")
