@@ -6,8 +6,10 @@
 // generator keyed by the request's seed and the index of the token being produced, so a request's
 // tokens do not depend on which other requests share the batch; the token is the first index
 // whose cumulative probability exceeds u.  The cumulative sum is taken in a fixed order (warp w
-// owns one contiguous stretch of the vocabulary, walked 32 entries at a time).  Any vocabulary
-// size is accepted.
+// owns one contiguous stretch of the vocabulary, walked 32 entries at a time).  A token of no probability (a logit of -inf: one
+// that a grammar or a ban forbids) is never chosen: the sum that says which warp's stretch the target falls into and the running sum
+// of the walk through it round differently, so the walk may not reach the target, and then ends at the stretch's last
+// token that has any.  Any vocabulary size is accepted.
 #include "common.cuh"
 
 namespace mlr {
@@ -122,19 +124,22 @@ sample_kernel(const float* logits, const float* __restrict__ temperatures,
   __syncthreads();
 
   float before = 0.f, everything = 0.f;  // sum of the warps before mine; sum of all
+  int last = -1;                         // the last warp whose stretch has any probability
   for (int w = 0; w < SAMPLE_WARPS; ++w) {
     if (w == warp) before = everything;
     everything += warp_totals[w];
+    if (warp_totals[w] > 0.f) last = w;
   }
   const unsigned long long seed = record != nullptr
       ? ((unsigned long long)record->seed_high << 32) | record->seed_low : (unsigned long long)seeds[blockIdx.x];
   const long long counter = record != nullptr ? (long long)record->counter : counters[blockIdx.x];
   const float u = uniform_from_seed(seed, counter);
   const float target = u * everything;
-  const bool mine = target >= before && (target < before + total);
+  // The intervals of the warps follow one another; what rounding leaves behind the last of them belongs to it.
+  const bool mine = target >= before && (target < before + total || warp == last);
   if (mine) {
     float running = before;
-    int found = -1;
+    int found = -1, possible = -1;       // possible: the last entry of the walk so far with any probability
     for (int base = begin; base < end && found < 0; base += 32) {
       const int i = base + lane;
       const float e = i < end ? expf((row[i] - row_max) * inv_t) : 0.f;
@@ -144,15 +149,16 @@ sample_kernel(const float* logits, const float* __restrict__ temperatures,
         const float up = __shfl_up_sync(0xffffffffu, inclusive, offset);
         if (lane >= offset) inclusive += up;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, i < end && running + inclusive > target);
+      const unsigned some = __ballot_sync(0xffffffffu, e > 0.f);
+      const unsigned hit = __ballot_sync(0xffffffffu, running + inclusive > target) & some;
       if (hit != 0u) found = base + (__ffs(hit) - 1);
+      if (some != 0u) possible = base + 31 - __clz(some);
       running += __shfl_sync(0xffffffffu, inclusive, 31);
     }
-    if (lane == 0) chosen = found >= 0 ? found : end - 1;
+    if (lane == 0) chosen = found >= 0 ? found : possible;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    // Rounding can leave the target just past the last stretch; take the last token then.
     const int token = chosen >= 0 ? chosen : vocab - 1;
     tokens[blockIdx.x] = token;
     if (record != nullptr) {
