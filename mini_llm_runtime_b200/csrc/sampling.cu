@@ -9,7 +9,7 @@
 // owns one contiguous stretch of the vocabulary, walked 32 entries at a time).  A token of no probability (a logit of -inf: one
 // that a grammar or a ban forbids) is never chosen: the sum that says which warp's stretch the target falls into and the running sum
 // of the walk through it round differently, so the walk may not reach the target, and then ends at the stretch's last
-// token that has any.  Any vocabulary size is accepted.
+// token that has any.  A row of -inf throughout has no distribution: token 0, as greedy.  Any vocabulary size is accepted.
 #include "common.cuh"
 
 namespace mlr {
@@ -159,7 +159,8 @@ sample_kernel(const float* logits, const float* __restrict__ temperatures,
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    const int token = chosen >= 0 ? chosen : vocab - 1;
+    // No probabilities at all (every logit -inf; infinite or NaN ones): what the greedy choice would be.
+    const int token = chosen >= 0 ? chosen : scratch_index[0];
     tokens[blockIdx.x] = token;
     if (record != nullptr) {
       record->last_token = token;

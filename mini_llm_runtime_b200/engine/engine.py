@@ -237,7 +237,7 @@ class ContinuousBatchEngine:
 
     def allow_tokens(self, request_id: str, tokens: "Collection[int] | None") -> None:
         """The tokens that the request may choose from its next step on (None: all), as a grammar finds them after each token.  A
-        request that allows nothing chooses token 0 if greedy."""
+        request that allows nothing chooses token 0."""
         if self.runner.rules is None:
             raise ValueError("allowed tokens need an engine made with logit_rules=True")
         if self.step_ahead:

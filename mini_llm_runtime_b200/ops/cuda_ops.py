@@ -2647,7 +2647,7 @@ class CudaOps:
         """The rules of each row's request on its logits, float32 [rows, vocab] on a 16-byte boundary; ``row_slot`` int32 [rows] names the slot whose
         row of the tables holds (a row of no slot passes unchanged).  A token of the history: x / repetition where x > 0, else
         x * repetition; then less frequency times how often it was generated, less presence if it was; then its bias; tokens
-        that are not allowed get -inf.  A row that allows nothing is -inf throughout (greedy sampling then takes token 0)."""
+        that are not allowed get -inf.  A row that allows nothing is -inf throughout (sampling then takes token 0)."""
         return self._shape_logits(logits, row_slot, tables, None)
 
     def shape_logits_(self, logits: torch.Tensor, row_slot: torch.Tensor, tables: LogitTables) -> torch.Tensor:

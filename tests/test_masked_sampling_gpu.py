@@ -93,3 +93,18 @@ def test_shares_of_allowed_tokens():
     for place, weight in zip(places, weights):
         share = weight / sum(weights)
         assert abs(int((tokens == place).sum()) - share * count) < 5 * math.sqrt(count * share * (1 - share))
+
+
+@pytest.mark.parametrize("vocab", [40, 1000, 152064])
+@pytest.mark.parametrize("temperature", [0.0, 0.05, 1.0, 7.0])
+def test_a_row_that_allows_nothing(vocab, temperature):
+    """Token 0 at any temperature."""
+    assert not draw(torch.full((vocab,), -math.inf), range(20), temperature).any()
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_an_infinite_logit_is_the_choice(temperature):
+    row = torch.full((1000,), -math.inf)
+    row[::3] = torch.linspace(-5, 5, 334)
+    row[333] = math.inf
+    assert draw(row, range(20), temperature).unique().tolist() == [333]
