@@ -1183,12 +1183,13 @@ class CudaOps:
         chunk, parts, units, own_parts = prefix_parts(counts["tile_keys"], counts["least_shared"], segments, batch.max_kv_len, num_heads,
                                                       num_kv_heads, head_dim, self.sm_count(q.device))
         states = (parts + own_parts) * segments * num_heads
-        scratch = torch.empty(states * (head_dim + 2), dtype=torch.float32, device=q.device)
+        outputs = -(-states * head_dim // 4) * 4      # pairs of (largest exponent, sum) lie behind them, read as pairs
+        scratch = torch.empty(outputs + 2 * states, dtype=torch.float32, device=q.device)
         _check(_declared_library("attention_prefix").mlr_attention_prefix(
             q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), batch.seg_q_start.data_ptr(), batch.seg_pos0.data_ptr(),
             batch.seg_slot.data_ptr(), batch.block_table.data_ptr(), plan["seg_keys"].data_ptr(), plan["members"].data_ptr(),
             plan["tile_first"].data_ptr(), plan["tile_count"].data_ptr(), plan["tile_keys"].data_ptr(), scratch.data_ptr(),
-            scratch.data_ptr() + states * head_dim * 4, segments, counts["tiles"], num_heads, num_kv_heads, head_dim, page_size,
+            scratch.data_ptr() + outputs * 4, segments, counts["tiles"], num_heads, num_kv_heads, head_dim, page_size,
             k_pool.shape[0], batch.block_table.shape[1], chunk, parts, own_parts, units, scale, _code(q.dtype), int(fast), self._error_word(q.device).data_ptr(), _raw_stream()), "shared_prefix_attention")
         return out
 

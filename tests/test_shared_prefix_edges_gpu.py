@@ -1,0 +1,26 @@
+"""Attention behind shared prefixes at the edges of what a call may bring."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from mini_llm_runtime_b200 import ops
+from test_shared_prefix_gpu import Step
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def every_prefix_by_itself(monkeypatch):
+    monkeypatch.setattr(ops.current(), "shared_prefix_least", 0)
+
+
+@pytest.mark.parametrize("dim", [1, 7, 33, 127, 255])
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 1), (9, 3)])
+@pytest.mark.parametrize("groups,alone,own", [([(3, 40)], 0, (1,)), ([(2, 300)], 1, (5, 300)), ([], 1, (9,))])
+def test_odd_heads_of_odd_sizes(dim, heads, kv_heads, groups, alone, own):
+    """Three, one or five requests: the numbers of states are odd too."""
+    for dtype in (torch.float32, torch.bfloat16):
+        step = Step(groups, alone, own, heads, kv_heads, dim, 8, dtype, seed=dim)
+        step.check(step.run())
