@@ -55,8 +55,9 @@ __device__ __forceinline__ float penalised(float x, int word, float repetition, 
 // next, the arithmetic of the present one.  (A CTA per portion lives through that chain, 4 us, for 16 KB: 64 x 152,064 logits 36 us, 256 x
 // 151,936 94 us; as it stands 23 and 68, 4.75 TB/s, where a copy of the same logits takes 18.5 and 55 and the bytes alone 12.6 and 50. Few
 // rows are latency: a row of 151,936 4.1 us in a captured step, 8 from the host.)
-// Pieces lie on 16-byte boundaries.  WHOLE: the vocabulary is a multiple of four and every piece is one row's; else a row starts inside a
-// piece, and its first and last piece go entry by entry.
+// Pieces lie on 16-byte boundaries.  WHOLE: the vocabulary is a multiple of four, every piece is one row's, and so are the words of the
+// history, which start on such a boundary too; else a row starts inside a piece, its first and last piece go entry by entry, and the words
+// of a slot whose row of them starts on another boundary as well.
 // IN_PLACE: logits that no rule touches are neither read nor written.
 template <bool IN_PLACE, bool WHOLE>
 __global__ void __launch_bounds__(RULE_THREADS)
@@ -106,7 +107,7 @@ logit_rules_kernel(const float* logits, float* out, const int* row_slot, int voc
     if (allowed != nullptr) open = (four_bits<WHOLE>(allowed, t + shift, words) << shift & 15u) | ((1u << shift) - 1u);
     return (known & open) | (open ^ 15u) << 4;
   };
-  const bool aligned = WHOLE || ((size_t)(ruled ? slot : 0) * vocab + first & 3) == 0;
+  const bool aligned = WHOLE || ((uintptr_t)(counts + first) & 15) == 0;      // the slot's words, piece by piece
   int word[4], word_ahead[4];
   auto load_words = [&](int t, unsigned bits, int* w, float* v) {
     if ((bits & 15u) == 0u) return;
@@ -204,7 +205,7 @@ static void launch_rules(const float* logits, float* out, const int* row_slot, i
   const int portions = (vocab + 3 + PORTION - 1) / PORTION;
   const int each = (int)min(4ll, 1 + (long long)rows * portions / (8 * sm_count()));
   const dim3 grid((portions + each - 1) / each, rows);
-  const bool whole = (vocab & 3) == 0;
+  const bool whole = (vocab & 3) == 0 && ((uintptr_t)tables.counts & 15) == 0;
   auto kernel = logits == out ? (whole ? logit_rules_kernel<true, true> : logit_rules_kernel<true, false>)
                               : (whole ? logit_rules_kernel<false, true> : logit_rules_kernel<false, false>);
   launch_kernel(kernel, grid, dim3(RULE_THREADS), 0, stream, logits, out, row_slot, vocab, each * PORTION, tables);
