@@ -24,7 +24,7 @@ constexpr int IN_PROMPT = 1 << 30;
 struct RuleTables {
   const float* penalties;      // [slots][3]: repetition, presence, frequency; null: none
   const int* counts;           // [slots][vocab], with `penalties`
-  const unsigned* seen;        // [slots][words], with `penalties`
+  const unsigned* seen;        // [slots][words], with `penalties`; bits behind the vocabulary say nothing
   const int* bias_tokens;      // [slots][biases], ascending, the unused end 2^31 - 1; null: none
   const float* bias_values;    // [slots][biases]
   const unsigned* allowed;     // [slots][words]; null: everything
@@ -104,6 +104,7 @@ logit_rules_kernel(const float* logits, float* out, const int* row_slot, int voc
     const int shift = !WHOLE && t < 0 ? -t : 0;
     unsigned known = 0u, open = 15u;
     if (seen != nullptr) known = four_bits<WHOLE>(seen, t + shift, words) << shift & 15u;
+    if (!WHOLE && t + 4 > vocab) known &= (1u << (vocab - t)) - 1u;      // behind the vocabulary there are no words
     if (allowed != nullptr) open = (four_bits<WHOLE>(allowed, t + shift, words) << shift & 15u) | ((1u << shift) - 1u);
     return (known & open) | (open ^ 15u) << 4;
   };

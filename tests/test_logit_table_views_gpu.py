@@ -51,3 +51,22 @@ def test_all_slots_but_the_first():
     view = LogitTables(**{name: tensor[1:] for name, tensor in device.items()})
     assert view.counts.data_ptr() % 16
     check(both_ways(logits, row_slot, view), logits, row_slot, {name: tensor[1:] for name, tensor in tables.items()}, 0)
+
+
+@pytest.mark.parametrize("vocab", [1, 3, 5, 30, 33, 1000, 1021, 4093, 4097])
+def test_bits_behind_the_vocabulary_say_nothing(vocab):
+    """The last word of ``seen`` and ``allowed`` has bits for tokens that do not exist, set or not."""
+    slots, rows = 3, 4
+    g = torch.Generator().manual_seed(vocab)
+    logits = torch.randn((rows, vocab), generator=g) * 4
+    row_slot = torch.tensor([2, 0, 1, 2], dtype=torch.int32)      # the last slot's words end where the table ends
+    tables = made(vocab, slots, vocab, grammar=True, known=0.6)
+    filled = {name: tensor.to(DEVICE) for name, tensor in tables.items()}
+    want = both_ways(logits, row_slot, LogitTables(**filled))
+    if vocab % 32:
+        behind = -1 << (vocab % 32)
+        filled["seen"][:, -1] |= behind
+        filled["allowed"][:, -1] ^= behind
+    got = both_ways(logits, row_slot, LogitTables(**filled))
+    assert torch.equal(got, want)
+    check(got, logits, row_slot, tables, 0)
