@@ -10,7 +10,8 @@
 //   0 .. prefix_parts - 1              `chunk` keys of the prefix each, as many as the request's prefix has
 //   prefix_parts .. + own_parts - 1    equal parts of the request's own keys, as many as there are (see own_range)
 // Rows of a work item: of a prefix, the query heads of one kv head of up to 128 / heads_per_kv requests; of own keys, those of
-// one request.
+// one request.  A request whose context ends before its group's keys do sees those of its context (pos0 is device memory: what the lists
+// were made for is not known to the host of a captured step).
 #include "mma_attention.cuh"
 #include "tcgen05.cuh"
 
@@ -98,6 +99,9 @@ prefix_parts_plain_kernel(const PrefixCall c) {
 #pragma unroll
   for (int r = 0; r < PLAIN_ROWS; ++r) acc[r][0] = acc[r][1] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};      // of rows 2 * warp and 2 * warp + 1, the same in every lane
+  int row_end[2];                                              // the end of their contexts
+#pragma unroll
+  for (int i = 0; i < 2; ++i) row_end[i] = 2 * warp + i < rows ? min(end, c.pos0[segment_of(2 * warp + i)] + 1) : end;
   for (int key0 = begin; key0 < end; key0 += PLAIN_KEYS) {
     __syncthreads();
     for (int k = warp; k < PLAIN_KEYS; k += PLAIN_THREADS / 32) {
@@ -115,7 +119,7 @@ prefix_parts_plain_kernel(const PrefixCall c) {
       const int r = 2 * warp + i;
       float s = 0.f;
       for (int d = 0; d < dim; ++d) s = fmaf(q[r * dim + d], keys[lane * pitch + d], s);
-      if (!open[lane]) s = -INFINITY;
+      if (!open[lane] || key0 + lane >= row_end[i]) s = -INFINITY;
       const float top = fmaxf(m[i], warp_max(s));
       const float base = top == -INFINITY ? 0.f : top;
       const float e = exp2f(s - base), shrink = exp2f(m[i] - base);
@@ -260,6 +264,8 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
   const bool live = r < rows;
   const int segment = live ? c.members[first_member + r / per] : 0, head = kv_head * per + r % per;
   const int q_at = live ? c.q_row[segment] * c.heads + head : -1;      // in units of a head
+  // keys of the row from this thread's first one on: all of the part's, or as far as its context reaches
+  int row_keys = (live ? min(end, c.pos0[segment] + 1) : end) - begin - (threadIdx.x >= PT_ROWS ? PT_HALF : 0);
   int first_pages[STAGES + 2];
   if (warp >= PT_LOAD_WARP) {
 #pragma unroll
@@ -383,17 +389,17 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
       bool step = false;
       float alpha = 1.f;
       if (warp_live) {
-        const int mine = key0 + side * PT_HALF;      // this thread's first key
 #pragma unroll
         for (int i = 0; i < PT_HALF; i += 16)
           fa_tmem_load16(scores + side * PT_HALF + i, reinterpret_cast<uint32_t*>(s) + i);
         fa_tmem_wait_ld();
         fa_fence_before();
-        if (ragged) {
+        if (row_keys < PT_HALF) {
 #pragma unroll
           for (int i = 0; i < PT_HALF; ++i)
-            if (mine + i >= end) s[i] = -INFINITY;
+            if (i >= row_keys) s[i] = -INFINITY;
         }
+        row_keys -= PT_KEYS;
         float part_max[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
         for (int i = 4; i < PT_HALF - 4; i += 8)

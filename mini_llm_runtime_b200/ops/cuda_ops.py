@@ -363,7 +363,7 @@ PREFIX_TILE_ROWS = 128    # attention_prefix.cu: query rows of one work item of 
 def plan_shared_prefix(groups, num_segments: int, heads_per_kv: int) -> tuple[dict, dict]:
     """Work lists of ``shared_prefix_attention`` for a step of ``num_segments`` decoded tokens: ``groups`` lists (segments, keys)
     pairs, the requests of ``segments`` having their first ``keys`` keys on the same pages.  A segment belongs to one group at
-    most, and ``keys`` reaches no further than the shortest context of the group.  int32 arrays by name, and counts by name, as from
+    most; one whose context is shorter than ``keys`` attends to its context.  int32 arrays by name, and counts by name, as from
     ``plan_attention``.
 
     ``seg_keys``: shared keys before each segment's own.  ``members``: the segments of the groups, one behind the other.

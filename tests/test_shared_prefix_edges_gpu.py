@@ -24,3 +24,14 @@ def test_odd_heads_of_odd_sizes(dim, heads, kv_heads, groups, alone, own):
     for dtype in (torch.float32, torch.bfloat16):
         step = Step(groups, alone, own, heads, kv_heads, dim, 8, dtype, seed=dim)
         step.check(step.run())
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(14, 2, 64, torch.bfloat16), (28, 4, 128, torch.bfloat16), (16, 1, 64, torch.bfloat16),
+                                                      (6, 2, 64, torch.float32), (6, 2, 80, torch.bfloat16)])
+def test_members_with_fewer_keys_than_their_group(heads, kv_heads, dim, dtype):
+    """A request attends to its own context, whatever number of keys its group was planned with."""
+    step = Step([(6, 320), (3, 700)], 1, (5, 90, 33), heads, kv_heads, dim, 16, dtype, seed=dim)
+    for member, context in ((0, 1), (3, 64), (5, 65), (7, 319), (8, 200)):
+        step.contexts[member] = min(context, step.contexts[member])
+        step.batch.seg_pos0[member] = step.contexts[member] - 1
+    step.check(step.run())
