@@ -937,7 +937,7 @@ MLR_DEFINE_PDL_SWITCH
 
 // q, out [rows, heads * dim], pools [pages, kv_heads, page_size, dim] of one dtype.  acc, state: float32, (prefix_parts + own_parts) *
 // segments * heads * dim and * 2 of them, on boundaries of 16 and 8 bytes.  fast: the tensor cores (bfloat16, dim 64 or 128, at most 16 heads per kv head, pages of a
-// power of two from 8 on); else any type and size.  chunk: keys of a prefix part; prefix_parts of them
+// power of two from 8 on, a scale above zero); else any type, size and scale.  chunk: keys of a prefix part; prefix_parts of them
 // reach the longest prefix, and all items have `units` parts together.
 MLR_EXPORT int mlr_attention_prefix(const void* q, const void* k_pool, const void* v_pool, void* out, const int* q_row, const int* pos0,
                                     const int* seg_slot, const int* block_table, const int* seg_keys, const int* members,
@@ -956,7 +956,7 @@ MLR_EXPORT int mlr_attention_prefix(const void* q, const void* k_pool, const voi
   if (fast) {
     const bool boxes = page_size >= 8 && (page_size & (page_size - 1)) == 0;      // a box of a tile is eight rows at least
     const bool rows_fit = (long long)pages * kv_heads * page_size <= 0x7fffffff && chunk % PT_KEYS == 0;
-    if (dtype != MLR_BF16 || heads / kv_heads > 16 || !boxes || !rows_fit) return MLR_BAD_SIZE;
+    if (dtype != MLR_BF16 || heads / kv_heads > 16 || !boxes || !rows_fit || !(scale > 0.f)) return MLR_BAD_SIZE;
     if ((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) != 0) return MLR_BAD_ALIGNMENT;
     if (dim == 64) return heads / kv_heads <= 8 ? run_fast<64, 1>(c, units, error_word, stream) : run_fast<64, 2>(c, units, error_word, stream);
     if (dim == 128) return heads / kv_heads <= 8 ? run_fast<128, 1>(c, units, error_word, stream) : run_fast<128, 2>(c, units, error_word, stream);

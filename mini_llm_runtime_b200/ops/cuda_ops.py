@@ -1161,8 +1161,9 @@ class CudaOps:
         _need(batch.block_table, "block_table", torch.int32, 2)
         _need_here(q=q, k_pool=k_pool, v_pool=v_pool, prefix=prefix, block_table=batch.block_table)
         page_size = k_pool.shape[2] if k_pool.dim() == 4 else 0
+        # (a scale of zero or below turns the order of the scores round, which the kernels on the tensor cores take before scaling)
         fast = (self.use_mma_attention and q.dtype == torch.bfloat16 and head_dim in (64, 128) and num_heads // num_kv_heads <= 16
-                and page_size >= 8 and page_size & (page_size - 1) == 0)
+                and page_size >= 8 and page_size & (page_size - 1) == 0 and scale > 0)
         _need(k_pool, "k_pool", q.dtype, 4)
         _need(v_pool, "v_pool", q.dtype, 4)
         if q.shape[1] != num_heads * head_dim:

@@ -35,3 +35,15 @@ def test_members_with_fewer_keys_than_their_group(heads, kv_heads, dim, dtype):
         step.contexts[member] = min(context, step.contexts[member])
         step.batch.seg_pos0[member] = step.contexts[member] - 1
     step.check(step.run())
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(14, 2, 64, torch.bfloat16), (8, 2, 128, torch.bfloat16), (6, 2, 48, torch.float32)])
+@pytest.mark.parametrize("scale", [0.0, -0.125, -4.0])
+def test_scales_of_zero_and_below(heads, kv_heads, dim, dtype, scale):
+    """softmax(q k scale) of a negative scale is that of -q with its magnitude; of zero, the mean of the values."""
+    step = Step([(6, 300)], 1, (5, 90), heads, kv_heads, dim, 16, dtype, seed=dim)
+    step.scale = scale
+    got = step.run()
+    step.scale = abs(scale)
+    step.q = -step.q
+    step.check(got)
