@@ -943,6 +943,7 @@ MLR_EXPORT int mlr_attention_prefill_mma(const void* q, const void* k_pool, cons
     return MLR_BAD_SIZE;
   if (head_dim != 64 && head_dim != 128) return MLR_BAD_SIZE;
   if (heads > 65535) return MLR_TOO_LARGE;
+  if (((uintptr_t)k_pool & 15) || ((uintptr_t)v_pool & 15) || ((uintptr_t)q & 15)) return MLR_BAD_ALIGNMENT;
   const size_t shared = (size_t)(TILE_Q + 4 * TILE_KV) * head_dim * 2;
   const int page_shift = shift_of(page_size);
   dim3 grid(tiles, heads);
@@ -973,6 +974,7 @@ MLR_EXPORT int mlr_attention_decode_mma(const void* q, const void* k_pool, const
     return MLR_BAD_SIZE;
   if (heads / kv_heads > 16 || rows > 65535 || kv_heads > 65535) return MLR_TOO_LARGE;
   if (head_dim != 64 && head_dim != 128) return MLR_BAD_SIZE;
+  if (((uintptr_t)k_pool & 15) || ((uintptr_t)v_pool & 15) || ((uintptr_t)q & 15)) return MLR_BAD_ALIGNMENT;
   // the final merge keeps 2 * 16 * max_splits + 16 floats in the warps' merge area
   if ((size_t)(2 * 16 * max_splits + 16) > (size_t)ATTN_WARPS * 16 * (head_dim + 2)) return MLR_TOO_LARGE;
   // long chunks on a grid of several waves: fewer stages, more CTAs per SM
@@ -1025,7 +1027,7 @@ MLR_EXPORT int mlr_attention_decode_tma(const void* q, const void* k_pool, const
   if (qkv != nullptr && (inv_freq == nullptr || slots == nullptr)) return MLR_BAD_SIZE;
   const int page_shift = shift_of(page_size);
   if (page_shift < 3) return MLR_BAD_SIZE;
-  if (((uintptr_t)k_pool & 15) || ((uintptr_t)v_pool & 15)) return MLR_BAD_ALIGNMENT;
+  if (((uintptr_t)k_pool & 15) || ((uintptr_t)v_pool & 15) || ((uintptr_t)q & 15)) return MLR_BAD_ALIGNMENT;
   const long long pool_rows = (long long)pool_pages * kv_heads * page_size;
   if (pool_rows >= (1ll << 31)) return MLR_TOO_LARGE;           // tile coordinates are 32-bit
   if ((size_t)(2 * 16 * max_splits + 16) > (size_t)ATTN_WARPS * 16 * (head_dim + 2)) return MLR_TOO_LARGE;

@@ -1163,7 +1163,8 @@ class CudaOps:
         page_size = k_pool.shape[2] if k_pool.dim() == 4 else 0
         # (a scale of zero or below turns the order of the scores round, which the kernels on the tensor cores take before scaling)
         fast = (self.use_mma_attention and q.dtype == torch.bfloat16 and head_dim in (64, 128) and num_heads // num_kv_heads <= 16
-                and page_size >= 8 and page_size & (page_size - 1) == 0 and scale > 0)
+                and page_size >= 8 and page_size & (page_size - 1) == 0 and scale > 0
+                and not (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr()) % 16)
         _need(k_pool, "k_pool", q.dtype, 4)
         _need(v_pool, "v_pool", q.dtype, 4)
         if q.shape[1] != num_heads * head_dim:
@@ -1179,8 +1180,7 @@ class CudaOps:
             # what paged_attention runs for such a step
             self._decode_attention(q, k_pool, v_pool, out, batch, num_heads, num_kv_heads, head_dim, scale, None, mma=True)
             return out
-        fast = (fast and k_pool.shape[0] * num_kv_heads * page_size < 1 << 31
-                and not (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr()) % 16)
+        fast = fast and k_pool.shape[0] * num_kv_heads * page_size < 1 << 31
         chunk, parts, units, own_parts = prefix_parts(counts["tile_keys"], counts["least_shared"], segments, batch.max_kv_len, num_heads,
                                                       num_kv_heads, head_dim, self.sm_count(q.device))
         states = (parts + own_parts) * segments * num_heads

@@ -47,3 +47,21 @@ def test_scales_of_zero_and_below(heads, kv_heads, dim, dtype, scale):
     step.scale = abs(scale)
     step.q = -step.q
     step.check(got)
+
+
+@pytest.mark.parametrize("least", [0, 1 << 40])
+@pytest.mark.parametrize("name", ["q", "k", "v"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_tensors_on_no_16_byte_boundary(monkeypatch, dim, name, least):
+    """They go through the general kernels, also where sharing saves too little; ``paged_attention``'s kernels refuse them."""
+    monkeypatch.setattr(ops.current(), "shared_prefix_least", least)
+    step = Step([(6, 320)], 1, (5, 90, 33), 14, 2, dim, 16, torch.bfloat16, seed=dim)
+    tensor = getattr(step, name)
+    view = torch.empty(tensor.numel() + 8, dtype=tensor.dtype, device=tensor.device)[1:tensor.numel() + 1].view(tensor.shape)
+    setattr(step, name, view.copy_(tensor))
+    step.check(step.run())
+    kernels = ops.current()
+    for use_tma in (True, False):
+        monkeypatch.setattr(kernels, "use_tma_attention", use_tma)
+        with pytest.raises(ops.KernelError, match="aligned"):
+            kernels.paged_attention(step.q, step.k, step.v, step.batch, 14, 2, dim, step.scale, None)

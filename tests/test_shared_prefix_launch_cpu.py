@@ -58,3 +58,18 @@ def test_states_lie_on_their_boundaries(library, dim, heads, kv_heads, segments,
     assert (call["acc"] % 16, call["state"] % 8) == (0, 0)
     assert call["acc"] + 4 * states * dim <= call["state"]
     assert call["state"] + 8 * states <= scratch.data_ptr() + 4 * scratch.numel()
+
+
+@pytest.mark.parametrize("least", [0, 1 << 40])
+@pytest.mark.parametrize("moved", ["q", "k", "v"])
+def test_tensors_on_no_16_byte_boundary_take_the_general_kernels(monkeypatch, library, moved, least):
+    kernels = CudaOps()
+    kernels.shared_prefix_least = least
+    decoding = []
+    monkeypatch.setattr(kernels, "_decode_attention", lambda *args, **named: decoding.append(args))
+    tensors = {"q": torch.zeros((3, 4 * 64), dtype=torch.bfloat16), "k": torch.zeros((9, 2, 16, 64), dtype=torch.bfloat16),
+               "v": torch.zeros((9, 2, 16, 64), dtype=torch.bfloat16)}
+    place = tensors[moved]
+    tensors[moved] = torch.zeros(place.numel() + 8, dtype=torch.bfloat16)[1:place.numel() + 1].view(place.shape)
+    kernels.shared_prefix_attention(tensors["q"], tensors["k"], tensors["v"], decoded(3, 900, pages=60), shared([(range(3), 16)], 3, 2), 4, 2, 64, 0.3)
+    assert not decoding and library.calls[-1]["fast"] == 0
