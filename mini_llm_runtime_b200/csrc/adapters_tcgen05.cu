@@ -8,12 +8,12 @@
 // not finite stays with its own rows.  All of it accumulates where the shared product does, in float32 in tensor memory, so the result is
 // rounded once and an adapter costs its products and the reading of B, no pass over y.  (A kernel that adds the adapters to a shared
 // product in float32 reads and writes 0.5 GB more at 2,048 x 37,888 with K = 3,584 and rank 64: 1,135 us against 500, of which the sums u
-// are 20; 1.12 PFLOP/s, the tensor pipe busy for 72 %.)  u comes in two bfloat16 parts, u = high + low to 2^-17, two left operands for one
-// right one.
+// are 20; 1.12 PFLOP/s, the tensor pipe busy for 72 %.)  u comes in bfloat16 parts of eight bits each, as many left operands for one right
+// one: two for a bfloat16 result, u to 2^-17, a small part of that result's own rounding (2^-8); three for a float32 result, all of u.
 //
 // One CTA computes 128 or 256 rows (one or two accumulators) x BN columns.  Warp 0 loads (bulk tensor copies into a ring of
 // 128-byte-swizzled tiles), warp 1 issues the products, warps 2 to 5 list the tile's adapters while the shared product runs,
-// lay out u where the first two stages held x, and write the result.  (Left operands of each adapter by itself, with zeros in
+// lay out u where the first stages held x, and write the result.  (Left operands of each adapter by itself, with zeros in
 // the other rows, built anew for each: 160 rows of 40 adapters, 896 x 1,152, 105 us.)
 // Every wait is bounded; one that runs out stores a code into the error word, and the CTA frees its tensor memory and ends.
 #include "tcgen05.cuh"
@@ -25,6 +25,7 @@ constexpr int AT_MAX_STAGES = 6;
 
 struct AdapterGemm {
   int M, N, K, adapters, rank, stages;
+  int parts, held;            // parts of u, and how many of them lie in shared memory at a time: no more than there are stages
   const bf16* bias;
   const float* u;             // [M, rank]
   const int* row_adapter;     // [M]
@@ -40,6 +41,15 @@ __device__ __forceinline__ void at_mma_rows(uint32_t tmem_d, uint64_t a_desc, ui
       "setp.ne.b32 p, 1, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n\t}"
       ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(off.x), "r"(off.y), "r"(off.z), "r"(off.w) : "memory");
+}
+// The next bfloat16 part of two numbers, taken off them: the number rounded to eight bits; the third is what is left, exactly.  An
+// infinity is all of its number (what is left of it would be NaN).
+__device__ __forceinline__ uint32_t at_take_part(float& x0, float& x1) {
+  const __nv_bfloat162 pair = __floats2bfloat162_rn(x0, x1);
+  const float h0 = __bfloat162float(pair.x), h1 = __bfloat162float(pair.y);
+  x0 = fabsf(h0) < INFINITY ? x0 - h0 : 0.f;
+  x1 = fabsf(h1) < INFINITY ? x1 - h1 : 0.f;
+  return *reinterpret_cast<const uint32_t*>(&pair);
 }
 __device__ __forceinline__ void at_wait(uint64_t* bar, uint32_t parity, int* error_word, int code, bool& gave_up) {
   if (!gave_up) gave_up = !mbar_wait(bar, parity, error_word, code);
@@ -62,7 +72,8 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int stages = p.stages;
   const int row0 = blockIdx.x * BM, n0 = blockIdx.y * BN;
-  const int base_blocks = (p.K + 63) / 64, chunks = (p.rank + 63) / 64;
+  // the extension's rounds: 64 ranks, `held` parts of u
+  const int base_blocks = (p.K + 63) / 64, passes = (p.parts + p.held - 1) / p.held, rounds = (p.rank + 63) / 64 * passes;
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     mbar_init(&listed, 1);
@@ -112,14 +123,14 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
         load_w(s, i * 64);
       }
       at_wait(&listed, 0u, p.error_word, 0x92, gave_up);
-      const int blocks = gave_up ? 0 : list_count * chunks;
+      const int blocks = gave_up ? 0 : list_count * rounds;
       for (int e = 0; e < blocks; ++e) {
         const int i = base_blocks + e, s = i % stages;
         if (i >= stages) at_wait(&empty[s], (unsigned)(i / stages - 1) & 1u, p.error_word, 0x93, gave_up);
         if (gave_up) break;
         mbar_expect_tx(&full[s], B_BYTES);
-        const int chunk = e / list_count, adapter = list[e - chunk * list_count];
-        tma_load_2d(&up_map, &full[s], tiles + (size_t)s * STAGE_BYTES + A_BYTES, chunk * 64, adapter * p.N + n0);
+        const int round = e / list_count, adapter = list[e - round * list_count];
+        tma_load_2d(&up_map, &full[s], tiles + (size_t)s * STAGE_BYTES + A_BYTES, round / passes * 64, adapter * p.N + n0);
       }
     }
   } else if (warp == 1) {
@@ -149,11 +160,11 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
     at_wait(&listed, 0u, p.error_word, 0x95, gave_up);
     gave_up = __any_sync(0xffffffffu, gave_up);
     const int count = list_count;
-    for (int chunk = 0; chunk < chunks && count > 0 && !gave_up; ++chunk) {
-      at_wait(&u_ready, (unsigned)chunk & 1u, p.error_word, 0x97, gave_up);
-      const int steps = min(4, (p.rank - chunk * 64 + 15) / 16);
+    for (int round = 0; round < rounds && count > 0 && !gave_up; ++round) {
+      at_wait(&u_ready, (unsigned)round & 1u, p.error_word, 0x97, gave_up);
+      const int steps = min(4, (p.rank - round / passes * 64 + 15) / 16), parts = min(p.held, p.parts - round % passes * p.held);
       for (int l = 0; l < count; ++l) {
-        const int i = base_blocks + chunk * count + l, s = i % stages;
+        const int i = base_blocks + round * count + l, s = i % stages;
         at_wait(&full[s], (unsigned)(i / stages) & 1u, p.error_word, 0x96, gave_up);
         gave_up = __any_sync(0xffffffffu, gave_up);
         if (gave_up) break;
@@ -163,7 +174,7 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
           for (int half = 0; half < HALVES; ++half) {
             const uint4 off = rows_off[l][half];
             if ((off.x & off.y & off.z & off.w) == 0xffffffffu) continue;      // none of its rows are in this half
-            for (int part = 0; part < 2; ++part)
+            for (int part = 0; part < parts; ++part)
               for (int k = 0; k < steps; ++k)
                 at_mma_rows(tmem_base + half * BN, a_desc0 + (uint64_t)((part * STAGE_BYTES + half * HALF_BYTES + k * 32) >> 4),
                             b + (uint64_t)((k * 32) >> 4), idesc, off);
@@ -222,7 +233,8 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
     asm volatile("bar.sync 1, 128;" ::: "memory");
     if (t == 0) mbar_arrive(&listed);
     const int count = list_count;
-    for (int chunk = 0; chunk < chunks && count > 0; ++chunk) {
+    for (int round = 0; round < rounds && count > 0; ++round) {
+      const int chunk = round / passes, part0 = round % passes * p.held, part1 = min(p.parts, part0 + p.held);
       // the sums are asked for before their place is free
       float v[HALVES][64];
 #pragma unroll
@@ -235,26 +247,20 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
           v[half][c] = four.x; v[half][c + 1] = four.y; v[half][c + 2] = four.z; v[half][c + 3] = four.w;
         }
       }
-      if (chunk == 0) at_wait(&base_done, 0u, p.error_word, 0x9a, gave_up);
-      else at_wait(&u_free, (unsigned)(chunk - 1) & 1u, p.error_word, 0x98, gave_up);
+      if (round == 0) at_wait(&base_done, 0u, p.error_word, 0x9a, gave_up);
+      else at_wait(&u_free, (unsigned)(round - 1) & 1u, p.error_word, 0x98, gave_up);
+      for (int part = 0; part < part1; ++part) {      // a part is taken off, and kept if it is this round's
+        const bool kept = part >= part0;
 #pragma unroll
-      for (int half = 0; half < HALVES; ++half) {
-        uint8_t* row = tiles + half * HALF_BYTES + t * 128;      // high parts; the low ones a stage on
+        for (int half = 0; half < HALVES; ++half) {
+          uint8_t* row = tiles + (part - part0) * STAGE_BYTES + half * HALF_BYTES + t * 128;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint32_t high[4], low[4];
+          for (int c = 0; c < 8; ++c) {
+            uint32_t packed[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float x0 = v[half][c * 8 + 2 * q], x1 = v[half][c * 8 + 2 * q + 1];
-            const __nv_bfloat162 pair = __floats2bfloat162_rn(x0, x1);
-            const float h0 = __bfloat162float(pair.x), h1 = __bfloat162float(pair.y);
-            const __nv_bfloat162 rest = __floats2bfloat162_rn(fabsf(h0) < INFINITY ? x0 - h0 : 0.f, fabsf(h1) < INFINITY ? x1 - h1 : 0.f);
-            high[q] = *reinterpret_cast<const uint32_t*>(&pair);
-            low[q] = *reinterpret_cast<const uint32_t*>(&rest);
+            for (int q = 0; q < 4; ++q) packed[q] = at_take_part(v[half][c * 8 + 2 * q], v[half][c * 8 + 2 * q + 1]);
+            if (kept) *reinterpret_cast<uint4*>(row + ((c ^ (t & 7)) << 4)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
           }
-          const int at = (c ^ (t & 7)) << 4;
-          *reinterpret_cast<uint4*>(row + at) = make_uint4(high[0], high[1], high[2], high[3]);
-          *reinterpret_cast<uint4*>(row + STAGE_BYTES + at) = make_uint4(low[0], low[1], low[2], low[3]);
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -324,6 +330,8 @@ template <int BN, int HALVES>
 static int launch(const void* x, const void* w, const void* up, AdapterGemm p, int stages, cudaStream_t stream) {
   constexpr size_t STAGE = HALVES * 128 * 128 + BN * 128;
   p.stages = stages;
+  p.parts = p.out_f32 ? 3 : 2;
+  p.held = p.parts < stages ? p.parts : stages;
   static OncePerDevice once;
   if (cudaError_t err = once([] {
         return cudaFuncSetAttribute(adapter_gemm_kernel<BN, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, 193 * 1024);
@@ -379,7 +387,7 @@ MLR_EXPORT int mlr_adapter_gemm(const void* x, const void* w, const void* up, co
   if (M == 0) return MLR_OK;
   if (K % 8 != 0 || rank % 8 != 0 || (((uintptr_t)x | (uintptr_t)w | (uintptr_t)up | (uintptr_t)u | (uintptr_t)out) & 15) != 0) return MLR_BAD_ALIGNMENT;
   if ((long long)adapters * N > 0x7fffffffll) return MLR_TOO_LARGE;
-  AdapterGemm p{M, N, K, adapters, rank, 0, (const bf16*)bias, u, row_adapter, out, out_f32, error_word};
+  AdapterGemm p{M, N, K, adapters, rank, 0, 0, 0, (const bf16*)bias, u, row_adapter, out, out_f32, error_word};
   const AdapterPlan chosen = plan(M, N, K, sm_count());
   if (chosen.shape == 2) return launch<256, 2>(x, w, up, p, chosen.stages, stream);
   if (chosen.shape == 1) return launch<256, 1>(x, w, up, p, chosen.stages, stream);
