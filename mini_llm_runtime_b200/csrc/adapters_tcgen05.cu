@@ -9,7 +9,8 @@
 // rounded once and an adapter costs its products and the reading of B, no pass over y.  (A kernel that adds the adapters to a shared
 // product in float32 reads and writes 0.5 GB more at 2,048 x 37,888 with K = 3,584 and rank 64: 1,135 us against 500, of which the sums u
 // are 20; 1.12 PFLOP/s, the tensor pipe busy for 72 %.)  u comes in bfloat16 parts of eight bits each, as many left operands for one right
-// one: two for a bfloat16 result, u to 2^-17, a small part of that result's own rounding (2^-8); three for a float32 result, all of u.
+// one: two for a bfloat16 result, u to 2^-16, a small part of that result's own rounding (2^-8); three for a float32 result, all of u.
+// Every part has u's sign and is zero only where u is: an infinite entry of B gives an infinity with each of them, as it does with u.
 //
 // One CTA computes 128 or 256 rows (one or two accumulators) x BN columns.  Warp 0 loads (bulk tensor copies into a ring of
 // 128-byte-swizzled tiles), warp 1 issues the products, warps 2 to 5 list the tile's adapters while the shared product runs,
@@ -42,13 +43,20 @@ __device__ __forceinline__ void at_mma_rows(uint32_t tmem_d, uint64_t a_desc, ui
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n\t}"
       ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(off.x), "r"(off.y), "r"(off.z), "r"(off.w) : "memory");
 }
-// The next bfloat16 part of two numbers, taken off them: the number rounded to eight bits; the third is what is left, exactly.  An
-// infinity is all of its number (what is left of it would be NaN).
-__device__ __forceinline__ uint32_t at_take_part(float& x0, float& x1) {
-  const __nv_bfloat162 pair = __floats2bfloat162_rn(x0, x1);
-  const float h0 = __bfloat162float(pair.x), h1 = __bfloat162float(pair.y);
-  x0 = fabsf(h0) < INFINITY ? x0 - h0 : 0.f;
-  x1 = fabsf(h1) < INFINITY ? x1 - h1 : 0.f;
+// The first eight bits of the number one step of float32 closer to zero than x: of x's sign and less in magnitude, so that what is left of x
+// has its sign too and is not zero.  (Of an infinity the largest bfloat16, which leaves the infinity; NaN leaves NaN.)
+__device__ __forceinline__ float at_part(float x) {
+  const uint32_t bits = __float_as_uint(x);
+  return __uint_as_float((bits - ((bits << 1) != 0u ? 1u : 0u)) & 0xffff0000u);
+}
+template <int N> struct Parts { static constexpr int value = N; };
+// The next bfloat16 part of two numbers, taken off them; last: what is left of them, rounded (of the third part exactly: of u's 24 bits no
+// more than eight are left, or the one that follows them).
+__device__ __forceinline__ uint32_t at_take_part(float& x0, float& x1, bool last) {
+  const float h0 = last ? x0 : at_part(x0), h1 = last ? x1 : at_part(x1);
+  x0 -= h0;
+  x1 -= h1;
+  const __nv_bfloat162 pair = __floats2bfloat162_rn(h0, h1);
   return *reinterpret_cast<const uint32_t*>(&pair);
 }
 __device__ __forceinline__ void at_wait(uint64_t* bar, uint32_t parity, int* error_word, int code, bool& gave_up) {
@@ -234,7 +242,7 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
     if (t == 0) mbar_arrive(&listed);
     const int count = list_count;
     for (int round = 0; round < rounds && count > 0; ++round) {
-      const int chunk = round / passes, part0 = round % passes * p.held, part1 = min(p.parts, part0 + p.held);
+      const int chunk = round / passes, part0 = round % passes * p.held, part1 = part0 + p.held;      // parts kept: [part0, part1)
       // the sums are asked for before their place is free
       float v[HALVES][64];
 #pragma unroll
@@ -249,20 +257,27 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
       }
       if (round == 0) at_wait(&base_done, 0u, p.error_word, 0x9a, gave_up);
       else at_wait(&u_free, (unsigned)(round - 1) & 1u, p.error_word, 0x98, gave_up);
-      for (int part = 0; part < part1; ++part) {      // a part is taken off, and kept if it is this round's
-        const bool kept = part >= part0;
+      auto lay_out = [&](auto parts) {
 #pragma unroll
         for (int half = 0; half < HALVES; ++half) {
-          uint8_t* row = tiles + (part - part0) * STAGE_BYTES + half * HALF_BYTES + t * 128;
+          uint8_t* row = tiles + half * HALF_BYTES + t * 128;      // the first part kept; the next ones a stage on
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
-            uint32_t packed[4];
+            uint8_t* to = row + ((c ^ (t & 7)) << 4);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) packed[q] = at_take_part(v[half][c * 8 + 2 * q], v[half][c * 8 + 2 * q + 1]);
-            if (kept) *reinterpret_cast<uint4*>(row + ((c ^ (t & 7)) << 4)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+            for (int part = 0; part < parts.value; ++part) {
+              uint32_t packed[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                packed[q] = at_take_part(v[half][c * 8 + 2 * q], v[half][c * 8 + 2 * q + 1], part == parts.value - 1);
+              if (parts.value == 2 || (part >= part0 && part < part1))
+                *reinterpret_cast<uint4*>(to + (part - part0) * STAGE_BYTES) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+            }
           }
         }
-      }
+      };
+      if (p.parts == 2) lay_out(Parts<2>());
+      else lay_out(Parts<3>());
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&u_ready);
