@@ -28,7 +28,8 @@ row through its slot.
 
 Shared pages.  A request may start with the leading whole pages of another one that holds the same tokens (``create_request(...,
 prefix=(request, tokens))``): its block table names them, its own pages follow, and the tokens on them count as committed.  The
-request they belong to cannot be released before those that share its pages.  (Whole pages of groups that keep every key; a
+request they belong to cannot be released before those that share its pages.  Created ``lasting``, it is not expected to end: a request that
+does not fit beside such ones is refused instead of left waiting.  (Whole pages of groups that keep every key; a
 window gives pages back and a fixed-size state has none.)
 
 Two admission modes.  With a *promise* (``create_request(..., lifetime_tokens=n)``) the pages of
@@ -99,6 +100,7 @@ class RequestCache:
     shared_pages: int = 0             # leading pages, of every group, that belong to ``prefix_of``
     prefix_of: str | None = None
     sharers: int = 0                  # requests that start with pages of this one
+    lasting: bool = False             # held until its owner releases it, not until it has run
 
     def own(self, group: int) -> list[int]:
         """The pages the request itself holds."""
@@ -230,14 +232,33 @@ class CacheManager:
             return False
         return all(n <= g.num_pages for g, n in zip(self.groups, self.lifetime_pages(lifetime_tokens)))
 
+    def can_be_admitted(self, lifetime_tokens: int, prefix: tuple[str, int] | None = None, *, beside: int = 0) -> bool:
+        """Whether a request will find room once the running ones have ended: beside the lasting requests' pages, and ``beside`` more
+        tokens' pages of a further lasting one."""
+        if not self.can_ever_hold(lifetime_tokens):
+            return False
+        shared = 0
+        if prefix is not None and self.get(prefix[0]).lasting:      # another source's pages are held for this request alone
+            shared = prefix[1] // self.page_size
+        lasting = [request for request in self.requests.values() if request.lasting]
+        return all(count - shared + sum(request.promised[group.index] for request in lasting) + more <= group.num_pages
+                   for group, count, more in zip(self.groups, self.lifetime_pages(lifetime_tokens), self.lifetime_pages(beside)))
+
+    def why_not_admitted(self, request_id: str, lifetime_tokens: int, shared_pages: int) -> str:
+        kept = tuple(sum(r.promised[g.index] for r in self.requests.values() if r.lasting) for g in self.groups)
+        return (f"request {request_id!r} can never be admitted: it needs "
+                f"{tuple(n - shared_pages for n in self.lifetime_pages(lifetime_tokens))} pages per group and "
+                f"{lifetime_tokens} tokens; the pools hold {tuple(g.num_pages for g in self.groups)} pages, "
+                f"{kept} of them kept for requests to share, and requests are limited to {self.max_tokens_per_request} tokens")
+
     # ------------------------------------------------------------------ requests
     def create_request(self, request_id: str, *, lifetime_tokens: int | None = None,
                        temperature: float = 0.0, seed: int = 0,
-                       prefix: tuple[str, int] | None = None) -> RequestCache | None:
+                       prefix: tuple[str, int] | None = None, lasting: bool = False) -> RequestCache | None:
         """Register a request and give it a slot.  With ``lifetime_tokens`` its pages are promised
         now; returns None (nothing changed) if the promise cannot be kept or no slot is free.
         ``temperature`` and ``seed`` go into the slot's record for the sampling kernel.  ``prefix``: the request
-        starts with that many tokens of another one, on its pages."""
+        starts with that many tokens of another one, on its pages.  ``lasting`` (with a promise): others must not wait for it to end."""
         if request_id in self.requests:
             raise ValueError(f"request {request_id!r} already has a cache")
         source, shared = self._shared_pages(request_id, lifetime_tokens, prefix)
@@ -246,15 +267,13 @@ class CacheManager:
                 raise OutOfPages(f"no free request slot (max_requests={self.max_requests})")
             return None
         promised = [0] * len(self.groups)
+        if lasting and lifetime_tokens is None:
+            raise ValueError("a lasting request needs its lifetime_tokens")
         if lifetime_tokens is not None:
             if lifetime_tokens <= 0:
                 raise ValueError("lifetime_tokens must be > 0")
-            if not self.can_ever_hold(lifetime_tokens):
-                raise ValueError(f"request {request_id!r} can never be admitted: it needs "
-                                 f"{self.lifetime_pages(lifetime_tokens)} pages per group and "
-                                 f"{lifetime_tokens} tokens; the pools hold "
-                                 f"{tuple(g.num_pages for g in self.groups)} pages and requests "
-                                 f"are limited to {self.max_tokens_per_request} tokens")
+            if not self.can_be_admitted(lifetime_tokens, prefix):
+                raise ValueError(self.why_not_admitted(request_id, lifetime_tokens, shared))
             wanted = tuple(count - shared for count in self.lifetime_pages(lifetime_tokens))
             done = []
             for group, count in zip(self.groups, wanted):
@@ -269,7 +288,8 @@ class CacheManager:
                                pages=[[] for _ in self.groups],
                                first_live=[0] * len(self.groups),
                                promised=promised,
-                               step_new_pages=[[] for _ in self.groups])
+                               step_new_pages=[[] for _ in self.groups],
+                               lasting=lasting)
         if source is not None:
             source.sharers += 1
             request.shared_pages, request.prefix_of, request.committed = shared, source.request_id, shared * self.page_size

@@ -162,6 +162,8 @@ class ContinuousBatchEngine:
         if any(request_id == self._holder(name) for name in self._prefixes):
             raise ValueError(f"{request_id!r} is the name under which the cache holds a prefix")
         holder, shared = self._shared_by(prefix, prompt_token_ids)
+        if self._prefixes and not self.manager.can_be_admitted(longest, None if holder is None else (holder, shared)):
+            raise ValueError(self.manager.why_not_admitted(request_id, longest, shared // self.manager.page_size))
         request = self.scheduler.submit(request_id, prompt_token_ids, max_new_tokens=max_new_tokens,
                                         eos_token_ids=eos_token_ids, sampling=sampling, prefix=holder, shared=shared)
         self.metrics.register_request(request_id, arrival_ns)
@@ -192,7 +194,14 @@ class ContinuousBatchEngine:
         holder = self._holder(name)
         if self.manager.slots.free_count <= self.scheduler.max_running_requests - len(self.scheduler.running_request_ids):
             raise ValueError(f"the engine was made for {self.manager.max_requests - self.scheduler.max_running_requests} prefixes")
-        if self.manager.create_request(holder, lifetime_tokens=shared) is None:
+        for request_id in self.scheduler.waiting_request_ids:
+            request = self.scheduler.get_request(request_id)
+            named = None if request.prefix is None else (request.prefix, request.shared)
+            if (self.manager.can_be_admitted(request.lifetime_tokens, named)
+                    and not self.manager.can_be_admitted(request.lifetime_tokens, named, beside=shared)):
+                raise OutOfPages(f"beside the {shared // page} pages of prefix {name!r} the waiting request {request_id!r} could never be admitted")
+        beside_others = not self.manager.can_ever_hold(shared) or self.manager.can_be_admitted(shared)
+        if not beside_others or self.manager.create_request(holder, lifetime_tokens=shared, lasting=True) is None:
             raise OutOfPages(f"no room for the {shared // page} pages of prefix {name!r}")
         try:
             portion = self.scheduler.max_batch_tokens
