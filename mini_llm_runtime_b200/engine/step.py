@@ -217,8 +217,11 @@ class ModelRunner:
         self.graph_capture_after = 3
         self._graphs: dict[tuple, _CapturedStep] = {}       # by _graph_key: (batch, sample, feed, context limit, groups of shared prefixes ..)
         self._graph_seen: dict[tuple, int] = {}
-        # Groups of shared prefixes come in many sizes: of the captured steps that hold any, the ones used last are kept.
+        # Groups of shared prefixes come in many sizes: of the captured steps that hold any, the ones used last are kept, and of the sizes
+        # that were not captured yet the ones seen last.
         self.graph_max_shared = 32
+        self.graph_max_shared_seen = 4096
+        self._shared_seen: dict[tuple, int] = {}
         self._shared_shapes: dict[tuple, bool] = {}      # by (requests, sizes of their groups): whether the step's work lists hold them
         self.graph_replays = 0
         # Rules of the requests on their logits (sampling/rules.py), or None.  To be set before the first step: a captured step
@@ -496,8 +499,11 @@ class ModelRunner:
         key = self._graph_key(requests, sample, feed)
         if key in self._graphs:
             return True
-        seen = self._graph_seen.get(key, 0) + 1
-        self._graph_seen[key] = seen
+        known = self._graph_seen if len(key) <= 4 else self._shared_seen
+        seen = known.pop(key, 0) + 1
+        known[key] = seen
+        if known is self._shared_seen and len(known) > self.graph_max_shared_seen:
+            del known[next(iter(known))]
         return seen >= self.graph_capture_after
 
     def _prepare_decode(self, ctx: StepContext, feed: bool) -> None:
@@ -565,7 +571,7 @@ class ModelRunner:
         if len(key) > 4 and len(shaped) >= self.graph_max_shared:
             torch.cuda.synchronize(self.device)            # its last replay has ended
             del self._graphs[shaped[0]]
-            self._graph_seen.pop(shaped[0], None)
+            self._shared_seen.pop(shaped[0], None)
         # first time at this size: give the graph its own buffer for the step's layout, run the
         # step eagerly on it, then capture
         packed = self._pack(entries, requests, want_slots=sample, fixed=True)
