@@ -354,6 +354,8 @@ class ContinuousBatchEngine:
                 self._ahead.wait()
                 self._ahead = None
             failed = self.scheduler.fail_requests(touched)
+            for request_id in failed:
+                self._allowed.pop(request_id, None)
             self.metrics.record_completed(failed, self._clock_ns())
 
     def _start_token_copy(self, request_ids: tuple[str, ...], tokens: torch.Tensor) -> _TokensInFlight:
