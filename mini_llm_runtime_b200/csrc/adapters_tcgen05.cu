@@ -116,6 +116,7 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
       };
       auto load_w = [&](int s, int k) { tma_load_2d(&w_map, &full[s], tiles + (size_t)s * STAGE_BYTES + A_BYTES, k, n0); };
       const int ahead = min(stages, base_blocks);
+      int issued = ahead;      // blocks asked for
       // The kernel before, which makes u, let this one in after its own wait: x was complete then.  The warps that read u wait.
       for (int i = 0; i < ahead; ++i) {
         mbar_expect_tx(&full[i], STAGE_BYTES);
@@ -129,6 +130,7 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
         mbar_expect_tx(&full[s], STAGE_BYTES);
         load_x(s, i * 64);
         load_w(s, i * 64);
+        issued = i + 1;
       }
       at_wait(&listed, 0u, p.error_word, 0x92, gave_up);
       const int blocks = gave_up ? 0 : list_count * rounds;
@@ -139,7 +141,10 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
         mbar_expect_tx(&full[s], B_BYTES);
         const int round = e / list_count, adapter = list[e - round * list_count];
         tma_load_2d(&up_map, &full[s], tiles + (size_t)s * STAGE_BYTES + A_BYTES, round / passes * 64, adapter * p.N + n0);
+        issued = i + 1;
       }
+      // no copy is under way when the CTA ends, should a wait of another warp have run out
+      for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(&full[i % stages], (unsigned)(i / stages) & 1u, p.error_word, 0x9b);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ products

@@ -287,6 +287,7 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
   if (warp >= PT_LOAD_WARP) {
     // ------------------------------------------------------------ loads: keys by one warp, values by another
     const bool values = warp > PT_LOAD_WARP;
+    int issued = 0;      // tiles asked for
     auto load = [&](int j, int page) {
       const int stage = j % STAGES;
       // a stage of keys is free once the scores that read it exist, one of values once its product is done
@@ -302,6 +303,7 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
         uint8_t* dst = ring + (size_t)stage * Shape::STAGE_BYTES + (values ? Shape::TILE_BYTES : 0) + half * Shape::HALF + box * box_rows * 128;
         tma_load_2d(values ? &v_map : &k_map, full, dst, half * 64, (page * c.kv_heads + kv_head) * c.page_size + offset);
       }
+      issued = j + 1;
     };
 #pragma unroll
     for (int j = 0; j < STAGES; ++j)
@@ -313,6 +315,9 @@ prefix_parts_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __g
       pages[0] = pages[1];
       pages[1] = after;
     }
+    // no copy is under way when the CTA ends, should a wait of another warp have run out
+    for (int j = max(0, issued - STAGES); j < issued; ++j)
+      mbar_wait(values ? &ctl.v_full[j % STAGES] : &ctl.k_full[j % STAGES], (unsigned)(j / STAGES) & 1u, error_word, 0x7c);
   } else if (warp == PT_MMA_WARP) {
     // ------------------------------------------------------------ MMAs
     constexpr uint32_t idesc_qk = fa_idesc(PT_ROWS, PT_KEYS, false);
@@ -585,6 +590,7 @@ prefix_own_mma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     const int per = c.heads / c.kv_heads;
     bool gave_up = false;
     if (warp == 4) {
+      int issued = 0;
       for (int j0 = 0; j0 < tiles; j0 += STAGES) {
 #pragma unroll
         for (int i = 0; i < STAGES; ++i) {
@@ -604,10 +610,14 @@ prefix_own_mma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                 tma_load_2d(&k_map, &full[i], dst, half * 64, y);
                 tma_load_2d(&v_map, &full[i], dst + Shape::TILE_BYTES, half * 64, y);
               }
+              issued = j + 1;
             }
           }
         }
       }
+      // no copy is under way when the states take the tiles' place, should a wait of another warp have run out
+      for (int j = max(0, issued - STAGES); j < issued; ++j)
+        mbar_wait(&full[j % STAGES], (unsigned)(j / STAGES) & 1u, error_word, 0x7d);
     }
     // of heads 2t and 2t + 1 (t = lane & 3) of each eight: output rows d = 16 i + g and 8 further (g = lane / 4)
     float o[D / 16][NT][4];
