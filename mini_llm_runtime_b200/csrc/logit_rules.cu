@@ -12,8 +12,9 @@
 // generated.  Beside it a plane of bits, one per word that is not zero.  A row has some thousand known tokens among
 // 152,000, so this kernel reads the plane (19 KB) instead of the words (608 KB) and fetches a word where its bit is set.
 //
-// Bound by memory: 8.25 bytes per logit (read, write, two bits) out of place; in place the bits and the few logits
-// that change.
+// What it has to move: 8.25 bytes per logit (read, write, two bits) out of place; in place the bits and the few logits that change.  Out of
+// place it comes within a quarter of a copy; in place it takes as long (64 x 152,064 18.0 us in a row of captured calls, apart 19.4; 256 x
+// 151,936 68.0 and 67.8): the chains of reads and the issue of instructions per piece (2.3 a cycle), not bytes, are its limit.
 #include "common.cuh"
 
 namespace mlr {
@@ -42,7 +43,8 @@ __device__ __forceinline__ unsigned four_bits(const unsigned* plane, int t0, int
 }
 
 // Without branches: every second warp has a known token among its 128.  x / repetition is x times the reciprocal, which is rounded
-// once per row: up to a second half step of float32 (2^-24), and the division took a third of the kernel's instructions.
+// once per row: up to a second half step of float32 (2^-24).  With a division for each entry 64 x 152,064 takes 24.4 us instead of 23.0, 256 x
+// 151,936 74.9 instead of 68.0.
 __device__ __forceinline__ float penalised(float x, int word, float repetition, float reciprocal, float presence, float frequency) {
   const int made = word & (IN_PROMPT - 1);
   x *= x > 0.f ? reciprocal : repetition;
@@ -54,7 +56,7 @@ __device__ __forceinline__ float penalised(float x, int word, float repetition, 
 // bits, then the words of known tokens), so three portions are under way: the bits of the one after next, the logits and words of the
 // next, the arithmetic of the present one.  (A CTA per portion lives through that chain, 4 us, for 16 KB: 64 x 152,064 logits 36 us, 256 x
 // 151,936 94 us; as it stands 23 and 68, 4.75 TB/s, where a copy of the same logits takes 18.5 and 55 and the bytes alone 12.6 and 50. Few
-// rows are latency: a row of 151,936 4.1 us in a captured step, 8 from the host.)
+// rows are latency: a row of 151,936 2.3 us in a row of captured calls, 8 from the host.)
 // Pieces lie on 16-byte boundaries.  WHOLE: the vocabulary is a multiple of four, every piece is one row's, and so are the words of the
 // history, which start on such a boundary too; else a row starts inside a piece, its first and last piece go entry by entry, and the words
 // of a slot whose row of them starts on another boundary as well.

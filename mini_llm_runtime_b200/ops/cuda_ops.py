@@ -1133,11 +1133,14 @@ class CudaOps:
     # of 64 over 2, 8 x 2,048 keys (7 MB) 9.7 / 7.3, 32 x 2,048 (32 MB) 10.2 / 9.3, 16 x 8,192 (63 MB) 13.0 / 14.6, 64 x 2,048 (66 MB) 10.3 / 13.2,
     # 64 x 8,192 (264 MB) 19 / 28; 28 heads of 128 over 4, 2 x 8,192 (17 MB) 15.6 / 14.9, 8 x 2,048 (29 MB) 11.3 / 12.1, 32 x 512 (32 MB) 11.1 /
     # 12.3, 4 x 8,192 (50 MB) 14.2 / 15.7, 64 x 512 (66 MB) 13.5 / 16.7, 64 x 8,192 (1 GB) 25 / 126; 40 heads of 128 over 8, 2 x 8,192 (33 MB) 13.0 /
-    # 15.6, 8 x 2,048 (59 MB) 9.8 / 13.2, 64 x 8,192 (2 GB) 33 / 181.  From the host 21 / 17 where neither's kernels take longer.
+    # 15.6, 8 x 2,048 (59 MB) 9.8 / 13.2, 64 x 8,192 (2 GB) 33 / 181.  From the host 21 / 17 where neither's kernels take longer.  One border for
+    # all: it is right for two kv heads; with four and eight, where the heads' walks fill the device sooner, prefixes of 29 to 48 MB go the way that
+    # takes 1 to 3 us longer in a captured step.
     SHARED_PREFIX_LEAST = 48 << 20
 
     def shares_prefix(self, dtype: torch.dtype, counts: dict, num_kv_heads: int, head_dim: int) -> bool:
-        """Whether the prefixes of ``plan_shared_prefix`` are worth their own walk on the tensor cores."""
+        """Whether the prefixes of ``plan_shared_prefix`` are worth their own walk on the tensor cores.  (Never in 32 bits or at other head
+        sizes: a model's decode steps attend request by request there.  The general kernels, which read a prefix once, serve direct calls.)"""
         return (self.use_mma_attention and dtype == torch.bfloat16 and head_dim in (64, 128) and counts["heads_per_kv"] <= 16
                 and 4 * counts["saved_keys"] * num_kv_heads * head_dim >= self.shared_prefix_least)
 

@@ -18,7 +18,7 @@ from .params import SamplingParams
 
 
 class LogitRules:
-    """The tables of ``max_requests`` slots over ``vocab_size`` tokens (4.4 bytes per slot and token)."""
+    """The tables of ``max_requests`` slots over ``vocab_size`` tokens (4.25 bytes per slot and token, 8 per bias of a slot)."""
 
     def __init__(self, max_requests: int, vocab_size: int, device: torch.device | str, *, max_biases: int = 300) -> None:
         if max_requests <= 0 or vocab_size <= 0 or max_biases < 0:
