@@ -165,13 +165,14 @@ prefix_parts_plain_kernel(const PrefixCall c) {
 // 70, 33 and 25 requests behind 16,384, 9,001 and 4,100 keys, 40 heads of 128 over 8: 54 us, of which a CTA's 36 tiles of 64 keys take 39, at
 // 1,830 cycles each and 1.7 GHz (two CTAs on an SM: 710 exponentials and sums, 310 the row's largest score and the other half's, 370
 // storing the probabilities, 190 the previous product, 250 the scores and reading them).  Where a part is short the rest is the larger half: 64
-// requests behind 8,192 keys, 28 heads of 128 over 4, eight tiles a CTA, 18.7 us, of a CTA's 15: 2.4 until lists and tables are read and tensor memory is
-// there, 2.8 to the scores of the second tile, 6.6 the other tiles, 1.4 the last product, 1.9 the output.  Eleven warps: eight of softmax, two threads per query row (tensor-memory lane), 32 keys of a tile each, which lend each
-// other their largest score; one that issues S = Q K^T two key tiles ahead and O += P V, P in tensor memory where S was; one that loads K and
-// one that loads V, page by page through bulk tensor copies into a ring (one warp for both, sixteen copies per tile with pages of 16 keys, was
-// the limit before: 58 us).  Probabilities are rounded to bfloat16 for the product with V, as in the other attention kernels on tensor cores: half
-// a step (2^-8) of each weight, not of the sums, which add the 32-bit ones (a result's error 0.0023 of its size, where 32-bit weights and the
-// rounding of the result make 0.0017); a second part would add half as many products again.  The output stays in tensor memory relative to a base exponent that follows the running max in steps of 2^8.
+// requests behind 8,192 keys, 28 heads of 128 over 4, eight tiles a CTA, 18.7 us, of a CTA's 15: 2.4 until lists are read and tensor memory is
+// there, 2.8 to the scores of the second tile, 6.5 the other tiles, 1.4 the last product, 1.9 the output.  Eleven warps: eight of softmax, two
+// threads per query row (tensor-memory lane), 32 keys of a tile each, which lend each other their largest score; one that issues S = Q K^T two
+// key tiles ahead and O += P V, P in tensor memory where S was; one that loads K and one that loads V, page by page through bulk tensor copies
+// into a ring (one warp for both, sixteen copies per tile with pages of 16 keys, was the limit before: 58 us).  Probabilities are rounded to
+// bfloat16 for the product with V, as in the other attention kernels on tensor cores: half a step (2^-8) of each weight, not of the sums, which
+// add the 32-bit ones (a result's error 0.0023 of its size, where 32-bit weights and the rounding of the result make 0.0017); a second part
+// would add half as many products again.  The output stays in tensor memory relative to a base exponent that follows the running max in steps of 2^8.
 // The query rows lie in the q of as many requests: the softmax threads gather them.  (One thread per row with P in shared memory: the
 // whole call 102 us where two and P in tensor memory took 97.  Q in tensor memory too leaves room for one tile's scores, softmax and products
 // in turn: slower.)

@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS)
 sample_kernel(const float* logits, const float* __restrict__ temperatures,
               const long long* __restrict__ seeds, const long long* __restrict__ counters,
               int* __restrict__ tokens, int vocab, const int* __restrict__ row_slot, SlotState* state,
-              int advance) {
+              int advance, int wide) {
   // With `state`, a row's temperature, seed and counter come from the slot record of its request
   // (row_slot[row]); the chosen token is also written there as the request's last token, the
   // counter grows by one and, with `advance`, so does the slot's length (a step in which every
@@ -49,7 +49,7 @@ sample_kernel(const float* logits, const float* __restrict__ temperatures,
   // ---- argmax with the lowest index on ties (also gives the softmax's max)
   float best = -INFINITY;
   int best_index = vocab;
-  if ((vocab & 3) == 0) {
+  if (wide) {
     // 16-byte loads, four rounds in flight: the row is walked by one CTA, so the loop is a chain of
     // load latencies and fewer, wider rounds are what shortens it
     const float4* row4 = reinterpret_cast<const float4*>(row);
@@ -139,7 +139,7 @@ sample_kernel(const float* logits, const float* __restrict__ temperatures,
   const bool mine = target >= before && (target < before + total || warp == last);
   if (mine) {
     float running = before;
-    int found = -1, possible = -1;       // possible: the last entry of the walk so far with any probability
+    int found = -1;
     for (int base = begin; base < end && found < 0; base += 32) {
       const int i = base + lane;
       const float e = i < end ? expf((row[i] - row_max) * inv_t) : 0.f;
@@ -149,13 +149,17 @@ sample_kernel(const float* logits, const float* __restrict__ temperatures,
         const float up = __shfl_up_sync(0xffffffffu, inclusive, offset);
         if (lane >= offset) inclusive += up;
       }
-      const unsigned some = __ballot_sync(0xffffffffu, e > 0.f);
-      const unsigned hit = __ballot_sync(0xffffffffu, running + inclusive > target) & some;
+      const unsigned hit = __ballot_sync(0xffffffffu, e > 0.f && running + inclusive > target);
       if (hit != 0u) found = base + (__ffs(hit) - 1);
-      if (some != 0u) possible = base + 31 - __clz(some);
       running += __shfl_sync(0xffffffffu, inclusive, 31);
     }
-    if (lane == 0) chosen = found >= 0 ? found : possible;
+    // not reached (one draw in a million): back to the last entry with any probability
+    for (int base = begin + (end - begin - 1) / 32 * 32; base >= begin && found < 0; base -= 32) {
+      const int i = base + lane;
+      const unsigned some = __ballot_sync(0xffffffffu, i < end && expf((row[i] - row_max) * inv_t) > 0.f);
+      if (some != 0u) found = base + 31 - __clz(some);
+    }
+    if (lane == 0) chosen = found;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -176,6 +180,9 @@ using namespace mlr;
 
 MLR_DEFINE_PDL_SWITCH
 
+// Rows are read 16 bytes at a time where they start on such boundaries.
+static int starts_wide(const float* logits, int vocab) { return (vocab & 3) == 0 && ((uintptr_t)logits & 15) == 0; }
+
 // temperatures[r] <= 0 selects greedy for row r.  tokens: int32 [rows].
 MLR_EXPORT int mlr_sample(const float* logits, const float* temperatures, const long long* seeds,
                           const long long* counters, int* tokens, int rows, int vocab,
@@ -183,7 +190,7 @@ MLR_EXPORT int mlr_sample(const float* logits, const float* temperatures, const 
   if (rows == 0) return MLR_OK;
   if (rows < 0 || vocab <= 0) return MLR_BAD_SIZE;
   launch_kernel(sample_kernel, dim3(rows), dim3(SAMPLE_THREADS), 0, stream, logits, temperatures, seeds, counters,
-                tokens, vocab, (const int*)nullptr, (SlotState*)nullptr, 0);
+                tokens, vocab, (const int*)nullptr, (SlotState*)nullptr, 0, starts_wide(logits, vocab));
   return launch_status();
 }
 
@@ -196,6 +203,6 @@ MLR_EXPORT int mlr_sample_slots(const float* logits, const int* row_slot, void* 
   if (rows < 0 || vocab <= 0 || row_slot == nullptr || state == nullptr) return MLR_BAD_SIZE;
   launch_kernel(sample_kernel, dim3(rows), dim3(SAMPLE_THREADS), 0, stream, logits, (const float*)nullptr,
                 (const long long*)nullptr, (const long long*)nullptr, tokens, vocab, row_slot, (SlotState*)state,
-                advance);
+                advance, starts_wide(logits, vocab));
   return launch_status();
 }

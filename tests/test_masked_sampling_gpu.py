@@ -108,3 +108,20 @@ def test_an_infinite_logit_is_the_choice(temperature):
     row[::3] = torch.linspace(-5, 5, 334)
     row[333] = math.inf
     assert draw(row, range(20), temperature).unique().tolist() == [333]
+
+
+@pytest.mark.parametrize("vocab", [1000, 1003, 32000])
+@pytest.mark.parametrize("entries", [0, 1, 2, 3])
+def test_logits_on_any_boundary(vocab, entries):
+    """A view into a larger tensor: the same tokens as from a tensor of its own, greedy and drawn."""
+    rows = 5
+    g = torch.Generator().manual_seed(vocab)
+    logits = torch.randn((rows, vocab), generator=g).to(DEVICE)
+    view = torch.empty(rows * vocab + 8, device=DEVICE)[entries:entries + rows * vocab].view(rows, vocab)
+    view.copy_(logits)
+    for temperature in (0.0, 1.0):
+        options = (torch.full((rows,), temperature, device=DEVICE), torch.arange(rows, device=DEVICE), torch.arange(rows, device=DEVICE))
+        got = ops.current().sample(view, *options)
+        assert torch.equal(got, ops.current().sample(logits, *options))
+        if temperature == 0:
+            assert torch.equal(got.long(), logits.argmax(dim=1))
