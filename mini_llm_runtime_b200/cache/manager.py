@@ -211,6 +211,7 @@ class CacheManager:
         # step's slots is taken at begin_step)
         self.backup_state = True
         self.requests: dict[str, RequestCache] = {}
+        self._lasting: dict[str, RequestCache] = {}
         self._step: list[tuple[RequestCache, int]] | None = None
         self._state_backup: tuple[torch.Tensor, dict[int, torch.Tensor]] | None = None
 
@@ -240,16 +241,17 @@ class CacheManager:
         shared = 0
         if prefix is not None and self.get(prefix[0]).lasting:      # another source's pages are held for this request alone
             shared = prefix[1] // self.page_size
-        lasting = [request for request in self.requests.values() if request.lasting]
-        return all(count - shared + sum(request.promised[group.index] for request in lasting) + more <= group.num_pages
-                   for group, count, more in zip(self.groups, self.lifetime_pages(lifetime_tokens), self.lifetime_pages(beside)))
+        return all(count - shared + kept + more <= group.num_pages for group, count, kept, more in zip(
+            self.groups, self.lifetime_pages(lifetime_tokens), self._lasting_pages(), self.lifetime_pages(beside)))
+
+    def _lasting_pages(self) -> tuple[int, ...]:
+        return tuple(sum(request.promised[group.index] for request in self._lasting.values()) for group in self.groups)
 
     def why_not_admitted(self, request_id: str, lifetime_tokens: int, shared_pages: int) -> str:
-        kept = tuple(sum(r.promised[g.index] for r in self.requests.values() if r.lasting) for g in self.groups)
         return (f"request {request_id!r} can never be admitted: it needs "
                 f"{tuple(n - shared_pages for n in self.lifetime_pages(lifetime_tokens))} pages per group and "
                 f"{lifetime_tokens} tokens; the pools hold {tuple(g.num_pages for g in self.groups)} pages, "
-                f"{kept} of them kept for requests to share, and requests are limited to {self.max_tokens_per_request} tokens")
+                f"{self._lasting_pages()} of them kept for requests to share, and requests are limited to {self.max_tokens_per_request} tokens")
 
     # ------------------------------------------------------------------ requests
     def create_request(self, request_id: str, *, lifetime_tokens: int | None = None,
@@ -298,6 +300,8 @@ class CacheManager:
                 group.table[slot, :shared] = request.pages[group.index]
                 group.dirty.add(slot)
         self.requests[request_id] = request
+        if lasting:
+            self._lasting[request_id] = request
         for tensor in self._state_tensors():
             tensor[slot].zero_()
         self.slot_mirror[slot] = slot_record(length=request.committed, temperature=temperature, seed=seed)
@@ -351,6 +355,7 @@ class CacheManager:
             freed[group.index] = ids
         self.slots.free([request.slot])
         del self.requests[request_id]
+        self._lasting.pop(request_id, None)
         if request.prefix_of is not None:
             self.requests[request.prefix_of].sharers -= 1
         return freed
