@@ -5,6 +5,8 @@
 //
 // A part of a row's keys leaves a state (m, l, o): the largest exponent, the sum and the unnormalised output relative to it.
 // States of parts add up after scaling by exp(m - max m), in the order of the parts, so the split changes only roundings.
+// Exponents, sums and outputs are 32-bit; on the tensor cores the weights p are rounded to bfloat16 for their product with V (beside the
+// prefix kernel: what that costs), as they are where each request attends by itself.
 //
 // Parts of one (request, head), each with a place of its own in scratch memory:
 //   0 .. prefix_parts - 1              `chunk` keys of the prefix each, as many as the request's prefix has
