@@ -1179,8 +1179,8 @@ class CudaOps:
         if segments == 0:
             return out
         if (fast and segments * num_kv_heads <= self.ATTENTION_COUNTERS and "decode_seg" in batch.plan
-                and not self.shares_prefix(q.dtype, counts, num_kv_heads, head_dim)):
-            # what paged_attention runs for such a step
+                and 4 * counts["saved_keys"] * num_kv_heads * head_dim < self.shared_prefix_least):
+            # not what shares_prefix calls worth it: what paged_attention runs for such a step
             self._decode_attention(q, k_pool, v_pool, out, batch, num_heads, num_kv_heads, head_dim, scale, None, mma=True)
             return out
         fast = fast and k_pool.shape[0] * num_kv_heads * page_size < 1 << 31
