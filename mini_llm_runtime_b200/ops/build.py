@@ -68,6 +68,9 @@ LIBRARIES: dict[str, tuple[str, ...]] = {
     "adapters_small": (),
     "adapters_tcgen05": (),
     "attention_prefix": (),
+    "quantized_pages": (),
+    "copy_pages": (),
+    "attention_quantized": (),
 }
 
 _loaded: dict[str, ctypes.CDLL] = {}

@@ -111,6 +111,9 @@ _PROTOTYPES = {
     "adapters_small": {"mlr_adapter_small": "pppppppp" "iiiiiii" "p"},
     "adapters_tcgen05": {"mlr_adapter_gemm": "ppppppp" "iiiiii" "pp"},
     "logit_rules": {"mlr_logit_rules": "pppiipp", "mlr_count_tokens": "ppippiiip"},
+    "quantized_pages": {"mlr_quantize_kv": "plplp" "pppp" "iiiiii" "ip", "mlr_dequantize_pages": "ppppppp" "iiiiii" "ip"},
+    "copy_pages": {"mlr_copy_pages": "pippip"},
+    "attention_quantized": {"mlr_attention_quantized": "pppppp" "ppppppp" "iiiiiiiii" "fip"},
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 _declared: dict[str, ctypes.CDLL] = {}
@@ -268,6 +271,39 @@ class AdapterStack:
         # what a call asks for, once
         for name, value in (("count", adapters), ("rank", rank), ("inner", self.down.shape[2]), ("outer", self.up.shape[1]),
                             ("dtype", self.down.dtype), ("device", self.down.device)):
+            object.__setattr__(self, name, value)
+
+
+@dataclass(frozen=True)
+class QuantizedPool:
+    """Keys and values of a paged cache in 8 bits: ``key`` and ``value`` int8 [pages, kv_heads, page_size, dim], ``key_scales`` and
+    ``value_scales`` float32 [pages, kv_heads, page_size / block]: one scale (>= 0) for each block of ``block`` tokens of a page and kv
+    head.  A number stands for code * scale; codes lie between -127 and 127.  A block of one token up to a page.  Checked here, once,
+    and against the step at each call."""
+
+    key: torch.Tensor
+    value: torch.Tensor
+    key_scales: torch.Tensor
+    value_scales: torch.Tensor
+
+    def __post_init__(self) -> None:
+        for name in ("key", "value"):
+            _need(getattr(self, name), name, torch.int8, 4)
+            _need(getattr(self, name + "_scales"), name + "_scales", torch.float32, 3)
+        pages, kv_heads, page_size, dim = self.key.shape
+        if self.value.shape != self.key.shape or self.value_scales.shape != self.key_scales.shape:
+            raise KernelError(f"keys {tuple(self.key.shape)} and values {tuple(self.value.shape)}, scales {tuple(self.key_scales.shape)} and "
+                              f"{tuple(self.value_scales.shape)} must have one shape each")
+        blocks = self.key_scales.shape[2]
+        if min(pages, kv_heads, page_size, dim, blocks) < 1 or dim > 256:
+            raise KernelError(f"a pool of shape {tuple(self.key.shape)} is not supported (head sizes of 1 to 256)")
+        if self.key_scales.shape[:2] != (pages, kv_heads) or page_size % blocks:
+            raise KernelError(f"scales of shape {tuple(self.key_scales.shape)} do not belong to pages of shape {tuple(self.key.shape)}")
+        if pages * kv_heads * page_size >= 1 << 31:
+            raise KernelError("a pool holds fewer than 2^31 heads' tokens")
+        _need_together(self.key, self.value, self.key_scales, self.value_scales)
+        for name, value in (("pages", pages), ("kv_heads", kv_heads), ("page_size", page_size), ("dim", dim), ("block", page_size // blocks),
+                            ("device", self.key.device)):
             object.__setattr__(self, name, value)
 
 
@@ -1124,6 +1160,124 @@ class CudaOps:
                 page_size, int(window or 0), ctypes.c_float(scale), _code(q.dtype), _stream()),
                 "paged_attention")
         return out
+
+    # ------------------------------------------------------------------ a cache in 8 bits
+    def quantize_kv_write(self, key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, pool: QuantizedPool) -> None:
+        """Store keys and values [rows, kv_heads * dim] (float32 or bfloat16; rows may lie apart, as column ranges of wider rows do) at
+        ``slots`` int64 [rows] (page * page_size + offset) of the pool.  The first token of a block sets the block's scale anew; with
+        later ones it grows to the larger of itself and amax / 127, and the tokens before are rounded to it.  The rows of a
+        block follow one another in ascending order, as a request's tokens do, and no slot comes twice; a slot
+        outside the pool is passed over.  A block with an infinite or NaN entry gets the scale NaN."""
+        width = pool.kv_heads * pool.dim
+        _code(key.dtype)
+        _need(slots, "slots", torch.int64, 1)
+        rows = slots.shape[0]
+        strides = []
+        for name, tensor in (("key", key), ("value", value)):
+            if (not tensor.is_cuda or tensor.dtype != key.dtype or tensor.shape != (rows, width) or (width > 1 and tensor.stride(1) != 1)
+                    or (rows > 1 and tensor.stride(0) < width)):
+                raise KernelError(f"{name} must be a {key.dtype} CUDA view [{rows}, {width}] with unit column stride, got {tensor.dtype} "
+                                  f"{tuple(tensor.shape)}")
+            strides.append(tensor.stride(0) if rows > 1 else width)
+        _need_here(key=key, value=value, slots=slots, pool=pool)
+        if rows == 0:
+            return
+        _check(_declared_library("quantized_pages").mlr_quantize_kv(
+            key.data_ptr(), strides[0], value.data_ptr(), strides[1], slots.data_ptr(), pool.key.data_ptr(), pool.value.data_ptr(), pool.key_scales.data_ptr(),
+            pool.value_scales.data_ptr(), rows, pool.kv_heads, pool.dim, pool.page_size, pool.block, pool.pages, _code(key.dtype),
+            _raw_stream()), "quantize_kv_write")
+
+    def dequantize_pages(self, pool: QuantizedPool, pages: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+        """What the codes of ``pages`` int32 [n] stand for: keys and values [n, kv_heads, page_size, dim].  A page that the pool does not
+        have (-1 in a block table) gives zeros."""
+        _need(pages, "pages", torch.int32, 1)
+        _need_here(pages=pages, pool=pool)
+        shape = (pages.shape[0], pool.kv_heads, pool.page_size, pool.dim)
+        key, value = (torch.empty(shape, dtype=out_dtype, device=pool.device) for _ in range(2))
+        if pages.shape[0] == 0:
+            return key, value
+        _check(_declared_library("quantized_pages").mlr_dequantize_pages(
+            pool.key.data_ptr(), pool.value.data_ptr(), pool.key_scales.data_ptr(), pool.value_scales.data_ptr(), pages.data_ptr(),
+            key.data_ptr(), value.data_ptr(), pages.shape[0], pool.kv_heads, pool.dim, pool.page_size, pool.block, pool.pages, _code(out_dtype),
+            _raw_stream()), "dequantize_pages")
+        return key, value
+
+    def quantized_attention(self, q: torch.Tensor, pool: QuantizedPool, batch: AttentionBatch, num_heads: int, num_kv_heads: int, head_dim: int,
+                            scale: float, window: int | None = None) -> torch.Tensor:
+        """``paged_attention`` over keys and values in 8 bits: every row of the step attends to its request's cached keys, its own
+        among them.  ``q`` [rows, heads * dim] in float32 or bfloat16, the result likewise."""
+        _need(q, "q", dims=2)
+        _code(q.dtype)
+        if num_kv_heads < 1 or num_heads < 1 or num_heads % num_kv_heads:
+            raise KernelError(f"{num_heads} heads over {num_kv_heads} kv heads are not supported")
+        if q.shape[1] != num_heads * head_dim:
+            raise KernelError(f"q rows have {q.shape[1]} entries, expected {num_heads * head_dim}")
+        if pool.kv_heads != num_kv_heads or pool.dim != head_dim:
+            raise KernelError(f"the pool holds {pool.kv_heads} kv heads of {pool.dim}, expected {num_kv_heads} of {head_dim}")
+        if "tile_seg" not in batch.plan:
+            raise KernelError("the batch carries no attention work lists (plan_attention)")
+        _need(batch.block_table, "block_table", torch.int32, 2)
+        _need_here(q=q, pool=pool, block_table=batch.block_table)
+        out = torch.empty_like(q)
+        if q.shape[0] == 0:
+            return out
+        plan, counts = batch.plan, batch.counts
+        _check(_declared_library("attention_quantized").mlr_attention_quantized(
+            q.data_ptr(), pool.key.data_ptr(), pool.value.data_ptr(), pool.key_scales.data_ptr(), pool.value_scales.data_ptr(), out.data_ptr(),
+            plan["tile_seg"].data_ptr(), plan["tile_row0"].data_ptr(), batch.seg_q_start.data_ptr(), batch.seg_q_len.data_ptr(),
+            batch.seg_pos0.data_ptr(), batch.block_table.data_ptr(), batch.seg_slot.data_ptr(), batch.block_table.shape[1], counts["tiles"],
+            num_heads, num_kv_heads, head_dim, pool.page_size, pool.block, pool.pages, int(window or 0), scale, _code(q.dtype), _raw_stream()),
+            "quantized_attention")
+        return out
+
+    # ------------------------------------------------------------------ pages of a cache
+    COPY_POOLS = 8      # of one launch (copy_pages.cu)
+
+    def copy_pages(self, pools, source, target, into=None) -> None:
+        """``pool[:, target[i]] = pool[:, source[i]]`` for each of ``pools``, contiguous tensors [entries, pages, ..] of one number of pages and
+        any types.  ``into``: the pools that the pages go to, of the same entries and page shapes, each its own memory (default:
+        ``pools`` themselves, and then no page may be source and target).  ``source`` and ``target`` are page numbers on the host, no
+        target twice."""
+        pools = list(pools)
+        targets = pools if into is None else list(into)
+        source, target = (np.ascontiguousarray(list(pages), dtype=np.int64) for pages in (source, target))
+        if source.ndim != 1 or source.shape != target.shape:
+            raise KernelError("source and target need one page number each")
+        if len(targets) != len(pools):
+            raise KernelError(f"{len(pools)} pools cannot be copied into {len(targets)}")
+        for what, side, numbers in (("source", pools, source), ("target", targets, target)):
+            for pool in side:
+                _need(pool, f"a {what} pool")
+                _need_here(**{f"a {what} pool": pool})
+                if pool.dim() < 2 or pool.shape[1] != side[0].shape[1]:
+                    raise KernelError(f"the {what} pools must have one number of pages")
+            if side and len(numbers) and (numbers.min() < 0 or numbers.max() >= side[0].shape[1]):
+                raise KernelError(f"{what} pages must lie in [0, {side[0].shape[1]})")
+        if len(np.unique(target)) != len(target):
+            raise KernelError("a page is the target of one copy")
+        if into is None:
+            if np.isin(target, source).any():
+                raise KernelError("a page cannot be source and target")
+        else:
+            for pool, other in zip(pools, targets):
+                if other.dtype != pool.dtype or other.shape[0] != pool.shape[0] or other.shape[2:] != pool.shape[2:]:
+                    raise KernelError(f"pages of {tuple(pool.shape)} {pool.dtype} do not fit {tuple(other.shape)} {other.dtype}")
+            spans = [[(pool.data_ptr(), pool.data_ptr() + pool.numel() * pool.element_size()) for pool in group] for group in (pools, targets)]
+            if any(first < end and begin < last for begin, end in spans[0] for first, last in spans[1]):
+                raise KernelError("the pools that pages go to must not be those that they come from")
+        count = len(source)
+        fields = []
+        for pool, other in zip(pools, targets):
+            page = pool[0, 0].numel() * pool.element_size() if pool.numel() else 0
+            if page:
+                fields.append((pool.data_ptr(), other.data_ptr(), pool.shape[1] * page, other.shape[1] * page, page, pool.shape[0]))
+        if not fields or not count:
+            return
+        source, target = source.astype(np.int32), target.astype(np.int32)
+        entry = _declared_library("copy_pages").mlr_copy_pages
+        for first in range(0, len(fields), self.COPY_POOLS):
+            some = np.asarray(fields[first:first + self.COPY_POOLS], dtype=np.int64)
+            _check(entry(some.ctypes.data, len(some), source.ctypes.data, target.ctypes.data, count, _raw_stream()), "copy_pages")
 
     def plan_shared_prefix(self, groups, num_segments, heads_per_kv):
         return plan_shared_prefix(groups, num_segments, heads_per_kv)
