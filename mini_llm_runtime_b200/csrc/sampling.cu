@@ -10,20 +10,12 @@
 // that a grammar or a ban forbids) is never chosen: the sum that says which warp's stretch the target falls into and the running sum
 // of the walk through it round differently, so the walk may not reach the target, and then ends at the stretch's last
 // token that has any.  A row of -inf throughout has no distribution: token 0, as greedy.  Any vocabulary size is accepted.
-#include "common.cuh"
+#include "uniform.cuh"
 
 namespace mlr {
 
 constexpr int SAMPLE_THREADS = 1024;
 constexpr int SAMPLE_WARPS = SAMPLE_THREADS / 32;
-
-__device__ __forceinline__ float uniform_from_seed(unsigned long long seed, long long index) {
-  unsigned long long z = seed + (unsigned long long)(index + 1) * 0x9E3779B97F4A7C15ull;
-  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
-  z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-  z = z ^ (z >> 31);
-  return (float)(z >> 40) * (1.0f / 16777216.0f);
-}
 
 __global__ void __launch_bounds__(SAMPLE_THREADS)
 sample_kernel(const float* logits, const float* __restrict__ temperatures,

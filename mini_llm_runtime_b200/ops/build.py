@@ -70,6 +70,7 @@ LIBRARIES: dict[str, tuple[str, ...]] = {
     "attention_prefix": (),
     "quantized_pages": (),
     "copy_pages": (),
+    "sampling_limits": (),
     "attention_quantized": (),
 }
 

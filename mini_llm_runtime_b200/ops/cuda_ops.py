@@ -113,6 +113,7 @@ _PROTOTYPES = {
     "logit_rules": {"mlr_logit_rules": "pppiipp", "mlr_count_tokens": "ppippiiip"},
     "quantized_pages": {"mlr_quantize_kv": "plplp" "pppp" "iiiiii" "ip", "mlr_dequantize_pages": "ppppppp" "iiiiii" "ip"},
     "copy_pages": {"mlr_copy_pages": "pippip"},
+    "sampling_limits": {"mlr_sample_limited": "pppppppp" "ii" "p" "ii" "p"},
     "attention_quantized": {"mlr_attention_quantized": "pppppp" "ppppppp" "iiiiiiiii" "fip"},
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
@@ -240,6 +241,37 @@ class LogitTables:
                                                   0 if self.bias_tokens is None else self.bias_tokens.shape[1], slots))):
             object.__setattr__(self, name, value)
         object.__setattr__(self, "rules_at", ctypes.addressof(self.rules))
+
+
+@dataclass(frozen=True)
+class SamplingLimits:
+    """What may be drawn, one entry per row of logits or, read by slot, per slot: ``temperatures`` float32 (0 and below take the best
+    token), ``top_k`` int32 (the k best tokens; 0 and below: no limit), ``top_p`` float32 (the fewest tokens that hold p of the probability;
+    1 and above: no limit), ``min_p`` float32 (tokens at least so many times as probable as the best; 0: no limit, above 1 counts as 1).  The best
+    token always stays.  Each but the temperatures may be None, and these where the slot records hold them.  Checked here, once."""
+
+    temperatures: torch.Tensor | None = None
+    top_k: torch.Tensor | None = None
+    top_p: torch.Tensor | None = None
+    min_p: torch.Tensor | None = None
+
+    def __post_init__(self) -> None:
+        entries = None
+        for name, dtype in (("temperatures", torch.float32), ("top_k", torch.int32), ("top_p", torch.float32), ("min_p", torch.float32)):
+            tensor = getattr(self, name)
+            if tensor is None:
+                continue
+            _need(tensor, name, dtype, 1)
+            if entries is not None and tensor.shape[0] != entries:
+                raise KernelError(f"{name} has {tensor.shape[0]} entries, the limits before it {entries}")
+            entries = tensor.shape[0]
+        if entries is None:
+            raise KernelError("the limits hold none")
+        _need_together(self.temperatures, self.top_k, self.top_p, self.min_p)
+        first = next(t for t in (self.temperatures, self.top_k, self.top_p, self.min_p) if t is not None)
+        for name, value in (("entries", entries), ("device", first.device),
+                            ("addresses", tuple(_address(t) for t in (self.temperatures, self.top_k, self.top_p, self.min_p)))):
+            object.__setattr__(self, name, value)
 
 
 @dataclass(frozen=True)
@@ -748,15 +780,20 @@ class CudaOps:
             "advance_slots")
 
     def sample_slots(self, logits: torch.Tensor, row_slot: torch.Tensor, slot_state: torch.Tensor,
-                     advance: bool = False) -> torch.Tensor:
+                     advance: bool = False, limits: SamplingLimits | None = None) -> torch.Tensor:
         """``sample`` with temperature, seed and counter read from the slot record of each row's
         request; the record receives the token and its counter grows by one (with ``advance`` its
-        length too).  A request may own at most one row."""
+        length too).  A request may own at most one row.  ``limits``: the same draw under the limits of the row's slot
+        (``sample_limited``, which sums in 64 bits)."""
         _need(logits, "logits", torch.float32, 2)
         _need(row_slot, "row_slot", torch.int32, 1)
         _need(slot_state, "slot_state", torch.int32, 2)
         if row_slot.shape[0] != logits.shape[0]:
             raise KernelError("row_slot needs one entry per logits row")
+        if limits is not None:
+            if limits.entries != slot_state.shape[0]:
+                raise KernelError(f"the limits have {limits.entries} slots, the records {slot_state.shape[0]}")
+            return self._sample_limited(logits, None, limits, row_slot, slot_state, advance)
         tokens = torch.empty((logits.shape[0],), dtype=torch.int32, device=logits.device)
         _check(build.load_library("sampling").mlr_sample_slots(
             _ptr(logits), _ptr(row_slot), _ptr(slot_state), _ptr(tokens), logits.shape[0], logits.shape[1],
@@ -2782,6 +2819,37 @@ class CudaOps:
         lib = build.load_library("sampling")
         _check(lib.mlr_sample(_ptr(logits), _ptr(temperatures), _ptr(seeds), _ptr(counters), _ptr(tokens),
                               rows, logits.shape[1], _stream()), "sample")
+        return tokens
+
+    def sample_limited(self, logits: torch.Tensor, uniforms: torch.Tensor, limits: SamplingLimits,
+                       row_slot: torch.Tensor | None = None) -> torch.Tensor:
+        """One token per row of float32 logits, drawn under ``limits`` with the given random numbers ``uniforms`` float32 [rows] in [0, 1).  Of the
+        tokens by falling logit (ties by rising index) the first ``top_k`` stay, of them those at least ``min_p`` times as probable
+        as the best, of them the fewest whose probability comes to ``top_p`` of theirs; the token is the first, in the order of the vocabulary,
+        at which the sum of what stays exceeds the random number times the whole.  ``row_slot`` int32 [rows]: the entry of ``limits`` that
+        holds for the row (an entry that they do not have: the best token).  NaN logits count as -inf; a row of -inf takes token 0."""
+        _need(uniforms, "uniforms", torch.float32, 1)
+        if limits.temperatures is None:
+            raise KernelError("sample_limited needs temperatures")
+        rows = logits.shape[0]
+        if uniforms.shape[0] != rows or (row_slot is None and limits.entries != rows):
+            raise KernelError("uniforms and limits need one entry per logits row")
+        return self._sample_limited(logits, uniforms, limits, row_slot, None, False)
+
+    def _sample_limited(self, logits, uniforms, limits, row_slot, slot_state, advance):
+        _need(logits, "logits", torch.float32, 2)
+        rows = logits.shape[0]
+        if row_slot is not None:
+            _need(row_slot, "row_slot", torch.int32, 1)
+            if row_slot.shape[0] != rows:
+                raise KernelError("row_slot needs one entry per logits row")
+        _need_here(logits=logits, uniforms=uniforms, limits=limits, row_slot=row_slot, slot_state=slot_state)
+        tokens = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+        if rows == 0:
+            return tokens
+        _check(_declared_library("sampling_limits").mlr_sample_limited(
+            logits.data_ptr(), _address(uniforms), *limits.addresses, _address(row_slot), _address(slot_state), limits.entries, int(bool(advance)),
+            tokens.data_ptr(), rows, logits.shape[1], _raw_stream()), "sample_limited")
         return tokens
 
     # ------------------------------------------------------------------ rules on logits
