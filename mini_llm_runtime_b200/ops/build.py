@@ -72,6 +72,7 @@ LIBRARIES: dict[str, tuple[str, ...]] = {
     "copy_pages": (),
     "sampling_limits": (),
     "attention_quantized": (),
+    "attention_quantized_decode": (),
 }
 
 _loaded: dict[str, ctypes.CDLL] = {}

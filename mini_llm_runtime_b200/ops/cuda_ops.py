@@ -113,6 +113,8 @@ _PROTOTYPES = {
     "logit_rules": {"mlr_logit_rules": "pppiipp", "mlr_count_tokens": "ppippiiip"},
     "quantized_pages": {"mlr_quantize_kv": "plplp" "pppp" "iiiiii" "ip", "mlr_dequantize_pages": "ppppppp" "iiiiii" "ip"},
     "copy_pages": {"mlr_copy_pages": "pippip"},
+    "attention_quantized_decode": {"mlr_attention_quantized_decode": "pppppp" "ppppp" "iiiiiiiii" "fi" "ppp",
+                                   "mlr_attention_quantized_decode_scratch": "i"},
     "sampling_limits": {"mlr_sample_limited": "pppppppp" "ii" "p" "ii" "p"},
     "attention_quantized": {"mlr_attention_quantized": "pppppp" "ppppppp" "iiiiiiiii" "fip"},
 }
@@ -1259,13 +1261,35 @@ class CudaOps:
         if q.shape[0] == 0:
             return out
         plan, counts = batch.plan, batch.counts
+        tiles = counts["tiles"]
+        if self._quantized_on_tensor_cores(q, pool, num_heads) and 0 < batch.num_decode <= self.QUANTIZED_DECODES \
+                and batch.num_decode * num_kv_heads <= self.ATTENTION_COUNTERS:
+            space = self._workspace(q.device)
+            listed = None if batch.num_decode == batch.num_segments else plan["decode_seg"]
+            _check(_declared_library("attention_quantized_decode").mlr_attention_quantized_decode(
+                q.data_ptr(), pool.key.data_ptr(), pool.value.data_ptr(), pool.key_scales.data_ptr(), pool.value_scales.data_ptr(), out.data_ptr(),
+                _address(listed), batch.seg_q_start.data_ptr(), batch.seg_pos0.data_ptr(), batch.block_table.data_ptr(), batch.seg_slot.data_ptr(),
+                batch.block_table.shape[1], batch.num_decode, num_heads, num_kv_heads, head_dim, pool.page_size, pool.block, pool.pages,
+                int(window or 0), scale, int(batch.max_kv_len), space["attention_scratch"].data_ptr(), space["attention_counters"].data_ptr(),
+                _raw_stream()), "quantized_attention (decoded tokens)")
+            tiles -= batch.num_decode          # the work list's last
+        if tiles == 0:
+            return out
         _check(_declared_library("attention_quantized").mlr_attention_quantized(
             q.data_ptr(), pool.key.data_ptr(), pool.value.data_ptr(), pool.key_scales.data_ptr(), pool.value_scales.data_ptr(), out.data_ptr(),
             plan["tile_seg"].data_ptr(), plan["tile_row0"].data_ptr(), batch.seg_q_start.data_ptr(), batch.seg_q_len.data_ptr(),
-            batch.seg_pos0.data_ptr(), batch.block_table.data_ptr(), batch.seg_slot.data_ptr(), batch.block_table.shape[1], counts["tiles"],
+            batch.seg_pos0.data_ptr(), batch.block_table.data_ptr(), batch.seg_slot.data_ptr(), batch.block_table.shape[1], tiles,
             num_heads, num_kv_heads, head_dim, pool.page_size, pool.block, pool.pages, int(window or 0), scale, _code(q.dtype), _raw_stream()),
             "quantized_attention")
         return out
+
+    QUANTIZED_DECODES = 2048      # requests of one launch (attention_quantized_decode.cu)
+
+    def _quantized_on_tensor_cores(self, q: torch.Tensor, pool: QuantizedPool, num_heads: int) -> bool:
+        """bfloat16 queries over pages that whole groups of 16 keys lie on; everything else takes the general kernel."""
+        return (self.use_mma_attention and q.dtype == torch.bfloat16 and pool.dim in (64, 128) and num_heads // pool.kv_heads <= 16
+                and pool.page_size >= 16 and pool.page_size & (pool.page_size - 1) == 0 and pool.block & (pool.block - 1) == 0
+                and not (q.data_ptr() | pool.key.data_ptr() | pool.value.data_ptr()) % 16)
 
     # ------------------------------------------------------------------ pages of a cache
     COPY_POOLS = 8      # of one launch (copy_pages.cu)
