@@ -115,6 +115,8 @@ _PROTOTYPES = {
     "copy_pages": {"mlr_copy_pages": "pippip"},
     "attention_quantized_decode": {"mlr_attention_quantized_decode": "pppppp" "ppppp" "iiiiiiiii" "fi" "ppp",
                                    "mlr_attention_quantized_decode_scratch": "i"},
+    "attention_quantized_prompt": {"mlr_attention_quantized_prompt": "pppppp" "ppppppp" "iiiiiiiiiiii" "fi" "pppp" "l" "pip",
+                                   "mlr_attention_quantized_prompt_bytes": "iiiiii"},
     "sampling_limits": {"mlr_sample_limited": "pppppppp" "ii" "p" "ii" "p"},
     "attention_quantized": {"mlr_attention_quantized": "pppppp" "ppppppp" "iiiiiiiii" "fip"},
 }
@@ -128,6 +130,8 @@ def _declared_library(name: str) -> ctypes.CDLL:
     if _declared.get(name) is not library:
         for symbol, codes in _PROTOTYPES[name].items():
             getattr(library, symbol).argtypes = [_CTYPES[code] for code in codes]
+            if symbol.endswith("_bytes"):
+                getattr(library, symbol).restype = ctypes.c_longlong
         _declared[name] = library
     return library
 
@@ -379,7 +383,8 @@ def plan_attention(lengths: np.ndarray, position_start: np.ndarray) -> tuple[dic
         # one prompt portion (the common prefill step): its tiles in order, heaviest (= last) first
         # where the general path sorts; a dozen array operations instead of forty
         rows = int(lengths[0])
-        arrays, counts = {"decode_seg": np.zeros(0, dtype=np.int32)}, {"decode": 0, "prompt_keys": int(position_start[0]) + rows}
+        arrays, counts = {"decode_seg": np.zeros(0, dtype=np.int32)}, {
+            "decode": 0, "prompt_keys": int(position_start[0]) + rows, "prompt_tiles": (int(position_start[0]) + rows + 63) // 64}
         for prefix, count_name, tile_rows, heavy_first in (("tile", "tiles", GENERIC_TILE_ROWS, False),
                                                            ("wide_tile", "wide", MMA_TILE_ROWS, True),
                                                            ("big_tile", "big", TCGEN05_TILE_ROWS, True)):
@@ -400,7 +405,8 @@ def plan_attention(lengths: np.ndarray, position_start: np.ndarray) -> tuple[dic
               "big_tile_seg": big_seg, "big_tile_row0": big_row0}
     counts = {"tiles": int(tile_seg.shape[0]), "decode": int(decode_seg.shape[0]),
               "wide": int(wide_seg.shape[0]), "big": int(big_seg.shape[0]),
-              "prompt_keys": int((position_start + lengths)[longer].max()) if longer.shape[0] else 0}
+              "prompt_keys": int((position_start + lengths)[longer].max()) if longer.shape[0] else 0,
+              "prompt_tiles": int(((position_start + lengths + 63) // 64)[longer].sum())}
     return arrays, counts
 
 
@@ -1261,26 +1267,38 @@ class CudaOps:
         if q.shape[0] == 0:
             return out
         plan, counts = batch.plan, batch.counts
-        tiles = counts["tiles"]
-        if self._quantized_on_tensor_cores(q, pool, num_heads) and 0 < batch.num_decode <= self.QUANTIZED_DECODES \
-                and batch.num_decode * num_kv_heads <= self.ATTENTION_COUNTERS:
+        cores = self._quantized_on_tensor_cores(q, pool, num_heads)
+        first, rest = 0, counts["tiles"]          # of the work list, the decoded tokens' last: what the general kernel takes
+        pools = (pool.key.data_ptr(), pool.value.data_ptr(), pool.key_scales.data_ptr(), pool.value_scales.data_ptr())
+        segments = (batch.seg_q_start.data_ptr(), batch.seg_q_len.data_ptr(), batch.seg_pos0.data_ptr(), batch.block_table.data_ptr(),
+                    batch.seg_slot.data_ptr(), batch.block_table.shape[1])
+        sizes = (num_heads, num_kv_heads, head_dim, pool.page_size, pool.block, pool.pages, int(window or 0), scale)
+        if cores and counts["big"] > 0 and scale > 0:
+            # codes to float16 once, then tcgen05 products (scores are ordered before they are scaled: scale > 0)
+            library = _declared_library("attention_quantized_prompt")
+            shape = (counts["prompt_tiles"], q.shape[0], num_heads, num_kv_heads, head_dim)
+            prepared = torch.empty(library.mlr_attention_quantized_prompt_bytes(*shape, batch.num_segments), dtype=torch.uint8, device=q.device)
+            space = self._workspace(q.device)
+            _check(library.mlr_attention_quantized_prompt(
+                q.data_ptr(), *pools, out.data_ptr(), plan["big_tile_seg"].data_ptr(), plan["big_tile_row0"].data_ptr(), *segments, batch.num_segments,
+                counts["big"], counts["prompt_tiles"], q.shape[0], *sizes, int(batch.max_kv_len), prepared.data_ptr(),
+                space["prefill_queue"].data_ptr(), space["error_word"].data_ptr(), space["prefill_scratch"].data_ptr(),
+                space["prefill_scratch"].numel(), space["prefill_counters"].data_ptr(), space["prefill_counters"].numel(), _raw_stream()),
+                "quantized_attention (prompts)")
+            first, rest = rest - batch.num_decode, batch.num_decode
+        if cores and 0 < batch.num_decode <= self.QUANTIZED_DECODES and batch.num_decode * num_kv_heads <= self.ATTENTION_COUNTERS:
             space = self._workspace(q.device)
             listed = None if batch.num_decode == batch.num_segments else plan["decode_seg"]
+            q_start, _, pos0, *table = segments
             _check(_declared_library("attention_quantized_decode").mlr_attention_quantized_decode(
-                q.data_ptr(), pool.key.data_ptr(), pool.value.data_ptr(), pool.key_scales.data_ptr(), pool.value_scales.data_ptr(), out.data_ptr(),
-                _address(listed), batch.seg_q_start.data_ptr(), batch.seg_pos0.data_ptr(), batch.block_table.data_ptr(), batch.seg_slot.data_ptr(),
-                batch.block_table.shape[1], batch.num_decode, num_heads, num_kv_heads, head_dim, pool.page_size, pool.block, pool.pages,
-                int(window or 0), scale, int(batch.max_kv_len), space["attention_scratch"].data_ptr(), space["attention_counters"].data_ptr(),
-                _raw_stream()), "quantized_attention (decoded tokens)")
-            tiles -= batch.num_decode          # the work list's last
-        if tiles == 0:
-            return out
-        _check(_declared_library("attention_quantized").mlr_attention_quantized(
-            q.data_ptr(), pool.key.data_ptr(), pool.value.data_ptr(), pool.key_scales.data_ptr(), pool.value_scales.data_ptr(), out.data_ptr(),
-            plan["tile_seg"].data_ptr(), plan["tile_row0"].data_ptr(), batch.seg_q_start.data_ptr(), batch.seg_q_len.data_ptr(),
-            batch.seg_pos0.data_ptr(), batch.block_table.data_ptr(), batch.seg_slot.data_ptr(), batch.block_table.shape[1], tiles,
-            num_heads, num_kv_heads, head_dim, pool.page_size, pool.block, pool.pages, int(window or 0), scale, _code(q.dtype), _raw_stream()),
-            "quantized_attention")
+                q.data_ptr(), *pools, out.data_ptr(), _address(listed), q_start, pos0, *table, batch.num_decode, *sizes, int(batch.max_kv_len),
+                space["attention_scratch"].data_ptr(), space["attention_counters"].data_ptr(), _raw_stream()),
+                "quantized_attention (decoded tokens)")
+            rest -= batch.num_decode
+        if rest > 0:
+            _check(_declared_library("attention_quantized").mlr_attention_quantized(
+                q.data_ptr(), *pools, out.data_ptr(), plan["tile_seg"].data_ptr() + 4 * first, plan["tile_row0"].data_ptr() + 4 * first, *segments,
+                rest, *sizes, _code(q.dtype), _raw_stream()), "quantized_attention")
         return out
 
     QUANTIZED_DECODES = 2048      # requests of one launch (attention_quantized_decode.cu)

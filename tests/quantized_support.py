@@ -98,7 +98,11 @@ class Step:
         errors of a weight and of its place in the sum: twice the score's error (a dot product of dim terms in 32 bits, the scales'
         products and the sum with a value's exponent, |log2 vs| < 16: (dim + 8) 2^-24 sum |q||k| scale + 16 2^-23), e^x off by 2^-20, sums
         of n terms 4 sqrt(n) 2^-24.  On the tensor cores weights times the values' scales are held in float16 relative to the row's
-        largest: half a step 2^-11 of each, and 2^-25 of the largest for those too small to have all bits."""
+        largest: half a step 2^-11 of each, and 2^-25 of the largest for those too small to have all bits.  A prompt's keys and values
+        are there in float16 themselves, code times scale rounded by half a step 2^-11 relative to each (beside powers of two, exact): the
+        values' rounding moves o by 2^-11 A at most, the keys' a score by 2^-11 sum |q||k| scale, and a weight, which has its own score
+        in it and the others' in the sum that divides it, by twice that; 2^-25 of the tile's largest scale for values too small to have
+        all bits, weighed by p, sum p = 1."""
         assert got.dtype == self.q.dtype and bool(torch.isfinite(got).all())
         u = torch.finfo(got.dtype).eps / 2
         cores = got.dtype == torch.bfloat16
@@ -123,6 +127,8 @@ class Step:
             bound = u * want.abs() + a * relative
             if cores:
                 bound = bound + a * 2.0 ** -11 + n * 2.0 ** -25 * 127 * (p * vs[:, None, None, :]).amax(-1, keepdim=True)
+                if rows > 1 and self.dim in (64, 128):
+                    bound = bound + a * (2.0 ** -11 + 2 * 2.0 ** -11 * size) + 2.0 ** -25 * 127 * vs.amax(-1)[:, None, None, None]
             mine = got[at:at + rows].double().view(rows, self.kv_heads, per, self.dim).permute(1, 2, 0, 3)
             worst = ((mine - want).abs() / bound.clamp_min(1e-300)).max()
             assert float(worst) <= 1.0, f"request {i} of {rows} rows behind {first}: {float(worst):.3f} of what is allowed"
