@@ -2,20 +2,22 @@
 // and 128, up to 16 query heads per kv head, pages of a power of two of at least 16 tokens.
 //
 //   x_j = (q . kc_j) ks_j scale log2 e + log2 vs_j,  M = max x_j,  p_j = 2^(x_j - M),  out = sum p_j vc_j / sum (p_j / vs_j)
-// so that the weights that multiply the codes vc_j carry the values' scales and lie in (0, 1] whatever the scales are: they
-// fit float16, whose 11 bits round them less than bfloat16 would.  Codes are exact in float16, and queries are there
-// after a power of two per head has brought the largest near one.
+// so that the weights that multiply the codes vc_j carry the values' scales and lie near (0, 1] whatever the scales are: they
+// fit float16, whose 11 bits round them less than bfloat16 would.  (M follows the largest x in steps of more than 2^8: most tiles
+// then need no maximum over their keys, only the look whether one has passed it.)  Codes are exact in float16, and queries are
+// there after a power of two per head has brought the largest near one.
 //
 // Reading 2 * dim bytes per key and kv head is what bounds it.  A warp takes 16 keys (head size 64: 32) at a time and has three such
 // tiles on their way.  The heads of a group are the narrow side of the products (n = 8), keys and dimensions the wide one:
 //   scores^T [16 keys x 8 heads] = K [16 x dim] Q^T,   out^T [dim x 8 heads] += V^T [dim x 16 keys] P^T
 // The order of the dimensions within a product is free, so a thread asks for 16 bytes of a key that are four steps' operands, and
 // for 16 (8) dimensions of four keys that are eight (four) tiles' operands: every thread copies asynchronously just the bytes it reads
-// itself, conflict-free and without a barrier.  A byte becomes a float16 by a byte permutation (1024 + 128 + code) and a
-// subtraction, both exact.
+// itself, conflict-free and without a barrier.  A byte becomes a float16 by a byte permutation: 1024 + 128 + code.  Of the values
+// the 1152 is subtracted (exactly); of the keys it is left in, and 1152 times the sum of the query taken off where the scores'
+// sums begin (32 bits: 1152 sum |q| 2^-24 beside scores of up to 127 sum |q|).
 //
 // The keys of all requests and kv heads form one line that the CTAs share evenly, whatever the contexts: a CTA's share may
-// end one request's keys and begin another's.  Pairs of a request and a kv head that more than one CTA walks are merged by the
+// end one request's keys and begin another's.  Each beginning counts as QD_BEGIN tiles more, about what it costs.  Pairs of a request and a kv head that more than one CTA walks are merged by the
 // CTA that ends last, in the order of the CTAs.
 #include <cuda_fp16.h>
 
@@ -25,7 +27,10 @@ namespace mlr {
 
 constexpr int QD_WARPS = 8, QD_THREADS = QD_WARPS * 32, QD_STAGES = 3;
 constexpr int QD_MOST_REQUESTS = 2048;       // whose tiles a CTA counts
-constexpr int QD_LEAST_SHARE = 16;           // tiles of a CTA, at least: two per warp
+constexpr int QD_BEGIN = 24;                 // what the beginning of a pair of a request and a kv head costs a CTA, in tiles
+constexpr int QD_LEAST_SHARE = QD_BEGIN + 16;      // of a CTA, at least: two tiles per warp
+// The largest exponent follows the maximum in steps of more than this; weights up to 2^8 are far from float16's end.
+constexpr float QD_LAZY = 8.f;
 
 template <int D>
 struct QdShape {
@@ -55,15 +60,33 @@ __device__ __forceinline__ uint32_t qd_transposed(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
+// The larger of two numbers; NaN if one is.
+__device__ __forceinline__ float qd_max(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float qd_log2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float qd_inverse(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float qd_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Codes 0 and 1 (HIGH: 2 and 3) of a word with its sign bits turned round, as float16.
+// Codes 0 and 1 (HIGH: 2 and 3) of a word with its sign bits turned round, as float16: with 1152 on them, without.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t qd_raised(uint32_t turned) { return __byte_perm(turned, 0x64646464u, HIGH ? 0x4342 : 0x4140); }
 template <bool HIGH>
 __device__ __forceinline__ uint32_t qd_half2(uint32_t turned) {
-  const uint32_t raised = __byte_perm(turned, 0x64646464u, HIGH ? 0x4342 : 0x4140);
+  const uint32_t raised = qd_raised<HIGH>(turned);
   const uint32_t offset = 0x64806480u;        // 1152
   const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&raised), *reinterpret_cast<const __half2*>(&offset));
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -117,8 +140,9 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
   }
   if (threadIdx.x == 0) before[requests] = carried;
   __syncthreads();
-  // the line: request after request, a request's kv heads one behind the other
-  const long long units = (long long)carried * kv_heads;
+  // the line: request after request, a request's kv heads one behind the other, each QD_BEGIN longer than its tiles
+  auto line_of = [&](int index) { return ((long long)before[index] + (long long)index * QD_BEGIN) * kv_heads; };
+  const long long units = line_of(requests);
   const long long share = max((long long)QD_LEAST_SHARE, (units + gridDim.x - 1) / gridDim.x);
   long long at = share * blockIdx.x;
   const long long end = min(units, at + share);
@@ -127,7 +151,7 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
     int low = 0, high = requests - 1;
     while (low < high) {
       const int middle = (low + high + 1) >> 1;
-      if ((long long)before[middle] * kv_heads <= at) low = middle;
+      if (line_of(middle) <= at) low = middle;
       else high = middle - 1;
     }
     request = low;
@@ -137,15 +161,20 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
   uint8_t* stages = qd_shared + warp * QD_STAGES * Shape::STAGE;
   const uint32_t stage_at = (uint32_t)__cvta_generic_to_shared(stages);
   while (at < end) {
-    const long long first_unit = (long long)before[request] * kv_heads;
-    const int request_tiles = before[request + 1] - before[request];
-    const int kv_head = (int)((at - first_unit) / request_tiles);
-    const long long pair_begin = first_unit + (long long)kv_head * request_tiles, pair_end = pair_begin + request_tiles;
+    const int request_tiles = before[request + 1] - before[request], length = request_tiles + QD_BEGIN;
+    const int kv_head = (int)((at - line_of(request)) / length);
+    const long long pair_begin = line_of(request) + (long long)kv_head * length, pair_end = pair_begin + length;
     const long long my_end = min(end, pair_end);
-    const int segment = segment_of(request), row = seg_q_start[segment], position = seg_pos0[segment];
+    // its tiles, of the pair's
+    const int from = max(0, (int)(at - pair_begin) - QD_BEGIN), until = (int)(my_end - pair_begin) - QD_BEGIN;
+    const int here = request;
+    at = my_end;
+    if (kv_head == kv_heads - 1 && my_end == pair_end) ++request;
+    if (until <= 0) continue;                       // a share that ends in a pair's beginning has none
+    const int segment = segment_of(here), row = seg_q_start[segment], position = seg_pos0[segment];
     const int* table = block_table + (size_t)(seg_slot != nullptr ? seg_slot[segment] : segment) * table_width;
     const int lowest = lowest_of(position);
-    const int first_tile = lowest / KEYS + (int)(at - pair_begin), tiles = (int)(my_end - at);
+    const int first_tile = lowest / KEYS + from, tiles = until - from;
 
     // ---- loads: tile n of this warp is tile first_tile + warp + n * QD_WARPS
     const int my_tiles = tiles > warp ? (tiles - warp + QD_WARPS - 1) / QD_WARPS : 0;
@@ -154,30 +183,32 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
       const int page = n < my_tiles && logical < table_width ? table[logical] : 0;
       return page >= 0 && page < pool_pages ? page : 0;
     };
-    auto issue = [&](int n, const int (&pages)[SUB]) {
+    const int lane_k = g * D + 16 * t, lane_v = 2 * t * D + (D / 8) * g;
+    auto issue = [&](int n, int to, const int (&pages)[SUB]) {
       if (n < my_tiles) {
-        const uint32_t dst = stage_at + (n % QD_STAGES) * Shape::STAGE;
+        const uint32_t dst = stage_at + to * Shape::STAGE;
 #pragma unroll
         for (int sub = 0; sub < SUB; ++sub) {
           const int key0 = (first_tile + warp + n * QD_WARPS) * KEYS + sub * 16, offset = key0 & (page_size - 1);
           const size_t line = (size_t)pages[sub] * kv_heads + kv_head;
-          const int8_t* k_src = k_pool + ((line << page_shift) + offset) * D;
-          const int8_t* v_src = v_pool + ((line << page_shift) + offset) * D;
+          const size_t token = (line << page_shift) + offset;
+          const int8_t* k_src = k_pool + (token * D + lane_k);
+          const int8_t* v_src = v_pool + (token * D + lane_v);
           const uint32_t k_dst = dst + sub * (32 * D) + lane * 16;
 #pragma unroll
           for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int j = 0; j < JD; ++j) qd_copy16(k_dst + (half * JD + j) * 512, k_src + (g + 8 * half) * D + 64 * j + 16 * t);
+            for (int j = 0; j < JD; ++j) qd_copy16(k_dst + (half * JD + j) * 512, k_src + 8 * half * D + 64 * j);
           const uint32_t v_dst = dst + sub * (32 * D) + 16 * D + lane * (VW * 4);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int8_t* src = v_src + (2 * t + (i & 1) + 8 * (i >> 1)) * D + (D / 8) * g;
+            const int8_t* src = v_src + ((i & 1) + 8 * (i >> 1)) * D;
             if constexpr (D == 128) qd_copy16(v_dst + i * 512, src);
             else qd_copy8(v_dst + i * 256, src);
           }
           // lanes 0..15 the keys' scales, 16..31 the values'
           const float* scales = lane < 16 ? k_scales : v_scales;
-          qd_copy4(dst + Shape::DATA + sub * 128 + lane * 4, scales + ((line << page_shift) + offset + (lane & 15) >> block_shift));
+          qd_copy4(dst + Shape::DATA + sub * 128 + lane * 4, scales + ((token + (lane & 15)) >> block_shift));
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -187,7 +218,7 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
     for (int n = 0; n < QD_STAGES; ++n) {
 #pragma unroll
       for (int sub = 0; sub < SUB; ++sub) pages[sub] = page_of(n, sub);
-      issue(n, pages);
+      issue(n, n, pages);
     }
 #pragma unroll
     for (int sub = 0; sub < SUB; ++sub) pages[sub] = page_of(QD_STAGES, sub);
@@ -195,6 +226,7 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
     // ---- queries: head 8 h + g, the thread's 16 dimensions of each 64, as float16 times a power of two
     uint32_t qf[NH][JD * 4][2];
     float factor[NH][2];      // of heads 2 t, 2 t + 1: scale, log2 e and the power of two back
+    float start[NH][2];       // -1152 times the sum of the query
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
       const int head = 8 * h + g;
@@ -221,6 +253,7 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
       const bool scaled = exponent >= 1u && top < 0x7f800000u;
       const float down = scaled ? __uint_as_float((254u - exponent) << 23) : 1.f;
       const float up = scaled ? __uint_as_float(exponent << 23) : 1.f;
+      float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < JD; ++j)
 #pragma unroll
@@ -230,10 +263,17 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
           for (int e = 0; e < 4; ++e) {
             const __half2 pair = __floats2half2_rn(__uint_as_float(words[e] << 16) * down, __uint_as_float(words[e] & 0xffff0000u) * down);
             qf[h][j * 4 + 2 * i + (e >> 1)][e & 1] = *reinterpret_cast<const uint32_t*>(&pair);
+            const float2 rounded = __half22float2(pair);
+            sum += rounded.x + rounded.y;
           }
         }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) factor[h][e] = __shfl_sync(0xffffffffu, up, (2 * t + e) * 4) * scale_log2;
+      for (int e = 0; e < 2; ++e) {
+        factor[h][e] = __shfl_sync(0xffffffffu, up, (2 * t + e) * 4) * scale_log2;
+        start[h][e] = -1152.f * __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4);
+      }
     }
 
     // ---- the walk
@@ -245,10 +285,11 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) o[h][i][0] = o[h][i][1] = o[h][i][2] = o[h][i][3] = 0.f;
     }
+    int stage_of = 0;
     for (int n = 0; n < my_tiles; ++n) {
       asm volatile("cp.async.wait_group %0;" ::"n"(QD_STAGES - 1) : "memory");
       __syncwarp();
-      const uint8_t* stage = stages + (n % QD_STAGES) * Shape::STAGE;
+      const uint8_t* stage = stages + stage_of * Shape::STAGE;
       const int key_tile = (first_tile + warp + n * QD_WARPS) * KEYS;
 #pragma unroll
       for (int sub = 0; sub < SUB; ++sub) {
@@ -259,7 +300,7 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
         // scores^T: rows keys g, g + 8, columns heads 2 t, 2 t + 1
         float s[NH][4];
 #pragma unroll
-        for (int h = 0; h < NH; ++h) s[h][0] = s[h][1] = s[h][2] = s[h][3] = 0.f;
+        for (int h = 0; h < NH; ++h) { s[h][0] = s[h][2] = start[h][0]; s[h][1] = s[h][3] = start[h][1]; }
 #pragma unroll
         for (int j = 0; j < JD; ++j) {
           const uint4 low = *reinterpret_cast<const uint4*>(k_data + j * 512), high = *reinterpret_cast<const uint4*>(k_data + (JD + j) * 512);
@@ -267,46 +308,42 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const uint32_t first = a[w] ^ 0x80808080u, second = b[w] ^ 0x80808080u;
-            const uint32_t k[4] = {qd_half2<false>(first), qd_half2<false>(second), qd_half2<true>(first), qd_half2<true>(second)};
+            const uint32_t k[4] = {qd_raised<false>(first), qd_raised<false>(second), qd_raised<true>(first), qd_raised<true>(second)};
 #pragma unroll
             for (int h = 0; h < NH; ++h) qd_mma(s[h], k, qf[h][j * 4 + w][0], qf[h][j * 4 + w][1]);
           }
         }
-        // scales of the two keys; one too small for a reciprocal counts as 2^-100 (its values are below 2^-93 then)
+        // scales of the two keys; a value's below 2^-100 counts as 2^-100 (what it stands for is below 2^-93 then)
         float ks[2], lv[2], iv[2];
+        const bool ragged = key0 < lowest || key0 + 15 > position;
+        bool hidden[2] = {false, false};
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+          const float vs = qd_max(scales[16 + g + 8 * e], 7.888609e-31f);
           ks[e] = scales[g + 8 * e];
-          const float vs = scales[16 + g + 8 * e], safe = vs > 7.888609e-31f ? vs : vs == vs ? 7.888609e-31f : vs;
-          lv[e] = __log2f(safe);
-          iv[e] = safe < INFINITY ? __fdividef(1.f, safe) : 1.f;      // (not finite: the weight itself says so)
-          if (!(safe < INFINITY)) lv[e] = __int_as_float(0x7fffffff);
+          lv[e] = qd_log2(vs);
+          iv[e] = qd_inverse(vs);
+          if (ragged && (key0 + g + 8 * e < lowest || key0 + g + 8 * e > position)) { hidden[e] = true; iv[e] = 0.f; }
         }
-        const bool ragged = key0 < lowest || key0 + 15 > position;
         uint32_t p[NH][2];
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
           float x[2][2];
-          bool rises = false;
 #pragma unroll
           for (int e = 0; e < 2; ++e)      // key
 #pragma unroll
             for (int c = 0; c < 2; ++c) {  // head
               x[e][c] = fmaf(s[h][2 * e + c] * ks[e], factor[h][c], lv[e]);
-              if (ragged && (key0 + g + 8 * e < lowest || key0 + g + 8 * e > position)) x[e][c] = -INFINITY;
+              if (hidden[e]) x[e][c] = -INFINITY;
             }
-          float top[2];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            top[c] = fmaxf(x[0][c], x[1][c]);
-            top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
-            top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
-            top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
-            rises |= top[c] > m[h][c];
-          }
-          if (__any_sync(0xffffffffu, rises)) {
+          float top[2] = {fmaxf(x[0][0], x[1][0]), fmaxf(x[0][1], x[1][1])};
+          // (-inf) - (-inf) is NaN and compares false: nothing visible yet
+          if (__any_sync(0xffffffffu, top[0] - m[h][0] > QD_LAZY || top[1] - m[h][1] > QD_LAZY)) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
+              top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
+              top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
+              top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
               const float higher = fmaxf(m[h][c], top[c]);
               const float alpha = higher == -INFINITY ? 1.f : qd_exp2(m[h][c] - higher);
               m[h][c] = higher;
@@ -346,7 +383,8 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
         }
       }
       __syncwarp();
-      issue(n + QD_STAGES, pages);
+      issue(n + QD_STAGES, stage_of, pages);
+      stage_of = stage_of + 1 == QD_STAGES ? 0 : stage_of + 1;
 #pragma unroll
       for (int sub = 0; sub < SUB; ++sub) pages[sub] = page_of(n + QD_STAGES + 1, sub);
     }
@@ -375,10 +413,10 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
         }
       }
     __syncthreads();
-    const bool whole = at == pair_begin && my_end == pair_end;
+    const bool whole = from == 0 && my_end == pair_end;
     constexpr int STATE = D + 2;
     // a CTA holds at most two pairs in part: one that began before its share, one that ends behind it
-    float* mine = scratch + ((size_t)blockIdx.x * 2 + (pair_begin < at ? 0 : 1)) * 16 * STATE;
+    float* mine = scratch + ((size_t)blockIdx.x * 2 + (from > 0 ? 0 : 1)) * 16 * STATE;
     for (int idx = threadIdx.x; idx < group * D; idx += QD_THREADS) {
       const int head = idx / D, d = idx - head * D;
       float top = -INFINITY;
@@ -400,8 +438,8 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
       }
     }
     if (!whole) {
-      const int pair = request * kv_heads + kv_head;
-      const int first_cta = (int)(pair_begin / share), last_cta = (int)((pair_end - 1) / share);
+      const int pair = here * kv_heads + kv_head;
+      const int first_cta = (int)((pair_begin + QD_BEGIN) / share), last_cta = (int)((pair_end - 1) / share);
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) last_flag = atomicAdd(&counters[pair], 1) == last_cta - first_cta;
@@ -412,7 +450,7 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
           const int head = idx / D, d = idx - head * D;
           float top = -INFINITY, sum = 0.f, value = 0.f;
           for (int c = first_cta; c <= last_cta; ++c) {
-            const float* theirs = scratch + ((size_t)c * 2 + (pair_begin < c * share ? 0 : 1)) * 16 * STATE + head * STATE;
+            const float* theirs = scratch + ((size_t)c * 2 + (c > first_cta ? 0 : 1)) * 16 * STATE + head * STATE;
             const float their_top = __ldcg(theirs), their_sum = __ldcg(theirs + 1), theirs_value = __ldcg(theirs + 2 + d);
             const float higher = fmaxf(top, their_top);
             const float down = top == -INFINITY ? 0.f : qd_exp2(top - higher), share_of = their_top == -INFINITY ? 0.f : qd_exp2(their_top - higher);
@@ -426,8 +464,6 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
       }
     }
     __syncthreads();        // the stages are filled again, the flag is written again
-    at = my_end;
-    if (at == first_unit + (long long)request_tiles * kv_heads) ++request;
   }
 }
 
@@ -435,7 +471,7 @@ template <int D, int NH>
 static int quantized_decode_launch(const void* q, const void* k_pool, const void* v_pool, const float* k_scales, const float* v_scales, void* out,
                                    const int* decode_seg, const int* seg_q_start, const int* seg_pos0, const int* block_table, const int* seg_slot,
                                    int table_width, int requests, int heads, int kv_heads, int page_shift, int block_shift, int pool_pages, int window,
-                                   float scale, long long most_tiles, float* scratch, int* counters, cudaStream_t stream) {
+                                   float scale, long long most_units, float* scratch, int* counters, cudaStream_t stream) {
   auto kernel = attention_quantized_decode_kernel<D, NH>;
   constexpr size_t ring = (size_t)QD_WARPS * QD_STAGES * QdShape<D>::STAGE;
   static_assert((size_t)QD_WARPS * 8 * NH * (D + 2) * sizeof(float) <= ring, "the states lie where the stages were");
@@ -444,7 +480,7 @@ static int quantized_decode_launch(const void* q, const void* k_pool, const void
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ring + (QD_MOST_REQUESTS + 1) * sizeof(int)));
   });
   if (err != cudaSuccess) return (int)err;
-  const long long shares = (most_tiles + QD_LEAST_SHARE - 1) / QD_LEAST_SHARE, resident = 2 * sm_count();
+  const long long shares = (most_units + QD_LEAST_SHARE - 1) / QD_LEAST_SHARE, resident = 2 * sm_count();
   const int ctas = (int)(shares < resident ? shares : resident);
   launch_kernel(kernel, dim3(ctas), dim3(QD_THREADS), ring + (requests + 1) * sizeof(int), stream, (const bf16*)q, (const int8_t*)k_pool,
                 (const int8_t*)v_pool, k_scales, v_scales, (bf16*)out, decode_seg, seg_q_start, seg_pos0, block_table, seg_slot, table_width, requests,
@@ -482,7 +518,7 @@ MLR_EXPORT int mlr_attention_quantized_decode(const void* q, const void* k_pool,
   if (heads / kv_heads > 16 || requests > QD_MOST_REQUESTS) return MLR_TOO_LARGE;
   if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) return MLR_BAD_ALIGNMENT;
   const int keys = window > 0 && window < longest ? window + 16 : longest, tile = 16 * (128 / dim);
-  const long long most = (long long)requests * kv_heads * (keys / tile + 2);
+  const long long most = (long long)requests * kv_heads * (keys / tile + 2 + QD_BEGIN);
   const bool wide = heads / kv_heads > 8;
 #define MLR_DECODE(D_, N_)                                                                                                                       \
   return quantized_decode_launch<D_, N_>(q, k_pool, v_pool, k_scales, v_scales, out, decode_seg, seg_q_start, seg_pos0, block_table, seg_slot,   \
