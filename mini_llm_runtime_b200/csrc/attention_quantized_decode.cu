@@ -16,9 +16,9 @@
 // the 1152 is subtracted (exactly); of the keys it is left in, and 1152 times the sum of the query taken off where the scores'
 // sums begin (32 bits: 1152 sum |q| 2^-24 beside scores of up to 127 sum |q|).
 //
-// The keys of all requests and kv heads form one line that the CTAs share evenly, whatever the contexts: a CTA's share may
-// end one request's keys and begin another's.  Each beginning counts as QD_BEGIN tiles more, about what it costs.  Pairs of a request and a kv head that more than one CTA walks are merged by the
-// CTA that ends last, in the order of the CTAs.
+// The keys of all requests and kv heads form one line that the warps share evenly, whatever the contexts: a warp's share may
+// end one request's keys and begin another's.  Each beginning counts as QD_BEGIN tiles more, about what it costs.  No warp waits for
+// another.  Pairs of a request and a kv head that several warps walk are merged by a second launch, in the order of the warps.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -27,8 +27,9 @@ namespace mlr {
 
 constexpr int QD_WARPS = 8, QD_THREADS = QD_WARPS * 32, QD_STAGES = 3;
 constexpr int QD_MOST_REQUESTS = 2048;       // whose tiles a CTA counts
-constexpr int QD_BEGIN = 24;                 // what the beginning of a pair of a request and a kv head costs a CTA, in tiles
-constexpr int QD_LEAST_SHARE = QD_BEGIN + 16;      // of a CTA, at least: two tiles per warp
+constexpr int QD_BEGIN = 1;                  // what the beginning of a pair of a request and a kv head costs a warp, in tiles
+constexpr int QD_LEAST_SHARE = QD_BEGIN + 2;       // of a warp, at least
+constexpr int QD_MOST_PARTS = 128;           // warps of a pair
 // The largest exponent follows the maximum in steps of more than this; weights up to 2^8 are far from float16's end.
 constexpr float QD_LAZY = 8.f;
 
@@ -99,13 +100,12 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
                                   bf16* __restrict__ out, const int* __restrict__ decode_seg, const int* __restrict__ seg_q_start,
                                   const int* __restrict__ seg_pos0, const int* __restrict__ block_table, const int* __restrict__ seg_slot,
                                   int table_width, int requests, int heads, int kv_heads, int page_shift, int block_shift, int pool_pages, int window,
-                                  float scale_log2, float* __restrict__ scratch, int* __restrict__ counters) {
+                                  float scale_log2, float* __restrict__ states, float2* __restrict__ sums, int* __restrict__ lines) {
   using Shape = QdShape<D>;
   constexpr int SUB = Shape::SUB, KEYS = Shape::KEYS, JD = D / 64, VW = D / 32;      // VW: words of a thread's dimensions of a key
   extern __shared__ __align__(128) uint8_t qd_shared[];
   int* before = reinterpret_cast<int*>(qd_shared + QD_WARPS * QD_STAGES * Shape::STAGE);      // [requests + 1] tiles before a request's
-  __shared__ int warp_sums[QD_WARPS];
-  __shared__ int last_flag;
+  __shared__ int warp_sums[QD_WARPS], warp_most[QD_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group = heads / kv_heads, page_size = 1 << page_shift;
   pdl_trigger();
@@ -113,7 +113,7 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
   auto segment_of = [&](int index) { return decode_seg != nullptr ? decode_seg[index] : index; };
   auto lowest_of = [&](int position) { return window > 0 ? max(0, position - window + 1) : 0; };
   // ---- tiles before each request's (positions are metadata of the step: read before the wait)
-  int carried = 0;
+  int carried = 0, most = 0;
   for (int first = 0; first < requests; first += QD_THREADS) {
     const int index = first + threadIdx.x;
     int tiles = 0;
@@ -121,19 +121,21 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
       const int position = seg_pos0[segment_of(index)];
       tiles = position / KEYS - lowest_of(position) / KEYS + 1;
     }
+    const int warp_top = (int)__reduce_max_sync(0xffffffffu, (unsigned)tiles);
     int inclusive = tiles;
 #pragma unroll
     for (int offset = 1; offset < 32; offset <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, inclusive, offset);
       if (lane >= offset) inclusive += up;
     }
-    if (lane == 31) warp_sums[warp] = inclusive;
+    if (lane == 31) { warp_sums[warp] = inclusive; warp_most[warp] = warp_top; }
     __syncthreads();
     int base = carried;
 #pragma unroll
     for (int w = 0; w < QD_WARPS; ++w) {
       if (w < warp) base += warp_sums[w];
       carried += warp_sums[w];
+      most = max(most, warp_most[w]);
     }
     if (index < requests) before[index] = base + inclusive - tiles;
     __syncthreads();
@@ -142,9 +144,11 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
   __syncthreads();
   // the line: request after request, a request's kv heads one behind the other, each QD_BEGIN longer than its tiles
   auto line_of = [&](int index) { return ((long long)before[index] + (long long)index * QD_BEGIN) * kv_heads; };
-  const long long units = line_of(requests);
-  const long long share = max((long long)QD_LEAST_SHARE, (units + gridDim.x - 1) / gridDim.x);
-  long long at = share * blockIdx.x;
+  const long long units = line_of(requests), walkers = (long long)gridDim.x * QD_WARPS;
+  long long share = (units + walkers - 1) / walkers;
+  share = max(share, (long long)max(QD_LEAST_SHARE, (most + QD_MOST_PARTS - 2) / (QD_MOST_PARTS - 1)));
+  const long long walker = (long long)blockIdx.x * QD_WARPS + warp;
+  long long at = share * walker;
   const long long end = min(units, at + share);
   int request = 0;
   if (at < end) {                                   // the last one that begins at or before `at`
@@ -157,6 +161,10 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
     request = low;
   }
   pdl_wait();
+  if (blockIdx.x == 0) {                            // for the merge
+    for (int index = threadIdx.x; index <= requests; index += QD_THREADS) lines[1 + index] = before[index];
+    if (threadIdx.x == 0) lines[0] = (int)share;
+  }
 
   uint8_t* stages = qd_shared + warp * QD_STAGES * Shape::STAGE;
   const uint32_t stage_at = (uint32_t)__cvta_generic_to_shared(stages);
@@ -174,12 +182,11 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
     const int segment = segment_of(here), row = seg_q_start[segment], position = seg_pos0[segment];
     const int* table = block_table + (size_t)(seg_slot != nullptr ? seg_slot[segment] : segment) * table_width;
     const int lowest = lowest_of(position);
-    const int first_tile = lowest / KEYS + from, tiles = until - from;
+    const int first_tile = lowest / KEYS + from, my_tiles = until - from;
 
-    // ---- loads: tile n of this warp is tile first_tile + warp + n * QD_WARPS
-    const int my_tiles = tiles > warp ? (tiles - warp + QD_WARPS - 1) / QD_WARPS : 0;
+    // ---- loads
     auto page_of = [&](int n, int sub) -> int {
-      const int key0 = (first_tile + warp + n * QD_WARPS) * KEYS + sub * 16, logical = key0 >> page_shift;
+      const int key0 = (first_tile + n) * KEYS + sub * 16, logical = key0 >> page_shift;
       const int page = n < my_tiles && logical < table_width ? table[logical] : 0;
       return page >= 0 && page < pool_pages ? page : 0;
     };
@@ -189,7 +196,7 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
         const uint32_t dst = stage_at + to * Shape::STAGE;
 #pragma unroll
         for (int sub = 0; sub < SUB; ++sub) {
-          const int key0 = (first_tile + warp + n * QD_WARPS) * KEYS + sub * 16, offset = key0 & (page_size - 1);
+          const int key0 = (first_tile + n) * KEYS + sub * 16, offset = key0 & (page_size - 1);
           const size_t line = (size_t)pages[sub] * kv_heads + kv_head;
           const size_t token = (line << page_shift) + offset;
           const int8_t* k_src = k_pool + (token * D + lane_k);
@@ -290,7 +297,7 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
       asm volatile("cp.async.wait_group %0;" ::"n"(QD_STAGES - 1) : "memory");
       __syncwarp();
       const uint8_t* stage = stages + stage_of * Shape::STAGE;
-      const int key_tile = (first_tile + warp + n * QD_WARPS) * KEYS;
+      const int key_tile = (first_tile + n) * KEYS;
 #pragma unroll
       for (int sub = 0; sub < SUB; ++sub) {
         const int key0 = key_tile + sub * 16;
@@ -389,13 +396,12 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
       for (int sub = 0; sub < SUB; ++sub) pages[sub] = page_of(n + QD_STAGES + 1, sub);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();
+    __syncwarp();
 
-    // ---- the warps' states, then those of the CTAs; the stages' memory is free now
-    constexpr int HEADS = 8 * NH;
-    float* states = reinterpret_cast<float*>(qd_shared);               // [warp][head][D]
-    float* tops = states + QD_WARPS * HEADS * D;                       // [warp][head]
-    float* sums = tops + QD_WARPS * HEADS;
+    // ---- the pair's outputs, or this warp's part of them
+    const bool whole = from == 0 && my_end == pair_end;
+    // a warp holds at most two pairs in part: one that began before its share, one that ends behind it
+    const size_t slot = (size_t)walker * 2 + (from > 0 ? 0 : 1);
 #pragma unroll
     for (int h = 0; h < NH; ++h)
 #pragma unroll
@@ -405,86 +411,106 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
         sum += __shfl_xor_sync(0xffffffffu, sum, 8);
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         const int head = 8 * h + 2 * t + c;
-        if (g == 0) { tops[warp * HEADS + head] = m[h][c]; sums[warp * HEADS + head] = sum; }
-        if (head < group) {
-          float* mine = states + (warp * HEADS + head) * D + (D / 8) * g;
+        if (head >= group) continue;
+        if (whole) {
+          const float inverse = 1.f / sum;
+          uint32_t packed[D / 16];
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i) *reinterpret_cast<float2*>(mine + 2 * i) = make_float2(o[h][i][c], o[h][i][2 + c]);
-        }
-      }
-    __syncthreads();
-    const bool whole = from == 0 && my_end == pair_end;
-    constexpr int STATE = D + 2;
-    // a CTA holds at most two pairs in part: one that began before its share, one that ends behind it
-    float* mine = scratch + ((size_t)blockIdx.x * 2 + (from > 0 ? 0 : 1)) * 16 * STATE;
-    for (int idx = threadIdx.x; idx < group * D; idx += QD_THREADS) {
-      const int head = idx / D, d = idx - head * D;
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < QD_WARPS; ++w) top = fmaxf(top, tops[w * HEADS + head]);
-      float sum = 0.f, value = 0.f;
-#pragma unroll
-      for (int w = 0; w < QD_WARPS; ++w) {
-        const float share_of = tops[w * HEADS + head] == -INFINITY ? 0.f : qd_exp2(tops[w * HEADS + head] - top);
-        // (a warp without keys has nothing to add; one whose scores are no numbers has a NaN sum and no top)
-        sum += sums[w * HEADS + head] * (sums[w * HEADS + head] == sums[w * HEADS + head] ? share_of : 1.f);
-        value = fmaf(states[(w * HEADS + head) * D + d], share_of, value);
-      }
-      if (whole) {
-        out[((size_t)row * heads + kv_head * group + head) * D + d] = __float2bfloat16_rn(value / sum);
-      } else {
-        mine[head * STATE + 2 + d] = value;
-        if (d == 0) { mine[head * STATE] = top; mine[head * STATE + 1] = sum; }
-      }
-    }
-    if (!whole) {
-      const int pair = here * kv_heads + kv_head;
-      const int first_cta = (int)((pair_begin + QD_BEGIN) / share), last_cta = (int)((pair_end - 1) / share);
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) last_flag = atomicAdd(&counters[pair], 1) == last_cta - first_cta;
-      __syncthreads();
-      if (last_flag) {
-        __threadfence();
-        for (int idx = threadIdx.x; idx < group * D; idx += QD_THREADS) {
-          const int head = idx / D, d = idx - head * D;
-          float top = -INFINITY, sum = 0.f, value = 0.f;
-          for (int c = first_cta; c <= last_cta; ++c) {
-            const float* theirs = scratch + ((size_t)c * 2 + (c > first_cta ? 0 : 1)) * 16 * STATE + head * STATE;
-            const float their_top = __ldcg(theirs), their_sum = __ldcg(theirs + 1), theirs_value = __ldcg(theirs + 2 + d);
-            const float higher = fmaxf(top, their_top);
-            const float down = top == -INFINITY ? 0.f : qd_exp2(top - higher), share_of = their_top == -INFINITY ? 0.f : qd_exp2(their_top - higher);
-            sum = sum * (sum == sum ? down : 1.f) + their_sum * (their_sum == their_sum ? share_of : 1.f);
-            value = fmaf(theirs_value, share_of, value * down);
-            top = higher;
+          for (int i = 0; i < D / 16; ++i) {
+            const __nv_bfloat162 pair = __floats2bfloat162_rn(o[h][i][c] * inverse, o[h][i][2 + c] * inverse);
+            packed[i] = *reinterpret_cast<const uint32_t*>(&pair);
           }
-          out[((size_t)row * heads + kv_head * group + head) * D + d] = __float2bfloat16_rn(value / sum);
+          uint4* dst = reinterpret_cast<uint4*>(out + ((size_t)row * heads + kv_head * group + head) * D + (D / 8) * g);
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) dst[i] = make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
+        } else {
+          float4* dst = reinterpret_cast<float4*>(states + (slot * 8 * NH + head) * D + (D / 8) * g);
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) dst[i] = make_float4(o[h][2 * i][c], o[h][2 * i][2 + c], o[h][2 * i + 1][c], o[h][2 * i + 1][2 + c]);
+          if (g == 0) sums[slot * 8 * NH + head] = make_float2(m[h][c], sum);
         }
-        if (threadIdx.x == 0) counters[pair] = 0;       // ready for the next launch
       }
-    }
-    __syncthreads();        // the stages are filled again, the flag is written again
   }
+}
+
+// The parts of pairs that several warps walked.  A CTA per pair, a thread per head and four dimensions.
+template <int D, int NH>
+__global__ void __launch_bounds__(8 * NH * D / 4)
+merge_quantized_decode_kernel(const float* states, const float2* sums, const int* lines, bf16* __restrict__ out,
+                              const int* __restrict__ decode_seg, const int* __restrict__ seg_q_start, int heads, int kv_heads) {
+  pdl_trigger();
+  const int request = blockIdx.x / kv_heads, kv_head = blockIdx.x - request * kv_heads, group = heads / kv_heads;
+  const int head = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4);
+  const int row = seg_q_start[decode_seg != nullptr ? decode_seg[request] : request];
+  pdl_wait();
+  const int share = __ldcg(lines), before = __ldcg(lines + 1 + request), length = __ldcg(lines + 2 + request) - before + QD_BEGIN;
+  const long long begin = ((long long)before + (long long)request * QD_BEGIN) * kv_heads + (long long)kv_head * length;
+  const long long first = (begin + QD_BEGIN) / share, last = (begin + length - 1) / share;
+  if (first == last || head >= group) return;      // one warp wrote the outputs
+  const int parts = (int)(last - first) + 1;
+  // part i: the first one's pair begins in its share, the others' began before
+  auto slot_of = [&](int i) { return (size_t)((first + i) * 2 + (i == 0 ? 1 : 0)) * 8 * NH + head; };
+  float top = -INFINITY;
+  for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(sums + slot_of(i)).x);
+  float total = 0.f;
+  float4 value = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const float2 state = __ldcg(sums + slot_of(i));
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(states + slot_of(i) * D) + d);
+    // (a part whose scores are no numbers has no largest one and a NaN sum, which stays)
+    const float weight = state.x == -INFINITY ? 0.f : qd_exp2(state.x - top);
+    total += state.y * (state.y == state.y ? weight : 1.f);
+    value.x = fmaf(v.x, weight, value.x);
+    value.y = fmaf(v.y, weight, value.y);
+    value.z = fmaf(v.z, weight, value.z);
+    value.w = fmaf(v.w, weight, value.w);
+  }
+  const float inverse = 1.f / total;
+  const __nv_bfloat162 low = __floats2bfloat162_rn(value.x * inverse, value.y * inverse), high = __floats2bfloat162_rn(value.z * inverse, value.w * inverse);
+  reinterpret_cast<uint2*>(out + ((size_t)row * heads + kv_head * group + head) * D)[d] =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&low), *reinterpret_cast<const uint32_t*>(&high));
+}
+
+// Warps of a launch, and where the parts' memory lies (bytes).
+struct QdLayout {
+  int ctas;
+  long long sums, lines, total;
+};
+static QdLayout qd_layout(int requests, int kv_heads, int group, int dim, int window, int longest) {
+  const int keys = window > 0 && window < longest ? window + 16 : longest, tile = 16 * (128 / dim), per = group > 8 ? 16 : 8;
+  const long long units = (long long)requests * kv_heads * (keys / tile + 2 + QD_BEGIN), most = 2 * sm_count();
+  const long long ctas = (units + QD_LEAST_SHARE * QD_WARPS - 1) / (QD_LEAST_SHARE * QD_WARPS);
+  QdLayout at;
+  at.ctas = (int)(ctas < most ? ctas : most);
+  const long long slots = (long long)at.ctas * QD_WARPS * 2 * per;
+  at.sums = slots * dim * 4;
+  at.lines = at.sums + slots * 8;
+  at.total = at.lines + ((long long)requests + 2) * 4;
+  return at;
 }
 
 template <int D, int NH>
 static int quantized_decode_launch(const void* q, const void* k_pool, const void* v_pool, const float* k_scales, const float* v_scales, void* out,
                                    const int* decode_seg, const int* seg_q_start, const int* seg_pos0, const int* block_table, const int* seg_slot,
                                    int table_width, int requests, int heads, int kv_heads, int page_shift, int block_shift, int pool_pages, int window,
-                                   float scale, long long most_units, float* scratch, int* counters, cudaStream_t stream) {
+                                   float scale, int longest, uint8_t* scratch, cudaStream_t stream) {
   auto kernel = attention_quantized_decode_kernel<D, NH>;
   constexpr size_t ring = (size_t)QD_WARPS * QD_STAGES * QdShape<D>::STAGE;
-  static_assert((size_t)QD_WARPS * 8 * NH * (D + 2) * sizeof(float) <= ring, "the states lie where the stages were");
   static OncePerDevice once;
   const cudaError_t err = once([&] {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ring + (QD_MOST_REQUESTS + 1) * sizeof(int)));
   });
   if (err != cudaSuccess) return (int)err;
-  const long long shares = (most_units + QD_LEAST_SHARE - 1) / QD_LEAST_SHARE, resident = 2 * sm_count();
-  const int ctas = (int)(shares < resident ? shares : resident);
-  launch_kernel(kernel, dim3(ctas), dim3(QD_THREADS), ring + (requests + 1) * sizeof(int), stream, (const bf16*)q, (const int8_t*)k_pool,
+  const QdLayout at = qd_layout(requests, kv_heads, heads / kv_heads, D, window, longest);
+  float* states = (float*)scratch;
+  float2* sums = (float2*)(scratch + at.sums);
+  int* lines = (int*)(scratch + at.lines);
+  launch_kernel(kernel, dim3(at.ctas), dim3(QD_THREADS), ring + (requests + 1) * sizeof(int), stream, (const bf16*)q, (const int8_t*)k_pool,
                 (const int8_t*)v_pool, k_scales, v_scales, (bf16*)out, decode_seg, seg_q_start, seg_pos0, block_table, seg_slot, table_width, requests,
-                heads, kv_heads, page_shift, block_shift, pool_pages, window, scale * 1.4426950408889634f, scratch, counters);
+                heads, kv_heads, page_shift, block_shift, pool_pages, window, scale * 1.4426950408889634f, states, sums, lines);
+  launch_kernel(merge_quantized_decode_kernel<D, NH>, dim3(requests * kv_heads), dim3(8 * NH * D / 4), 0, stream, states, sums, lines, (bf16*)out,
+                decode_seg, seg_q_start, heads, kv_heads);
   return launch_status();
 }
 
@@ -500,30 +526,30 @@ using namespace mlr;
 
 MLR_DEFINE_PDL_SWITCH
 
-// Floats of scratch memory that a launch needs.
-MLR_EXPORT int mlr_attention_quantized_decode_scratch(int dim) { return 2 * sm_count() * 2 * 16 * (dim + 2); }
+// Bytes of scratch memory (on a 16-byte boundary) that a call needs.
+MLR_EXPORT long long mlr_attention_quantized_decode_bytes(int requests, int kv_heads, int group, int dim, int window, int longest) {
+  return qd_layout(requests, kv_heads, group, dim, window, longest).total;
+}
 
 // q, out: [rows, heads * dim] bfloat16, of which the rows of `requests` decoded tokens are attended (decode_seg: their segments, or null for
-// segments 0, 1, ..); pools [pages, kv_heads, page_size, dim]; scales [pages, kv_heads, page_size / block]; longest: keys of the longest context;
-// counters: requests * kv_heads zeroed ints (left zeroed).
+// segments 0, 1, ..); pools [pages, kv_heads, page_size, dim]; scales [pages, kv_heads, page_size / block]; longest: keys of the longest context
+// (a longer one is attended all the same); scratch: memory of the size above.
 MLR_EXPORT int mlr_attention_quantized_decode(const void* q, const void* k_pool, const void* v_pool, const float* k_scales, const float* v_scales,
                                               void* out, const int* decode_seg, const int* seg_q_start, const int* seg_pos0, const int* block_table,
                                               const int* seg_slot, int table_width, int requests, int heads, int kv_heads, int dim, int page_size,
-                                              int block, int pool_pages, int window, float scale, int longest, void* scratch, int* counters,
+                                              int block, int pool_pages, int window, float scale, int longest, void* scratch,
                                               cudaStream_t stream) {
   if (requests == 0) return MLR_OK;
   if (requests < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || table_width <= 0 || pool_pages <= 0 || longest <= 0) return MLR_BAD_SIZE;
   const int page_shift = shift_of(page_size), block_shift = shift_of(block);
   if ((dim != 64 && dim != 128) || page_shift < 4 || block_shift < 0 || block > page_size) return MLR_BAD_SIZE;
   if (heads / kv_heads > 16 || requests > QD_MOST_REQUESTS) return MLR_TOO_LARGE;
-  if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) return MLR_BAD_ALIGNMENT;
-  const int keys = window > 0 && window < longest ? window + 16 : longest, tile = 16 * (128 / dim);
-  const long long most = (long long)requests * kv_heads * (keys / tile + 2 + QD_BEGIN);
+  if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)scratch) & 15) return MLR_BAD_ALIGNMENT;
   const bool wide = heads / kv_heads > 8;
 #define MLR_DECODE(D_, N_)                                                                                                                       \
   return quantized_decode_launch<D_, N_>(q, k_pool, v_pool, k_scales, v_scales, out, decode_seg, seg_q_start, seg_pos0, block_table, seg_slot,   \
-                                         table_width, requests, heads, kv_heads, page_shift, block_shift, pool_pages, window, scale, most,       \
-                                         (float*)scratch, counters, stream)
+                                         table_width, requests, heads, kv_heads, page_shift, block_shift, pool_pages, window, scale, longest,    \
+                                         (uint8_t*)scratch, stream)
   if (dim == 64) { if (wide) MLR_DECODE(64, 2); MLR_DECODE(64, 1); }
   if (wide) MLR_DECODE(128, 2);
   MLR_DECODE(128, 1);

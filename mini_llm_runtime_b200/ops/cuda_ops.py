@@ -113,8 +113,8 @@ _PROTOTYPES = {
     "logit_rules": {"mlr_logit_rules": "pppiipp", "mlr_count_tokens": "ppippiiip"},
     "quantized_pages": {"mlr_quantize_kv": "plplp" "pppp" "iiiiii" "ip", "mlr_dequantize_pages": "ppppppp" "iiiiii" "ip"},
     "copy_pages": {"mlr_copy_pages": "pippip"},
-    "attention_quantized_decode": {"mlr_attention_quantized_decode": "pppppp" "ppppp" "iiiiiiiii" "fi" "ppp",
-                                   "mlr_attention_quantized_decode_scratch": "i"},
+    "attention_quantized_decode": {"mlr_attention_quantized_decode": "pppppp" "ppppp" "iiiiiiiii" "fi" "pp",
+                                   "mlr_attention_quantized_decode_bytes": "iiiiii"},
     "attention_quantized_prompt": {"mlr_attention_quantized_prompt": "pppppp" "ppppppp" "iiiiiiiiiiii" "fi" "pppp" "l" "pip",
                                    "mlr_attention_quantized_prompt_bytes": "iiiiii"},
     "sampling_limits": {"mlr_sample_limited": "pppppppp" "ii" "p" "ii" "p"},
@@ -1286,14 +1286,16 @@ class CudaOps:
                 space["prefill_scratch"].numel(), space["prefill_counters"].data_ptr(), space["prefill_counters"].numel(), _raw_stream()),
                 "quantized_attention (prompts)")
             first, rest = rest - batch.num_decode, batch.num_decode
-        if cores and 0 < batch.num_decode <= self.QUANTIZED_DECODES and batch.num_decode * num_kv_heads <= self.ATTENTION_COUNTERS:
-            space = self._workspace(q.device)
+        if cores and 0 < batch.num_decode <= self.QUANTIZED_DECODES:
+            library = _declared_library("attention_quantized_decode")
+            scratch = torch.empty(library.mlr_attention_quantized_decode_bytes(
+                batch.num_decode, num_kv_heads, num_heads // num_kv_heads, head_dim, int(window or 0), int(batch.max_kv_len)),
+                dtype=torch.uint8, device=q.device)
             listed = None if batch.num_decode == batch.num_segments else plan["decode_seg"]
             q_start, _, pos0, *table = segments
-            _check(_declared_library("attention_quantized_decode").mlr_attention_quantized_decode(
+            _check(library.mlr_attention_quantized_decode(
                 q.data_ptr(), *pools, out.data_ptr(), _address(listed), q_start, pos0, *table, batch.num_decode, *sizes, int(batch.max_kv_len),
-                space["attention_scratch"].data_ptr(), space["attention_counters"].data_ptr(), _raw_stream()),
-                "quantized_attention (decoded tokens)")
+                scratch.data_ptr(), _raw_stream()), "quantized_attention (decoded tokens)")
             rest -= batch.num_decode
         if rest > 0:
             _check(_declared_library("attention_quantized").mlr_attention_quantized(
