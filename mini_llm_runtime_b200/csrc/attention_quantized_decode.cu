@@ -8,20 +8,22 @@
 // there after a power of two per head has brought the largest near one.
 //
 // Reading 2 * dim bytes per key and kv head is what bounds it.  A warp takes 16 keys (head size 64: 32) at a time and has three such
-// tiles on their way.  The heads of a group are the narrow side of the products (n = 8), keys and dimensions the wide one:
+// tiles on their way, by bulk tensor copies of 16 keys into a ring of its own (a copy per 16 bytes and thread into the same ring: 15 %
+// slower, with seven times the instructions of a tile spent on them).  The heads of a group are the narrow side of the
+// products (n = 8), keys and dimensions the wide one:
 //   scores^T [16 keys x 8 heads] = K [16 x dim] Q^T,   out^T [dim x 8 heads] += V^T [dim x 16 keys] P^T
-// The order of the dimensions within a product is free, so a thread asks for 16 bytes of a key that are four steps' operands, and
-// for 16 (8) dimensions of four keys that are eight (four) tiles' operands: every thread copies asynchronously just the bytes it reads
-// itself, conflict-free and without a barrier.  A byte becomes a float16 by a byte permutation: 1024 + 128 + code.  Of the values
-// the 1152 is subtracted (exactly); of the keys it is left in, and 1152 times the sum of the query taken off where the scores'
-// sums begin (32 bits: 1152 sum |q| 2^-24 beside scores of up to 127 sum |q|).
+// The order of the dimensions within a product is free, so a thread reads 16 bytes of a key that are four steps' operands, and 16
+// (8) dimensions of four keys that are eight (four) tiles' operands; the copies' swizzle keeps the reads free of conflicts.  A byte
+// becomes a float16 by a byte permutation: 1024 + 128 + code.  Of the values the 1152 is subtracted (exactly); of the keys it
+// is left in, and 1152 times the sum of the query taken off where the scores' sums begin (32 bits: 1152 sum |q| 2^-24 beside scores of
+// up to 127 sum |q|).
 //
 // The keys of all requests and kv heads form one line that the warps share evenly, whatever the contexts: a warp's share may
 // end one request's keys and begin another's.  Each beginning counts as QD_BEGIN tiles more, about what it costs.  No warp waits for
 // another.  Pairs of a request and a kv head that several warps walk are merged by a second launch, in the order of the warps.
 #include <cuda_fp16.h>
 
-#include "common.cuh"
+#include "tma.cuh"
 
 namespace mlr {
 
@@ -37,16 +39,18 @@ template <int D>
 struct QdShape {
   static constexpr int SUB = 128 / D;                 // groups of 16 keys in a tile
   static constexpr int KEYS = 16 * SUB;
-  static constexpr int DATA = KEYS * D * 2;           // bytes of a tile: 4096
-  static constexpr int STAGE = DATA + SUB * 128;      // and the scales of its keys
+  static constexpr int PART = 16 * D;                 // bytes of the keys (the values) of a group
+  static constexpr int DATA = 2 * SUB * PART;         // of a tile: 4096
+  static constexpr int SCALES = SUB * 128;            // the scales of its keys
+  static constexpr int RING = QD_WARPS * QD_STAGES * DATA;
+  static constexpr int SHARED = RING + QD_WARPS * QD_STAGES * (SCALES + 8);      // and a barrier per tile
 };
+// Where 16 bytes of row `row` lie in a group of 16 rows as the copies leave them: 128-byte rows, or 64-byte ones.
+template <int D>
+__device__ __forceinline__ int qd_place(int row, int chunk) {
+  return row * D + ((chunk ^ (D == 128 ? row & 7 : (row >> 1) & 3)) << 4);
+}
 
-__device__ __forceinline__ void qd_copy16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void qd_copy8(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void qd_copy4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -96,18 +100,30 @@ __device__ __forceinline__ uint32_t qd_half2(uint32_t turned) {
 // NH: groups of 8 query heads.
 template <int D, int NH>
 __global__ void __launch_bounds__(QD_THREADS, 2)
-attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int8_t* v_pool, const float* k_scales, const float* v_scales,
-                                  bf16* __restrict__ out, const int* __restrict__ decode_seg, const int* __restrict__ seg_q_start,
+attention_quantized_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const bf16* q,
+                                  const float* k_scales, const float* v_scales, bf16* __restrict__ out, const int* __restrict__ decode_seg, const int* __restrict__ seg_q_start,
                                   const int* __restrict__ seg_pos0, const int* __restrict__ block_table, const int* __restrict__ seg_slot,
                                   int table_width, int requests, int heads, int kv_heads, int page_shift, int block_shift, int pool_pages, int window,
-                                  float scale_log2, float* __restrict__ states, float2* __restrict__ sums, int* __restrict__ lines) {
+                                  float scale_log2, float* __restrict__ states, float2* __restrict__ sums, int* __restrict__ lines, int* error_word) {
   using Shape = QdShape<D>;
   constexpr int SUB = Shape::SUB, KEYS = Shape::KEYS, JD = D / 64, VW = D / 32;      // VW: words of a thread's dimensions of a key
-  extern __shared__ __align__(128) uint8_t qd_shared[];
-  int* before = reinterpret_cast<int*>(qd_shared + QD_WARPS * QD_STAGES * Shape::STAGE);      // [requests + 1] tiles before a request's
+  extern __shared__ uint8_t qd_shared_raw[];
+  uint8_t* qd_shared = (uint8_t*)(((uintptr_t)qd_shared_raw + 1023) & ~(uintptr_t)1023);      // what swizzled copies need
+  int* before = reinterpret_cast<int*>(qd_shared + Shape::SHARED);      // [requests + 1] tiles before a request's
   __shared__ int warp_sums[QD_WARPS], warp_most[QD_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group = heads / kv_heads, page_size = 1 << page_shift;
+  uint8_t* stages = qd_shared + warp * QD_STAGES * Shape::DATA;
+  uint8_t* scale_stages = qd_shared + Shape::RING + warp * QD_STAGES * Shape::SCALES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(qd_shared + Shape::RING + QD_WARPS * QD_STAGES * Shape::SCALES) + warp * QD_STAGES;
+  if (lane == 0) {
+    for (int i = 0; i < QD_STAGES; ++i) mbar_init(full + i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
+  }
   pdl_trigger();
 
   auto segment_of = [&](int index) { return decode_seg != nullptr ? decode_seg[index] : index; };
@@ -166,9 +182,10 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
     if (threadIdx.x == 0) lines[0] = (int)share;
   }
 
-  uint8_t* stages = qd_shared + warp * QD_STAGES * Shape::STAGE;
-  const uint32_t stage_at = (uint32_t)__cvta_generic_to_shared(stages);
-  while (at < end) {
+  const uint32_t scales_at = smem_u32(scale_stages);
+  unsigned tiles_before = 0;        // of this warp's earlier pairs: the ring and its phases run on
+  bool gave_up = false;             // a wait ran out: the warp ends, the host raises
+  while (at < end && !gave_up) {
     const int request_tiles = before[request + 1] - before[request], length = request_tiles + QD_BEGIN;
     const int kv_head = (int)((at - line_of(request)) / length);
     const long long pair_begin = line_of(request) + (long long)kv_head * length, pair_end = pair_begin + length;
@@ -190,42 +207,32 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
       const int page = n < my_tiles && logical < table_width ? table[logical] : 0;
       return page >= 0 && page < pool_pages ? page : 0;
     };
-    const int lane_k = g * D + 16 * t, lane_v = 2 * t * D + (D / 8) * g;
     auto issue = [&](int n, int to, const int (&pages)[SUB]) {
       if (n < my_tiles) {
-        const uint32_t dst = stage_at + to * Shape::STAGE;
+        if (lane == 0) mbar_expect_tx(full + to, Shape::DATA);
 #pragma unroll
         for (int sub = 0; sub < SUB; ++sub) {
-          const int key0 = (first_tile + n) * KEYS + sub * 16, offset = key0 & (page_size - 1);
-          const size_t line = (size_t)pages[sub] * kv_heads + kv_head;
-          const size_t token = (line << page_shift) + offset;
-          const int8_t* k_src = k_pool + (token * D + lane_k);
-          const int8_t* v_src = v_pool + (token * D + lane_v);
-          const uint32_t k_dst = dst + sub * (32 * D) + lane * 16;
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int j = 0; j < JD; ++j) qd_copy16(k_dst + (half * JD + j) * 512, k_src + 8 * half * D + 64 * j);
-          const uint32_t v_dst = dst + sub * (32 * D) + 16 * D + lane * (VW * 4);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int8_t* src = v_src + ((i & 1) + 8 * (i >> 1)) * D;
-            if constexpr (D == 128) qd_copy16(v_dst + i * 512, src);
-            else qd_copy8(v_dst + i * 256, src);
+          const int key0 = (first_tile + n) * KEYS + sub * 16;
+          const int token = ((pages[sub] * kv_heads + kv_head) << page_shift) + (key0 & (page_size - 1));
+          if (lane == 0) {
+            uint8_t* dst = stages + to * Shape::DATA + sub * 2 * Shape::PART;
+            tma_load_2d(&k_map, full + to, dst, 0, token);
+            tma_load_2d(&v_map, full + to, dst + Shape::PART, 0, token);
           }
           // lanes 0..15 the keys' scales, 16..31 the values'
           const float* scales = lane < 16 ? k_scales : v_scales;
-          qd_copy4(dst + Shape::DATA + sub * 128 + lane * 4, scales + ((token + (lane & 15)) >> block_shift));
+          qd_copy4(scales_at + to * Shape::SCALES + sub * 128 + lane * 4, scales + ((token + (lane & 15)) >> block_shift));
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    int stage_of = (int)(tiles_before % QD_STAGES);
     int pages[SUB];
 #pragma unroll
     for (int n = 0; n < QD_STAGES; ++n) {
 #pragma unroll
       for (int sub = 0; sub < SUB; ++sub) pages[sub] = page_of(n, sub);
-      issue(n, n, pages);
+      issue(n, (stage_of + n) % QD_STAGES, pages);
     }
 #pragma unroll
     for (int sub = 0; sub < SUB; ++sub) pages[sub] = page_of(QD_STAGES, sub);
@@ -292,25 +299,32 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) o[h][i][0] = o[h][i][1] = o[h][i][2] = o[h][i][3] = 0.f;
     }
-    int stage_of = 0;
     for (int n = 0; n < my_tiles; ++n) {
       asm volatile("cp.async.wait_group %0;" ::"n"(QD_STAGES - 1) : "memory");
+      gave_up = !mbar_wait(full + stage_of, ((tiles_before + n) / QD_STAGES) & 1u, error_word, 0x91);
+      gave_up = __any_sync(0xffffffffu, gave_up);
+      if (gave_up) {                  // the copies under way end before the warp does
+        for (int later = n; later < my_tiles && later < n + QD_STAGES; ++later)
+          mbar_wait(full + (tiles_before + later) % QD_STAGES, ((tiles_before + later) / QD_STAGES) & 1u, error_word, 0x92);
+        break;
+      }
       __syncwarp();
-      const uint8_t* stage = stages + stage_of * Shape::STAGE;
+      const uint8_t* stage = stages + stage_of * Shape::DATA;
       const int key_tile = (first_tile + n) * KEYS;
 #pragma unroll
       for (int sub = 0; sub < SUB; ++sub) {
         const int key0 = key_tile + sub * 16;
-        const uint8_t* k_data = stage + sub * (32 * D) + lane * 16;
-        const uint8_t* v_data = stage + sub * (32 * D) + 16 * D + lane * (VW * 4);
-        const float* scales = reinterpret_cast<const float*>(stage + Shape::DATA + sub * 128);
+        const uint8_t* k_data = stage + sub * 2 * Shape::PART;
+        const uint8_t* v_data = k_data + Shape::PART;
+        const float* scales = reinterpret_cast<const float*>(scale_stages + stage_of * Shape::SCALES + sub * 128);
         // scores^T: rows keys g, g + 8, columns heads 2 t, 2 t + 1
         float s[NH][4];
 #pragma unroll
         for (int h = 0; h < NH; ++h) { s[h][0] = s[h][2] = start[h][0]; s[h][1] = s[h][3] = start[h][1]; }
 #pragma unroll
         for (int j = 0; j < JD; ++j) {
-          const uint4 low = *reinterpret_cast<const uint4*>(k_data + j * 512), high = *reinterpret_cast<const uint4*>(k_data + (JD + j) * 512);
+          const uint4 low = *reinterpret_cast<const uint4*>(k_data + qd_place<D>(g, 4 * j + t));
+          const uint4 high = *reinterpret_cast<const uint4*>(k_data + qd_place<D>(g + 8, 4 * j + t));
           const uint32_t a[4] = {low.x, low.y, low.z, low.w}, b[4] = {high.x, high.y, high.z, high.w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -374,8 +388,9 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
         uint32_t v[4][VW];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if constexpr (D == 128) *reinterpret_cast<uint4*>(v[i]) = *reinterpret_cast<const uint4*>(v_data + i * 512);
-          else *reinterpret_cast<uint2*>(v[i]) = *reinterpret_cast<const uint2*>(v_data + i * 256);
+          const int key = 2 * t + (i & 1) + 8 * (i >> 1);
+          if constexpr (D == 128) *reinterpret_cast<uint4*>(v[i]) = *reinterpret_cast<const uint4*>(v_data + qd_place<D>(key, g));
+          else *reinterpret_cast<uint2*>(v[i]) = *reinterpret_cast<const uint2*>(v_data + qd_place<D>(key, g >> 1) + 8 * (g & 1));
         }
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
@@ -397,6 +412,7 @@ attention_quantized_decode_kernel(const bf16* q, const int8_t* k_pool, const int
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncwarp();
+    tiles_before += (unsigned)my_tiles;
 
     // ---- the pair's outputs, or this warp's part of them
     const bool whole = from == 0 && my_end == pair_end;
@@ -450,21 +466,34 @@ merge_quantized_decode_kernel(const float* states, const float2* sums, const int
   const int parts = (int)(last - first) + 1;
   // part i: the first one's pair begins in its share, the others' began before
   auto slot_of = [&](int i) { return (size_t)((first + i) * 2 + (i == 0 ? 1 : 0)) * 8 * NH + head; };
-  float top = -INFINITY;
-  for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(sums + slot_of(i)).x);
-  float total = 0.f;
+  constexpr int AHEAD = 8;         // parts whose numbers are asked for at once
+  float top = -INFINITY, total = 0.f;
   float4 value = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const float2 state = __ldcg(sums + slot_of(i));
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(states + slot_of(i) * D) + d);
+  for (int base = 0; base < parts; base += AHEAD) {
+    float2 state[AHEAD];
+    float4 v[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      state[i] = base + i < parts ? __ldcg(sums + slot_of(base + i)) : make_float2(-INFINITY, 0.f);
+      v[i] = base + i < parts ? __ldcg(reinterpret_cast<const float4*>(states + slot_of(base + i) * D) + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float higher = top;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) higher = fmaxf(higher, state[i].x);
+    const float down = top == -INFINITY ? 0.f : qd_exp2(top - higher);
+    top = higher;
     // (a part whose scores are no numbers has no largest one and a NaN sum, which stays)
-    const float weight = state.x == -INFINITY ? 0.f : qd_exp2(state.x - top);
-    total += state.y * (state.y == state.y ? weight : 1.f);
-    value.x = fmaf(v.x, weight, value.x);
-    value.y = fmaf(v.y, weight, value.y);
-    value.z = fmaf(v.z, weight, value.z);
-    value.w = fmaf(v.w, weight, value.w);
+    total *= total == total ? down : 1.f;
+    value = make_float4(value.x * down, value.y * down, value.z * down, value.w * down);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const float weight = state[i].x == -INFINITY ? 0.f : qd_exp2(state[i].x - top);
+      total += state[i].y * (state[i].y == state[i].y ? weight : 1.f);
+      value.x = fmaf(v[i].x, weight, value.x);
+      value.y = fmaf(v[i].y, weight, value.y);
+      value.z = fmaf(v[i].z, weight, value.z);
+      value.w = fmaf(v[i].w, weight, value.w);
+    }
   }
   const float inverse = 1.f / total;
   const __nv_bfloat162 low = __floats2bfloat162_rn(value.x * inverse, value.y * inverse), high = __floats2bfloat162_rn(value.z * inverse, value.w * inverse);
@@ -490,25 +519,56 @@ static QdLayout qd_layout(int requests, int kv_heads, int group, int dim, int wi
   return at;
 }
 
+// rows x dim bytes, row-major, a box of 16 rows; the maps of pools are kept, as in cached_tile_map.
+static bool qd_map(CUtensorMap* out, const void* base, long long rows, int dim) {
+  constexpr int SLOTS = 1024;
+  static TileMapKey keys[SLOTS];
+  static CUtensorMap maps[SLOTS];
+  const TileMapKey key{base, rows, dim, 16};
+  const unsigned long long h = (unsigned long long)(uintptr_t)base * 0x9E3779B97F4A7C15ull + (unsigned long long)rows * 0xBF58476D1CE4E5B9ull + dim;
+  const int slot = (int)((h >> 40) % SLOTS);
+  if (!(keys[slot] == key) || base == nullptr) {
+    auto encode = encode_tiled();
+    if (encode == nullptr) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)dim};
+    cuuint32_t box[2] = {(cuuint32_t)dim, 16u};
+    cuuint32_t element_strides[2] = {1, 1};
+    keys[slot] = TileMapKey{nullptr, 0, 0, 0};
+    if (encode(&maps[slot], CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, element_strides,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+    keys[slot] = key;
+  }
+  *out = maps[slot];
+  return true;
+}
+
 template <int D, int NH>
 static int quantized_decode_launch(const void* q, const void* k_pool, const void* v_pool, const float* k_scales, const float* v_scales, void* out,
                                    const int* decode_seg, const int* seg_q_start, const int* seg_pos0, const int* block_table, const int* seg_slot,
                                    int table_width, int requests, int heads, int kv_heads, int page_shift, int block_shift, int pool_pages, int window,
-                                   float scale, int longest, uint8_t* scratch, cudaStream_t stream) {
+                                   float scale, int longest, uint8_t* scratch, int* error_word, cudaStream_t stream) {
   auto kernel = attention_quantized_decode_kernel<D, NH>;
-  constexpr size_t ring = (size_t)QD_WARPS * QD_STAGES * QdShape<D>::STAGE;
+  constexpr size_t shared = 1024 + QdShape<D>::SHARED;
+  static_assert(2 * (shared + (QD_MOST_REQUESTS + 1) * sizeof(int) + 1024) <= 228 * 1024, "two CTAs per SM");
+  const long long pool_rows = ((long long)pool_pages * kv_heads) << page_shift;
+  if (pool_rows >= (1ll << 31)) return MLR_TOO_LARGE;
+  CUtensorMap k_map, v_map;
+  if (!qd_map(&k_map, k_pool, pool_rows, D) || !qd_map(&v_map, v_pool, pool_rows, D)) return MLR_BAD_SIZE;
   static OncePerDevice once;
   const cudaError_t err = once([&] {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ring + (QD_MOST_REQUESTS + 1) * sizeof(int)));
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(shared + (QD_MOST_REQUESTS + 1) * sizeof(int)));
   });
   if (err != cudaSuccess) return (int)err;
   const QdLayout at = qd_layout(requests, kv_heads, heads / kv_heads, D, window, longest);
   float* states = (float*)scratch;
   float2* sums = (float2*)(scratch + at.sums);
   int* lines = (int*)(scratch + at.lines);
-  launch_kernel(kernel, dim3(at.ctas), dim3(QD_THREADS), ring + (requests + 1) * sizeof(int), stream, (const bf16*)q, (const int8_t*)k_pool,
-                (const int8_t*)v_pool, k_scales, v_scales, (bf16*)out, decode_seg, seg_q_start, seg_pos0, block_table, seg_slot, table_width, requests,
-                heads, kv_heads, page_shift, block_shift, pool_pages, window, scale * 1.4426950408889634f, states, sums, lines);
+  launch_kernel(kernel, dim3(at.ctas), dim3(QD_THREADS), shared + (requests + 1) * sizeof(int), stream, k_map, v_map, (const bf16*)q, k_scales,
+                v_scales, (bf16*)out, decode_seg, seg_q_start, seg_pos0, block_table, seg_slot, table_width, requests,
+                heads, kv_heads, page_shift, block_shift, pool_pages, window, scale * 1.4426950408889634f, states, sums, lines, error_word);
   launch_kernel(merge_quantized_decode_kernel<D, NH>, dim3(requests * kv_heads), dim3(8 * NH * D / 4), 0, stream, states, sums, lines, (bf16*)out,
                 decode_seg, seg_q_start, heads, kv_heads);
   return launch_status();
@@ -533,14 +593,16 @@ MLR_EXPORT long long mlr_attention_quantized_decode_bytes(int requests, int kv_h
 
 // q, out: [rows, heads * dim] bfloat16, of which the rows of `requests` decoded tokens are attended (decode_seg: their segments, or null for
 // segments 0, 1, ..); pools [pages, kv_heads, page_size, dim]; scales [pages, kv_heads, page_size / block]; longest: keys of the longest context
-// (a longer one is attended all the same); scratch: memory of the size above.
+// (a longer one is attended all the same); scratch: memory of the size above; error_word: host-visible int that
+// receives a code if a wait runs out.
 MLR_EXPORT int mlr_attention_quantized_decode(const void* q, const void* k_pool, const void* v_pool, const float* k_scales, const float* v_scales,
                                               void* out, const int* decode_seg, const int* seg_q_start, const int* seg_pos0, const int* block_table,
                                               const int* seg_slot, int table_width, int requests, int heads, int kv_heads, int dim, int page_size,
                                               int block, int pool_pages, int window, float scale, int longest, void* scratch,
-                                              cudaStream_t stream) {
+                                              int* error_word, cudaStream_t stream) {
   if (requests == 0) return MLR_OK;
-  if (requests < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || table_width <= 0 || pool_pages <= 0 || longest <= 0) return MLR_BAD_SIZE;
+  if (requests < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || table_width <= 0 || pool_pages <= 0 || longest <= 0 || error_word == nullptr)
+    return MLR_BAD_SIZE;
   const int page_shift = shift_of(page_size), block_shift = shift_of(block);
   if ((dim != 64 && dim != 128) || page_shift < 4 || block_shift < 0 || block > page_size) return MLR_BAD_SIZE;
   if (heads / kv_heads > 16 || requests > QD_MOST_REQUESTS) return MLR_TOO_LARGE;
@@ -549,7 +611,7 @@ MLR_EXPORT int mlr_attention_quantized_decode(const void* q, const void* k_pool,
 #define MLR_DECODE(D_, N_)                                                                                                                       \
   return quantized_decode_launch<D_, N_>(q, k_pool, v_pool, k_scales, v_scales, out, decode_seg, seg_q_start, seg_pos0, block_table, seg_slot,   \
                                          table_width, requests, heads, kv_heads, page_shift, block_shift, pool_pages, window, scale, longest,    \
-                                         (uint8_t*)scratch, stream)
+                                         (uint8_t*)scratch, error_word, stream)
   if (dim == 64) { if (wide) MLR_DECODE(64, 2); MLR_DECODE(64, 1); }
   if (wide) MLR_DECODE(128, 2);
   MLR_DECODE(128, 1);

@@ -113,7 +113,7 @@ _PROTOTYPES = {
     "logit_rules": {"mlr_logit_rules": "pppiipp", "mlr_count_tokens": "ppippiiip"},
     "quantized_pages": {"mlr_quantize_kv": "plplp" "pppp" "iiiiii" "ip", "mlr_dequantize_pages": "ppppppp" "iiiiii" "ip"},
     "copy_pages": {"mlr_copy_pages": "pippip"},
-    "attention_quantized_decode": {"mlr_attention_quantized_decode": "pppppp" "ppppp" "iiiiiiiii" "fi" "pp",
+    "attention_quantized_decode": {"mlr_attention_quantized_decode": "pppppp" "ppppp" "iiiiiiiii" "fi" "ppp",
                                    "mlr_attention_quantized_decode_bytes": "iiiiii"},
     "attention_quantized_prompt": {"mlr_attention_quantized_prompt": "pppppp" "ppppppp" "iiiiiiiiiiii" "fi" "pppp" "l" "pip",
                                    "mlr_attention_quantized_prompt_bytes": "iiiiii"},
@@ -1295,7 +1295,7 @@ class CudaOps:
             q_start, _, pos0, *table = segments
             _check(library.mlr_attention_quantized_decode(
                 q.data_ptr(), *pools, out.data_ptr(), _address(listed), q_start, pos0, *table, batch.num_decode, *sizes, int(batch.max_kv_len),
-                scratch.data_ptr(), _raw_stream()), "quantized_attention (decoded tokens)")
+                scratch.data_ptr(), self._error_word(q.device).data_ptr(), _raw_stream()), "quantized_attention (decoded tokens)")
             rest -= batch.num_decode
         if rest > 0:
             _check(_declared_library("attention_quantized").mlr_attention_quantized(
