@@ -97,6 +97,15 @@ __device__ __forceinline__ uint32_t qd_half2(uint32_t turned) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// The lowest key that a position sees, its tiles, and what a warp takes of a line of `units`, whose longest pair has `most` tiles.
+__device__ __forceinline__ int qd_lowest(int position, int window) { return window > 0 ? max(0, position - window + 1) : 0; }
+template <int KEYS>
+__device__ __forceinline__ int qd_tiles(int position, int window) { return position / KEYS - qd_lowest(position, window) / KEYS + 1; }
+__device__ __forceinline__ long long qd_share(long long units, int most, int ctas) {
+  const long long walkers = (long long)ctas * QD_WARPS;
+  return max((units + walkers - 1) / walkers, (long long)max(QD_LEAST_SHARE, (most + QD_MOST_PARTS - 2) / (QD_MOST_PARTS - 1)));
+}
+
 // NH: groups of 8 query heads.
 template <int D, int NH>
 __global__ void __launch_bounds__(QD_THREADS, 2)
@@ -104,7 +113,7 @@ attention_quantized_decode_kernel(const __grid_constant__ CUtensorMap k_map, con
                                   const float* k_scales, const float* v_scales, bf16* __restrict__ out, const int* __restrict__ decode_seg, const int* __restrict__ seg_q_start,
                                   const int* __restrict__ seg_pos0, const int* __restrict__ block_table, const int* __restrict__ seg_slot,
                                   int table_width, int requests, int heads, int kv_heads, int page_shift, int block_shift, int pool_pages, int window,
-                                  float scale_log2, float* __restrict__ states, float2* __restrict__ sums, int* __restrict__ lines, int* error_word) {
+                                  float scale_log2, float* __restrict__ states, float2* __restrict__ sums, int* error_word) {
   using Shape = QdShape<D>;
   constexpr int SUB = Shape::SUB, KEYS = Shape::KEYS, JD = D / 64, VW = D / 32;      // VW: words of a thread's dimensions of a key
   extern __shared__ uint8_t qd_shared_raw[];
@@ -127,7 +136,7 @@ attention_quantized_decode_kernel(const __grid_constant__ CUtensorMap k_map, con
   pdl_trigger();
 
   auto segment_of = [&](int index) { return decode_seg != nullptr ? decode_seg[index] : index; };
-  auto lowest_of = [&](int position) { return window > 0 ? max(0, position - window + 1) : 0; };
+  auto lowest_of = [&](int position) { return qd_lowest(position, window); };
   // ---- tiles before each request's (positions are metadata of the step: read before the wait)
   int carried = 0, most = 0;
   for (int first = 0; first < requests; first += QD_THREADS) {
@@ -135,7 +144,7 @@ attention_quantized_decode_kernel(const __grid_constant__ CUtensorMap k_map, con
     int tiles = 0;
     if (index < requests) {
       const int position = seg_pos0[segment_of(index)];
-      tiles = position / KEYS - lowest_of(position) / KEYS + 1;
+      tiles = qd_tiles<KEYS>(position, window);
     }
     const int warp_top = (int)__reduce_max_sync(0xffffffffu, (unsigned)tiles);
     int inclusive = tiles;
@@ -160,9 +169,7 @@ attention_quantized_decode_kernel(const __grid_constant__ CUtensorMap k_map, con
   __syncthreads();
   // the line: request after request, a request's kv heads one behind the other, each QD_BEGIN longer than its tiles
   auto line_of = [&](int index) { return ((long long)before[index] + (long long)index * QD_BEGIN) * kv_heads; };
-  const long long units = line_of(requests), walkers = (long long)gridDim.x * QD_WARPS;
-  long long share = (units + walkers - 1) / walkers;
-  share = max(share, (long long)max(QD_LEAST_SHARE, (most + QD_MOST_PARTS - 2) / (QD_MOST_PARTS - 1)));
+  const long long units = line_of(requests), share = qd_share(units, most, gridDim.x);
   const long long walker = (long long)blockIdx.x * QD_WARPS + warp;
   long long at = share * walker;
   const long long end = min(units, at + share);
@@ -177,10 +184,6 @@ attention_quantized_decode_kernel(const __grid_constant__ CUtensorMap k_map, con
     request = low;
   }
   pdl_wait();
-  if (blockIdx.x == 0) {                            // for the merge
-    for (int index = threadIdx.x; index <= requests; index += QD_THREADS) lines[1 + index] = before[index];
-    if (threadIdx.x == 0) lines[0] = (int)share;
-  }
 
   const uint32_t scales_at = smem_u32(scale_stages);
   unsigned tiles_before = 0;        // of this warp's earlier pairs: the ring and its phases run on
@@ -452,21 +455,40 @@ attention_quantized_decode_kernel(const __grid_constant__ CUtensorMap k_map, con
 // The parts of pairs that several warps walked.  A CTA per pair, a thread per head and four dimensions.
 template <int D, int NH>
 __global__ void __launch_bounds__(8 * NH * D / 4)
-merge_quantized_decode_kernel(const float* states, const float2* sums, const int* lines, bf16* __restrict__ out,
-                              const int* __restrict__ decode_seg, const int* __restrict__ seg_q_start, int heads, int kv_heads) {
+merge_quantized_decode_kernel(const float* states, const float2* sums, bf16* __restrict__ out, const int* __restrict__ decode_seg,
+                              const int* __restrict__ seg_q_start, const int* __restrict__ seg_pos0, int requests, int heads, int kv_heads,
+                              int window, int ctas) {
+  constexpr int KEYS = QdShape<D>::KEYS, THREADS = 8 * NH * D / 4;
+  __shared__ int found[3];       // tiles of the requests before this one, of all, of the longest
   pdl_trigger();
   const int request = blockIdx.x / kv_heads, kv_head = blockIdx.x - request * kv_heads, group = heads / kv_heads;
-  const int head = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4);
-  const int row = seg_q_start[decode_seg != nullptr ? decode_seg[request] : request];
-  pdl_wait();
-  const int share = __ldcg(lines), before = __ldcg(lines + 1 + request), length = __ldcg(lines + 2 + request) - before + QD_BEGIN;
+  const int head = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4), lane = threadIdx.x & 31;
+  auto segment_of = [&](int index) { return decode_seg != nullptr ? decode_seg[index] : index; };
+  if (threadIdx.x < 3) found[threadIdx.x] = 0;
+  __syncthreads();
+  unsigned sum = 0, all = 0, most = 0;
+  for (int index = threadIdx.x; index < requests; index += THREADS) {
+    const unsigned tiles = (unsigned)qd_tiles<KEYS>(seg_pos0[segment_of(index)], window);
+    if (index < request) sum += tiles;
+    all += tiles;
+    most = max(most, tiles);
+  }
+  sum = __reduce_add_sync(0xffffffffu, sum);
+  all = __reduce_add_sync(0xffffffffu, all);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) { atomicAdd(&found[0], (int)sum); atomicAdd(&found[1], (int)all); atomicMax(&found[2], (int)most); }
+  const int segment = segment_of(request), row = seg_q_start[segment], length = qd_tiles<KEYS>(seg_pos0[segment], window) + QD_BEGIN;
+  __syncthreads();
+  const int before = found[0];
+  const long long share = qd_share(((long long)found[1] + (long long)requests * QD_BEGIN) * kv_heads, found[2], ctas);
   const long long begin = ((long long)before + (long long)request * QD_BEGIN) * kv_heads + (long long)kv_head * length;
   const long long first = (begin + QD_BEGIN) / share, last = (begin + length - 1) / share;
+  pdl_wait();                                      // (all: whoever waits for this launch waits for the one before it too)
   if (first == last || head >= group) return;      // one warp wrote the outputs
   const int parts = (int)(last - first) + 1;
   // part i: the first one's pair begins in its share, the others' began before
   auto slot_of = [&](int i) { return (size_t)((first + i) * 2 + (i == 0 ? 1 : 0)) * 8 * NH + head; };
-  constexpr int AHEAD = 8;         // parts whose numbers are asked for at once
+  constexpr int AHEAD = 12;        // parts whose numbers are asked for at once
   float top = -INFINITY, total = 0.f;
   float4 value = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int base = 0; base < parts; base += AHEAD) {
@@ -504,7 +526,7 @@ merge_quantized_decode_kernel(const float* states, const float2* sums, const int
 // Warps of a launch, and where the parts' memory lies (bytes).
 struct QdLayout {
   int ctas;
-  long long sums, lines, total;
+  long long sums, total;
 };
 static QdLayout qd_layout(int requests, int kv_heads, int group, int dim, int window, int longest) {
   const int keys = window > 0 && window < longest ? window + 16 : longest, tile = 16 * (128 / dim), per = group > 8 ? 16 : 8;
@@ -514,8 +536,7 @@ static QdLayout qd_layout(int requests, int kv_heads, int group, int dim, int wi
   at.ctas = (int)(ctas < most ? ctas : most);
   const long long slots = (long long)at.ctas * QD_WARPS * 2 * per;
   at.sums = slots * dim * 4;
-  at.lines = at.sums + slots * 8;
-  at.total = at.lines + ((long long)requests + 2) * 4;
+  at.total = at.sums + slots * 8;
   return at;
 }
 
@@ -565,12 +586,11 @@ static int quantized_decode_launch(const void* q, const void* k_pool, const void
   const QdLayout at = qd_layout(requests, kv_heads, heads / kv_heads, D, window, longest);
   float* states = (float*)scratch;
   float2* sums = (float2*)(scratch + at.sums);
-  int* lines = (int*)(scratch + at.lines);
   launch_kernel(kernel, dim3(at.ctas), dim3(QD_THREADS), shared + (requests + 1) * sizeof(int), stream, k_map, v_map, (const bf16*)q, k_scales,
                 v_scales, (bf16*)out, decode_seg, seg_q_start, seg_pos0, block_table, seg_slot, table_width, requests,
-                heads, kv_heads, page_shift, block_shift, pool_pages, window, scale * 1.4426950408889634f, states, sums, lines, error_word);
-  launch_kernel(merge_quantized_decode_kernel<D, NH>, dim3(requests * kv_heads), dim3(8 * NH * D / 4), 0, stream, states, sums, lines, (bf16*)out,
-                decode_seg, seg_q_start, heads, kv_heads);
+                heads, kv_heads, page_shift, block_shift, pool_pages, window, scale * 1.4426950408889634f, states, sums, error_word);
+  launch_kernel(merge_quantized_decode_kernel<D, NH>, dim3(requests * kv_heads), dim3(8 * NH * D / 4), 0, stream, states, sums, (bf16*)out, decode_seg,
+                seg_q_start, seg_pos0, requests, heads, kv_heads, window, at.ctas);
   return launch_status();
 }
 

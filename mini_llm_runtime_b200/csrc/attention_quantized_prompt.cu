@@ -122,13 +122,13 @@ quantized_prompt_prepare_kernel(const bf16* q, const int8_t* k_pool, const int8_
   }
   __syncthreads();
   const int segment = found_segment;
+  pdl_wait();                              // (all: whoever waits for this launch waits for the one before it too)
   if (segment < 0) return;                 // a window left fewer tiles than were counted
   const int q_len = seg_q_len[segment], pos0 = seg_pos0[segment];
   const QpSegment mine = qp_segment(q_len, pos0, window);
   const int within = unit - found_first * kv_heads, kv_head = within / mine.tiles, key0 = (mine.base_tile + within - kv_head * mine.tiles) * QP_KEYS;
   const int last = pos0 + q_len - 1, lowest = window > 0 ? max(0, pos0 - window + 1) : 0;
   const int* table = block_table + (size_t)(seg_slot != nullptr ? seg_slot[segment] : segment) * table_width;
-  pdl_wait();
   auto line_of = [&](int key, int* offset) -> long long {      // -1: no such key
     const int logical = key / page_size;
     const int page = key >= lowest && key <= last && logical < table_width ? table[logical] : -1;

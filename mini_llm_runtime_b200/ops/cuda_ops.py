@@ -341,7 +341,10 @@ class QuantizedPool:
             raise KernelError("a pool holds fewer than 2^31 heads' tokens")
         _need_together(self.key, self.value, self.key_scales, self.value_scales)
         for name, value in (("pages", pages), ("kv_heads", kv_heads), ("page_size", page_size), ("dim", dim), ("block", page_size // blocks),
-                            ("device", self.key.device)):
+                            ("device", self.key.device),
+                            # what a call asks for, once (of tensors held here)
+                            ("addresses", tuple(_address(t) for t in (self.key, self.value, self.key_scales, self.value_scales))),
+                            ("wide", not (self.key.data_ptr() | self.value.data_ptr()) % 16)):
             object.__setattr__(self, name, value)
 
 
@@ -519,6 +522,12 @@ def latent_prompt_on_tcgen05(batch: AttentionBatch, rows: int, window: int) -> b
     16 / 18 (21 / 23), 96 keys 20 / 19 (25 / 25); 24 rows, 96 keys 21 / 21 (27 / 25); beside a decoded row 4 rows, 64 keys 26 / 26
     (30 / 32), 128 keys 32 / 26, 8 rows, 96 keys 30 / 30 (36 / 38), 128 keys 32 / 28."""
     return prompt_keys(batch, window) > 96 or rows - batch.num_decode > 64
+
+
+@functools.lru_cache(maxsize=256)
+def _quantized_decode_bytes(*sizes) -> int:
+    """Scratch memory of a decode step over keys and values in 8 bits (the last size: the device's index)."""
+    return _declared_library("attention_quantized_decode").mlr_attention_quantized_decode_bytes(*sizes[:-1])
 
 
 class CudaOps:
@@ -1228,9 +1237,8 @@ class CudaOps:
         if rows == 0:
             return
         _check(_declared_library("quantized_pages").mlr_quantize_kv(
-            key.data_ptr(), strides[0], value.data_ptr(), strides[1], slots.data_ptr(), pool.key.data_ptr(), pool.value.data_ptr(), pool.key_scales.data_ptr(),
-            pool.value_scales.data_ptr(), rows, pool.kv_heads, pool.dim, pool.page_size, pool.block, pool.pages, _code(key.dtype),
-            _raw_stream()), "quantize_kv_write")
+            key.data_ptr(), strides[0], value.data_ptr(), strides[1], slots.data_ptr(), *pool.addresses, rows, pool.kv_heads,
+            pool.dim, pool.page_size, pool.block, pool.pages, _code(key.dtype), _raw_stream()), "quantize_kv_write")
 
     def dequantize_pages(self, pool: QuantizedPool, pages: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
         """What the codes of ``pages`` int32 [n] stand for: keys and values [n, kv_heads, page_size, dim].  A page that the pool does not
@@ -1242,8 +1250,7 @@ class CudaOps:
         if pages.shape[0] == 0:
             return key, value
         _check(_declared_library("quantized_pages").mlr_dequantize_pages(
-            pool.key.data_ptr(), pool.value.data_ptr(), pool.key_scales.data_ptr(), pool.value_scales.data_ptr(), pages.data_ptr(),
-            key.data_ptr(), value.data_ptr(), pages.shape[0], pool.kv_heads, pool.dim, pool.page_size, pool.block, pool.pages, _code(out_dtype),
+            *pool.addresses, pages.data_ptr(), key.data_ptr(), value.data_ptr(), pages.shape[0], pool.kv_heads, pool.dim, pool.page_size, pool.block, pool.pages, _code(out_dtype),
             _raw_stream()), "dequantize_pages")
         return key, value
 
@@ -1266,13 +1273,16 @@ class CudaOps:
         out = torch.empty_like(q)
         if q.shape[0] == 0:
             return out
-        plan, counts = batch.plan, batch.counts
-        cores = self._quantized_on_tensor_cores(q, pool, num_heads)
+        plan, counts, decodes = batch.plan, batch.counts, batch.num_decode
+        window = int(window or 0)
+        group = num_heads // num_kv_heads
+        # bfloat16 queries over pages that whole groups of 16 keys lie on: tensor cores; everything else takes the general kernel
+        cores = (self.use_mma_attention and q.dtype == torch.bfloat16 and head_dim in (64, 128) and group <= 16 and pool.page_size >= 16
+                 and pool.page_size & (pool.page_size - 1) == 0 and pool.block & (pool.block - 1) == 0 and pool.wide and not q.data_ptr() % 16)
+        q_start, pos0, slot = batch.seg_q_start.data_ptr(), batch.seg_pos0.data_ptr(), batch.seg_slot.data_ptr()
+        table, width = batch.block_table.data_ptr(), batch.block_table.shape[1]
+        sizes = (num_heads, num_kv_heads, head_dim, pool.page_size, pool.block, pool.pages, window, scale)
         first, rest = 0, counts["tiles"]          # of the work list, the decoded tokens' last: what the general kernel takes
-        pools = (pool.key.data_ptr(), pool.value.data_ptr(), pool.key_scales.data_ptr(), pool.value_scales.data_ptr())
-        segments = (batch.seg_q_start.data_ptr(), batch.seg_q_len.data_ptr(), batch.seg_pos0.data_ptr(), batch.block_table.data_ptr(),
-                    batch.seg_slot.data_ptr(), batch.block_table.shape[1])
-        sizes = (num_heads, num_kv_heads, head_dim, pool.page_size, pool.block, pool.pages, int(window or 0), scale)
         if cores and counts["big"] > 0 and scale > 0:
             # codes to float16 once, then tcgen05 products (scores are ordered before they are scaled: scale > 0)
             library = _declared_library("attention_quantized_prompt")
@@ -1280,36 +1290,28 @@ class CudaOps:
             prepared = torch.empty(library.mlr_attention_quantized_prompt_bytes(*shape, batch.num_segments), dtype=torch.uint8, device=q.device)
             space = self._workspace(q.device)
             _check(library.mlr_attention_quantized_prompt(
-                q.data_ptr(), *pools, out.data_ptr(), plan["big_tile_seg"].data_ptr(), plan["big_tile_row0"].data_ptr(), *segments, batch.num_segments,
-                counts["big"], counts["prompt_tiles"], q.shape[0], *sizes, int(batch.max_kv_len), prepared.data_ptr(),
-                space["prefill_queue"].data_ptr(), space["error_word"].data_ptr(), space["prefill_scratch"].data_ptr(),
-                space["prefill_scratch"].numel(), space["prefill_counters"].data_ptr(), space["prefill_counters"].numel(), _raw_stream()),
-                "quantized_attention (prompts)")
-            first, rest = rest - batch.num_decode, batch.num_decode
-        if cores and 0 < batch.num_decode <= self.QUANTIZED_DECODES:
-            library = _declared_library("attention_quantized_decode")
-            scratch = torch.empty(library.mlr_attention_quantized_decode_bytes(
-                batch.num_decode, num_kv_heads, num_heads // num_kv_heads, head_dim, int(window or 0), int(batch.max_kv_len)),
-                dtype=torch.uint8, device=q.device)
-            listed = None if batch.num_decode == batch.num_segments else plan["decode_seg"]
-            q_start, _, pos0, *table = segments
-            _check(library.mlr_attention_quantized_decode(
-                q.data_ptr(), *pools, out.data_ptr(), _address(listed), q_start, pos0, *table, batch.num_decode, *sizes, int(batch.max_kv_len),
-                scratch.data_ptr(), self._error_word(q.device).data_ptr(), _raw_stream()), "quantized_attention (decoded tokens)")
-            rest -= batch.num_decode
+                q.data_ptr(), *pool.addresses, out.data_ptr(), plan["big_tile_seg"].data_ptr(), plan["big_tile_row0"].data_ptr(), q_start,
+                batch.seg_q_len.data_ptr(), pos0, table, slot, width, batch.num_segments, counts["big"], counts["prompt_tiles"], q.shape[0], *sizes,
+                int(batch.max_kv_len), prepared.data_ptr(), space["prefill_queue"].data_ptr(), space["error_word"].data_ptr(),
+                space["prefill_scratch"].data_ptr(), space["prefill_scratch"].numel(), space["prefill_counters"].data_ptr(),
+                space["prefill_counters"].numel(), _raw_stream()), "quantized_attention (prompts)")
+            first, rest = rest - decodes, decodes
+        if cores and 0 < decodes <= self.QUANTIZED_DECODES:
+            longest = int(batch.max_kv_len)
+            scratch = torch.empty(_quantized_decode_bytes(decodes, num_kv_heads, group, head_dim, window, longest, q.device.index), dtype=torch.uint8,
+                                  device=q.device)
+            _check(_declared_library("attention_quantized_decode").mlr_attention_quantized_decode(
+                q.data_ptr(), *pool.addresses, out.data_ptr(), None if decodes == batch.num_segments else plan["decode_seg"].data_ptr(), q_start, pos0,
+                table, slot, width, decodes, *sizes, longest, scratch.data_ptr(), self._error_word(q.device).data_ptr(), _raw_stream()),
+                "quantized_attention (decoded tokens)")
+            rest -= decodes
         if rest > 0:
             _check(_declared_library("attention_quantized").mlr_attention_quantized(
-                q.data_ptr(), *pools, out.data_ptr(), plan["tile_seg"].data_ptr() + 4 * first, plan["tile_row0"].data_ptr() + 4 * first, *segments,
-                rest, *sizes, _code(q.dtype), _raw_stream()), "quantized_attention")
+                q.data_ptr(), *pool.addresses, out.data_ptr(), plan["tile_seg"].data_ptr() + 4 * first, plan["tile_row0"].data_ptr() + 4 * first, q_start,
+                batch.seg_q_len.data_ptr(), pos0, table, slot, width, rest, *sizes, _code(q.dtype), _raw_stream()), "quantized_attention")
         return out
 
     QUANTIZED_DECODES = 2048      # requests of one launch (attention_quantized_decode.cu)
-
-    def _quantized_on_tensor_cores(self, q: torch.Tensor, pool: QuantizedPool, num_heads: int) -> bool:
-        """bfloat16 queries over pages that whole groups of 16 keys lie on; everything else takes the general kernel."""
-        return (self.use_mma_attention and q.dtype == torch.bfloat16 and pool.dim in (64, 128) and num_heads // pool.kv_heads <= 16
-                and pool.page_size >= 16 and pool.page_size & (pool.page_size - 1) == 0 and pool.block & (pool.block - 1) == 0
-                and not (q.data_ptr() | pool.key.data_ptr() | pool.value.data_ptr()) % 16)
 
     # ------------------------------------------------------------------ pages of a cache
     COPY_POOLS = 8      # of one launch (copy_pages.cu)
