@@ -1250,8 +1250,8 @@ class CudaOps:
         if pages.shape[0] == 0:
             return key, value
         _check(_declared_library("quantized_pages").mlr_dequantize_pages(
-            *pool.addresses, pages.data_ptr(), key.data_ptr(), value.data_ptr(), pages.shape[0], pool.kv_heads, pool.dim, pool.page_size, pool.block, pool.pages, _code(out_dtype),
-            _raw_stream()), "dequantize_pages")
+            *pool.addresses, pages.data_ptr(), key.data_ptr(), value.data_ptr(), pages.shape[0], pool.kv_heads, pool.dim, pool.page_size,
+            pool.block, pool.pages, _code(out_dtype), _raw_stream()), "dequantize_pages")
         return key, value
 
     def quantized_attention(self, q: torch.Tensor, pool: QuantizedPool, batch: AttentionBatch, num_heads: int, num_kv_heads: int, head_dim: int,
@@ -1323,44 +1323,57 @@ class CudaOps:
         target twice."""
         pools = list(pools)
         targets = pools if into is None else list(into)
-        source, target = (np.ascontiguousarray(list(pages), dtype=np.int64) for pages in (source, target))
-        if source.ndim != 1 or source.shape != target.shape:
+        try:
+            numbers = np.array([source, target], dtype=np.int64)      # (unlike lengths raise)
+        except ValueError:
+            numbers = np.empty(0)
+        if numbers.ndim != 2:
             raise KernelError("source and target need one page number each")
+        count = numbers.shape[1]
         if len(targets) != len(pools):
             raise KernelError(f"{len(pools)} pools cannot be copied into {len(targets)}")
-        for what, side, numbers in (("source", pools, source), ("target", targets, target)):
+        device = torch._C._cuda_getDevice()
+        for what, side in (("source", pools), ("target", targets)):
+            if side is pools and what == "target":
+                break                                  # checked as sources
             for pool in side:
                 _need(pool, f"a {what} pool")
-                _need_here(**{f"a {what} pool": pool})
+                if pool.device.index != device:
+                    _need_here(pool=pool)
                 if pool.dim() < 2 or pool.shape[1] != side[0].shape[1]:
                     raise KernelError(f"the {what} pools must have one number of pages")
-            if side and len(numbers) and (numbers.min() < 0 or numbers.max() >= side[0].shape[1]):
+        if not pools or not count:
+            return
+        ends, begins = numbers.max(axis=1), numbers.min(axis=1)
+        for i, (what, side) in enumerate((("source", pools), ("target", targets))):
+            if begins[i] < 0 or ends[i] >= side[0].shape[1]:
                 raise KernelError(f"{what} pages must lie in [0, {side[0].shape[1]})")
-        if len(np.unique(target)) != len(target):
-            raise KernelError("a page is the target of one copy")
-        if into is None:
-            if np.isin(target, source).any():
+        if count > 1 or into is None:
+            taken = np.zeros(int(max(ends)) + 1, dtype=bool)
+            taken[numbers[1]] = True
+            if np.count_nonzero(taken) != count:
+                raise KernelError("a page is the target of one copy")
+            if into is None and taken[numbers[0]].any():
                 raise KernelError("a page cannot be source and target")
-        else:
+        if into is not None:
             for pool, other in zip(pools, targets):
                 if other.dtype != pool.dtype or other.shape[0] != pool.shape[0] or other.shape[2:] != pool.shape[2:]:
                     raise KernelError(f"pages of {tuple(pool.shape)} {pool.dtype} do not fit {tuple(other.shape)} {other.dtype}")
             spans = [[(pool.data_ptr(), pool.data_ptr() + pool.numel() * pool.element_size()) for pool in group] for group in (pools, targets)]
             if any(first < end and begin < last for begin, end in spans[0] for first, last in spans[1]):
                 raise KernelError("the pools that pages go to must not be those that they come from")
-        count = len(source)
         fields = []
         for pool, other in zip(pools, targets):
-            page = pool[0, 0].numel() * pool.element_size() if pool.numel() else 0
+            entries, pages = pool.shape[:2]
+            page = pool.numel() // (entries * pages) * pool.element_size() if entries else 0
             if page:
-                fields.append((pool.data_ptr(), other.data_ptr(), pool.shape[1] * page, other.shape[1] * page, page, pool.shape[0]))
-        if not fields or not count:
-            return
-        source, target = source.astype(np.int32), target.astype(np.int32)
+                fields += (pool.data_ptr(), other.data_ptr(), pages * page, other.shape[1] * page, page, entries)
+        numbers = numbers.astype(np.int32)
+        at = numbers.ctypes.data
         entry = _declared_library("copy_pages").mlr_copy_pages
-        for first in range(0, len(fields), self.COPY_POOLS):
-            some = np.asarray(fields[first:first + self.COPY_POOLS], dtype=np.int64)
-            _check(entry(some.ctypes.data, len(some), source.ctypes.data, target.ctypes.data, count, _raw_stream()), "copy_pages")
+        for first in range(0, len(fields), 6 * self.COPY_POOLS):
+            some = fields[first:first + 6 * self.COPY_POOLS]
+            _check(entry((ctypes.c_longlong * len(some))(*some), len(some) // 6, at, at + 4 * count, count, _raw_stream()), "copy_pages")
 
     def plan_shared_prefix(self, groups, num_segments, heads_per_kv):
         return plan_shared_prefix(groups, num_segments, heads_per_kv)
