@@ -15,11 +15,12 @@
 // once.  Logits are compared as whole numbers of the same order (`order_key`).  While a slice arrives its keys are counted in
 // 4,096 bins (sign, exponent, three bits of mantissa), the CTAs add the bins up through distributed shared memory, and every
 // CTA finds from them the lowest bin that a cut can lie in: exactly for top-k, by bounds of the bins' weights for top-p.
-//   few candidates (<= LIST above that bin)   they go to the first CTA, in the order of the vocabulary, which cuts and draws alone
-//   many                                      the cuts are found together: an eightfold split of the interval of keys that holds
-//                                             the cut, weights summed for each part, until few enough keys are in it for one CTA;
-//                                             then every CTA sums its kept weights and the one that the draw falls into walks there
-// Sums are taken in a fixed order (no floating-point atomics): a row's token depends on its row alone.
+//   few candidates (<= SL_LIST above that bin)   they go to the first CTA, which sorts them, cuts, sorts what stays by index and draws
+//   many                                         the cuts are found together: an eightfold split of the interval of keys that holds
+//                                                the cut, weights summed for each part, until few enough keys are in it for one CTA to
+//                                                sort; then every CTA sums its kept weights and the one that the draw falls into
+//                                                walks there
+// Sums are taken in a fixed order, of sorted numbers or of places (no floating-point atomics): a row's token depends on its row alone.
 #include <cooperative_groups.h>
 
 #include "uniform.cuh"
@@ -31,9 +32,10 @@ namespace cg = cooperative_groups;
 constexpr int SL_THREADS = 512, SL_WARPS = SL_THREADS / 32;
 constexpr int SL_BINS = 4096, SL_BIN_SHIFT = 20, SL_BINS_PER_THREAD = SL_BINS / SL_THREADS;
 constexpr int SL_LIST = 2048;            // candidates that one CTA cuts and draws from
-constexpr int SL_CUT = 1024;             // keys of an interval that one CTA cuts
+constexpr int SL_CUT = 1024;             // keys of an interval that one CTA sorts
 constexpr int SL_PARTS = 8;
-constexpr int SL_MAX_CLUSTER = 16;
+constexpr int SL_MOST_RANKS = 8;
+static_assert(SL_BINS_PER_THREAD == 8, "a thread reads eight bins");
 
 struct LimitSource {
   const float* uniforms;          // by row
@@ -58,16 +60,18 @@ struct LimitShared {
   int cut_index;
   double kept;
   // of this CTA alone
-  double warp_double[SL_WARPS + 1];
-  float warp_float[SL_WARPS + 1], warp_float2[SL_WARPS + 1];
-  int warp_int[SL_WARPS + 1];
-  unsigned warp_key[SL_WARPS];
-  unsigned found_key[2];
+  double warp_double[SL_WARPS], part_double[SL_PARTS][SL_WARPS];
+  float warp_float[SL_WARPS], warp_float2[SL_WARPS];
+  int warp_int[SL_WARPS], part_int[SL_PARTS][SL_WARPS];
+  unsigned found_key;
   int found[4];
 };
 
-struct ListEntry { unsigned key; int index; };
-struct FullEntry { double weight; unsigned key; int index; };
+// A token in the order of the limits, as a whole number: falling logit, rising index.
+typedef unsigned long long Place;
+__device__ __forceinline__ Place place_of(unsigned key, int index) { return ((Place)~key << 32) | (unsigned)index; }
+__device__ __forceinline__ unsigned key_of(Place place) { return ~(unsigned)(place >> 32); }
+__device__ __forceinline__ int index_of(Place place) { return (int)(unsigned)place; }
 
 __device__ __forceinline__ unsigned order_key(float x) {      // larger for larger x
   const unsigned b = __float_as_uint(x);
@@ -149,78 +153,25 @@ __device__ __forceinline__ int ties_kept(double above, double w, double target, 
   return wanted < 1.0 ? 1 : wanted < (double)ties ? (int)wanted : ties;
 }
 
-// The cut of a list in the order of the vocabulary, by one CTA.  BY_WEIGHT: the shortest beginning whose weights, `above` before
-// them, come to `target`; else the first `target - above` (at least 1).  `kept` limits the list before.
-template <bool BY_WEIGHT>
-__device__ Cut cut_list(const FullEntry* list, int n, Cut kept, double above, double target, unsigned lo, unsigned hi, LimitShared* s) {
-  // the smallest key t with sum(key > t) < target
-  while (lo < hi) {
-    const unsigned step = (hi - lo) / SL_PARTS + 1;      // parts from the top: (hi - step, hi], ..
-    double part[SL_PARTS];
-#pragma unroll
-    for (int j = 0; j < SL_PARTS; ++j) part[j] = 0.0;
-    for (int i = threadIdx.x; i < n; i += SL_THREADS) {
-      const FullEntry e = list[i];
-      if (e.key >= lo && e.key <= hi && kept.keeps(e.key, e.index)) {
-        const unsigned at = (hi - e.key) / step;
-        const double w = BY_WEIGHT ? e.weight : 1.0;
-#pragma unroll
-        for (int j = 0; j < SL_PARTS; ++j) part[j] += at == (unsigned)j ? w : 0.0;
+// Rising order, by one CTA; the array has room up to the next power of two, which is filled with the largest number.  A bitonic
+// network: a warp's 32 pairs lie in 64 neighbouring numbers as long as the pairs are at most 32 apart, and wait for no other warp.
+__device__ void sort_places(Place* a, int n) {
+  int size = 64;
+  while (size < n) size *= 2;
+  for (int i = n + threadIdx.x; i < size; i += SL_THREADS) a[i] = ~(Place)0;
+  __syncthreads();
+  for (int run = 2; run <= size; run *= 2) {
+    for (int apart = run / 2; apart > 0; apart /= 2) {
+      for (int pair = threadIdx.x; pair < size / 2; pair += SL_THREADS) {
+        const int low = 2 * pair - (pair & (apart - 1)), high = low + apart;
+        const Place x = a[low], y = a[high];
+        if ((x > y) == ((low & run) == 0)) { a[low] = y; a[high] = x; }
       }
+      if (apart > 32) __syncthreads();
+      else __syncwarp();
     }
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < SL_PARTS; ++j) {
-      part[j] = warp_sum64(part[j]);
-    }
-    // [part][warp]
-    __shared__ double rooms[SL_PARTS][SL_WARPS];
-    if ((threadIdx.x & 31) == 0)
-#pragma unroll
-      for (int j = 0; j < SL_PARTS; ++j) rooms[j][threadIdx.x >> 5] = part[j];
-    __syncthreads();
-    int chosen = SL_PARTS - 1;
-    double before = above;
-    bool open = true;
-#pragma unroll
-    for (int j = 0; j < SL_PARTS; ++j) {
-      double sum = 0.0;
-#pragma unroll
-      for (int w = 0; w < SL_WARPS; ++w) sum += rooms[j][w];
-      if (open) {
-        const bool last = (unsigned)(j + 1) * (unsigned long long)step > (unsigned long long)(hi - lo);
-        if (before + sum >= target || last) { chosen = j; open = false; }
-        else before += sum;
-      }
-    }
-    above = before;
-    const unsigned long long top = (unsigned long long)hi - (unsigned long long)chosen * step;
-    const unsigned long long bottom = top >= (unsigned long long)lo + step - 1 ? top - (step - 1) : lo;
-    hi = (unsigned)top;
-    lo = (unsigned)bottom;
   }
-  // ties of the key in their order: the index of the last one that stays
-  int mine = 0, total;
-  const int each = (n + SL_THREADS - 1) / SL_THREADS, first = min(n, (int)threadIdx.x * each), last = min(n, first + each);
-  double weight = 0.0;
-  for (int i = first; i < last; ++i)
-    if (list[i].key == lo && kept.keeps(list[i].key, list[i].index)) { ++mine; weight = list[i].weight; }
-  const int before = before_block(mine, s->warp_int, &total);
-  if (mine > 0) s->warp_double[SL_WARPS] = weight;      // equal logits, equal weights
-  if (threadIdx.x == 0) s->found[0] = 0x7fffffff;
-  __syncthreads();
-  int stay;
-  if constexpr (BY_WEIGHT) stay = ties_kept(above, s->warp_double[SL_WARPS], target, total);
-  else stay = min(total, max(1, (int)(target - above)));
-  if (before < stay && stay <= before + mine) {
-    int place = before;
-    for (int i = first; i < last; ++i)
-      if (list[i].key == lo && kept.keeps(list[i].key, list[i].index) && ++place == stay) s->found[0] = list[i].index;
-  }
-  __syncthreads();
-  const Cut cut{lo, s->found[0]};
-  __syncthreads();
-  return cut;
 }
 
 template <bool RESIDENT>
@@ -232,14 +183,13 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
   const int row = blockIdx.x / ranks;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   extern __shared__ __align__(16) uint8_t limit_shared[];
-  float* held = reinterpret_cast<float*>(limit_shared);                          // the slice; the first CTA's candidates after it
-  FullEntry* full = reinterpret_cast<FullEntry*>(limit_shared);
-  ListEntry* list = reinterpret_cast<ListEntry*>(limit_shared + room_bytes);     // [SL_LIST]
-  unsigned* bins = reinterpret_cast<unsigned*>(list + SL_LIST);                  // [SL_BINS]; later an interval's keys [SL_CUT]
-  FullEntry* interval = reinterpret_cast<FullEntry*>(bins);
+  float* held = reinterpret_cast<float*>(limit_shared);                          // the slice
+  Place* list = reinterpret_cast<Place*>(limit_shared + room_bytes);             // [SL_LIST] this CTA's candidates
+  unsigned* bins = reinterpret_cast<unsigned*>(list + SL_LIST);                  // [SL_BINS]
+  Place* all_listed = reinterpret_cast<Place*>(bins);                            // later the candidates of all CTAs [SL_LIST]
   unsigned* segment = bins + SL_BINS;                                            // [SL_BINS / ranks]
   __shared__ LimitShared s;
-  static_assert(SL_CUT * sizeof(FullEntry) <= SL_BINS * sizeof(unsigned), "an interval lies where the bins were");
+  static_assert(SL_LIST * sizeof(Place) <= SL_BINS * sizeof(unsigned), "the candidates lie where the bins were");
 
   pdl_wait();
   // ---- the row's limits
@@ -348,10 +298,10 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
       unsigned key = min(max(order_key(cleaned(guess)), no_key + 1), top_key);
       for (int i = 0; i < 64 && key < top_key && weight(of_key(key)) < wanted; ++i) ++key;
       for (int i = 0; i < 64 && key > no_key + 1 && weight(of_key(key - 1)) >= wanted; ++i) --key;
-      s.found_key[0] = key;
+      s.found_key = key;
     }
     __syncthreads();
-    kept.key = s.found_key[0];
+    kept.key = s.found_key;
   }
 
   // ---- from the bins: the lowest key that can be kept, the interval that holds the cut
@@ -361,7 +311,9 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     const int per = SL_BINS / ranks;
     for (int b = threadIdx.x; b < per; b += SL_THREADS) {
       unsigned sum = 0u;
-      for (int c = 0; c < ranks; ++c) sum += cluster.map_shared_rank(bins, c)[rank * per + b];
+#pragma unroll
+      for (int c = 0; c < SL_MOST_RANKS; ++c)
+        if (c < ranks) sum += cluster.map_shared_rank(bins, c)[rank * per + b];
       segment[b] = sum;
     }
     cluster.sync();
@@ -373,12 +325,15 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
       const float x = fminf(of_key(key), top);
       return x >= top ? 1.f : x == x ? expf((x - top) / temperature) : 0.f;
     };
-#pragma unroll
-    for (int j = 0; j < SL_BINS_PER_THREAD; ++j) {
-      const int bin = first_bin - j;
-      count[j] = (int)cluster.map_shared_rank(segment, bin / per)[bin % per];
-      mine += count[j];
+    {
+      const int lowest_bin = first_bin - (SL_BINS_PER_THREAD - 1), owner = lowest_bin / per;
+      const uint4* theirs = reinterpret_cast<const uint4*>(cluster.map_shared_rank(segment, owner) + (lowest_bin - owner * per));
+      const uint4 low4 = theirs[0], high4 = theirs[1];
+      count[0] = (int)high4.w; count[1] = (int)high4.z; count[2] = (int)high4.y; count[3] = (int)high4.x;
+      count[4] = (int)low4.w; count[5] = (int)low4.z; count[6] = (int)low4.y; count[7] = (int)low4.x;
     }
+#pragma unroll
+    for (int j = 0; j < SL_BINS_PER_THREAD; ++j) mine += count[j];
     const int before = before_block(mine, s.warp_int, &total);
     if (threadIdx.x == 0) { s.found[0] = s.found[1] = 0; }
     __syncthreads();
@@ -445,96 +400,113 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
       visit(i, i >= 0 ? at(i) : -INFINITY);
     }
   };
-  // keys of [low, high] in `kept` to the list; all CTAs, counts known to fit
+  // tokens of [low, high] in `limit` to this CTA's list, in no order; counts known to fit
   auto collect = [&](unsigned low, unsigned high, Cut limit, int room) {
-    int mine = 0;
-    walk([&](int i, float x) {
-      const unsigned key = order_key(x);
-      mine += __popc(__ballot_sync(0xffffffffu, i >= 0 && key >= low && key <= high && limit.keeps(key, begin + i)));
-    });
+    if (threadIdx.x == 0) s.count = 0;
     __syncthreads();
-    if (lane == 0) s.warp_int[warp] = mine;
-    __syncthreads();
-    int place = 0, total = 0;
-    for (int w = 0; w < SL_WARPS; ++w) {
-      if (w == warp) place = total;
-      total += s.warp_int[w];
-    }
-    walk([&](int i, float x) {
-      const unsigned key = order_key(x);
-      const bool in = i >= 0 && key >= low && key <= high && limit.keeps(key, begin + i);
-      const unsigned mask = __ballot_sync(0xffffffffu, in);
-      const int to = place + __popc(mask & ((1u << lane) - 1u));
-      if (in && to < room) list[to] = ListEntry{key, begin + i};
-      place += __popc(mask);
-    });
-    if (threadIdx.x == 0) s.count = min(total, room);
-  };
-  // the lists of all CTAs, one behind the other, with their weights; the first CTA
-  auto gather = [&](FullEntry* to, int room) -> int {
-    int n = 0;
-    for (int c = 0; c < ranks; ++c) {
-      const ListEntry* theirs = cluster.map_shared_rank(list, c);
-      const int count = min(cluster.map_shared_rank(&s, c)->count, room - n);
-      for (int i = threadIdx.x; i < count; i += SL_THREADS) {
-        const ListEntry e = theirs[i];
-        to[n + i] = FullEntry{weight(of_key(e.key)), e.key, e.index};
+    for (int i = threadIdx.x; i < size; i += SL_THREADS) {
+      const unsigned key = order_key(at(i));
+      if (key >= low && key <= high && limit.keeps(key, begin + i)) {
+        const int to = atomicAdd(&s.count, 1);
+        if (to < room) list[to] = place_of(key, begin + i);
       }
-      n += count;
     }
+  };
+  // the lists of all CTAs, sorted; the first CTA, the others wait
+  auto gather = [&](int room) -> int {
+    int until[SL_MOST_RANKS], n = 0;
+#pragma unroll
+    for (int c = 0; c < SL_MOST_RANKS; ++c) until[c] = c < ranks ? cluster.map_shared_rank(&s, c)->count : 0;
+#pragma unroll
+    for (int c = 0; c < SL_MOST_RANKS; ++c) { n = min(n + until[c], room); until[c] = n; }
+    for (int i = threadIdx.x; i < n; i += SL_THREADS) {
+      int owner = 0, before = 0;
+#pragma unroll
+      for (int c = 0; c + 1 < SL_MOST_RANKS; ++c)
+        if (i >= until[c]) { owner = c + 1; before = until[c]; }
+      all_listed[i] = cluster.map_shared_rank(list, owner)[i - before];
+    }
+    __syncthreads();
     return n;
   };
 
   if (binned && candidates <= SL_LIST) {
     // ---- few candidates: the first CTA cuts and draws
     const unsigned lowest = max(lo, kept.key);
+    collect(lowest, 0xffffffffu, kept, SL_LIST);
+    double tail = 0.0;
     if (by_weight && !by_count) {
-      double tail = 0.0;
       for (int i = threadIdx.x; i < size; i += SL_THREADS) {
         const float x = at(i);
         const unsigned key = order_key(x);
         if (key < lowest && key >= kept.key) tail += weight(x);
       }
       tail = sum_block(tail, s.warp_double);
-      if (threadIdx.x == 0) s.tail = tail;
-    } else if (threadIdx.x == 0) {
-      s.tail = 0.0;
     }
-    collect(lowest, 0xffffffffu, kept, SL_LIST);
+    if (threadIdx.x == 0) s.tail = tail;
     cluster.sync();
     int n = 0;
-    double tail = 0.0;
     if (rank == 0) {
-      n = gather(full, SL_LIST);
+      n = gather(SL_LIST);
+      tail = 0.0;
       for (int c = 0; c < ranks; ++c) tail += cluster.map_shared_rank(&s, c)->tail;
     }
     cluster.sync();
     if (rank != 0) return;
-    if (by_count && n > k) kept.tighten(cut_list<false>(full, n, kept, 0.0, (double)k, lowest, top_key, &s));
+    sort_places(all_listed, n);
+    // thread t: SL_EACH neighbours
+    constexpr int SL_EACH = SL_LIST / SL_THREADS;
+    int stay = by_count ? min(n, k) : n;
+    const int each = (n + SL_THREADS - 1) / SL_THREADS, first = threadIdx.x * each;
+    double w[SL_EACH], all;
     if (by_weight) {
-      double sum = 0.0;
-      for (int i = threadIdx.x; i < n; i += SL_THREADS)
-        if (kept.keeps(full[i].key, full[i].index)) sum += full[i].weight;
-      sum = sum_block(sum, s.warp_double) + tail;
-      kept.tighten(cut_list<true>(full, n, kept, 0.0, (double)p * sum, lowest, top_key, &s));
+      double mine = 0.0;
+#pragma unroll
+      for (int i = 0; i < SL_EACH; ++i) {
+        w[i] = i < each && first + i < stay ? weight(of_key(key_of(all_listed[first + i]))) : 0.0;
+        mine += w[i];
+      }
+      double run = before_block(mine, s.warp_double, &all);
+      const double target = (double)p * (all + tail);
+      int passed = 0;          // tokens whose sums stay below the target
+#pragma unroll
+      for (int i = 0; i < SL_EACH; ++i) {
+        run += w[i];
+        passed += i < each && first + i < stay && run < target;
+      }
+      stay = min(stay, 1 + sum_block(passed, s.warp_int));
     }
-    const int each = (n + SL_THREADS - 1) / SL_THREADS, first = min(n, (int)threadIdx.x * each), last = min(n, first + each);
-    double mine = 0.0, all;
-    int last_kept = -1;
-    for (int i = first; i < last; ++i)
-      if (kept.keeps(full[i].key, full[i].index) && full[i].weight > 0.0) { mine += full[i].weight; last_kept = i; }
+    // what stays, in the order of the vocabulary: index, key
+    __syncthreads();
+    for (int i = threadIdx.x; i < stay; i += SL_THREADS) {
+      const Place place = all_listed[i];
+      all_listed[i] = ((Place)(unsigned)index_of(place) << 32) | key_of(place);
+    }
+    sort_places(all_listed, stay);
+    const int share = (stay + SL_THREADS - 1) / SL_THREADS, from_place = threadIdx.x * share;
+    double mine = 0.0;
+#pragma unroll
+    for (int i = 0; i < SL_EACH; ++i) {
+      w[i] = i < share && from_place + i < stay ? weight(of_key((unsigned)all_listed[from_place + i])) : 0.0;
+      mine += w[i];
+    }
     double run = before_block(mine, s.warp_double, &all);
     const double target = (double)u * all;
-    if (threadIdx.x == 0) { s.found[0] = 0x7fffffff; s.found[1] = -1; }
+    if (threadIdx.x == 0) { s.found[0] = 0x7fffffff; s.found[1] = 0; }
     __syncthreads();
-    for (int i = first; i < last; ++i)
-      if (kept.keeps(full[i].key, full[i].index) && full[i].weight > 0.0) {
-        run += full[i].weight;
-        if (run > target) { atomicMin(&s.found[0], i); break; }
+    int reached = 0x7fffffff, last_kept = -1;
+#pragma unroll
+    for (int i = 0; i < SL_EACH; ++i) {
+      run += w[i];
+      if (w[i] > 0.0) {
+        last_kept = from_place + i;
+        if (run > target && reached == 0x7fffffff) reached = from_place + i;
       }
+    }
+    if (reached != 0x7fffffff) atomicMin(&s.found[0], reached);
     if (last_kept >= 0) atomicMax(&s.found[1], last_kept);
     __syncthreads();
-    if (threadIdx.x == 0) finish(full[s.found[0] < n ? s.found[0] : max(0, s.found[1])].index);
+    if (threadIdx.x == 0) finish((int)(all_listed[s.found[0] < stay ? s.found[0] : s.found[1]] >> 32));
     return;
   }
 
@@ -544,9 +516,19 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
   auto exchange = [&](double (&sums)[SL_PARTS], int (&counts)[SL_PARTS]) {
 #pragma unroll
     for (int j = 0; j < SL_PARTS; ++j) {
-      const double sum = sum_block(sums[j], s.warp_double);
-      const int count = sum_block(counts[j], s.warp_int);
-      if (threadIdx.x == 0) { s.sums[turn][j] = sum; s.counts[turn][j] = count; }
+      sums[j] = warp_sum64(sums[j]);
+      counts[j] = (int)__reduce_add_sync(0xffffffffu, (unsigned)counts[j]);
+    }
+    if (lane == 0)
+#pragma unroll
+      for (int j = 0; j < SL_PARTS; ++j) { s.part_double[j][warp] = sums[j]; s.part_int[j][warp] = counts[j]; }
+    __syncthreads();
+    if (threadIdx.x < SL_PARTS) {
+      double sum = 0.0;
+      int count = 0;
+      for (int w = 0; w < SL_WARPS; ++w) { sum += s.part_double[threadIdx.x][w]; count += s.part_int[threadIdx.x][w]; }
+      s.sums[turn][threadIdx.x] = sum;
+      s.counts[turn][threadIdx.x] = count;
     }
     cluster.sync();
 #pragma unroll
@@ -599,11 +581,31 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
       collect(low, high, kept, SL_CUT);
       cluster.sync();
       if (rank == 0) {
-        const int n = gather(interval, SL_CUT);
-        __syncthreads();
-        const Cut cut = weighed ? cut_list<true>(interval, n, kept, above, target, low, high, &s)
-                                : cut_list<false>(interval, n, kept, above, target, low, high, &s);
-        if (threadIdx.x == 0) { s.cut_key = cut.key; s.cut_index = cut.index; }
+        const int n = gather(SL_CUT);
+        sort_places(all_listed, n);
+        constexpr int EACH = SL_CUT / SL_THREADS;
+        const int each = (n + SL_THREADS - 1) / SL_THREADS, first = threadIdx.x * each;
+        int stay = min(n, max(1, (int)(target - above)));
+        if (weighed) {
+          double w[EACH], mine = 0.0, all;
+#pragma unroll
+          for (int i = 0; i < EACH; ++i) {
+            w[i] = i < each && first + i < n ? weight(of_key(key_of(all_listed[first + i]))) : 0.0;
+            mine += w[i];
+          }
+          double run = above + before_block(mine, s.warp_double, &all);
+          int passed = 0;
+#pragma unroll
+          for (int i = 0; i < EACH; ++i) {
+            run += w[i];
+            passed += i < each && first + i < n && run < target;
+          }
+          stay = min(n, 1 + sum_block(passed, s.warp_int));
+        }
+        if (threadIdx.x == 0) {
+          s.cut_key = n > 0 ? key_of(all_listed[stay - 1]) : low;
+          s.cut_index = n > 0 ? index_of(all_listed[stay - 1]) : 0x7fffffff;
+        }
       }
       cluster.sync();
       const LimitShared* first = cluster.map_shared_rank(&s, 0);
@@ -751,22 +753,20 @@ MLR_EXPORT int mlr_sample_limited(const float* logits, const float* uniforms, co
   if (rows == 0) return MLR_OK;
   if (rows < 0 || vocab <= 0 || slots < 0) return MLR_BAD_SIZE;
   if (state == nullptr ? uniforms == nullptr || temperatures == nullptr : row_slot == nullptr) return MLR_BAD_SIZE;
-  if ((long long)rows * SL_MAX_CLUSTER > 0x7fffffffLL) return MLR_TOO_LARGE;
+  if ((long long)rows * SL_MOST_RANKS > 0x7fffffffLL) return MLR_TOO_LARGE;
   const LimitSource source{uniforms, temperatures, top_k, top_p, min_p, row_slot, (SlotState*)state, slots, advance};
   // CTAs per row: enough that a slice fits twice on an SM, more while the row's CTAs find an SM each
   constexpr int RESIDENT_MOST = 24 * 1024, LEAST = 2048;
   int ranks = 1;
-  while (ranks < 8 && (vocab > ranks * RESIDENT_MOST || (vocab > ranks * LEAST && rows * ranks * 2 <= sm_count()))) ranks *= 2;
+  while (ranks < SL_MOST_RANKS && (vocab > ranks * RESIDENT_MOST || (vocab > ranks * LEAST && rows * ranks * 2 <= sm_count()))) ranks *= 2;
   const int slice = ((vocab + ranks - 1) / ranks + 3) / 4 * 4;
   const bool resident = slice <= RESIDENT_MOST;
   const int most = RESIDENT_MOST * 4;
-  int room = resident ? slice * 4 : 0;
-  const int least_room = SL_LIST * (int)sizeof(FullEntry);
-  room = ((room > least_room ? room : least_room) + 15) / 16 * 16;
-  const size_t rest = SL_LIST * sizeof(ListEntry) + SL_BINS * sizeof(unsigned) + SL_BINS / ranks * sizeof(unsigned);
+  const int room = resident ? (slice * 4 + 15) / 16 * 16 : 0;
+  const size_t rest = SL_LIST * sizeof(Place) + SL_BINS * sizeof(unsigned) + SL_BINS / ranks * sizeof(unsigned);
   static OncePerDevice once;
   const cudaError_t err = once([&] {
-    const int bytes = most + (int)(SL_LIST * sizeof(ListEntry) + 2 * SL_BINS * sizeof(unsigned));
+    const int bytes = most + (int)(SL_LIST * sizeof(Place) + 2 * SL_BINS * sizeof(unsigned));
     cudaError_t e = cudaFuncSetAttribute(sample_limited_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     return e == cudaSuccess ? cudaFuncSetAttribute(sample_limited_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) : e;
   });
