@@ -12,14 +12,16 @@
 // two tokens by 1e-7 of the whole, as much as a token of a flat row is wide a hundred times over.
 //
 // A cluster of CTAs takes a row; each CTA keeps its slice of the row in shared memory, so that the logits are read from memory
-// once.  Logits are compared as whole numbers of the same order (`order_key`).  While a slice arrives its keys are counted in
-// 4,096 bins (sign, exponent, three bits of mantissa), the CTAs add the bins up through distributed shared memory, and every
-// CTA finds from them the lowest bin that a cut can lie in: exactly for top-k, by bounds of the bins' weights for top-p.
-//   few candidates (<= SL_LIST above that bin)   they go to the first CTA, which sorts them, cuts, sorts what stays by index and draws
-//   many                                         the cuts are found together: an eightfold split of the interval of keys that holds
-//                                                the cut, weights summed for each part, until few enough keys are in it for one CTA to
-//                                                sort; then every CTA sums its kept weights and the one that the draw falls into
-//                                                walks there
+// once.  Logits are compared as whole numbers of the same order (`order_key`).
+//   top-k, min-p   A lower bound of the k-th logit: each thread has met a largest one while it read, and at least k logits are as large
+//                  as the k-th of these.  Tokens above it (above min-p's border) are few: they go to the first CTA, which sorts them, cuts,
+//                  sorts what stays by index and draws.
+//   else           The cuts are found together.  All logits are counted in 4,096 bins of T / 128; the CTAs add the bins up through distributed
+//                  shared memory, and the bin that holds the cut is known for top-k, and for top-p but for a bin or two (a bin's weights
+//                  are within a hundredth of one another).  The weights above it are summed, the tokens around it go to the first CTA, which
+//                  sorts them and cuts.  If the cut is not there after all, or more tokens are than one CTA sorts (equal logits, say),
+//                  an interval of keys that surely holds it is split eightfold until it is found.  Then the draw: sums by CTA,
+//                  by warp, by part of a warp's stretch, and a walk.
 // Sums are taken in a fixed order, of sorted numbers or of places (no floating-point atomics): a row's token depends on its row alone.
 #include <cooperative_groups.h>
 
@@ -30,7 +32,9 @@ namespace mlr {
 namespace cg = cooperative_groups;
 
 constexpr int SL_THREADS = 512, SL_WARPS = SL_THREADS / 32;
-constexpr int SL_BINS = 4096, SL_BIN_SHIFT = 20, SL_BINS_PER_THREAD = SL_BINS / SL_THREADS;
+constexpr int SL_BINS = 4096, SL_BINS_PER_THREAD = SL_BINS / SL_THREADS;
+constexpr float SL_BINS_PER_T = 128.f;
+constexpr int SL_MOST_K = 1200;          // a top-k whose candidates surely fit a list (of 4,096 largest ones, the k-th bounds about 1.15 k)
 constexpr int SL_LIST = 2048;            // candidates that one CTA cuts and draws from
 constexpr int SL_CUT = 1024;             // keys of an interval that one CTA sorts
 constexpr int SL_PARTS = 8;
@@ -50,10 +54,9 @@ struct LimitSource {
 
 // What a CTA shows the others of its cluster.
 struct LimitShared {
-  float max;
+  float max, least_max;           // the largest logit, the smallest of the threads' largest ones
   int argmax;
   int count;                      // candidates in the list
-  double tail;                    // weights below the candidates
   double sums[2][SL_PARTS];       // of the parts of an interval, two steps by turns
   int counts[2][SL_PARTS];
   unsigned cut_key;               // what the first CTA found
@@ -64,7 +67,8 @@ struct LimitShared {
   float warp_float[SL_WARPS], warp_float2[SL_WARPS];
   int warp_int[SL_WARPS], part_int[SL_PARTS][SL_WARPS];
   unsigned found_key;
-  int found[4];
+  float bound, mark_mass[3];
+  int found[2], mark_bin[3], mark_tokens[3];
 };
 
 // A token in the order of the limits, as a whole number: falling logit, rising index.
@@ -81,14 +85,30 @@ __device__ __forceinline__ float of_key(unsigned key) { return __uint_as_float((
 // NaN as -inf, -0 as 0 (they tie)
 __device__ __forceinline__ float cleaned(float x) { return x == x ? x + 0.f : -INFINITY; }
 
+// exp((x - top) / T) in 64 bits by Tang's method (table-driven exponentials, 1989): a = (n + 64 m) ln 2 / 64 + r with |r| < ln 2 / 128,
+// exp a = 2^m 2^(n / 64) (1 + r + r^2 / 2 ..  r^5 / 120); the polynomial's remainder is below 2^-54.  `table` holds 2^(n / 64).
 struct Weights {
   double inverse, top;
   float max;
+  const double* table;
   __device__ __forceinline__ double operator()(float x) const {
     if (x == max) return 1.0;
-    if (x == -INFINITY) return 0.0;
-    const double w = exp(((double)x - top) * inverse);
-    return w > 0.0 ? w : 0.0;
+    if (!(x > -INFINITY)) return 0.0;
+    const double a = ((double)x - top) * inverse;
+    if (!(a > -700.0)) return 0.0;             // (a NaN too: an infinite temperature beside an infinite logit)
+    constexpr double RAISE = 6755399441055744.0;      // 1.5 * 2^52
+    const double raised = fma(a, 92.33248261689366, RAISE), whole = raised - RAISE;      // 64 / ln 2
+    const int n = __double2loint(raised);
+    // ln 2 / 64 in two parts, the first of 21 bits: its product with a whole number is exact
+    double r = fma(whole, -0x1.62e42p-7, a);
+    r = fma(whole, -0x1.fdf473de6af28p-28, r);
+    double q = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+    q = fma(r, q, 1.0 / 6.0);
+    q = fma(r, q, 0.5);
+    q = fma(r, q, 1.0);
+    const double t = table[n & 63];
+    const double value = fma(t, q * r, t);
+    return __hiloint2double(__double2hiint(value) + ((n >> 6) << 20), __double2loint(value));
   }
 };
 
@@ -186,11 +206,13 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
   float* held = reinterpret_cast<float*>(limit_shared);                          // the slice
   Place* list = reinterpret_cast<Place*>(limit_shared + room_bytes);             // [SL_LIST] this CTA's candidates
   unsigned* bins = reinterpret_cast<unsigned*>(list + SL_LIST);                  // [SL_BINS]
-  Place* all_listed = reinterpret_cast<Place*>(bins);                            // later the candidates of all CTAs [SL_LIST]
+  Place* all_listed = reinterpret_cast<Place*>(bins);                            // when the bins have been read, the candidates of all CTAs [SL_LIST]
   unsigned* segment = bins + SL_BINS;                                            // [SL_BINS / ranks]
   __shared__ LimitShared s;
+  __shared__ double table[64];
   static_assert(SL_LIST * sizeof(Place) <= SL_BINS * sizeof(unsigned), "the candidates lie where the bins were");
 
+  if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 64.0));
   pdl_wait();
   // ---- the row's limits
   const int slot = source.row_slot != nullptr ? source.row_slot[row] : row;
@@ -210,66 +232,69 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
   u = fmaxf(u, 0.f);
   if (p <= 0.f) { k = 1; p = 1.f; }
   const bool by_count = !greedy && k > 0 && k < vocab, by_weight = !greedy && p < 1.f;
-  const bool binned = by_count || by_weight;
 
-  // ---- the slice, its best token, its bins
+  // ---- the slice and its largest logit
   const int begin = min(vocab, rank * slice), size = min(vocab, begin + slice) - begin;
   const float* from = logits + (size_t)row * vocab + begin;
   auto at = [&](int i) -> float {
     if constexpr (RESIDENT) return held[i];
     else return cleaned(__ldcg(from + i));
   };
-  if (binned) {
-    for (int b = threadIdx.x; b < SL_BINS; b += SL_THREADS) bins[b] = 0u;
+  float mine = -INFINITY;      // the largest that this thread met
+  {
+    // 16 bytes at a time where slice and row begin on such boundaries together (a resident slice begins on one)
+    const bool wide = ((uintptr_t)from & 15) == 0;
+    const int pieces = wide ? size / 4 : 0;
+    constexpr int AHEAD = 5;
+    for (int i = threadIdx.x; i < pieces; i += AHEAD * SL_THREADS) {
+      float4 v[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (i + j * SL_THREADS < pieces) v[j] = __ldcg(reinterpret_cast<const float4*>(from) + i + j * SL_THREADS);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (i + j * SL_THREADS < pieces) {
+          const float4 x = make_float4(cleaned(v[j].x), cleaned(v[j].y), cleaned(v[j].z), cleaned(v[j].w));
+          if constexpr (RESIDENT) reinterpret_cast<float4*>(held)[i + j * SL_THREADS] = x;
+          mine = fmaxf(mine, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)));
+        }
+    }
+    for (int i = 4 * pieces + threadIdx.x; i < size; i += 4 * SL_THREADS) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j * SL_THREADS < size) v[j] = __ldcg(from + i + j * SL_THREADS);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j * SL_THREADS < size) {
+          const float x = cleaned(v[j]);
+          if constexpr (RESIDENT) held[i + j * SL_THREADS] = x;
+          mine = fmaxf(mine, x);
+        }
+    }
+  }
+  // the row's largest; of the threads' largest ones the smallest
+  {
+    const float high = warp_max(mine), low = -warp_max(mine > -INFINITY ? -mine : -INFINITY);
+    if (lane == 0) { s.warp_float[warp] = high; s.warp_float2[warp] = low; }
     __syncthreads();
-  }
-  float best = -INFINITY;
-  int best_index = vocab;
-  auto take = [&](int i, float x) {
-    if constexpr (RESIDENT) held[i] = x;
-    if (x > best) { best = x; best_index = begin + i; }
-    if (binned) atomicAdd(&bins[order_key(x) >> SL_BIN_SHIFT], 1u);
-  };
-  const int lead = min(size, (int)((16 - ((uintptr_t)from & 15)) & 15) / 4), pieces = (size - lead) / 4;
-  for (int i = threadIdx.x; i < lead; i += SL_THREADS) take(i, cleaned(__ldcg(from + i)));
-  const float4* wide = reinterpret_cast<const float4*>(from + lead);
-  for (int i = threadIdx.x; i < pieces; i += 4 * SL_THREADS) {
-    float4 v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i + j * SL_THREADS < pieces) v[j] = __ldcg(wide + i + j * SL_THREADS);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i + j * SL_THREADS < pieces) {
-        const int first = lead + 4 * (i + j * SL_THREADS);
-        take(first, cleaned(v[j].x));
-        take(first + 1, cleaned(v[j].y));
-        take(first + 2, cleaned(v[j].z));
-        take(first + 3, cleaned(v[j].w));
-      }
-  }
-  for (int i = lead + 4 * pieces + threadIdx.x; i < size; i += SL_THREADS) take(i, cleaned(__ldcg(from + i)));
-#pragma unroll
-  for (int offset = 16; offset > 0; offset >>= 1) {
-    const float other = __shfl_xor_sync(0xffffffffu, best, offset);
-    const int other_index = __shfl_xor_sync(0xffffffffu, best_index, offset);
-    if (other > best || (other == best && other_index < best_index)) { best = other; best_index = other_index; }
-  }
-  if (lane == 0) { s.warp_float[warp] = best; s.warp_int[warp] = best_index; }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < SL_WARPS; ++w)
-      if (s.warp_float[w] > best || (s.warp_float[w] == best && s.warp_int[w] < best_index)) { best = s.warp_float[w]; best_index = s.warp_int[w]; }
-    s.max = best;
-    s.argmax = best_index;
+    if (threadIdx.x == 0) {
+      float highest = s.warp_float[0], lowest = s.warp_float2[0];
+      for (int w = 1; w < SL_WARPS; ++w) { highest = fmaxf(highest, s.warp_float[w]); lowest = fminf(lowest, s.warp_float2[w]); }
+      s.max = highest;
+      s.least_max = lowest;
+      s.argmax = 0x7fffffff;
+    }
   }
   cluster.sync();
-  float top = -INFINITY;
-  int top_index = vocab;
-  for (int c = 0; c < ranks; ++c) {
-    const LimitShared* theirs = cluster.map_shared_rank(&s, c);
-    if (theirs->max > top) { top = theirs->max; top_index = theirs->argmax; }      // slices in order: the lowest index of a tie
-  }
+  float top = -INFINITY, least_max = INFINITY;
+#pragma unroll
+  for (int c = 0; c < SL_MOST_RANKS; ++c)
+    if (c < ranks) {
+      const LimitShared* theirs = cluster.map_shared_rank(&s, c);
+      top = fmaxf(top, theirs->max);
+      least_max = fminf(least_max, theirs->least_max);
+    }
   auto finish = [&](int token) {      // by one thread of the cluster
     tokens[row] = token;
     if (record != nullptr) {
@@ -279,14 +304,23 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     }
   };
   if (greedy || top == -INFINITY) {
-    if (rank == 0 && threadIdx.x == 0) finish(top_index < vocab ? top_index : 0);
-    cluster.sync();            // the others may still read this CTA's best
+    if (top > -INFINITY && s.max == top)      // its first place
+      for (int i = threadIdx.x; i < size; i += SL_THREADS)
+        if (at(i) == top) atomicMin(&s.argmax, begin + i);
+    cluster.sync();
+    if (rank == 0 && threadIdx.x == 0) {
+      int token = 0x7fffffff;
+      for (int c = 0; c < ranks; ++c) token = min(token, cluster.map_shared_rank(&s, c)->argmax);
+      finish(token < vocab ? token : 0);
+    }
+    cluster.sync();            // the first CTA has read the others'
     return;
   }
   Weights weight;
   weight.inverse = 1.0 / (double)temperature;
   weight.top = (double)top;
   weight.max = top;
+  weight.table = table;
   const unsigned top_key = order_key(top), no_key = order_key(-INFINITY);
 
   // ---- min-p: the lowest key whose weight reaches it
@@ -304,11 +338,15 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     kept.key = s.found_key;
   }
 
-  // ---- from the bins: the lowest key that can be kept, the interval that holds the cut
-  unsigned lo = 0u, hi = top_key;
-  int candidates = vocab, above_count = 0, interval_count = 0;
-  if (binned) {
-    const int per = SL_BINS / ranks;
+  // counts in bins: those of all CTAs, SL_BINS_PER_THREAD neighbours per thread
+  int count[SL_BINS_PER_THREAD];
+  const int per = SL_BINS / ranks, first_bin = (int)threadIdx.x * SL_BINS_PER_THREAD;
+  auto clear_bins = [&]() {
+    for (int b = threadIdx.x; b < SL_BINS; b += SL_THREADS) bins[b] = 0u;
+    __syncthreads();
+  };
+  auto add_up_bins = [&]() {
+    cluster.sync();
     for (int b = threadIdx.x; b < per; b += SL_THREADS) {
       unsigned sum = 0u;
 #pragma unroll
@@ -317,102 +355,32 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
       segment[b] = sum;
     }
     cluster.sync();
-    // thread t: SL_BINS_PER_THREAD bins from the top
-    int count[SL_BINS_PER_THREAD], mine = 0, total;
-    float low_sum = 0.f, high_sum = 0.f;
-    const int first_bin = SL_BINS - 1 - (int)threadIdx.x * SL_BINS_PER_THREAD;
-    auto edge_weight = [&](unsigned key) {
-      const float x = fminf(of_key(key), top);
-      return x >= top ? 1.f : x == x ? expf((x - top) / temperature) : 0.f;
-    };
-    {
-      const int lowest_bin = first_bin - (SL_BINS_PER_THREAD - 1), owner = lowest_bin / per;
-      const uint4* theirs = reinterpret_cast<const uint4*>(cluster.map_shared_rank(segment, owner) + (lowest_bin - owner * per));
-      const uint4 low4 = theirs[0], high4 = theirs[1];
-      count[0] = (int)high4.w; count[1] = (int)high4.z; count[2] = (int)high4.y; count[3] = (int)high4.x;
-      count[4] = (int)low4.w; count[5] = (int)low4.z; count[6] = (int)low4.y; count[7] = (int)low4.x;
-    }
-#pragma unroll
-    for (int j = 0; j < SL_BINS_PER_THREAD; ++j) mine += count[j];
-    const int before = before_block(mine, s.warp_int, &total);
-    if (threadIdx.x == 0) { s.found[0] = s.found[1] = 0; }
-    __syncthreads();
-    if (by_count) {
-      int run = before;
-#pragma unroll
-      for (int j = 0; j < SL_BINS_PER_THREAD; ++j) {
-        if (run < k && run + count[j] >= k) { s.found[0] = first_bin - j; s.found[2] = run; s.found[3] = run + count[j]; }
-        run += count[j];
-      }
-      __syncthreads();
-      lo = (unsigned)s.found[0] << SL_BIN_SHIFT;
-      hi = lo | ((1u << SL_BIN_SHIFT) - 1u);
-      above_count = s.found[2];
-      interval_count = s.found[3] - above_count;
-      candidates = s.found[3];
-    } else {
-      // bounds of the weights above each bin; a margin of 1e-3 covers the roundings
-      float low[SL_BINS_PER_THREAD], high[SL_BINS_PER_THREAD];
-#pragma unroll
-      for (int j = 0; j < SL_BINS_PER_THREAD; ++j) {
-        const unsigned edge = (unsigned)(first_bin - j) << SL_BIN_SHIFT, end = edge | ((1u << SL_BIN_SHIFT) - 1u);
-        // a bin that min-p cuts through holds none for sure
-        low[j] = count[j] == 0 || edge < kept.key ? 0.f : (float)count[j] * edge_weight(edge);
-        high[j] = count[j] == 0 || end < kept.key ? 0.f : (float)count[j] * edge_weight(end);
-        low_sum += low[j];
-        high_sum += high[j];
-      }
-      float low_all, high_all, low_end, high_end;
-      float low_run = before_block(low_sum, s.warp_float, &low_all, &low_end);
-      float high_run = before_block(high_sum, s.warp_float2, &high_all, &high_end);
-      low_all = fmaxf(low_all, 1.f);
-      const float surely = p * high_all * 1.001f, maybe = p * low_all * 0.999f;
-      if (threadIdx.x == 0) { s.found[0] = 0; s.found[1] = SL_BINS - 1; s.found[2] = total; }
-      __syncthreads();
-      if (low_run < surely && low_end >= surely) {      // one thread's
-        int run = before, place = 0;
-#pragma unroll
-        for (int j = 0; j < SL_BINS_PER_THREAD; ++j)
-          if (low_run < surely) { run += count[j]; low_run += low[j]; place = j; }
-        s.found[0] = first_bin - place;
-        s.found[2] = run;
-      }
-      if (high_run < maybe && high_end >= maybe) {
-        int place = 0;
-#pragma unroll
-        for (int j = 0; j < SL_BINS_PER_THREAD; ++j)
-          if (high_run < maybe) { high_run += high[j]; place = j; }
-        s.found[1] = first_bin - place;
-      }
-      __syncthreads();
-      lo = max((unsigned)s.found[0] << SL_BIN_SHIFT, kept.key);
-      hi = max(lo, ((unsigned)s.found[1] << SL_BIN_SHIFT) | ((1u << SL_BIN_SHIFT) - 1u));
-      candidates = s.found[2];
-    }
-  }
-
-  // a warp's stretch of the slice, in the order of the vocabulary
-  const int stretch = ((size + SL_WARPS - 1) / SL_WARPS + 31) / 32 * 32;
-  const int walk_begin = min(size, warp * stretch), walk_end = min(size, walk_begin + stretch);
-  auto walk = [&](auto&& visit) {      // every lane of the warp, `i` < 0 behind the end
-    for (int base = walk_begin; base < walk_end; base += 32) {
-      const int i = base + lane < walk_end ? base + lane : -1;
-      visit(i, i >= 0 ? at(i) : -INFINITY);
-    }
+    const int owner = first_bin / per;
+    const uint4* theirs = reinterpret_cast<const uint4*>(cluster.map_shared_rank(segment, owner) + (first_bin - owner * per));
+    const uint4 low4 = theirs[0], high4 = theirs[1];
+    count[0] = (int)low4.x; count[1] = (int)low4.y; count[2] = (int)low4.z; count[3] = (int)low4.w;
+    count[4] = (int)high4.x; count[5] = (int)high4.y; count[6] = (int)high4.z; count[7] = (int)high4.w;
   };
-  // tokens of [low, high] in `limit` to this CTA's list, in no order; counts known to fit
-  auto collect = [&](unsigned low, unsigned high, Cut limit, int room) {
+  // tokens of [low, high] in `limit` to this CTA's list, in no order
+  auto collect = [&](unsigned low, unsigned high, Cut limit) {
     if (threadIdx.x == 0) s.count = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < size; i += SL_THREADS) {
       const unsigned key = order_key(at(i));
       if (key >= low && key <= high && limit.keeps(key, begin + i)) {
         const int to = atomicAdd(&s.count, 1);
-        if (to < room) list[to] = place_of(key, begin + i);
+        if (to < SL_LIST) list[to] = place_of(key, begin + i);
       }
     }
   };
-  // the lists of all CTAs, sorted; the first CTA, the others wait
+  auto listed = [&]() {      // by all CTAs, after a barrier of the cluster
+    int n = 0;
+#pragma unroll
+    for (int c = 0; c < SL_MOST_RANKS; ++c)
+      if (c < ranks) n += cluster.map_shared_rank(&s, c)->count;
+    return n;
+  };
+  // the lists of all CTAs one behind the other; the first CTA, the others wait
   auto gather = [&](int room) -> int {
     int until[SL_MOST_RANKS], n = 0;
 #pragma unroll
@@ -429,88 +397,106 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     __syncthreads();
     return n;
   };
-
-  if (binned && candidates <= SL_LIST) {
-    // ---- few candidates: the first CTA cuts and draws
-    const unsigned lowest = max(lo, kept.key);
-    collect(lowest, 0xffffffffu, kept, SL_LIST);
-    double tail = 0.0;
-    if (by_weight && !by_count) {
-      for (int i = threadIdx.x; i < size; i += SL_THREADS) {
-        const float x = at(i);
-        const unsigned key = order_key(x);
-        if (key < lowest && key >= kept.key) tail += weight(x);
-      }
-      tail = sum_block(tail, s.warp_double);
-    }
-    if (threadIdx.x == 0) s.tail = tail;
-    cluster.sync();
-    int n = 0;
-    if (rank == 0) {
-      n = gather(SL_LIST);
-      tail = 0.0;
-      for (int c = 0; c < ranks; ++c) tail += cluster.map_shared_rank(&s, c)->tail;
-    }
-    cluster.sync();
-    if (rank != 0) return;
-    sort_places(all_listed, n);
-    // thread t: SL_EACH neighbours
-    constexpr int SL_EACH = SL_LIST / SL_THREADS;
-    int stay = by_count ? min(n, k) : n;
+  constexpr int SL_EACH = SL_LIST / SL_THREADS;
+  // of n sorted tokens the first whose weights, `above` before them, come to `target`
+  auto cut_sorted = [&](int n, double above, double target) -> int {
     const int each = (n + SL_THREADS - 1) / SL_THREADS, first = threadIdx.x * each;
-    double w[SL_EACH], all;
-    if (by_weight) {
-      double mine = 0.0;
-#pragma unroll
-      for (int i = 0; i < SL_EACH; ++i) {
-        w[i] = i < each && first + i < stay ? weight(of_key(key_of(all_listed[first + i]))) : 0.0;
-        mine += w[i];
-      }
-      double run = before_block(mine, s.warp_double, &all);
-      const double target = (double)p * (all + tail);
-      int passed = 0;          // tokens whose sums stay below the target
-#pragma unroll
-      for (int i = 0; i < SL_EACH; ++i) {
-        run += w[i];
-        passed += i < each && first + i < stay && run < target;
-      }
-      stay = min(stay, 1 + sum_block(passed, s.warp_int));
-    }
-    // what stays, in the order of the vocabulary: index, key
-    __syncthreads();
-    for (int i = threadIdx.x; i < stay; i += SL_THREADS) {
-      const Place place = all_listed[i];
-      all_listed[i] = ((Place)(unsigned)index_of(place) << 32) | key_of(place);
-    }
-    sort_places(all_listed, stay);
-    const int share = (stay + SL_THREADS - 1) / SL_THREADS, from_place = threadIdx.x * share;
-    double mine = 0.0;
+    double w[SL_EACH], sum = 0.0, all;
 #pragma unroll
     for (int i = 0; i < SL_EACH; ++i) {
-      w[i] = i < share && from_place + i < stay ? weight(of_key((unsigned)all_listed[from_place + i])) : 0.0;
-      mine += w[i];
+      w[i] = i < each && first + i < n ? weight(of_key(key_of(all_listed[first + i]))) : 0.0;
+      sum += w[i];
     }
-    double run = before_block(mine, s.warp_double, &all);
-    const double target = (double)u * all;
-    if (threadIdx.x == 0) { s.found[0] = 0x7fffffff; s.found[1] = 0; }
-    __syncthreads();
-    int reached = 0x7fffffff, last_kept = -1;
+    double run = above + before_block(sum, s.warp_double, &all);
+    int passed = 0;          // tokens whose sums stay below the target
 #pragma unroll
     for (int i = 0; i < SL_EACH; ++i) {
       run += w[i];
-      if (w[i] > 0.0) {
-        last_kept = from_place + i;
-        if (run > target && reached == 0x7fffffff) reached = from_place + i;
-      }
+      passed += i < each && first + i < n && run < target;
     }
-    if (reached != 0x7fffffff) atomicMin(&s.found[0], reached);
-    if (last_kept >= 0) atomicMax(&s.found[1], last_kept);
-    __syncthreads();
-    if (threadIdx.x == 0) finish((int)(all_listed[s.found[0] < stay ? s.found[0] : s.found[1]] >> 32));
-    return;
+    return min(n, 1 + sum_block(passed, s.warp_int));
+  };
+
+  if ((by_count && k <= SL_MOST_K) || kept.key != 0u || vocab <= SL_LIST) {
+    // ---- few candidates, it is likely
+    float bound = -INFINITY;
+    if (by_count && k <= SL_MOST_K && k <= ranks * SL_THREADS && vocab > SL_LIST) {
+      const float scale = top > least_max && top < INFINITY ? (float)(SL_BINS - 1) / (top - least_max) : 0.f;
+      clear_bins();
+      if (threadIdx.x == 0) s.bound = -INFINITY;
+      if (mine > -INFINITY) atomicAdd(&bins[scale > 0.f ? min(SL_BINS - 1, (int)((top - mine) * scale)) : 0], 1u);
+      add_up_bins();
+      int here = 0, total, until;
+#pragma unroll
+      for (int j = 0; j < SL_BINS_PER_THREAD; ++j) here += count[j];
+      const int before = before_block(here, s.warp_int, &total, &until);
+      if (before < k && until >= k) {      // one thread's (none's where fewer threads met a number)
+        int run = before, bin = first_bin;
+#pragma unroll
+        for (int j = 0; j < SL_BINS_PER_THREAD; ++j)
+          if (run < k) { run += count[j]; bin = first_bin + j; }
+        // (a hundredth of a bin is more than the roundings)
+        s.bound = scale > 0.f ? top - ((float)bin + 1.01f) / scale : least_max;
+      }
+      __syncthreads();
+      bound = s.bound;
+    }
+    const unsigned lowest = max(order_key(bound), kept.key);
+    collect(lowest, 0xffffffffu, kept);
+    cluster.sync();
+    const int found = listed();
+    if (found <= SL_LIST) {
+      int n = 0;
+      if (rank == 0) n = gather(SL_LIST);
+      cluster.sync();
+      if (rank != 0) return;
+      sort_places(all_listed, n);
+      int stay = by_count ? min(n, k) : n;
+      if (by_weight) {
+        double part = 0.0;
+        for (int i = threadIdx.x; i < stay; i += SL_THREADS) part += weight(of_key(key_of(all_listed[i])));
+        stay = cut_sorted(stay, 0.0, (double)p * sum_block(part, s.warp_double));
+      }
+      // what stays, in the order of the vocabulary: index, key
+      __syncthreads();
+      for (int i = threadIdx.x; i < stay; i += SL_THREADS) {
+        const Place place = all_listed[i];
+        all_listed[i] = ((Place)(unsigned)index_of(place) << 32) | key_of(place);
+      }
+      sort_places(all_listed, stay);
+      const int each = (stay + SL_THREADS - 1) / SL_THREADS, first = threadIdx.x * each;
+      double w[SL_EACH], sum = 0.0, all;
+#pragma unroll
+      for (int i = 0; i < SL_EACH; ++i) {
+        w[i] = i < each && first + i < stay ? weight(of_key((unsigned)all_listed[first + i])) : 0.0;
+        sum += w[i];
+      }
+      double run = before_block(sum, s.warp_double, &all);
+      const double target = (double)u * all;
+      if (threadIdx.x == 0) { s.found[0] = 0x7fffffff; s.found[1] = 0; }
+      __syncthreads();
+      int reached = 0x7fffffff, last_kept = -1;
+#pragma unroll
+      for (int i = 0; i < SL_EACH; ++i) {
+        run += w[i];
+        if (w[i] > 0.0) {
+          last_kept = first + i;
+          if (run > target && reached == 0x7fffffff) reached = first + i;
+        }
+      }
+      if (reached != 0x7fffffff) atomicMin(&s.found[0], reached);
+      if (last_kept >= 0) atomicMax(&s.found[1], last_kept);
+      __syncthreads();
+      if (threadIdx.x == 0) finish((int)(all_listed[s.found[0] < stay ? s.found[0] : s.found[1]] >> 32));
+      return;
+    }
+    cluster.sync();            // the counts have been read
   }
 
-  // ---- many candidates: the cuts are found together
+  // ---- the cuts are found together
+  // a warp's stretch of the slice
+  const int stretch = ((size + SL_WARPS - 1) / SL_WARPS + 31) / 32 * 32;
+  const int walk_begin = min(size, warp * stretch), walk_end = min(size, walk_begin + stretch);
   int turn = 0;
   // sums and counts of the parts of all CTAs
   auto exchange = [&](double (&sums)[SL_PARTS], int (&counts)[SL_PARTS]) {
@@ -525,10 +511,10 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     __syncthreads();
     if (threadIdx.x < SL_PARTS) {
       double sum = 0.0;
-      int count = 0;
-      for (int w = 0; w < SL_WARPS; ++w) { sum += s.part_double[threadIdx.x][w]; count += s.part_int[threadIdx.x][w]; }
+      int all = 0;
+      for (int w = 0; w < SL_WARPS; ++w) { sum += s.part_double[threadIdx.x][w]; all += s.part_int[threadIdx.x][w]; }
       s.sums[turn][threadIdx.x] = sum;
-      s.counts[turn][threadIdx.x] = count;
+      s.counts[turn][threadIdx.x] = all;
     }
     cluster.sync();
 #pragma unroll
@@ -543,9 +529,10 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     }
     turn ^= 1;
   };
-  // the cut in [low, high], which holds `count` kept keys; `above` before them
-  auto cut_together = [&](bool weighed, unsigned low, unsigned high, double above, double target, int count) -> Cut {
-    while (count > SL_CUT && low < high) {
+  // The cut in [low, high], which holds `inside` kept keys, `above` before them; `ready`: they are in the lists already.
+  auto cut_together = [&](bool weighed, unsigned low, unsigned high, double above, double target, int inside, bool ready) -> Cut {
+    while (inside > SL_CUT && low < high) {
+      ready = false;
       const unsigned step = (high - low) / SL_PARTS + 1;
       double sums[SL_PARTS];
       int counts[SL_PARTS];
@@ -569,7 +556,7 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
       for (int j = 0; j < SL_PARTS; ++j) {
         if (open) {
           const bool last = (unsigned long long)(j + 1) * step > (unsigned long long)(high - low);
-          if (above + sums[j] >= target || last) { chosen = j; count = counts[j]; open = false; }
+          if (above + sums[j] >= target || last) { chosen = j; inside = counts[j]; open = false; }
           else above += sums[j];
         }
       }
@@ -577,31 +564,15 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
       low = end >= (unsigned long long)low + step - 1 ? (unsigned)(end - (step - 1)) : low;
       high = (unsigned)end;
     }
-    if (count <= SL_CUT) {
-      collect(low, high, kept, SL_CUT);
-      cluster.sync();
+    if (inside <= SL_CUT) {
+      if (!ready) {
+        collect(low, high, kept);
+        cluster.sync();
+      }
       if (rank == 0) {
         const int n = gather(SL_CUT);
         sort_places(all_listed, n);
-        constexpr int EACH = SL_CUT / SL_THREADS;
-        const int each = (n + SL_THREADS - 1) / SL_THREADS, first = threadIdx.x * each;
-        int stay = min(n, max(1, (int)(target - above)));
-        if (weighed) {
-          double w[EACH], mine = 0.0, all;
-#pragma unroll
-          for (int i = 0; i < EACH; ++i) {
-            w[i] = i < each && first + i < n ? weight(of_key(key_of(all_listed[first + i]))) : 0.0;
-            mine += w[i];
-          }
-          double run = above + before_block(mine, s.warp_double, &all);
-          int passed = 0;
-#pragma unroll
-          for (int i = 0; i < EACH; ++i) {
-            run += w[i];
-            passed += i < each && first + i < n && run < target;
-          }
-          stay = min(n, 1 + sum_block(passed, s.warp_int));
-        }
+        const int stay = weighed ? cut_sorted(n, above, target) : min(n, max(1, (int)(target - above)));
         if (threadIdx.x == 0) {
           s.cut_key = n > 0 ? key_of(all_listed[stay - 1]) : low;
           s.cut_index = n > 0 ? index_of(all_listed[stay - 1]) : 0x7fffffff;
@@ -613,12 +584,15 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
       cluster.sync();
       return cut;
     }
-    // more equal keys than an interval holds: the index of the last one that stays, by counting
-    const int stay = weighed ? ties_kept(above, weight(of_key(low)), target, count) : min(count, max(1, (int)(target - above)));
-    int mine = 0;
-    walk([&](int i, float x) { mine += __popc(__ballot_sync(0xffffffffu, i >= 0 && order_key(x) == low && kept.keeps(low, begin + i))); });
+    // more equal keys than a CTA sorts: the index of the last one that stays, by counting
+    const int stay = weighed ? ties_kept(above, weight(of_key(low)), target, inside) : min(inside, max(1, (int)(target - above)));
+    int here = 0;
+    for (int base = walk_begin; base < walk_end; base += 32) {
+      const int i = base + lane;
+      here += __popc(__ballot_sync(0xffffffffu, i < walk_end && order_key(at(i)) == low && kept.keeps(low, begin + i)));
+    }
     __syncthreads();
-    if (lane == 0) s.warp_int[warp] = mine;
+    if (lane == 0) s.warp_int[warp] = here;
     __syncthreads();
     if (threadIdx.x == 0) {
       int all = 0;
@@ -630,13 +604,14 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     int place = 0;
     for (int c = 0; c < rank; ++c) place += cluster.map_shared_rank(&s, c)->count;
     for (int w = 0; w < warp; ++w) place += s.warp_int[w];
-    if (place < stay && stay <= place + mine)
-      walk([&](int i, float x) {
-        const bool in = i >= 0 && order_key(x) == low && kept.keeps(low, begin + i);
+    if (place < stay && stay <= place + here)
+      for (int base = walk_begin; base < walk_end; base += 32) {
+        const int i = base + lane;
+        const bool in = i < walk_end && order_key(at(i)) == low && kept.keeps(low, begin + i);
         const unsigned mask = __ballot_sync(0xffffffffu, in);
         if (in && place + __popc(mask & ((2u << lane) - 1u)) == stay) s.cut_index = begin + i;
         place += __popc(mask);
-      });
+      }
     cluster.sync();
     Cut cut{low, 0x7fffffff};
     for (int c = 0; c < ranks; ++c) {
@@ -647,42 +622,141 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     return cut;
   };
 
-  if (by_count) {
-    // every key of the interval, min-p or not: the smaller of the two beginnings stays
-    const Cut before = kept;
-    kept = Cut{0u, 0x7fffffff};
-    Cut cut = cut_together(false, lo, hi, (double)above_count, (double)k, interval_count);
-    kept = before;
-    kept.tighten(cut);
-    lo = kept.key;
-    hi = top_key;
+  // ---- bins of T / 128 below the largest logit; the last holds all the rest
+  const float bin_scale = SL_BINS_PER_T / temperature;
+  if (by_count || by_weight) {
+    clear_bins();
+    for (int i = threadIdx.x; i < size; i += SL_THREADS)
+      atomicAdd(&bins[(int)fminf((top - at(i)) * bin_scale, (float)(SL_BINS - 1))], 1u);      // (infinity times zero: bin 0)
+    add_up_bins();
   }
-  if (by_weight) {
-    double sums[SL_PARTS];
-    int counts[SL_PARTS];
+  // keys that surely lie below a bin's beginning (all above: the first bin's)
+  auto key_below = [&](float bin) { return bin >= (float)(SL_BINS - 1) ? 0u : order_key(cleaned(top - bin / bin_scale)); };
+  double certain = 0.0;            // of this warp's stretch: weights that stay whatever the cut of the weights
+  unsigned open_low = 0u, open_high = top_key;      // keys that it lies among
+  bool summed = false;
+  if (by_count) {
+    int here = 0, total, until;
 #pragma unroll
-    for (int j = 0; j < SL_PARTS; ++j) { sums[j] = 0.0; counts[j] = 0; }
+    for (int j = 0; j < SL_BINS_PER_THREAD; ++j) here += count[j];
+    const int before = before_block(here, s.warp_int, &total, &until);
+    if (before < k && until >= k) {
+      int run = before, bin = first_bin;
+#pragma unroll
+      for (int j = 0; j < SL_BINS_PER_THREAD; ++j)
+        if (run < k) { run += count[j]; bin = first_bin + j; }
+      s.found[0] = bin;
+    }
+    __syncthreads();
+    const int bin = s.found[0];
+    const unsigned low = key_below((float)bin + 1.01f), high = bin == 0 ? top_key : key_below((float)bin - 0.01f);
+    // every key counts, min-p or not: the smaller of the two beginnings stays
+    const Cut before_k = kept;
+    kept = Cut{0u, 0x7fffffff};
+    double sums[SL_PARTS] = {};
+    int counts[SL_PARTS] = {};
+    collect(low, high, kept);
     for (int i = threadIdx.x; i < size; i += SL_THREADS) {
-      const float x = at(i);
-      const unsigned key = order_key(x);
-      if (kept.keeps(key, begin + i)) {
-        const double w = weight(x);
-        sums[0] += w;
-        if (key > hi) sums[1] += w;
-        else if (key >= lo) counts[0] += 1;
-      }
+      const unsigned key = order_key(at(i));
+      counts[0] += key > high;
+      counts[1] += key >= low && key <= high;
     }
     exchange(sums, counts);
-    kept.tighten(cut_together(true, lo, hi, sums[1], (double)p * sums[0], counts[0]));
+    const bool holds = counts[0] < k && counts[0] + counts[1] >= k;
+    const Cut cut = holds ? cut_together(false, low, high, (double)counts[0], (double)k, counts[1], true)
+                          : cut_together(false, 0u, top_key, 0.0, (double)k, vocab, false);
+    kept = before_k;
+    kept.tighten(cut);
+  }
+  if (by_weight) {
+    // Weights taken in the middle of their bins: the bins where they come to p of theirs, and to a little less and more.  What the
+    // estimate is off (single large tokens) shows in the exact sums above an interval; with that known the next one is found.
+    float mass[SL_BINS_PER_THREAD], here = 0.f, all, until;
+    int tokens_here = 0, tokens_all, tokens_until;
+    const int last_bin = kept.key > 0u ? (int)fminf((top - of_key(max(kept.key, no_key))) * bin_scale, (float)(SL_BINS - 1)) : SL_BINS - 1;
+#pragma unroll
+    for (int j = 0; j < SL_BINS_PER_THREAD; ++j) {
+      mass[j] = count[j] > 0 && first_bin + j <= last_bin ? (float)count[j] * expf(-((float)(first_bin + j) + 0.5f) / SL_BINS_PER_T) : 0.f;
+      here += mass[j];
+      tokens_here += count[j];
+    }
+    const float before = before_block(here, s.warp_float, &all, &until);
+    const int tokens_before = before_block(tokens_here, s.warp_int, &tokens_all, &tokens_until);
+    float wanted = p * all;
+    Cut cut{0u, 0x7fffffff};
+    bool found = false;
+    double whole = 0.0;
+    for (int attempt = 0; attempt < 3 && !found; ++attempt) {
+      __syncthreads();
+      if (threadIdx.x < 3) { s.mark_bin[threadIdx.x] = last_bin; s.mark_mass[threadIdx.x] = all; s.mark_tokens[threadIdx.x] = tokens_all; }
+      __syncthreads();
+#pragma unroll
+      for (int m = 0; m < 3; ++m) {
+        const float mark = wanted + (float)(m - 1) * 0.003f * all;
+        if ((before < mark || threadIdx.x == 0) && until >= mark) {
+          float run = before, at_bin = before;
+          int bin = first_bin, run_tokens = tokens_before, at_tokens = tokens_before;
+#pragma unroll
+          for (int j = 0; j < SL_BINS_PER_THREAD; ++j)
+            if (run < mark || j == 0) {
+              at_bin = run;
+              at_tokens = run_tokens;
+              run += mass[j];
+              run_tokens += count[j];
+              bin = first_bin + j;
+            }
+          s.mark_bin[m] = bin;
+          s.mark_mass[m] = at_bin;           // what lies before the bin
+          s.mark_tokens[m] = m == 2 ? run_tokens : at_tokens;
+        }
+      }
+      __syncthreads();
+      float estimate;                        // of what lies above the interval
+      if (s.mark_tokens[2] - s.mark_tokens[0] <= SL_CUT) {
+        open_low = key_below((float)s.mark_bin[2] + 1.01f);
+        open_high = s.mark_bin[0] == 0 ? top_key : key_below((float)s.mark_bin[0] - 0.01f);
+        estimate = s.mark_mass[0];
+      } else {
+        open_low = key_below((float)s.mark_bin[1] + 1.25f);
+        open_high = s.mark_bin[1] == 0 ? top_key : key_below((float)s.mark_bin[1] - 0.25f);
+        estimate = s.mark_mass[1];
+      }
+      collect(open_low, open_high, kept);
+      double sums[SL_PARTS] = {};
+      int counts[SL_PARTS] = {};
+      certain = 0.0;
+      for (int i = walk_begin + lane; i < walk_end; i += 32) {
+        const float x = at(i);
+        const unsigned key = order_key(x);
+        if (kept.keeps(key, begin + i)) {
+          const double w = weight(x);
+          if (key > open_high) certain += w;
+          else if (key >= open_low) { sums[1] += w; counts[1] += 1; }
+          else sums[2] += w;
+        }
+      }
+      sums[0] = certain;
+      certain = warp_sum64(certain);
+      exchange(sums, counts);
+      whole = sums[0] + sums[1] + sums[2];
+      const double target = (double)p * whole;
+      found = sums[0] < target && (sums[0] + sums[1] >= target || open_low == 0u);
+      if (found) cut = cut_together(true, open_low, open_high, sums[0], target, counts[1], true);
+      wanted = (float)(target - sums[0]) + estimate;
+    }
+    summed = found;
+    if (!found) cut = cut_together(true, 0u, top_key, 0.0, (double)p * whole, vocab, false);
+    kept.tighten(cut);
   }
 
   // ---- the draw
   double sum = 0.0;
-  walk([&](int i, float x) {
+  for (int i = walk_begin + lane; i < walk_end; i += 32) {
+    const float x = at(i);
     const unsigned key = order_key(x);
-    if (i >= 0 && kept.keeps(key, begin + i)) sum += weight(x);
-  });
-  sum = warp_sum64(sum);
+    if (kept.keeps(key, begin + i) && (!summed || key <= open_high)) sum += weight(x);
+  }
+  sum = warp_sum64(sum) + (summed ? certain : 0.0);
   __syncthreads();
   if (lane == 0) s.warp_double[warp] = sum;
   __syncthreads();
@@ -701,23 +775,34 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     if (theirs > 0.0) last_rank = c;
   }
   const double target = (double)u * all;
-  const double my_end = run + s.kept;
-  // the CTA, then the warp, whose sums the draw falls into; what rounding leaves behind the last belongs to it
-  if (target >= run && s.kept > 0.0 && (target < my_end || rank == last_rank)) {
-    double begin_sum = run;
-    int last_warp = 0, chosen = -1;
-    for (int w = 0; w < SL_WARPS; ++w)
-      if (s.warp_double[w] > 0.0) last_warp = w;
-    double so_far = run;
-    for (int w = 0; w < SL_WARPS && chosen < 0; ++w) {
-      if (s.warp_double[w] > 0.0 && (target < so_far + s.warp_double[w] || w == last_warp)) { chosen = w; begin_sum = so_far; }
-      so_far += s.warp_double[w];
+  // the CTA, then the warp's stretch, then its part, whose sums the draw falls into; what rounding leaves behind the last belongs to it
+  if (target >= run && s.kept > 0.0 && (target < run + s.kept || rank == last_rank)) {
+    auto chosen_of = [&](double& so_far) {
+      int last = 0, chosen = -1;
+      for (int w = 0; w < SL_WARPS; ++w)
+        if (s.warp_double[w] > 0.0) last = w;
+      for (int w = 0; w < SL_WARPS && chosen < 0; ++w) {
+        if (s.warp_double[w] > 0.0 && (target < so_far + s.warp_double[w] || w == last)) chosen = w;
+        else so_far += s.warp_double[w];
+      }
+      return max(chosen, 0);
+    };
+    const int stretch_begin = min(size, chosen_of(run) * stretch), stretch_end = min(size, stretch_begin + stretch);
+    const int part = ((stretch + SL_WARPS - 1) / SL_WARPS + 31) / 32 * 32;
+    const int part_begin = min(stretch_end, stretch_begin + warp * part), part_end = min(stretch_end, part_begin + part);
+    double in_part = 0.0;
+    for (int i = part_begin + lane; i < part_end; i += 32) {
+      const float x = at(i);
+      if (kept.keeps(order_key(x), begin + i)) in_part += weight(x);
     }
-    if (warp == chosen) {
+    in_part = warp_sum64(in_part);
+    __syncthreads();
+    if (lane == 0) s.warp_double[warp] = in_part;
+    __syncthreads();
+    if (warp == chosen_of(run)) {
       int found = -1, last_kept = -1;
-      double running = begin_sum;
-      for (int base = walk_begin; base < walk_end && found < 0; base += 32) {
-        const int i = base + lane < walk_end ? base + lane : -1;
+      for (int base = part_begin; base < part_end && found < 0; base += 32) {
+        const int i = base + lane < part_end ? base + lane : -1;
         const float x = i >= 0 ? at(i) : -INFINITY;
         const double w = i >= 0 && kept.keeps(order_key(x), begin + i) ? weight(x) : 0.0;
         double inclusive = w;
@@ -727,10 +812,10 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
           if (lane >= offset) inclusive += up;
         }
         const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
-        const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && running + inclusive > target);
+        const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && run + inclusive > target);
         if (some != 0u) last_kept = base + 31 - __clz(some);
         if (hit != 0u) found = base + __ffs(hit) - 1;
-        running += __shfl_sync(0xffffffffu, inclusive, 31);
+        run += __shfl_sync(0xffffffffu, inclusive, 31);
       }
       if (lane == 0) finish(begin + (found >= 0 ? found : max(0, last_kept)));
     }
