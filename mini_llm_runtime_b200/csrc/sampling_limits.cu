@@ -13,7 +13,7 @@
 //
 // A cluster of CTAs takes a row; each CTA keeps its slice of the row in shared memory, so that the logits are read from memory
 // once.  Logits are compared as whole numbers of the same order (`order_key`).
-//   top-k, min-p   A lower bound of the k-th logit: each thread has met a largest one while it read, and at least k logits are as large
+//   top-k, min-p   A lower bound of the k-th logit: each thread has met a largest one while it read, and k logits of a slice are as large
 //                  as the k-th of these.  Tokens above it (above min-p's border) are few: they go to the first CTA, which sorts them, cuts,
 //                  sorts what stays by index and draws.
 //   else           The cuts are found together.  All logits are counted in 4,096 bins of T / 128; the CTAs add the bins up through distributed
@@ -33,8 +33,9 @@ namespace cg = cooperative_groups;
 
 constexpr int SL_THREADS = 512, SL_WARPS = SL_THREADS / 32;
 constexpr int SL_BINS = 4096, SL_BINS_PER_THREAD = SL_BINS / SL_THREADS;
+constexpr int SL_BOUND_BINS = 1024;
 constexpr float SL_BINS_PER_T = 128.f;
-constexpr int SL_MOST_K = 1200;          // a top-k whose candidates surely fit a list (of 4,096 largest ones, the k-th bounds about 1.15 k)
+constexpr int SL_MOST_K = 1200;          // a top-k whose candidates fit a list, it is likely
 constexpr int SL_LIST = 2048;            // candidates that one CTA cuts and draws from
 constexpr int SL_CUT = 1024;             // keys of an interval that one CTA sorts
 constexpr int SL_PARTS = 8;
@@ -54,7 +55,7 @@ struct LimitSource {
 
 // What a CTA shows the others of its cluster.
 struct LimitShared {
-  float max, least_max;           // the largest logit, the smallest of the threads' largest ones
+  float max, bounds[2];           // the slice's largest logit; lower bounds of its k-th and of its k / ranks-th one
   int argmax;
   int count;                      // candidates in the list
   double sums[2][SL_PARTS];       // of the parts of an interval, two steps by turns
@@ -67,7 +68,7 @@ struct LimitShared {
   float warp_float[SL_WARPS], warp_float2[SL_WARPS];
   int warp_int[SL_WARPS], part_int[SL_PARTS][SL_WARPS];
   unsigned found_key;
-  float bound, mark_mass[3];
+  float mark_mass[3];
   int found[2], mark_bin[3], mark_tokens[3];
 };
 
@@ -173,25 +174,66 @@ __device__ __forceinline__ int ties_kept(double above, double w, double target, 
   return wanted < 1.0 ? 1 : wanted < (double)ties ? (int)wanted : ties;
 }
 
-// Rising order, by one CTA; the array has room up to the next power of two, which is filled with the largest number.  A bitonic
-// network: a warp's 32 pairs lie in 64 neighbouring numbers as long as the pairs are at most 32 apart, and wait for no other warp.
-__device__ void sort_places(Place* a, int n) {
-  int size = 64;
-  while (size < n) size *= 2;
-  for (int i = n + threadIdx.x; i < size; i += SL_THREADS) a[i] = ~(Place)0;
-  __syncthreads();
-  for (int run = 2; run <= size; run *= 2) {
-    for (int apart = run / 2; apart > 0; apart /= 2) {
-      for (int pair = threadIdx.x; pair < size / 2; pair += SL_THREADS) {
-        const int low = 2 * pair - (pair & (apart - 1)), high = low + apart;
-        const Place x = a[low], y = a[high];
-        if ((x > y) == ((low & run) == 0)) { a[low] = y; a[high] = x; }
+// Rising order by a bitonic network, EACH neighbouring numbers per thread in registers: pairs of a thread, of a warp by shuffles, of
+// further ones through the array itself.  THREADS 32: one warp, which waits for no other.
+template <int EACH, int THREADS>
+__device__ __forceinline__ void sort_in_registers(Place* a, int n) {
+  constexpr int SIZE = EACH * THREADS;
+  const int thread = THREADS == 32 ? (int)(threadIdx.x & 31) : (int)threadIdx.x, first = thread * EACH;
+  Place v[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) v[i] = first + i < n ? a[first + i] : ~(Place)0;
+  auto exchange = [&](Place& low, Place& high, bool rising) {
+    if ((low > high) == rising) { const Place x = low; low = high; high = x; }
+  };
+  for (int run = 2; run <= SIZE; run *= 2) {
+    for (int apart = run / 2; apart >= EACH; apart /= 2) {
+      if (apart < EACH * 32) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          const Place other = __shfl_xor_sync(0xffffffffu, v[i], apart / EACH);
+          const bool smaller = (((first + i) & run) == 0) == (((first + i) & apart) == 0);
+          v[i] = (other < v[i]) == smaller ? other : v[i];
+        }
+      } else {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) a[first + i] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          const Place other = a[(first + i) ^ apart];
+          const bool smaller = (((first + i) & run) == 0) == (((first + i) & apart) == 0);
+          v[i] = (other < v[i]) == smaller ? other : v[i];
+        }
       }
-      if (apart > 32) __syncthreads();
-      else __syncwarp();
     }
-    __syncthreads();
+    if constexpr (EACH == 4) {
+      if (run >= 4) { exchange(v[0], v[2], (first & run) == 0); exchange(v[1], v[3], (first & run) == 0); }
+    }
+    if constexpr (EACH >= 2) {
+#pragma unroll
+      for (int i = 0; i < EACH; i += 2) exchange(v[i], v[i + 1], ((first + i) & run) == 0);
+    }
   }
+  if (THREADS == 32) __syncwarp();
+  else __syncthreads();
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) a[first + i] = v[i];
+}
+// The array has room up to the next size that is sorted; behind n lie the largest numbers.
+__device__ __noinline__ void sort_places(Place* a, int n) {
+  __syncthreads();
+  if (n <= 128) {
+    if (threadIdx.x < 32) sort_in_registers<4, 32>(a, n);
+  } else if (n <= SL_THREADS) {
+    sort_in_registers<1, SL_THREADS>(a, n);
+  } else if (n <= 2 * SL_THREADS) {
+    sort_in_registers<2, SL_THREADS>(a, n);
+  } else {
+    sort_in_registers<4, SL_THREADS>(a, n);
+  }
+  __syncthreads();
 }
 
 template <bool RESIDENT>
@@ -212,27 +254,7 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
   __shared__ double table[64];
   static_assert(SL_LIST * sizeof(Place) <= SL_BINS * sizeof(unsigned), "the candidates lie where the bins were");
 
-  if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 64.0));
   pdl_wait();
-  // ---- the row's limits
-  const int slot = source.row_slot != nullptr ? source.row_slot[row] : row;
-  const bool known = slot >= 0 && slot < source.slots;
-  SlotState* record = known && source.state != nullptr ? source.state + slot : nullptr;
-  float temperature = 0.f, u = 0.f, p = 1.f, least = 0.f;
-  int k = 0;
-  if (known) {
-    temperature = record != nullptr ? record->temperature : source.temperatures[slot];
-    if (record != nullptr) u = uniform_from_seed(((unsigned long long)record->seed_high << 32) | record->seed_low, (long long)record->counter);
-    else u = source.uniforms[row];
-    if (source.top_k != nullptr) k = source.top_k[slot];
-    if (source.top_p != nullptr) p = source.top_p[slot];
-    if (source.min_p != nullptr) least = source.min_p[slot] > 0.f ? fminf(source.min_p[slot], 1.f) : 0.f;      // NaN: none
-  }
-  const bool greedy = !(temperature > 0.f);
-  u = fmaxf(u, 0.f);
-  if (p <= 0.f) { k = 1; p = 1.f; }
-  const bool by_count = !greedy && k > 0 && k < vocab, by_weight = !greedy && p < 1.f;
-
   // ---- the slice and its largest logit
   const int begin = min(vocab, rank * slice), size = min(vocab, begin + slice) - begin;
   const float* from = logits + (size_t)row * vocab + begin;
@@ -273,28 +295,76 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
         }
     }
   }
-  // the row's largest; of the threads' largest ones the smallest
+  if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 64.0));
+  // ---- the row's limits
+  const int slot = source.row_slot != nullptr ? source.row_slot[row] : row;
+  const bool known = slot >= 0 && slot < source.slots;
+  SlotState* record = known && source.state != nullptr ? source.state + slot : nullptr;
+  float temperature = 0.f, u = 0.f, p = 1.f, at_least = 0.f;
+  int k = 0;
+  if (known) {
+    temperature = record != nullptr ? record->temperature : source.temperatures[slot];
+    if (record != nullptr) u = uniform_from_seed(((unsigned long long)record->seed_high << 32) | record->seed_low, (long long)record->counter);
+    else u = source.uniforms[row];
+    if (source.top_k != nullptr) k = source.top_k[slot];
+    if (source.top_p != nullptr) p = source.top_p[slot];
+    if (source.min_p != nullptr) at_least = source.min_p[slot] > 0.f ? fminf(source.min_p[slot], 1.f) : 0.f;      // NaN: none
+  }
+  const bool greedy = !(temperature > 0.f);
+  u = fmaxf(u, 0.f);
+  if (p <= 0.f) { k = 1; p = 1.f; }
+  const bool by_count = !greedy && k > 0 && k < vocab, by_weight = !greedy && p < 1.f;
+
+  // ---- the slice's largest logit, and two of the threads' largest ones: the k-th, and the k / ranks-th.  All slices together hold k logits that
+  // are as large as the least of their k / ranks-th ones, and each holds k as large as its k-th.
   {
     const float high = warp_max(mine), low = -warp_max(mine > -INFINITY ? -mine : -INFINITY);
     if (lane == 0) { s.warp_float[warp] = high; s.warp_float2[warp] = low; }
+    const bool bounded = by_count && k <= SL_MOST_K && vocab > SL_LIST;
+    if (bounded) for (int b = threadIdx.x; b < SL_BOUND_BINS; b += SL_THREADS) bins[b] = 0u;
     __syncthreads();
+    float highest = s.warp_float[0], lowest = s.warp_float2[0];
+#pragma unroll
+    for (int w = 1; w < SL_WARPS; ++w) { highest = fmaxf(highest, s.warp_float[w]); lowest = fminf(lowest, s.warp_float2[w]); }
     if (threadIdx.x == 0) {
-      float highest = s.warp_float[0], lowest = s.warp_float2[0];
-      for (int w = 1; w < SL_WARPS; ++w) { highest = fmaxf(highest, s.warp_float[w]); lowest = fminf(lowest, s.warp_float2[w]); }
       s.max = highest;
-      s.least_max = lowest;
+      s.bounds[0] = s.bounds[1] = -INFINITY;
       s.argmax = 0x7fffffff;
+    }
+    if (bounded) {
+      const float scale = highest > lowest && highest < INFINITY ? (float)(SL_BOUND_BINS - 1) / (highest - lowest) : 0.f;
+      if (mine > -INFINITY) atomicAdd(&bins[scale > 0.f ? min(SL_BOUND_BINS - 1, (int)((highest - mine) * scale)) : 0], 1u);
+      __syncthreads();
+      constexpr int EACH = SL_BOUND_BINS / SL_THREADS;
+      int counts[EACH], here = 0, total, until;
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) { counts[j] = (int)bins[threadIdx.x * EACH + j]; here += counts[j]; }
+      const int before = before_block(here, s.warp_int, &total, &until);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const int place = m == 0 ? k : (k + ranks - 1) / ranks;
+        if (before < place && until >= place) {      // one thread's (none's where fewer threads met a number)
+          int run = before, bin = 0;
+#pragma unroll
+          for (int j = 0; j < EACH; ++j)
+            if (run < place) { run += counts[j]; bin = (int)threadIdx.x * EACH + j; }
+          // (a hundredth of a bin is more than the roundings)
+          s.bounds[m] = scale > 0.f ? highest - ((float)bin + 1.01f) / scale : lowest;
+        }
+      }
     }
   }
   cluster.sync();
-  float top = -INFINITY, least_max = INFINITY;
+  float top = -INFINITY, bound = -INFINITY, least = INFINITY;
 #pragma unroll
   for (int c = 0; c < SL_MOST_RANKS; ++c)
     if (c < ranks) {
       const LimitShared* theirs = cluster.map_shared_rank(&s, c);
       top = fmaxf(top, theirs->max);
-      least_max = fminf(least_max, theirs->least_max);
+      bound = fmaxf(bound, theirs->bounds[0]);
+      least = fminf(least, theirs->bounds[1]);
     }
+  bound = fmaxf(bound, least);
   auto finish = [&](int token) {      // by one thread of the cluster
     tokens[row] = token;
     if (record != nullptr) {
@@ -325,9 +395,9 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
 
   // ---- min-p: the lowest key whose weight reaches it
   Cut kept{0u, 0x7fffffff};
-  if (least > 0.f) {
+  if (at_least > 0.f) {
     if (threadIdx.x == 0) {
-      const double wanted = (double)least;
+      const double wanted = (double)at_least;
       float guess = (float)fma((double)temperature, log(wanted), weight.top);
       unsigned key = min(max(order_key(cleaned(guess)), no_key + 1), top_key);
       for (int i = 0; i < 64 && key < top_key && weight(of_key(key)) < wanted; ++i) ++key;
@@ -419,28 +489,6 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
 
   if ((by_count && k <= SL_MOST_K) || kept.key != 0u || vocab <= SL_LIST) {
     // ---- few candidates, it is likely
-    float bound = -INFINITY;
-    if (by_count && k <= SL_MOST_K && k <= ranks * SL_THREADS && vocab > SL_LIST) {
-      const float scale = top > least_max && top < INFINITY ? (float)(SL_BINS - 1) / (top - least_max) : 0.f;
-      clear_bins();
-      if (threadIdx.x == 0) s.bound = -INFINITY;
-      if (mine > -INFINITY) atomicAdd(&bins[scale > 0.f ? min(SL_BINS - 1, (int)((top - mine) * scale)) : 0], 1u);
-      add_up_bins();
-      int here = 0, total, until;
-#pragma unroll
-      for (int j = 0; j < SL_BINS_PER_THREAD; ++j) here += count[j];
-      const int before = before_block(here, s.warp_int, &total, &until);
-      if (before < k && until >= k) {      // one thread's (none's where fewer threads met a number)
-        int run = before, bin = first_bin;
-#pragma unroll
-        for (int j = 0; j < SL_BINS_PER_THREAD; ++j)
-          if (run < k) { run += count[j]; bin = first_bin + j; }
-        // (a hundredth of a bin is more than the roundings)
-        s.bound = scale > 0.f ? top - ((float)bin + 1.01f) / scale : least_max;
-      }
-      __syncthreads();
-      bound = s.bound;
-    }
     const unsigned lowest = max(order_key(bound), kept.key);
     collect(lowest, 0xffffffffu, kept);
     cluster.sync();
