@@ -73,6 +73,7 @@ LIBRARIES: dict[str, tuple[str, ...]] = {
     "sampling_limits": (),
     "attention_quantized": (),
     "attention_quantized_decode": (),
+    "attention_quantized_split": (),
     "attention_quantized_prompt": (),
 }
 

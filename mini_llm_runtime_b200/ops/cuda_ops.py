@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import os
 from dataclasses import dataclass
 
@@ -115,6 +116,7 @@ _PROTOTYPES = {
     "copy_pages": {"mlr_copy_pages": "pippip"},
     "attention_quantized_decode": {"mlr_attention_quantized_decode": "pppppp" "ppppp" "iiiiiiiii" "fi" "ppp",
                                    "mlr_attention_quantized_decode_bytes": "iiiiii"},
+    "attention_quantized_split": {"mlr_attention_quantized_split": "pppppp" "ppppp" "iiiiiiiii" "fii" "pip"},
     "attention_quantized_prompt": {"mlr_attention_quantized_prompt": "pppppp" "ppppppp" "iiiiiiiiiiii" "fi" "pppp" "l" "pip",
                                    "mlr_attention_quantized_prompt_bytes": "iiiiii"},
     "sampling_limits": {"mlr_sample_limited": "pppppppp" "ii" "p" "ii" "p"},
@@ -1305,12 +1307,27 @@ class CudaOps:
                 table, slot, width, decodes, *sizes, longest, scratch.data_ptr(), self._error_word(q.device).data_ptr(), _raw_stream()),
                 "quantized_attention (decoded tokens)")
             rest -= decodes
+        elif decodes > 0 and decodes * num_kv_heads <= 65535:
+            chunk, longest = self.QUANTIZED_CHUNK, int(batch.max_kv_len)
+            keys = min(longest, window + self.QUANTIZED_CHUNK) if window else longest
+            each = decodes * num_heads * (head_dim + 2) * 4
+            while -(-keys // chunk) > 1 and -(-keys // chunk) * each > self.QUANTIZED_SCRATCH_BYTES:
+                chunk *= 2
+            parts = -(-keys // chunk) + (1 if window else 0)
+            scratch = torch.empty(parts * each, dtype=torch.uint8, device=q.device)
+            _check(_declared_library("attention_quantized_split").mlr_attention_quantized_split(
+                q.data_ptr(), *pool.addresses, out.data_ptr(), None if decodes == batch.num_segments else plan["decode_seg"].data_ptr(), q_start, pos0,
+                table, slot, width, decodes, *sizes, chunk, parts, scratch.data_ptr(), _code(q.dtype), _raw_stream()),
+                "quantized_attention (decoded tokens)")
+            rest -= decodes
         if rest > 0:
             _check(_declared_library("attention_quantized").mlr_attention_quantized(
                 q.data_ptr(), *pool.addresses, out.data_ptr(), plan["tile_seg"].data_ptr() + 4 * first, plan["tile_row0"].data_ptr() + 4 * first, q_start,
                 batch.seg_q_len.data_ptr(), pos0, table, slot, width, rest, *sizes, _code(q.dtype), _raw_stream()), "quantized_attention")
         return out
 
+    QUANTIZED_CHUNK = 256                     # keys of a part in attention_quantized_split.cu, while the parts' states fit
+    QUANTIZED_SCRATCH_BYTES = 256 << 20
     QUANTIZED_DECODES = 2048      # requests of one launch (attention_quantized_decode.cu)
 
     # ------------------------------------------------------------------ pages of a cache
@@ -1323,53 +1340,61 @@ class CudaOps:
         target twice."""
         pools = list(pools)
         targets = pools if into is None else list(into)
-        try:
-            numbers = np.array([source, target], dtype=np.int64)      # (unlike lengths raise)
-        except ValueError:
-            numbers = np.empty(0)
-        if numbers.ndim != 2:
+        count = len(source)
+        if len(target) != count:
             raise KernelError("source and target need one page number each")
-        count = numbers.shape[1]
         if len(targets) != len(pools):
             raise KernelError(f"{len(pools)} pools cannot be copied into {len(targets)}")
         device = torch._C._cuda_getDevice()
-        for what, side in (("source", pools), ("target", targets)):
-            if side is pools and what == "target":
-                break                                  # checked as sources
-            for pool in side:
-                _need(pool, f"a {what} pool")
-                if pool.device.index != device:
-                    _need_here(pool=pool)
-                if pool.dim() < 2 or pool.shape[1] != side[0].shape[1]:
-                    raise KernelError(f"the {what} pools must have one number of pages")
-        if not pools or not count:
-            return
-        ends, begins = numbers.max(axis=1), numbers.min(axis=1)
-        for i, (what, side) in enumerate((("source", pools), ("target", targets))):
-            if begins[i] < 0 or ends[i] >= side[0].shape[1]:
-                raise KernelError(f"{what} pages must lie in [0, {side[0].shape[1]})")
-        if count > 1 or into is None:
-            taken = np.zeros(int(max(ends)) + 1, dtype=bool)
-            taken[numbers[1]] = True
-            if np.count_nonzero(taken) != count:
-                raise KernelError("a page is the target of one copy")
-            if into is None and taken[numbers[0]].any():
-                raise KernelError("a page cannot be source and target")
-        if into is not None:
-            for pool, other in zip(pools, targets):
-                if other.dtype != pool.dtype or other.shape[0] != pool.shape[0] or other.shape[2:] != pool.shape[2:]:
-                    raise KernelError(f"pages of {tuple(pool.shape)} {pool.dtype} do not fit {tuple(other.shape)} {other.dtype}")
-            spans = [[(pool.data_ptr(), pool.data_ptr() + pool.numel() * pool.element_size()) for pool in group] for group in (pools, targets)]
-            if any(first < end and begin < last for begin, end in spans[0] for first, last in spans[1]):
-                raise KernelError("the pools that pages go to must not be those that they come from")
         fields = []
         for pool, other in zip(pools, targets):
-            entries, pages = pool.shape[:2]
-            page = pool.numel() // (entries * pages) * pool.element_size() if entries else 0
-            if page:
+            for what, tensor, first in (("source", pool, pools[0]), ("target", other, targets[0])):
+                if tensor is other and what == "source":
+                    continue                           # one tensor, looked at once
+                _need(tensor, f"a {what} pool")
+                if tensor.get_device() != device:
+                    _need_here(pool=tensor)
+                if tensor.dim() < 2 or tensor.shape[1] != first.shape[1]:
+                    raise KernelError(f"the {what} pools must have one number of pages")
+            entries, pages, *inner = pool.shape
+            if into is not None and (other.dtype != pool.dtype or other.shape[0] != entries or list(other.shape[2:]) != inner):
+                raise KernelError(f"pages of {tuple(pool.shape)} {pool.dtype} do not fit {tuple(other.shape)} {other.dtype}")
+            page = math.prod(inner) * pool.element_size()
+            if page and entries:
                 fields += (pool.data_ptr(), other.data_ptr(), pages * page, other.shape[1] * page, page, entries)
-        numbers = numbers.astype(np.int32)
-        at = numbers.ctypes.data
+        if into is not None:
+            spans = [[(at, at + size * entries) for at, size, entries in zip(fields[side::6], fields[2 + side::6], fields[5::6])] for side in (0, 1)]
+            if any(first < end and begin < last for begin, end in spans[0] for first, last in spans[1]):
+                raise KernelError("the pools that pages go to must not be those that they come from")
+        if not pools or not count:
+            return
+        # page numbers: few in Python, many in numpy (a conversion costs more than what is done with it below some fifty)
+        few = count <= 48
+        if few:
+            source, target = [int(page) for page in source], [int(page) for page in target]
+        else:
+            source, target = np.asarray(source, dtype=np.int64), np.asarray(target, dtype=np.int64)
+        for what, side, numbers in (("source", pools, source), ("target", targets, target)):
+            low, high = (min(numbers), max(numbers)) if few else (numbers.min(), numbers.max())
+            if low < 0 or high >= side[0].shape[1]:
+                raise KernelError(f"{what} pages must lie in [0, {side[0].shape[1]})")
+        if few:
+            places = set(target)
+            once, apart = len(places) == count, places.isdisjoint(source)
+        else:
+            taken = np.zeros(max(pools[0].shape[1], targets[0].shape[1]), dtype=bool)
+            taken[target] = True
+            once, apart = np.count_nonzero(taken) == count, not taken[source].any()
+        if not once:
+            raise KernelError("a page is the target of one copy")
+        if into is None and not apart:
+            raise KernelError("a page cannot be source and target")
+        if few:
+            numbers = (ctypes.c_int * (2 * count))(*source, *target)
+            at = ctypes.addressof(numbers)
+        else:
+            numbers = np.concatenate([source, target]).astype(np.int32)
+            at = numbers.ctypes.data
         entry = _declared_library("copy_pages").mlr_copy_pages
         for first in range(0, len(fields), 6 * self.COPY_POOLS):
             some = fields[first:first + 6 * self.COPY_POOLS]
