@@ -77,6 +77,30 @@ class PoolAllocator:
             self._held.discard(i)
             heapq.heappush(self._free, i)
 
+    # ---- items that several hold, items that move
+    def hand_over(self, item: int, *, from_promise: bool, to_promise: bool) -> None:
+        """A held item counts for another holder from now on, under a promise or none (a promise of the one it counted for goes with it)."""
+        if item not in self._held:
+            raise ValueError(f"{self.what} {item} is not held")
+        change = int(to_promise) - int(from_promise)
+        self._promised += change
+        self._drawn += change
+
+    @property
+    def needed(self) -> int:
+        """Items that are held or promised: the least total that serves them."""
+        return len(self._held) + max(0, self._promised - self._drawn)
+
+    def move(self, places: dict[int, int], total: int) -> None:
+        """Held items get other numbers, and there are ``total`` items."""
+        if set(places) != self._held or len(set(places.values())) != len(places) or any(not 0 <= place < total for place in places.values()):
+            raise ValueError(f"the moves do not name every held {self.what} once, in [0, {total})")
+        if total < self.total and total < self.needed:
+            raise OutOfPages(f"{self.needed} {self.what}s are held or promised, more than {total}")
+        self.total = int(total)
+        self._held = set(places.values())
+        self._free = [item for item in range(self.total) if item not in self._held]
+
     # ---- promises (counted reservations)
     @property
     def promised(self) -> int:

@@ -32,6 +32,16 @@ request they belong to cannot be released before those that share its pages.  Cr
 does not fit beside such ones is refused instead of left waiting.  (Whole pages of groups that keep every key; a
 window gives pages back and a fixed-size state has none.)
 
+Forks.  A request may also start with any number of tokens of another one (``create_request(..., fork=(request, tokens))``): whole pages are
+held by both, the page it ends in is copied (all layers at once).  Such pages count for the request that held them first; when it ends,
+they count for the next one.  Neither has to outlive the other.
+
+Moving.  ``compact`` moves pages into the lowest numbers of their pools, ``resize`` into pools of another size.
+
+8 bits.  With ``quantized_block`` the pools hold codes of 8 bits and a float32 scale for each block of so many tokens and kv head
+(``ops.QuantizedPool``).  With blocks of more than a token, a step that fails after its tokens were stored may leave the scale of a
+request's last block larger than it was, and its tokens rounded to it.
+
 Two admission modes.  With a *promise* (``create_request(..., lifetime_tokens=n)``) the pages of
 the request's whole life are counted against the pool at creation, as the reference reserves them
 (src/mini_llm_runtime/block_admission.py:35-67), so the pool cannot run dry mid-request; pages are
@@ -47,6 +57,7 @@ from typing import Sequence
 import numpy as np
 import torch
 
+from .. import ops
 from ..parts.base import KVCacheNeed, StateNeed
 from .allocator import OutOfPages, PoolAllocator
 from .slots import SLOT_WORDS, slot_record
@@ -71,10 +82,19 @@ class CacheGroup:
     table: np.ndarray | None = None    # host mirror: int32 [max_requests, max_pages_per_request], -1 = no page
     device_table: torch.Tensor | None = None   # the same table where the kernels read it
     dirty: set = field(default_factory=set)    # slots whose row differs from the device's copy
+    key_scales: torch.Tensor | None = None     # of pools in 8 bits: [entries, pages, kv_heads, page_size / block]
+    value_scales: torch.Tensor | None = None
+    quantized: list = field(default_factory=list)      # the entries' ``QuantizedPool``s
+    borrowers: dict = field(default_factory=dict)      # page -> requests that hold it beside the one it counts for, in order
 
     @property
     def window(self) -> int | None:
         return self.need.window
+
+    @property
+    def pools(self) -> list[torch.Tensor]:
+        """Everything that belongs to the pages: [entries, pages, ..] each."""
+        return [pool for pool in (self.key, self.value, self.key_scales, self.value_scales) if pool is not None]
 
     def bytes_per_page(self, itemsize: int) -> int:
         return (len(self.entries) * self.need.num_kv_heads * self.page_size
@@ -101,10 +121,11 @@ class RequestCache:
     prefix_of: str | None = None
     sharers: int = 0                  # requests that start with pages of this one
     lasting: bool = False             # held until its owner releases it, not until it has run
+    borrowed: list[set[int]] = field(default_factory=list)      # per group: pages held since a fork that count for another request
 
     def own(self, group: int) -> list[int]:
-        """The pages the request itself holds."""
-        return [p for p in self.pages[group][self.shared_pages:] if p >= 0]
+        """The pages that count for the request."""
+        return [p for p in self.pages[group][self.shared_pages:] if p >= 0 and not (self.borrowed and p in self.borrowed[group])]
 
     def held(self, group: int) -> int:
         return len(self.own(group))
@@ -128,9 +149,12 @@ class CacheManager:
     def __init__(self, needs: Sequence[KVCacheNeed | StateNeed | None], *, page_size: int,
                  num_pages: int | Sequence[int], max_requests: int, max_tokens_per_request: int,
                  dtype: torch.dtype, device: torch.device | str, max_step_tokens: int | None = None,
-                 allocate_device_memory: bool = True) -> None:
+                 allocate_device_memory: bool = True, quantized_block: int | None = None) -> None:
         if page_size <= 0 or max_requests <= 0 or max_tokens_per_request <= 0:
             raise ValueError("page_size, max_requests and max_tokens_per_request must be > 0")
+        if quantized_block is not None and (quantized_block <= 0 or page_size % quantized_block):
+            raise ValueError(f"a block of {quantized_block} tokens does not divide a page of {page_size}")
+        self.quantized_block = quantized_block
         self.page_size = int(page_size)
         self.max_requests = int(max_requests)
         self.max_tokens_per_request = int(max_tokens_per_request)
@@ -172,10 +196,10 @@ class CacheManager:
             group.num_pages = count
             group.allocator = PoolAllocator(count, "page")
             group.table = np.full((self.max_requests, self.max_pages_per_request), -1, dtype=np.int32)
+            if quantized_block is not None and group.need.value_head_dim != group.need.head_dim:
+                raise ValueError("a cache in 8 bits holds keys and values of one size")
             if allocate_device_memory:
-                shape = (len(group.entries), count, group.need.num_kv_heads, self.page_size)
-                group.key = torch.zeros((*shape, group.need.head_dim), dtype=dtype, device=self.device)
-                group.value = torch.zeros((*shape, group.need.value_head_dim), dtype=dtype, device=self.device)
+                self._allocate_pools(group, count)
                 if self.device.type == "cuda":
                     group.device_table = torch.full((self.max_requests, self.max_pages_per_request), -1,
                                                     dtype=torch.int32, device=self.device)
@@ -214,6 +238,16 @@ class CacheManager:
         self._lasting: dict[str, RequestCache] = {}
         self._step: list[tuple[RequestCache, int]] | None = None
         self._state_backup: tuple[torch.Tensor, dict[int, torch.Tensor]] | None = None
+
+    def _allocate_pools(self, group: CacheGroup, count: int) -> None:
+        shape = (len(group.entries), count, group.need.num_kv_heads, self.page_size)
+        dtype = self.dtype if self.quantized_block is None else torch.int8
+        group.key = torch.zeros((*shape, group.need.head_dim), dtype=dtype, device=self.device)
+        group.value = torch.zeros((*shape, group.need.value_head_dim), dtype=dtype, device=self.device)
+        if self.quantized_block is not None:
+            blocks = (*shape[:3], self.page_size // self.quantized_block)
+            group.key_scales, group.value_scales = (torch.zeros(blocks, dtype=torch.float32, device=self.device) for _ in range(2))
+            group.quantized = [ops.QuantizedPool(*pools) for pools in zip(group.key, group.value, group.key_scales, group.value_scales)]
 
     # ------------------------------------------------------------------ sizing
     def pages_for_lifetime(self, group: CacheGroup, lifetime_tokens: int) -> int:
@@ -256,14 +290,23 @@ class CacheManager:
     # ------------------------------------------------------------------ requests
     def create_request(self, request_id: str, *, lifetime_tokens: int | None = None,
                        temperature: float = 0.0, seed: int = 0,
-                       prefix: tuple[str, int] | None = None, lasting: bool = False) -> RequestCache | None:
+                       prefix: tuple[str, int] | None = None, lasting: bool = False,
+                       fork: tuple[str, int] | None = None) -> RequestCache | None:
         """Register a request and give it a slot.  With ``lifetime_tokens`` its pages are promised
         now; returns None (nothing changed) if the promise cannot be kept or no slot is free.
         ``temperature`` and ``seed`` go into the slot's record for the sampling kernel.  ``prefix``: the request
-        starts with that many tokens of another one, on its pages.  ``lasting`` (with a promise): others must not wait for it to end."""
+        starts with that many tokens of another one, on its pages.  ``lasting`` (with a promise): others must not wait for it to end.
+        ``fork``: the request starts with that many tokens of another one, whole pages held by both, the last one copied."""
         if request_id in self.requests:
             raise ValueError(f"request {request_id!r} already has a cache")
+        if fork is not None:
+            if prefix is not None or lasting:
+                raise ValueError("a fork has the prefix of the request it starts with, and ends by itself")
+            parent, whole = self._forked_pages(request_id, lifetime_tokens, fork)
+            if parent.prefix_of is not None and whole:
+                prefix = (parent.prefix_of, min(whole, parent.shared_pages) * self.page_size)
         source, shared = self._shared_pages(request_id, lifetime_tokens, prefix)
+        borrowed = 0 if fork is None else whole - shared       # pages that will count for the parent
         if self.slots.free_count == 0:
             if lifetime_tokens is None:
                 raise OutOfPages(f"no free request slot (max_requests={self.max_requests})")
@@ -276,7 +319,7 @@ class CacheManager:
                 raise ValueError("lifetime_tokens must be > 0")
             if not self.can_be_admitted(lifetime_tokens, prefix):
                 raise ValueError(self.why_not_admitted(request_id, lifetime_tokens, shared))
-            wanted = tuple(count - shared for count in self.lifetime_pages(lifetime_tokens))
+            wanted = tuple(count - shared - borrowed for count in self.lifetime_pages(lifetime_tokens))
             done = []
             for group, count in zip(self.groups, wanted):
                 if not group.allocator.promise(count):
@@ -285,6 +328,18 @@ class CacheManager:
                     return None
                 done.append((group, count))
             promised = list(wanted)
+        tail: list[list[int]] = [[] for _ in self.groups]       # the page that a fork ends in
+        if fork is not None and fork[1] % self.page_size:
+            try:
+                for group in self.groups:
+                    tail[group.index] = group.allocator.allocate(1, promised=bool(promised[group.index]))
+            except OutOfPages:
+                for group in self.groups:
+                    group.allocator.free(tail[group.index], promised=bool(promised[group.index]))
+                    group.allocator.unpromise(promised[group.index])
+                if lifetime_tokens is None:
+                    raise
+                return None                          # others hold, without a promise, what the promise counts on
         slot = self.slots.allocate(1)[0]
         request = RequestCache(request_id, slot,
                                pages=[[] for _ in self.groups],
@@ -299,6 +354,8 @@ class CacheManager:
                 request.pages[group.index] = source.pages[group.index][:shared]
                 group.table[slot, :shared] = request.pages[group.index]
                 group.dirty.add(slot)
+        if fork is not None:
+            self._fork(request, parent, whole, fork[1], tail)
         self.requests[request_id] = request
         if lasting:
             self._lasting[request_id] = request
@@ -328,6 +385,54 @@ class CacheManager:
             raise ValueError(f"request {request_id!r} would have no token of its own behind {tokens} shared ones")
         return source, tokens // self.page_size
 
+    def _forked_pages(self, request_id: str, lifetime_tokens: int | None, fork) -> tuple["RequestCache", int]:
+        """The request that a fork starts with and the whole pages of it, checked."""
+        parent, tokens = self.get(fork[0]), int(fork[1])
+        if not self.can_share_pages:
+            raise ValueError("requests fork in models whose layers keep every key, without windows or states")
+        if not 0 < tokens <= parent.committed:
+            raise ValueError(f"request {request_id!r} cannot start with {tokens} of the {parent.committed} tokens of {parent.request_id!r}")
+        if tokens >= (lifetime_tokens if lifetime_tokens is not None else self.max_tokens_per_request):
+            raise ValueError(f"request {request_id!r} would have no token of its own behind {tokens} forked ones")
+        return parent, tokens // self.page_size
+
+    def _fork(self, request: RequestCache, parent: RequestCache, whole: int, tokens: int, tail: list[list[int]]) -> None:
+        request.borrowed = [set() for _ in self.groups]
+        request.committed = tokens
+        for group in self.groups:
+            index = group.index
+            held = parent.pages[index][request.shared_pages:whole]
+            for page in held:
+                group.borrowers.setdefault(page, []).append(request.request_id)
+            request.borrowed[index].update(held)
+            request.pages[index] = parent.pages[index][:whole] + tail[index]
+            group.table[request.slot, :len(request.pages[index])] = request.pages[index]
+            group.dirty.add(request.slot)
+            if tail[index] and group.pools:
+                # stream order: the parent's tokens were written by launches before this one
+                ops.current().copy_pages(group.pools, [parent.pages[index][whole]], tail[index])
+
+    def _hand_over(self, request: RequestCache) -> None:
+        """Of the pages that count for the request, those that others hold too count for the next of them."""
+        for group in self.groups:
+            for page in request.own(group.index) if group.borrowers else ():
+                heirs = group.borrowers.get(page)
+                if heirs is None:
+                    continue
+                heir = self.requests[heirs.pop(0)]
+                if not heirs:
+                    del group.borrowers[page]
+                heir.borrowed[group.index].discard(page)
+                group.allocator.hand_over(page, from_promise=bool(request.promised[group.index]), to_promise=bool(heir.promised[group.index]))
+                request.promised[group.index] -= bool(request.promised[group.index])
+                heir.promised[group.index] += bool(heir.promised[group.index])
+                request.pages[group.index][request.pages[group.index].index(page)] = -1
+            for page in request.borrowed[group.index] if request.borrowed else ():
+                holders = group.borrowers[page]
+                holders.remove(request.request_id)
+                if not holders:
+                    del group.borrowers[page]
+
     def _state_tensors(self):
         for by_name in self.states.values():
             yield from by_name.values()
@@ -346,6 +451,7 @@ class CacheManager:
         if request.sharers:
             raise RuntimeError(f"request {request_id!r} has pages that {request.sharers} other requests start with")
         freed: dict[int, list[int]] = {}
+        self._hand_over(request)
         for group in self.groups:
             ids = request.own(group.index)
             group.allocator.free(ids, promised=bool(request.promised[group.index]))
@@ -518,11 +624,73 @@ class CacheManager:
     def resident_updates_sent(self) -> None:
         self._unconfirmed = None
 
+    # ------------------------------------------------------------------ moving pages
+    def _moved(self, group: CacheGroup, places: dict[int, int], pages: int) -> None:
+        """The host's side of a move: every list of pages follows ``places``, the pool has ``pages`` pages."""
+        group.allocator.move(places, pages)
+        group.num_pages = pages
+        group.borrowers = {places[page]: holders for page, holders in group.borrowers.items()}
+        group.table[:] = -1
+        for request in self.requests.values():
+            request.pages[group.index] = [page if page < 0 else places[page] for page in request.pages[group.index]]
+            if request.borrowed:
+                request.borrowed[group.index] = {places[page] for page in request.borrowed[group.index]}
+            group.table[request.slot, :len(request.pages[group.index])] = request.pages[group.index]
+            group.dirty.add(request.slot)
+
+    def compact(self) -> int:
+        """Move pages from behind free ones into the lowest numbers of their pools, between steps; returns how many moved."""
+        if self._step is not None:
+            raise RuntimeError("pages move between steps")
+        moved = 0
+        for group in self.groups:
+            held = sorted(group.allocator.held)
+            source = [page for page in held if page >= len(held)]
+            if not source:
+                continue
+            low = set(held)
+            target = [page for page in range(len(held)) if page not in low]
+            if group.pools:
+                ops.current().copy_pages(group.pools, source, target)
+            places = {page: page for page in held}
+            places.update(zip(source, target))
+            self._moved(group, places, group.num_pages)
+            moved += len(source)
+        return moved
+
+    def can_resize(self, num_pages: int | Sequence[int]) -> tuple[int, ...]:
+        """The groups' numbers of pages, if pools of so many hold what is held and promised."""
+        counts = [int(num_pages)] * len(self.groups) if isinstance(num_pages, int) else [int(n) for n in num_pages]
+        if len(counts) != len(self.groups):
+            raise ValueError(f"num_pages names {len(counts)} groups, the model has {len(self.groups)}")
+        for group, count in zip(self.groups, counts):
+            if count < 1 or (count < group.num_pages and count < group.allocator.needed):
+                raise OutOfPages(f"{group.allocator.needed} pages of group {group.index} are held or promised, more than {count}")
+        return tuple(counts)
+
+    def resize(self, num_pages: int | Sequence[int]) -> None:
+        """Pools of another size, between steps: what they hold moves into the lowest pages of the new ones.  Captured steps that read the
+        old ones must not run again (``ModelRunner.forget_captured_steps``)."""
+        if self._step is not None:
+            raise RuntimeError("pages move between steps")
+        for group, count in zip(self.groups, self.can_resize(num_pages)):
+            held = sorted(group.allocator.held)
+            before = group.pools
+            if before:
+                self._allocate_pools(group, count)
+                ops.current().copy_pages(before, held, range(len(held)), into=group.pools)
+            self._moved(group, {page: place for place, page in enumerate(held)}, count)
+
     # ------------------------------------------------------------------ views and numbers
     def entry_pools(self, entry: int) -> tuple[torch.Tensor, torch.Tensor, CacheGroup]:
         group_index, local = self.entry_group[entry]
         group = self.groups[group_index]
         return group.key[local], group.value[local], group
+
+    def quantized_pool(self, entry: int):
+        """The entry's keys and values where they are held in 8 bits, else None."""
+        group_index, local = self.entry_group[entry]
+        return self.groups[group_index].quantized[local] if self.groups[group_index].quantized else None
 
     def slot_mapping(self, group: CacheGroup, request: RequestCache, start: int, count: int) -> np.ndarray:
         """Flat slot (page * page_size + offset) of tokens start..start+count-1."""
@@ -565,6 +733,9 @@ class CacheManager:
                                              f"{owners[page_id]!r} and {request.request_id!r}")
                     owners[page_id] = request.request_id
                 row = group.table[request.slot]
+                for page_id in request.borrowed[group.index] if request.borrowed else ():
+                    if request.request_id not in group.borrowers.get(page_id, ()) or page_id not in pages:
+                        raise AssertionError(f"{request.request_id!r} holds page {page_id} of a fork that does not know it")
                 if list(row[:len(pages)]) != pages or (row[len(pages):] != -1).any():
                     raise AssertionError(f"block table row of {request.request_id!r} differs from its page list")
             if set(owners) != set(group.allocator.held):

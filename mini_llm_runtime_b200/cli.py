@@ -63,6 +63,9 @@ def build_parser() -> argparse.ArgumentParser:
         sub.add_argument("--presence-penalty", type=float, default=0.0, help="off the logit of every generated token")
         sub.add_argument("--frequency-penalty", type=float, default=0.0, help="the same for each time it was generated")
         sub.add_argument("--logit-bias", type=_bias_list, default=None, help="comma-separated token:bias pairs (-inf bans a token)")
+        sub.add_argument("--top-k", type=int, default=0, help="draw from the k most probable tokens (0: no limit)")
+        sub.add_argument("--top-p", type=float, default=1.0, help="draw from the fewest tokens that hold p of the probability (1: no limit)")
+        sub.add_argument("--min-p", type=float, default=0.0, help="draw from tokens at least so many times as probable as the best (0: no limit)")
         sub.add_argument("--eos-id", type=_int_list, default=None, help="comma-separated EOS token ids")
         sub.add_argument("--output-dir", type=Path, default=None, help="optional folder for result.json")
         sub.add_argument("--device", default="cuda:0")
@@ -99,6 +102,14 @@ def _rules(args) -> dict:
     return rules if SamplingParams(**rules).has_rules else {}
 
 
+def _limits(args) -> dict:
+    """The request's limits on what is drawn, empty where there are none."""
+    from .sampling import SamplingParams
+
+    limits = {"top_k": args.top_k, "top_p": args.top_p, "min_p": args.min_p}
+    return limits if SamplingParams(**limits).has_limits else {}
+
+
 def _engine(args):
     import torch
 
@@ -110,7 +121,7 @@ def _engine(args):
         args.model, dtype=args.dtype, device=args.device, block_size=args.block_size,
         total_blocks=args.total_blocks, max_running_requests=args.max_running_requests,
         max_batch_tokens=args.max_batch_tokens, max_mixed_prefill_tokens=args.max_mixed_prefill_tokens,
-        max_model_len=args.max_model_len, step_ahead=args.step_ahead, logit_rules=bool(_rules(args)))
+        max_model_len=args.max_model_len, step_ahead=args.step_ahead, logit_rules=bool(_rules(args)), sampling_limits=bool(_limits(args)))
 
 
 def _write(args, record: dict) -> None:
@@ -124,7 +135,7 @@ def command_generate(args) -> int:
     engine = _engine(args)
     started = time.perf_counter()
     engine.submit("cli", list(args.prompt_ids), max_new_tokens=args.max_new_tokens,
-                  eos_token_ids=args.eos_id, temperature=args.temperature, seed=args.seed, **_rules(args))
+                  eos_token_ids=args.eos_id, temperature=args.temperature, seed=args.seed, **_rules(args), **_limits(args))
     engine.run()
     request = engine.scheduler.get_request("cli")
     _write(args, {"prompt_ids": list(args.prompt_ids), "generated_ids": list(request.generated_token_ids),
@@ -148,7 +159,7 @@ def command_serve_batch(args) -> int:
                 torch.randint(0, vocab, (args.prompt_length,), generator=generator).tolist()
             rid = f"run{run}-req{index}"
             engine.submit(rid, prompt, max_new_tokens=args.generation_lengths[index % len(args.generation_lengths)],
-                          eos_token_ids=args.eos_id, temperature=args.temperature, seed=args.seed + index, **_rules(args))
+                          eos_token_ids=args.eos_id, temperature=args.temperature, seed=args.seed + index, **_rules(args), **_limits(args))
             ids.append(rid)
         steps = engine.run()
         seconds = time.perf_counter() - started

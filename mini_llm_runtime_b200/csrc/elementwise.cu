@@ -195,7 +195,7 @@ __global__ void rope_kv_write_kernel(const T* qkv, const int* __restrict__ posit
   const int row_width = (heads + 2 * kv_heads) * head_dim;
   const T* row = qkv + (size_t)token * row_width;
   const float position = (float)positions[token];
-  const long long slot = slots[token];
+  const long long slot = slots != nullptr ? slots[token] : token;      // (no slots: rows one behind the other)
   const long long page = slot >= 0 ? slot / page_size : 0;
   const int offset = slot >= 0 ? (int)(slot - page * page_size) : 0;
   const bool store = write_kv != 0 && slot >= 0;

@@ -29,7 +29,7 @@ from .. import ops
 from ..cache.allocator import OutOfPages
 from ..cache.manager import CacheManager
 from ..models.decoder import DecoderModel
-from ..sampling import LogitRules, SamplingParams
+from ..sampling import LogitRules, RequestLimits, SamplingParams
 from .metrics import RequestMetricsCollector
 from .scheduler import BatchingPolicy, CacheGate, Request, RequestScheduler, RequestStatus, StepOutcome, StepPlan, WorkKind
 from .step import ModelRunner, StepEntry
@@ -102,9 +102,16 @@ class ContinuousBatchEngine:
                    max_mixed_prefill_tokens: int | None = None, max_model_len: int | None = None,
                    batching_policy: BatchingPolicy = BatchingPolicy.CONTINUOUS,
                    chunked_prefill: bool = True, enable_nvtx: bool = False,
-                   step_ahead: bool = False, logit_rules: bool = False, max_prefixes: int = 0) -> "ContinuousBatchEngine":
+                   step_ahead: bool = False, logit_rules: bool = False, max_prefixes: int = 0,
+                   sampling_limits: bool = False, cache_dtype: str | None = None, cache_block: int = 1) -> "ContinuousBatchEngine":
         """``logit_rules``: requests may bring penalties, biases and grammars (``submit``, ``allow_tokens``); every step then applies them.
-        ``max_prefixes``: how many prefixes the cache may hold for requests to share (``add_prefix``)."""
+        ``max_prefixes``: how many prefixes the cache may hold for requests to share (``add_prefix``).  ``sampling_limits``: requests may
+        limit what is drawn for them by top-k, top-p and min-p; every step then draws under the limits of its requests.
+        ``cache_dtype="int8"``: the cache holds keys and values in 8 bits with a scale for each ``cache_block`` tokens and kv head (models
+        whose layers all attend to such a cache).  With blocks of one token a request's results do not depend on how its
+        prompt was cut; larger blocks save four bytes per token and head less one."""
+        if cache_dtype not in (None, "int8"):
+            raise ValueError(f"unknown cache dtype {cache_dtype!r}; known: int8, or None for the model's own")
         # a model without a position limit of its own gets this engine's default
         max_model_len = min(max_model_len or min(model.spec.max_positions, cls.DEFAULT_MODEL_LEN),
                             model.spec.max_positions)
@@ -114,13 +121,16 @@ class ContinuousBatchEngine:
             total_blocks = (max_running_requests + max_prefixes) * -(-max_model_len // block_size)
         cache = CacheManager(model.cache_needs(), page_size=block_size, num_pages=total_blocks,
                              max_requests=max_running_requests + max_prefixes, max_tokens_per_request=max_model_len,
-                             dtype=model.compute_dtype, device=model.device, max_step_tokens=max_batch_tokens)
+                             dtype=model.compute_dtype, device=model.device, max_step_tokens=max_batch_tokens,
+                             quantized_block=None if cache_dtype is None else cache_block)
         scheduler = RequestScheduler(max_running_requests=max_running_requests, max_batch_tokens=max_batch_tokens,
                                      max_mixed_prefill_tokens=max_mixed_prefill_tokens, gate=CacheGate(cache),
                                      batching_policy=batching_policy, chunked_prefill=chunked_prefill)
         runner = ModelRunner(model, cache)
         if logit_rules:
             runner.rules = LogitRules(cache.max_requests, runner.vocab_size, model.device)
+        if sampling_limits:
+            runner.limits = RequestLimits(cache.max_requests, model.device)
         return cls(scheduler=scheduler, runner=runner, enable_nvtx=enable_nvtx, step_ahead=step_ahead)
 
     @classmethod
@@ -141,10 +151,12 @@ class ContinuousBatchEngine:
     # ------------------------------------------------------------------ requests
     def submit(self, request_id: str, prompt_token_ids: Sequence[int], *, max_new_tokens: int,
                eos_token_ids: int | Collection[int] | None = None, temperature: float = 0.0,
-               seed: int = 0, prefix: str | None = None, **rules) -> Request:
+               seed: int = 0, prefix: str | None = None, fork_of: str | None = None, **rules) -> Request:
         """``prefix``: a prefix of ``add_prefix`` that the prompt starts with; its whole pages are shared, not computed again.
+        ``fork_of``: a request, waiting or running, whose prompt and output so far begin like the prompt; what its cache holds of them when the
+        new request is admitted is taken from there (whole pages held by both, the last one copied), and computed if it has ended.
         ``rules``: ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty``, ``logit_bias`` of ``SamplingParams`` (an engine
-        made with ``logit_rules=True``)."""
+        made with ``logit_rules=True``), and its ``top_k``, ``top_p``, ``min_p`` (an engine made with ``sampling_limits=True``)."""
         arrival_ns = self._clock_ns()
         vocab = self.runner.vocab_size
         outside = [t for t in prompt_token_ids if not isinstance(t, int) or isinstance(t, bool) or not 0 <= t < vocab]
@@ -159,15 +171,51 @@ class ContinuousBatchEngine:
             self.runner.rules.check(sampling)
         elif sampling.has_rules:
             raise ValueError("rules on logits need an engine made with logit_rules=True")
+        if sampling.has_limits and self.runner.limits is None:
+            raise ValueError("limits on what is drawn need an engine made with sampling_limits=True")
         if any(request_id == self._holder(name) for name in self._prefixes):
             raise ValueError(f"{request_id!r} is the name under which the cache holds a prefix")
+        common = self._common_tokens(request_id, fork_of, prefix, prompt_token_ids)
         holder, shared = self._shared_by(prefix, prompt_token_ids)
         if self._prefixes and not self.manager.can_be_admitted(longest, None if holder is None else (holder, shared)):
             raise ValueError(self.manager.why_not_admitted(request_id, longest, shared // self.manager.page_size))
         request = self.scheduler.submit(request_id, prompt_token_ids, max_new_tokens=max_new_tokens,
-                                        eos_token_ids=eos_token_ids, sampling=sampling, prefix=holder, shared=shared)
+                                        eos_token_ids=eos_token_ids, sampling=sampling, prefix=holder, shared=shared,
+                                        fork=None if not common else (fork_of, common))
         self.metrics.register_request(request_id, arrival_ns)
         return request
+
+    # ------------------------------------------------------------------ forks
+    def _common_tokens(self, request_id: str, fork_of: str | None, prefix: str | None, prompt: Sequence[int]) -> int:
+        """How many of the prompt's tokens, less one, are the first of the other request."""
+        if fork_of is None:
+            return 0
+        if prefix is not None:
+            raise ValueError("a fork shares the prefix of the request it starts with; prefix and fork_of exclude one another")
+        if not self.manager.can_share_pages:
+            raise ValueError("requests fork in models whose layers keep every key, without windows or states")
+        if fork_of == request_id:
+            raise ValueError(f"request {request_id!r} cannot fork from itself")
+        other = self.scheduler.get_request(fork_of)
+        known = (*other.prompt, *other.output)
+        common = 0
+        for mine, theirs in zip(prompt[:len(prompt) - 1], known):
+            if mine != theirs:
+                break
+            common += 1
+        return common
+
+    def resize_cache(self, total_blocks: int | Sequence[int]) -> None:
+        """Pools of another size for the cache, between steps: memory given back to others, or more room.  What requests hold moves along;
+        decode steps are captured anew."""
+        manager = self.manager
+        counts = manager.can_resize(total_blocks)
+        for request_id in self.scheduler.waiting_request_ids:
+            request = self.scheduler.get_request(request_id)
+            if any(need > count for need, count in zip(manager.lifetime_pages(request.lifetime_tokens), counts)):
+                raise OutOfPages(f"the waiting request {request_id!r} could never be admitted to pools of {counts} pages")
+        self.runner.forget_captured_steps()
+        manager.resize(counts)
 
     # ------------------------------------------------------------------ shared prefixes
     @staticmethod
@@ -300,6 +348,8 @@ class ContinuousBatchEngine:
                 entries.append(StepEntry(item.request_id, tokens, [len(tokens) - 1] if item.emits else []))
                 if item.admitted and self.runner.rules is not None:
                     self._admit_rules(item.request_id)
+                if item.admitted and self.runner.limits is not None:
+                    self.runner.limits.admit(self.manager.get(item.request_id).slot, self.scheduler.get_request(item.request_id).sampling)
                 if item.admitted:
                     self.metrics.record_prefill_started(item.request_id, self._clock_ns())
                 if item.emits:
@@ -408,8 +458,14 @@ class ContinuousBatchEngine:
 
     def generate(self, prompts: Sequence[Sequence[int]], *, max_new_tokens: int,
                  eos_token_ids: int | Collection[int] | None = None, temperature: float = 0.0,
-                 seed: int = 0, **rules) -> list[list[int]]:
-        """Token ids in, generated token ids out, for a list of prompts (host lists both ways); ``rules`` as for ``submit``."""
+                 seed: int = 0, answers: int = 1, **rules) -> list[list[int]]:
+        """Token ids in, generated token ids out, for a list of prompts (host lists both ways); ``rules`` as for ``submit``.  ``answers``:
+        so many outputs for each prompt, one behind the other, each drawn with a seed of its own; a prompt is computed once."""
+        if isinstance(answers, bool) or not isinstance(answers, int) or answers <= 0:
+            raise ValueError("answers must be a positive integer")
+        if answers > 1:
+            return self._generate_answers(prompts, answers, max_new_tokens=max_new_tokens, eos_token_ids=eos_token_ids, temperature=temperature,
+                                          seed=seed, **rules)
         scheduler = self.scheduler
         first = (len(scheduler.finished_request_ids) + len(scheduler.running_request_ids)
                  + len(scheduler.waiting_request_ids))
@@ -419,6 +475,27 @@ class ContinuousBatchEngine:
                         eos_token_ids=eos_token_ids, temperature=temperature, seed=seed + i, **rules)
         self.run()
         return [list(scheduler.get_request(request_id).generated_token_ids) for request_id in ids]
+
+
+    def _generate_answers(self, prompts, answers: int, *, seed: int, **options) -> list[list[int]]:
+        scheduler = self.scheduler
+        first = len(scheduler.finished_request_ids) + len(scheduler.running_request_ids) + len(scheduler.waiting_request_ids)
+        ids = [[f"generate-{first + i}-{j}" for j in range(answers)] for i in range(len(prompts))]
+        for i, prompt in enumerate(prompts):
+            self.submit(ids[i][0], list(prompt), seed=seed + i * answers, **options)
+        forks = self.manager.can_share_pages
+        open_prompts = set(range(len(prompts)))
+        while open_prompts or scheduler.has_unfinished_requests:
+            # the other answers follow as soon as the first one's prompt is in the cache (or its request has ended)
+            for i in sorted(open_prompts):
+                request = scheduler.get_request(ids[i][0])
+                if request.output or request.status is RequestStatus.FINISHED or not forks:
+                    open_prompts.discard(i)
+                    for j in range(1, answers):
+                        self.submit(ids[i][j], list(prompts[i]), seed=seed + i * answers + j, fork_of=ids[i][0] if forks else None, **options)
+            if scheduler.has_unfinished_requests and self.step() is None:
+                raise RuntimeError("requests are waiting but nothing can be scheduled")
+        return [list(scheduler.get_request(request_id).generated_token_ids) for group in ids for request_id in group]
 
 
 @dataclass(frozen=True)

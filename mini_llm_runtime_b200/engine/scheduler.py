@@ -91,6 +91,7 @@ class Request:
     slot: int | None = None
     prefix: str | None = None                   # the cached request whose pages hold the prompt's first ``shared`` tokens
     shared: int = 0
+    fork: tuple[str, int] | None = None         # another request and how many of the prompt's tokens are its first
     _prompt_array: "np.ndarray | None" = field(default=None, repr=False, compare=False)
 
     @property
@@ -202,10 +203,24 @@ class CacheGate:
         self.cache = cache
 
     def admit(self, request: Request) -> int | None:
+        if request.fork is not None:
+            return self._admit_fork(request)
         held = self.cache.create_request(request.request_id, lifetime_tokens=request.lifetime_tokens,
                                          temperature=request.sampling.temperature, seed=request.sampling.seed,
                                          prefix=None if request.prefix is None else (request.prefix, request.shared))
         return None if held is None else held.slot
+
+    def _admit_fork(self, request: Request) -> int | None:
+        """With what the other request's cache holds of the prompt now, if it is still there."""
+        other, common = request.fork
+        tokens = min(common, self.cache.get(other).committed) if other in self.cache.requests else 0
+        held = self.cache.create_request(request.request_id, lifetime_tokens=request.lifetime_tokens,
+                                         temperature=request.sampling.temperature, seed=request.sampling.seed,
+                                         fork=(other, tokens) if tokens else None)
+        if held is None:
+            return None
+        request.shared = request.cursor = tokens
+        return held.slot
 
     def release(self, request_id: str):
         return self.cache.release(request_id) if request_id in self.cache.requests else {}
@@ -289,9 +304,10 @@ class RequestScheduler:
     def submit(self, request_id: str, prompt_token_ids: Sequence[int], *, max_new_tokens: int,
                eos_token_ids: int | Collection[int] | None = None, temperature: float = 0.0,
                seed: int = 0, sampling: SamplingParams | None = None, prefix: str | None = None,
-               shared: int = 0) -> Request:
+               shared: int = 0, fork: tuple[str, int] | None = None) -> Request:
         """Queue a request; allowed at any time, also while a plan is outstanding.  ``prefix``, ``shared``: the prompt's first tokens
-        are on the pages of that cached request; only those behind them run through the model."""
+        are on the pages of that cached request; only those behind them run through the model.  ``fork``: another request and how many of
+        the prompt's first tokens are its own; the gate takes what is cached of them when this one is admitted."""
         if not request_id:
             raise ValueError("request_id must not be empty")
         if request_id in self._by_id:
@@ -301,6 +317,8 @@ class RequestScheduler:
             raise ValueError("prompt_token_ids must not be empty")
         if (prefix is None) != (shared == 0) or not 0 <= shared < len(prompt):
             raise ValueError("a shared prefix is shorter than the prompt and names the request it belongs to")
+        if fork is not None and (prefix is not None or fork[0] not in self._by_id or not 0 < fork[1] < len(prompt)):
+            raise ValueError("a fork names another request and fewer of its tokens than the prompt has, and no prefix")
         if not self.chunked_prefill and len(prompt) - shared > self.max_batch_tokens:
             raise ValueError(f"prompt length={len(prompt) - shared} exceeds max_batch_tokens={self.max_batch_tokens} "
                              "and chunked prefill is off")
@@ -314,7 +332,7 @@ class RequestScheduler:
         if sampling is None:
             sampling = SamplingParams(temperature, seed) if (temperature or seed) else GREEDY
         request = Request(request_id, prompt, max_new_tokens, stop, sampling, order=self._arrivals, cursor=shared, prefix=prefix,
-                          shared=shared)
+                          shared=shared, fork=fork)
         self._arrivals += 1
         self._by_id[request_id] = request
         self._queue.append(request)

@@ -65,6 +65,7 @@ class HostBatch:
     num_rows: int
     # of a step of decoded tokens: (segments, keys) of requests whose first keys are on the same pages
     shared: tuple = ()
+    quantized: bool = False      # the cache holds keys and values in 8 bits
 
     @property
     def num_segments(self) -> int:
@@ -86,6 +87,7 @@ class CacheView:
     states: dict = field(default_factory=dict)   # every fixed-size state of the entry by name ("state" is ``state``)
     group: int = -1                          # entries of one group share pages, table and ``shared``
     shared: dict = field(default_factory=dict)   # per step and group: mixers may keep derived objects here
+    quantized: object = None                 # ``ops.QuantizedPool``: the keys and values where the cache holds them in 8 bits
 
 
 @dataclass
@@ -195,6 +197,9 @@ class ModelRunner:
     def __init__(self, model: DecoderModel, cache: CacheManager) -> None:
         if model.device is None:
             raise ValueError("load the model's weights before building a runner")
+        if cache.quantized_block is not None and not all(
+                block.mixer.supports_quantized_cache for block in model.blocks if block.cache_need() is not None):
+            raise ValueError("a cache in 8 bits needs a model whose layers all attend to keys and values in 8 bits")
         self.model = model
         self.cache = cache
         self.device = model.device
@@ -227,6 +232,8 @@ class ModelRunner:
         # Rules of the requests on their logits (sampling/rules.py), or None.  To be set before the first step: a captured step
         # holds the launches of its time.
         self.rules = None
+        # The requests' limits on what is drawn (sampling/limits.py), or None; set before the first step likewise.
+        self.limits = None
 
     # ------------------------------------------------------------------ metadata
     def _upload(self, packer: _Packer, device_buffer: torch.Tensor | None = None) -> dict[str, torch.Tensor]:
@@ -290,7 +297,7 @@ class ModelRunner:
         np.cumsum(lengths[:-1], out=row_start[1:])
         position_start = np.array([r.pending[0] for r in requests], dtype=np.int32)
         shared = self._shared_groups(requests) if (lengths == 1).all() else ()
-        return HostBatch(lengths, row_start, position_start, int(lengths.sum()), shared)
+        return HostBatch(lengths, row_start, position_start, int(lengths.sum()), shared, self.cache.quantized_block is not None)
 
     def _shared_groups(self, requests: list[RequestCache]) -> tuple:
         """(segments, keys) of the requests that start with the same pages, two of them at least; longest prefixes first."""
@@ -318,7 +325,8 @@ class ModelRunner:
             if len(self._shared_shapes) >= 4096:
                 self._shared_shapes.clear()
             ones = np.ones(count, dtype=np.int32)
-            host = HostBatch(ones, np.arange(count, dtype=np.int32), np.full(count, shapes[0][1], dtype=np.int32), count, shared)
+            host = HostBatch(ones, np.arange(count, dtype=np.int32), np.full(count, shapes[0][1], dtype=np.int32), count, shared,
+                             self.cache.quantized_block is not None)
             known = any(name.startswith("shared.") for arrays, _ in self._step_plans(host).values() for name in arrays)
             self._shared_shapes[count, shapes] = known
         return known
@@ -413,7 +421,7 @@ class ModelRunner:
                 k_pool, v_pool, group = cache.entry_pools(entry)
                 view = CacheView(entry, k_pool, v_pool, dev[f"places{group.index}"],
                                  group.device_table, cache.page_size, group.window,
-                                 group=group.index, shared=shared_by_group[group.index])
+                                 group=group.index, shared=shared_by_group[group.index], quantized=cache.quantized_pool(entry))
             else:
                 view = CacheView(entry)
             view.state = cache.state.get(entry)
@@ -465,7 +473,10 @@ class ModelRunner:
         if sample:
             if self.rules is not None:
                 kernels.shape_logits_(logits, ctx.wanted_slot, self.rules.tables)
-            tokens = kernels.sample_slots(logits, ctx.wanted_slot, state, advance=lengths_by_device)
+            if self.limits is None:
+                tokens = kernels.sample_slots(logits, ctx.wanted_slot, state, advance=lengths_by_device)
+            else:
+                tokens = kernels.sample_slots(logits, ctx.wanted_slot, state, advance=lengths_by_device, limits=self.limits.tables)
             if self.rules is not None:
                 kernels.count_tokens(tokens, ctx.wanted_slot, self.rules.tables)
         if lengths_by_device:
@@ -596,6 +607,12 @@ class ModelRunner:
         captured.launches = cuda_ops.launches - before
         captured.graph = graph
         return logits, tokens
+
+    def forget_captured_steps(self) -> None:
+        """Captured decode steps read the cache's pools where they were: they are captured anew after a ``resize``."""
+        if self._graphs:
+            torch.cuda.synchronize(self.device)            # their last replays have ended
+        self._graphs.clear()
 
     def launches_per_replay(self, batch: int, sampling: bool, feed: bool | None = None) -> int:
         """Kernels one replay of the captured step of this batch size launches (0 if not captured)."""

@@ -1242,6 +1242,34 @@ class CudaOps:
             key.data_ptr(), strides[0], value.data_ptr(), strides[1], slots.data_ptr(), *pool.addresses, rows, pool.kv_heads,
             pool.dim, pool.page_size, pool.block, pool.pages, _code(key.dtype), _raw_stream()), "quantize_kv_write")
 
+    def rope_quantize_kv_write(self, qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, slots: torch.Tensor, pool: QuantizedPool,
+                               num_heads: int, num_kv_heads: int, head_dim: int, write_kv: bool = True) -> torch.Tensor:
+        """``rope_kv_write`` into a pool in 8 bits: q turned by position is returned, keys turned (and rounded to their type) and values
+        are stored by ``quantize_kv_write``."""
+        _need(qkv, "qkv", dims=2)
+        _need(positions, "positions", torch.int32, 1)
+        _need(inv_freq, "inv_freq", torch.float32, 1)
+        _need(slots, "slots", torch.int64, 1)
+        rows, width = qkv.shape[0], num_kv_heads * head_dim
+        if num_kv_heads < 1 or num_heads < 1 or head_dim % 2 or qkv.shape[1] != num_heads * head_dim + 2 * width:
+            raise KernelError(f"qkv rows have {qkv.shape[1]} entries, expected {num_heads * head_dim + 2 * width}, heads of an even size")
+        if inv_freq.shape[0] != head_dim // 2 or positions.shape[0] != rows or slots.shape[0] != rows:
+            raise KernelError("one position and slot per row, head_dim/2 frequencies")
+        if pool.kv_heads != num_kv_heads or pool.dim != head_dim:
+            raise KernelError(f"the pool holds {pool.kv_heads} kv heads of {pool.dim}, expected {num_kv_heads} of {head_dim}")
+        _need_here(qkv=qkv, positions=positions, inv_freq=inv_freq, slots=slots, pool=pool)
+        q = qkv.new_empty((rows, num_heads * head_dim))
+        if rows == 0:
+            return q
+        turned = qkv.new_empty((2, rows, width))          # keys, values
+        _check(_declared_library("elementwise").mlr_rope_kv_write(
+            qkv.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), None, q.data_ptr(), turned.data_ptr(),
+            turned.data_ptr() + rows * width * turned.element_size(), rows, num_heads, num_kv_heads, head_dim, 1, int(bool(write_kv)),
+            _code(qkv.dtype), _raw_stream()), "rope_quantize_kv_write")
+        if write_kv:
+            self.quantize_kv_write(turned[0], turned[1], slots, pool)
+        return q
+
     def dequantize_pages(self, pool: QuantizedPool, pages: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
         """What the codes of ``pages`` int32 [n] stand for: keys and values [n, kv_heads, page_size, dim].  A page that the pool does not
         have (-1 in a block table) gives zeros."""

@@ -44,6 +44,7 @@ class PagedAttention(Mixer):
 
 class GQAAttention(PagedAttention):
     supports_norm_fusion = True
+    supports_quantized_cache = True
 
     def __init__(self, spec, compute_dtype):
         super().__init__(spec, compute_dtype)
@@ -112,7 +113,7 @@ class GQAAttention(PagedAttention):
         """The attention kernels' work lists and, where requests of the step share enough leading pages, those of their prefixes."""
         arrays, counts = super().step_plan(host)
         shared = getattr(host, "shared", ())
-        if shared and self.window is None:
+        if shared and self.window is None and not getattr(host, "quantized", False):
             k = ops.current()
             lists, numbers = k.plan_shared_prefix(shared, host.num_segments, self.num_heads // self.num_kv_heads)
             if k.shares_prefix(self.compute_dtype, numbers, self.num_kv_heads, self.head_dim):
@@ -141,6 +142,9 @@ class GQAAttention(PagedAttention):
         qkv = k.linear(x, self.w_qkv, self.b_qkv, rms_eps=self.input_norm_eps if raw_input else None)
         batch = self._batch(ctx, view)
         frequencies = self._no_rotation if self.position is None else self.position.rotary_frequencies()
+        if view.quantized is not None:
+            mixed = self._quantized(qkv, ctx, view, batch, frequencies, writes_cache)
+            return k.linear(mixed, self.w_o, self.b_o, residual=residual)
         prefix = self._shared_prefix(batch, view)
         if prefix is not None:
             if frequencies is not None:
@@ -161,6 +165,16 @@ class GQAAttention(PagedAttention):
             mixed = k.paged_attention(q, view.k_pool, view.v_pool, batch, self.num_heads, self.num_kv_heads,
                                       self.head_dim, self.scale, self.window)
         return k.linear(mixed, self.w_o, self.b_o, residual=residual)
+
+
+    def _quantized(self, qkv, ctx, view, batch, frequencies, writes_cache):
+        """Over a cache in 8 bits: queries and keys are turned, keys and values stored, then attended to."""
+        if frequencies is None:
+            raise ValueError("a cache in 8 bits needs a rotary position encoding or none")
+        k = ops.current()
+        q = k.rope_quantize_kv_write(qkv, ctx.positions, frequencies, view.slots, view.quantized, self.num_heads, self.num_kv_heads,
+                                     self.head_dim, writes_cache)
+        return k.quantized_attention(q, view.quantized, batch, self.num_heads, self.num_kv_heads, self.head_dim, self.scale, self.window)
 
 
 class DifferentialAttention(PagedAttention):

@@ -170,6 +170,8 @@ class Mixer(Part):
     # ``residual=`` in forward: the block may hand it the un-normalised stream (the part applies the
     # row scale inside its first product) and let it add its output into the stream in place.
     supports_norm_fusion = False
+    # A mixer that sets this takes a cache entry whose keys and values are held in 8 bits (``view.quantized``).
+    supports_quantized_cache = False
     # Mixers whose kernels need host-made work lists name them here; mixers with equal keys share
     # one list per step.  The step function calls ``step_plan`` once per key and step, sends the
     # arrays with its own metadata and hands the device copies back in ``ctx.plans[plan_key]``.

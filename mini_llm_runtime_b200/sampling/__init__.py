@@ -1,4 +1,5 @@
+from .limits import RequestLimits
 from .params import GREEDY, SamplingParams
 from .rules import LogitRules
 
-__all__ = ["GREEDY", "LogitRules", "SamplingParams"]
+__all__ = ["GREEDY", "LogitRules", "RequestLimits", "SamplingParams"]

@@ -11,6 +11,9 @@ therefore depend neither on what else is in its batch nor on how its prompt was 
 Beside that a request may carry rules on its logits (sampling/rules.py): penalties for the tokens of its prompt and its output,
 and biases.  A repetition penalty r divides the logit of every known token by r where it is positive and multiplies it by r
 where it is not; frequency and presence penalties are taken off a generated token's logit, once per occurrence and once.
+
+And it may limit what is drawn (sampling/limits.py): the ``top_k`` most probable tokens (0: no limit), the fewest that hold ``top_p`` of
+the probability (1: no limit), those at least ``min_p`` times as probable as the best (0: no limit).
 """
 
 from __future__ import annotations
@@ -31,6 +34,9 @@ class SamplingParams:
     presence_penalty: float = 0.0
     frequency_penalty: float = 0.0
     logit_bias: tuple[tuple[int, float], ...] = ()      # (token, what is added), ascending; a mapping is taken too
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
 
     def __post_init__(self) -> None:
         if isinstance(self.temperature, bool) or not isinstance(self.temperature, (int, float)) \
@@ -61,6 +67,18 @@ class SamplingParams:
         if len({token for token, _ in biases}) != len(biases):
             raise ValueError("logit_bias names a token twice")
         object.__setattr__(self, "logit_bias", biases)
+        if isinstance(self.top_k, bool) or not isinstance(self.top_k, int) or not 0 <= self.top_k < 1 << 31:
+            raise ValueError("top_k must be an integer in [0, 2^31) (0: no limit)")
+        for name, fits, allowed in (("top_p", lambda x: 0.0 < x <= 1.0, "in (0, 1] (1: no limit)"), ("min_p", lambda x: 0.0 <= x <= 1.0, "in [0, 1] (0: no limit)")):
+            value = getattr(self, name)
+            if isinstance(value, bool) or not isinstance(value, (int, float)) or not fits(value):
+                raise ValueError(f"{name} must be a number {allowed}")
+            # the device holds 32 bits; a top_p that rounds to 0 would be none
+            object.__setattr__(self, name, max(float(value), _LEAST_FLOAT32) if name == "top_p" else float(value))
+
+    @property
+    def has_limits(self) -> bool:
+        return (self.top_k, self.top_p, self.min_p) != (0, 1.0, 0.0)
 
     @property
     def greedy(self) -> bool:
