@@ -11,17 +11,21 @@
 // Weights, sums and the places of the cuts are held in 64 bits: a sum of 150,000 weights in 32 bits moves the border between
 // two tokens by 1e-7 of the whole, as much as a token of a flat row is wide a hundred times over.
 //
-// A cluster of CTAs takes a row; each CTA keeps its slice of the row in shared memory, so that the logits are read from memory
-// once.  Logits are compared as whole numbers of the same order (`order_key`).
-//   top-k, min-p   A lower bound of the k-th logit: each thread has met a largest one while it read, and k logits of a slice are as large
-//                  as the k-th of these.  Tokens above it (above min-p's border) are few: they go to the first CTA, which sorts them, cuts,
-//                  sorts what stays by index and draws.
+// A cluster of CTAs takes a row, a slice each, which stays in shared memory where it fits and is read again (from the L2 cache, mostly) where
+// not.  While it is read the largest logits of blocks of 40 are noted: the k-th of them bounds the k-th logit from below, and
+// later passes look only into blocks that reach a bound.
+//   few            Logits above such a bound (top-k up to 1,200), above min-p's border, or, for top-p alone, the thousand largest, if a sample of
+//                  the rest says that they hold p: the whole is then summed in the pass that finds them.  They go to the first CTA
+//                  in the order of the vocabulary; each learns its rank among them, the cut follows, and the draw.
 //   else           The cuts are found together.  All logits are counted in 4,096 bins of T / 128; the CTAs add the bins up through distributed
 //                  shared memory, and the bin that holds the cut is known for top-k, and for top-p but for a bin or two (a bin's weights
 //                  are within a hundredth of one another).  The weights above it are summed, the tokens around it go to the first CTA, which
-//                  sorts them and cuts.  If the cut is not there after all, or more tokens are than one CTA sorts (equal logits, say),
+//                  ranks them and cuts.  If the cut is not there after all, or more tokens are than one CTA ranks (equal logits, say),
 //                  an interval of keys that surely holds it is split eightfold until it is found.  Then the draw: sums by CTA,
-//                  by warp, by part of a warp's stretch, and a walk.
+//                  by warp, by chunk of a warp's stretch, by thread.
+// Bound by memory while no more than a few logits of a row need weights, by 64-bit arithmetic where all do (13 instructions each; the pass of
+// rows without limits runs at half that pipe's rate), by the steps between CTAs for few rows.  256 rows of 152,064 logits, T 0.8: greedy
+// 43 us, top-k 50 71, 1,000 116, top-p 0.9 226, min-p 0.05 58, no limit 121; one row: 7, 12, 20, 28, 10 and 13 us.
 // Sums are taken in a fixed order, of sorted numbers or of places (no floating-point atomics): a row's token depends on its row alone.
 #include <cooperative_groups.h>
 
@@ -31,16 +35,21 @@ namespace mlr {
 
 namespace cg = cooperative_groups;
 
-constexpr int SL_THREADS = 512, SL_WARPS = SL_THREADS / 32;
+constexpr int SL_THREADS = 256, SL_WARPS = SL_THREADS / 32;
 constexpr int SL_BINS = 4096, SL_BINS_PER_THREAD = SL_BINS / SL_THREADS;
 constexpr int SL_BOUND_BINS = 1024;
 constexpr float SL_BINS_PER_T = 128.f;
 constexpr int SL_MOST_K = 1200;          // a top-k whose candidates fit a list, it is likely
+constexpr int SL_NUCLEUS = 1000;         // largest logits among which a top-p is looked for first
 constexpr int SL_LIST = 2048;            // candidates that one CTA cuts and draws from
-constexpr int SL_CUT = 1024;             // keys of an interval that one CTA sorts
+constexpr int SL_CUT = 1024;             // keys of an interval that one CTA orders
+constexpr int SL_EACH = SL_LIST / SL_THREADS;
+constexpr int SL_AHEAD = 10;             // reads of 16 bytes that a thread has in flight while it looks for the largest logit: a block
+constexpr int SL_TOPS = 16;              // largest logits that a thread remembers, of a block each or of some
+constexpr int SL_BUCKETS = 4096, SL_BUCKET_MOST = 64;
 constexpr int SL_PARTS = 8;
 constexpr int SL_MOST_RANKS = 8;
-static_assert(SL_BINS_PER_THREAD == 8, "a thread reads eight bins");
+static_assert(SL_BINS_PER_THREAD % 4 == 0, "a thread reads bins by fours");
 
 struct LimitSource {
   const float* uniforms;          // by row
@@ -60,14 +69,16 @@ struct LimitShared {
   int count;                      // candidates in the list
   double sums[2][SL_PARTS];       // of the parts of an interval, two steps by turns
   int counts[2][SL_PARTS];
-  unsigned cut_key;               // what the first CTA found
+  unsigned key_range[2];
+  float cut_x;                    // what the first CTA found
+  int cut_listed;                 // tokens of the interval that stay, in order in `all_listed`; -1: not there
   int cut_index;
   double kept;
   // of this CTA alone
   double warp_double[SL_WARPS], part_double[SL_PARTS][SL_WARPS];
   float warp_float[SL_WARPS], warp_float2[SL_WARPS];
   int warp_int[SL_WARPS], part_int[SL_PARTS][SL_WARPS];
-  unsigned found_key;
+  float found_x;
   float mark_mass[3];
   int found[2], mark_bin[3], mark_tokens[3];
 };
@@ -86,30 +97,28 @@ __device__ __forceinline__ float of_key(unsigned key) { return __uint_as_float((
 // NaN as -inf, -0 as 0 (they tie)
 __device__ __forceinline__ float cleaned(float x) { return x == x ? x + 0.f : -INFINITY; }
 
-// exp((x - top) / T) in 64 bits by Tang's method (table-driven exponentials, 1989): a = (n + 64 m) ln 2 / 64 + r with |r| < ln 2 / 128,
-// exp a = 2^m 2^(n / 64) (1 + r + r^2 / 2 ..  r^5 / 120); the polynomial's remainder is below 2^-54.  `table` holds 2^(n / 64).
+// exp((x - top) / T) in 64 bits by Tang's method (table-driven exponentials, 1989): (x - top) 16 / (T ln 2) = n + f with n whole and
+// |f| <= 1/2; the weight is 2^(n / 16) (1 + g + g^2 / 2 .. g^6 / 720) with g = f ln 2 / 16, |g| < 0.022: the remainder is below 2^-50.
+// `table` holds 2^(n / 16), sixteen numbers: they fill the banks of shared memory once, so that a warp reads any of them together.
 struct Weights {
-  double inverse, top;
-  float max;
+  double scale, top;
+  float least;                 // weights of logits up to it are below exp(-700), taken as 0
   const double* table;
   __device__ __forceinline__ double operator()(float x) const {
-    if (x == max) return 1.0;
-    if (!(x > -INFINITY)) return 0.0;
-    const double a = ((double)x - top) * inverse;
-    if (!(a > -700.0)) return 0.0;             // (a NaN too: an infinite temperature beside an infinite logit)
     constexpr double RAISE = 6755399441055744.0;      // 1.5 * 2^52
-    const double raised = fma(a, 92.33248261689366, RAISE), whole = raised - RAISE;      // 64 / ln 2
+    constexpr double G = 0.043321698784996581;        // ln 2 / 16
+    const double z = ((double)fminf(x, 3.402823466e38f) - top) * scale;
+    const double raised = z + RAISE, f = z - (raised - RAISE);
     const int n = __double2loint(raised);
-    // ln 2 / 64 in two parts, the first of 21 bits: its product with a whole number is exact
-    double r = fma(whole, -0x1.62e42p-7, a);
-    r = fma(whole, -0x1.fdf473de6af28p-28, r);
-    double q = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-    q = fma(r, q, 1.0 / 6.0);
-    q = fma(r, q, 0.5);
-    q = fma(r, q, 1.0);
-    const double t = table[n & 63];
-    const double value = fma(t, q * r, t);
-    return __hiloint2double(__double2hiint(value) + ((n >> 6) << 20), __double2loint(value));
+    double q = fma(f, G * G * G * G * G * G / 720.0, G * G * G * G * G / 120.0);
+    q = fma(f, q, G * G * G * G / 24.0);
+    q = fma(f, q, G * G * G / 6.0);
+    q = fma(f, q, G * G / 2.0);
+    q = fma(f, q, G);
+    const double t = table[n & 15];
+    const double value = fma(t, f * q, t);
+    const double scaled = __hiloint2double(__double2hiint(value) + ((n >> 4) << 20), __double2loint(value));
+    return x > least ? scaled : 0.0;                 // (0 for a NaN too)
   }
 };
 
@@ -157,13 +166,13 @@ __device__ __forceinline__ V before_block(V v, V* room, V* total, V* until = nul
   return base + (lane > 0 ? previous : (V)0);
 }
 
-// A set of kept tokens: keys above `key`, and of those equal to it the indexes up to `index`.
+// A set of kept tokens: logits above `x`, and of those equal to it the indexes up to `index`.  (NaN, which fills up a slice, is never kept.)
 struct Cut {
-  unsigned key;
+  float x;
   int index;
-  __device__ __forceinline__ bool keeps(unsigned k, int i) const { return k > key || (k == key && i <= index); }
+  __device__ __forceinline__ bool keeps(float other, int i) const { return other > x || (other == x && i <= index); }
   __device__ __forceinline__ void tighten(const Cut& other) {
-    if (other.key > key || (other.key == key && other.index < index)) *this = other;
+    if (other.x > x || (other.x == x && other.index < index)) *this = other;
   }
 };
 
@@ -175,11 +184,11 @@ __device__ __forceinline__ int ties_kept(double above, double w, double target, 
 }
 
 // Rising order by a bitonic network, EACH neighbouring numbers per thread in registers: pairs of a thread, of a warp by shuffles, of
-// further ones through the array itself.  THREADS 32: one warp, which waits for no other.
-template <int EACH, int THREADS>
+// further ones through the array itself.
+template <int EACH>
 __device__ __forceinline__ void sort_in_registers(Place* a, int n) {
-  constexpr int SIZE = EACH * THREADS;
-  const int thread = THREADS == 32 ? (int)(threadIdx.x & 31) : (int)threadIdx.x, first = thread * EACH;
+  constexpr int SIZE = EACH * SL_THREADS;
+  const int first = (int)threadIdx.x * EACH;
   Place v[EACH];
 #pragma unroll
   for (int i = 0; i < EACH; ++i) v[i] = first + i < n ? a[first + i] : ~(Place)0;
@@ -208,33 +217,185 @@ __device__ __forceinline__ void sort_in_registers(Place* a, int n) {
         }
       }
     }
-    if constexpr (EACH == 4) {
-      if (run >= 4) { exchange(v[0], v[2], (first & run) == 0); exchange(v[1], v[3], (first & run) == 0); }
-    }
-    if constexpr (EACH >= 2) {
 #pragma unroll
-      for (int i = 0; i < EACH; i += 2) exchange(v[i], v[i + 1], ((first + i) & run) == 0);
-    }
+    for (int apart = EACH / 2; apart > 0; apart /= 2)
+      if (apart < run)
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+          if ((i & apart) == 0) exchange(v[i], v[i + apart], ((first + i) & run) == 0);
   }
-  if (THREADS == 32) __syncwarp();
-  else __syncthreads();
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < EACH; ++i) a[first + i] = v[i];
 }
 // The array has room up to the next size that is sorted; behind n lie the largest numbers.
 __device__ __noinline__ void sort_places(Place* a, int n) {
   __syncthreads();
-  if (n <= 128) {
-    if (threadIdx.x < 32) sort_in_registers<4, 32>(a, n);
-  } else if (n <= SL_THREADS) {
-    sort_in_registers<1, SL_THREADS>(a, n);
-  } else if (n <= 2 * SL_THREADS) {
-    sort_in_registers<2, SL_THREADS>(a, n);
-  } else {
-    sort_in_registers<4, SL_THREADS>(a, n);
+  if (n <= SL_LIST / 2) sort_in_registers<SL_LIST / 2 / SL_THREADS>(a, n);
+  else sort_in_registers<SL_LIST / SL_THREADS>(a, n);
+  __syncthreads();
+}
+
+// What one thread owns of up to SL_LIST listed tokens: `each` neighbours from `first` on.
+struct Owned {
+  int each, first;
+  __device__ __forceinline__ explicit Owned(int n) : each((n + SL_THREADS - 1) / SL_THREADS), first((int)threadIdx.x * each) {}
+  __device__ __forceinline__ bool has(int i, int n) const { return i < each && first + i < n; }
+};
+// How many of the listed tokens come before each of this thread's own, by the whole CTA.  Up to 256 are compared with one another by several
+// threads each (60 tokens: 0.5 us, where a warp sorted them in 2.4).  More fall into buckets of equal width in [low, high],
+// and are compared with those of their bucket (1,150 tokens: 5 us, sorted 14).  Where a bucket holds too many, a copy is sorted.
+// `buckets` [SL_BUCKETS]; `spare` has room for the next size that is sorted.
+__device__ __noinline__ void ranks_of(Place* listed, int n, float low, float high, unsigned* buckets, Place* spare, int* room, int (&ranks)[SL_EACH]) {
+  const Owned own(n);
+#pragma unroll
+  for (int i = 0; i < SL_EACH; ++i) ranks[i] = 0;
+  if (n <= 256) {
+    int threads = 1;                        // per token
+    while (threads < 32 && n * threads * 2 <= SL_THREADS) threads *= 2;
+    if (threadIdx.x == 0) listed[n] = ~(Place)0;      // pairs
+    __syncthreads();
+    const int token = (int)threadIdx.x / threads, sub = (int)threadIdx.x % threads;
+    const Place me = token < n ? listed[token] : 0;
+    int smaller = 0;
+    for (int j = 2 * sub; j < n; j += 2 * threads) {
+      const ulonglong2 pair = *reinterpret_cast<const ulonglong2*>(listed + j);
+      smaller += (pair.x < me) + (pair.y < me);
+    }
+    for (int apart = 1; apart < threads; apart *= 2) smaller += __shfl_xor_sync(0xffffffffu, smaller, apart);
+    if (sub == 0) buckets[token] = (unsigned)smaller;
+    __syncthreads();
+    if (own.has(0, n)) ranks[0] = (int)buckets[own.first];
+    __syncthreads();
+    return;
+  }
+  const float scale = high > low && low > -INFINITY && high < INFINITY ? (float)SL_BUCKETS / (high - low) : 0.f;
+  for (int b = threadIdx.x; b < SL_BUCKETS / 4; b += SL_THREADS) reinterpret_cast<uint4*>(buckets)[b] = make_uint4(0u, 0u, 0u, 0u);
+  __syncthreads();
+  Place places[SL_EACH];
+  int bucket[SL_EACH], order[SL_EACH];
+#pragma unroll
+  for (int i = 0; i < SL_EACH; ++i) {
+    if (!own.has(i, n)) continue;
+    places[i] = listed[own.first + i];
+    bucket[i] = (int)fminf((high - of_key(key_of(places[i]))) * scale, (float)(SL_BUCKETS - 1));
+    order[i] = (int)atomicAdd(&buckets[bucket[i]], 1u);
+  }
+  __syncthreads();
+  constexpr int MINE = SL_BUCKETS / SL_THREADS;
+  int counts[MINE], here = 0, most = 0, total;
+  int4* my_buckets = reinterpret_cast<int4*>(buckets) + MINE / 4 * threadIdx.x;
+#pragma unroll
+  for (int j = 0; j < MINE; j += 4) {
+    const int4 four = my_buckets[j / 4];
+    counts[j] = four.x, counts[j + 1] = four.y, counts[j + 2] = four.z, counts[j + 3] = four.w;
+  }
+#pragma unroll
+  for (int j = 0; j < MINE; ++j) { here += counts[j]; most = max(most, counts[j]); }
+  const bool crowded = __syncthreads_or(most > SL_BUCKET_MOST);
+  if (crowded) {
+#pragma unroll
+    for (int i = 0; i < SL_EACH; ++i)
+      if (own.has(i, n)) spare[own.first + i] = places[i];
+    sort_places(spare, n);
+#pragma unroll
+    for (int i = 0; i < SL_EACH; ++i) {
+      if (!own.has(i, n)) continue;
+      int from = 0, until = n;
+      while (from < until) {
+        const int middle = (from + until) / 2;
+        if (spare[middle] < places[i]) from = middle + 1;
+        else until = middle;
+      }
+      ranks[i] = from;
+    }
+    __syncthreads();
+    return;
+  }
+  int run = before_block(here, room, &total);
+#pragma unroll
+  for (int j = 0; j < MINE; ++j) { const int count = counts[j]; counts[j] = run; run += count; }
+#pragma unroll
+  for (int j = 0; j < MINE; j += 4) my_buckets[j / 4] = make_int4(counts[j], counts[j + 1], counts[j + 2], counts[j + 3]);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < SL_EACH; ++i)
+    if (own.has(i, n)) spare[buckets[bucket[i]] + order[i]] = places[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < SL_EACH; ++i) {
+    if (!own.has(i, n)) continue;
+    const int begin = (int)buckets[bucket[i]], end = bucket[i] + 1 < SL_BUCKETS ? (int)buckets[bucket[i] + 1] : n;
+    ranks[i] = begin;
+    for (int j = begin; j < end; ++j) ranks[i] += spare[j] < places[i];
   }
   __syncthreads();
 }
+
+// Quads (four neighbouring logits) of a warp's stretch where a slice has at most so many; the blocks of a thread's `tops`, and how many of them.
+__host__ __device__ __forceinline__ int quads_of_warp(int quads) { return (quads + SL_WARPS - 1) / SL_WARPS; }
+__host__ __device__ __forceinline__ int blocks_per_top(int quads) {
+  const int most = 32 * SL_AHEAD * SL_TOPS, per = (quads_of_warp(quads) + most - 1) / most;
+  return per > 1 ? per : 1;
+}
+__host__ __device__ __forceinline__ int tops_of(int quads) {      // (more quads never make it more than SL_TOPS)
+  const int per = blocks_per_top(quads) * 32 * SL_AHEAD;
+  return (quads_of_warp(quads) + per - 1) / per;
+}
+
+constexpr float NOTHING = __builtin_nanf("");
+
+__device__ __noinline__ float4 edge_quad(const float* from, int size, int i) {
+  auto one = [&](int e) { return e >= 0 && e < size ? cleaned(__ldcg(from + e)) : NOTHING; };
+  return make_float4(one(i), one(i + 1), one(i + 2), one(i + 3));
+}
+// A slice of a row by quads: quad q holds the logits 4 q - shift .. 4 q - shift + 3, NaN where these lie outside.
+template <bool RESIDENT>
+struct Slice {
+  const float* from;
+  float4* held;               // in shared memory, once they have been read
+  int shift, size;
+  // from memory: the quads first, first + 32, .. before `end`, NaN from there on; a warp's `first`s are neighbours
+  template <int COUNT>
+  __device__ __forceinline__ void read(int first, int end, float4 (&x)[COUNT]) const {
+    const float4* quads = reinterpret_cast<const float4*>(from - shift);
+    const int inner_begin = shift > 0 ? 1 : 0, inner_end = (size + shift) / 4, until = min(end, inner_end);      // these lie inside as a whole
+    const int lowest = first - (int)(threadIdx.x & 31);
+    if (lowest >= inner_begin && lowest + 32 * COUNT <= until) {
+#pragma unroll
+      for (int j = 0; j < COUNT; ++j) x[j] = __ldcg(quads + first + 32 * j);
+#pragma unroll
+      for (int j = 0; j < COUNT; ++j) x[j] = make_float4(cleaned(x[j].x), cleaned(x[j].y), cleaned(x[j].z), cleaned(x[j].w));
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+      x[j] = make_float4(NOTHING, NOTHING, NOTHING, NOTHING);
+      if (first + 32 * j >= inner_begin && first + 32 * j < until) x[j] = __ldcg(quads + first + 32 * j);
+    }
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j)
+      if (first + 32 * j >= inner_begin && first + 32 * j < until)
+        x[j] = make_float4(cleaned(x[j].x), cleaned(x[j].y), cleaned(x[j].z), cleaned(x[j].w));
+    if (lowest < inner_begin || (end > inner_end && lowest + 32 * COUNT > inner_end)) {      // the slice's first or last quad, in part
+#pragma unroll
+      for (int j = 0; j < COUNT; ++j) {
+        const int q = first + 32 * j;
+        if (q < end && (q < inner_begin || q >= inner_end)) x[j] = edge_quad(from, size, 4 * q - shift);
+      }
+    }
+  }
+  template <int COUNT>
+  __device__ __forceinline__ void get(int first, int end, float4 (&x)[COUNT]) const {
+    if constexpr (RESIDENT) {
+#pragma unroll
+      for (int j = 0; j < COUNT; ++j)
+        x[j] = first + 32 * j < end ? held[first + 32 * j] : make_float4(NOTHING, NOTHING, NOTHING, NOTHING);
+    } else {
+      read(first, end, x);
+    }
+  }
+};
 
 template <bool RESIDENT>
 __global__ void __launch_bounds__(SL_THREADS, 2)
@@ -250,52 +411,42 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
   unsigned* bins = reinterpret_cast<unsigned*>(list + SL_LIST);                  // [SL_BINS]
   Place* all_listed = reinterpret_cast<Place*>(bins);                            // when the bins have been read, the candidates of all CTAs [SL_LIST]
   unsigned* segment = bins + SL_BINS;                                            // [SL_BINS / ranks]
+  float* tops = reinterpret_cast<float*>(segment + SL_BINS / ranks);
+  double (*chunks)[32] = reinterpret_cast<double (*)[32]>(bins);                 // at last, [SL_WARPS][32] sums of a warp's chunks
   __shared__ LimitShared s;
-  __shared__ double table[64];
+  __shared__ double table[16];
   static_assert(SL_LIST * sizeof(Place) <= SL_BINS * sizeof(unsigned), "the candidates lie where the bins were");
 
-  pdl_wait();
-  // ---- the slice and its largest logit
+  // ---- the slice and its largest logits
   const int begin = min(vocab, rank * slice), size = min(vocab, begin + slice) - begin;
   const float* from = logits + (size_t)row * vocab + begin;
-  auto at = [&](int i) -> float {
-    if constexpr (RESIDENT) return held[i];
-    else return cleaned(__ldcg(from + i));
-  };
-  float mine = -INFINITY;      // the largest that this thread met
-  {
-    // 16 bytes at a time where slice and row begin on such boundaries together (a resident slice begins on one)
-    const bool wide = ((uintptr_t)from & 15) == 0;
-    const int pieces = wide ? size / 4 : 0;
-    constexpr int AHEAD = 5;
-    for (int i = threadIdx.x; i < pieces; i += AHEAD * SL_THREADS) {
-      float4 v[AHEAD];
+  // Four logits at a time, from 16-byte boundaries on: quad q holds the slice's logits 4 q - shift .. 4 q - shift + 3, NaN where these lie outside.
+  // A warp looks at neighbouring quads, its stretch, in every pass.
+  const int shift = (int)(((uintptr_t)from >> 2) & 3), quads = size > 0 ? (size + shift + 3) / 4 : 0;
+  const int per_warp = quads_of_warp(quads), quad_begin = min(quads, warp * per_warp), quad_end = min(quads, quad_begin + per_warp);
+  const Slice<RESIDENT> quads_of{from, reinterpret_cast<float4*>(held), shift, size};
+  const int per_top = blocks_per_top(quads), num_tops = tops_of(quads);
+  float* my_tops = tops + threadIdx.x;                   // [num_tops][SL_THREADS]
+  pdl_wait();
+  float mine = -INFINITY, least_top = INFINITY;
+  for (int t = 0; t < num_tops; ++t) {
+    float high = -INFINITY;
+    for (int block = t * per_top; block < (t + 1) * per_top; ++block) {
+      const int q = quad_begin + block * 32 * SL_AHEAD + lane;
+      float4 v[SL_AHEAD];
+      quads_of.read(q, quad_end, v);
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j)
-        if (i + j * SL_THREADS < pieces) v[j] = __ldcg(reinterpret_cast<const float4*>(from) + i + j * SL_THREADS);
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j)
-        if (i + j * SL_THREADS < pieces) {
-          const float4 x = make_float4(cleaned(v[j].x), cleaned(v[j].y), cleaned(v[j].z), cleaned(v[j].w));
-          if constexpr (RESIDENT) reinterpret_cast<float4*>(held)[i + j * SL_THREADS] = x;
-          mine = fmaxf(mine, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)));
-        }
+      for (int j = 0; j < SL_AHEAD; ++j) {
+        if constexpr (RESIDENT)
+          if (q + 32 * j < quad_end) reinterpret_cast<float4*>(held)[q + 32 * j] = v[j];
+        high = fmaxf(high, fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
+      }
     }
-    for (int i = 4 * pieces + threadIdx.x; i < size; i += 4 * SL_THREADS) {
-      float v[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (i + j * SL_THREADS < size) v[j] = __ldcg(from + i + j * SL_THREADS);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (i + j * SL_THREADS < size) {
-          const float x = cleaned(v[j]);
-          if constexpr (RESIDENT) held[i + j * SL_THREADS] = x;
-          mine = fmaxf(mine, x);
-        }
-    }
+    my_tops[t * SL_THREADS] = high;
+    mine = fmaxf(mine, high);
+    if (high > -INFINITY) least_top = fminf(least_top, high);
   }
-  if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 64.0));
+  if (threadIdx.x < 16) table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 16.0));
   // ---- the row's limits
   const int slot = source.row_slot != nullptr ? source.row_slot[row] : row;
   const bool known = slot >= 0 && slot < source.slots;
@@ -315,12 +466,13 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
   if (p <= 0.f) { k = 1; p = 1.f; }
   const bool by_count = !greedy && k > 0 && k < vocab, by_weight = !greedy && p < 1.f;
 
-  // ---- the slice's largest logit, and two of the threads' largest ones: the k-th, and the k / ranks-th.  All slices together hold k logits that
+  // ---- the slice's largest logit, and two of the blocks' largest ones: the k-th, and the k / ranks-th.  All slices together hold k logits that
   // are as large as the least of their k / ranks-th ones, and each holds k as large as its k-th.
   {
-    const float high = warp_max(mine), low = -warp_max(mine > -INFINITY ? -mine : -INFINITY);
+    const float high = warp_max(mine), low = -warp_max(-least_top);
     if (lane == 0) { s.warp_float[warp] = high; s.warp_float2[warp] = low; }
-    const bool bounded = by_count && k <= SL_MOST_K && vocab > SL_LIST;
+    const bool bounded = (by_count ? k <= SL_MOST_K : by_weight) && vocab > SL_LIST;
+    const int wanted = by_count ? k : SL_NUCLEUS;
     if (bounded) for (int b = threadIdx.x; b < SL_BOUND_BINS; b += SL_THREADS) bins[b] = 0u;
     __syncthreads();
     float highest = s.warp_float[0], lowest = s.warp_float2[0];
@@ -333,7 +485,10 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     }
     if (bounded) {
       const float scale = highest > lowest && highest < INFINITY ? (float)(SL_BOUND_BINS - 1) / (highest - lowest) : 0.f;
-      if (mine > -INFINITY) atomicAdd(&bins[scale > 0.f ? min(SL_BOUND_BINS - 1, (int)((highest - mine) * scale)) : 0], 1u);
+      for (int t = 0; t < num_tops; ++t) {
+        const float one = my_tops[t * SL_THREADS];
+        if (one > -INFINITY) atomicAdd(&bins[scale > 0.f ? min(SL_BOUND_BINS - 1, (int)((highest - one) * scale)) : 0], 1u);
+      }
       __syncthreads();
       constexpr int EACH = SL_BOUND_BINS / SL_THREADS;
       int counts[EACH], here = 0, total, until;
@@ -342,8 +497,8 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
       const int before = before_block(here, s.warp_int, &total, &until);
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const int place = m == 0 ? k : (k + ranks - 1) / ranks;
-        if (before < place && until >= place) {      // one thread's (none's where fewer threads met a number)
+        const int place = m == 0 ? wanted : (wanted + ranks - 1) / ranks;
+        if (before < place && until >= place) {      // one thread's (none's where fewer blocks hold a number)
           int run = before, bin = 0;
 #pragma unroll
           for (int j = 0; j < EACH; ++j)
@@ -365,6 +520,54 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
       least = fminf(least, theirs->bounds[1]);
     }
   bound = fmaxf(bound, least);
+  // f(quad, its four logits) for the warp's stretch; f(logit, place in the slice) for those as large as `low`, which threads look for only in
+  // blocks whose largest one is as large.
+  auto for_quads = [&](auto&& f) {
+    if constexpr (RESIDENT) {
+      for (int base = quad_begin; base < quad_end; base += 32) {
+        float4 x[1];
+        quads_of.get(base + lane, quad_end, x);
+        f(base + lane, x[0]);
+      }
+    } else {
+      constexpr int AHEAD = 4;
+      float4 next[AHEAD];
+      quads_of.get(quad_begin + lane, quad_end, next);
+      for (int base = quad_begin; base < quad_end; base += 32 * AHEAD) {
+        float4 x[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) x[j] = next[j];
+        quads_of.get(base + 32 * AHEAD + lane, quad_end, next);      // (while these are looked at)
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+          if (base + 32 * j < quad_end) f(base + 32 * j + lane, x[j]);
+      }
+    }
+  };
+  auto for_high = [&](float low, auto&& f) {
+    constexpr int AHEAD = 5;
+    static_assert(SL_AHEAD % AHEAD == 0, "whole steps of a block");
+    for (int t = 0; t < num_tops; ++t) {
+      const bool look = my_tops[t * SL_THREADS] >= low;
+      if (__ballot_sync(0xffffffffu, look) == 0u) continue;
+      const int end = min(quad_end, quad_begin + (t + 1) * per_top * 32 * SL_AHEAD);
+      for (int q = quad_begin + t * per_top * 32 * SL_AHEAD + lane; q - lane < end; q += 32 * AHEAD) {
+        float4 four[AHEAD];
+        quads_of.get(q, look ? end : 0, four);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+          const float4 x = four[j];
+          if (fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) >= low) {
+            const int i = 4 * (q + 32 * j) - shift;
+            if (x.x >= low) f(x.x, i);
+            if (x.y >= low) f(x.y, i + 1);
+            if (x.z >= low) f(x.z, i + 2);
+            if (x.w >= low) f(x.w, i + 3);
+          }
+        }
+      }
+    }
+  };
   auto finish = [&](int token) {      // by one thread of the cluster
     tokens[row] = token;
     if (record != nullptr) {
@@ -375,8 +578,7 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
   };
   if (greedy || top == -INFINITY) {
     if (top > -INFINITY && s.max == top)      // its first place
-      for (int i = threadIdx.x; i < size; i += SL_THREADS)
-        if (at(i) == top) atomicMin(&s.argmax, begin + i);
+      for_high(top, [&](float, int i) { atomicMin(&s.argmax, begin + i); });
     cluster.sync();
     if (rank == 0 && threadIdx.x == 0) {
       int token = 0x7fffffff;
@@ -387,14 +589,18 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     return;
   }
   Weights weight;
-  weight.inverse = 1.0 / (double)temperature;
-  weight.top = (double)top;
-  weight.max = top;
+  weight.scale = 23.083120654223414 / (double)temperature;      // 16 / ln 2
+  // Logits above the float nearest to top - 700 T are above that number itself; the largest one weighs whatever T is.  An infinite logit
+  // counts as the largest number, and no other beside it.
+  weight.top = (double)fminf(top, 3.402823466e38f);
+  const float next_lower = of_key(order_key(top) - (top == 0.f ? 2u : 1u));      // (-0 is none)
+  weight.least = top < INFINITY ? fminf((float)(weight.top - 700.0 * (double)temperature), next_lower) : next_lower;
   weight.table = table;
   const unsigned top_key = order_key(top), no_key = order_key(-INFINITY);
 
-  // ---- min-p: the lowest key whose weight reaches it
-  Cut kept{0u, 0x7fffffff};
+  // ---- min-p: the lowest logit whose weight reaches it
+  const Cut everything{-INFINITY, 0x7fffffff};
+  Cut kept = everything;
   if (at_least > 0.f) {
     if (threadIdx.x == 0) {
       const double wanted = (double)at_least;
@@ -402,17 +608,17 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
       unsigned key = min(max(order_key(cleaned(guess)), no_key + 1), top_key);
       for (int i = 0; i < 64 && key < top_key && weight(of_key(key)) < wanted; ++i) ++key;
       for (int i = 0; i < 64 && key > no_key + 1 && weight(of_key(key - 1)) >= wanted; ++i) --key;
-      s.found_key = key;
+      s.found_x = of_key(key);
     }
     __syncthreads();
-    kept.key = s.found_key;
+    kept.x = s.found_x;
   }
 
   // counts in bins: those of all CTAs, SL_BINS_PER_THREAD neighbours per thread
   int count[SL_BINS_PER_THREAD];
   const int per = SL_BINS / ranks, first_bin = (int)threadIdx.x * SL_BINS_PER_THREAD;
   auto clear_bins = [&]() {
-    for (int b = threadIdx.x; b < SL_BINS; b += SL_THREADS) bins[b] = 0u;
+    for (int b = threadIdx.x; b < SL_BINS / 4; b += SL_THREADS) reinterpret_cast<uint4*>(bins)[b] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
   };
   auto add_up_bins = [&]() {
@@ -426,21 +632,91 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     }
     cluster.sync();
     const int owner = first_bin / per;
-    const uint4* theirs = reinterpret_cast<const uint4*>(cluster.map_shared_rank(segment, owner) + (first_bin - owner * per));
-    const uint4 low4 = theirs[0], high4 = theirs[1];
-    count[0] = (int)low4.x; count[1] = (int)low4.y; count[2] = (int)low4.z; count[3] = (int)low4.w;
-    count[4] = (int)high4.x; count[5] = (int)high4.y; count[6] = (int)high4.z; count[7] = (int)high4.w;
+    const int4* theirs = reinterpret_cast<const int4*>(cluster.map_shared_rank(segment, owner) + (first_bin - owner * per));
+#pragma unroll
+    for (int j = 0; j < SL_BINS_PER_THREAD; j += 4) {
+      const int4 four = theirs[j / 4];
+      count[j] = four.x, count[j + 1] = four.y, count[j + 2] = four.z, count[j + 3] = four.w;
+    }
   };
-  // tokens of [low, high] in `limit` to this CTA's list, in no order
-  auto collect = [&](unsigned low, unsigned high, Cut limit) {
+  // to this CTA's list, in no order (its length was set to 0 before a barrier)
+  auto append = [&](float x, int i) {
+    const int to = atomicAdd(&s.count, 1);
+    if (to < SL_LIST) list[to] = place_of(order_key(x), begin + i);
+  };
+  auto empty_list = [&]() {
     if (threadIdx.x == 0) s.count = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < size; i += SL_THREADS) {
-      const unsigned key = order_key(at(i));
-      if (key >= low && key <= high && limit.keeps(key, begin + i)) {
-        const int to = atomicAdd(&s.count, 1);
-        if (to < SL_LIST) list[to] = place_of(key, begin + i);
+  };
+  // a warp's quads, from place i on, in order: the wanted ones to list[to ..), no further than list[room)
+  auto put_quad = [&](const float4& x, int i, int& to, int room, auto&& wanted) {
+    const bool a = wanted(x.x, i), b = wanted(x.y, i + 1), c = wanted(x.z, i + 2), d = wanted(x.w, i + 3);
+    const unsigned before = (1u << lane) - 1u;
+    const unsigned as = __ballot_sync(0xffffffffu, a), bs = __ballot_sync(0xffffffffu, b), cs = __ballot_sync(0xffffffffu, c),
+                   ds = __ballot_sync(0xffffffffu, d);
+    int at_place = to + __popc(as & before) + __popc(bs & before) + __popc(cs & before) + __popc(ds & before);
+    auto put = [&](bool in, float one, int place) {
+      if (in) {
+        if (at_place < room) list[at_place] = place_of(order_key(one), begin + place);
+        ++at_place;
       }
+    };
+    put(a, x.x, i), put(b, x.y, i + 1), put(c, x.z, i + 2), put(d, x.w, i + 3);
+    to += __popc(as) + __popc(bs) + __popc(cs) + __popc(ds);
+  };
+  // Each warp has put `found` tokens into a part of the list of its own: these are moved together.  False: a part is full.
+  constexpr int PART = SL_LIST / SL_WARPS;
+  auto pack = [&](int found, int& to, int& all) -> bool {
+    __syncthreads();
+    if (lane == 0) s.warp_int[warp] = found;
+    __syncthreads();
+    all = 0;
+    bool fits = true;
+#pragma unroll
+    for (int w = 0; w < SL_WARPS; ++w) {
+      const int theirs = s.warp_int[w];
+      if (w == warp) to = all;
+      all += theirs;
+      fits = fits && theirs <= PART;
+    }
+    if (threadIdx.x == 0) s.count = all;
+    if (!fits || all > SL_LIST) return false;
+    Place moved[PART / 32];
+#pragma unroll
+    for (int j = 0; j < PART / 32; ++j)
+      if (32 * j + lane < found) moved[j] = list[warp * PART + 32 * j + lane];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PART / 32; ++j)
+      if (32 * j + lane < found) list[to + 32 * j + lane] = moved[j];
+    return true;
+  };
+  // the tokens of [low, high] that `limit` keeps to the list, in the order of the vocabulary
+  auto collect = [&](float low, float high, Cut limit) {
+    auto wanted = [&](float x, int i) { return x >= low && x <= high && limit.keeps(x, begin + i); };
+    // the warp's tokens to list[to ..), no further than list[room); returns how many there are
+    auto find = [&](int to, int room) {
+      const int start = to;
+      for (int block = 0; block < num_tops * per_top; ++block) {
+        const bool look = my_tops[block / per_top * SL_THREADS] >= low;
+        if (__ballot_sync(0xffffffffu, look) == 0u) continue;
+        const int first = quad_begin + block * 32 * SL_AHEAD + lane;
+        float4 v[SL_AHEAD];
+        quads_of.get(first, look ? quad_end : 0, v);
+#pragma unroll
+        for (int j = 0; j < SL_AHEAD; ++j) {
+          const float4 x = v[j];
+          if (__ballot_sync(0xffffffffu, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) >= low) == 0u) continue;
+          put_quad(x, 4 * (first + 32 * j) - shift, to, room, wanted);
+        }
+      }
+      return to - start;
+    };
+    int to = 0, all;
+    const int found = find(warp * PART, (warp + 1) * PART);
+    if (!pack(found, to, all) && all <= SL_LIST) {      // a part is full: all over again, one behind the other
+      __syncthreads();
+      if (found > 0) find(to, SL_LIST);
     }
   };
   auto listed = [&]() {      // by all CTAs, after a barrier of the cluster
@@ -467,56 +743,139 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     __syncthreads();
     return n;
   };
-  constexpr int SL_EACH = SL_LIST / SL_THREADS;
-  // of n sorted tokens the first whose weights, `above` before them, come to `target`
-  auto cut_sorted = [&](int n, double above, double target) -> int {
-    const int each = (n + SL_THREADS - 1) / SL_THREADS, first = threadIdx.x * each;
-    double w[SL_EACH], sum = 0.0, all;
+  // Of n listed tokens the first `stay` in their order have the weights `w`: so many of them, `above` before them, stay until the weights come
+  // to `target`, or to `share` of theirs.
+  auto cut_by_weight = [&](const double (&w)[SL_EACH], const int (&ranks)[SL_EACH], int n, int stay, double above, double target, double share,
+                           double* in_order) -> int {
+    const Owned own(n), sorted(stay);
+#pragma unroll
+    for (int i = 0; i < SL_EACH; ++i)
+      if (own.has(i, n) && ranks[i] < stay) in_order[ranks[i]] = w[i];
+    __syncthreads();
+    double next[SL_EACH], sum = 0.0, all;
 #pragma unroll
     for (int i = 0; i < SL_EACH; ++i) {
-      w[i] = i < each && first + i < n ? weight(of_key(key_of(all_listed[first + i]))) : 0.0;
-      sum += w[i];
+      next[i] = sorted.has(i, stay) ? in_order[sorted.first + i] : 0.0;
+      sum += next[i];
     }
     double run = above + before_block(sum, s.warp_double, &all);
+    if (share > 0.0) target = share * all;
     int passed = 0;          // tokens whose sums stay below the target
 #pragma unroll
     for (int i = 0; i < SL_EACH; ++i) {
-      run += w[i];
-      passed += i < each && first + i < n && run < target;
+      run += next[i];
+      passed += sorted.has(i, stay) && run < target;
     }
-    return min(n, 1 + sum_block(passed, s.warp_int));
+    return min(stay, 1 + sum_block(passed, s.warp_int));
   };
 
-  if ((by_count && k <= SL_MOST_K) || kept.key != 0u || vocab <= SL_LIST) {
-    // ---- few candidates, it is likely
-    const unsigned lowest = max(order_key(bound), kept.key);
-    collect(lowest, 0xffffffffu, kept);
+  int turn = 0;
+  // sums and counts of the parts of all CTAs
+  auto exchange = [&](auto& sums, auto& counts) {
+    constexpr int PARTS = sizeof(counts) / sizeof(int);
+#pragma unroll
+    for (int j = 0; j < PARTS; ++j) {
+      sums[j] = warp_sum64(sums[j]);
+      counts[j] = (int)__reduce_add_sync(0xffffffffu, (unsigned)counts[j]);
+    }
+    if (lane == 0)
+#pragma unroll
+      for (int j = 0; j < PARTS; ++j) { s.part_double[j][warp] = sums[j]; s.part_int[j][warp] = counts[j]; }
+    __syncthreads();
+    if (threadIdx.x < PARTS) {
+      double sum = 0.0;
+      int all = 0;
+      for (int w = 0; w < SL_WARPS; ++w) { sum += s.part_double[threadIdx.x][w]; all += s.part_int[threadIdx.x][w]; }
+      s.sums[turn][threadIdx.x] = sum;
+      s.counts[turn][threadIdx.x] = all;
+    }
     cluster.sync();
+#pragma unroll
+    for (int j = 0; j < PARTS; ++j) {
+      sums[j] = 0.0;
+      counts[j] = 0;
+      for (int c = 0; c < ranks; ++c) {
+        const LimitShared* theirs = cluster.map_shared_rank(&s, c);
+        sums[j] += theirs->sums[turn][j];
+        counts[j] += theirs->counts[turn][j];
+      }
+    }
+    turn ^= 1;
+  };
+  bool few = (by_count && k <= SL_MOST_K) || kept.x > -INFINITY || vocab <= SL_LIST;
+  const float lowest = by_count || !few ? fmaxf(bound, kept.x) : kept.x;
+  double whole = 0.0;              // all weights, where top-p alone is looked for among the largest logits
+  if (few) {
+    collect(lowest, INFINITY, kept);
+    cluster.sync();
+  } else if (by_weight && !by_count && lowest > -INFINITY) {
+    // Do the largest logits hold p of all weights?  Of them the blocks' largest ones are at hand, of the rest some quads are looked at.
+    constexpr int LOOKED_AT = 4;
+    float large = 0.f, rest = 0.f;
+    for (int t = 0; t < num_tops; ++t) {
+      const float one = my_tops[t * SL_THREADS];
+      if (one >= lowest) large += expf((one - top) / temperature);
+    }
+    float4 some[LOOKED_AT];
+    const int apart = (per_warp / LOOKED_AT + 31) / 32 * 32, looked_at = min(LOOKED_AT, (per_warp + max(apart, 1) - 1) / max(apart, 1));
+#pragma unroll
+    for (int j = 0; j < LOOKED_AT; ++j) {
+      float4 x[1] = {make_float4(NOTHING, NOTHING, NOTHING, NOTHING)};
+      if (j < looked_at) quads_of.get(quad_begin + j * apart + lane, quad_end, x);
+      some[j] = x[0];
+    }
+    auto small = [&](float other) { return other < lowest ? expf((other - top) / temperature) : 0.f; };
+#pragma unroll
+    for (int j = 0; j < LOOKED_AT; ++j) rest += (small(some[j].x) + small(some[j].y)) + (small(some[j].z) + small(some[j].w));
+    rest *= (float)per_warp / (float)max(1, min(per_warp, 32 * looked_at));
+    double sums[2] = {(double)large, (double)rest};
+    int counts[2] = {};
+    exchange(sums, counts);
+    if (sums[0] > (double)p * (sums[0] + sums[1])) {
+      // all weights are summed, and the largest logits go to the list
+      int to = warp * PART, moved_to, all;
+      sums[0] = sums[1] = 0.0;
+      for_quads([&](int q, const float4& x) {
+        sums[0] += (weight(x.x) + weight(x.y)) + (weight(x.z) + weight(x.w));
+        if (__ballot_sync(0xffffffffu, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) >= lowest) != 0u)
+          put_quad(x, 4 * q - shift, to, (warp + 1) * PART, [&](float one, int) { return one >= lowest; });
+      });
+      const bool fits = pack(to - warp * PART, moved_to, all);
+      counts[0] = fits ? 0 : 1;             // (each lane's)
+      __syncthreads();
+      if (fits)
+        for (int i = threadIdx.x; i < all; i += SL_THREADS) sums[1] += weight(of_key(key_of(list[i])));
+      exchange(sums, counts);
+      whole = sums[0];
+      few = counts[0] == 0 && sums[1] >= (double)p * whole * (1.0 + 1e-12);
+    }
+  }
+  if (few) {
+    // ---- few candidates, it is likely
     const int found = listed();
     if (found <= SL_LIST) {
       int n = 0;
       if (rank == 0) n = gather(SL_LIST);
       cluster.sync();
       if (rank != 0) return;
-      sort_places(all_listed, n);
-      int stay = by_count ? min(n, k) : n;
-      if (by_weight) {
-        double part = 0.0;
-        for (int i = threadIdx.x; i < stay; i += SL_THREADS) part += weight(of_key(key_of(all_listed[i])));
-        stay = cut_sorted(stay, 0.0, (double)p * sum_block(part, s.warp_double));
+      const Owned own(n);
+      int ranks[SL_EACH], stay = by_count ? min(n, k) : n;
+      Place* spare = reinterpret_cast<Place*>(held);      // (the slice has served)
+      if (by_weight || stay < n) {
+        ranks_of(all_listed, n, lowest, top, reinterpret_cast<unsigned*>(list), spare, s.warp_int, ranks);
+      } else {
+#pragma unroll
+        for (int i = 0; i < SL_EACH; ++i) ranks[i] = 0;
       }
-      // what stays, in the order of the vocabulary: index, key
-      __syncthreads();
-      for (int i = threadIdx.x; i < stay; i += SL_THREADS) {
-        const Place place = all_listed[i];
-        all_listed[i] = ((Place)(unsigned)index_of(place) << 32) | key_of(place);
-      }
-      sort_places(all_listed, stay);
-      const int each = (stay + SL_THREADS - 1) / SL_THREADS, first = threadIdx.x * each;
-      double w[SL_EACH], sum = 0.0, all;
+      double w[SL_EACH];
+#pragma unroll
+      for (int i = 0; i < SL_EACH; ++i)
+        w[i] = own.has(i, n) && ranks[i] < stay ? weight(of_key(key_of(all_listed[own.first + i]))) : 0.0;
+      if (by_weight) stay = cut_by_weight(w, ranks, n, stay, 0.0, (double)p * whole, whole > 0.0 ? 0.0 : (double)p, reinterpret_cast<double*>(spare));
+      double sum = 0.0, all;
 #pragma unroll
       for (int i = 0; i < SL_EACH; ++i) {
-        w[i] = i < each && first + i < stay ? weight(of_key((unsigned)all_listed[first + i])) : 0.0;
+        w[i] = ranks[i] < stay ? w[i] : 0.0;
         sum += w[i];
       }
       double run = before_block(sum, s.warp_double, &all);
@@ -528,75 +887,70 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
       for (int i = 0; i < SL_EACH; ++i) {
         run += w[i];
         if (w[i] > 0.0) {
-          last_kept = first + i;
-          if (run > target && reached == 0x7fffffff) reached = first + i;
+          last_kept = own.first + i;
+          if (run > target && reached == 0x7fffffff) reached = own.first + i;
         }
       }
       if (reached != 0x7fffffff) atomicMin(&s.found[0], reached);
       if (last_kept >= 0) atomicMax(&s.found[1], last_kept);
       __syncthreads();
-      if (threadIdx.x == 0) finish((int)(all_listed[s.found[0] < stay ? s.found[0] : s.found[1]] >> 32));
+      if (threadIdx.x == 0) finish(index_of(all_listed[s.found[0] < n ? s.found[0] : s.found[1]]));
       return;
     }
     cluster.sync();            // the counts have been read
   }
 
   // ---- the cuts are found together
-  // a warp's stretch of the slice
-  const int stretch = ((size + SL_WARPS - 1) / SL_WARPS + 31) / 32 * 32;
-  const int walk_begin = min(size, warp * stretch), walk_end = min(size, walk_begin + stretch);
-  int turn = 0;
-  // sums and counts of the parts of all CTAs
-  auto exchange = [&](double (&sums)[SL_PARTS], int (&counts)[SL_PARTS]) {
-#pragma unroll
-    for (int j = 0; j < SL_PARTS; ++j) {
-      sums[j] = warp_sum64(sums[j]);
-      counts[j] = (int)__reduce_add_sync(0xffffffffu, (unsigned)counts[j]);
-    }
-    if (lane == 0)
-#pragma unroll
-      for (int j = 0; j < SL_PARTS; ++j) { s.part_double[j][warp] = sums[j]; s.part_int[j][warp] = counts[j]; }
-    __syncthreads();
-    if (threadIdx.x < SL_PARTS) {
-      double sum = 0.0;
-      int all = 0;
-      for (int w = 0; w < SL_WARPS; ++w) { sum += s.part_double[threadIdx.x][w]; all += s.part_int[threadIdx.x][w]; }
-      s.sums[turn][threadIdx.x] = sum;
-      s.counts[turn][threadIdx.x] = all;
-    }
-    cluster.sync();
-#pragma unroll
-    for (int j = 0; j < SL_PARTS; ++j) {
-      sums[j] = 0.0;
-      counts[j] = 0;
+  int listed_stay = -1;            // what the last cut keeps of its interval, in the first CTA's list; -1: not there
+  // The cut in [low, high], which holds `inside` kept keys, `above` before them; `ready`: they are in the lists already.
+  auto cut_together = [&](bool weighed, unsigned low, unsigned high, double above, double target, int inside, bool ready) __attribute__((always_inline)) -> Cut {
+    bool whole_interval = true;
+    while (inside > SL_CUT && low < high) {
+      ready = whole_interval = false;
+      // the least and the largest key that it holds: few different ones lie in it where logits were rounded to 16 bits
+      unsigned least_key = 0xffffffffu, most_key = 0u;
+      auto within = [&](float x, int i, auto&& f) {
+        const unsigned key = order_key(x);
+        if (x == x && key >= low && key <= high && kept.keeps(x, begin + i)) f(key);
+      };
+      auto for_each = [&](auto&& f) {
+        for_quads([&](int q, const float4& x) {
+          const int i = 4 * q - shift;
+          f(x.x, i), f(x.y, i + 1), f(x.z, i + 2), f(x.w, i + 3);
+        });
+      };
+      for_each([&](float x, int i) {
+        within(x, i, [&](unsigned key) { least_key = min(least_key, key); most_key = max(most_key, key); });
+      });
+      least_key = __reduce_min_sync(0xffffffffu, least_key);
+      most_key = __reduce_max_sync(0xffffffffu, most_key);
+      if (threadIdx.x == 0) { s.key_range[0] = 0xffffffffu; s.key_range[1] = 0u; }
+      __syncthreads();
+      if (lane == 0) { atomicMin(&s.key_range[0], least_key); atomicMax(&s.key_range[1], most_key); }
+      cluster.sync();
       for (int c = 0; c < ranks; ++c) {
         const LimitShared* theirs = cluster.map_shared_rank(&s, c);
-        sums[j] += theirs->sums[turn][j];
-        counts[j] += theirs->counts[turn][j];
+        least_key = min(least_key, theirs->key_range[0]);
+        most_key = max(most_key, theirs->key_range[1]);
       }
-    }
-    turn ^= 1;
-  };
-  // The cut in [low, high], which holds `inside` kept keys, `above` before them; `ready`: they are in the lists already.
-  auto cut_together = [&](bool weighed, unsigned low, unsigned high, double above, double target, int inside, bool ready) -> Cut {
-    while (inside > SL_CUT && low < high) {
-      ready = false;
+      cluster.sync();
+      low = max(low, least_key);
+      high = min(high, most_key);
+      if (low >= high) { low = high; break; }
       const unsigned step = (high - low) / SL_PARTS + 1;
       double sums[SL_PARTS];
       int counts[SL_PARTS];
 #pragma unroll
       for (int j = 0; j < SL_PARTS; ++j) { sums[j] = 0.0; counts[j] = 0; }
-      for (int i = threadIdx.x; i < size; i += SL_THREADS) {
-        const float x = at(i);
-        const unsigned key = order_key(x);
-        if (key >= low && key <= high && kept.keeps(key, begin + i)) {
+      for_each([&](float x, int i) {
+        within(x, i, [&](unsigned key) {
           const unsigned place = (high - key) / step;
           const double w = weighed ? weight(x) : 1.0;
 #pragma unroll
           for (int j = 0; j < SL_PARTS; ++j)
             if (place == (unsigned)j) { sums[j] += w; counts[j] += 1; }
-        }
-      }
+        });
+      });
       exchange(sums, counts);
       int chosen = 0;
       bool open = true;
@@ -614,31 +968,56 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     }
     if (inside <= SL_CUT) {
       if (!ready) {
-        collect(low, high, kept);
+        // (-0, which no logit is, would take 0 along)
+        collect(of_key(low), of_key(high == 0x7fffffffu ? high - 1u : high), kept);
         cluster.sync();
       }
       if (rank == 0) {
         const int n = gather(SL_CUT);
-        sort_places(all_listed, n);
-        const int stay = weighed ? cut_sorted(n, above, target) : min(n, max(1, (int)(target - above)));
-        if (threadIdx.x == 0) {
-          s.cut_key = n > 0 ? key_of(all_listed[stay - 1]) : low;
-          s.cut_index = n > 0 ? index_of(all_listed[stay - 1]) : 0x7fffffff;
+        const Owned own(n);
+        Place* spare = all_listed + SL_CUT;
+        int ranks[SL_EACH], stay = min(n, max(1, (int)(target - above)));
+        ranks_of(all_listed, n, of_key(low), of_key(high), reinterpret_cast<unsigned*>(list), spare, s.warp_int, ranks);
+        if (weighed) {
+          double w[SL_EACH];
+#pragma unroll
+          for (int i = 0; i < SL_EACH; ++i) w[i] = own.has(i, n) ? weight(of_key(key_of(all_listed[own.first + i]))) : 0.0;
+          stay = cut_by_weight(w, ranks, n, n, above, target, 0.0, reinterpret_cast<double*>(spare));
         }
+        if (threadIdx.x == 0) {
+          s.cut_listed = stay;
+          if (n == 0) { s.cut_x = of_key(low); s.cut_index = 0x7fffffff; }
+        }
+        Place places[SL_EACH];
+#pragma unroll
+        for (int i = 0; i < SL_EACH; ++i)
+          if (own.has(i, n)) places[i] = all_listed[own.first + i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < SL_EACH; ++i)
+          if (own.has(i, n)) {
+            all_listed[ranks[i]] = places[i];
+            if (ranks[i] == stay - 1) {
+              s.cut_x = of_key(key_of(places[i]));
+              s.cut_index = index_of(places[i]);
+            }
+          }
       }
       cluster.sync();
       const LimitShared* first = cluster.map_shared_rank(&s, 0);
-      const Cut cut{first->cut_key, first->cut_index};
+      const Cut cut{first->cut_x, first->cut_index};
+      listed_stay = whole_interval ? first->cut_listed : -1;
       cluster.sync();
       return cut;
     }
+    listed_stay = -1;
     // more equal keys than a CTA sorts: the index of the last one that stays, by counting
-    const int stay = weighed ? ties_kept(above, weight(of_key(low)), target, inside) : min(inside, max(1, (int)(target - above)));
+    const float low_x = of_key(low);
+    const int stay = weighed ? ties_kept(above, weight(low_x), target, inside) : min(inside, max(1, (int)(target - above)));
+    auto tie = [&](float x, int i) { return x == low_x && kept.keeps(x, begin + i); };
     int here = 0;
-    for (int base = walk_begin; base < walk_end; base += 32) {
-      const int i = base + lane;
-      here += __popc(__ballot_sync(0xffffffffu, i < walk_end && order_key(at(i)) == low && kept.keeps(low, begin + i)));
-    }
+    for_high(low_x, [&](float x, int i) { here += tie(x, i); });
+    here = (int)__reduce_add_sync(0xffffffffu, (unsigned)here);
     __syncthreads();
     if (lane == 0) s.warp_int[warp] = here;
     __syncthreads();
@@ -652,16 +1031,30 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     int place = 0;
     for (int c = 0; c < rank; ++c) place += cluster.map_shared_rank(&s, c)->count;
     for (int w = 0; w < warp; ++w) place += s.warp_int[w];
-    if (place < stay && stay <= place + here)
-      for (int base = walk_begin; base < walk_end; base += 32) {
-        const int i = base + lane;
-        const bool in = i < walk_end && order_key(at(i)) == low && kept.keeps(low, begin + i);
-        const unsigned mask = __ballot_sync(0xffffffffu, in);
-        if (in && place + __popc(mask & ((2u << lane) - 1u)) == stay) s.cut_index = begin + i;
-        place += __popc(mask);
+    if (place < stay && stay <= place + here)      // this warp's, which looks again, in the order of the vocabulary
+      for (int base = quad_begin; base < quad_end; base += 32 * SL_AHEAD) {
+        float4 v[SL_AHEAD];
+        quads_of.get(base + lane, quad_end, v);
+#pragma unroll
+        for (int j = 0; j < SL_AHEAD; ++j) {
+          const int i = 4 * (base + 32 * j + lane) - shift;
+          const bool in[4] = {tie(v[j].x, i), tie(v[j].y, i + 1), tie(v[j].z, i + 2), tie(v[j].w, i + 3)};
+          int before = place;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const unsigned mask = __ballot_sync(0xffffffffu, in[e]);
+            before += __popc(mask & ((1u << lane) - 1u));
+            place += __popc(mask);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            before += in[e];
+            if (in[e] && before == stay) s.cut_index = begin + i + e;
+          }
+        }
       }
     cluster.sync();
-    Cut cut{low, 0x7fffffff};
+    Cut cut{low_x, 0x7fffffff};
     for (int c = 0; c < ranks; ++c) {
       const int found = cluster.map_shared_rank(&s, c)->cut_index;
       if (found >= 0) cut.index = found;
@@ -674,14 +1067,18 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
   const float bin_scale = SL_BINS_PER_T / temperature;
   if (by_count || by_weight) {
     clear_bins();
-    for (int i = threadIdx.x; i < size; i += SL_THREADS)
-      atomicAdd(&bins[(int)fminf((top - at(i)) * bin_scale, (float)(SL_BINS - 1))], 1u);      // (infinity times zero: bin 0)
+    // (with 2^23 added without rounding up, the whole number stands in the low bits; NaN from infinities goes to the last bin)
+    auto count_one = [&](float x) {
+      const unsigned bin = __float_as_uint(__fadd_rz(fminf((top - x) * bin_scale, (float)(SL_BINS - 1)), 8388608.f)) & (2 * SL_BINS - 1);
+      if (x == x) atomicAdd(&bins[bin], 1u);
+    };
+    for_quads([&](int, const float4& x) { count_one(x.x), count_one(x.y), count_one(x.z), count_one(x.w); });
     add_up_bins();
   }
-  // keys that surely lie below a bin's beginning (all above: the first bin's)
-  auto key_below = [&](float bin) { return bin >= (float)(SL_BINS - 1) ? 0u : order_key(cleaned(top - bin / bin_scale)); };
+  // a logit that surely lies below a bin's beginning
+  auto below_bin = [&](float bin) { return bin >= (float)(SL_BINS - 1) ? -INFINITY : cleaned(top - bin / bin_scale); };
   double certain = 0.0;            // of this warp's stretch: weights that stay whatever the cut of the weights
-  unsigned open_low = 0u, open_high = top_key;      // keys that it lies among
+  float open_low = -INFINITY, open_high = top;      // logits that it lies among
   bool summed = false;
   if (by_count) {
     int here = 0, total, until;
@@ -697,22 +1094,25 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     }
     __syncthreads();
     const int bin = s.found[0];
-    const unsigned low = key_below((float)bin + 1.01f), high = bin == 0 ? top_key : key_below((float)bin - 0.01f);
-    // every key counts, min-p or not: the smaller of the two beginnings stays
+    const float low = below_bin((float)bin + 1.01f), high = bin == 0 ? top : below_bin((float)bin - 0.01f);
+    // every logit counts, min-p or not: the smaller of the two beginnings stays
     const Cut before_k = kept;
-    kept = Cut{0u, 0x7fffffff};
-    double sums[SL_PARTS] = {};
-    int counts[SL_PARTS] = {};
-    collect(low, high, kept);
-    for (int i = threadIdx.x; i < size; i += SL_THREADS) {
-      const unsigned key = order_key(at(i));
-      counts[0] += key > high;
-      counts[1] += key >= low && key <= high;
-    }
+    kept = everything;
+    double sums[2] = {};
+    int counts[2] = {};
+    empty_list();
+    for_high(low, [&](float x, int i) {
+      if (x > high) {
+        counts[0] += 1;
+      } else {
+        counts[1] += 1;
+        append(x, i);
+      }
+    });
     exchange(sums, counts);
     const bool holds = counts[0] < k && counts[0] + counts[1] >= k;
-    const Cut cut = holds ? cut_together(false, low, high, (double)counts[0], (double)k, counts[1], true)
-                          : cut_together(false, 0u, top_key, 0.0, (double)k, vocab, false);
+    const Cut cut = cut_together(false, holds ? order_key(low) : no_key, holds ? order_key(high) : top_key, holds ? (double)counts[0] : 0.0,
+                                 (double)k, holds ? counts[1] : vocab, holds);
     kept = before_k;
     kept.tighten(cut);
   }
@@ -721,7 +1121,7 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     // estimate is off (single large tokens) shows in the exact sums above an interval; with that known the next one is found.
     float mass[SL_BINS_PER_THREAD], here = 0.f, all, until;
     int tokens_here = 0, tokens_all, tokens_until;
-    const int last_bin = kept.key > 0u ? (int)fminf((top - of_key(max(kept.key, no_key))) * bin_scale, (float)(SL_BINS - 1)) : SL_BINS - 1;
+    const int last_bin = (int)fminf((top - kept.x) * bin_scale, (float)(SL_BINS - 1));
 #pragma unroll
     for (int j = 0; j < SL_BINS_PER_THREAD; ++j) {
       mass[j] = count[j] > 0 && first_bin + j <= last_bin ? (float)count[j] * expf(-((float)(first_bin + j) + 0.5f) / SL_BINS_PER_T) : 0.f;
@@ -731,9 +1131,10 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
     const float before = before_block(here, s.warp_float, &all, &until);
     const int tokens_before = before_block(tokens_here, s.warp_int, &tokens_all, &tokens_until);
     float wanted = p * all;
-    Cut cut{0u, 0x7fffffff};
+    double above = 0.0;
+    int inside = vocab;
     bool found = false;
-    double whole = 0.0;
+    whole = 0.0;
     for (int attempt = 0; attempt < 3 && !found; ++attempt) {
       __syncthreads();
       if (threadIdx.x < 3) { s.mark_bin[threadIdx.x] = last_bin; s.mark_mass[threadIdx.x] = all; s.mark_tokens[threadIdx.x] = tokens_all; }
@@ -761,48 +1162,92 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
       __syncthreads();
       float estimate;                        // of what lies above the interval
       if (s.mark_tokens[2] - s.mark_tokens[0] <= SL_CUT) {
-        open_low = key_below((float)s.mark_bin[2] + 1.01f);
-        open_high = s.mark_bin[0] == 0 ? top_key : key_below((float)s.mark_bin[0] - 0.01f);
+        open_low = below_bin((float)s.mark_bin[2] + 1.01f);
+        open_high = s.mark_bin[0] == 0 ? top : below_bin((float)s.mark_bin[0] - 0.01f);
         estimate = s.mark_mass[0];
       } else {
-        open_low = key_below((float)s.mark_bin[1] + 1.25f);
-        open_high = s.mark_bin[1] == 0 ? top_key : key_below((float)s.mark_bin[1] - 0.25f);
+        open_low = below_bin((float)s.mark_bin[1] + 1.25f);
+        open_high = s.mark_bin[1] == 0 ? top : below_bin((float)s.mark_bin[1] - 0.25f);
         estimate = s.mark_mass[1];
       }
-      collect(open_low, open_high, kept);
-      double sums[SL_PARTS] = {};
-      int counts[SL_PARTS] = {};
-      certain = 0.0;
-      for (int i = walk_begin + lane; i < walk_end; i += 32) {
-        const float x = at(i);
-        const unsigned key = order_key(x);
-        if (kept.keeps(key, begin + i)) {
-          const double w = weight(x);
-          if (key > open_high) certain += w;
-          else if (key >= open_low) { sums[1] += w; counts[1] += 1; }
-          else sums[2] += w;
+      empty_list();
+      double sums[3] = {};                   // above the interval, in it, all
+      int counts[3] = {};
+      const bool limited = kept.x > -INFINITY;
+      for_quads([&](int q, float4 x) {
+        const int i = 4 * q - shift;
+        if (limited) {
+          x.x = kept.keeps(x.x, begin + i) ? x.x : NOTHING;
+          x.y = kept.keeps(x.y, begin + i + 1) ? x.y : NOTHING;
+          x.z = kept.keeps(x.z, begin + i + 2) ? x.z : NOTHING;
+          x.w = kept.keeps(x.w, begin + i + 3) ? x.w : NOTHING;
         }
-      }
-      sums[0] = certain;
-      certain = warp_sum64(certain);
+        const double w[4] = {weight(x.x), weight(x.y), weight(x.z), weight(x.w)};
+        sums[2] += (w[0] + w[1]) + (w[2] + w[3]);
+        sums[0] += ((x.x > open_high ? w[0] : 0.0) + (x.y > open_high ? w[1] : 0.0)) + ((x.z > open_high ? w[2] : 0.0) + (x.w > open_high ? w[3] : 0.0));
+        auto in = [&](float one) { return one >= open_low && one <= open_high; };
+        if (in(x.x) || in(x.y) || in(x.z) || in(x.w)) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float one = j == 0 ? x.x : j == 1 ? x.y : j == 2 ? x.z : x.w;
+            if (in(one)) {
+              sums[1] += w[j];
+              counts[1] += 1;
+              append(one, i + j);
+            }
+          }
+        }
+      });
+      certain = warp_sum64(sums[0]);
       exchange(sums, counts);
-      whole = sums[0] + sums[1] + sums[2];
+      whole = sums[2];
       const double target = (double)p * whole;
-      found = sums[0] < target && (sums[0] + sums[1] >= target || open_low == 0u);
-      if (found) cut = cut_together(true, open_low, open_high, sums[0], target, counts[1], true);
+      found = sums[0] < target && (sums[0] + sums[1] >= target || open_low == -INFINITY);
+      above = found ? sums[0] : 0.0;
+      inside = found ? counts[1] : vocab;
       wanted = (float)(target - sums[0]) + estimate;
     }
     summed = found;
-    if (!found) cut = cut_together(true, 0u, top_key, 0.0, (double)p * whole, vocab, false);
-    kept.tighten(cut);
+    kept.tighten(cut_together(true, found ? order_key(open_low) : no_key, found ? order_key(open_high) : top_key, above, (double)p * whole, inside,
+                              found));
   }
 
   // ---- the draw
   double sum = 0.0;
-  for (int i = walk_begin + lane; i < walk_end; i += 32) {
-    const float x = at(i);
-    const unsigned key = order_key(x);
-    if (kept.keeps(key, begin + i) && (!summed || key <= open_high)) sum += weight(x);
+  const int chunk = max(128, ((per_warp + 31) / 32 + 31) / 32 * 32);      // quads: a warp sums its stretch by at most 32 chunks
+  if (summed && listed_stay >= 0) {
+    // the interval's tokens that stay, from the first CTA's list: those of this warp's stretch
+    const Place* theirs = cluster.map_shared_rank(all_listed, 0);
+    for (int i = threadIdx.x; i < listed_stay; i += SL_THREADS) list[i] = theirs[i];
+    __syncthreads();
+    const int low = begin + max(0, 4 * quad_begin - shift), high = begin + min(size, max(0, 4 * quad_end - shift));
+    for (int i = lane; i < listed_stay; i += 32) {
+      const Place place = list[i];
+      if (index_of(place) >= low && index_of(place) < high) sum += weight(of_key(key_of(place)));
+    }
+  } else if (summed) {
+    for_high(kept.x, [&](float x, int i) { if (x <= open_high && kept.keeps(x, begin + i)) sum += weight(x); });
+  } else {
+    double in_chunk = 0.0;
+    int rows_left = chunk / 32, at_chunk = 0;
+    for_quads([&](int q, const float4& x) {
+      const int i = begin + 4 * q - shift;
+      double w[4] = {weight(x.x), weight(x.y), weight(x.z), weight(x.w)};
+      if (kept.x > -INFINITY) {
+        w[0] = kept.keeps(x.x, i) ? w[0] : 0.0;
+        w[1] = kept.keeps(x.y, i + 1) ? w[1] : 0.0;
+        w[2] = kept.keeps(x.z, i + 2) ? w[2] : 0.0;
+        w[3] = kept.keeps(x.w, i + 3) ? w[3] : 0.0;
+      }
+      in_chunk += (w[0] + w[1]) + (w[2] + w[3]);
+      if (--rows_left == 0 || q - lane + 32 >= quad_end) {
+        in_chunk = warp_sum64(in_chunk);
+        if (lane == 0) { chunks[warp][at_chunk] = in_chunk; sum += in_chunk; }
+        in_chunk = 0.0;
+        rows_left = chunk / 32;
+        ++at_chunk;
+      }
+    });
   }
   sum = warp_sum64(sum) + (summed ? certain : 0.0);
   __syncthreads();
@@ -825,47 +1270,85 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
   const double target = (double)u * all;
   // the CTA, then the warp's stretch, then its part, whose sums the draw falls into; what rounding leaves behind the last belongs to it
   if (target >= run && s.kept > 0.0 && (target < run + s.kept || rank == last_rank)) {
-    auto chosen_of = [&](double& so_far) {
+    auto chosen_of = [&](const double* sums, int count, double& so_far) {
       int last = 0, chosen = -1;
-      for (int w = 0; w < SL_WARPS; ++w)
-        if (s.warp_double[w] > 0.0) last = w;
-      for (int w = 0; w < SL_WARPS && chosen < 0; ++w) {
-        if (s.warp_double[w] > 0.0 && (target < so_far + s.warp_double[w] || w == last)) chosen = w;
-        else so_far += s.warp_double[w];
+      for (int w = 0; w < count; ++w)
+        if (sums[w] > 0.0) last = w;
+      for (int w = 0; w < count && chosen < 0; ++w) {
+        if (sums[w] > 0.0 && (target < so_far + sums[w] || w == last)) chosen = w;
+        else so_far += sums[w];
       }
       return max(chosen, 0);
     };
-    const int stretch_begin = min(size, chosen_of(run) * stretch), stretch_end = min(size, stretch_begin + stretch);
-    const int part = ((stretch + SL_WARPS - 1) / SL_WARPS + 31) / 32 * 32;
-    const int part_begin = min(stretch_end, stretch_begin + warp * part), part_end = min(stretch_end, part_begin + part);
-    double in_part = 0.0;
-    for (int i = part_begin + lane; i < part_end; i += 32) {
-      const float x = at(i);
-      if (kept.keeps(order_key(x), begin + i)) in_part += weight(x);
+    const int stretch = chosen_of(s.warp_double, SL_WARPS, run);
+    int part_begin = min(quads, stretch * per_warp), part_end = min(quads, part_begin + per_warp);
+    if (!summed) {
+      part_begin = min(part_end, part_begin + chunk * chosen_of(chunks[stretch], (part_end - part_begin + chunk - 1) / chunk, run));
+      part_end = min(part_end, part_begin + chunk);
     }
-    in_part = warp_sum64(in_part);
-    __syncthreads();
-    if (lane == 0) s.warp_double[warp] = in_part;
-    __syncthreads();
-    if (warp == chosen_of(run)) {
-      int found = -1, last_kept = -1;
-      for (int base = part_begin; base < part_end && found < 0; base += 32) {
-        const int i = base + lane < part_end ? base + lane : -1;
-        const float x = i >= 0 ? at(i) : -INFINITY;
-        const double w = i >= 0 && kept.keeps(order_key(x), begin + i) ? weight(x) : 0.0;
-        double inclusive = w;
+    auto weights_of = [&](int q, const float4& x, double (&w)[4]) {
+      const int i = begin + 4 * q - shift;
+      w[0] = kept.keeps(x.x, i) ? weight(x.x) : 0.0;
+      w[1] = kept.keeps(x.y, i + 1) ? weight(x.y) : 0.0;
+      w[2] = kept.keeps(x.z, i + 2) ? weight(x.z) : 0.0;
+      w[3] = kept.keeps(x.w, i + 3) ? weight(x.w) : 0.0;
+    };
+    constexpr int AHEAD = 4;
+    while (part_end - part_begin > 32 * SL_WARPS) {
+      const int each = (part_end - part_begin + SL_WARPS - 1) / SL_WARPS;
+      const int my_begin = min(part_end, part_begin + warp * each), my_end = min(part_end, my_begin + each);
+      double in_part = 0.0;
+      float4 ahead[AHEAD];
+      quads_of.get(my_begin + lane, my_end, ahead);
+#pragma unroll 1
+      for (int base = my_begin; base < my_end; base += 32) {
+        const float4 x = ahead[0];
+        float4 next[1];
 #pragma unroll
-        for (int offset = 1; offset < 32; offset <<= 1) {
-          const double up = __shfl_up_sync(0xffffffffu, inclusive, offset);
-          if (lane >= offset) inclusive += up;
-        }
-        const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
-        const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && run + inclusive > target);
-        if (some != 0u) last_kept = base + 31 - __clz(some);
-        if (hit != 0u) found = base + __ffs(hit) - 1;
-        run += __shfl_sync(0xffffffffu, inclusive, 31);
+        for (int j = 0; j + 1 < AHEAD; ++j) ahead[j] = ahead[j + 1];
+        quads_of.get(base + 32 * AHEAD + lane, my_end, next);
+        ahead[AHEAD - 1] = next[0];
+        double w[4];
+        weights_of(base + lane, x, w);
+        in_part += (w[0] + w[1]) + (w[2] + w[3]);
       }
-      if (lane == 0) finish(begin + (found >= 0 ? found : max(0, last_kept)));
+      in_part = warp_sum64(in_part);
+      __syncthreads();
+      if (lane == 0) s.warp_double[warp] = in_part;
+      __syncthreads();
+      part_begin = min(part_end, part_begin + chosen_of(s.warp_double, SL_WARPS, run) * each);
+      part_end = min(part_end, part_begin + each);
+    }
+    // a quad per thread: the warp, then its quad and the logit
+    const int q = part_begin + (int)threadIdx.x, i = 4 * q - shift;
+    float4 x[1];
+    quads_of.get(q, part_end, x);
+    double w[4];
+    weights_of(q, x[0], w);
+    const double until[4] = {w[0], w[0] + w[1], (w[0] + w[1]) + w[2], ((w[0] + w[1]) + w[2]) + w[3]};
+    double inclusive = until[3];
+#pragma unroll
+    for (int offset = 1; offset < 32; offset <<= 1) {
+      const double up = __shfl_up_sync(0xffffffffu, inclusive, offset);
+      if (lane >= offset) inclusive += up;
+    }
+    __syncthreads();
+    if (lane == 31) s.warp_double[warp] = inclusive;
+    __syncthreads();
+    if (warp == chosen_of(s.warp_double, SL_WARPS, run)) {
+      const double up = __shfl_up_sync(0xffffffffu, inclusive, 1), before = run + (lane > 0 ? up : 0.0);
+      int found = -1, last_kept = -1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (w[e] > 0.0) {
+          last_kept = i + e;
+          if (found < 0 && before + until[e] > target) found = i + e;
+        }
+      const unsigned some = __ballot_sync(0xffffffffu, last_kept >= 0), hit = __ballot_sync(0xffffffffu, found >= 0);
+      // what rounding leaves behind the last belongs to it
+      const int token = hit != 0u ? __shfl_sync(0xffffffffu, found, __ffs(hit) - 1)
+                                  : __shfl_sync(0xffffffffu, last_kept, some != 0u ? 31 - __clz(some) : 0);
+      if (lane == 0) finish(begin + max(0, token));
     }
   }
   cluster.sync();      // the others may still read this CTA's sum
@@ -886,22 +1369,28 @@ MLR_EXPORT int mlr_sample_limited(const float* logits, const float* uniforms, co
   if (rows == 0) return MLR_OK;
   if (rows < 0 || vocab <= 0 || slots < 0) return MLR_BAD_SIZE;
   if (state == nullptr ? uniforms == nullptr || temperatures == nullptr : row_slot == nullptr) return MLR_BAD_SIZE;
-  if ((long long)rows * SL_MOST_RANKS > 0x7fffffffLL) return MLR_TOO_LARGE;
+  if ((long long)rows * SL_MOST_RANKS > 0x7fffffffLL || vocab > 1 << 30) return MLR_TOO_LARGE;
   const LimitSource source{uniforms, temperatures, top_k, top_p, min_p, row_slot, (SlotState*)state, slots, advance};
-  // CTAs per row: enough that a slice fits twice on an SM, more while the row's CTAs find an SM each
-  constexpr int RESIDENT_MOST = 24 * 1024, LEAST = 2048;
+  // CTAs per row: eight or fewer of at least 2,048 logits while the device holds them at once, two to an SM (a tenth of the SMs lies in no group
+  // that holds a cluster of eight); up to four of 4,096 in any case, as a row of top-p alone has work for them.  256 rows of 152,064 logits
+  // under various limits: 217 us with one each, 145 with two, 119 with four, 138 with eight; 256 of 8,000: 42, 45, 67, 91; 33 of
+  // 152,064: 84, 54, 34, 30.
+  constexpr int LEAST = 2048, USUAL = 4096;
   int ranks = 1;
-  while (ranks < SL_MOST_RANKS && (vocab > ranks * RESIDENT_MOST || (vocab > ranks * LEAST && rows * ranks * 2 <= sm_count()))) ranks *= 2;
-  const int slice = ((vocab + ranks - 1) / ranks + 3) / 4 * 4;
-  const bool resident = slice <= RESIDENT_MOST;
-  const int most = RESIDENT_MOST * 4;
-  const int room = resident ? (slice * 4 + 15) / 16 * 16 : 0;
-  const size_t rest = SL_LIST * sizeof(Place) + SL_BINS * sizeof(unsigned) + SL_BINS / ranks * sizeof(unsigned);
+  while (ranks < SL_MOST_RANKS && ((ranks < 4 && vocab > 2 * ranks * USUAL) || (vocab > ranks * LEAST && (long long)rows * ranks * 2 <= 2LL * sm_count() * 9 / 10)))
+    ranks *= 2;
+  const int slice = ((vocab + ranks - 1) / ranks + 3) / 4 * 4, quads = slice / 4 + 1;
+  const int blocks = (quads_of_warp(quads) + 32 * SL_AHEAD - 1) / (32 * SL_AHEAD), num_tops = blocks < SL_TOPS ? blocks : SL_TOPS;
+  const int rest = (int)(SL_LIST * sizeof(Place) + SL_BINS * sizeof(unsigned) + SL_BINS / ranks * sizeof(unsigned)) + num_tops * SL_THREADS * 4;
+  // The slice stays in shared memory where two CTAs of an SM, or one on an SM of its own, hold theirs; else it is read again, from the L2 cache
+  // as far as that goes.
+  constexpr int TWO = 111 * 1024, ONE = 220 * 1024;
+  const bool resident = (long long)quads * 16 + rest <= ((long long)rows * ranks <= sm_count() ? ONE : TWO);
+  const int room = max(resident ? quads * 16 : 0, (int)(SL_LIST * sizeof(Place)));
   static OncePerDevice once;
   const cudaError_t err = once([&] {
-    const int bytes = most + (int)(SL_LIST * sizeof(Place) + 2 * SL_BINS * sizeof(unsigned));
-    cudaError_t e = cudaFuncSetAttribute(sample_limited_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    return e == cudaSuccess ? cudaFuncSetAttribute(sample_limited_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) : e;
+    const cudaError_t e = cudaFuncSetAttribute(sample_limited_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, ONE);
+    return e == cudaSuccess ? cudaFuncSetAttribute(sample_limited_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, ONE) : e;
   });
   if (err != cudaSuccess) return (int)err;
   auto kernel = resident ? sample_limited_kernel<true> : sample_limited_kernel<false>;

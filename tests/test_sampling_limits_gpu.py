@@ -170,3 +170,35 @@ def test_what_is_refused():
                  lambda: k.sample_slots(logits, slots, torch.zeros((5, 8), dtype=torch.int32, device=DEVICE), limits=limits)):
         with pytest.raises(ops.KernelError):
             call()
+
+
+@pytest.mark.parametrize("rows,vocab", [(300, 50257), (280, 8191), (70, 152065), (20, 1400001)])
+def test_many_rows_on_odd_boundaries(rows, vocab):
+    """One to four CTAs a row, slices that stay in shared memory and such that are read again, rows that begin on no 16-byte boundary."""
+    logits, uniforms = case(rows, vocab, 2.5, rows)
+    limits = [LIMITS[i % len(LIMITS)] for i in range(rows)]
+    got = ops.current().sample_limited(logits, uniforms, limits_of(limits)).tolist()
+    for row in range(0, rows, 3):
+        t, k, p, least = limits[row]
+        want, near = chosen(logits[row], float(uniforms[row]), *(float(torch.tensor(x)) if x is not k else x for x in (t, k, p, least)))
+        assert got[row] == want or near < NEAR, (row, limits[row])
+
+
+@pytest.mark.parametrize("rows", [1, 60])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_logits_rounded_to_16_bits(rows, dtype):
+    """Many equal logits in every place, more than a thousand at a cut."""
+    logits, uniforms = case(rows, 151936, 2.0, 13)
+    logits = logits.to(dtype).float()
+    check(logits, uniforms, [[(1.0, 0, 0.9, 0.0), (1.0, 0, 0.5, 0.0), (0.6, 0, 0.95, 0.0), (1.0, 9000, 0.99, 0.0), (1.0, 0, 0.97, 1e-4)][i % 5] for i in range(rows)])
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_the_likely_tokens_side_by_side(rows):
+    """All in one warp's stretch, in falling and in rising order, and a few far above the rest."""
+    vocab = 100352
+    logits, uniforms = case(rows, vocab, 1.0, 14)
+    falling = torch.sort(logits, dim=1, descending=True).values
+    for kind in (falling, falling.flip(1), torch.cat([falling[:, :6] + 9.0, logits[:, 6:]], 1)):
+        for limits in ((0.8, 1000, 1.0, 0.0), (0.8, 1200, 0.95, 0.0), (0.4, 0, 0.9, 0.0), (0.25, 0, 0.8, 0.0), (0.5, 0, 1.0, 0.05), (1.0, 0, 1.0, 0.0)):
+            check(kind.contiguous(), uniforms, [limits] * rows)
