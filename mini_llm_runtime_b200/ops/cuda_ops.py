@@ -117,8 +117,8 @@ _PROTOTYPES = {
     "attention_quantized_decode": {"mlr_attention_quantized_decode": "pppppp" "ppppp" "iiiiiiiii" "fi" "ppp",
                                    "mlr_attention_quantized_decode_bytes": "iiiiii"},
     "attention_quantized_split": {"mlr_attention_quantized_split": "pppppp" "ppppp" "iiiiiiiii" "fii" "pip"},
-    "attention_quantized_prompt": {"mlr_attention_quantized_prompt": "pppppp" "ppppppp" "iiiiiiiiiiii" "fi" "pppp" "l" "pip",
-                                   "mlr_attention_quantized_prompt_bytes": "iiiiii"},
+    "attention_quantized_prompt": {"mlr_attention_quantized_prompt": "pppppp" "ppppppp" "iiiiiiiiiiii" "fi" "ppp",
+                                   "mlr_attention_quantized_prompt_bytes": "iiiiiiii"},
     "sampling_limits": {"mlr_sample_limited": "pppppppp" "ii" "p" "ii" "p"},
     "attention_quantized": {"mlr_attention_quantized": "pppppp" "ppppppp" "iiiiiiiii" "fip"},
 }
@@ -1316,15 +1316,14 @@ class CudaOps:
         if cores and counts["big"] > 0 and scale > 0:
             # codes to float16 once, then tcgen05 products (scores are ordered before they are scaled: scale > 0)
             library = _declared_library("attention_quantized_prompt")
-            shape = (counts["prompt_tiles"], q.shape[0], num_heads, num_kv_heads, head_dim)
-            prepared = torch.empty(library.mlr_attention_quantized_prompt_bytes(*shape, batch.num_segments), dtype=torch.uint8, device=q.device)
-            space = self._workspace(q.device)
+            longest = int(batch.max_kv_len)
+            prepared = torch.empty(library.mlr_attention_quantized_prompt_bytes(
+                counts["prompt_tiles"], q.shape[0], num_heads, num_kv_heads, head_dim, batch.num_segments, counts["big"], longest),
+                dtype=torch.uint8, device=q.device)
             _check(library.mlr_attention_quantized_prompt(
                 q.data_ptr(), *pool.addresses, out.data_ptr(), plan["big_tile_seg"].data_ptr(), plan["big_tile_row0"].data_ptr(), q_start,
                 batch.seg_q_len.data_ptr(), pos0, table, slot, width, batch.num_segments, counts["big"], counts["prompt_tiles"], q.shape[0], *sizes,
-                int(batch.max_kv_len), prepared.data_ptr(), space["prefill_queue"].data_ptr(), space["error_word"].data_ptr(),
-                space["prefill_scratch"].data_ptr(), space["prefill_scratch"].numel(), space["prefill_counters"].data_ptr(),
-                space["prefill_counters"].numel(), _raw_stream()), "quantized_attention (prompts)")
+                longest, prepared.data_ptr(), self._error_word(q.device).data_ptr(), _raw_stream()), "quantized_attention (prompts)")
             first, rest = rest - decodes, decodes
         if cores and 0 < decodes <= self.QUANTIZED_DECODES:
             longest = int(batch.max_kv_len)

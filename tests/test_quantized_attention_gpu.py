@@ -104,3 +104,36 @@ def test_no_row_and_what_is_refused():
                  lambda: k.quantized_attention(step.q.t().contiguous().t(), step.pool, batch, 14, 2, 64, 0.125)):
         with pytest.raises(ops.KernelError):
             call()
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page,block,dtype", [SHAPES[0], SHAPES[1], SHAPES[6]])
+def test_calls_side_by_side_and_two_graphs(heads, kv_heads, dim, page, block, dtype):
+    """Steps on two streams at once, eager and captured, share no memory of theirs: prompts whose keys are cut into parts beside decoded tokens."""
+    steps = [Step([300, 1, 40, 1], [900 + 500 * i, 700, 100, 1300], heads, kv_heads, dim, page, block, dtype, 20 + i) for i in range(2)]
+    batches = [step.batch() for step in steps]
+    want = [step.run() for step in steps]
+    for step, alone in zip(steps, want):
+        step.check(alone)
+    call = lambda i: ops.current().quantized_attention(steps[i].q, steps[i].pool, batches[i], heads, kv_heads, dim, steps[i].scale)
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    got, graphs, captured = [[], []], [], []
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    for i, stream in enumerate(streams):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            captured.append(call(i))
+        graphs.append(graph)
+    for _ in range(20):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    ops.current().raise_if_device_error()
+    for i in range(2):
+        for one in (*got[i], captured[i]):
+            assert torch.equal(one, want[i])
