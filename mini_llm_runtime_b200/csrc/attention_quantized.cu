@@ -3,8 +3,9 @@
 //
 // k_j = kc_j * ks, v_j = vc_j * vs (ks, vs of j's block); row i of a request sees its keys max(0, p - window + 1) .. p;
 // out = sum softmax(q.k * scale) v, by the running maximum and sum of a softmax, keys in tiles of 32 at absolute
-// positions: a row's result does not depend on how the prompt was cut nor on the rest of the batch.  A key that a row
-// does not see gives it nothing, whatever lies there (an infinite or NaN scale included).
+// positions: a row's result does not depend on how the prompt was cut nor on the rest of the batch (decoded tokens have kernels of
+// their own).  A key that a row does not see gives it nothing, whatever lies there (an infinite or NaN scale included).  Multiply-adds and
+// the reads of shared memory beside them bound it; prompts of bfloat16 with head sizes 64 and 128 go to the tensor cores.
 #include "common.cuh"
 
 namespace mlr {

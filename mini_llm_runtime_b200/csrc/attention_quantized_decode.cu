@@ -8,8 +8,8 @@
 // there after a power of two per head has brought the largest near one.
 //
 // Reading 2 * dim bytes per key and kv head is what bounds it.  A warp takes 16 keys (head size 64: 32) at a time and has three such
-// tiles on their way, by bulk tensor copies of 16 keys into a ring of its own (a copy per 16 bytes and thread into the same ring: 15 %
-// slower, with seven times the instructions of a tile spent on them).  The heads of a group are the narrow side of the
+// tiles on their way, by bulk tensor copies of 16 keys into a ring of its own (a copy per 16 bytes and thread into the same ring
+// spent seven times the instructions of a tile on them: 64 x 8,192 keys 77 us, so 63).  The heads of a group are the narrow side of the
 // products (n = 8), keys and dimensions the wide one:
 //   scores^T [16 keys x 8 heads] = K [16 x dim] Q^T,   out^T [dim x 8 heads] += V^T [dim x 16 keys] P^T
 // The order of the dimensions within a product is free, so a thread reads 16 bytes of a key that are four steps' operands, and 16
@@ -21,6 +21,7 @@
 // The keys of all requests and kv heads form one line that the warps share evenly, whatever the contexts: a warp's share may
 // end one request's keys and begin another's.  Each beginning counts as QD_BEGIN tiles more, about what it costs.  No warp waits for
 // another.  Pairs of a request and a kv head that several warps walk are merged by a second launch, in the order of the warps.
+// 64 requests of up to 8,192 keys, 28 heads of 128 over 4: 59 us (4.7 TB/s); 100 of up to 16,384, 40 over 8: 300 us (5.8 TB/s).
 #include <cuda_fp16.h>
 
 #include "tma.cuh"

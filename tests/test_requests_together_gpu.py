@@ -105,12 +105,13 @@ def test_several_limited_answers_out_of_one_cache(cache, step_ahead):
     assert len({tuple(answer) for answer in got}) > 3
 
 
-def test_pools_that_change_their_size_while_requests_run():
+@pytest.mark.parametrize("step_ahead", [False, True])
+def test_pools_that_change_their_size_while_requests_run(step_ahead):
     config, page = TINY["A"]
     tiny = TinyEngine(config, page, torch.float32, DEVICE)
     prompts = {name: random_prompt(config.vocab_size, n, n) for name, n in (("a", 40), ("b", 17), ("c", 60))}
     for cache in ({}, {"cache_dtype": "int8", "cache_block": 16}):
-        still, moved = engine_of(tiny, page, **cache), engine_of(tiny, page, **cache)
+        still, moved = (engine_of(tiny, page, step_ahead=step_ahead, **cache) for _ in range(2))
         for engine in (still, moved):
             for name, prompt in prompts.items():
                 engine.submit(name, prompt, max_new_tokens=12)
