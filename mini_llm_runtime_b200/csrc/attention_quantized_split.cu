@@ -1,5 +1,5 @@
 // Decoded tokens over keys and values in 8 bits on the CUDA cores in float32: queries of either type, every head size up to 256, every page
-// and block size, any number of query heads per kv head (eight at a time).
+// and block size, any number of query heads per kv head (four or eight at a time).
 //
 //   out = sum_j e^(q.k_j scale - m) v_j / sum_j e^(q.k_j scale - m),  k_j = kc_j ks, v_j = vc_j vs
 // A CTA walks a part of one request's keys for one kv head and up to eight of its query heads, in tiles of 64 keys: every code is read
@@ -7,18 +7,19 @@
 // product times ks, a weight is multiplied by vs).  Scores: a thread per key and a quarter of the heads.  Sums: a thread per four
 // dimensions and a part of the keys, the weights broadcast from shared memory.  Shared-memory reads bound it: a float of a key or
 // value serves two and eight multiply-adds.  Parts are `chunk` keys from absolute positions, whatever else is in the batch; a second
-// launch merges them in order.  24 requests of up to 2,500 keys, 12 heads of 96 over 4, float32: 50 us (1,029 with 16 rows of a prompt's kernel).
+// launch merges them in order.  24 requests of up to 2,500 keys, 12 heads of 96 over 4, float32: 34 us
+// (49 with room for eight heads where four are enough; 1,029 with 16 rows of a prompt's kernel).
 // A key that a row does not see gives it nothing, whatever lies there.
 #include "common.cuh"
 
 namespace mlr {
 
-constexpr int QS_KEYS = 64, QS_THREADS = 256, QS_HEADS = 8;
+constexpr int QS_KEYS = 64, QS_THREADS = 256;
 constexpr int QS_MAX_DIM = 256;
 
 // [part][request][head]: top, sum; outputs behind them
-template <typename T>
-__global__ void __launch_bounds__(QS_THREADS)
+template <typename T, int HEADS>
+__global__ void __launch_bounds__(QS_THREADS, HEADS == 4 ? 3 : 2)
 attention_quantized_split_kernel(const T* q, const int8_t* k_pool, const int8_t* v_pool, const float* k_scales, const float* v_scales,
                                  float2* __restrict__ sums, float* __restrict__ states, const int* __restrict__ decode_seg,
                                  const int* __restrict__ seg_q_start, const int* __restrict__ seg_pos0, const int* __restrict__ block_table,
@@ -26,7 +27,7 @@ attention_quantized_split_kernel(const T* q, const int8_t* k_pool, const int8_t*
                                  int block, int pool_pages, int window, float scale, int chunk) {
   pdl_trigger();
   const int request = blockIdx.y / kv_heads, kv_head = blockIdx.y - request * kv_heads, group = heads / kv_heads;
-  const int head0 = kv_head * group + blockIdx.z * QS_HEADS, mine = min(QS_HEADS, group - (int)blockIdx.z * QS_HEADS);
+  const int head0 = kv_head * group + blockIdx.z * HEADS, mine = min(HEADS, group - (int)blockIdx.z * HEADS);
   const int segment = decode_seg != nullptr ? decode_seg[request] : request, row = seg_q_start[segment], position = seg_pos0[segment];
   const int lowest = window > 0 ? max(0, position - window + 1) : 0;
   const int first_part = lowest / chunk, part = blockIdx.x;
@@ -38,26 +39,26 @@ attention_quantized_split_kernel(const T* q, const int8_t* k_pool, const int8_t*
   extern __shared__ __align__(16) float qs_shared[];
   // rows of `wide` floats: a multiple of four, and of an odd number of them (rows of neighbouring keys start in other banks)
   const int wide = ((dim + 3) / 4 | 1) * 4, quads = (dim + 3) / 4;
-  float* queries = qs_shared;                        // [QS_HEADS][wide]
-  float* keys = queries + QS_HEADS * wide;           // [QS_KEYS][wide]
+  float* queries = qs_shared;                        // [HEADS][wide]
+  float* keys = queries + HEADS * wide;           // [QS_KEYS][wide]
   float* values = keys + QS_KEYS * wide;             // [QS_KEYS][wide]
-  float* weights = values + QS_KEYS * wide;          // [QS_KEYS][QS_HEADS]
-  float* scales = weights + QS_KEYS * QS_HEADS;      // [2][QS_KEYS]
-  float* tops = scales + 2 * QS_KEYS;                // [QS_HEADS]: the maximum, the factor of what came before, the sum
-  float* factors = tops + QS_HEADS;
-  float* totals = factors + QS_HEADS;
+  float* weights = values + QS_KEYS * wide;          // [QS_KEYS][HEADS]
+  float* scales = weights + QS_KEYS * HEADS;      // [2][QS_KEYS]
+  float* tops = scales + 2 * QS_KEYS;                // [HEADS]: the maximum, the factor of what came before, the sum
+  float* factors = tops + HEADS;
+  float* totals = factors + HEADS;
   const int thread = threadIdx.x, lane = thread & 31, warp = thread >> 5, per_page = page_size / block;
 
-  for (int i = thread; i < QS_HEADS * wide; i += QS_THREADS) {
+  for (int i = thread; i < HEADS * wide; i += QS_THREADS) {
     const int h = i / wide, d = i - h * wide;
     queries[i] = h < mine && d < dim ? to_float(q[((size_t)row * heads + head0 + h) * dim + d]) * scale : 0.f;
   }
-  if (thread < QS_HEADS) { tops[thread] = -INFINITY; totals[thread] = 0.f; }
+  if (thread < HEADS) { tops[thread] = -INFINITY; totals[thread] = 0.f; }
   // sums: thread -> four dimensions, of `slices` parts of the keys
   const int slices = QS_THREADS / quads, slice = thread / quads, quad = thread - slice * quads;
-  float4 out[QS_HEADS];
+  float4 out[HEADS];
 #pragma unroll
-  for (int h = 0; h < QS_HEADS; ++h) out[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int h = 0; h < HEADS; ++h) out[h] = make_float4(0.f, 0.f, 0.f, 0.f);
 
   // codes: 16 at a time where rows lie on such boundaries, else one
   const bool wide_rows = dim % 16 == 0 && ((((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0);
@@ -100,35 +101,40 @@ attention_quantized_split_kernel(const T* q, const int8_t* k_pool, const int8_t*
       }
     }
     __syncthreads();
-    // ---- scores: thread -> key, two heads
+    // ---- scores: thread -> key, a quarter of the heads
     {
-      const int j = thread & (QS_KEYS - 1), pair = thread / QS_KEYS;      // four pairs
+      constexpr int EACH = HEADS / 4;
+      const int j = thread & (QS_KEYS - 1), quarter = thread / QS_KEYS;
       const float4* k_row = reinterpret_cast<const float4*>(keys + j * wide);
-      const float4* q_row = reinterpret_cast<const float4*>(queries + 2 * pair * wide);
-      float s[2] = {0.f, 0.f};
-      if (2 * pair < mine) {
+      const float4* q_row = reinterpret_cast<const float4*>(queries + EACH * quarter * wide);
+      float s[EACH] = {};
+      if (EACH * quarter < mine) {
 #pragma unroll 4
         for (int c = 0; c < quads; ++c) {
-          const float4 k = k_row[c], a = q_row[c], b = q_row[wide / 4 + c];
-          s[0] = fmaf(k.x, a.x, fmaf(k.y, a.y, fmaf(k.z, a.z, fmaf(k.w, a.w, s[0]))));
-          s[1] = fmaf(k.x, b.x, fmaf(k.y, b.y, fmaf(k.z, b.z, fmaf(k.w, b.w, s[1]))));
+          const float4 k = k_row[c];
+#pragma unroll
+          for (int h = 0; h < EACH; ++h) {
+            const float4 a = q_row[h * (wide / 4) + c];
+            s[h] = fmaf(k.x, a.x, fmaf(k.y, a.y, fmaf(k.z, a.z, fmaf(k.w, a.w, s[h]))));
+          }
         }
       }
       const bool seen = key0 + j >= begin && key0 + j < end;
       const float ks = scales[j];
-      *reinterpret_cast<float2*>(weights + j * QS_HEADS + 2 * pair) = seen ? make_float2(s[0] * ks, s[1] * ks) : make_float2(-INFINITY, -INFINITY);
+#pragma unroll
+      for (int h = 0; h < EACH; ++h) weights[j * HEADS + EACH * quarter + h] = seen ? s[h] * ks : -INFINITY;
     }
     __syncthreads();
     // ---- maxima and weights: a warp per head
     if (warp < mine) {
-      const float a = weights[lane * QS_HEADS + warp], b = weights[(lane + 32) * QS_HEADS + warp];
+      const float a = weights[lane * HEADS + warp], b = weights[(lane + 32) * HEADS + warp];
       const float before = tops[warp], top = fmaxf(before, warp_max(fmaxf(a, b)));      // (NaN is passed over; its weight is NaN)
       const float base = top == -INFINITY ? 0.f : top;
       const float wa = a == -INFINITY ? 0.f : expf(a - base), wb = b == -INFINITY ? 0.f : expf(b - base);
       const float sum = warp_sum(wa + wb), factor = before == -INFINITY ? 0.f : expf(before - base);
       // a key that is not seen has weight zero, and its value's scale counts for nothing
-      weights[lane * QS_HEADS + warp] = wa == 0.f ? 0.f : wa * scales[QS_KEYS + lane];
-      weights[(lane + 32) * QS_HEADS + warp] = wb == 0.f ? 0.f : wb * scales[QS_KEYS + lane + 32];
+      weights[lane * HEADS + warp] = wa == 0.f ? 0.f : wa * scales[QS_KEYS + lane];
+      weights[(lane + 32) * HEADS + warp] = wb == 0.f ? 0.f : wb * scales[QS_KEYS + lane + 32];
       __syncwarp();
       if (lane == 0) {
         tops[warp] = top;
@@ -140,17 +146,21 @@ attention_quantized_split_kernel(const T* q, const int8_t* k_pool, const int8_t*
     // ---- sums
     if (slice < slices) {
 #pragma unroll
-      for (int h = 0; h < QS_HEADS; ++h)
+      for (int h = 0; h < HEADS; ++h)
         if (h < mine) {
           const float f = factors[h];
           out[h] = make_float4(out[h].x * f, out[h].y * f, out[h].z * f, out[h].w * f);
         }
       for (int j = slice; j < QS_KEYS; j += slices) {
         const float4 v = reinterpret_cast<const float4*>(values + j * wide)[quad];
-        const float4 w0 = *reinterpret_cast<const float4*>(weights + j * QS_HEADS), w1 = *reinterpret_cast<const float4*>(weights + j * QS_HEADS + 4);
-        const float w[QS_HEADS] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+        float w[HEADS];
 #pragma unroll
-        for (int h = 0; h < QS_HEADS; ++h)
+        for (int h = 0; h < HEADS; h += 4) {
+          const float4 four = *reinterpret_cast<const float4*>(weights + j * HEADS + h);
+          w[h] = four.x, w[h + 1] = four.y, w[h + 2] = four.z, w[h + 3] = four.w;
+        }
+#pragma unroll
+        for (int h = 0; h < HEADS; ++h)
           if (h < mine) {
             out[h].x = fmaf(w[h], v.x, out[h].x);
             out[h].y = fmaf(w[h], v.y, out[h].y);
@@ -167,7 +177,7 @@ attention_quantized_split_kernel(const T* q, const int8_t* k_pool, const int8_t*
     if (slice < slices) {
       float4 v = out[0];
 #pragma unroll
-      for (int i = 1; i < QS_HEADS; ++i)
+      for (int i = 1; i < HEADS; ++i)
         if (i == h) v = out[i];
       reinterpret_cast<float4*>(keys)[slice * quads + quad] = v;
     }
@@ -209,22 +219,22 @@ merge_quantized_split_kernel(const float2* sums, const float* states, T* __restr
   }
 }
 
-template <typename T>
+template <typename T, int HEADS>
 static int split_launch(const void* q, const void* k_pool, const void* v_pool, const float* k_scales, const float* v_scales, void* out,
                         const int* decode_seg, const int* seg_q_start, const int* seg_pos0, const int* block_table, const int* seg_slot,
                         int table_width, int requests, int heads, int kv_heads, int dim, int page_size, int block, int pool_pages, int window,
                         float scale, int chunk, int parts, uint8_t* scratch, cudaStream_t stream) {
   const int wide = ((dim + 3) / 4 | 1) * 4, group = heads / kv_heads;
-  auto bytes = [](int w) { return sizeof(float) * ((size_t)(QS_HEADS + 2 * QS_KEYS) * w + QS_KEYS * QS_HEADS + 2 * QS_KEYS + 3 * QS_HEADS); };
+  auto bytes = [](int w) { return sizeof(float) * ((size_t)(HEADS + 2 * QS_KEYS) * w + QS_KEYS * HEADS + 2 * QS_KEYS + 3 * HEADS); };
   static OncePerDevice once;
   const cudaError_t err = once([&] {
-    return cudaFuncSetAttribute(attention_quantized_split_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes(QS_MAX_DIM + 4));
+    return cudaFuncSetAttribute(attention_quantized_split_kernel<T, HEADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes(QS_MAX_DIM + 4));
   });
   if (err != cudaSuccess) return (int)err;
   const size_t states = (size_t)parts * requests * heads;
   float2* sums = (float2*)scratch;
   float* outputs = (float*)(scratch + states * sizeof(float2));
-  launch_kernel(attention_quantized_split_kernel<T>, dim3(parts, requests * kv_heads, (group + QS_HEADS - 1) / QS_HEADS), dim3(QS_THREADS), bytes(wide),
+  launch_kernel(attention_quantized_split_kernel<T, HEADS>, dim3(parts, requests * kv_heads, (group + HEADS - 1) / HEADS), dim3(QS_THREADS), bytes(wide),
                 stream, (const T*)q, (const int8_t*)k_pool, (const int8_t*)v_pool, k_scales, v_scales, sums, outputs, decode_seg, seg_q_start, seg_pos0,
                 block_table, seg_slot, table_width, requests, heads, kv_heads, dim, page_size, block, pool_pages, window, scale, chunk);
   launch_kernel(merge_quantized_split_kernel<T>, dim3(requests * heads), dim3(128), 0, stream, sums, outputs, (T*)out, decode_seg, seg_q_start, seg_pos0,
@@ -252,11 +262,18 @@ MLR_EXPORT int mlr_attention_quantized_split(const void* q, const void* k_pool, 
     return MLR_BAD_SIZE;
   if (dim > QS_MAX_DIM || (long long)requests * kv_heads > 65535 || (long long)requests * heads > 0x7fffffffLL) return MLR_TOO_LARGE;
   if ((uintptr_t)scratch & 15) return MLR_BAD_ALIGNMENT;
-  if (dtype == MLR_F32)
-    return split_launch<float>(q, k_pool, v_pool, k_scales, v_scales, out, decode_seg, seg_q_start, seg_pos0, block_table, seg_slot, table_width, requests,
-                               heads, kv_heads, dim, page_size, block, pool_pages, window, scale, chunk, parts, (uint8_t*)scratch, stream);
-  if (dtype == MLR_BF16)
-    return split_launch<bf16>(q, k_pool, v_pool, k_scales, v_scales, out, decode_seg, seg_q_start, seg_pos0, block_table, seg_slot, table_width, requests,
-                              heads, kv_heads, dim, page_size, block, pool_pages, window, scale, chunk, parts, (uint8_t*)scratch, stream);
+#define MLR_SPLIT(T_, HEADS_)                                                                                                                        \
+  return split_launch<T_, HEADS_>(q, k_pool, v_pool, k_scales, v_scales, out, decode_seg, seg_q_start, seg_pos0, block_table, seg_slot, table_width, \
+                                  requests, heads, kv_heads, dim, page_size, block, pool_pages, window, scale, chunk, parts, (uint8_t*)scratch, stream)
+  const bool few = heads / kv_heads <= 4;
+  if (dtype == MLR_F32) {
+    if (few) MLR_SPLIT(float, 4);
+    MLR_SPLIT(float, 8);
+  }
+  if (dtype == MLR_BF16) {
+    if (few) MLR_SPLIT(bf16, 4);
+    MLR_SPLIT(bf16, 8);
+  }
+#undef MLR_SPLIT
   return MLR_BAD_DTYPE;
 }
