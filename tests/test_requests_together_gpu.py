@@ -218,3 +218,40 @@ def test_refusals_of_what_turns_and_stores():
         with pytest.raises((ops.KernelError, ValueError, TypeError)):
             call(**other)
     assert call(qkv=qkv[:0], positions=positions[:0], slots=slots[:0]).shape == (0, 64)
+
+
+@pytest.mark.parametrize("cache", [{}, {"cache_dtype": "int8"}])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_all_of_it_in_one_engine(cache, dtype):
+    """A shared prefix, a fork of a request that starts with it, a fork of one that has ended, rules and limits beside one another: in float32 each
+    request's tokens are those it gets alone, in bfloat16 all run to their ends."""
+    config, page = TINY["D"]
+    config = dataclasses.replace(config, use_sliding_window=False)
+    tiny = TinyEngine(config, page, dtype, DEVICE)
+    options = {"sampling_limits": True, "logit_rules": True, "max_prefixes": 1, **cache}
+    system = random_prompt(config.vocab_size, 40, 1)
+    drawn = {"temperature": 1.1, "top_k": 25, "top_p": 0.95, "repetition_penalty": 1.2, "logit_bias": {3: -5.0, 5: float("-inf")}}
+    prompts = {"a": system + [7, 8, 9], "b": system + [7, 8, 9], "c": system[:21] + [1, 2], "d": random_prompt(config.vocab_size, 9, 2)}
+    engine = engine_of(tiny, page, **options)
+    assert engine.add_prefix("system", system) == 32
+    engine.submit("d", prompts["d"], max_new_tokens=2, seed=4)
+    engine.submit("a", prompts["a"], max_new_tokens=14, seed=1, prefix="system", **drawn)
+    engine.step()
+    engine.step()
+    engine.submit("b", prompts["b"], max_new_tokens=14, seed=2, fork_of="a", **drawn)
+    engine.submit("c", prompts["c"], max_new_tokens=14, seed=3, fork_of="a", min_p=0.1, temperature=0.9)
+    engine.step()
+    engine.manager.check_consistency()
+    engine.run()
+    engine.runner.check_device()
+    engine.submit("late", prompts["d"] + list(engine.scheduler.get_request("d").generated_token_ids), max_new_tokens=5, seed=5, fork_of="d")
+    engine.run()
+    engine.drop_prefix("system")
+    engine.manager.check_consistency()
+    assert engine.manager.stats().free_pages == (60,)
+    for name, how in (("a", {"seed": 1, **drawn}), ("b", {"seed": 2, **drawn}), ("c", {"seed": 3, "min_p": 0.1, "temperature": 0.9})):
+        got = list(engine.scheduler.get_request(name).generated_token_ids)
+        assert len(got) == 14 and (name == "c" or 5 not in got)
+        if dtype == torch.float32:
+            alone = engine_of(tiny, page, **options)
+            assert got == alone.generate([prompts[name]], max_new_tokens=14, **how)[0], name
