@@ -25,7 +25,7 @@
 //                  by warp, by chunk of a warp's stretch, by thread.
 // Bound by memory while no more than a few logits of a row need weights, by 64-bit arithmetic where all do (13 instructions each; the pass of
 // rows without limits runs at half that pipe's rate), by the steps between CTAs for few rows.  256 rows of 152,064 logits, T 0.8: greedy
-// 43 us, top-k 50 71, 1,000 116, top-p 0.9 226, min-p 0.05 58, no limit 121; one row: 7, 12, 20, 28, 10 and 13 us.
+// 48 us, top-k 50 76, 1,000 122, top-p 0.9 232, min-p 0.05 63, no limit 125, all kinds mixed 104; one row: 6, 11, 20, 29, 10 and 13 us.
 // Sums are taken in a fixed order, of sorted numbers or of places (no floating-point atomics): a row's token depends on its row alone.
 #include <cooperative_groups.h>
 
@@ -46,6 +46,7 @@ constexpr int SL_CUT = 1024;             // keys of an interval that one CTA ord
 constexpr int SL_EACH = SL_LIST / SL_THREADS;
 constexpr int SL_AHEAD = 10;             // reads of 16 bytes that a thread has in flight while it looks for the largest logit: a block
 constexpr int SL_TOPS = 16;              // largest logits that a thread remembers, of a block each or of some
+constexpr int SL_ORDERED = 2048;         // rows that are brought into order
 constexpr int SL_BUCKETS = 4096, SL_BUCKET_MOST = 64;
 constexpr int SL_PARTS = 8;
 constexpr int SL_MOST_RANKS = 8;
@@ -399,11 +400,11 @@ struct Slice {
 
 template <bool RESIDENT>
 __global__ void __launch_bounds__(SL_THREADS, 2)
-sample_limited_kernel(const float* logits, const LimitSource source, int* __restrict__ tokens, int vocab, int slice, int room_bytes) {
+sample_limited_kernel(const float* logits, const LimitSource source, int* __restrict__ tokens, int vocab, int slice, int room_bytes, int ordered_rows) {
   pdl_trigger();
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int row = blockIdx.x / ranks;
+  int row = blockIdx.x / ranks;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   extern __shared__ __align__(16) uint8_t limit_shared[];
   float* held = reinterpret_cast<float*>(limit_shared);                          // the slice
@@ -417,6 +418,35 @@ sample_limited_kernel(const float* logits, const LimitSource source, int* __rest
   __shared__ double table[16];
   static_assert(SL_LIST * sizeof(Place) <= SL_BINS * sizeof(unsigned), "the candidates lie where the bins were");
 
+  if (ordered_rows > 0) {
+    // ---- rows whose weights are all needed take longest, and begin first
+    pdl_wait();
+    constexpr int MOST = SL_ORDERED / SL_THREADS;
+    const int each = (ordered_rows + SL_THREADS - 1) / SL_THREADS, first = (int)threadIdx.x * each;
+    unsigned heavy = 0u;
+#pragma unroll
+    for (int j = 0; j < MOST; ++j)
+      if (j < each && first + j < ordered_rows) {
+        const int slot = source.row_slot != nullptr ? source.row_slot[first + j] : first + j;
+        if (slot >= 0 && slot < source.slots) {
+          const float temperature = source.state != nullptr ? source.state[slot].temperature : source.temperatures[slot];
+          const int k = source.top_k != nullptr ? source.top_k[slot] : 0;
+          const float least = source.min_p != nullptr ? source.min_p[slot] : 0.f;
+          heavy |= (unsigned)(temperature > 0.f && !(k > 0 && k <= SL_MOST_K) && !(least > 0.f)) << j;
+        }
+      }
+    int all, before = before_block(__popc(heavy), s.warp_int, &all);
+    const int place = row;
+#pragma unroll
+    for (int j = 0; j < MOST; ++j)
+      if (j < each && first + j < ordered_rows) {
+        const bool one = heavy >> j & 1u;
+        if ((one ? before : all + first + j - before) == place) s.found[0] = first + j;
+        before += one;
+      }
+    __syncthreads();
+    row = s.found[0];
+  }
   // ---- the slice and its largest logits
   const int begin = min(vocab, rank * slice), size = min(vocab, begin + slice) - begin;
   const float* from = logits + (size_t)row * vocab + begin;
@@ -1373,7 +1403,7 @@ MLR_EXPORT int mlr_sample_limited(const float* logits, const float* uniforms, co
   const LimitSource source{uniforms, temperatures, top_k, top_p, min_p, row_slot, (SlotState*)state, slots, advance};
   // CTAs per row: eight or fewer of at least 2,048 logits while the device holds them at once, two to an SM (a tenth of the SMs lies in no group
   // that holds a cluster of eight); up to four of 4,096 in any case, as a row of top-p alone has work for them.  256 rows of 152,064 logits
-  // under various limits: 217 us with one each, 145 with two, 119 with four, 138 with eight; 256 of 8,000: 42, 45, 67, 91; 33 of
+  // under various limits: 217 us with one each, 145 with two, 119 with four, 138 with eight, in the order they come in; 256 of 8,000: 42, 45, 67, 91; 33 of
   // 152,064: 84, 54, 34, 30.
   constexpr int LEAST = 2048, USUAL = 4096;
   int ranks = 1;
@@ -1393,7 +1423,12 @@ MLR_EXPORT int mlr_sample_limited(const float* logits, const float* uniforms, co
     return e == cudaSuccess ? cudaFuncSetAttribute(sample_limited_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, ONE) : e;
   });
   if (err != cudaSuccess) return (int)err;
+  // Rows that take longest first, where not all are taken at once: 256 rows of 152,064 logits under various limits 99 us, so 118 without; under the same
+  // kind of limits 94, so 88 (looking at all rows costs each CTA 1.5 us).  Short slices gain nothing: 256 rows of 32,000 72, so 72.
+  constexpr int LONG_SLICE = 16384;
+  const bool ordered = (long long)rows * ranks > 2 * sm_count() && rows <= SL_ORDERED && slice >= LONG_SLICE;
   auto kernel = resident ? sample_limited_kernel<true> : sample_limited_kernel<false>;
-  launch_kernel_clustered(kernel, dim3(rows * ranks), dim3(SL_THREADS), room + rest, stream, ranks, logits, source, tokens, vocab, slice, room);
+  launch_kernel_clustered(kernel, dim3(rows * ranks), dim3(SL_THREADS), room + rest, stream, ranks, logits, source, tokens, vocab, slice, room,
+                          ordered ? rows : 0);
   return launch_status();
 }

@@ -202,3 +202,19 @@ def test_the_likely_tokens_side_by_side(rows):
     for kind in (falling, falling.flip(1), torch.cat([falling[:, :6] + 9.0, logits[:, 6:]], 1)):
         for limits in ((0.8, 1000, 1.0, 0.0), (0.8, 1200, 0.95, 0.0), (0.4, 0, 0.9, 0.0), (0.25, 0, 0.8, 0.0), (0.5, 0, 1.0, 0.05), (1.0, 0, 1.0, 0.0)):
             check(kind.contiguous(), uniforms, [limits] * rows)
+
+
+def test_long_rows_in_an_order_of_their_own():
+    """More rows than are taken at once, read by slot: the order in which they are taken changes none of them."""
+    rows, vocab = 110, 81931
+    logits, uniforms = case(rows, vocab, 2.5, 15)
+    limits = [LIMITS[i % len(LIMITS)] for i in range(rows + 7)]
+    slots = torch.randperm(rows + 7, generator=torch.Generator().manual_seed(16))[:rows].to(torch.int32)
+    slots[[3, 50]] = torch.tensor([-1, rows + 7], dtype=torch.int32)
+    tables, k = limits_of(limits), ops.current()
+    got = k.sample_limited(logits, uniforms, tables, slots.to(DEVICE)).tolist()
+    for row, slot in enumerate(slots.tolist()):
+        alone = k.sample_limited(logits[row:row + 1], uniforms[row:row + 1], tables, slots[row:row + 1].to(DEVICE))
+        assert got[row] == int(alone), (row, slot)
+        if row in (3, 50):
+            assert got[row] == int(logits[row].argmax())
