@@ -26,7 +26,8 @@
 // Bound by memory while no more than a few logits of a row need weights, by 64-bit arithmetic where all do (13 instructions each; the pass of
 // rows without limits runs at half that pipe's rate), by the steps between CTAs for few rows.  256 rows of 152,064 logits, T 0.8: greedy
 // 48 us, top-k 50 76, 1,000 122, top-p 0.9 232, min-p 0.05 63, no limit 125, all kinds mixed 104; one row: 6, 11, 20, 29, 10 and 13 us.
-// Sums are taken in a fixed order, of sorted numbers or of places (no floating-point atomics): a row's token depends on its row alone.
+// Sums are taken in a fixed order, of ranks or of places (no floating-point atomics): a row's token depends on its row alone (and, where the draw lies
+// within the last bits of a sum from a border, on how many CTAs a row gets in a batch of this size).
 #include <cooperative_groups.h>
 
 #include "uniform.cuh"
