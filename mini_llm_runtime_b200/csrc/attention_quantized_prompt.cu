@@ -94,7 +94,8 @@ quantized_prompt_prepare_kernel(const bf16* q, const int8_t* k_pool, const int8_
     if (lane == 0) q_factor[pair] = scaled ? __uint_as_float(exponent << 23) : 1.f;
     return;
   }
-  // ---- which segment's tile (the segments' sizes are metadata of the step)
+  // ---- which segment's tile (the segments' sizes are metadata of the step; the call's own memory is not written before the wait: launches
+  // before this one may still use it for a call of their own)
   const int unit = blockIdx.x;
   if (threadIdx.x == 0) found_segment = -1;
   int carried = 0;
@@ -117,10 +118,7 @@ quantized_prompt_prepare_kernel(const bf16* q, const int8_t* k_pool, const int8_
       carried += warp_sums[w];
     }
     const int before = base + inclusive - tiles;
-    if (index < segments) {
-      if (unit / kv_heads >= before && unit / kv_heads < before + tiles) { found_segment = index; found_first = before; }
-      if (unit == 0) seg_tile0[index] = before;
-    }
+    if (index < segments && unit / kv_heads >= before && unit / kv_heads < before + tiles) { found_segment = index; found_first = before; }
   }
   __syncthreads();
   const int segment = found_segment;
@@ -128,6 +126,7 @@ quantized_prompt_prepare_kernel(const bf16* q, const int8_t* k_pool, const int8_
   if (unit == 0)
     for (int i = threadIdx.x; i < control_len; i += QP_PREPARE) control[i] = 0;      // the queue and the counters of the launch that follows
   if (segment < 0) return;                 // a window left fewer tiles than were counted
+  if (unit == found_first * kv_heads && threadIdx.x == 0) seg_tile0[segment] = found_first;      // (read of segments that have tiles)
   const int q_len = seg_q_len[segment], pos0 = seg_pos0[segment];
   const QpSegment mine = qp_segment(q_len, pos0, window);
   const int within = unit - found_first * kv_heads, kv_head = within / mine.tiles, key0 = (mine.base_tile + within - kv_head * mine.tiles) * QP_KEYS;
