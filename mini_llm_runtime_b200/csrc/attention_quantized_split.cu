@@ -54,8 +54,9 @@ attention_quantized_split_kernel(const T* q, const int8_t* k_pool, const int8_t*
     queries[i] = h < mine && d < dim ? to_float(q[((size_t)row * heads + head0 + h) * dim + d]) * scale : 0.f;
   }
   if (thread < HEADS) { tops[thread] = -INFINITY; totals[thread] = 0.f; }
-  // sums: thread -> four dimensions, of `slices` parts of the keys
-  const int slices = QS_THREADS / quads, slice = thread / quads, quad = thread - slice * quads;
+  // sums: thread -> four dimensions, of `slices` parts of the keys (no more than there are keys: at the end `slices` rows of `quads` take the
+  // place of the QS_KEYS rows of `wide` >= 4 quads floats)
+  const int slices = min(QS_THREADS / quads, QS_KEYS), slice = thread / quads, quad = thread - slice * quads;
   float4 out[HEADS];
 #pragma unroll
   for (int h = 0; h < HEADS; ++h) out[h] = make_float4(0.f, 0.f, 0.f, 0.f);

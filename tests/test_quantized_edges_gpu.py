@@ -48,3 +48,15 @@ def test_prompts_of_other_sizes_one_behind_the_other_on_one_stream(heads, kv_hea
     assert 0 < taken[0] <= arena.numel()
     for i, one in got:
         assert torch.equal(one, want[i])
+
+
+@pytest.mark.parametrize("dim", [1, 2, 3, 4, 5, 8, 12])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (4, 1), (3, 1), (10, 2), (9, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_decoded_tokens_of_small_heads(heads, kv_heads, dim, dtype):
+    """Heads of so few dimensions that a thread block has more threads than a tile's keys times a row's pieces."""
+    first = [0, 1, 15, 16, 63, 64, 65, 255, 256, 700]
+    step = Step([1] * len(first), first, heads, kv_heads, dim, 16, 4, dtype, 50 + dim)
+    step.check(step.run())
+    step = Step([5, 1, 30, 1], [0, 70, 40, 600], heads, kv_heads, dim, 16, 16, dtype, 60 + dim)
+    step.check(step.run())
