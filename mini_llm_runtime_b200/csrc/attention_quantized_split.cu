@@ -133,9 +133,10 @@ attention_quantized_split_kernel(const T* q, const int8_t* k_pool, const int8_t*
       const float base = top == -INFINITY ? 0.f : top;
       const float wa = a == -INFINITY ? 0.f : expf(a - base), wb = b == -INFINITY ? 0.f : expf(b - base);
       const float sum = warp_sum(wa + wb), factor = before == -INFINITY ? 0.f : expf(before - base);
-      // a key that is not seen has weight zero, and its value's scale counts for nothing
-      weights[lane * HEADS + warp] = wa == 0.f ? 0.f : wa * scales[QS_KEYS + lane];
-      weights[(lane + 32) * HEADS + warp] = wb == 0.f ? 0.f : wb * scales[QS_KEYS + lane + 32];
+      // a key that is not seen has weight zero, and its value's scale counts for nothing; a seen one's counts however small its weight (NaN stays)
+      auto seen = [&](int j) { return key0 + j >= begin && key0 + j < end; };
+      weights[lane * HEADS + warp] = seen(lane) ? wa * scales[QS_KEYS + lane] : 0.f;
+      weights[(lane + 32) * HEADS + warp] = seen(lane + 32) ? wb * scales[QS_KEYS + lane + 32] : 0.f;
       __syncwarp();
       if (lane == 0) {
         tops[warp] = top;

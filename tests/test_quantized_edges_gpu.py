@@ -60,3 +60,47 @@ def test_decoded_tokens_of_small_heads(heads, kv_heads, dim, dtype):
     step.check(step.run())
     step = Step([5, 1, 30, 1], [0, 70, 40, 600], heads, kv_heads, dim, 16, 16, dtype, 60 + dim)
     step.check(step.run())
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(12, 3, 96, torch.float32), (20, 2, 64, torch.float32), (6, 2, 80, torch.bfloat16),
+                                                      (14, 2, 64, torch.bfloat16), (8, 2, 128, torch.bfloat16), (20, 1, 64, torch.bfloat16)])
+def test_a_value_without_number_counts_however_small_its_weight(heads, kv_heads, dim, dtype):
+    """A seen key whose score lies so far below the others' that its weight is zero, its value's scale NaN: decoded tokens and a prompt's rows."""
+    step = Step([1, 6, 1], [300, 90, 40], heads, kv_heads, dim, 16, 1, dtype, 70)
+    step.q.abs_().clamp_(min=0.5)
+    for i, at in ((0, 150), (1, 20)):
+        page, offset = step.place(i, at + 1)
+        page, offset = int(page[at]), int(offset[at])
+        step.pool.key[page, :, offset] = -127
+        step.pool.key_scales[page, :, offset] = 100.0
+        step.pool.value_scales[page, :, offset] = float("nan")
+    # With a number there, the weight is none: the rows are those of any other number.  In 32 bits to the last bit; the tensor cores' weights
+    # carry the values' scales, of a prompt their largest power of two among 64 keys, which this one's scale is one of: weights in float16
+    # are off by 2^-11 of their contributions, sum p |v| <= 2.1 here (scales up to 2.1 / 127), and, relative to a largest of at least one, by 2^-25
+    # times a value of at most 254 steps of a scale of at most one, for each of n keys; each of the two results by half a step beside that.
+    values, held = [], step.pool.value_scales.clone()
+    for number in (0.0, 1.0):
+        step.pool.value_scales.copy_(torch.where(held.isnan(), number, held))
+        values.append(step.run())
+    assert bool(torch.isfinite(values[0]).all())
+    if dtype == torch.float32 or dim not in (64, 128):
+        assert torch.equal(*values)
+    else:
+        zero, one = values[0].double(), values[1].double()
+        allowed = torch.finfo(dtype).eps * torch.maximum(zero.abs(), one.abs()) + 2 * (2.0 ** -11 * 2.1 + 301 * 2.0 ** -25 * 254)
+        assert bool(((zero - one).abs() <= allowed).all())
+    step.pool.value_scales.copy_(held)
+    got = step.run()
+    assert bool(torch.isnan(got[:7]).all()) and torch.equal(got[7:], values[0][7:])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_places_that_no_key_is_seen_at_give_nothing(dtype):
+    """Beside them in a tile: keys before the window and behind the row, their scales not finite."""
+    step = Step([1, 1], [300, 70], 12, 3, 96, 16, 1, dtype, 71)
+    want = step.run(window=50)
+    for i, seen in ((0, range(251, 301)), (1, range(21, 71))):
+        page, offset = step.place(i, int(step.first[i]) // 16 * 16 + 16)
+        for at in set(range(len(page))) - set(seen):
+            step.pool.value_scales[page[at], :, offset[at]] = float("inf" if at % 2 else "nan")
+    assert torch.equal(step.run(window=50), want)
