@@ -199,7 +199,7 @@ class CacheManager:
             if quantized_block is not None and group.need.value_head_dim != group.need.head_dim:
                 raise ValueError("a cache in 8 bits holds keys and values of one size")
             if allocate_device_memory:
-                self._allocate_pools(group, count)
+                self._take_pools(group, self._new_pools(group, count))
                 if self.device.type == "cuda":
                     group.device_table = torch.full((self.max_requests, self.max_pages_per_request), -1,
                                                     dtype=torch.int32, device=self.device)
@@ -239,15 +239,21 @@ class CacheManager:
         self._step: list[tuple[RequestCache, int]] | None = None
         self._state_backup: tuple[torch.Tensor, dict[int, torch.Tensor]] | None = None
 
-    def _allocate_pools(self, group: CacheGroup, count: int) -> None:
+    def _new_pools(self, group: CacheGroup, count: int) -> list[torch.Tensor]:
+        """Zeros for ``count`` pages, in the order of ``group.pools``."""
         shape = (len(group.entries), count, group.need.num_kv_heads, self.page_size)
         dtype = self.dtype if self.quantized_block is None else torch.int8
-        group.key = torch.zeros((*shape, group.need.head_dim), dtype=dtype, device=self.device)
-        group.value = torch.zeros((*shape, group.need.value_head_dim), dtype=dtype, device=self.device)
+        pools = [torch.zeros((*shape, dim), dtype=dtype, device=self.device) for dim in (group.need.head_dim, group.need.value_head_dim)]
         if self.quantized_block is not None:
             blocks = (*shape[:3], self.page_size // self.quantized_block)
-            group.key_scales, group.value_scales = (torch.zeros(blocks, dtype=torch.float32, device=self.device) for _ in range(2))
-            group.quantized = [ops.QuantizedPool(*pools) for pools in zip(group.key, group.value, group.key_scales, group.value_scales)]
+            pools += [torch.zeros(blocks, dtype=torch.float32, device=self.device) for _ in range(2)]
+        return pools
+
+    def _take_pools(self, group: CacheGroup, pools: list[torch.Tensor]) -> None:
+        quantized = [] if self.quantized_block is None else [ops.QuantizedPool(*entry) for entry in zip(*pools)]
+        group.key, group.value = pools[:2]
+        group.key_scales, group.value_scales = pools[2:] or (None, None)
+        group.quantized = quantized
 
     # ------------------------------------------------------------------ sizing
     def pages_for_lifetime(self, group: CacheGroup, lifetime_tokens: int) -> int:
@@ -669,17 +675,22 @@ class CacheManager:
         return tuple(counts)
 
     def resize(self, num_pages: int | Sequence[int]) -> None:
-        """Pools of another size, between steps: what they hold moves into the lowest pages of the new ones.  Captured steps that read the
-        old ones must not run again (``ModelRunner.forget_captured_steps``)."""
+        """Pools of another size, between steps: what they hold moves into the lowest pages of the new ones.  Old and new ones exist side by side
+        until then; a call that fails, for want of memory say, leaves the cache as it was.  Captured steps that read the old ones must not run
+        again (``ModelRunner.forget_captured_steps``)."""
         if self._step is not None:
             raise RuntimeError("pages move between steps")
-        for group, count in zip(self.groups, self.can_resize(num_pages)):
-            held = sorted(group.allocator.held)
-            before = group.pools
-            if before:
-                self._allocate_pools(group, count)
-                ops.current().copy_pages(before, held, range(len(held)), into=group.pools)
-            self._moved(group, {page: place for place, page in enumerate(held)}, count)
+        counts = self.can_resize(num_pages)
+        held = [sorted(group.allocator.held) for group in self.groups]
+        # everything that may fail comes first: until all new pools exist and hold what the old ones do, the old ones are the cache
+        pools = [self._new_pools(group, count) if group.pools else [] for group, count in zip(self.groups, counts)]
+        for group, pages, new in zip(self.groups, held, pools):
+            if new:
+                ops.current().copy_pages(group.pools, pages, range(len(pages)), into=new)
+        for group, pages, new, count in zip(self.groups, held, pools, counts):
+            if new:
+                self._take_pools(group, new)
+            self._moved(group, {page: place for place, page in enumerate(pages)}, count)
 
     # ------------------------------------------------------------------ views and numbers
     def entry_pools(self, entry: int) -> tuple[torch.Tensor, torch.Tensor, CacheGroup]:
