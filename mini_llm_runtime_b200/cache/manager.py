@@ -268,21 +268,25 @@ class CacheManager:
     def lifetime_pages(self, lifetime_tokens: int) -> tuple[int, ...]:
         return tuple(self.pages_for_lifetime(g, lifetime_tokens) for g in self.groups)
 
-    def can_ever_hold(self, lifetime_tokens: int) -> bool:
+    def can_ever_hold(self, lifetime_tokens: int, pools: Sequence[int] | None = None) -> bool:
+        """``pools``: the groups' pages, if not those that they have."""
         if lifetime_tokens > self.max_tokens_per_request:
             return False
-        return all(n <= g.num_pages for g, n in zip(self.groups, self.lifetime_pages(lifetime_tokens)))
+        pools = [group.num_pages for group in self.groups] if pools is None else pools
+        return all(n <= pages for pages, n in zip(pools, self.lifetime_pages(lifetime_tokens)))
 
-    def can_be_admitted(self, lifetime_tokens: int, prefix: tuple[str, int] | None = None, *, beside: int = 0) -> bool:
+    def can_be_admitted(self, lifetime_tokens: int, prefix: tuple[str, int] | None = None, *, beside: int = 0,
+                        pools: Sequence[int] | None = None) -> bool:
         """Whether a request will find room once the running ones have ended: beside the lasting requests' pages, and ``beside`` more
-        tokens' pages of a further lasting one."""
-        if not self.can_ever_hold(lifetime_tokens):
+        tokens' pages of a further lasting one, in pools of the size that they have or of ``pools`` pages."""
+        pools = [group.num_pages for group in self.groups] if pools is None else pools
+        if not self.can_ever_hold(lifetime_tokens, pools):
             return False
         shared = 0
         if prefix is not None and self.get(prefix[0]).lasting:      # another source's pages are held for this request alone
             shared = prefix[1] // self.page_size
-        return all(count - shared + kept + more <= group.num_pages for group, count, kept, more in zip(
-            self.groups, self.lifetime_pages(lifetime_tokens), self._lasting_pages(), self.lifetime_pages(beside)))
+        return all(count - shared + kept + more <= pages for pages, count, kept, more in zip(
+            pools, self.lifetime_pages(lifetime_tokens), self._lasting_pages(), self.lifetime_pages(beside)))
 
     def _lasting_pages(self) -> tuple[int, ...]:
         return tuple(sum(request.promised[group.index] for request in self._lasting.values()) for group in self.groups)

@@ -212,7 +212,8 @@ class ContinuousBatchEngine:
         counts = manager.can_resize(total_blocks)
         for request_id in self.scheduler.waiting_request_ids:
             request = self.scheduler.get_request(request_id)
-            if any(need > count for need, count in zip(manager.lifetime_pages(request.lifetime_tokens), counts)):
+            named = None if request.prefix is None else (request.prefix, request.shared)
+            if not manager.can_be_admitted(request.lifetime_tokens, named, pools=counts):      # beside the prefixes' pages
                 raise OutOfPages(f"the waiting request {request_id!r} could never be admitted to pools of {counts} pages")
         self.runner.forget_captured_steps()
         manager.resize(counts)

@@ -85,3 +85,48 @@ def test_a_resize_whose_copies_fail_leaves_the_cache_as_it_was(kernels, monkeypa
     m.check_consistency()
     write(m, "a", [8, 9])
     assert held(m, "a")[0] == list(range(1, 10)) and held(m, "c")[0] == [30, 31, 32]
+
+
+# ------------------------------------------------------------------ the engine
+@pytest.fixture
+def tiny():
+    return TinyEngine(*TINY["A"], torch.float32, "cpu")
+
+
+def test_a_size_leaves_waiting_requests_room_beside_the_prefixes(tiny):
+    """A prefix of three pages, a waiting request of five that does not start with it and one of five that does."""
+    engine = engine_of(tiny, total_blocks=20, max_running_requests=1, max_prefixes=1)
+    page = engine.manager.page_size
+    tokens = random_prompt(tiny.config.vocab_size, 3 * page, 1)
+    assert engine.add_prefix("p", tokens) == 3 * page
+    prompts = {"first": random_prompt(tiny.config.vocab_size, 4, 2), "other": random_prompt(tiny.config.vocab_size, 5 * page - 6, 3),
+               "sharing": tokens + random_prompt(tiny.config.vocab_size, 2 * page - 6, 4)}
+    engine.submit("first", prompts["first"], max_new_tokens=3)
+    engine.step()
+    engine.submit("other", prompts["other"], max_new_tokens=6)
+    engine.submit("sharing", prompts["sharing"], max_new_tokens=6, prefix="p")
+    needs = engine.manager.lifetime_pages(engine.scheduler.get_request("other").lifetime_tokens)
+    assert needs == (5,) and engine.manager.can_resize(7) == (7,)
+    for size in (5, 7):
+        with pytest.raises(OutOfPages, match="'other' could never be admitted"):
+            engine.resize_cache(size)
+        assert engine.manager.groups[0].num_pages == 20
+    engine.resize_cache(8)
+    engine.run()
+    for name, prompt in prompts.items():
+        assert list(engine.scheduler.get_request(name).generated_token_ids) == plain.greedy_tokens(
+            tiny.tensors, tiny.config_dict, prompt, 3 if name == "first" else 6), name
+
+
+def test_a_request_that_shares_a_prefix_needs_the_rest_of_its_pages(tiny):
+    engine = engine_of(tiny, total_blocks=20, max_running_requests=1, max_prefixes=1)
+    page = engine.manager.page_size
+    tokens = random_prompt(tiny.config.vocab_size, 3 * page, 1)
+    engine.add_prefix("p", tokens)
+    prompt = tokens + random_prompt(tiny.config.vocab_size, 2 * page - 6, 4)
+    engine.submit("sharing", prompt, max_new_tokens=6, prefix="p")
+    with pytest.raises(OutOfPages):
+        engine.resize_cache(4)
+    engine.resize_cache(5)
+    engine.run()
+    assert list(engine.scheduler.get_request("sharing").generated_token_ids) == plain.greedy_tokens(tiny.tensors, tiny.config_dict, prompt, 6)
