@@ -343,13 +343,16 @@ class CacheManager:
             try:
                 for group in self.groups:
                     tail[group.index] = group.allocator.allocate(1, promised=bool(promised[group.index]))
-            except OutOfPages:
+                    if group.pools:
+                        # stream order: the parent's tokens were written by launches before this one
+                        ops.current().copy_pages(group.pools, [parent.pages[group.index][whole]], tail[group.index])
+            except BaseException as error:
                 for group in self.groups:
                     group.allocator.free(tail[group.index], promised=bool(promised[group.index]))
                     group.allocator.unpromise(promised[group.index])
-                if lifetime_tokens is None:
-                    raise
-                return None                          # others hold, without a promise, what the promise counts on
+                if isinstance(error, OutOfPages) and lifetime_tokens is not None:
+                    return None                      # others hold, without a promise, what the promise counts on
+                raise
         slot = self.slots.allocate(1)[0]
         request = RequestCache(request_id, slot,
                                pages=[[] for _ in self.groups],
@@ -418,9 +421,6 @@ class CacheManager:
             request.pages[index] = parent.pages[index][:whole] + tail[index]
             group.table[request.slot, :len(request.pages[index])] = request.pages[index]
             group.dirty.add(request.slot)
-            if tail[index] and group.pools:
-                # stream order: the parent's tokens were written by launches before this one
-                ops.current().copy_pages(group.pools, [parent.pages[index][whole]], tail[index])
 
     def _hand_over(self, request: RequestCache) -> None:
         """Of the pages that count for the request, those that others hold too count for the next of them."""
