@@ -373,7 +373,11 @@ class RequestScheduler:
             if room <= 0 or (not self.chunked_prefill and len(request.prompt) - request.shared > room):
                 break
             if self.gate is not None:
-                slot = self.gate.admit(request)
+                try:
+                    slot = self.gate.admit(request)
+                except BaseException:      # there will be no plan: those admitted for it go back
+                    self._give_back([self._by_id[item.request_id] for item in items if item.admitted])
+                    raise
                 if slot is None:
                     break
                 request.slot = slot
@@ -449,16 +453,22 @@ class RequestScheduler:
         for request in returned:
             if request.cursor != request.shared or request.output:
                 raise RuntimeError(f"request {request.request_id!r} already has results; its step cannot be aborted")
-        for request in reversed(returned):
+        self._give_back(returned)
+        self._plan = None
+        self._step_index = plan.index
+        return plan
+
+    def _give_back(self, admitted: Sequence[Request]) -> None:
+        """Requests admitted for a plan that does not come about: back to the head of the queue, in their order."""
+        for request in reversed(admitted):
             del self._live[request.request_id]
             if self.gate is not None and request.slot is not None:
                 self.gate.release(request.request_id)
             request.slot = None
             request.status = RequestStatus.WAITING
+            if request.fork is not None:
+                request.shared = request.cursor = 0      # it takes what the other request's cache holds when it is admitted again
             self._queue.appendleft(request)
-        self._plan = None
-        self._step_index = plan.index
-        return plan
 
     def fail_requests(self, request_ids: Collection[str]) -> tuple[str, ...]:
         """End the named requests with ``FinishReason.ERROR`` wherever they are, give their resources
