@@ -34,7 +34,8 @@ window gives pages back and a fixed-size state has none.)
 
 Forks.  A request may also start with any number of tokens of another one (``create_request(..., fork=(request, tokens))``): whole pages are
 held by both, the page it ends in is copied (all layers at once).  Such pages count for the request that held them first; when it ends,
-they count for the next one.  Neither has to outlive the other.
+they count for the next one.  Neither has to outlive the other, and a request may still start with tokens of one that has ended as long as a
+fork of it holds them (``holder_of``).
 
 Moving.  ``compact`` moves pages into the lowest numbers of their pools, ``resize`` into pools of another size.
 
@@ -122,6 +123,7 @@ class RequestCache:
     sharers: int = 0                  # requests that start with pages of this one
     lasting: bool = False             # held until its owner releases it, not until it has run
     borrowed: list[set[int]] = field(default_factory=list)      # per group: pages held since a fork that count for another request
+    begins_as: dict[str, int] = field(default_factory=dict)     # of a fork: a request, ended perhaps, and how many of its first tokens this one began with
 
     def own(self, group: int) -> list[int]:
         """The pages that count for the request."""
@@ -409,9 +411,23 @@ class CacheManager:
             raise ValueError(f"request {request_id!r} would have no token of its own behind {tokens} forked ones")
         return parent, tokens // self.page_size
 
+    def holder_of(self, request_id: str, tokens: int) -> tuple[str | None, int]:
+        """A request whose cache holds the first ``tokens`` tokens of the named one, or the most of them: itself, or, when it has ended, one
+        that began as a fork of it; and how many it holds."""
+        own = self.requests.get(request_id)
+        if own is not None:
+            return request_id, min(tokens, own.committed)
+        found, most = None, 0
+        for request in self.requests.values():
+            held = min(tokens, request.begins_as.get(request_id, 0))
+            if held > most:
+                found, most = request.request_id, held
+        return found, most
+
     def _fork(self, request: RequestCache, parent: RequestCache, whole: int, tokens: int, tail: list[list[int]]) -> None:
         request.borrowed = [set() for _ in self.groups]
         request.committed = tokens
+        request.begins_as[parent.request_id] = tokens
         for group in self.groups:
             index = group.index
             held = parent.pages[index][request.shared_pages:whole]

@@ -154,10 +154,18 @@ class ContinuousBatchEngine:
                seed: int = 0, prefix: str | None = None, fork_of: str | None = None, **rules) -> Request:
         """``prefix``: a prefix of ``add_prefix`` that the prompt starts with; its whole pages are shared, not computed again.
         ``fork_of``: a request, waiting or running, whose prompt and output so far begin like the prompt; what its cache holds of them when the
-        new request is admitted is taken from there (whole pages held by both, the last one copied), and computed if it has ended.
+        new request is admitted is taken from there (whole pages held by both, the last one copied), or from another fork of it if it has ended,
+        and computed if there is none.
         ``rules``: ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty``, ``logit_bias`` of ``SamplingParams`` (an engine
         made with ``logit_rules=True``), and its ``top_k``, ``top_p``, ``min_p`` (an engine made with ``sampling_limits=True``)."""
         arrival_ns = self._clock_ns()
+        request = self.scheduler.submit(request_id, prompt_token_ids, **self._checked(
+            request_id, prompt_token_ids, max_new_tokens, eos_token_ids, temperature, seed, prefix, fork_of, rules))
+        self.metrics.register_request(request_id, arrival_ns)
+        return request
+
+    def _checked(self, request_id, prompt_token_ids, max_new_tokens, eos_token_ids, temperature, seed, prefix, fork_of, rules) -> dict:
+        """What the scheduler is told of a request that the engine can run; an error for another."""
         vocab = self.runner.vocab_size
         outside = [t for t in prompt_token_ids if not isinstance(t, int) or isinstance(t, bool) or not 0 <= t < vocab]
         if outside:
@@ -179,11 +187,8 @@ class ContinuousBatchEngine:
         holder, shared = self._shared_by(prefix, prompt_token_ids)
         if self._prefixes and not self.manager.can_be_admitted(longest, None if holder is None else (holder, shared)):
             raise ValueError(self.manager.why_not_admitted(request_id, longest, shared // self.manager.page_size))
-        request = self.scheduler.submit(request_id, prompt_token_ids, max_new_tokens=max_new_tokens,
-                                        eos_token_ids=eos_token_ids, sampling=sampling, prefix=holder, shared=shared,
-                                        fork=None if not common else (fork_of, common))
-        self.metrics.register_request(request_id, arrival_ns)
-        return request
+        return {"max_new_tokens": max_new_tokens, "eos_token_ids": eos_token_ids, "sampling": sampling, "prefix": holder, "shared": shared,
+                "fork": None if not common else (fork_of, common)}
 
     # ------------------------------------------------------------------ forks
     def _common_tokens(self, request_id: str, fork_of: str | None, prefix: str | None, prompt: Sequence[int]) -> int:
@@ -461,7 +466,8 @@ class ContinuousBatchEngine:
                  eos_token_ids: int | Collection[int] | None = None, temperature: float = 0.0,
                  seed: int = 0, answers: int = 1, **rules) -> list[list[int]]:
         """Token ids in, generated token ids out, for a list of prompts (host lists both ways); ``rules`` as for ``submit``.  ``answers``:
-        so many outputs for each prompt, one behind the other, each drawn with a seed of its own; a prompt is computed once."""
+        so many outputs for each prompt, one behind the other, each drawn with a seed of its own.  A prompt is computed once where one of its
+        answers still runs when another begins (not with one running request, one new token or no room), in models whose requests can fork."""
         if isinstance(answers, bool) or not isinstance(answers, int) or answers <= 0:
             raise ValueError("answers must be a positive integer")
         if answers > 1:
@@ -478,22 +484,38 @@ class ContinuousBatchEngine:
         return [list(scheduler.get_request(request_id).generated_token_ids) for request_id in ids]
 
 
+    def _check_answers(self, prompts, ids, *, max_new_tokens, eos_token_ids=None, temperature=0.0, prefix=None, **rules) -> None:
+        for prompt, names in zip(prompts, ids):
+            self.scheduler.check(names[0], list(prompt), **self._checked(names[0], list(prompt), max_new_tokens, eos_token_ids, temperature, 0, prefix,
+                                                                         None, rules))
+
     def _generate_answers(self, prompts, answers: int, *, seed: int, **options) -> list[list[int]]:
         scheduler = self.scheduler
         first = len(scheduler.finished_request_ids) + len(scheduler.running_request_ids) + len(scheduler.waiting_request_ids)
         ids = [[f"generate-{first + i}-{j}" for j in range(answers)] for i in range(len(prompts))]
-        for i, prompt in enumerate(prompts):
-            self.submit(ids[i][0], list(prompt), seed=seed + i * answers, **options)
+        self._check_answers(prompts, ids, **options)          # before the first one runs
         forks = self.manager.can_share_pages
-        open_prompts = set(range(len(prompts)))
-        while open_prompts or scheduler.has_unfinished_requests:
+        # a fork has its first answer's prefix; by itself it needs room for all of its pages
+        alone = {name: value for name, value in options.items() if name != "prefix"}
+        fits = [forks and self.manager.can_be_admitted(len(prompt) + options["max_new_tokens"] - 1) for prompt in prompts]
+        to_begin, leading = list(reversed(range(len(prompts)))), []
+        while to_begin or leading or scheduler.has_unfinished_requests:
             # the other answers follow as soon as the first one's prompt is in the cache (or its request has ended)
-            for i in sorted(open_prompts):
+            for i in list(leading):
                 request = scheduler.get_request(ids[i][0])
                 if request.output or request.status is RequestStatus.FINISHED or not forks:
-                    open_prompts.discard(i)
+                    leading.remove(i)
                     for j in range(1, answers):
-                        self.submit(ids[i][j], list(prompts[i]), seed=seed + i * answers + j, fork_of=ids[i][0] if forks else None, **options)
+                        if fits[i]:
+                            self.submit(ids[i][j], list(prompts[i]), seed=seed + i * answers + j, fork_of=ids[i][0], **alone)
+                        else:
+                            self.submit(ids[i][j], list(prompts[i]), seed=seed + i * answers + j, **options)
+            # the next prompt as soon as the requests that run and those still to follow leave a place, so that a prompt's answers run together
+            while to_begin and (not forks or len(scheduler.waiting_request_ids) + len(scheduler.running_request_ids)
+                                + len(leading) * (answers - 1) < scheduler.max_running_requests):
+                i = to_begin.pop()
+                self.submit(ids[i][0], list(prompts[i]), seed=seed + i * answers, **options)
+                leading.append(i)
             if scheduler.has_unfinished_requests and self.step() is None:
                 raise RuntimeError("requests are waiting but nothing can be scheduled")
         return [list(scheduler.get_request(request_id).generated_token_ids) for group in ids for request_id in group]

@@ -211,14 +211,16 @@ class CacheGate:
         return None if held is None else held.slot
 
     def _admit_fork(self, request: Request) -> int | None:
-        """With what the other request's cache holds of the prompt now, if it is still there."""
+        """With what the other request's cache holds of the prompt now, or, if it has ended, that of a fork of it."""
         other, common = request.fork
-        tokens = min(common, self.cache.get(other).committed) if other in self.cache.requests else 0
+        source, tokens = self.cache.holder_of(other, common)
         held = self.cache.create_request(request.request_id, lifetime_tokens=request.lifetime_tokens,
                                          temperature=request.sampling.temperature, seed=request.sampling.seed,
-                                         fork=(other, tokens) if tokens else None)
+                                         fork=(source, tokens) if tokens else None)
         if held is None:
             return None
+        if tokens:
+            held.begins_as[other] = tokens           # whoever takes its place if it has ended
         request.shared = request.cursor = tokens
         return held.slot
 
@@ -308,6 +310,18 @@ class RequestScheduler:
         """Queue a request; allowed at any time, also while a plan is outstanding.  ``prefix``, ``shared``: the prompt's first tokens
         are on the pages of that cached request; only those behind them run through the model.  ``fork``: another request and how many of
         the prompt's first tokens are its own; the gate takes what is cached of them when this one is admitted."""
+        request = self.check(request_id, prompt_token_ids, max_new_tokens=max_new_tokens, eos_token_ids=eos_token_ids, temperature=temperature,
+                             seed=seed, sampling=sampling, prefix=prefix, shared=shared, fork=fork)
+        self._arrivals += 1
+        self._by_id[request_id] = request
+        self._queue.append(request)
+        return request
+
+    def check(self, request_id: str, prompt_token_ids: Sequence[int], *, max_new_tokens: int,
+              eos_token_ids: int | Collection[int] | None = None, temperature: float = 0.0,
+              seed: int = 0, sampling: SamplingParams | None = None, prefix: str | None = None,
+              shared: int = 0, fork: tuple[str, int] | None = None) -> Request:
+        """What ``submit`` would queue, or its error."""
         if not request_id:
             raise ValueError("request_id must not be empty")
         if request_id in self._by_id:
@@ -331,12 +345,8 @@ class RequestScheduler:
                              for t in ((eos_token_ids,) if isinstance(eos_token_ids, int) else eos_token_ids))
         if sampling is None:
             sampling = SamplingParams(temperature, seed) if (temperature or seed) else GREEDY
-        request = Request(request_id, prompt, max_new_tokens, stop, sampling, order=self._arrivals, cursor=shared, prefix=prefix,
-                          shared=shared, fork=fork)
-        self._arrivals += 1
-        self._by_id[request_id] = request
-        self._queue.append(request)
-        return request
+        return Request(request_id, prompt, max_new_tokens, stop, sampling, order=self._arrivals, cursor=shared, prefix=prefix,
+                       shared=shared, fork=fork)
 
     # ------------------------------------------------------------------ the next step
     def schedule_step(self) -> StepPlan | None:
