@@ -15,7 +15,7 @@ import torch
 from .. import ops
 from ..config.spec import PartSpec
 from ..ops import AttentionBatch, SharedPrefix
-from .base import KVCacheNeed, Mixer, TensorSpec, build_part, register_part
+from .base import KVCacheNeed, Mixer, PositionEncoding, TensorSpec, build_part, register_part
 
 
 class PagedAttention(Mixer):
@@ -44,7 +44,6 @@ class PagedAttention(Mixer):
 
 class GQAAttention(PagedAttention):
     supports_norm_fusion = True
-    supports_quantized_cache = True
 
     def __init__(self, spec, compute_dtype):
         super().__init__(spec, compute_dtype)
@@ -63,6 +62,8 @@ class GQAAttention(PagedAttention):
         self.scale = float(self.head_dim) ** -0.5
         # the position encoding is optional: without one, q and k are used as projected
         self.position = build_part("position", a["position"], compute_dtype) if a.get("position") else None
+        # (an encoding of another kind than by frequencies stores the keys itself, in their own type)
+        self.supports_quantized_cache = self.position is None or type(self.position).rotary_frequencies is not PositionEncoding.rotary_frequencies
         self._no_rotation: torch.Tensor | None = None
         self.w_qkv = self.b_qkv = self.w_o = self.b_o = None
         self.input_norm_eps: float | None = None     # set once the preceding norm's weight is folded in
