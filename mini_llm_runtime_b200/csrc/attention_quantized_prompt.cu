@@ -10,6 +10,9 @@
 //               the weights' own rounding adds; codes times scales have too many bits for any 16.
 //   attend      scores s = Q' K'^T; x = s * 2^(a + c) scale log2 e + b; weights 2^(x - base), which carry V's powers of two, in float16; out = sum
 //               weights V' / sum (weights / 2^b): a factor and an exponent for each tile of 64 keys, nothing per key.
+//   wide tiles  The largest scale may be that of a key which a row does not see.  Where a tile's value scales lie further apart than 2^4, or
+//               a key's scale too far below the largest for K' to have all bits, every key has its own a and b: then a row's weights
+//               and sums are those of the keys that it sees, whatever lies beside them.
 //
 // The attending kernel is the one of the bfloat16 cache in its roles: 128 query rows of one head are a work item; four warps of
 // softmax (a thread per row), one that issues the products, one that loads; two CTAs per SM; items drawn heaviest first, long ones
@@ -45,17 +48,20 @@ __device__ __forceinline__ uint32_t qp_pack(float a, float b) {
   const __half2 pair = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&pair);
 }
-// 2^e as the largest power of two not above a positive number (2^-60 for zero and below)
-__device__ __forceinline__ float qp_power(float x) {
-  return x > 8.673617e-19f ? __uint_as_float(__float_as_uint(x) & 0x7f800000u) : 8.673617e-19f;
-}
+// 2^e as the largest power of two not above a positive number (2^-100 for zero and below)
+constexpr float QP_LEAST = 7.888609e-31f;
+__device__ __forceinline__ float qp_power(float x) { return x > QP_LEAST ? __uint_as_float(__float_as_uint(x) & 0x7f800000u) : QP_LEAST; }
+__device__ __forceinline__ float qp_exponent(float power) { return (float)((int)(__float_as_uint(power) >> 23) - 127); }
+// Scales of a tile that share their powers of two: of values within 2^4 (weights of a row that sees only the smallest keep 20 of float16's 24
+// powers of two below the largest), of keys within 2^14 (codes times them are ordinary float16 numbers; zeros always).
+constexpr float QP_NEAR_VALUES = 1.f / 16.f, QP_NEAR_KEYS = 1.f / 16384.f;
 
 // Units: tiles of a kv head, then groups of 8 (row, head) pairs of q.
 template <int D>
 __global__ void __launch_bounds__(QP_PREPARE)
 quantized_prompt_prepare_kernel(const bf16* q, const int8_t* k_pool, const int8_t* v_pool, const float* k_scales, const float* v_scales,
                                 __half* __restrict__ q_out, float* __restrict__ q_factor, __half* __restrict__ k_out, __half* __restrict__ v_out,
-                                float2* __restrict__ tile_factor, int* __restrict__ seg_tile0, const int* __restrict__ seg_q_len,
+                                float2* __restrict__ tile_factor, float2* __restrict__ key_factor, int* __restrict__ seg_tile0, const int* __restrict__ seg_q_len,
                                 const int* __restrict__ seg_pos0, const int* __restrict__ block_table, const int* __restrict__ seg_slot, int segments,
                                 int table_width, int pairs, int kv_heads, int page_size, int block, int pool_pages, int window, int most_tiles,
                                 int* __restrict__ control, int control_len) {
@@ -146,6 +152,7 @@ quantized_prompt_prepare_kernel(const bf16* q, const int8_t* k_pool, const int8_
   }
   __syncthreads();
   float power[2];
+  bool near = true;            // of this lane's keys
 #pragma unroll
   for (int values = 0; values < 2; ++values) {
     float top = 0.f;
@@ -156,7 +163,19 @@ quantized_prompt_prepare_kernel(const bf16* q, const int8_t* k_pool, const int8_
     }
     power[values] = qp_power(warp_max(top));
   }
-  if (threadIdx.x == 0) tile_factor[unit] = make_float2(power[0], (float)((int)(__float_as_uint(power[1]) >> 23) - 127));
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int key = key0 + lane + 32 * e;
+    const float ks = scales[0][lane + 32 * e], vs = scales[1][lane + 32 * e];
+    if (key < lowest || key > last || !(ks < INFINITY && vs < INFINITY)) continue;      // no row sees it, or it gives NaN
+    near = near && (ks <= 0.f || qp_power(ks) >= power[0] * QP_NEAR_KEYS) && qp_power(vs) >= power[1] * QP_NEAR_VALUES;
+  }
+  const bool wide = !__all_sync(0xffffffffu, near);      // the same in every warp
+  if (threadIdx.x == 0) tile_factor[unit] = make_float2(wide ? -1.f : power[0], wide ? 0.f : qp_exponent(power[1]));
+  if (wide && threadIdx.x < QP_KEYS) {
+    const float ks = scales[0][threadIdx.x], vs = scales[1][threadIdx.x];
+    key_factor[(size_t)unit * QP_KEYS + threadIdx.x] = make_float2(ks < INFINITY ? qp_power(ks) : 1.f, vs < INFINITY ? qp_exponent(qp_power(vs)) : 0.f);
+  }
   const float inverse[2] = {1.f / power[0], 1.f / power[1]};
   constexpr int PIECES = D / 16;
 #pragma unroll
@@ -167,7 +186,8 @@ quantized_prompt_prepare_kernel(const bf16* q, const int8_t* k_pool, const int8_
     uint4 raw = make_uint4(0u, 0u, 0u, 0u);
     if (line >= 0) raw = __ldcg(reinterpret_cast<const uint4*>((values ? v_pool : k_pool) + (line * page_size + offset) * D) + c);
     const bool finite = scales[0][j] < INFINITY && scales[1][j] < INFINITY;
-    const float factor = finite ? scales[values][j] * inverse[values] : values ? 0.f : __int_as_float(0x7fffffff);
+    const float own = scales[values][j];
+    const float factor = finite ? own * (wide ? 1.f / qp_power(own) : inverse[values]) : values ? 0.f : __int_as_float(0x7fffffff);
     const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
     uint32_t packed[8];
 #pragma unroll
@@ -207,8 +227,8 @@ __host__ __device__ constexpr uint32_t qp_idesc(int m, int n, bool b_mn_major) {
 template <int D>
 __global__ void __launch_bounds__(QP_THREADS, 2)
 quantized_prompt_attention_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                                  const __grid_constant__ CUtensorMap v_map, const float* q_factor, const float2* tile_factor, const int* seg_tile0,
-                                  bf16* __restrict__ out, const int* __restrict__ tile_seg, const int* __restrict__ tile_row0,
+                                  const __grid_constant__ CUtensorMap v_map, const float* q_factor, const float2* tile_factor, const float2* key_factor,
+                                  const int* seg_tile0, bf16* __restrict__ out, const int* __restrict__ tile_seg, const int* __restrict__ tile_row0,
                                   const int* __restrict__ seg_q_start, const int* __restrict__ seg_q_len, const int* __restrict__ seg_pos0,
                                   int num_tiles, int heads, int kv_heads, int window, float scale_log2, int* queue, int* error_word, int max_parts,
                                   int tiles_per_unit, float* __restrict__ scratch, int* __restrict__ counters, int shared_bytes) {
@@ -370,7 +390,10 @@ quantized_prompt_attention_kernel(const __grid_constant__ CUtensorMap q_map, con
       for (int j = 0; j < tiles; ++j) {
         const unsigned t = tiles_before + (unsigned)j;
         const int buffer = t & 1, stage = t % STAGES, key0 = (tile_begin + j) * QP_KEYS;
-        const float factor = next.x * row_factor, exponent = next.y;
+        const bool wide = next.x < 0.f;
+        // (a product too small for a number would make NaN of what is hidden; scores that small are zero)
+        const float factor = wide ? 1.f : fmaxf(next.x * row_factor, 1e-36f), exponent = next.y;
+        const float4* key_pairs = reinterpret_cast<const float4*>(key_factor + (size_t)(prepared0 + j) * QP_KEYS);
         if (j + 1 < tiles) next = __ldcg(tile_factor + prepared0 + j + 1);
         fa_wait(&ctl.qk_done[stage], (t / STAGES) & 1u, error_word, 0x86, gave_up);
         fa_fence_after();
@@ -384,6 +407,14 @@ quantized_prompt_attention_kernel(const __grid_constant__ CUtensorMap q_map, con
           for (int c = 0; c < QP_KEYS; ++c) {
             const int key = key0 + c;
             if (!(key >= limit_lo && key <= limit_hi)) s[c] = -INFINITY;
+          }
+        }
+        if (wide) {
+#pragma unroll
+          for (int c = 0; c < QP_KEYS; c += 2) {
+            const float4 pair = __ldcg(key_pairs + c / 2);
+            s[c] = fmaf(s[c], fmaxf(pair.x * row_factor, 1e-36f), pair.y);
+            s[c + 1] = fmaf(s[c + 1], fmaxf(pair.z * row_factor, 1e-36f), pair.w);
           }
         }
         float part_max[4] = {s[0], s[1], s[2], s[3]};
@@ -414,7 +445,16 @@ quantized_prompt_attention_kernel(const __grid_constant__ CUtensorMap q_map, con
           }
         }
         const float2 sum2 = __fadd2_rn(__fadd2_rn(part_sum[0], part_sum[1]), __fadd2_rn(part_sum[2], part_sum[3]));
-        l = fmaf(l, alpha, (sum2.x + sum2.y) * fa_exp2(-exponent));
+        float tile_sum = (sum2.x + sum2.y) * fa_exp2(-exponent);
+        if (wide) {
+          tile_sum = 0.f;
+#pragma unroll
+          for (int c = 0; c < QP_KEYS; c += 2) {
+            const float4 pair = __ldcg(key_pairs + c / 2);
+            tile_sum += fmaf(s[c], fa_exp2(-pair.y), s[c + 1] * fa_exp2(-pair.w));
+          }
+        }
+        l = fmaf(l, alpha, tile_sum);
 
         // The output rows in tensor memory are touched only when a row of this warp moved its base.  The previous tile's product is
         // waited for on every tile all the same: the one buffer of weights must have been read.
@@ -581,7 +621,7 @@ static QpParts qp_parts(long long items, int longest, int dim) {
 // one, which may run beside it on another stream: `control` is the attending kernel's queue and a counter per item in parts, zeroed by
 // the preparing one.
 struct QpLayout {
-  long long q, q_factor, k, v, tile_factor, seg_tile0, control, states, total;
+  long long q, q_factor, k, v, tile_factor, key_factor, seg_tile0, control, states, total;
   int control_len;
 };
 static QpLayout qp_layout(long long key_tiles, long long q_rows, int heads, int kv_heads, int dim, int segments, int tiles, int longest) {
@@ -593,7 +633,8 @@ static QpLayout qp_layout(long long key_tiles, long long q_rows, int heads, int 
   at.v = next(at.k + key_tiles * kv_heads * QP_KEYS * dim * 2);
   at.q_factor = next(at.v + key_tiles * kv_heads * QP_KEYS * dim * 2);
   at.tile_factor = next(at.q_factor + q_rows * heads * 4);
-  at.seg_tile0 = next(at.tile_factor + key_tiles * kv_heads * 8);
+  at.key_factor = next(at.tile_factor + key_tiles * kv_heads * 8);
+  at.seg_tile0 = next(at.key_factor + key_tiles * kv_heads * QP_KEYS * 8);
   at.control = next(at.seg_tile0 + (long long)segments * 4);
   at.control_len = 1 + (parts > 1 ? (int)items : 0);
   at.states = next(at.control + (long long)at.control_len * 4);
@@ -618,8 +659,8 @@ static int qp_launch(const void* q, const void* k_pool, const void* v_pool, cons
   const int pairs = q_rows * heads, per = QP_PREPARE / 32;
   launch_kernel(quantized_prompt_prepare_kernel<D>, dim3(key_tiles * kv_heads + (pairs + per - 1) / per), dim3(QP_PREPARE), 0, stream, (const bf16*)q,
                 (const int8_t*)k_pool, (const int8_t*)v_pool, k_scales, v_scales, (__half*)(prepared + at.q), (float*)(prepared + at.q_factor),
-                (__half*)(prepared + at.k), (__half*)(prepared + at.v), (float2*)(prepared + at.tile_factor), (int*)(prepared + at.seg_tile0), seg_q_len,
-                seg_pos0, block_table, seg_slot, segments, table_width, pairs, kv_heads, page_size, block, pool_pages, window, key_tiles,
+                (__half*)(prepared + at.k), (__half*)(prepared + at.v), (float2*)(prepared + at.tile_factor), (float2*)(prepared + at.key_factor),
+                (int*)(prepared + at.seg_tile0), seg_q_len, seg_pos0, block_table, seg_slot, segments, table_width, pairs, kv_heads, page_size, block, pool_pages, window, key_tiles,
                 control, at.control_len);
   int status = launch_status();
   if (status != MLR_OK) return status;
@@ -634,8 +675,8 @@ static int qp_launch(const void* q, const void* k_pool, const void* v_pool, cons
   const auto [parts, per_unit] = qp_parts(items, longest, D);
   const long long units = items * parts;
   launch_kernel(quantized_prompt_attention_kernel<D>, dim3((int)(units < resident ? units : resident)), dim3(QP_THREADS), shared, stream, q_map, k_map,
-                v_map, (const float*)(prepared + at.q_factor), (const float2*)(prepared + at.tile_factor), (const int*)(prepared + at.seg_tile0), (bf16*)out,
-                tile_seg, tile_row0, seg_q_start, seg_q_len, seg_pos0, tiles, heads, kv_heads, window, scale * 1.4426950408889634f, control, error_word,
+                v_map, (const float*)(prepared + at.q_factor), (const float2*)(prepared + at.tile_factor), (const float2*)(prepared + at.key_factor),
+                (const int*)(prepared + at.seg_tile0), (bf16*)out, tile_seg, tile_row0, seg_q_start, seg_q_len, seg_pos0, tiles, heads, kv_heads, window, scale * 1.4426950408889634f, control, error_word,
                 parts, per_unit, (float*)(prepared + at.states), control + 1, (int)shared);
   return launch_status();
 }

@@ -2,6 +2,9 @@
 
 from __future__ import annotations
 
+import copy
+
+import numpy as np
 import pytest
 import torch
 
@@ -104,3 +107,56 @@ def test_places_that_no_key_is_seen_at_give_nothing(dtype):
         for at in set(range(len(page))) - set(seen):
             step.pool.value_scales[page[at], :, offset[at]] = float("inf" if at % 2 else "nan")
     assert torch.equal(step.run(window=50), want)
+
+
+def rows_before(step, i, rows):
+    """The step's request i as if it had only its first ``rows`` rows, and where these lie in the step."""
+    short = copy.copy(step)
+    at = int(step.start[i])
+    short.lengths, short.first, short.slots, short.start = (np.asarray([rows], dtype=np.int32), step.first[i:i + 1], step.slots[i:i + 1],
+                                                            np.zeros(1, dtype=np.int32))
+    short.q = step.q[at:at + rows]
+    return short, slice(at, at + rows)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(14, 2, 64, torch.bfloat16), (8, 2, 128, torch.bfloat16), (12, 3, 96, torch.float32)])
+@pytest.mark.parametrize("which", ["keys", "values", "both"])
+@pytest.mark.parametrize("power", [5, 30, 60])
+def test_scales_of_later_keys_do_not_reach_the_rows_before_them(heads, kv_heads, dim, dtype, which, power):
+    """Rows of a prompt whose later keys' scales are larger by far, in the same 64 keys and behind: held to the errors of what they see."""
+    step = Step([100, 1, 40], [70, 33, 0], heads, kv_heads, dim, 16, 1, dtype, 80)
+    for i, cut in ((0, 95), (2, 21)):      # positions from which on
+        page, offset = step.place(i, int(step.first[i] + step.lengths[i]))
+        for name, scales in (("keys", step.pool.key_scales), ("values", step.pool.value_scales)):
+            if which in (name, "both"):
+                scales[page[cut:], :, offset[cut:]] *= 2.0 ** power
+    got = step.run()
+    for i, cut in ((0, 95), (2, 21)):
+        short, rows = rows_before(step, i, cut - int(step.first[i]))
+        short.check(got[rows])
+    short, rows = rows_before(step, 1, 1)
+    short.check(got[rows])
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(14, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("key,value,query", [(1e-20, 1.0, 1e-30), (1.0, 1e-25, 1.0), (1e-25, 1e-25, 1.0), (1e6, 1e-6, 1e-6), (1e-12, 1e20, 1e12)])
+def test_scales_and_queries_far_from_one(heads, kv_heads, dim, key, value, query):
+    step = Step([1, 90, 1, 3], [100, 30, 3, 500], heads, kv_heads, dim, 16, 4, torch.bfloat16, 81)
+    step.pool.key_scales.mul_(key)
+    step.pool.value_scales.mul_(value)
+    step.q.mul_(query)
+    step.check(step.run())
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(14, 2, 64), (8, 2, 128)])
+def test_scales_of_one_request_further_apart_than_float16_is_wide(heads, kv_heads, dim):
+    """Every key with a power of two of its own between 2^-30 and 1, a tenth of the blocks zeros: each key by itself, over several tiles, windows too."""
+    step = Step([1, 150, 1, 64], [300, 100, 7, 1000], heads, kv_heads, dim, 16, 1, torch.bfloat16, 82)
+    g = torch.Generator(device=DEVICE).manual_seed(83)
+    for scales, codes in ((step.pool.value_scales, step.pool.value), (step.pool.key_scales, step.pool.key)):
+        scales *= 2.0 ** torch.randint(-30, 1, scales.shape, generator=g, device=DEVICE).float()
+        empty = torch.rand(scales.shape, generator=g, device=DEVICE) < 0.1
+        scales[empty] = 0.0
+        codes.view(*scales.shape, -1, dim)[empty] = 0
+    step.check(step.run())
+    step.check(step.run(window=40), window=40)
