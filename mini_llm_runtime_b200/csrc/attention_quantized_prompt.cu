@@ -48,9 +48,10 @@ __device__ __forceinline__ uint32_t qp_pack(float a, float b) {
   const __half2 pair = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&pair);
 }
-// 2^e as the largest power of two not above a positive number (2^-100 for zero and below)
-constexpr float QP_LEAST = 7.888609e-31f;
-__device__ __forceinline__ float qp_power(float x) { return x > QP_LEAST ? __uint_as_float(__float_as_uint(x) & 0x7f800000u) : QP_LEAST; }
+// 2^e as the largest power of two not above a positive number, from 2^-100 (zero and below too) to 2^126; 2^-e; e
+constexpr float QP_LEAST = 7.888609e-31f, QP_MOST = 8.507059e37f;
+__device__ __forceinline__ float qp_power(float x) { return __uint_as_float(__float_as_uint(fminf(fmaxf(x, QP_LEAST), QP_MOST)) & 0x7f800000u); }
+__device__ __forceinline__ float qp_over(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 __device__ __forceinline__ float qp_exponent(float power) { return (float)((int)(__float_as_uint(power) >> 23) - 127); }
 // Scales of a tile that share their powers of two: of values within 2^4 (weights of a row that sees only the smallest keep 20 of float16's 24
 // powers of two below the largest), of keys within 2^14 (codes times them are ordinary float16 numbers; zeros always).
@@ -176,7 +177,7 @@ quantized_prompt_prepare_kernel(const bf16* q, const int8_t* k_pool, const int8_
     const float ks = scales[0][threadIdx.x], vs = scales[1][threadIdx.x];
     key_factor[(size_t)unit * QP_KEYS + threadIdx.x] = make_float2(ks < INFINITY ? qp_power(ks) : 1.f, vs < INFINITY ? qp_exponent(qp_power(vs)) : 0.f);
   }
-  const float inverse[2] = {1.f / power[0], 1.f / power[1]};
+  const float inverse[2] = {qp_over(power[0]), qp_over(power[1])};
   constexpr int PIECES = D / 16;
 #pragma unroll
   for (int idx = threadIdx.x; idx < QP_KEYS * PIECES * 2; idx += QP_PREPARE) {
@@ -187,7 +188,7 @@ quantized_prompt_prepare_kernel(const bf16* q, const int8_t* k_pool, const int8_
     if (line >= 0) raw = __ldcg(reinterpret_cast<const uint4*>((values ? v_pool : k_pool) + (line * page_size + offset) * D) + c);
     const bool finite = scales[0][j] < INFINITY && scales[1][j] < INFINITY;
     const float own = scales[values][j];
-    const float factor = finite ? own * (wide ? 1.f / qp_power(own) : inverse[values]) : values ? 0.f : __int_as_float(0x7fffffff);
+    const float factor = finite ? own * (wide ? qp_over(qp_power(own)) : inverse[values]) : values ? 0.f : __int_as_float(0x7fffffff);
     const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
     uint32_t packed[8];
 #pragma unroll
