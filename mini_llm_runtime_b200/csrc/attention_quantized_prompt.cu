@@ -10,7 +10,7 @@
 //               the weights' own rounding adds; codes times scales have too many bits for any 16.
 //   attend      scores s = Q' K'^T; x = s * 2^(a + c) scale log2 e + b; weights 2^(x - base), which carry V's powers of two, in float16; out = sum
 //               weights V' / sum (weights / 2^b): a factor and an exponent for each tile of 64 keys, nothing per key.
-//   wide tiles  The largest scale may be that of a key which a row does not see.  Where a tile's value scales lie further apart than 2^4, or
+//   wide tiles  The largest scale may be that of a key which a row does not see.  Where a tile's value scales lie further apart than 2^6, or
 //               a key's scale too far below the largest for K' to have all bits, every key has its own a and b: then a row's weights
 //               and sums are those of the keys that it sees, whatever lies beside them.
 //
@@ -19,7 +19,8 @@
 // cut into parts that the last one merges.  The prepared keys of a request and kv head lie one behind the other, so a tile
 // is one or two bulk copies and there is no block table to read.  Every wait is bounded; a wait that runs out reports through the
 // error word, and the CTA goes on without waiting (its result is invalid, the host raises).  2,048 rows behind 6,000 keys, 28 heads
-// of 128 over 4: 271 us (0.76 PFLOP/s), 20 of them to prepare.
+// of 128 over 4: 283 us (0.73 PFLOP/s), 19 of them to prepare.  The chain from scores to weights to the next product bounds it: one group of
+// softmax warps and one buffer of weights a CTA, so that tile j's weights wait for tile j - 1's product (tensor pipe 37 % of cycles, 1.4 instructions of four).
 #include <cuda_fp16.h>
 
 #include "tcgen05.cuh"
@@ -52,10 +53,13 @@ __device__ __forceinline__ uint32_t qp_pack(float a, float b) {
 constexpr float QP_LEAST = 7.888609e-31f, QP_MOST = 8.507059e37f;
 __device__ __forceinline__ float qp_power(float x) { return __uint_as_float(__float_as_uint(fminf(fmaxf(x, QP_LEAST), QP_MOST)) & 0x7f800000u); }
 __device__ __forceinline__ float qp_over(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
+// 2^-e for whole e: with 1.5 * 2^23 on it, 127 - e stands in the low bits
+__device__ __forceinline__ float qp_two_to_minus(float e) { return __uint_as_float(__float_as_uint(12583039.f - e) << 23); }
 __device__ __forceinline__ float qp_exponent(float power) { return (float)((int)(__float_as_uint(power) >> 23) - 127); }
-// Scales of a tile that share their powers of two: of values within 2^4 (weights of a row that sees only the smallest keep 20 of float16's 24
-// powers of two below the largest), of keys within 2^14 (codes times them are ordinary float16 numbers; zeros always).
-constexpr float QP_NEAR_VALUES = 1.f / 16.f, QP_NEAR_KEYS = 1.f / 16384.f;
+// Scales of a tile that share their powers of two: of values within 2^6 (weights of a row that sees only the smallest keep 18 of float16's 24
+// powers of two below the largest), of keys within 2^14 (codes times them are ordinary float16 numbers; zeros always).  Numbers of
+// their own cost a tile two reads of them in the middle of its softmax: 2,048 rows behind 6,000 with all tiles wide 520 us, with none 283.
+constexpr float QP_NEAR_VALUES = 1.f / 64.f, QP_NEAR_KEYS = 1.f / 16384.f;
 
 // Units: tiles of a kv head, then groups of 8 (row, head) pairs of q.
 template <int D>
@@ -452,7 +456,7 @@ quantized_prompt_attention_kernel(const __grid_constant__ CUtensorMap q_map, con
 #pragma unroll
           for (int c = 0; c < QP_KEYS; c += 2) {
             const float4 pair = __ldcg(key_pairs + c / 2);
-            tile_sum += fmaf(s[c], fa_exp2(-pair.y), s[c + 1] * fa_exp2(-pair.w));
+            tile_sum += fmaf(s[c], qp_two_to_minus(pair.y), s[c + 1] * qp_two_to_minus(pair.w));
           }
         }
         l = fmaf(l, alpha, tile_sum);

@@ -121,7 +121,7 @@ def rows_before(step, i, rows):
 
 @pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(14, 2, 64, torch.bfloat16), (8, 2, 128, torch.bfloat16), (12, 3, 96, torch.float32)])
 @pytest.mark.parametrize("which", ["keys", "values", "both"])
-@pytest.mark.parametrize("power", [5, 30, 60])
+@pytest.mark.parametrize("power", [5, 7, 30, 60])
 def test_scales_of_later_keys_do_not_reach_the_rows_before_them(heads, kv_heads, dim, dtype, which, power):
     """Rows of a prompt whose later keys' scales are larger by far, in the same 64 keys and behind: held to the errors of what they see."""
     step = Step([100, 1, 40], [70, 33, 0], heads, kv_heads, dim, 16, 1, dtype, 80)
