@@ -41,7 +41,8 @@ Moving.  ``compact`` moves pages into the lowest numbers of their pools, ``resiz
 
 8 bits.  With ``quantized_block`` the pools hold codes of 8 bits and a float32 scale for each block of so many tokens and kv head
 (``ops.QuantizedPool``).  With blocks of more than a token, a step that fails after its tokens were stored may leave the scale of a
-request's last block larger than it was, and its tokens rounded to it.
+request's last block larger than it was, and its tokens rounded to it; a fork that ends inside a block has the scale that the block has by
+then, its parent's later tokens included.
 
 Two admission modes.  With a *promise* (``create_request(..., lifetime_tokens=n)``) the pages of
 the request's whole life are counted against the pool at creation, as the reference reserves them

@@ -21,7 +21,8 @@
 // The keys of all requests and kv heads form one line that the warps share evenly, whatever the contexts: a warp's share may
 // end one request's keys and begin another's.  Each beginning counts as QD_BEGIN tiles more, about what it costs.  No warp waits for
 // another.  Pairs of a request and a kv head that several warps walk are merged by a second launch, in the order of the warps.
-// 64 requests of up to 8,192 keys, 28 heads of 128 over 4: 59 us (4.7 TB/s); 100 of up to 16,384, 40 over 8: 300 us (5.8 TB/s).
+// 64 requests of up to 8,192 keys, 28 heads of 128 over 4: 62 us (4.4 TB/s); 100 of up to 16,384, 40 over 8: 332 us (5.2 TB/s), the merge's
+// launch included.
 #include <cuda_fp16.h>
 
 #include "tma.cuh"

@@ -25,7 +25,7 @@
 //                  by warp, by chunk of a warp's stretch, by thread.
 // Bound by memory while no more than a few logits of a row need weights, by 64-bit arithmetic where all do (13 instructions each; the pass of
 // rows without limits runs at half that pipe's rate), by the steps between CTAs for few rows.  256 rows of 152,064 logits, T 0.8: greedy
-// 48 us, top-k 50 76, 1,000 122, top-p 0.9 232, min-p 0.05 63, no limit 125, all kinds mixed 104; one row: 6, 11, 20, 29, 10 and 13 us.
+// 48 us, top-k 50 76, 1,000 122, top-p 0.9 232, min-p 0.05 63, no limit 125, all kinds mixed 104 to 115; one row: 6, 11, 20, 29, 10 and 13 us.
 // Sums are taken in a fixed order, of ranks or of places (no floating-point atomics): a row's token depends on its row alone (and, where the draw lies
 // within the last bits of a sum from a border, on how many CTAs a row gets in a batch of this size).
 #include <cooperative_groups.h>
@@ -1424,8 +1424,9 @@ MLR_EXPORT int mlr_sample_limited(const float* logits, const float* uniforms, co
     return e == cudaSuccess ? cudaFuncSetAttribute(sample_limited_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, ONE) : e;
   });
   if (err != cudaSuccess) return (int)err;
-  // Rows that take longest first, where not all are taken at once: 256 rows of 152,064 logits under various limits 99 us, so 118 without; under the same
-  // kind of limits 94, so 88 (looking at all rows costs each CTA 1.5 us).  Short slices gain nothing: 256 rows of 32,000 72, so 72.
+  // Rows that take longest first, where not all are taken at once: 256 rows of 152,064 logits under various limits, three drawings, caches flushed,
+  // 111, 113 and 127 us, so 131, 135 and 144 without; all rows under the same limits lose by it, as each CTA looks at all rows' limits: greedy 64, so
+  // 57, top-k 50 88, so 84, none 138, so 135.  Short slices gain nothing: 256 rows of 32,000 72, so 72.
   constexpr int LONG_SLICE = 16384;
   const bool ordered = (long long)rows * ranks > 2 * sm_count() && rows <= SL_ORDERED && slice >= LONG_SLICE;
   auto kernel = resident ? sample_limited_kernel<true> : sample_limited_kernel<false>;

@@ -108,8 +108,8 @@ class ContinuousBatchEngine:
         ``max_prefixes``: how many prefixes the cache may hold for requests to share (``add_prefix``).  ``sampling_limits``: requests may
         limit what is drawn for them by top-k, top-p and min-p; every step then draws under the limits of its requests.
         ``cache_dtype="int8"``: the cache holds keys and values in 8 bits with a scale for each ``cache_block`` tokens and kv head (models
-        whose layers all attend to such a cache).  With blocks of one token a request's results do not depend on how its
-        prompt was cut; larger blocks save four bytes per token and head less one."""
+        whose layers all attend to such a cache).  With blocks of one token what is held for a token does not depend on how its
+        prompt was cut nor on what follows it; larger blocks save up to four bytes per token and head."""
         if cache_dtype not in (None, "int8"):
             raise ValueError(f"unknown cache dtype {cache_dtype!r}; known: int8, or None for the model's own")
         # a model without a position limit of its own gets this engine's default
