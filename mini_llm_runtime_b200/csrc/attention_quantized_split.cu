@@ -7,8 +7,8 @@
 // product times ks, a weight is multiplied by vs).  Scores: a thread per key and a quarter of the heads.  Sums: a thread per four
 // dimensions and a part of the keys, the weights broadcast from shared memory.  Shared-memory reads bound it: a float of a key or
 // value serves two and eight multiply-adds.  Parts are `chunk` keys from absolute positions: 256, or twice as many
-// until the parts' states of a large batch fit the host's limit; a second launch merges them in order.  24 requests of up to 2,500 keys, 12 heads of 96 over 3, float32: 34 us
-// (49 with room for eight heads where four are enough; 1,029 with 16 rows of a prompt's kernel).
+// until the parts' states of a large batch fit the host's limit; a second launch merges them in order.  24 requests of up to 2,500 keys, 12 heads of 96
+// over 3, float32: 34 us (49 with room for eight heads where four are enough; 1,029 with 16 rows of a prompt's kernel).
 // A key that a row does not see gives it nothing, whatever lies there.
 #include "common.cuh"
 
